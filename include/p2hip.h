@@ -355,6 +355,88 @@ size_t p2h_conformer_stack_workspace_bytes(int mode, int T, int n_blocks);
 int    p2h_conformer_stack(int mode, const P2hBlock *blocks, int n_blocks, int T, const float *dPE, float *dX,
                            void *workspace, size_t workspace_bytes, void *stream);
 
+/* ── a decoder layer's step: 4-bit linears, head norms with rotation, attention over many or cached keys ──────────
+ *  No counterpart in the reference, whose decoder is an LSTM: for callers that put a text decoder behind the encoder,
+ *  or that run attention over more rows than one window with a bounded context. Rows are as everywhere here (row-major,
+ *  heads side by side, head h at columns head_dim·h; fused q | k | v rows as the block's qkv linear makes them), but of
+ *  any of three element types, one type for all the rows and caches of a call. Sums, softmax statistics, norms and
+ *  states are held in 32 bits and outputs rounded once.
+ *
+ *  Query heads are shared evenly: query head h reads key head h / (heads / kv_heads). head_dim is 64 or 128. Pointers
+ *  to rows and caches are 16-byte aligned and row pitches whole multiples of 16 bytes unless an entry says otherwise.
+ *  Entries are asynchronous on their stream, allocate nothing and can be captured. Arrays of positions, slots, lengths
+ *  and page numbers are read on the device when the call runs, so a captured graph sees their new values; no value in
+ *  them makes a kernel read or write outside the buffers it was given. */
+enum { P2H_F32 = 0, P2H_F16 = 1, P2H_BF16 = 2 };
+
+/* A device-resident weight [K, N] of 4-bit codes with a scale, and if wanted a zero point, for every `group` (32, 64
+ * or 128) of its rows: w[k][n] = (code[k][n] − zero[k / group][n]) · scale[k / group][n], zero 8 where there are no
+ * zero points. codes [K][ceil(N / 2)]: column n in the low (n even) or high half of byte n / 2; scales fp16 bits
+ * [ceil(K / group)][N]; zeros packed as the codes, [ceil(K / group)][ceil(N / 2)], or NULL. Any K and N >= 1. */
+typedef struct P2hQ4Weight P2hQ4Weight;
+
+/* From host memory, or from device memory (read during the call only). Synchronous; NULL on failure. */
+P2hQ4Weight *p2h_q4_weight_upload(const unsigned char *codes, const uint16_t *scales, const unsigned char *zeros,
+                                  int K, int N, int group);
+P2hQ4Weight *p2h_q4_weight_wrap(const void *d_codes, const void *d_scales, const void *d_zeros, int K, int N,
+                                int group);
+void   p2h_q4_weight_free(P2hQ4Weight *w);
+int    p2h_q4_weight_shape(const P2hQ4Weight *w, int *K, int *N, int *group);
+size_t p2h_q4_weight_device_bytes(const P2hQ4Weight *w);
+
+/* Y [M][N] = alpha · X [M][K] · W + beta · Y for few rows (beta 0 does not read Y): a matrix-vector product per row,
+ * the weight read once for every 16 rows. X and Y of type `dtype`, pitches ldx >= K and ldy >= N elements, no alignment
+ * beyond the element's (16-byte aligned rows load faster). A row's outputs are the same bits whatever M is. X and Y
+ * must not overlap. */
+int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int ldx, const P2hQ4Weight *w, float beta,
+                void *dY, int ldy, void *stream);
+
+/* Keys and values kept between calls, in pages of `page` tokens (a power of two, 16 .. 1024): K and V each
+ * [pages][heads][page][head_dim]. A token's slot is its page number · page + its place in the page. The caller owns
+ * the memory and gives pages to sequences; nothing in a page needs a value before it is written. */
+typedef struct P2hKvCache {
+    int dtype, heads, head_dim, page, pages;
+    void *K, *V;
+} P2hKvCache;
+
+/* For each of T rows q | k | v of dQKV (heads, kv_heads and kv_heads heads of head_dim; pitch ldqkv): every query and
+ * key head x becomes n = x / sqrt(mean(x²) + eps) · gamma (gamma = dGammaQ or dGammaK [head_dim]), and the first `rot`
+ * (a multiple of 16, 0 .. head_dim) elements of n are turned by the row's position: pair i with the angle
+ * dPos[row] · dFreq[i], i < rot / 2, taken in 64 bits, is (n[i], n[i + rot / 2]), or with `interleaved`
+ * (n[2i], n[2i + 1]). Queries go to dQ (pitch ldq). Keys go to dK (pitch ldk) unless it is NULL, and, with a cache, keys
+ * and the row's values (as they are) into the row's slot dSlots[row]; a row whose slot lies outside the cache (a padded
+ * row: −1) is not put into it. Slots inside it are distinct. The value part of the rows is read only with a cache.
+ * dQ and dK may be the very q and k columns of dQKV; no other overlap. */
+int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, const void *dQKV, int ldqkv,
+                     const float *dGammaQ, const float *dGammaK, float eps, int rot, int interleaved,
+                     const float *dFreq, const int *dPos, void *dQ, int ldq, void *dK, int ldk,
+                     const P2hKvCache *cache, const int *dSlots, void *stream);
+
+/* O = softmax(scale · Q Kᵀ) V of n_seqs sequences packed row after row: sequence s has the query rows dQStart[s] ..
+ * dQStart[s + 1] − 1 and the key and value rows dKStart[s] .. dKStart[s + 1] − 1 (starts that do not descend, inside
+ * [0, q_rows] and [0, k_rows]; both NULL with n_seqs 1: all rows). The queries are the last of their sequence's places:
+ * query i of Lq stands at p = i + Lk − Lq. Key j is visible to it iff j <= p + ahead and (p − j < window or j <
+ * sinks): `window` >= 1 places back, itself included, `ahead` >= 0 places on, and the first `sinks` >= 0 places (1 << 30
+ * reaches everything). A query that sees no key gets zeros; rows outside every sequence are left as they were.
+ * scale > 0. At most 2^30 rows. O must not overlap the inputs. */
+int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const int *dQStart, const int *dKStart,
+                         int heads, int kv_heads, int head_dim, const void *dQ, int ldq, const void *dK, int ldk,
+                         const void *dV, int ldv, float scale, int window, int ahead, int sinks, void *dO, int ldo,
+                         void *stream);
+
+/* The same for one new token per sequence over a cache: query row s of dQ stands at the last of the dLen[s] tokens whose
+ * pages are dTable[s · table_ld ..] (token t in page dTable[s · table_ld + t / page]); the visible keys are those with
+ * len − 1 − t < window or t < sinks. Length 0 gives zeros; a length beyond table_ld · page (at most 2^30) counts as
+ * that. Tokens of a page number outside [0, pages) are not seen. The keys of one sequence are split over workgroups
+ * where there are few sequences, planned for lengths up to max_len (other lengths are right as well), and a second
+ * kernel joins the parts kept in the workspace, p2h_attention_paged_workspace_bytes(...) bytes, 16-byte aligned (0: the
+ * call does not split). Without a workspace (NULL) it runs unsplit. Calls sharing a workspace are stream-ordered. */
+size_t p2h_attention_paged_workspace_bytes(const P2hKvCache *cache, int n_seqs, int heads, int max_len, int window,
+                                           int sinks);
+int p2h_attention_paged(const P2hKvCache *cache, int n_seqs, int heads, const void *dQ, int ldq, const int *dTable,
+                        int table_ld, const int *dLen, int max_len, float scale, int window, int sinks, void *dO,
+                        int ldo, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

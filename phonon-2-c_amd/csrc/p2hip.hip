@@ -17,8 +17,15 @@
 #include <mutex>
 #include <vector>
 
+#include "p2hip_host.h"
 #include "p2hip_kernels.h"
 #include "p2hip_split.h"
+
+using p2host::align_up;
+using p2host::aligned;
+using p2host::ensure_init;
+using p2host::fail;
+using p2host::stream_of;
 
 namespace {
 
@@ -40,21 +47,6 @@ char g_init_err[512];
 char g_arch[64];
 int g_cus = 0;
 int g_wall_khz = 0;   /* rate of the constant wall clock that stream_hold reads */
-
-int fail(int rc, const char *fmt, ...)
-{
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(t_err, sizeof t_err, fmt, ap);
-    va_end(ap);
-    return rc;
-}
-
-#define HIPCHK(call)                                                                                            \
-    do {                                                                                                        \
-        hipError_t e_ = (call);                                                                                 \
-        if (e_ != hipSuccess) return fail(P2H_E_DEVICE, "%s: %s", #call, hipGetErrorString(e_));              \
-    } while (0)
 
 void load_switches();
 
@@ -109,21 +101,6 @@ int scratch_of_current_device(void **out)
     *out = g_scratch_ptr[dev];
     return P2H_OK;
 }
-
-int ensure_init()
-{
-    std::call_once(g_init_once, do_init);
-    if (g_init_rc != P2H_OK) return fail(g_init_rc, "%s", g_init_err);
-    return P2H_OK;
-}
-
-hipStream_t stream_of(void *s)
-{
-    if (s) return (hipStream_t)s;
-    return (hipStream_t)p2h_thread_stream();
-}
-
-inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 /* an integer from the environment (tuning and comparison switches), dflt when unset or empty */
 int env_int(const char *name, int dflt)
@@ -184,7 +161,6 @@ void load_switches()
 }
 
 inline int switch_of(const std::atomic<int> &v) { return v.load(std::memory_order_relaxed); }
-inline bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 /* Whether M rows of Y (pitch ldy floats) overlap M rows of X (pitch ldx) other than as the very same rows. */
 inline bool rows_overlap(const float *dX, int ldx, const float *dY, int ldy, int M)
@@ -195,6 +171,30 @@ inline bool rows_overlap(const float *dX, int ldx, const float *dY, int ldy, int
 }
 
 }  // namespace
+
+int p2host::fail(int rc, const char *fmt, ...)
+{
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(t_err, sizeof t_err, fmt, ap);
+    va_end(ap);
+    return rc;
+}
+
+int p2host::ensure_init()
+{
+    std::call_once(g_init_once, do_init);
+    if (g_init_rc != P2H_OK) return fail(g_init_rc, "%s", g_init_err);
+    return P2H_OK;
+}
+
+hipStream_t p2host::stream_of(void *s)
+{
+    if (s) return (hipStream_t)s;
+    return (hipStream_t)p2h_thread_stream();
+}
+
+int p2host::cu_count() { return g_cus; }
 
 struct P2hWeight {
     int K, N;

@@ -1,0 +1,970 @@
+/*  p2hip_decoder.h – gfx950 kernels of a decoder layer's step (included once, by p2hip_decoder.hip).
+ *
+ *  Kernels:
+ *    q4_records      4-bit codes, scales and zero points re-laid per matrix-core operand at upload
+ *    q4_gemv         few rows times a 4-bit weight
+ *    qk_norm_rope    norm and rotation of query and key heads, keys and values into cache pages
+ *    attention_win   attention of ragged sequences over a window and first keys
+ *    attention_page  one query per sequence over a paged cache; attention_join adds the parts of a split sequence
+ */
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "p2hip_index.h"
+
+namespace p2k {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+enum { T_F32 = 0, T_F16 = 1, T_BF16 = 2 };
+constexpr float kLog2e = 1.44269504088896340736f;
+
+/* ── element types ─────────────────────────────────────────────────────────────────────────────────────────── */
+
+template <int DT> struct Elem;
+template <> struct Elem<T_F32> {
+    typedef float type;
+    static __device__ __forceinline__ float get(float v) { return v; }
+    static __device__ __forceinline__ float put(float v) { return v; }
+};
+template <> struct Elem<T_F16> {
+    typedef _Float16 type;
+    static __device__ __forceinline__ float get(_Float16 v) { return (float)v; }
+    static __device__ __forceinline__ _Float16 put(float v) { return (_Float16)v; }
+};
+template <> struct Elem<T_BF16> {
+    typedef __bf16 type;
+    static __device__ __forceinline__ float get(__bf16 v) { return (float)v; }
+    static __device__ __forceinline__ __bf16 put(float v) { return (__bf16)v; }
+};
+
+/* 16 bytes of elements as floats, and back (each rounded to nearest even) */
+template <int DT> constexpr int kPer16 = DT == T_F32 ? 4 : 8;
+
+template <int DT> __device__ __forceinline__ void unpack(u4 r, float (&v)[kPer16<DT>])
+{
+    if constexpr (DT == T_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = __uint_as_float(r[i]);
+    } else if constexpr (DT == T_F16) {
+        const h8 x = __builtin_bit_cast(h8, r);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float)x[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = __uint_as_float(r[i] << 16);
+            v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+        }
+    }
+}
+
+template <int DT> __device__ __forceinline__ u4 pack(const float (&v)[kPer16<DT>])
+{
+    if constexpr (DT == T_F32) {
+        return u4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    } else if constexpr (DT == T_F16) {
+        h8 x;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (_Float16)v[i];
+        return __builtin_bit_cast(u4, x);
+    } else {
+        b8 x;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (__bf16)v[i];
+        return __builtin_bit_cast(u4, x);
+    }
+}
+
+/* the matrix products of 16-bit operands, bits as u4 */
+template <int DT> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c)
+{
+    if constexpr (DT == T_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+template <int DT> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c)
+{
+    if constexpr (DT == T_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+/* Transposing LDS read of 16-bit values: of the 4 × 16 values that the 16 lanes of a group address (lane i: 4 values,
+ * row i / 4, columns 4·(i % 4) ..), lane i gets column i's four. */
+__device__ __forceinline__ u2 lds_tr(const uint16_t *p)
+{
+    typedef __attribute__((address_space(3))) s4 *lds4;
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p)));
+}
+
+/* max and sum over lanes l, l ^ 16, l ^ 32, l ^ 48, and over l, l ^ 32 */
+__device__ __forceinline__ float max_halves(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float max_quarters(float v)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_quarters(float v)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+/* ── 4-bit weights ─────────────────────────────────────────────────────────────────────────────────────────── */
+
+/* Records: for each 16 columns and 128 rows 64 lanes × 16 bytes, word b of lane l holding column l % 16's codes of rows
+ * 32b + 8(l / 16) + j, j = 0..7: the operand of one 16 × 16 × 32 product. Code j sits in nibble j / 2 + 4·(j & 1), so
+ * that one mask takes two neighbouring rows. Scales: [column tile][unit][16 columns][groups in a unit], fp16 (SCALE2:
+ * with the zero point's half after each). Rows past K and columns past N have code 0 and scale 0. */
+__global__ void q4_records(int K, int N, int group, int tiles, int units, const uint8_t *__restrict__ codes,
+                           const uint16_t *__restrict__ scales, const uint8_t *__restrict__ zeros,
+                           uint32_t *__restrict__ rec, uint16_t *__restrict__ sc)
+{
+    const size_t half = ((size_t)N + 1) / 2, n_rec = (size_t)tiles * units * 256;
+    const int gpu = 128 / group;
+    const size_t n_sc = (size_t)tiles * units * 16 * gpu;
+    const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n_rec) {
+        const int b = (int)(i & 3), l = (int)(i >> 2) & 63;
+        const size_t tu = i >> 8;
+        const int u = (int)(tu % units), t = (int)(tu / units);
+        const int n = 16 * t + (l & 15);
+        uint32_t r = 0;
+        if (n < N)
+            for (int j = 0; j < 8; j++) {
+                const long long k = 128ll * u + 32 * b + 8 * (l >> 4) + j;
+                if (k < K) r |= ((codes[(size_t)k * half + (n >> 1)] >> (4 * (n & 1))) & 15u) << (4 * (j / 2 + 4 * (j & 1)));
+            }
+        rec[i] = r;
+    }
+    if (i < n_sc) {
+        const int g = (int)(i % gpu), c = (int)(i / gpu) & 15;
+        const size_t tu = i / gpu / 16;
+        const int u = (int)(tu % units), t = (int)(tu / units);
+        const long long gr = (long long)u * gpu + g;
+        const int n = 16 * t + c;
+        const bool in = n < N && gr * group < K;
+        const uint16_t s = in ? scales[(size_t)gr * N + n] : 0;
+        if (zeros) {
+            const int z = in ? (zeros[(size_t)gr * half + (n >> 1)] >> (4 * (n & 1))) & 15 : 8;
+            sc[2 * i] = s;
+            sc[2 * i + 1] = (uint16_t)(0xe400 | z);   /* −(1024 + z) as fp16 */
+        } else {
+            sc[i] = s;
+        }
+    }
+}
+
+struct Q4Args {
+    int M, N, K, units, ldx, ldy, vec;
+    float alpha, beta;
+    const void *x;
+    void *y;
+    const u4 *rec;
+    const void *sc;
+};
+
+/* Two codes of a record word, nibbles i and i + 4, as fp16 code − zero: 1024 + code has the code in its low bits, and
+ * adding −(1024 + zero) is exact. */
+__device__ __forceinline__ h2 q4_pair(uint32_t w, int i, h2 bias)
+{
+    const uint32_t t = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+    return __builtin_bit_cast(h2, t) + bias;
+}
+
+/* Eight fp32 values as three bf16 pieces each, the upper 16 bits of what is left after the pieces before: exact, as 8 + 8
+ * + 8 bits hold the 24 of a float. Nothing is left of an infinity. */
+__device__ __forceinline__ void cut3(uint32_t (&v)[8], u4 (&xp)[3])
+{
+#pragma unroll
+    for (int p = 0; p < 3; p++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) xp[p][i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x07060302u);
+        if (p == 2) break;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float left = __uint_as_float(v[j]) - __uint_as_float(v[j] & 0xffff0000u);
+            v[j] = p == 0 && (v[j] & 0x7fffffffu) == 0x7f800000u ? 0u : __float_as_uint(left);
+        }
+    }
+}
+
+/* Y rows 16·blockIdx.y .. of 16 columns: each of the WV waves sums its 128-row units of K, unit after unit, and the waves'
+ * sums are added in order in LDS. A group's products are summed as whole (code − zero) times x, exact factors in both
+ * operands, and scaled once per group in 32 bits.
+ *
+ * fp16 rows multiply as fp16. bf16 rows multiply as bf16 (whole numbers up to 15 are exact there too). fp32 rows are cut
+ * into three bf16 pieces (8 + 8 + 8 bits, the pieces of a non-finite value are that value and zeros), which sum to the
+ * row exactly: three products into the same sums. */
+template <int DT, int GROUP, bool ZP, int WV>
+__global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int GPU = 128 / GROUP, NP = DT == T_F32 ? 3 : 1;
+    __shared__ float part[WV][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int m0 = 16 * blockIdx.y, rows = imin(16, a.M - m0), tile = blockIdx.x;
+    const E *x = static_cast<const E *>(a.x) + (size_t)(m0 + imin(c, rows - 1)) * a.ldx;
+    const bool have = c < rows;
+    f4 total = {0, 0, 0, 0};
+    for (int u = wave; u < a.units; u += WV) {
+        const size_t tu = (size_t)tile * a.units + u;
+        const u4 r = a.rec[tu * 64 + lane];
+        float scale[GPU];
+        h2 bias[GPU];
+        if constexpr (ZP) {
+            const uint32_t *p = static_cast<const uint32_t *>(a.sc) + (tu * 16 + c) * GPU;
+#pragma unroll
+            for (int q = 0; q < GPU; q++) {
+                const h2 v = __builtin_bit_cast(h2, p[q]);
+                scale[q] = (float)v[0];
+                bias[q] = h2{v[1], v[1]};
+            }
+        } else {
+            const _Float16 *p = static_cast<const _Float16 *>(a.sc) + (tu * 16 + c) * GPU;
+#pragma unroll
+            for (int q = 0; q < GPU; q++) {
+                scale[q] = (float)p[q];
+                bias[q] = h2{(_Float16)-1032.0f, (_Float16)-1032.0f};
+            }
+        }
+        f4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const int k = 128 * u + 32 * b + 8 * g;
+            /* this lane's eight values of its row */
+            u4 xp[NP];
+            if (a.vec && k + 8 <= a.K) {
+                if constexpr (DT == T_F32) {
+                    const u4 v0 = *reinterpret_cast<const u4 *>(x + k), v1 = *reinterpret_cast<const u4 *>(x + k + 4);
+                    uint32_t v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] = have ? v[j] : 0u;
+                    cut3(v, xp);
+                } else {
+                    const u4 v = *reinterpret_cast<const u4 *>(x + k);
+                    xp[0] = have ? v : u4{0, 0, 0, 0};
+                }
+            } else {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = have && k + j < a.K ? Elem<DT>::get(x[k + j]) : 0.0f;
+                if constexpr (DT == T_F32) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) w[j] = __float_as_uint(v[j]);
+                    cut3(w, xp);
+                } else {
+                    xp[0] = pack<DT>(v);
+                }
+            }
+            u4 wv;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const h2 d = q4_pair(r[b], i, bias[b * GPU / 4]);
+                if constexpr (DT == T_F16) wv[i] = __builtin_bit_cast(uint32_t, d);
+                else   /* fp16 whole numbers → fp32 → their upper halves, which are all there is */
+                    wv[i] = __builtin_amdgcn_perm(__float_as_uint((float)d[1]), __float_as_uint((float)d[0]), 0x07060302u);
+            }
+#pragma unroll
+            for (int p = 0; p < NP; p++) acc = mfma16<DT == T_F16 ? T_F16 : T_BF16>(xp[p], wv, acc);
+            if ((b + 1) % (GROUP / 32) == 0) {
+                total += scale[b * GPU / 4] * acc;
+                acc = f4{0, 0, 0, 0};
+            }
+        }
+    }
+    /* row 4g + i, column c of this wave's sums */
+#pragma unroll
+    for (int i = 0; i < 4; i++) part[wave][16 * (4 * g + i) + c] = total[i];
+    __syncthreads();
+    for (int t = threadIdx.x; t < 16 * rows; t += 64 * WV) {
+        const int n = 16 * tile + (t & 15);
+        float s = part[0][t];
+#pragma unroll
+        for (int w = 1; w < WV; w++) s += part[w][t];
+        if (n < a.N) {
+            E *y = static_cast<E *>(a.y) + (size_t)(m0 + (t >> 4)) * a.ldy + n;
+            s *= a.alpha;
+            if (a.beta != 0.0f) s = __builtin_fmaf(a.beta, Elem<DT>::get(*y), s);
+            *y = Elem<DT>::put(s);
+        }
+    }
+}
+
+/* ── head norms, rotation and the cache ────────────────────────────────────────────────────────────────────── */
+
+struct RopeArgs {
+    int T, heads, kv, rot, interleaved;
+    int ldx, ldq, ldk, page_shift;
+    long long slots_in_cache;   /* pages · page, 0 without a cache */
+    float eps;
+    const void *x;
+    void *q, *k, *kc, *vc;
+    const float *gq, *gk, *freq;
+    const int *pos, *slots;
+};
+
+/* One workgroup per row: 16 bytes of a head per lane, a head's lanes side by side, so that the mean square is a
+ * reduction inside a row of lanes. The row's angles are made once, in 64 bits, as turns reduced to an eighth of a circle
+ * (float then holds them to 2^-27 of a radian) and their sines and cosines are shared by all heads through LDS. */
+template <int DT, int DH>
+__global__ __launch_bounds__(256) void qk_norm_rope(RopeArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int VE = kPer16<DT>, LPH = DH / VE, HPP = 256 / LPH;   /* lanes per head, heads per pass */
+    __shared__ float2 turn[DH / 2];   /* (cos, sin) */
+    const int t = blockIdx.x, hl = threadIdx.x / LPH, l = threadIdx.x % LPH, half = a.rot / 2;
+    if ((int)threadIdx.x < half) {
+        const double turns = (double)a.pos[t] * (double)a.freq[threadIdx.x] * 0.15915494309189533577;
+        const double f = turns - __builtin_rint(turns), qd = __builtin_rint(4.0 * f);
+        const float r = (float)(f - 0.25 * qd);   /* |r| <= 1/8 turn */
+        float s, c;
+        sincospif(2.0f * r, &s, &c);
+        const int q = (int)qd & 3;
+        const float cs = (q & 1) ? s : c, sn = (q & 1) ? c : s;
+        turn[threadIdx.x] = float2{(q == 1 || q == 2) ? -cs : cs, (q & 2) ? -sn : sn};
+    }
+    __syncthreads();
+    const E *row = static_cast<const E *>(a.x) + (size_t)t * a.ldx;
+    const int n_heads = a.heads + a.kv * (a.slots_in_cache ? 2 : 1);
+    long long slot = -1;
+    if (a.slots_in_cache) {
+        slot = a.slots[t];
+        if (slot >= a.slots_in_cache) slot = -1;
+    }
+    for (int h = hl; h < n_heads; h += HPP) {
+        const u4 raw = *reinterpret_cast<const u4 *>(row + (size_t)h * DH + VE * l);
+        u4 res = raw;
+        const bool is_q = h < a.heads, is_v = h >= a.heads + a.kv;
+        if (!is_v) {   /* the same for all lanes of a head */
+            float v[VE];
+            unpack<DT>(raw, v);
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VE; i++) ss = __builtin_fmaf(v[i], v[i], ss);
+#pragma unroll
+            for (int o = 1; o < LPH; o *= 2) ss += __shfl_xor(ss, o, LPH);
+            const float inv = 1.0f / sqrtf(ss * (1.0f / DH) + a.eps);
+            const float *gm = (is_q ? a.gq : a.gk) + VE * l;
+#pragma unroll
+            for (int i = 0; i < VE; i++) v[i] = v[i] * inv * gm[i];
+            if (a.interleaved) {
+                if (VE * l < a.rot) {
+#pragma unroll
+                    for (int i = 0; i < VE; i += 2) {
+                        const float2 cs = turn[(VE * l + i) / 2];
+                        const float x = v[i], y = v[i + 1];
+                        v[i] = x * cs.x - y * cs.y;
+                        v[i + 1] = y * cs.x + x * cs.y;
+                    }
+                }
+            } else if (a.rot) {
+                /* elements i and i + rot / 2 are rot / 2 / VE lanes apart: rot is a multiple of 16 */
+                const int d = half / VE;
+                const bool lo = l < d, in = l < 2 * d;
+                const int from = lo ? l + d : in ? l - d : l;
+#pragma unroll
+                for (int i = 0; i < VE; i++) {
+                    const float o = __shfl(v[i], from, LPH);
+                    const float2 cs = turn[(VE * (lo ? l : in ? l - d : 0) + i) & (DH / 2 - 1)];
+                    if (in) v[i] = lo ? v[i] * cs.x - o * cs.y : v[i] * cs.x + o * cs.y;
+                }
+            }
+            res = pack<DT>(v);
+        }
+        const int hk = is_q ? 0 : (h - a.heads) % a.kv;
+        if (is_q)
+            *reinterpret_cast<u4 *>(static_cast<E *>(a.q) + (size_t)t * a.ldq + (size_t)h * DH + VE * l) = res;
+        else if (!is_v && a.k)
+            *reinterpret_cast<u4 *>(static_cast<E *>(a.k) + (size_t)t * a.ldk + (size_t)hk * DH + VE * l) = res;
+        if (!is_q && slot >= 0) {
+            const size_t page = (size_t)(slot >> a.page_shift), off = (size_t)slot & ((1u << a.page_shift) - 1);
+            E *to = static_cast<E *>(is_v ? a.vc : a.kc) + (((page * a.kv + hk) << a.page_shift) + off) * DH + VE * l;
+            *reinterpret_cast<u4 *>(to) = res;
+        }
+    }
+}
+
+/* ── attention over a window ───────────────────────────────────────────────────────────────────────────────── */
+
+struct WinArgs {
+    int q_rows, k_rows, n_seqs, heads, kv, ldq, ldk, ldv, ldo, window, ahead, sinks, tiles;
+    float c;   /* scale · log2 e */
+    const int *qs, *ks;
+    const void *q, *k, *v;
+    void *o;
+};
+
+/* Which sequence and which of its tiles of `rows` queries tile number `id` is: the sequences' tile counts are summed 64 at
+ * a time over the lanes of a wave. False past the last tile. */
+__device__ __forceinline__ bool find_tile(const int *qs, int n_seqs, int q_rows, int rows, int id, int *seq, int *tile)
+{
+    if (!qs) {
+        *seq = 0;
+        *tile = id;
+        return (long long)id * rows < q_rows;
+    }
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int s0 = 0; s0 < n_seqs; s0 += 64) {
+        int n = 0;
+        if (s0 + lane < n_seqs) {
+            int a, b;
+            seq_rows(qs, s0 + lane, q_rows, &a, &b);
+            n = (b - a + rows - 1) / rows;
+        }
+        int sum = n;   /* of this lane's sequence and those before it */
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int v = __shfl_up(sum, o);
+            if (lane >= o) sum += v;
+        }
+        const unsigned long long in = __ballot(id < before + sum);
+        if (in) {
+            const int at = __ffsll(in) - 1;
+            *seq = s0 + at;
+            *tile = id - before - (__shfl(sum, at) - __shfl(n, at));
+            return true;
+        }
+        before += __shfl(sum, 63);
+    }
+    return false;
+}
+
+/* whether 16 bytes of elements hold an infinity or a NaN */
+template <int DT> __device__ __forceinline__ bool odd_values(u4 v)
+{
+    constexpr uint32_t E = DT == T_F32 ? 0x7f800000u : DT == T_F16 ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t H = E & 0xffff0000u, L = E & 0xffffu;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        odd |= (v[i] & H) == H;
+        if (DT != T_F32) odd |= (v[i] & L) == L;
+    }
+    return odd;
+}
+
+/* O for one tile of 32·WQ queries of one head. Each wave owns 32 queries (WK = 1), or the WK waves share 32 queries and
+ * take every WK-th block of KB = 32·NK keys, their sums joined at the end. Blocks without a visible key are not touched.
+ *
+ * Per block and wave S^T = K·Q^T by 32 × 32 products (keys in rows, queries in columns), so that a lane holds 16 keys of
+ * one query: the running maximum and sum of its softmax need one exchange with the lane 32 away, and the weights are
+ * already laid out as the operand of O^T += V^T·P^T, whatever order that product takes the keys in, as V's operand reads
+ * the same order out of LDS. 16-bit weights: the exponentials, at most 1, are rounded to the rows' type for that product
+ * and summed unrounded in 32 bits; fp32 rows multiply in fp32 throughout.
+ *
+ * V rows past the sequence are zeros in LDS. A value that is not finite, in a block where some query must not see it,
+ * would reach that query as 0 · inf: such a block is added key by key with the unseen ones left out. */
+template <int DT, int DH, int WQ, int WK, int NK>
+__global__ __launch_bounds__(256) void attention_win(WinArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    static_assert(WQ * WK == 4, "four waves");
+    constexpr bool F32 = DT == T_F32;
+    constexpr int KB = 32 * NK, RB = WK * KB, QB = 32 * WQ;       /* keys per block and per round, queries */
+    constexpr int EPC = kPer16<DT>, CH = DH / EPC;                /* elements per 16 bytes, those per row */
+    constexpr int VP = F32 ? DH : DH + 32;                        /* V row pitch: 64 bytes on, transposing reads of 8 rows
+                                                                     fall into different banks */
+    constexpr int LD = RB * CH / 256;                             /* 16-byte loads per thread and round, of K and of V */
+    constexpr int TILE_BYTES = RB * (DH + VP) * (int)sizeof(E), JOIN_BYTES = WK > 1 ? WK * 32 * (DH + 2) * 4 : 0;
+    __shared__ __align__(16) unsigned char lds[TILE_BYTES > JOIN_BYTES ? TILE_BYTES : JOIN_BYTES];
+    E *Ks = reinterpret_cast<E *>(lds), *Vs = Ks + RB * DH;
+
+    const int G = a.heads / a.kv, id = blockIdx.x % a.heads;
+    const int kvh = id % a.kv, head = kvh * G + id / a.kv;
+    int seq, tile;
+    /* later tiles, which see more keys, first */
+    if (!find_tile(a.qs, a.n_seqs, a.q_rows, QB, a.tiles - 1 - (int)(blockIdx.x / a.heads), &seq, &tile)) return;
+    int qa, qb, ka, kb;
+    seq_rows(a.qs, seq, a.q_rows, &qa, &qb);
+    seq_rows(a.ks, seq, a.k_rows, &ka, &kb);
+    const int Lq = qb - qa, Lk = kb - ka, i0 = tile * QB, off = Lk - Lq;
+    const int p0 = i0 + off, p1 = imin(i0 + QB, Lq) - 1 + off;   /* the tile's places */
+    const KeyBlocks blocks = key_blocks(p0 - a.window + 1, imin(Lk, p1 + a.ahead + 1), a.sinks, KB);
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    const int wq = WK == 1 ? wave : 0, wk = WK == 1 ? 0 : wave;
+    const int iq = i0 + 32 * wq + col, p = iq + off;
+    const int pw0 = i0 + 32 * wq + off, pw1 = imin(i0 + 32 * wq + 32, Lq) - 1 + off;   /* this wave's places */
+
+    constexpr int QR = DH / (2 * EPC);   /* this lane's query: elements EPC·(2s + h) .. of every 2·EPC */
+    u4 q[QR];
+    {
+        const E *row = static_cast<const E *>(a.q) + (size_t)(qa + imin(iq, Lq - 1)) * a.ldq + (size_t)head * DH;
+#pragma unroll
+        for (int s = 0; s < QR; s++) q[s] = *reinterpret_cast<const u4 *>(row + EPC * (2 * s + h));
+    }
+    f16v o[DH / 32];
+#pragma unroll
+    for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    const E *kh = static_cast<const E *>(a.k) + (size_t)ka * a.ldk + (size_t)kvh * DH;
+    const E *vh = static_cast<const E *>(a.v) + (size_t)ka * a.ldv + (size_t)kvh * DH;
+    u4 kr[LD], vr[LD];
+    auto fetch = [&](int round) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < LD; x++) {
+            const int e = threadIdx.x + 256 * x, r = e / CH, ch = e % CH;
+            const int b = round * WK + r / KB;
+            const int key = b < blocks.total ? blocks.at(b) * KB + r % KB : Lk;
+            kr[x] = vr[x] = u4{0, 0, 0, 0};
+            if (key < Lk) {
+                kr[x] = *reinterpret_cast<const u4 *>(kh + (size_t)key * a.ldk + EPC * ch);
+                vr[x] = *reinterpret_cast<const u4 *>(vh + (size_t)key * a.ldv + EPC * ch);
+            }
+        }
+    };
+    /* whether every query of places pa .. pb sees all KB keys from k0 on */
+    auto all_seen = [&](int k0, int pa, int pb) __attribute__((always_inline)) {
+        const int k1 = k0 + KB - 1;
+        return k1 < Lk && k1 - pa <= a.ahead && (pb - k0 < a.window || k1 < a.sinks);
+    };
+
+    const int rounds = (blocks.total + WK - 1) / WK;
+    if (rounds > 0) fetch(0);
+    for (int round = 0; round < rounds; round++) {
+        bool odd = false, partly = false;
+#pragma unroll
+        for (int w = 0; w < WK; w++) {
+            const int b = round * WK + w;
+            if (b < blocks.total) partly |= !all_seen(blocks.at(b) * KB, p0, p1);
+        }
+        if (partly) {
+            bool mine = false;
+#pragma unroll
+            for (int x = 0; x < LD; x++) mine |= odd_values<DT>(vr[x]);
+            odd = __syncthreads_or(mine);
+        } else {
+            __syncthreads();
+        }
+#pragma unroll
+        for (int x = 0; x < LD; x++) {
+            const int e = threadIdx.x + 256 * x, r = e / CH, ch = e % CH;
+            *reinterpret_cast<u4 *>(Ks + r * DH + EPC * (ch ^ (r & (CH - 1)))) = kr[x];
+            *reinterpret_cast<u4 *>(Vs + r * VP + EPC * ch) = vr[x];
+        }
+        if (round + 1 < rounds) fetch(round + 1);
+        __syncthreads();
+
+        const int b = round * WK + wk;
+        if (b >= blocks.total || pw1 < pw0) continue;
+        const int k0 = blocks.at(b) * KB;
+        /* no query of this wave sees any of the block */
+        if (k0 - pw1 > a.ahead || (pw0 - (k0 + KB - 1) >= a.window && k0 >= a.sinks)) continue;
+        const E *K = Ks + wk * KB * DH, *V = Vs + wk * KB * VP;
+        f16v s[NK];
+#pragma unroll
+        for (int n = 0; n < NK; n++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[n][i] = 0.0f;
+            const int r = 32 * n + col;
+#pragma unroll
+            for (int x = 0; x < QR; x++) {
+                const u4 kk = *reinterpret_cast<const u4 *>(K + r * DH + EPC * ((2 * x + h) ^ (r & (CH - 1))));
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kk[e]), __uint_as_float(q[x][e]), s[n],
+                                                                    0, 0, 0);
+                } else {
+                    s[n] = mfma32<DT>(kk, q[x], s[n]);
+                }
+            }
+        }
+        const bool full = all_seen(k0, pw0, pw1);
+        if (!full) {
+#pragma unroll
+            for (int n = 0; n < NK; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int key = k0 + 32 * n + 8 * (i / 4) + 4 * h + i % 4;
+                    if (!(key < Lk && key_visible(key, p, a.window, a.ahead, a.sinks))) s[n][i] = -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int n = 0; n < NK; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
+        const float mn = fmaxf(m, max_halves(top) * a.c), mu = mn == -INFINITY ? 0.0f : mn;
+        const float fade = exp2_fast(m - mu);
+        m = mn;
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NK; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                s[n][i] = exp2_fast(__builtin_fmaf(s[n][i], a.c, -mu));
+                sum += s[n][i];
+            }
+        l = __builtin_fmaf(l, fade, sum);
+        if (__any(fade != 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < DH / 32; d++) o[d] *= fade;
+        }
+        if (odd && !full) {
+            for (int key = 0; key < KB; key++) {
+                float w = 0.0f;   /* this query's weight of the key, from the lane that has it */
+#pragma unroll
+                for (int n = 0; n < NK; n++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (32 * n + 8 * (i / 4) + i % 4 == (key & ~4)) w = s[n][i];
+                w = __shfl(w, col + ((key & 4) ? 32 : 0));
+                const bool seen = k0 + key < Lk && key_visible(k0 + key, p, a.window, a.ahead, a.sinks);
+#pragma unroll
+                for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float x = Elem<DT>::get(V[key * VP + 32 * d + 8 * (i / 4) + 4 * h + i % 4]);
+                        if (seen) o[d][i] = __builtin_fmaf(w, x, o[d][i]);
+                    }
+            }
+            continue;
+        }
+        if constexpr (F32) {
+#pragma unroll
+            for (int n = 0; n < NK; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const E *row = V + (32 * n + 8 * (i / 4) + 4 * h + i % 4) * VP + col;
+#pragma unroll
+                    for (int d = 0; d < DH / 32; d++)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(row[32 * d], s[n][i], o[d], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NK; n++)
+#pragma unroll
+                for (int k2 = 0; k2 < 2; k2++) {   /* 16 keys: of each eight, this half of the lanes has four */
+                    float w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) w[j] = s[n][8 * k2 + j];
+                    const u4 pw = pack<DT>(w);
+                    const uint16_t *row = reinterpret_cast<const uint16_t *>(V) +
+                                          (32 * n + 16 * k2 + 4 * h + ((lane & 15) >> 2)) * VP + 16 * ((lane >> 4) & 1) +
+                                          4 * (lane & 3);
+#pragma unroll
+                    for (int d = 0; d < DH / 32; d++) {
+                        const u2 va = lds_tr(row + 32 * d), vb = lds_tr(row + 8 * VP + 32 * d);
+                        o[d] = mfma32<DT>(u4{va[0], va[1], vb[0], vb[1]}, pw, o[d]);
+                    }
+                }
+        }
+    }
+    l = sum_halves(l);
+    if constexpr (WK > 1) {
+        /* join the waves' sums: [wave][32 queries][DH + 2], the last two the maximum and the sum */
+        float *J = reinterpret_cast<float *>(lds);
+        __syncthreads();
+        float *mine = J + (wave * 32 + col) * (DH + 2);
+#pragma unroll
+        for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) mine[32 * d + 8 * (i / 4) + 4 * h + i % 4] = o[d][i];
+        if (h == 0) {
+            mine[DH] = m;
+            mine[DH + 1] = l;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < 32 * DH; e += 256) {
+            const int r = e / DH, d = e % DH;
+            if (i0 + r >= Lq) break;
+            float top = -INFINITY, num = 0.0f, den = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WK; w++) top = fmaxf(top, J[(w * 32 + r) * (DH + 2) + DH]);
+            const float mu = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < WK; w++) {
+                const float *j = J + (w * 32 + r) * (DH + 2);
+                const float f = exp2_fast(j[DH] - mu);
+                num = __builtin_fmaf(f, j[d], num);
+                den = __builtin_fmaf(f, j[DH + 1], den);
+            }
+            static_cast<E *>(a.o)[(size_t)(qa + i0 + r) * a.ldo + (size_t)head * DH + d] =
+                Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
+        }
+    } else if (iq < Lq) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        E *row = static_cast<E *>(a.o) + (size_t)(qa + iq) * a.ldo + (size_t)head * DH + 4 * h;
+#pragma unroll
+        for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) row[32 * d + 8 * (i / 4) + i % 4] = Elem<DT>::put(o[d][i] * inv);
+    }
+}
+
+/* ── attention of single tokens over a paged cache ─────────────────────────────────────────────────────────── */
+
+struct PageArgs {
+    int n_seqs, heads, kv, q_groups, splits, page_shift, pages, table_ld, ldq, ldo, window, sinks;
+    float c;
+    const void *q, *kc, *vc;
+    const int *table, *len;
+    void *o;
+    float *part;   /* [sequence][head][split][DH + 2] where splits > 1: sums, maximum, sum of weights */
+};
+
+/* One workgroup: one sequence, one key head, up to 16 of the query heads that read it, one part of its blocks of 32 (fp32:
+ * 16) keys, which its four waves take in turn. Per block S^T = K·Q^T by 16 × 16 products, K's operand straight from the
+ * pages (a lane reads 16 bytes of one key), then O^T += V^T·P^T as in attention_win: 16-bit V passes through LDS for its
+ * transposing read, fp32 V is read as the operand takes it. Keys that are not seen (past the end, outside the window, in
+ * a page that is not there) have no weight and their V is zeros, whatever lies in the page. */
+template <int DT, int DH>
+__global__ __launch_bounds__(256) void attention_page(PageArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr bool F32 = DT == T_F32;
+    constexpr int KB = F32 ? 16 : 32, EPC = kPer16<DT>, VP = DH + 16, NT = DH / 16;
+    constexpr int V_BYTES = F32 ? 0 : 4 * KB * VP * 2, J_BYTES = 4 * 16 * (DH + 2) * 4;
+    __shared__ __align__(16) unsigned char lds[V_BYTES > J_BYTES ? V_BYTES : J_BYTES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int split = blockIdx.x % a.splits, kvh = (blockIdx.x / a.splits) % a.kv;
+    const int qg = (blockIdx.x / a.splits / a.kv) % a.q_groups, seq = blockIdx.x / a.splits / a.kv / a.q_groups;
+    const int G = a.heads / a.kv, nq = imin(16, G - 16 * qg), head0 = kvh * G + 16 * qg;
+
+    const int *row = a.table + (size_t)seq * a.table_ld;
+    const int len = kept_length(a.len[seq], a.table_ld, 1 << a.page_shift);
+    const int w0 = imax(len - a.window, 0);
+    const KeyBlocks blocks = key_blocks(w0, len, a.sinks, KB);
+    int b0, b1;
+    split_range(blocks.total, a.splits, split, &b0, &b1);
+
+    u4 q[DH / (4 * EPC)];
+    {
+        const E *p = static_cast<const E *>(a.q) + (size_t)seq * a.ldq + (size_t)(head0 + imin(c, nq - 1)) * DH;
+#pragma unroll
+        for (int s = 0; s < DH / (4 * EPC); s++) q[s] = *reinterpret_cast<const u4 *>(p + EPC * (4 * s + g));
+    }
+    f4 o[NT];
+#pragma unroll
+    for (int d = 0; d < NT; d++) o[d] = f4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+    const size_t page_elems = (size_t)DH << a.page_shift;   /* of one head */
+    const E *kc = static_cast<const E *>(a.kc) + kvh * page_elems, *vc = static_cast<const E *>(a.vc) + kvh * page_elems;
+    const int in_page = (1 << a.page_shift) - 1;
+    auto seen = [&](int key) __attribute__((always_inline)) { return key < len && (key >= w0 || key < a.sinks); };
+
+    for (int b = b0 + wave; b < b1; b += 4) {
+        const int k0 = __builtin_amdgcn_readfirstlane(blocks.at(b) * KB);
+        int page[KB / 16];   /* of each 16 keys; pages hold at least 16 */
+        bool whole = true;
+#pragma unroll
+        for (int t = 0; t < KB / 16; t++) {
+            const int key = k0 + 16 * t;
+            page[t] = key < len ? page_of(row, a.table_ld, key, a.page_shift, a.pages) : -1;
+            whole &= page[t] >= 0 && key + 15 < len && (key >= w0 || key + 15 < a.sinks);
+        }
+        f4 s[KB / 16];
+        if constexpr (F32) {
+            s[0] = f4{0, 0, 0, 0};
+            float v[4][NT];
+            if (page[0] >= 0) {
+                const size_t at = (size_t)page[0] * a.kv * page_elems + (size_t)(k0 & in_page) * DH;
+                f4 s1 = {0, 0, 0, 0};
+                u4 k[NT];
+#pragma unroll
+                for (int x = 0; x < NT; x++) k[x] = *reinterpret_cast<const u4 *>(kc + at + c * DH + 4 * (4 * x + g));
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int d = 0; d < NT; d++) v[i][d] = vc[at + (4 * g + i) * DH + 16 * d + c];
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[x][e]), __uint_as_float(q[x][e]),
+                                                                    s[0], 0, 0, 0);
+                        s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[x][e + 1]),
+                                                                  __uint_as_float(q[x][e + 1]), s1, 0, 0, 0);
+                    }
+                s[0] += s1;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int d = 0; d < NT; d++) v[i][d] = 0.0f;
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (page[0] < 0 || !seen(k0 + 4 * g + i)) {
+                        s[0][i] = -INFINITY;
+#pragma unroll
+                        for (int d = 0; d < NT; d++) v[i][d] = 0.0f;
+                    }
+            }
+            const float top = max_quarters(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])));
+            const float mn = fmaxf(m, top * a.c), mu = mn == -INFINITY ? 0.0f : mn, fade = exp2_fast(m - mu);
+            m = mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s[0][i] = exp2_fast(__builtin_fmaf(s[0][i], a.c, -mu));
+                sum += s[0][i];
+            }
+            l = __builtin_fmaf(l, fade, sum);
+#pragma unroll
+            for (int d = 0; d < NT; d++) {
+                o[d] *= fade;
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d], s[0][i], o[d], 0, 0, 0);
+            }
+        } else {
+            constexpr int CH = DH / 8, RPL = 64 / CH;   /* 16-byte pieces of a row, rows per load */
+            u4 k[2][DH / 32], v[KB / RPL];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const size_t at = (size_t)imax(page[t], 0) * a.kv * page_elems + (size_t)((k0 + 16 * t) & in_page) * DH;
+                if (page[t] >= 0) {
+#pragma unroll
+                    for (int x = 0; x < DH / 32; x++)
+                        k[t][x] = *reinterpret_cast<const u4 *>(kc + at + c * DH + 8 * (4 * x + g));
+#pragma unroll
+                    for (int r = 0; r < 16 / RPL; r++)
+                        v[t * 16 / RPL + r] = *reinterpret_cast<const u4 *>(vc + at + (RPL * r) * DH + 8 * lane);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < DH / 32; x++) k[t][x] = u4{0, 0, 0, 0};
+#pragma unroll
+                    for (int r = 0; r < 16 / RPL; r++) v[t * 16 / RPL + r] = u4{0, 0, 0, 0};
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                s[t] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int x = 0; x < DH / 32; x++) s[t] = mfma16<DT>(k[t][x], q[x], s[t]);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (page[t] < 0 || !seen(k0 + 16 * t + 4 * g + i)) s[t][i] = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < KB / RPL; r++)
+                    if (!seen(k0 + RPL * r + lane / CH)) v[r] = u4{0, 0, 0, 0};
+            }
+            uint16_t *Vs = reinterpret_cast<uint16_t *>(lds) + wave * KB * VP;
+#pragma unroll
+            for (int r = 0; r < KB / RPL; r++)
+                *reinterpret_cast<u4 *>(Vs + (RPL * r + lane / CH) * VP + 8 * (lane % CH)) = v[r];
+            float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                              fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+            top = max_quarters(top);
+            const float mn = fmaxf(m, top * a.c), mu = mn == -INFINITY ? 0.0f : mn, fade = exp2_fast(m - mu);
+            m = mn;
+            float sum = 0.0f, w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                w[i] = exp2_fast(__builtin_fmaf(s[i / 4][i % 4], a.c, -mu));
+                sum += w[i];
+            }
+            l = __builtin_fmaf(l, fade, sum);
+            const u4 pw = pack<DT>(w);
+            /* a wave's LDS operations complete in order, and no other wave touches its part; the fence keeps the
+             * compiler from moving the reads above the writes */
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const uint16_t *vp = Vs + (4 * g + (c >> 2)) * VP + 4 * (c & 3);
+#pragma unroll
+            for (int d = 0; d < NT; d++) {
+                const u2 va = lds_tr(vp + 16 * d), vb = lds_tr(vp + 16 * VP + 16 * d);
+                o[d] = mfma16<DT>(u4{va[0], va[1], vb[0], vb[1]}, pw, o[d] * fade);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    l = sum_quarters(l);
+    /* join the four waves' sums: [wave][16 heads][DH + 2] */
+    float *J = reinterpret_cast<float *>(lds);
+    __syncthreads();
+    float *mine = J + (wave * 16 + c) * (DH + 2);
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mine[16 * d + 4 * g + i] = o[d][i];
+    if (g == 0) {
+        mine[DH] = m;
+        mine[DH + 1] = l;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < nq * DH; e += 256) {
+        const int r = e / DH, d = e % DH;
+        float top = -INFINITY, num = 0.0f, den = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) top = fmaxf(top, J[(w * 16 + r) * (DH + 2) + DH]);
+        const float mu = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float *j = J + (w * 16 + r) * (DH + 2);
+            const float f = exp2_fast(j[DH] - mu);
+            num = __builtin_fmaf(f, j[d], num);
+            den = __builtin_fmaf(f, j[DH + 1], den);
+        }
+        if (a.splits == 1) {
+            static_cast<E *>(a.o)[(size_t)seq * a.ldo + (size_t)(head0 + r) * DH + d] =
+                Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
+        } else {
+            float *to = a.part + (((size_t)seq * a.heads + head0 + r) * a.splits + split) * (DH + 2);
+            to[d] = num;
+            if (d == 0) {
+                to[DH] = top;
+                to[DH + 1] = den;
+            }
+        }
+    }
+}
+
+/* The parts of one sequence's head added up: one workgroup of DH threads. */
+template <int DT, int DH>
+__global__ __launch_bounds__(DH) void attention_join(PageArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    const int seq = blockIdx.x / a.heads, head = blockIdx.x % a.heads, d = threadIdx.x;
+    const float *p = a.part + ((size_t)seq * a.heads + head) * a.splits * (DH + 2);
+    float top = -INFINITY, num = 0.0f, den = 0.0f;
+    for (int s = 0; s < a.splits; s++) top = fmaxf(top, p[s * (DH + 2) + DH]);
+    const float mu = top == -INFINITY ? 0.0f : top;
+    for (int s = 0; s < a.splits; s++) {
+        const float f = exp2_fast(p[s * (DH + 2) + DH] - mu);
+        num = __builtin_fmaf(f, p[s * (DH + 2) + d], num);
+        den = __builtin_fmaf(f, p[s * (DH + 2) + DH + 1], den);
+    }
+    static_cast<E *>(a.o)[(size_t)seq * a.ldo + (size_t)head * DH + d] = Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
+}
+
+}  // namespace p2k

@@ -1,0 +1,83 @@
+/*  p2hip_index.h – which keys an attention kernel reads and where they lie: the arithmetic on positions, windows and
+ *  pages, apart from the kernels so that a host program can go over it (plain C++, no HIP types).
+ */
+#pragma once
+
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#define P2_HD __host__ __device__ __forceinline__
+#else
+#define P2_HD inline
+#endif
+
+namespace p2k {
+
+P2_HD int imin(int a, int b) { return a < b ? a : b; }
+P2_HD int imax(int a, int b) { return a > b ? a : b; }
+
+/* The aligned blocks of `bs` keys that hold a visible key, in order: blocks 0 .. sink − 1, then first, first + 1, …;
+ * `total` of them. Visible are keys [lo, hi) and the keys below `sinks` among [0, hi). */
+struct KeyBlocks {
+    int sink, first, total;
+    P2_HD int at(int b) const { return b < sink ? b : first + (b - sink); }
+};
+
+P2_HD KeyBlocks key_blocks(int lo, int hi, int sinks, int bs)
+{
+    KeyBlocks k{0, 0, 0};
+    if (hi <= 0) return k;
+    lo = imin(imax(lo, 0), hi);
+    const int s1 = imin(sinks, lo);
+    k.first = lo / bs;
+    const int end = lo < hi ? (hi - 1) / bs + 1 : k.first;
+    k.sink = s1 > 0 ? (s1 - 1) / bs + 1 : 0;
+    if (end > k.first) k.sink = imin(k.sink, k.first);   /* block `first` comes once */
+    k.total = k.sink + end - k.first;
+    return k;
+}
+
+/* Whether key j is visible to the query at place p. */
+P2_HD bool key_visible(int j, int p, int window, int ahead, int sinks)
+{
+    return j - p <= ahead && (p - j < window || j < sinks);
+}
+
+/* Part s of `splits` of `total` blocks: [begin, end). */
+P2_HD void split_range(int total, int splits, int s, int *begin, int *end)
+{
+    const int per = (total + splits - 1) / splits;
+    *begin = imin(per * s, total);
+    *end = imin(*begin + per, total);
+}
+
+/* The page of key t of a sequence whose table row has table_ld entries, or −1 where the table has none or a number
+ * outside the cache. Reads the table only inside the row. */
+P2_HD int page_of(const int32_t *row, int table_ld, int t, int page_shift, int pages)
+{
+    const int i = t >> page_shift;
+    if (t < 0 || i >= table_ld) return -1;
+    const int e = row[i];
+    return (uint32_t)e < (uint32_t)pages ? e : -1;
+}
+
+/* A sequence's length as the kernels take it. */
+P2_HD int kept_length(int len, int table_ld, int page)
+{
+    const long long most = (long long)table_ld * page;
+    return len < 0 ? 0 : len > most ? (int)most : len;
+}
+
+/* Sequence s's rows as the kernels take them: [a, b) inside [0, rows]. */
+P2_HD void seq_rows(const int32_t *start, int s, int rows, int *a, int *b)
+{
+    if (!start) {
+        *a = 0;
+        *b = rows;
+        return;
+    }
+    *a = imin(imax(start[s], 0), rows);
+    *b = imin(imax(start[s + 1], *a), rows);
+}
+
+}  // namespace p2k

@@ -19,6 +19,9 @@ BLAS_SO = os.path.join(LIBDIR, "libphonon2_gemm.so")
 INT8, EXACT, INT8W = 0, 1, 2
 MODES = {"int8": INT8, "exact": EXACT, "int8w": INT8W}
 Q_KALIGN = 128
+F32, F16, BF16 = 0, 1, 2
+TYPES = {"f32": F32, "f16": F16, "bf16": BF16}
+EVERY_KEY = 1 << 30   # a window or look-ahead that reaches everything
 
 
 class P2Error(RuntimeError):
@@ -108,6 +111,18 @@ _HIP_SIG = {
     "p2h_channel_major_rows": (_i, [_i, _vp, _vp, _vp]),
     "p2h_conformer_block_workspace_bytes": (_sz, [_i, _i]),
     "p2h_conformer_block": (_i, [_i, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
+    "p2h_q4_weight_upload": (_vp, [_vp, _vp, _vp, _i, _i, _i]),
+    "p2h_q4_weight_wrap": (_vp, [_vp, _vp, _vp, _i, _i, _i]),
+    "p2h_q4_weight_free": (None, [_vp]),
+    "p2h_q4_weight_shape": (_i, [_vp, C.POINTER(_i), C.POINTER(_i), C.POINTER(_i)]),
+    "p2h_q4_weight_device_bytes": (_sz, [_vp]),
+    "p2h_q4_gemv": (_i, [_i, _i, _i, _i, _f, _vp, _i, _vp, _f, _vp, _i, _vp]),
+    "p2h_qk_norm_rope": (_i, [_i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _f, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp,
+                              _vp]),
+    "p2h_attention_window": (_i, [_i, _i, _i, _i, _vp, _vp, _i, _i, _i, _vp, _i, _vp, _i, _vp, _i, _f, _i, _i, _i, _vp,
+                                  _i, _vp]),
+    "p2h_attention_paged_workspace_bytes": (_sz, [_vp, _i, _i, _i, _i, _i]),
+    "p2h_attention_paged": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _f, _i, _i, _vp, _i, _vp, _sz, _vp]),
 }
 
 _hip = None
@@ -859,6 +874,92 @@ def stack_workspace_bytes(mode, T, n_blocks):
 
 def block_workspace_bytes(mode, T):
     return hip().p2h_conformer_block_workspace_bytes(MODES.get(mode, mode), T)
+
+
+# ── a decoder layer's step: 4-bit linears, head norms with rotation, attention over many or cached keys ───────────
+# Device-pointer entry points, asynchronous on `stream`; dtype "f32", "f16" or "bf16" is the type of every row and cache.
+
+class Q4Weight:
+    """A device-resident weight [K, N] of 4-bit codes [K, ceil(N/2)] with fp16 scales [ceil(K/group), N] and, if given,
+    zero points packed as the codes, uploaded from host arrays."""
+
+    def __init__(self, codes, scales, zeros, K, N, group):
+        c = np.ascontiguousarray(codes, np.uint8)
+        s = np.ascontiguousarray(scales, np.float16)
+        z = None if zeros is None else np.ascontiguousarray(zeros, np.uint8)
+        groups, half = -(-K // group), (N + 1) // 2
+        assert c.size == K * half and s.size == groups * N and (z is None or z.size == groups * half)
+        self.K, self.N, self.group = K, N, group
+        self.ptr = hip().p2h_q4_weight_upload(c.ctypes.data, s.ctypes.data, None if z is None else z.ctypes.data, K, N,
+                                              group)
+        if not self.ptr:
+            raise P2Error(f"p2h_q4_weight_upload: {last_error()}")
+
+    @classmethod
+    def wrap(cls, d_codes, d_scales, d_zeros, K, N, group):
+        """A weight made from codes, scales and zero points (or None) in device memory, read during the call only."""
+        self = cls.__new__(cls)
+        self.K, self.N, self.group, self.ptr = K, N, group, None
+        self.ptr = hip().p2h_q4_weight_wrap(d_codes, d_scales, d_zeros, K, N, group)
+        if not self.ptr:
+            raise P2Error(f"p2h_q4_weight_wrap: {last_error()}")
+        return self
+
+    def device_bytes(self):
+        return hip().p2h_q4_weight_device_bytes(self.ptr)
+
+    def free(self):
+        if self.ptr:
+            hip().p2h_q4_weight_free(self.ptr)
+            self.ptr = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class KvCache(C.Structure):
+    """P2hKvCache: `pages` pages of `page` tokens of `heads` key heads at device addresses dK and dV, each
+    [pages][heads][page][head_dim]. The memory stays the caller's."""
+    _fields_ = [("dtype", _i), ("heads", _i), ("head_dim", _i), ("page", _i), ("pages", _i), ("K", _vp), ("V", _vp)]
+
+    def __init__(self, dtype, heads, head_dim, page, pages, dK, dV):
+        super().__init__(TYPES.get(dtype, dtype), heads, head_dim, page, pages, dK, dV)
+
+
+def q4_gemv_dev(dtype, M, N, K, alpha, dX, ldx, w, beta, dY, ldy, stream=None):
+    """Y [M, N] = alpha·X·W + beta·Y for a Q4Weight w and few rows."""
+    _ok(hip().p2h_q4_gemv(TYPES.get(dtype, dtype), M, N, K, alpha, dX, ldx, w.ptr, beta, dY, ldy, stream),
+        "p2h_q4_gemv")
+
+
+def qk_norm_rope_dev(dtype, T, heads, kv_heads, head_dim, dQKV, ldqkv, dGammaQ, dGammaK, eps, rot, interleaved, dFreq,
+                     dPos, dQ, ldq, dK=None, ldk=0, cache=None, dSlots=None, stream=None):
+    """Norm and rotation of the query and key heads of q | k | v rows; keys (and values) into a KvCache if given."""
+    _ok(hip().p2h_qk_norm_rope(TYPES.get(dtype, dtype), T, heads, kv_heads, head_dim, dQKV, ldqkv, dGammaQ, dGammaK, eps,
+                               rot, int(interleaved), dFreq, dPos, dQ, ldq, dK, ldk,
+                               None if cache is None else C.byref(cache), dSlots, stream), "p2h_qk_norm_rope")
+
+
+def attention_window_dev(dtype, q_rows, k_rows, n_seqs, dQStart, dKStart, heads, kv_heads, head_dim, dQ, ldq, dK, ldk,
+                         dV, ldv, scale, window, ahead, sinks, dO, ldo, stream=None):
+    """Attention of packed sequences over `window` places back, `ahead` on and the first `sinks`."""
+    _ok(hip().p2h_attention_window(TYPES.get(dtype, dtype), q_rows, k_rows, n_seqs, dQStart, dKStart, heads, kv_heads,
+                                   head_dim, dQ, ldq, dK, ldk, dV, ldv, scale, window, ahead, sinks, dO, ldo, stream),
+        "p2h_attention_window")
+
+
+def attention_paged_workspace_bytes(cache, n_seqs, heads, max_len, window=EVERY_KEY, sinks=0):
+    return hip().p2h_attention_paged_workspace_bytes(C.byref(cache), n_seqs, heads, max_len, window, sinks)
+
+
+def attention_paged_dev(cache, n_seqs, heads, dQ, ldq, dTable, table_ld, dLen, max_len, scale, window, sinks, dO, ldo,
+                        ws=None, ws_bytes=0, stream=None):
+    """One new token per sequence over a KvCache."""
+    _ok(hip().p2h_attention_paged(C.byref(cache), n_seqs, heads, dQ, ldq, dTable, table_ld, dLen, max_len, scale, window,
+                                  sinks, dO, ldo, ws, ws_bytes, stream), "p2h_attention_paged")
 
 
 # ── the generator ───────────────────────────────────────────────────────────────────────────────────────────────

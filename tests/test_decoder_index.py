@@ -1,0 +1,91 @@
+"""The index arithmetic of the attention kernels (phonon-2-c_amd/csrc/p2hip_index.h), compiled for the host and gone over by
+brute force: which key blocks are taken, how they are split, and that no page table is read outside its row."""
+import os
+import subprocess
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+CSRC = os.path.join(os.path.dirname(HERE), "phonon-2-c_amd", "csrc")
+
+PROGRAM = r"""
+#include <cstdio>
+#include <cstdlib>
+#include <vector>
+#include <climits>
+#include "p2hip_index.h"
+using namespace p2k;
+#define CHECK(c) do { if (!(c)) { printf("line %d: %s\n", __LINE__, #c); return 1; } } while (0)
+
+int main()
+{
+    /* every block with a visible key comes once, no other does, and the splits hand each out once */
+    const int sinks[] = {0, 1, 3, 16, 17, 40, 200, 1 << 30}, bss[] = {16, 32, 64};
+    for (int bs : bss)
+        for (int hi = 0; hi <= 150; hi++)
+            for (int lo = -3; lo <= hi; lo++)
+                for (int sk : sinks) {
+                    const KeyBlocks k = key_blocks(lo, hi, sk, bs);
+                    std::vector<int> want, got;
+                    for (int b = 0; b * bs < hi; b++) {
+                        bool any = false;
+                        for (int j = b * bs; j < (b + 1) * bs && j < hi; j++) any |= j >= lo || j < sk;
+                        if (any) want.push_back(b);
+                    }
+                    for (int i = 0; i < k.total; i++) got.push_back(k.at(i));
+                    CHECK(got == want);
+                    for (int splits : {1, 2, 3, 7, 256}) {
+                        int next = 0;
+                        for (int s = 0; s < splits; s++) {
+                            int a, b;
+                            split_range(k.total, splits, s, &a, &b);
+                            CHECK(a == next || (a == k.total && b == a));
+                            CHECK(a <= b && b <= k.total);
+                            if (b > a) next = b;
+                        }
+                        CHECK(next == k.total);
+                    }
+                }
+    /* the largest places and windows do not overflow */
+    const int big = (1 << 30) - 1;
+    CHECK(key_blocks(big - (1 << 30) + 1, big, 0, 64).total == (big - 1) / 64 + 1);
+    CHECK(key_blocks(-(1 << 30) - (1 << 30) + 1, 5, 1 << 30, 32).total == 1);
+    CHECK(key_visible(0, big - 1, 1 << 30, 0, 0) && !key_visible(big - 1, -big, 1 << 30, 1 << 30, 1 << 30));
+    CHECK(!key_visible(5, 4, 3, 0, 100) && key_visible(5, 4, 3, 1, 0) && !key_visible(1, 4, 3, 0, 0) && key_visible(1, 4, 3, 0, 2));
+
+    /* pages: the row lies between guards that must not be read (they would give a page inside the cache) */
+    const int ld = 5, pages = 9;
+    int32_t mem[ld + 2] = {3, 0, 8, -1, 9, INT_MIN, 3};
+    const int32_t *row = mem + 1;
+    const int want[ld] = {0, 8, -1, -1, -1};
+    for (int shift = 4; shift <= 10; shift++)
+        for (long long t = -20; t < (8ll << shift); t++) {
+            const int p = page_of(row, ld, (int)t, shift, pages);
+            CHECK(p == (t >= 0 && (t >> shift) < ld ? want[t >> shift] : -1));
+        }
+    CHECK(page_of(row, 0, 0, 4, pages) == -1 && page_of(row, ld, INT_MAX, 4, pages) == -1 && page_of(row, ld, 0, 4, 0) == -1);
+    CHECK(kept_length(-1, 5, 16) == 0 && kept_length(81, 5, 16) == 80 && kept_length(80, 5, 16) == 80);
+    CHECK(kept_length(INT_MAX, 1 << 20, 1024) == 1 << 30 && kept_length(7, 0, 16) == 0);
+
+    /* rows of a sequence stay inside the rows, whatever the starts */
+    const int32_t st[] = {-4, 3, 2, INT_MAX, INT_MIN, 50, 12};
+    for (int s = 0; s < 6; s++)
+        for (int rows : {0, 1, 10, 40}) {
+            int a, b;
+            seq_rows(st, s, rows, &a, &b);
+            CHECK(a >= 0 && a <= b && b <= rows);
+        }
+    int a, b;
+    seq_rows(nullptr, 0, 12, &a, &b);
+    CHECK(a == 0 && b == 12);
+    puts("ok");
+    return 0;
+}
+"""
+
+
+def test_index_arithmetic(tmp_path):
+    src, exe = tmp_path / "index.cpp", tmp_path / "index"
+    src.write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                    "-I", CSRC, "-o", str(exe), str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr

@@ -1,0 +1,552 @@
+"""A decoder layer's step on the GPU against plain 64-bit forms: 4-bit linears, head norms with rotation, windowed and paged
+attention, alone and together. Bounds are counted in tests/_decoder.py."""
+import numpy as np
+import pytest
+
+import _decoder as D
+import p2gemm as P
+
+pytestmark = pytest.mark.gpu
+
+EVERY = P.EVERY_KEY
+
+
+def rng_of(*key):
+    return np.random.default_rng([sum(str(k).encode()) for k in key])
+
+
+# ── 4-bit weights ───────────────────────────────────────────────────────────────────────────────────────────────
+
+Q4 = [(1, 1, 1, 32, False), (1, 31, 17, 32, True), (2, 33, 16, 64, True), (3, 128, 16, 128, False),
+      (16, 130, 33, 64, True), (17, 1000, 48, 32, True), (5, 4096, 250, 128, False), (1, 1024, 1024, 128, False),
+      (33, 257, 100, 128, True), (4, 2049, 31, 32, False)]
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("M,K,N,group,zeros", Q4)
+def test_q4(t, M, K, N, group, zeros):
+    rng = rng_of(t, M, K, N, group)
+    x, wt = D.rows(rng, t, M, K), D.q4_weight(rng, K, N, group, zeros)
+    got = D.to_f64(t, D.run_q4(t, x, wt, K, N, group))
+    w, x64 = D.q4_values(*wt, K, N, group), D.to_f64(t, x)
+    D.check(got, x64 @ w, D.q4_bound(t, x64, w, x64 @ w, 1.0, K), f"{t} {M}x{K}x{N}")
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_q4_pitches_alpha_beta(t):
+    M, K, N, group = 6, 300, 37, 64
+    rng = rng_of(t, "pitch")
+    x, wt, y0 = D.rows(rng, t, M, K), D.q4_weight(rng, K, N, group, True), D.rows(rng, t, M, N + 5)
+    got = D.to_f64(t, D.run_q4(t, x, wt, K, N, group, 0.75, -1.5, y0, K + 3, N + 5))
+    w, x64, old = D.q4_values(*wt, K, N, group), D.to_f64(t, x), D.to_f64(t, y0)
+    want = 0.75 * (x64 @ w) - 1.5 * old[:, :N]
+    D.check(got[:, :N], want, D.q4_bound(t, x64, w, want, 0.75, K) + 4 * D.FP32 * np.abs(old[:, :N]), t)
+    assert np.array_equal(got[:, N:], old[:, N:])
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_q4_rows_do_not_depend_on_their_number(t):
+    K, N, group = 1500, 80, 32
+    rng = rng_of(t, "rows")
+    x, wt = D.rows(rng, t, 19, K), D.q4_weight(rng, K, N, group, True)
+    many = D.run_q4(t, x, wt, K, N, group)
+    for m in (0, 3, 16, 18):
+        assert np.array_equal(D.run_q4(t, x[m:m + 1], wt, K, N, group)[0], many[m])
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_q4_every_code_and_zero(t):
+    """One row picked by a unit vector gives w itself: (code − zero)·scale, rounded once."""
+    K, N, group = 256, 16, 32
+    codes = np.tile(np.arange(256, dtype=np.uint8)[:, None], (1, 8))
+    zeros = np.tile(np.array([[0x10, 0x32, 0x54, 0x76, 0x98, 0xBA, 0xDC, 0xFE]], np.uint8), (8, 1))
+    scales = np.full((8, N), 2.0 ** -3, np.float16)
+    x = D.to_type(t, np.eye(256)[:, :K])
+    got = D.to_f64(t, D.run_q4(t, x, (codes, scales, zeros), K, N, group))
+    assert np.array_equal(got, D.q4_values(codes, scales, zeros, K, N, group))
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_q4_wide_range_and_non_finite(t):
+    K, N, group = 200, 32, 64
+    rng = rng_of(t, "inf")
+    big = 6e4 if t == "f16" else 1e30
+    wt = D.q4_weight(rng, K, N, group, False)
+    w = D.q4_values(*wt, K, N, group)
+    x = rng.standard_normal((5, K))
+    x[0, 3] = np.inf
+    x[1, 5] = np.nan
+    x[2] = 0.0
+    x[3, ::7] *= big / 100
+    x[4, 11] = -np.inf
+    xt = D.to_type(t, x)
+    got = D.to_f64(t, D.run_q4(t, xt, wt, K, N, group))
+    with np.errstate(invalid="ignore"):
+        want = D.to_f64(t, xt) @ w
+    assert np.isnan(got[1]).all() and (got[2] == 0).all()
+    for r in (0, 4):   # ±inf by the sign of its weight, NaN where that is 0
+        assert np.array_equal(np.isnan(got[r]), np.isnan(want[r]))
+        ok = ~np.isnan(want[r])
+        assert np.array_equal(got[r][ok], want[r][ok])
+    with np.errstate(over="ignore"):
+        lim = D.to_f64(t, D.to_type(t, want[3]))
+    fin = np.isfinite(lim)
+    x3 = D.to_f64(t, xt[3:4])
+    D.check(got[3:4, fin], want[3:4, fin], D.q4_bound(t, x3, w, want[3:4], 1.0, K)[:, fin], t)
+
+
+def test_q4_bytes_and_wrap():
+    K, N, group = 1024, 256, 128
+    rng = rng_of("wrap")
+    wt = D.q4_weight(rng, K, N, group, True)
+    d = [D.device(a) for a in wt]
+    w = P.Q4Weight.wrap(d[0].ptr, d[1].ptr, d[2].ptr, K, N, group)
+    assert w.device_bytes() == K * N // 2 + 4 * (K // group) * N
+    for b in d:
+        b.upload(np.zeros(b.nbytes, np.uint8))   # the codes are not read after the call
+    x = D.rows(rng, "f32", 2, K)
+    dx, dy = D.device(x), D.preset("f32", (2, N))
+    P.q4_gemv_dev("f32", 2, N, K, 1.0, dx.ptr, K, w, 0.0, dy.ptr, N)
+    assert np.array_equal(dy.download((2, N), np.float32), D.run_q4("f32", x, wt, K, N, group))
+
+
+# ── norm, rotation and the cache ────────────────────────────────────────────────────────────────────────────────
+
+def run_rope(t, qkv, H, Hk, Dh, gq, gk, eps, rot, inter, freq, pos, page=0, pages=0, slots=None, keys=True, pad=0,
+             in_place=False, stream=None):
+    T, W = qkv.shape
+    dx, dgq, dgk = D.device(qkv), D.device(gq), D.device(gk)
+    df, dp = D.device(np.asarray(freq, np.float32)), D.device(np.asarray(pos, np.int32))
+    ldq, ldk = (W, W) if in_place else (H * Dh + pad, Hk * Dh + pad)
+    dq = dx if in_place else D.preset(t, (max(T, 1), ldq))
+    dk = (dx if in_place else D.preset(t, (max(T, 1), ldk))) if keys else None
+    cache, ds, kc, vc = None, None, None, None
+    if pages:
+        fill = np.full((pages, Hk, page, Dh), 3.0)
+        kc, vc = D.device(D.to_type(t, fill)), D.device(D.to_type(t, -fill))
+        cache = P.KvCache(t, Hk, Dh, page, pages, kc.ptr, vc.ptr)
+        ds = D.device(np.asarray(slots, np.int32))
+    P.qk_norm_rope_dev(t, T, H, Hk, Dh, dx.ptr, W, dgq.ptr, dgk.ptr, eps, rot, inter, df.ptr, dp.ptr, dq.ptr, ldq,
+                       None if dk is None else dk.ptr + (H * Dh * D.size(t) if in_place else 0), ldk, cache,
+                       ds.ptr if ds else None, stream)
+    out = [dq.download((T, ldq), D.np_type(t), stream)]
+    out.append(dk.download((T, ldk), D.np_type(t), stream) if keys and not in_place else None)
+    if pages:
+        out += [b.download((pages, Hk, page, Dh), D.np_type(t), stream) for b in (kc, vc)]
+    return out
+
+
+ROPE = [(1, 1, 1, 64, 64, False), (3, 4, 2, 128, 128, True), (5, 8, 8, 128, 64, False), (2, 6, 3, 64, 16, True),
+        (7, 32, 8, 128, 128, False), (4, 5, 1, 128, 0, False), (130, 3, 1, 64, 48, False), (2, 40, 8, 64, 32, False)]
+
+
+def rope_inputs(t, T, H, Hk, Dh, rot, key, far=100000):
+    rng = rng_of(t, T, H, Dh, rot, key)
+    qkv = D.rows(rng, t, T, (H + 2 * Hk) * Dh, scale=3.0)
+    gq, gk = (rng.uniform(-1.5, 1.5, Dh).astype(np.float32) for _ in range(2))
+    freq = (10000.0 ** (-np.arange(0, max(rot, 2), 2) / max(rot, 1))).astype(np.float32)
+    return rng, qkv, gq, gk, freq, rng.integers(0, far, T).astype(np.int32)
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("T,H,Hk,Dh,rot,inter", ROPE)
+def test_rope(t, T, H, Hk, Dh, rot, inter):
+    rng, qkv, gq, gk, freq, pos = rope_inputs(t, T, H, Hk, Dh, rot, "plain")
+    q, k = run_rope(t, qkv, H, Hk, Dh, gq, gk, 1e-6, rot, inter, freq, pos, pad=16)
+    x = D.to_f64(t, qkv).reshape(T, H + 2 * Hk, Dh)
+    for got, part, g, n in ((q, x[:, :H], gq, H), (k, x[:, H:H + Hk], gk, Hk)):
+        want, size_of = D.norm_rope(part, g, 1e-6, rot, inter, freq, pos)
+        D.check(D.to_f64(t, got[:, :n * Dh]).reshape(T, n, Dh), want, D.rope_bound(t, want, size_of, Dh), t)
+        assert (got[:, n * Dh:].view(np.uint16) == 0xFFFF).all()   # the pitch's pad is left as it was
+    inq = run_rope(t, qkv, H, Hk, Dh, gq, gk, 1e-6, rot, inter, freq, pos, in_place=True)[0]
+    assert np.array_equal(inq[:, :H * Dh], q[:, :H * Dh])
+    assert np.array_equal(inq[:, H * Dh:(H + Hk) * Dh], k[:, :Hk * Dh])
+    assert np.array_equal(inq[:, (H + Hk) * Dh:], qkv[:, (H + Hk) * Dh:])
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("page", (16, 64))
+def test_rope_into_the_cache(t, page):
+    T, H, Hk, Dh, rot, pages = 21, 6, 3, 128, 128, 5
+    rng, qkv, gq, gk, freq, pos = rope_inputs(t, T, H, Hk, Dh, rot, page)
+    slots = rng.permutation(pages * page)[:T].astype(np.int32)
+    slots[4], slots[9], slots[13] = -1, pages * page, 2 ** 31 - 1   # rows that stay out of it
+    q, k, kc, vc = run_rope(t, qkv, H, Hk, Dh, gq, gk, 0.0, rot, False, freq, pos, page, pages, slots)
+    q2, _, kc2, _ = run_rope(t, qkv, H, Hk, Dh, gq, gk, 0.0, rot, False, freq, pos, page, pages, slots, keys=False)
+    assert np.array_equal(q, q2) and np.array_equal(kc, kc2)
+    want_k, want_v = D.to_type(t, np.full(kc.shape, 3.0)), D.to_type(t, np.full(kc.shape, -3.0))
+    v = qkv[:, (H + Hk) * Dh:].reshape(T, Hk, Dh)
+    for i in range(T):
+        if 0 <= slots[i] < pages * page:
+            want_k[slots[i] // page, :, slots[i] % page] = k[i].reshape(Hk, Dh)
+            want_v[slots[i] // page, :, slots[i] % page] = v[i]
+    assert np.array_equal(kc, want_k) and np.array_equal(vc, want_v)
+    plain = run_rope(t, qkv, H, Hk, Dh, gq, gk, 0.0, rot, False, freq, pos)
+    assert np.array_equal(plain[0], q) and np.array_equal(plain[1], k)
+
+
+@pytest.mark.parametrize("pos", (0, 1, 131071, 2 ** 31 - 1, -5))
+def test_rope_far_positions(pos):
+    """The angle is the product in 64 bits: 2^31 radians and more are reduced without loss."""
+    T, H, Hk, Dh, rot = 2, 1, 1, 64, 64
+    _, qkv, gq, gk, freq, _ = rope_inputs("f32", T, H, Hk, Dh, rot, "far")
+    at = np.full(T, pos, np.int32)
+    q, _ = run_rope("f32", qkv, H, Hk, Dh, gq, gk, 1e-5, rot, True, freq, at)
+    want, size_of = D.norm_rope(D.to_f64("f32", qkv).reshape(T, 3, Dh)[:, :1], gq, 1e-5, rot, True, freq, at)
+    # 2^31 radians in 64 bits: a product's rounding there is 2^-22, numpy's and the kernel's alike
+    extra = abs(pos) * 2.0 ** -51 * size_of
+    D.check(q.astype(np.float64).reshape(T, 1, Dh), want, D.rope_bound("f32", want, size_of, Dh) + extra, str(pos))
+
+
+def test_rope_zero_row_and_empty_call():
+    T, H, Hk, Dh = 2, 2, 1, 64
+    _, qkv, gq, gk, freq, pos = rope_inputs("bf16", T, H, Hk, Dh, 64, "zero")
+    qkv[:] = 0
+    q, k = run_rope("bf16", qkv, H, Hk, Dh, gq, gk, 1e-6, 64, False, freq, pos)
+    assert not (q & 0x7FFF).any() and not (k & 0x7FFF).any()
+    run_rope("bf16", qkv[:0], H, Hk, Dh, gq, gk, 1e-6, 64, False, freq, pos[:0])
+
+
+# ── windowed attention ──────────────────────────────────────────────────────────────────────────────────────────
+
+WIN = [  # query lengths, keys more than queries, heads, key heads, window, ahead, sinks
+    ((1,), 0, 1, 1, 1, 0, 0), ((5,), 0, 2, 1, EVERY, 0, 0), ((33,), 7, 3, 3, 4, 0, 2), ((64,), 0, 4, 2, 16, 5, 1),
+    ((130,), 0, 2, 2, EVERY, EVERY, 0), ((129,), 300, 4, 1, 100, 0, 33), ((0, 3, 0, 40, 1), 12, 2, 1, 20, 3, 4),
+    ((17,), -9, 2, 1, 6, 0, 3), ((300, 2, 77), 0, 8, 2, 64, 0, 70), ((50,), -50, 1, 1, 8, 2, 2),
+    ((1,) * 70, 5, 1, 1, EVERY, 0, 0)]
+
+
+def window_case(t, lens, past, H, Hk, Dh, key="w", scale=1.0):
+    rng = rng_of(t, lens, past, H, Dh, key)
+    kl = [max(n + past, 0) if n else 0 for n in lens]
+    nq, nk = sum(lens), sum(kl)
+    q, k, v = (D.rows(rng, t, n, h * Dh, scale=scale) for n, h in ((nq, H), (nk, Hk), (nk, Hk)))
+    return q, k, v, np.concatenate(([0], np.cumsum(lens))), np.concatenate(([0], np.cumsum(kl)))
+
+
+def window_want(t, q, k, v, qs, ks, H, Hk, Dh, scale, window, ahead, sinks):
+    want, bound = np.zeros((q.shape[0], H * Dh)), np.zeros((q.shape[0], H * Dh))
+    for s in range(len(qs) - 1):
+        a, b, c, d = qs[s], qs[s + 1], ks[s], ks[s + 1]
+        o, e = D.attention(t, D.to_f64(t, q[a:b]).reshape(b - a, H, Dh), D.to_f64(t, k[c:d]).reshape(d - c, Hk, Dh),
+                           D.to_f64(t, v[c:d]).reshape(d - c, Hk, Dh), D.visible(b - a, d - c, window, ahead, sinks), scale)
+        want[a:b], bound[a:b] = o.reshape(b - a, H * Dh), e.reshape(b - a, H * Dh)
+    return want, bound
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("Dh", (64, 128))
+@pytest.mark.parametrize("lens,past,H,Hk,window,ahead,sinks", WIN)
+def test_window(t, Dh, lens, past, H, Hk, window, ahead, sinks):
+    q, k, v, qs, ks = window_case(t, lens, past, H, Hk, Dh)
+    scale = Dh ** -0.5
+    got = D.run_window(t, q, k, v, H, Hk, Dh, scale, window, ahead, sinks, qs, ks)
+    want, bound = window_want(t, q, k, v, qs, ks, H, Hk, Dh, scale, window, ahead, sinks)
+    D.check(D.to_f64(t, got), want, bound, f"{t} {Dh} {lens}")
+    if len(lens) == 1:
+        alone = D.run_window(t, q, k, v, H, Hk, Dh, scale, window, ahead, sinks)
+        assert np.array_equal(alone, got)
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_window_many_rows(t):
+    """Enough tiles for the form with 128 queries a workgroup, ragged, with pitches wider than the heads."""
+    H, Hk, Dh, lens, window, ahead, sinks = 32, 4, 64, (700, 1, 333), 150, 0, 5
+    q, k, v, qs, ks = window_case(t, lens, 40, H, Hk, Dh)
+    pad = 16
+    wide = [np.concatenate((a, np.full((a.shape[0], pad), np.nan if t != "bf16" else 0x7FC0, a.dtype)), 1) for a in (q, k, v)]
+    got = D.run_window(t, *wide, H, Hk, Dh, 0.2, window, ahead, sinks, qs, ks, pad)
+    want, bound = window_want(t, q, k, v, qs, ks, H, Hk, Dh, 0.2, window, ahead, sinks)
+    D.check(D.to_f64(t, got[:, :H * Dh]), want, bound, t)
+    assert (got[:, H * Dh:].view(np.uint16) == 0xFFFF).all()
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("lens,H", (((90,), 2), ((1200,), 32)))
+def test_window_ignores_what_it_masks(t, lens, H):
+    """Infinities and NaN in keys and values that a query must not see do not reach it; those it sees do."""
+    Hk, Dh, window, sinks = 1, 64, 10, 2
+    q, k, v, qs, ks = window_case(t, lens, 0, H, Hk, Dh, "mask")
+    clean = D.run_window(t, q, k, v, H, Hk, Dh, 0.125, window, 0, sinks, qs, ks)
+    at = 40
+    k2, v2 = k.copy(), v.copy()
+    v2[at, :] = D.to_type(t, np.full(Dh, np.inf))
+    v2[at + 1, ::2] = D.to_type(t, np.full(Dh // 2, np.nan))
+    got = D.run_window(t, q, k2, v2, H, Hk, Dh, 0.125, window, 0, sinks, qs, ks)
+    sees = np.arange(lens[0])[(np.arange(lens[0]) >= at) & (np.arange(lens[0]) < at + 1 + window)]
+    out = np.setdiff1d(np.arange(lens[0]), sees)
+    f = D.to_f64(t, got)
+    want, bound = window_want(t, q, k, v, qs, ks, H, Hk, Dh, 0.125, window, 0, sinks)
+    D.check(f[out], want[out], bound[out], t)
+    assert not np.isfinite(f[sees]).all(1).any()
+    k2[at] = D.to_type(t, np.full(Dh, np.nan))
+    got = D.to_f64(t, D.run_window(t, q, k2, v, H, Hk, Dh, 0.125, window, 0, sinks, qs, ks))
+    seesk = np.arange(at, at + window)
+    assert np.isnan(got[seesk]).all()
+    rest = np.setdiff1d(np.arange(lens[0]), seesk)
+    D.check(got[rest], D.to_f64(t, clean)[rest], 2 * bound[rest], t)
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_window_large_scores(t):
+    """Scores in the hundreds: the running maximum keeps every exponential in range."""
+    H, Hk, Dh = 2, 1, 64
+    q, k, v, qs, ks = window_case(t, (70,), 30, H, Hk, Dh, "large", scale=8.0)
+    got = D.run_window(t, q, k, v, H, Hk, Dh, 1.0, EVERY, 0, 0)
+    want, bound = window_want(t, q, k, v, qs, ks, H, Hk, Dh, 1.0, EVERY, 0, 0)
+    D.check(D.to_f64(t, got), want, bound, t)
+
+
+def test_window_leaves_rows_outside_the_sequences():
+    H, Hk, Dh = 2, 2, 64
+    q, k, v, _, _ = window_case("f32", (40,), 0, H, Hk, Dh, "rest")
+    o0 = np.full((40, H * Dh), 7.5, np.float32)
+    got = D.run_window("f32", q, k, v, H, Hk, Dh, 0.1, EVERY, 0, 0, [3, 10, 10, 21], [0, 7, 9, 30], o0=o0)
+    assert (got[:3] == 7.5).all() and (got[21:] == 7.5).all() and (got[3:21] != 7.5).any(1).all()
+    # starts outside the rows or descending are held to the rows: nothing outside is touched
+    D.run_window("f32", q, k, v, H, Hk, Dh, 0.1, EVERY, 0, 0, [-5, 90, 12, 2 ** 31 - 1], [8, -3, 2 ** 31 - 1, 4], o0=o0)
+
+
+# ── paged attention ─────────────────────────────────────────────────────────────────────────────────────────────
+
+PAGED = [  # lengths, heads, key heads, page, window, sinks
+    ((1,), 1, 1, 16, EVERY, 0), ((0, 5, 16, 17), 4, 2, 16, EVERY, 0), ((33, 100), 8, 8, 64, 20, 3),
+    ((1000, 3, 257), 6, 1, 32, 64, 40), ((2500,), 8, 2, 256, EVERY, 0), ((700, 650), 40, 2, 16, 500, 16),
+    ((3000, 1, 0, 1024), 2, 1, 1024, 1, 1), ((90,), 3, 3, 16, 32, 200)]
+
+
+def paged_case(t, lens, H, Hk, page, Dh, key="p", spare=3):
+    rng = rng_of(t, lens, H, page, Dh, key)
+    per = [-(-n // page) for n in lens]
+    pages = sum(per) + spare
+    order = rng.permutation(pages)
+    ld = max(max(per), 1) + 1
+    table = np.full((len(lens), ld), -7, np.int32)   # entries past a sequence's pages are not pages
+    at = 0
+    for s, n in enumerate(per):
+        table[s, :n] = order[at:at + n]
+        at += n
+    q = D.rows(rng, t, len(lens), H * Dh)
+    kc, vc = (D.rows(rng, t, pages, Hk, page, Dh) for _ in range(2))
+    nan = np.uint16(0x7FC0) if t == "bf16" else np.nan
+    for s, n in enumerate(lens):   # what no token was written to holds anything
+        for p in range(n, per[s] * page):
+            kc[table[s, p // page], :, p % page] = nan
+            vc[table[s, p // page], :, p % page] = nan
+    return q, kc, vc, table
+
+
+def paged_want(t, q, kc, vc, table, lens, H, scale, window, sinks):
+    pages, Hk, page, Dh = kc.shape
+    want, bound = np.zeros((len(lens), H * Dh)), np.zeros((len(lens), H * Dh))
+    for s, n in enumerate(lens):
+        k, held = D.gather(t, kc, table[s], n, page, pages)
+        v, _ = D.gather(t, vc, table[s], n, page, pages)
+        seen = D.visible(1, n, window, 0, sinks) & held[None, :]
+        o, e = D.attention(t, D.to_f64(t, q[s]).reshape(1, H, Dh), k, v, seen, scale)
+        want[s], bound[s] = o.reshape(-1), e.reshape(-1)
+    return want, bound
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("Dh", (64, 128))
+@pytest.mark.parametrize("lens,H,Hk,page,window,sinks", PAGED)
+def test_paged(t, Dh, lens, H, Hk, page, window, sinks):
+    q, kc, vc, table = paged_case(t, lens, H, Hk, page, Dh)
+    want, bound = paged_want(t, q, kc, vc, table, lens, H, 0.1, window, sinks)
+    for split in (False, True):
+        got = D.run_paged(t, q, kc, vc, table, lens, H, 0.1, window, sinks, split)
+        D.check(D.to_f64(t, got), want, bound, f"{t} {Dh} {lens} split {split}")
+    # planned for other lengths than those that come
+    for most in (1, 40000):
+        got = D.run_paged(t, q, kc, vc, table, lens, H, 0.1, window, sinks, True, most)
+        D.check(D.to_f64(t, got), want, bound, f"{t} {Dh} {lens} planned for {most}")
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_paged_pages_that_are_not_there(t):
+    lens, H, Hk, page, Dh = (200, 64, 130), 4, 1, 16, 64
+    q, kc, vc, table = paged_case(t, lens, H, Hk, page, Dh, "holes")
+    table[0, 2], table[0, 11], table[1, :] = -1, kc.shape[0], 2 ** 31 - 1
+    want, bound = paged_want(t, q, kc, vc, table, lens, H, 0.1, EVERY, 0)
+    got = D.to_f64(t, D.run_paged(t, q, kc, vc, table, lens, H, 0.1, EVERY, 0))
+    D.check(got, want, bound, t)
+    assert (got[1] == 0).all()
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_paged_lengths_outside_the_table(t):
+    lens, H, Hk, page, Dh = (48, 20), 2, 1, 16, 64
+    q, kc, vc, table = paged_case(t, lens, H, Hk, page, Dh, "long")
+    table = np.ascontiguousarray(table[:, :3])
+    table[1] = table[0]
+    got = D.run_paged(t, q, kc, vc, table, (1 << 30, -4), H, 0.1, EVERY, 0, True, 100)
+    want = D.run_paged(t, q, kc, vc, table, (48, 0), H, 0.1, EVERY, 0, True, 100)
+    assert np.array_equal(got, want)
+
+
+def test_paged_equals_window():
+    """One new token over pages and the last query of a sequence in rows are the same attention."""
+    H, Hk, Dh, page, n, t = 4, 2, 128, 16, 333, "f32"
+    q, kc, vc, table = paged_case(t, (n,), H, Hk, page, Dh, "same")
+    k, v = (np.ascontiguousarray(D.gather(t, c, table[0], n, page, kc.shape[0])[0].reshape(n, -1).astype(np.float32))
+            for c in (kc, vc))
+    a = D.run_paged(t, q, kc, vc, table, (n,), H, 0.1, 100, 4)
+    b = D.run_window(t, q, k, v, H, Hk, Dh, 0.1, 100, 0, 4)
+    _, bound = paged_want(t, q, kc, vc, table, (n,), H, 0.1, 100, 4)
+    assert (np.abs(a.astype(np.float64) - b) <= 2 * bound).all()
+
+
+# ── together, streams and graphs ────────────────────────────────────────────────────────────────────────────────
+
+class Layer:
+    """A decoder layer's attention step on the device: qkv by a 4-bit weight, norm and rotation into the cache, attention
+    over it, the output projection onto the residual rows."""
+    H, Hk, DH, C, PAGE, WINDOW, SINKS = 4, 2, 64, 256, 16, 40, 3
+
+    def __init__(self, t, B, per, seed):
+        rng = rng_of(t, B, seed)
+        W = (self.H + 2 * self.Hk) * self.DH
+        self.t, self.B, self.W = t, B, W
+        self.wq, self.wo = D.q4_weight(rng, self.C, W, 64, True), D.q4_weight(rng, self.H * self.DH, self.C, 32, False)
+        self.q4q, self.q4o = P.Q4Weight(*self.wq, self.C, W, 64), P.Q4Weight(*self.wo, self.H * self.DH, self.C, 32)
+        self.gq, self.gk = (rng.uniform(0.5, 1.5, self.DH).astype(np.float32) for _ in range(2))
+        self.freq = (100.0 ** (-np.arange(0, self.DH, 2) / self.DH)).astype(np.float32)
+        self.pages = B * per
+        self.table = rng.permutation(self.pages).reshape(B, per).astype(np.int32)
+        z = D.to_type(t, np.full((self.pages, self.Hk, self.PAGE, self.DH), np.nan))
+        self.dk, self.dv, self.dt = D.device(z), D.device(z), D.device(self.table)
+        self.cache = P.KvCache(t, self.Hk, self.DH, self.PAGE, self.pages, self.dk.ptr, self.dv.ptr)
+        self.dgq, self.dgk, self.df = D.device(self.gq), D.device(self.gk), D.device(self.freq)
+        self.dx, self.dqkv = D.preset(t, (B, self.C)), D.preset(t, (B, W))
+        self.dq, self.do = D.preset(t, (B, self.H * self.DH)), D.preset(t, (B, self.H * self.DH))
+        self.dpos, self.dslot, self.dlen = (D.device(np.zeros(B, np.int32)) for _ in range(3))
+        self.most = per * self.PAGE
+        self.ws = P.Workspace(P.attention_paged_workspace_bytes(self.cache, B, self.H, self.most, self.WINDOW, self.SINKS))
+
+    def place(self, x, at):
+        """The step's inputs: rows x and every sequence's new token at place at[s]."""
+        at = np.asarray(at, np.int32)
+        self.dx.upload(x)
+        self.dpos.upload(at)
+        self.dslot.upload((self.table[np.arange(self.B), at // self.PAGE] * self.PAGE + at % self.PAGE).astype(np.int32))
+        self.dlen.upload(at + 1)
+
+    def step(self, stream=None):
+        t, B, H, Hk, DH = self.t, self.B, self.H, self.Hk, self.DH
+        P.q4_gemv_dev(t, B, self.W, self.C, 0.05, self.dx.ptr, self.C, self.q4q, 0.0, self.dqkv.ptr, self.W, stream)
+        P.qk_norm_rope_dev(t, B, H, Hk, DH, self.dqkv.ptr, self.W, self.dgq.ptr, self.dgk.ptr, 1e-6, DH, False,
+                           self.df.ptr, self.dpos.ptr, self.dq.ptr, H * DH, None, 0, self.cache, self.dslot.ptr, stream)
+        P.attention_paged_dev(self.cache, B, H, self.dq.ptr, H * DH, self.dt.ptr, self.table.shape[1], self.dlen.ptr,
+                              self.most, DH ** -0.5, self.WINDOW, self.SINKS, self.do.ptr, H * DH, self.ws.ptr,
+                              self.ws.nbytes, stream)
+        P.q4_gemv_dev(t, B, self.C, H * DH, 0.05, self.do.ptr, H * DH, self.q4o, 1.0, self.dx.ptr, self.C, stream)
+
+    def out(self, stream=None):
+        return self.dx.download((self.B, self.C), D.np_type(self.t), stream)
+
+    def plain(self, xs):
+        """xs [steps][B][C] in 64 bits, tokens 0, 1, …: the layer's outputs, nothing rounded in between."""
+        wq = D.q4_values(*self.wq, self.C, self.W, 64) * 0.05
+        wo = D.q4_values(*self.wo, self.H * self.DH, self.C, 32) * 0.05
+        S, H, Hk, DH = xs.shape[0], self.H, self.Hk, self.DH
+        out = np.zeros(xs.shape)
+        for s in range(self.B):
+            qkv = (xs[:, s] @ wq).reshape(S, H + 2 * Hk, DH)
+            pos = np.arange(S)
+            q, _ = D.norm_rope(qkv[:, :H], self.gq, 1e-6, DH, False, self.freq, pos)
+            k, _ = D.norm_rope(qkv[:, H:H + Hk], self.gk, 1e-6, DH, False, self.freq, pos)
+            o, _ = D.attention("f32", q, k, qkv[:, H + Hk:], D.visible(S, S, self.WINDOW, 0, self.SINKS), DH ** -0.5)
+            out[:, s] = xs[:, s] + o.reshape(S, -1) @ wo
+        return out
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_layer_token_by_token(t):
+    """Sixty tokens of three sequences, one step each. Four roundings to the type lie between the rows and the result (qkv,
+    the heads, the attention, the sum): relative to the size of what they round, against a layer that changes its rows by
+    its own size, 8 half steps of the root mean square cover them with the 32-bit sums' own errors (2^-16)."""
+    B, S = 3, 60
+    L = Layer(t, B, 4, "tokens")
+    xs = D.rows(rng_of(t, "xs"), t, S, B, L.C)
+    want = L.plain(D.to_f64(t, xs))
+    for n in range(S):
+        L.place(xs[n], np.full(B, n))
+        L.step()
+        got = D.to_f64(t, L.out())
+        rms = np.sqrt((want[n] ** 2).mean())
+        assert np.abs(got - want[n]).max() <= 6 * (8 * D.HALF[t] + 2.0 ** -16) * rms, (n, np.abs(got - want[n]).max() / rms)
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_layer_prompt_then_tokens(t):
+    """A prompt through p2h_attention_window and its keys put into the cache give the token-by-token bits of the cache."""
+    B, S = 2, 25
+    L, M = Layer(t, B, 4, "prompt"), Layer(t, B, 4, "prompt")
+    xs = D.rows(rng_of(t, "prompt"), t, S, B, L.C)
+    for n in range(S):
+        L.place(xs[n], np.full(B, n))
+        L.step()
+    flat = np.ascontiguousarray(xs.transpose(1, 0, 2).reshape(B * S, -1))   # sequence after sequence
+    H, Hk, DH, W = L.H, L.Hk, L.DH, L.W
+    dx, dqkv = D.device(flat), D.preset(t, (B * S, W))
+    P.q4_gemv_dev(t, B * S, W, L.C, 0.05, dx.ptr, L.C, M.q4q, 0.0, dqkv.ptr, W)
+    at = np.tile(np.arange(S, dtype=np.int32), B)
+    seq = np.repeat(np.arange(B), S)
+    slots = (M.table[seq, at // L.PAGE] * L.PAGE + at % L.PAGE).astype(np.int32)
+    dpos, dslot = D.device(at), D.device(slots)
+    es = D.size(t)
+    P.qk_norm_rope_dev(t, B * S, H, Hk, DH, dqkv.ptr, W, M.dgq.ptr, M.dgk.ptr, 1e-6, DH, False, M.df.ptr, dpos.ptr,
+                       dqkv.ptr, W, dqkv.ptr + H * DH * es, W, M.cache, dslot.ptr)
+    shape = (L.pages, Hk, L.PAGE, DH)
+    for a, b in ((L.dk, M.dk), (L.dv, M.dv)):
+        assert np.array_equal(a.download(shape, D.np_type(t)).view(np.uint16), b.download(shape, D.np_type(t)).view(np.uint16))
+    do, starts = D.preset(t, (B * S, H * DH)), D.device(np.array([0, S, 2 * S], np.int32))
+    P.attention_window_dev(t, B * S, B * S, B, starts.ptr, starts.ptr, H, Hk, DH, dqkv.ptr, W, dqkv.ptr + H * DH * es, W,
+                           dqkv.ptr + (H + Hk) * DH * es, W, DH ** -0.5, L.WINDOW, 0, L.SINKS, do.ptr, H * DH)
+    P.q4_gemv_dev(t, B * S, L.C, H * DH, 0.05, do.ptr, H * DH, M.q4o, 1.0, dx.ptr, L.C)
+    got = D.to_f64(t, dx.download((B, S, L.C), D.np_type(t)))
+    want = L.plain(D.to_f64(t, xs)).transpose(1, 0, 2)
+    rms = np.sqrt((want ** 2).mean())
+    assert np.abs(got - want).max() <= 6 * (8 * D.HALF[t] + 2.0 ** -16) * rms
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_layer_in_a_graph(t):
+    """A captured step replayed for token after token (the places come from device arrays), with eager work between."""
+    B, S = 3, 12
+    L, E = Layer(t, B, 3, "graph"), Layer(t, B, 3, "graph")
+    s = P.Stream()
+    xs = D.rows(rng_of(t, "graph"), t, S, B, L.C)
+    with P.Graph(s) as g:
+        L.step(s.ptr)
+    for n in range(S):
+        L.place(xs[n], np.full(B, n))
+        E.place(xs[n], np.full(B, n))
+        P.sync()
+        g.launch()
+        s.sync()
+        E.step()
+        P.sync()
+        assert np.array_equal(L.out(s.ptr).view(np.uint16), E.out().view(np.uint16)), n
+
+
+def test_two_streams_at_once():
+    """The same step on two streams with buffers of their own gives each its own result."""
+    t, B, S = "f16", 2, 8
+    layers = [Layer(t, B, 2, k) for k in ("one", "two")]
+    streams = [P.Stream(), P.Stream()]
+    alone = [Layer(t, B, 2, k) for k in ("one", "two")]
+    xs = D.rows(rng_of("two"), t, S, B, Layer.C)
+    for n in range(S):
+        for L in (*layers, *alone):
+            L.place(xs[n], np.full(B, n))
+        P.sync()
+        for L, s in zip(layers, streams):
+            L.step(s.ptr)
+        for s in streams:
+            s.sync()
+        for L, A, s in zip(layers, alone, streams):
+            A.step()
+            P.sync()
+            assert np.array_equal(L.out(s.ptr), A.out())
