@@ -472,53 +472,117 @@ template <int DT> __device__ __forceinline__ bool odd_values(u4 v)
     return odd;
 }
 
-/* O for one tile of 32·WQ queries of one head. Each wave owns 32 queries (WK = 1), or the WK waves share 32 queries and
- * take every WK-th block of KB = 32·NK keys, their sums joined at the end. Blocks without a visible key are not touched.
+/* the infinities and NaN among 16 bytes of elements replaced by zeros */
+template <int DT> __device__ __forceinline__ u4 only_finite(u4 v)
+{
+    constexpr uint32_t E = DT == T_F32 ? 0x7f800000u : DT == T_F16 ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t H = E & 0xffff0000u, L = E & 0xffffu;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t keep = 0xffffffffu;
+        if ((v[i] & H) == H) keep = DT == T_F32 ? 0u : keep & 0xffffu;
+        if (DT != T_F32 && (v[i] & L) == L) keep &= 0xffff0000u;
+        v[i] &= keep;
+    }
+    return v;
+}
+
+/* One sequence's tile of queries: its rows, places and the key blocks that any of its queries sees. */
+struct WinTile {
+    int i0, Lq, Lk, off, p0, p1, qa, ka;
+    KeyBlocks blocks;
+    __device__ __forceinline__ WinTile(const WinArgs &a, int seq, int tile, int qb, int kb)
+    {
+        int q1, k1;
+        seq_rows(a.qs, seq, a.q_rows, &qa, &q1);
+        seq_rows(a.ks, seq, a.k_rows, &ka, &k1);
+        Lq = q1 - qa;
+        Lk = k1 - ka;
+        i0 = tile * qb;
+        off = Lk - Lq;
+        p0 = i0 + off;
+        p1 = imin(i0 + qb, Lq) - 1 + off;
+        blocks = key_blocks(p0 - a.window + 1, imin(Lk, p1 + a.ahead + 1), a.sinks, kb);
+    }
+    /* whether every query of places pa .. pb sees all n keys from k0 on */
+    __device__ __forceinline__ bool all_seen(const WinArgs &a, int k0, int n, int pa, int pb) const
+    {
+        const int k1 = k0 + n - 1;
+        return k1 < Lk && k1 - pa <= a.ahead && (pb - k0 < a.window || k1 < a.sinks);
+    }
+};
+
+/* A value that is not finite, in a block where some query must not see it, would reach that query as 0 · inf, so such
+ * values enter the products as zeros (`odd` notes that there were some), and what they do to the queries that see them
+ * is added to the stored outputs here: any positive weight of an infinity or a NaN is that. Rare, so simple: one thread
+ * per output, over every key of the blocks concerned. */
+template <int DT, int DH>
+__device__ __forceinline__ void add_odd_values(const WinArgs &a, const WinTile &w, int kvh, int head, int qb, int kb)
+{
+    typedef typename Elem<DT>::type E;
+    const E *vh = static_cast<const E *>(a.v) + (size_t)w.ka * a.ldv + (size_t)kvh * DH;
+    const int n = imin(qb, w.Lq - w.i0);
+    for (int e = threadIdx.x; e < n * DH; e += blockDim.x) {
+        const int i = w.i0 + e / DH, d = e % DH, p = i + w.off;
+        float more = 0.0f;
+        for (int b = 0; b < w.blocks.total; b++) {
+            const int k0 = w.blocks.at(b) * kb;
+            if (w.all_seen(a, k0, kb, w.p0, w.p1)) continue;
+            for (int key = k0; key < imin(k0 + kb, w.Lk); key++) {
+                const float x = Elem<DT>::get(vh[(size_t)key * a.ldv + d]);
+                if (!(__builtin_fabsf(x) < INFINITY) && key_visible(key, p, a.window, a.ahead, a.sinks)) more += x;
+            }
+        }
+        if (!(__builtin_fabsf(more) < INFINITY)) {
+            E *o = static_cast<E *>(a.o) + (size_t)(w.qa + i) * a.ldo + (size_t)head * DH + d;
+            *o = Elem<DT>::put(Elem<DT>::get(*o) + more);
+        }
+    }
+}
+
+/* The window kernels' workgroups: a head and a tile. Query heads of one key head are apart by kv_heads, so that with 8 key
+ * heads (or a multiple) each XCD, which takes every eighth workgroup, reads the keys of its own. Later tiles, which see
+ * more keys where the window is long, come first. */
+__device__ __forceinline__ bool win_tile_of(const WinArgs &a, int qb, int *head, int *kvh, int *seq, int *tile)
+{
+    const int id = blockIdx.x % a.heads;
+    *kvh = id % a.kv;
+    *head = *kvh * (a.heads / a.kv) + id / a.kv;
+    return find_tile(a.qs, a.n_seqs, a.q_rows, qb, a.tiles - 1 - (int)(blockIdx.x / a.heads), seq, tile);
+}
+
+/* O for 128 queries of one head, 32 for each of the four waves, in blocks of KB = 32·NK keys that pass through LDS, two
+ * buffers in turn: while one is multiplied the next block is on its way into registers. Blocks without a visible key are
+ * not touched.
  *
  * Per block and wave S^T = K·Q^T by 32 × 32 products (keys in rows, queries in columns), so that a lane holds 16 keys of
  * one query: the running maximum and sum of its softmax need one exchange with the lane 32 away, and the weights are
  * already laid out as the operand of O^T += V^T·P^T, whatever order that product takes the keys in, as V's operand reads
  * the same order out of LDS. 16-bit weights: the exponentials, at most 1, are rounded to the rows' type for that product
- * and summed unrounded in 32 bits; fp32 rows multiply in fp32 throughout.
- *
- * V rows past the sequence are zeros in LDS. A value that is not finite, in a block where some query must not see it,
- * would reach that query as 0 · inf: such a block is added key by key with the unseen ones left out. */
-template <int DT, int DH, int WQ, int WK, int NK>
-__global__ __launch_bounds__(256) void attention_win(WinArgs a)
+ * and summed unrounded in 32 bits; fp32 rows multiply in fp32 throughout. */
+template <int DT, int DH, int NK>
+__global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
 {
     typedef typename Elem<DT>::type E;
-    static_assert(WQ * WK == 4, "four waves");
     constexpr bool F32 = DT == T_F32;
-    constexpr int KB = 32 * NK, RB = WK * KB, QB = 32 * WQ;       /* keys per block and per round, queries */
+    constexpr int KB = 32 * NK;
     constexpr int EPC = kPer16<DT>, CH = DH / EPC;                /* elements per 16 bytes, those per row */
     constexpr int VP = F32 ? DH : DH + 32;                        /* V row pitch: 64 bytes on, transposing reads of 8 rows
                                                                      fall into different banks */
-    constexpr int LD = RB * CH / 256;                             /* 16-byte loads per thread and round, of K and of V */
-    constexpr int TILE_BYTES = RB * (DH + VP) * (int)sizeof(E), JOIN_BYTES = WK > 1 ? WK * 32 * (DH + 2) * 4 : 0;
-    __shared__ __align__(16) unsigned char lds[TILE_BYTES > JOIN_BYTES ? TILE_BYTES : JOIN_BYTES];
-    E *Ks = reinterpret_cast<E *>(lds), *Vs = Ks + RB * DH;
+    constexpr int LD = KB * CH / 256;                             /* 16-byte loads per thread and block, of K and of V */
+    __shared__ __align__(16) E lds[2][KB * (DH + VP)];
 
-    const int G = a.heads / a.kv, id = blockIdx.x % a.heads;
-    const int kvh = id % a.kv, head = kvh * G + id / a.kv;
-    int seq, tile;
-    /* later tiles, which see more keys, first */
-    if (!find_tile(a.qs, a.n_seqs, a.q_rows, QB, a.tiles - 1 - (int)(blockIdx.x / a.heads), &seq, &tile)) return;
-    int qa, qb, ka, kb;
-    seq_rows(a.qs, seq, a.q_rows, &qa, &qb);
-    seq_rows(a.ks, seq, a.k_rows, &ka, &kb);
-    const int Lq = qb - qa, Lk = kb - ka, i0 = tile * QB, off = Lk - Lq;
-    const int p0 = i0 + off, p1 = imin(i0 + QB, Lq) - 1 + off;   /* the tile's places */
-    const KeyBlocks blocks = key_blocks(p0 - a.window + 1, imin(Lk, p1 + a.ahead + 1), a.sinks, KB);
-
+    int head, kvh, seq, tile;
+    if (!win_tile_of(a, 128, &head, &kvh, &seq, &tile)) return;
+    const WinTile w(a, seq, tile, 128, KB);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-    const int wq = WK == 1 ? wave : 0, wk = WK == 1 ? 0 : wave;
-    const int iq = i0 + 32 * wq + col, p = iq + off;
-    const int pw0 = i0 + 32 * wq + off, pw1 = imin(i0 + 32 * wq + 32, Lq) - 1 + off;   /* this wave's places */
+    const int iq = w.i0 + 32 * wave + col, p = iq + w.off;
+    const int pw0 = w.p0 + 32 * wave, pw1 = imin(pw0 + 31, w.Lq - 1 + w.off);   /* this wave's places */
 
     constexpr int QR = DH / (2 * EPC);   /* this lane's query: elements EPC·(2s + h) .. of every 2·EPC */
     u4 q[QR];
     {
-        const E *row = static_cast<const E *>(a.q) + (size_t)(qa + imin(iq, Lq - 1)) * a.ldq + (size_t)head * DH;
+        const E *row = static_cast<const E *>(a.q) + (size_t)(w.qa + imin(iq, w.Lq - 1)) * a.ldq + (size_t)head * DH;
 #pragma unroll
         for (int s = 0; s < QR; s++) q[s] = *reinterpret_cast<const u4 *>(row + EPC * (2 * s + h));
     }
@@ -528,69 +592,58 @@ __global__ __launch_bounds__(256) void attention_win(WinArgs a)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    bool odd = false;
 
-    const E *kh = static_cast<const E *>(a.k) + (size_t)ka * a.ldk + (size_t)kvh * DH;
-    const E *vh = static_cast<const E *>(a.v) + (size_t)ka * a.ldv + (size_t)kvh * DH;
+    const E *kh = static_cast<const E *>(a.k) + (size_t)w.ka * a.ldk + (size_t)kvh * DH;
+    const E *vh = static_cast<const E *>(a.v) + (size_t)w.ka * a.ldv + (size_t)kvh * DH;
     u4 kr[LD], vr[LD];
-    auto fetch = [&](int round) __attribute__((always_inline)) {
+    auto fetch = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
         for (int x = 0; x < LD; x++) {
-            const int e = threadIdx.x + 256 * x, r = e / CH, ch = e % CH;
-            const int b = round * WK + r / KB;
-            const int key = b < blocks.total ? blocks.at(b) * KB + r % KB : Lk;
+            const int e = threadIdx.x + 256 * x, key = k0 + e / CH, ch = e % CH;
             kr[x] = vr[x] = u4{0, 0, 0, 0};
-            if (key < Lk) {
+            if (key < w.Lk) {
                 kr[x] = *reinterpret_cast<const u4 *>(kh + (size_t)key * a.ldk + EPC * ch);
                 vr[x] = *reinterpret_cast<const u4 *>(vh + (size_t)key * a.ldv + EPC * ch);
             }
         }
     };
-    /* whether every query of places pa .. pb sees all KB keys from k0 on */
-    auto all_seen = [&](int k0, int pa, int pb) __attribute__((always_inline)) {
-        const int k1 = k0 + KB - 1;
-        return k1 < Lk && k1 - pa <= a.ahead && (pb - k0 < a.window || k1 < a.sinks);
-    };
 
-    const int rounds = (blocks.total + WK - 1) / WK;
-    if (rounds > 0) fetch(0);
-    for (int round = 0; round < rounds; round++) {
-        bool odd = false, partly = false;
+    if (w.blocks.total > 0) fetch(w.blocks.at(0) * KB);
+    for (int b = 0; b < w.blocks.total; b++) {
+        const int k0 = w.blocks.at(b) * KB;
+        E *K = lds[b & 1], *V = K + KB * DH;
+        if (!w.all_seen(a, k0, KB, w.p0, w.p1)) {
 #pragma unroll
-        for (int w = 0; w < WK; w++) {
-            const int b = round * WK + w;
-            if (b < blocks.total) partly |= !all_seen(blocks.at(b) * KB, p0, p1);
-        }
-        if (partly) {
-            bool mine = false;
-#pragma unroll
-            for (int x = 0; x < LD; x++) mine |= odd_values<DT>(vr[x]);
-            odd = __syncthreads_or(mine);
-        } else {
-            __syncthreads();
+            for (int x = 0; x < LD; x++)
+                if (odd_values<DT>(vr[x])) {
+                    odd = true;
+                    vr[x] = only_finite<DT>(vr[x]);
+                }
         }
 #pragma unroll
         for (int x = 0; x < LD; x++) {
             const int e = threadIdx.x + 256 * x, r = e / CH, ch = e % CH;
-            *reinterpret_cast<u4 *>(Ks + r * DH + EPC * (ch ^ (r & (CH - 1)))) = kr[x];
-            *reinterpret_cast<u4 *>(Vs + r * VP + EPC * ch) = vr[x];
+            *reinterpret_cast<u4 *>(K + r * DH + EPC * (ch ^ (r & (CH - 1)))) = kr[x];
+            *reinterpret_cast<u4 *>(V + r * VP + EPC * ch) = vr[x];
         }
-        if (round + 1 < rounds) fetch(round + 1);
+        /* a buffer is filled again two blocks on, and every wave has passed the barrier between only once it is done
+         * with the buffer */
         __syncthreads();
+        if (b + 1 < w.blocks.total) fetch(w.blocks.at(b + 1) * KB);
 
-        const int b = round * WK + wk;
-        if (b >= blocks.total || pw1 < pw0) continue;
-        const int k0 = blocks.at(b) * KB;
-        /* no query of this wave sees any of the block */
-        if (k0 - pw1 > a.ahead || (pw0 - (k0 + KB - 1) >= a.window && k0 >= a.sinks)) continue;
-        const E *K = Ks + wk * KB * DH, *V = Vs + wk * KB * VP;
+        /* no query of this wave sees any of the block, or it has no query */
+        if (pw1 < pw0 || k0 - pw1 > a.ahead || (pw0 - (k0 + KB - 1) >= a.window && k0 >= a.sinks)) continue;
         f16v s[NK];
 #pragma unroll
-        for (int n = 0; n < NK; n++) {
+        for (int n = 0; n < NK; n++)
 #pragma unroll
             for (int i = 0; i < 16; i++) s[n][i] = 0.0f;
-            const int r = 32 * n + col;
 #pragma unroll
-            for (int x = 0; x < QR; x++) {
+        for (int x = 0; x < QR; x++)
+#pragma unroll
+            for (int n = 0; n < NK; n++) {
+                const int r = 32 * n + col;
                 const u4 kk = *reinterpret_cast<const u4 *>(K + r * DH + EPC * ((2 * x + h) ^ (r & (CH - 1))));
                 if constexpr (F32) {
 #pragma unroll
@@ -601,15 +654,13 @@ __global__ __launch_bounds__(256) void attention_win(WinArgs a)
                     s[n] = mfma32<DT>(kk, q[x], s[n]);
                 }
             }
-        }
-        const bool full = all_seen(k0, pw0, pw1);
-        if (!full) {
+        if (!w.all_seen(a, k0, KB, pw0, pw1)) {
 #pragma unroll
             for (int n = 0; n < NK; n++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int key = k0 + 32 * n + 8 * (i / 4) + 4 * h + i % 4;
-                    if (!(key < Lk && key_visible(key, p, a.window, a.ahead, a.sinks))) s[n][i] = -INFINITY;
+                    if (!(key < w.Lk && key_visible(key, p, a.window, a.ahead, a.sinks))) s[n][i] = -INFINITY;
                 }
         }
         float top = s[0][0];
@@ -633,26 +684,6 @@ __global__ __launch_bounds__(256) void attention_win(WinArgs a)
 #pragma unroll
             for (int d = 0; d < DH / 32; d++) o[d] *= fade;
         }
-        if (odd && !full) {
-            for (int key = 0; key < KB; key++) {
-                float w = 0.0f;   /* this query's weight of the key, from the lane that has it */
-#pragma unroll
-                for (int n = 0; n < NK; n++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (32 * n + 8 * (i / 4) + i % 4 == (key & ~4)) w = s[n][i];
-                w = __shfl(w, col + ((key & 4) ? 32 : 0));
-                const bool seen = k0 + key < Lk && key_visible(k0 + key, p, a.window, a.ahead, a.sinks);
-#pragma unroll
-                for (int d = 0; d < DH / 32; d++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float x = Elem<DT>::get(V[key * VP + 32 * d + 8 * (i / 4) + 4 * h + i % 4]);
-                        if (seen) o[d][i] = __builtin_fmaf(w, x, o[d][i]);
-                    }
-            }
-            continue;
-        }
         if constexpr (F32) {
 #pragma unroll
             for (int n = 0; n < NK; n++)
@@ -668,10 +699,10 @@ __global__ __launch_bounds__(256) void attention_win(WinArgs a)
             for (int n = 0; n < NK; n++)
 #pragma unroll
                 for (int k2 = 0; k2 < 2; k2++) {   /* 16 keys: of each eight, this half of the lanes has four */
-                    float w[8];
+                    float pv[8];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) w[j] = s[n][8 * k2 + j];
-                    const u4 pw = pack<DT>(w);
+                    for (int j = 0; j < 8; j++) pv[j] = s[n][8 * k2 + j];
+                    const u4 pw = pack<DT>(pv);
                     const uint16_t *row = reinterpret_cast<const uint16_t *>(V) +
                                           (32 * n + 16 * k2 + 4 * h + ((lane & 15) >> 2)) * VP + 16 * ((lane >> 4) & 1) +
                                           4 * (lane & 3);
@@ -684,48 +715,19 @@ __global__ __launch_bounds__(256) void attention_win(WinArgs a)
         }
     }
     l = sum_halves(l);
-    if constexpr (WK > 1) {
-        /* join the waves' sums: [wave][32 queries][DH + 2], the last two the maximum and the sum */
-        float *J = reinterpret_cast<float *>(lds);
-        __syncthreads();
-        float *mine = J + (wave * 32 + col) * (DH + 2);
-#pragma unroll
-        for (int d = 0; d < DH / 32; d++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) mine[32 * d + 8 * (i / 4) + 4 * h + i % 4] = o[d][i];
-        if (h == 0) {
-            mine[DH] = m;
-            mine[DH + 1] = l;
-        }
-        __syncthreads();
-        for (int e = threadIdx.x; e < 32 * DH; e += 256) {
-            const int r = e / DH, d = e % DH;
-            if (i0 + r >= Lq) break;
-            float top = -INFINITY, num = 0.0f, den = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WK; w++) top = fmaxf(top, J[(w * 32 + r) * (DH + 2) + DH]);
-            const float mu = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-            for (int w = 0; w < WK; w++) {
-                const float *j = J + (w * 32 + r) * (DH + 2);
-                const float f = exp2_fast(j[DH] - mu);
-                num = __builtin_fmaf(f, j[d], num);
-                den = __builtin_fmaf(f, j[DH + 1], den);
-            }
-            static_cast<E *>(a.o)[(size_t)(qa + i0 + r) * a.ldo + (size_t)head * DH + d] =
-                Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
-        }
-    } else if (iq < Lq) {
+    if (iq < w.Lq) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        E *row = static_cast<E *>(a.o) + (size_t)(qa + iq) * a.ldo + (size_t)head * DH + 4 * h;
+        E *row = static_cast<E *>(a.o) + (size_t)(w.qa + iq) * a.ldo + (size_t)head * DH + 4 * h;
 #pragma unroll
         for (int d = 0; d < DH / 32; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) row[32 * d + 8 * (i / 4) + i % 4] = Elem<DT>::put(o[d][i] * inv);
     }
+    /* the barrier in it also puts the stores above before the reads behind it */
+    if (__syncthreads_or(odd)) add_odd_values<DT, DH>(a, w, kvh, head, 128, KB);
 }
 
-/* ── attention of single tokens over a paged cache ─────────────────────────────────────────────────────────── */
+/* ── attention of few queries ──────────────────────────────────────────────────────────────────────────────── */
 
 struct PageArgs {
     int n_seqs, heads, kv, q_groups, splits, page_shift, pages, table_ld, ldq, ldo, window, sinks;
@@ -736,19 +738,268 @@ struct PageArgs {
     float *part;   /* [sequence][head][split][DH + 2] where splits > 1: sums, maximum, sum of weights */
 };
 
-/* One workgroup: one sequence, one key head, up to 16 of the query heads that read it, one part of its blocks of 32 (fp32:
- * 16) keys, which its four waves take in turn. Per block S^T = K·Q^T by 16 × 16 products, K's operand straight from the
- * pages (a lane reads 16 bytes of one key), then O^T += V^T·P^T as in attention_win: 16-bit V passes through LDS for its
- * transposing read, fp32 V is read as the operand takes it. Keys that are not seen (past the end, outside the window, in
- * a page that is not there) have no weight and their V is zeros, whatever lies in the page. */
-template <int DT, int DH>
-__global__ __launch_bounds__(256) void attention_page(PageArgs a)
+/* The softmax state of up to 16 queries (lane % 16) over the blocks that one wave has taken: O^T tiles, running maximum
+ * and this lane's share of the sum of weights. */
+template <int DH> struct FewState {
+    f4 o[DH / 16];
+    float m, l;
+    __device__ __forceinline__ FewState() : m(-INFINITY), l(0.0f)
+    {
+#pragma unroll
+        for (int d = 0; d < DH / 16; d++) o[d] = f4{0, 0, 0, 0};
+    }
+};
+
+/* One block of 32 (fp32: 16) keys from global memory into the state of 16 queries: S^T = K·Q^T by 16 × 16 products, K's
+ * operand straight from its rows (a lane reads 16 bytes of one key), then O^T += V^T·P^T as in attention_win: 16-bit V
+ * passes through the wave's own LDS for its transposing read, fp32 V is read as the operand takes it.
+ *
+ * Each 16 keys t have their rows at kb[t] and vb[t] with pitches ldk and ldv; rows from have[t] on are read as the last
+ * one that is there (have[t] 0: none is read). seen(k) says whether this lane's query sees key k of the block, and kept(k)
+ * whether V row k enters the product at all; neither is asked where `whole`. */
+template <int DT, int DH, class Seen, class Kept>
+__device__ __forceinline__ void few_block(FewState<DH> &st, const u4 (&q)[DH / (4 * kPer16<DT>)], float c,
+                                          const typename Elem<DT>::type *const (&kb)[DT == T_F32 ? 1 : 2],
+                                          const typename Elem<DT>::type *const (&vb)[DT == T_F32 ? 1 : 2],
+                                          const int (&have)[DT == T_F32 ? 1 : 2], int ldk, int ldv, bool whole, Seen seen,
+                                          Kept kept, bool clean, bool &odd, uint16_t *Vs)
+{
+    constexpr int NT = DH / 16, VP = DH + 16;
+    const int lane = threadIdx.x & 63, g = lane >> 4, x16 = lane & 15;
+    auto soften = [&](float top) __attribute__((always_inline)) {
+        const float mn = fmaxf(st.m, max_quarters(top) * c), mu = mn == -INFINITY ? 0.0f : mn;
+        const float fade = exp2_fast(st.m - mu);
+        st.m = mn;
+        return float2{mu, fade};
+    };
+    if constexpr (DT == T_F32) {
+        float v[4][NT];
+        f4 s = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+        if (have[0] > 0) {
+            u4 k[NT];
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+                k[x] = *reinterpret_cast<const u4 *>(kb[0] + (size_t)imin(x16, have[0] - 1) * ldk + 4 * (4 * x + g));
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int d = 0; d < NT; d++) v[i][d] = vb[0][(size_t)imin(4 * g + i, have[0] - 1) * ldv + 16 * d + x16];
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[x][e]), __uint_as_float(q[x][e]), s, 0, 0, 0);
+                    s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[x][e + 1]), __uint_as_float(q[x][e + 1]), s1,
+                                                              0, 0, 0);
+                }
+            s += s1;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int d = 0; d < NT; d++) v[i][d] = 0.0f;
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (!seen(4 * g + i)) s[i] = -INFINITY;
+                const bool keep = kept(4 * g + i);
+#pragma unroll
+                for (int d = 0; d < NT; d++) {
+                    const bool fin = !clean || __builtin_fabsf(v[i][d]) < INFINITY;
+                    odd |= keep && !fin;
+                    if (!keep || !fin) v[i][d] = 0.0f;
+                }
+            }
+        }
+        const float2 mf = soften(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            s[i] = exp2_fast(__builtin_fmaf(s[i], c, -mf.x));
+            sum += s[i];
+        }
+        st.l = __builtin_fmaf(st.l, mf.y, sum);
+#pragma unroll
+        for (int d = 0; d < NT; d++) {
+            st.o[d] *= mf.y;
+#pragma unroll
+            for (int i = 0; i < 4; i++) st.o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d], s[i], st.o[d], 0, 0, 0);
+        }
+    } else {
+        constexpr int CH = DH / 8, RPL = 64 / CH;   /* 16-byte pieces of a row, rows per load */
+        u4 k[2][DH / 32], v[32 / RPL];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            if (have[t] > 0) {
+#pragma unroll
+                for (int x = 0; x < DH / 32; x++)
+                    k[t][x] = *reinterpret_cast<const u4 *>(kb[t] + (size_t)imin(x16, have[t] - 1) * ldk + 8 * (4 * x + g));
+#pragma unroll
+                for (int r = 0; r < 16 / RPL; r++)
+                    v[t * 16 / RPL + r] = *reinterpret_cast<const u4 *>(
+                        vb[t] + (size_t)imin(RPL * r + lane / CH, have[t] - 1) * ldv + 8 * (lane % CH));
+            } else {
+#pragma unroll
+                for (int x = 0; x < DH / 32; x++) k[t][x] = u4{0, 0, 0, 0};
+#pragma unroll
+                for (int r = 0; r < 16 / RPL; r++) v[t * 16 / RPL + r] = u4{0, 0, 0, 0};
+            }
+        }
+        f4 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            s[t] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int x = 0; x < DH / 32; x++) s[t] = mfma16<DT>(k[t][x], q[x], s[t]);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (!seen(16 * t + 4 * g + i)) s[t][i] = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 32 / RPL; r++) {
+                if (!kept(RPL * r + lane / CH)) v[r] = u4{0, 0, 0, 0};
+                if (clean && odd_values<DT>(v[r])) {
+                    odd = true;
+                    v[r] = only_finite<DT>(v[r]);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 32 / RPL; r++)
+            *reinterpret_cast<u4 *>(Vs + (RPL * r + lane / CH) * VP + 8 * (lane % CH)) = v[r];
+        const float2 mf = soften(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
+        float sum = 0.0f, w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            w[i] = exp2_fast(__builtin_fmaf(s[i / 4][i % 4], c, -mf.x));
+            sum += w[i];
+        }
+        st.l = __builtin_fmaf(st.l, mf.y, sum);
+        const u4 pw = pack<DT>(w);
+        /* a wave's LDS operations complete in order, and no other wave touches its part; the fences keep the compiler
+         * from moving reads and writes across each other */
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const uint16_t *vp = Vs + (4 * g + (x16 >> 2)) * VP + 4 * (x16 & 3);
+#pragma unroll
+        for (int d = 0; d < NT; d++) {
+            const u2 va = lds_tr(vp + 16 * d), vb2 = lds_tr(vp + 16 * VP + 16 * d);
+            st.o[d] = mfma16<DT>(u4{va[0], va[1], vb2[0], vb2[1]}, pw, st.o[d] * mf.y);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+/* the waves' states into LDS as [wave][16 queries][DH + 2], the last two the maximum and the sum, and one output of their
+ * join: sums relative to the returned maximum */
+template <int DH, int NW> __device__ __forceinline__ void few_store(FewState<DH> &st, float *J)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const float l = sum_quarters(st.l);
+    __syncthreads();   /* V's part of the LDS is done with */
+    float *mine = J + (wave * 16 + (lane & 15)) * (DH + 2);
+#pragma unroll
+    for (int d = 0; d < DH / 16; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mine[16 * d + 4 * g + i] = st.o[d][i];
+    if (g == 0) {
+        mine[DH] = st.m;
+        mine[DH + 1] = l;
+    }
+    __syncthreads();
+}
+template <int DH, int NW> __device__ __forceinline__ void few_join(const float *J, int r, int d, float *top, float *num,
+                                                                   float *den)
+{
+    float t = -INFINITY, n = 0.0f, e = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) t = fmaxf(t, J[(w * 16 + r) * (DH + 2) + DH]);
+    const float mu = t == -INFINITY ? 0.0f : t;
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        const float *j = J + (w * 16 + r) * (DH + 2);
+        const float f = exp2_fast(j[DH] - mu);
+        n = __builtin_fmaf(f, j[d], n);
+        e = __builtin_fmaf(f, j[DH + 1], e);
+    }
+    *top = t;
+    *num = n;
+    *den = e;
+}
+
+template <int DT, int DH, int NW> constexpr int few_lds_bytes()
+{
+    constexpr int V = DT == T_F32 ? 0 : NW * 32 * (DH + 16) * 2, J = NW * 16 * (DH + 2) * 4;
+    return V > J ? V : J;
+}
+
+/* attention_win for calls with too few tiles of 128 queries to fill the device: 16 queries of one head a workgroup, whose
+ * NW waves take the key blocks in turn, nothing shared between them until their sums are joined. */
+template <int DT, int DH, int NW>
+__global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_win_few(WinArgs a)
 {
     typedef typename Elem<DT>::type E;
-    constexpr bool F32 = DT == T_F32;
-    constexpr int KB = F32 ? 16 : 32, EPC = kPer16<DT>, VP = DH + 16, NT = DH / 16;
-    constexpr int V_BYTES = F32 ? 0 : 4 * KB * VP * 2, J_BYTES = 4 * 16 * (DH + 2) * 4;
-    __shared__ __align__(16) unsigned char lds[V_BYTES > J_BYTES ? V_BYTES : J_BYTES];
+    constexpr int NB = DT == T_F32 ? 1 : 2, KB = 16 * NB, EPC = kPer16<DT>;
+    __shared__ __align__(16) unsigned char lds[few_lds_bytes<DT, DH, NW>()];
+    int head, kvh, seq, tile;
+    if (!win_tile_of(a, 16, &head, &kvh, &seq, &tile)) return;
+    const WinTile w(a, seq, tile, 16, KB);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int i = imin(w.i0 + (lane & 15), w.Lq - 1), p = i + w.off;
+    u4 q[DH / (4 * EPC)];
+    {
+        const E *row = static_cast<const E *>(a.q) + (size_t)(w.qa + i) * a.ldq + (size_t)head * DH;
+#pragma unroll
+        for (int s = 0; s < DH / (4 * EPC); s++) q[s] = *reinterpret_cast<const u4 *>(row + EPC * (4 * s + g));
+    }
+    const E *kh = static_cast<const E *>(a.k) + (size_t)w.ka * a.ldk + (size_t)kvh * DH;
+    const E *vh = static_cast<const E *>(a.v) + (size_t)w.ka * a.ldv + (size_t)kvh * DH;
+    FewState<DH> st;
+    bool odd = false;
+    for (int b = wave; b < w.blocks.total; b += NW) {
+        const int k0 = __builtin_amdgcn_readfirstlane(w.blocks.at(b) * KB);
+        const E *kb[NB], *vb[NB];
+        int have[NB];
+#pragma unroll
+        for (int t = 0; t < NB; t++) {
+            have[t] = imax(imin(16, w.Lk - k0 - 16 * t), 0);
+            kb[t] = kh + (size_t)(k0 + 16 * t) * a.ldk;
+            vb[t] = vh + (size_t)(k0 + 16 * t) * a.ldv;
+        }
+        few_block<DT, DH>(
+            st, q, a.c, kb, vb, have, a.ldk, a.ldv, w.all_seen(a, k0, KB, w.p0, w.p1),
+            [&](int k) __attribute__((always_inline)) {
+                return k0 + k < w.Lk && key_visible(k0 + k, p, a.window, a.ahead, a.sinks);
+            },
+            [&](int k) __attribute__((always_inline)) { return k0 + k < w.Lk; }, true, odd,
+            reinterpret_cast<uint16_t *>(lds) + wave * 32 * (DH + 16));
+    }
+    float *J = reinterpret_cast<float *>(lds);
+    few_store<DH, NW>(st, J);
+    for (int e = threadIdx.x; e < imin(16, w.Lq - w.i0) * DH; e += 64 * NW) {
+        float top, num, den;
+        few_join<DH, NW>(J, e / DH, e % DH, &top, &num, &den);
+        static_cast<E *>(a.o)[(size_t)(w.qa + w.i0 + e / DH) * a.ldo + (size_t)head * DH + e % DH] =
+            Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
+    }
+    if (__syncthreads_or(odd)) add_odd_values<DT, DH>(a, w, kvh, head, 16, KB);
+}
+
+/* One workgroup: one sequence, one key head, up to 16 of the query heads that read it, one part of its key blocks, which
+ * its NW waves take in turn. Keys that are not seen (past the end, outside the window, in a page that is not there) have
+ * no weight and their V is zeros, whatever lies in the page: all queries here stand at one place. */
+template <int DT, int DH, int NW>
+__global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_page(PageArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int NB = DT == T_F32 ? 1 : 2, KB = 16 * NB, EPC = kPer16<DT>;
+    __shared__ __align__(16) unsigned char lds[few_lds_bytes<DT, DH, NW>()];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
     const int split = blockIdx.x % a.splits, kvh = (blockIdx.x / a.splits) % a.kv;
     const int qg = (blockIdx.x / a.splits / a.kv) % a.q_groups, seq = blockIdx.x / a.splits / a.kv / a.q_groups;
@@ -767,174 +1018,38 @@ __global__ __launch_bounds__(256) void attention_page(PageArgs a)
 #pragma unroll
         for (int s = 0; s < DH / (4 * EPC); s++) q[s] = *reinterpret_cast<const u4 *>(p + EPC * (4 * s + g));
     }
-    f4 o[NT];
-#pragma unroll
-    for (int d = 0; d < NT; d++) o[d] = f4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;
     const size_t page_elems = (size_t)DH << a.page_shift;   /* of one head */
     const E *kc = static_cast<const E *>(a.kc) + kvh * page_elems, *vc = static_cast<const E *>(a.vc) + kvh * page_elems;
     const int in_page = (1 << a.page_shift) - 1;
-    auto seen = [&](int key) __attribute__((always_inline)) { return key < len && (key >= w0 || key < a.sinks); };
-
-    for (int b = b0 + wave; b < b1; b += 4) {
+    FewState<DH> st;
+    bool odd = false;
+    for (int b = b0 + wave; b < b1; b += NW) {
         const int k0 = __builtin_amdgcn_readfirstlane(blocks.at(b) * KB);
-        int page[KB / 16];   /* of each 16 keys; pages hold at least 16 */
+        const E *kb[NB], *vb[NB];
+        int have[NB];
         bool whole = true;
 #pragma unroll
-        for (int t = 0; t < KB / 16; t++) {
+        for (int t = 0; t < NB; t++) {   /* pages hold a multiple of 16 tokens */
             const int key = k0 + 16 * t;
-            page[t] = key < len ? page_of(row, a.table_ld, key, a.page_shift, a.pages) : -1;
-            whole &= page[t] >= 0 && key + 15 < len && (key >= w0 || key + 15 < a.sinks);
+            const int page = key < len ? page_of(row, a.table_ld, key, a.page_shift, a.pages) : -1;
+            const size_t at = (size_t)imax(page, 0) * a.kv * page_elems + (size_t)(key & in_page) * DH;
+            have[t] = page >= 0 ? 16 : 0;
+            kb[t] = kc + at;
+            vb[t] = vc + at;
+            whole &= page >= 0 && key + 15 < len && (key >= w0 || key + 15 < a.sinks);
         }
-        f4 s[KB / 16];
-        if constexpr (F32) {
-            s[0] = f4{0, 0, 0, 0};
-            float v[4][NT];
-            if (page[0] >= 0) {
-                const size_t at = (size_t)page[0] * a.kv * page_elems + (size_t)(k0 & in_page) * DH;
-                f4 s1 = {0, 0, 0, 0};
-                u4 k[NT];
-#pragma unroll
-                for (int x = 0; x < NT; x++) k[x] = *reinterpret_cast<const u4 *>(kc + at + c * DH + 4 * (4 * x + g));
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int d = 0; d < NT; d++) v[i][d] = vc[at + (4 * g + i) * DH + 16 * d + c];
-#pragma unroll
-                for (int x = 0; x < NT; x++)
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[x][e]), __uint_as_float(q[x][e]),
-                                                                    s[0], 0, 0, 0);
-                        s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[x][e + 1]),
-                                                                  __uint_as_float(q[x][e + 1]), s1, 0, 0, 0);
-                    }
-                s[0] += s1;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int d = 0; d < NT; d++) v[i][d] = 0.0f;
-            }
-            if (!whole) {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (page[0] < 0 || !seen(k0 + 4 * g + i)) {
-                        s[0][i] = -INFINITY;
-#pragma unroll
-                        for (int d = 0; d < NT; d++) v[i][d] = 0.0f;
-                    }
-            }
-            const float top = max_quarters(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])));
-            const float mn = fmaxf(m, top * a.c), mu = mn == -INFINITY ? 0.0f : mn, fade = exp2_fast(m - mu);
-            m = mn;
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                s[0][i] = exp2_fast(__builtin_fmaf(s[0][i], a.c, -mu));
-                sum += s[0][i];
-            }
-            l = __builtin_fmaf(l, fade, sum);
-#pragma unroll
-            for (int d = 0; d < NT; d++) {
-                o[d] *= fade;
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d], s[0][i], o[d], 0, 0, 0);
-            }
-        } else {
-            constexpr int CH = DH / 8, RPL = 64 / CH;   /* 16-byte pieces of a row, rows per load */
-            u4 k[2][DH / 32], v[KB / RPL];
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const size_t at = (size_t)imax(page[t], 0) * a.kv * page_elems + (size_t)((k0 + 16 * t) & in_page) * DH;
-                if (page[t] >= 0) {
-#pragma unroll
-                    for (int x = 0; x < DH / 32; x++)
-                        k[t][x] = *reinterpret_cast<const u4 *>(kc + at + c * DH + 8 * (4 * x + g));
-#pragma unroll
-                    for (int r = 0; r < 16 / RPL; r++)
-                        v[t * 16 / RPL + r] = *reinterpret_cast<const u4 *>(vc + at + (RPL * r) * DH + 8 * lane);
-                } else {
-#pragma unroll
-                    for (int x = 0; x < DH / 32; x++) k[t][x] = u4{0, 0, 0, 0};
-#pragma unroll
-                    for (int r = 0; r < 16 / RPL; r++) v[t * 16 / RPL + r] = u4{0, 0, 0, 0};
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                s[t] = f4{0, 0, 0, 0};
-#pragma unroll
-                for (int x = 0; x < DH / 32; x++) s[t] = mfma16<DT>(k[t][x], q[x], s[t]);
-            }
-            if (!whole) {
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (page[t] < 0 || !seen(k0 + 16 * t + 4 * g + i)) s[t][i] = -INFINITY;
-#pragma unroll
-                for (int r = 0; r < KB / RPL; r++)
-                    if (!seen(k0 + RPL * r + lane / CH)) v[r] = u4{0, 0, 0, 0};
-            }
-            uint16_t *Vs = reinterpret_cast<uint16_t *>(lds) + wave * KB * VP;
-#pragma unroll
-            for (int r = 0; r < KB / RPL; r++)
-                *reinterpret_cast<u4 *>(Vs + (RPL * r + lane / CH) * VP + 8 * (lane % CH)) = v[r];
-            float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                              fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-            top = max_quarters(top);
-            const float mn = fmaxf(m, top * a.c), mu = mn == -INFINITY ? 0.0f : mn, fade = exp2_fast(m - mu);
-            m = mn;
-            float sum = 0.0f, w[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                w[i] = exp2_fast(__builtin_fmaf(s[i / 4][i % 4], a.c, -mu));
-                sum += w[i];
-            }
-            l = __builtin_fmaf(l, fade, sum);
-            const u4 pw = pack<DT>(w);
-            /* a wave's LDS operations complete in order, and no other wave touches its part; the fence keeps the
-             * compiler from moving the reads above the writes */
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            const uint16_t *vp = Vs + (4 * g + (c >> 2)) * VP + 4 * (c & 3);
-#pragma unroll
-            for (int d = 0; d < NT; d++) {
-                const u2 va = lds_tr(vp + 16 * d), vb = lds_tr(vp + 16 * VP + 16 * d);
-                o[d] = mfma16<DT>(u4{va[0], va[1], vb[0], vb[1]}, pw, o[d] * fade);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
+        auto seen = [&](int k) __attribute__((always_inline)) {
+            return have[NB == 2 ? k >> 4 : 0] > 0 && k0 + k < len && (k0 + k >= w0 || k0 + k < a.sinks);
+        };
+        few_block<DT, DH>(st, q, a.c, kb, vb, have, DH, DH, whole, seen, seen, false, odd,
+                          reinterpret_cast<uint16_t *>(lds) + wave * 32 * (DH + 16));
     }
-    l = sum_quarters(l);
-    /* join the four waves' sums: [wave][16 heads][DH + 2] */
     float *J = reinterpret_cast<float *>(lds);
-    __syncthreads();
-    float *mine = J + (wave * 16 + c) * (DH + 2);
-#pragma unroll
-    for (int d = 0; d < NT; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) mine[16 * d + 4 * g + i] = o[d][i];
-    if (g == 0) {
-        mine[DH] = m;
-        mine[DH + 1] = l;
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < nq * DH; e += 256) {
+    few_store<DH, NW>(st, J);
+    for (int e = threadIdx.x; e < nq * DH; e += 64 * NW) {
         const int r = e / DH, d = e % DH;
-        float top = -INFINITY, num = 0.0f, den = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; w++) top = fmaxf(top, J[(w * 16 + r) * (DH + 2) + DH]);
-        const float mu = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float *j = J + (w * 16 + r) * (DH + 2);
-            const float f = exp2_fast(j[DH] - mu);
-            num = __builtin_fmaf(f, j[d], num);
-            den = __builtin_fmaf(f, j[DH + 1], den);
-        }
+        float top, num, den;
+        few_join<DH, NW>(J, r, d, &top, &num, &den);
         if (a.splits == 1) {
             static_cast<E *>(a.o)[(size_t)seq * a.ldo + (size_t)(head0 + r) * DH + d] =
                 Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
@@ -949,22 +1064,47 @@ __global__ __launch_bounds__(256) void attention_page(PageArgs a)
     }
 }
 
-/* The parts of one sequence's head added up: one workgroup of DH threads. */
+/* The parts of one sequence's head added up by one workgroup: each wave takes every NW-th part, DH / 64 outputs a lane,
+ * all its loads independent of each other; the waves' sums are added in LDS. */
+constexpr int kJoinWaves = 8;
 template <int DT, int DH>
-__global__ __launch_bounds__(DH) void attention_join(PageArgs a)
+__global__ __launch_bounds__(64 * kJoinWaves) void attention_join(PageArgs a)
 {
     typedef typename Elem<DT>::type E;
-    const int seq = blockIdx.x / a.heads, head = blockIdx.x % a.heads, d = threadIdx.x;
+    constexpr int PER = DH / 64;
+    __shared__ float J[kJoinWaves][DH + 2];
+    const int seq = blockIdx.x / a.heads, head = blockIdx.x % a.heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float *p = a.part + ((size_t)seq * a.heads + head) * a.splits * (DH + 2);
-    float top = -INFINITY, num = 0.0f, den = 0.0f;
-    for (int s = 0; s < a.splits; s++) top = fmaxf(top, p[s * (DH + 2) + DH]);
+    float top = -INFINITY;   /* of all parts: 64 at a time */
+    for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, p[(size_t)s * (DH + 2) + DH]);
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
     const float mu = top == -INFINITY ? 0.0f : top;
-    for (int s = 0; s < a.splits; s++) {
-        const float f = exp2_fast(p[s * (DH + 2) + DH] - mu);
-        num = __builtin_fmaf(f, p[s * (DH + 2) + d], num);
-        den = __builtin_fmaf(f, p[s * (DH + 2) + DH + 1], den);
+    float num[PER], den = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; i++) num[i] = 0.0f;
+#pragma unroll 8
+    for (int s = wave; s < a.splits; s += kJoinWaves) {
+        const float *j = p + (size_t)s * (DH + 2);
+        const float f = exp2_fast(j[DH] - mu);
+#pragma unroll
+        for (int i = 0; i < PER; i++) num[i] = __builtin_fmaf(f, j[PER * lane + i], num[i]);
+        den = __builtin_fmaf(f, j[DH + 1], den);
     }
-    static_cast<E *>(a.o)[(size_t)seq * a.ldo + (size_t)head * DH + d] = Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
+#pragma unroll
+    for (int i = 0; i < PER; i++) J[wave][PER * lane + i] = num[i];
+    if (lane == 0) J[wave][DH] = den;
+    __syncthreads();
+    if (threadIdx.x < DH) {
+        float n = 0.0f, e = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWaves; w++) {
+            n += J[w][threadIdx.x];
+            e += J[w][DH];
+        }
+        static_cast<E *>(a.o)[(size_t)seq * a.ldo + (size_t)head * DH + threadIdx.x] =
+            Elem<DT>::put(e == 0.0f ? 0.0f : n / e);
+    }
 }
 
 }  // namespace p2k

@@ -347,9 +347,9 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
             return fail(P2H_E_ARG, "%s: dO overlaps dK or dV", name);
     }
     if (overlap(o, Rows{(const char *)dQ, ldq * es, q_w, q_rows})) return fail(P2H_E_ARG, "%s: dO overlaps dQ", name);
-    /* tiles of 32·WQ queries: at most one more per sequence than the rows fill */
+    /* tiles of 16 or 128 queries: at most one more per sequence than the rows fill */
     const bool few = (long long)((q_rows + 127) / 128) * heads < 256;
-    const int qb = few ? 32 : 128;
+    const int qb = few ? 16 : 128;
     const long long tiles = (long long)(dQStart ? q_rows / qb + p2k::imin(n_seqs, q_rows) : (q_rows + qb - 1) / qb);
     if (tiles * heads > INT_MAX) return fail(P2H_E_ARG, "%s: %lld tiles of %d heads", name, tiles, heads);
     if (int rc = ensure_init()) return rc;
@@ -362,8 +362,8 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
     const dim3 grid((unsigned)(tiles * heads));
     by_type_dim(dtype, head_dim, [&](auto t, auto d) {
         constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
-        if (few) hipLaunchKernelGGL((p2k::attention_win<DT, DH, 1, 4, 1>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((p2k::attention_win<DT, DH, 4, 1, DT == p2k::T_F32 ? 1 : 2>), grid, dim3(256), 0, s, a);
+        if (few) hipLaunchKernelGGL((p2k::attention_win_few<DT, DH, 8>), grid, dim3(512), 0, s, a);
+        else hipLaunchKernelGGL((p2k::attention_win<DT, DH, DT == p2k::T_F32 ? 1 : 2>), grid, dim3(256), 0, s, a);
     });
     HIPCHK(hipGetLastError());
     return P2H_OK;
@@ -436,9 +436,11 @@ int p2h_attention_paged(const P2hKvCache *cache, int n_seqs, int heads, const vo
     hipStream_t s = stream_of(stream);
     by_type_dim(dtype, cache->head_dim, [&](auto t, auto d) {
         constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
-        hipLaunchKernelGGL((p2k::attention_page<DT, DH>), dim3((unsigned)grid), dim3(256), 0, s, a);
+        if (grid >= cu_count()) hipLaunchKernelGGL((p2k::attention_page<DT, DH, 4>), dim3((unsigned)grid), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((p2k::attention_page<DT, DH, 8>), dim3((unsigned)grid), dim3(512), 0, s, a);
         if (splits > 1)
-            hipLaunchKernelGGL((p2k::attention_join<DT, DH>), dim3((unsigned)(n_seqs * heads)), dim3(DH), 0, s, a);
+            hipLaunchKernelGGL((p2k::attention_join<DT, DH>), dim3((unsigned)(n_seqs * heads)),
+                               dim3(64 * p2k::kJoinWaves), 0, s, a);
     });
     HIPCHK(hipGetLastError());
     return P2H_OK;
