@@ -363,7 +363,8 @@ int    p2h_conformer_stack(int mode, const P2hBlock *blocks, int n_blocks, int T
  *  states are held in 32 bits and outputs rounded once.
  *
  *  Query heads are shared evenly: query head h reads key head h / (heads / kv_heads). head_dim is 64 or 128. Pointers
- *  to rows and caches are 16-byte aligned and row pitches whole multiples of 16 bytes unless an entry says otherwise.
+ *  to rows and caches are 16-byte aligned and row pitches whole multiples of 16 bytes, below 2^23 elements, unless an
+ *  entry says otherwise.
  *  Entries are asynchronous on their stream, allocate nothing and can be captured. Arrays of positions, slots, lengths
  *  and page numbers are read on the device when the call runs, so a captured graph sees their new values; no value in
  *  them makes a kernel read or write outside the buffers it was given. */

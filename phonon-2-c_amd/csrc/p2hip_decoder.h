@@ -14,6 +14,7 @@
 
 #include <type_traits>
 
+#include "p2hip_async.h"
 #include "p2hip_index.h"
 
 namespace p2k {
@@ -449,11 +450,11 @@ __device__ __forceinline__ bool find_tile(const int *qs, int n_seqs, int q_rows,
         const unsigned long long in = __ballot(id < before + sum);
         if (in) {
             const int at = __ffsll(in) - 1;
-            *seq = s0 + at;
-            *tile = id - before - (__shfl(sum, at) - __shfl(n, at));
+            *seq = s0 + at;   /* the same in every lane: kept in scalar registers */
+            *tile = id - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(n, at));
             return true;
         }
-        before += __shfl(sum, 63);
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
 }
@@ -551,31 +552,35 @@ __device__ __forceinline__ bool win_tile_of(const WinArgs &a, int qb, int *head,
     return find_tile(a.qs, a.n_seqs, a.q_rows, qb, a.tiles - 1 - (int)(blockIdx.x / a.heads), seq, tile);
 }
 
-/* O for 128 queries of one head, 32 for each of the four waves, in blocks of KB = 32·NK keys that pass through LDS, two
- * buffers in turn: while one is multiplied the next block is on its way into registers. Blocks without a visible key are
- * not touched.
+/* O for 128 queries of one head, 32 for each of the four waves, in blocks of KB = 32·NK keys that pass through LDS by
+ * direct loads, two buffers in turn: while one is multiplied the next block is on its way. Blocks without a visible key
+ * are not touched.
  *
  * Per block and wave S^T = K·Q^T by 32 × 32 products (keys in rows, queries in columns), so that a lane holds 16 keys of
  * one query: the running maximum and sum of its softmax need one exchange with the lane 32 away, and the weights are
  * already laid out as the operand of O^T += V^T·P^T, whatever order that product takes the keys in, as V's operand reads
- * the same order out of LDS. 16-bit weights: the exponentials, at most 1, are rounded to the rows' type for that product
- * and summed unrounded in 32 bits; fp32 rows multiply in fp32 throughout. */
+ * the same order out of LDS. 16-bit weights: the exponentials are rounded to the rows' type for that product and summed
+ * unrounded in 32 bits; fp32 rows multiply in fp32 throughout.
+ *
+ * The exponentials are taken relative to a reference that is raised only when some query's maximum has come 2^kSlack
+ * above it, since most blocks raise some maximum a little and each time all of O would be scaled: weights stay below
+ * 2^kSlack, which every type holds, and relative to their sum nothing changes. */
+constexpr float kSlack = 8.0f;
 template <int DT, int DH, int NK>
 __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
 {
     typedef typename Elem<DT>::type E;
     constexpr bool F32 = DT == T_F32;
     constexpr int KB = 32 * NK;
-    constexpr int EPC = kPer16<DT>, CH = DH / EPC;                /* elements per 16 bytes, those per row */
-    constexpr int VP = F32 ? DH : DH + 32;                        /* V row pitch: 64 bytes on, transposing reads of 8 rows
-                                                                     fall into different banks */
-    constexpr int LD = KB * CH / 256;                             /* 16-byte loads per thread and block, of K and of V */
-    __shared__ __align__(16) E lds[2][KB * (DH + VP)];
+    constexpr int EPC = kPer16<DT>, CH = DH / EPC;   /* elements per 16 bytes, those per row */
+    constexpr int LD = KB * CH / 256, RPL = 64 / CH; /* direct loads per wave and block, of K and of V; rows of each */
+    __shared__ __align__(16) E lds[2][2 * KB * DH];
 
     int head, kvh, seq, tile;
     if (!win_tile_of(a, 128, &head, &kvh, &seq, &tile)) return;
     const WinTile w(a, seq, tile, 128, KB);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5,
+              col = lane & 31;
     const int iq = w.i0 + 32 * wave + col, p = iq + w.off;
     const int pw0 = w.p0 + 32 * wave, pw1 = imin(pw0 + 31, w.Lq - 1 + w.off);   /* this wave's places */
 
@@ -591,47 +596,58 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
     for (int d = 0; d < DH / 32; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, l = 0.0f;   /* the reference, in powers of two, and this lane's sum of weights */
     bool odd = false;
 
+    /* Row r's 16-byte piece cc lies at place cc ^ (r mod CH) of K's row, so that the operand reads (32 rows, one piece)
+     * fall into different banks. 16-bit V: its 64-byte piece s lies at place s ^ (r mod pieces), and a transposing read
+     * (8 rows, one 64-byte piece) falls into different banks; fp32 V is read along its rows. */
+    auto place = [](int r, int cc) { return F32 ? cc : cc ^ (CH == 16 ? 4 * (r & 3) : 4 * ((r >> 1) & 1)); };
     const E *kh = static_cast<const E *>(a.k) + (size_t)w.ka * a.ldk + (size_t)kvh * DH;
     const E *vh = static_cast<const E *>(a.v) + (size_t)w.ka * a.ldv + (size_t)kvh * DH;
-    u4 kr[LD], vr[LD];
-    auto fetch = [&](int k0) __attribute__((always_inline)) {
+    uint32_t koff[LD], voff[LD];
+#pragma unroll
+    for (int x = 0; x < LD; x++) {
+        const int r = RPL * (wave * LD + x) + lane / CH, cc = lane % CH;
+        koff[x] = (uint32_t)(r * a.ldk + EPC * (cc ^ (r & (CH - 1)))) * sizeof(E);
+        voff[x] = (uint32_t)(r * a.ldv + EPC * place(r, cc)) * sizeof(E);
+    }
+    auto fetch = [&](int k0, E *to) __attribute__((always_inline)) {
+        const E *kb = kh + (size_t)k0 * a.ldk, *vb = vh + (size_t)k0 * a.ldv;
+        const int left = w.Lk - k0;
 #pragma unroll
         for (int x = 0; x < LD; x++) {
-            const int e = threadIdx.x + 256 * x, key = k0 + e / CH, ch = e % CH;
-            kr[x] = vr[x] = u4{0, 0, 0, 0};
-            if (key < w.Lk) {
-                kr[x] = *reinterpret_cast<const u4 *>(kh + (size_t)key * a.ldk + EPC * ch);
-                vr[x] = *reinterpret_cast<const u4 *>(vh + (size_t)key * a.ldv + EPC * ch);
+            const int u = wave * LD + x;
+            uint32_t ko = koff[x], vo = voff[x];
+            if (left < KB) {   /* past the sequence its last row, which the masks leave out */
+                const int r = RPL * u + lane / CH, back = r < left ? 0 : r - (left - 1);
+                ko -= (uint32_t)(back * a.ldk) * sizeof(E);
+                vo -= (uint32_t)(back * a.ldv) * sizeof(E);
             }
+            dma_16(kb, ko, to + 64 * EPC * u);
+            dma_16(vb, vo, to + KB * DH + 64 * EPC * u);
         }
     };
 
-    if (w.blocks.total > 0) fetch(w.blocks.at(0) * KB);
+    if (w.blocks.total > 0) fetch(w.blocks.at(0) * KB, lds[0]);
     for (int b = 0; b < w.blocks.total; b++) {
         const int k0 = w.blocks.at(b) * KB;
         E *K = lds[b & 1], *V = K + KB * DH;
+        /* this wave's loads have come, then everyone's; and every wave is done with the other buffer */
+        wait_vm<0>();
+        __syncthreads();
+        if (b + 1 < w.blocks.total) fetch(w.blocks.at(b + 1) * KB, lds[(b + 1) & 1]);
         if (!w.all_seen(a, k0, KB, w.p0, w.p1)) {
 #pragma unroll
-            for (int x = 0; x < LD; x++)
-                if (odd_values<DT>(vr[x])) {
+            for (int x = 0; x < LD; x++) {
+                u4 *at = reinterpret_cast<u4 *>(V) + 256 * x + threadIdx.x;
+                if (odd_values<DT>(*at)) {
                     odd = true;
-                    vr[x] = only_finite<DT>(vr[x]);
+                    *at = only_finite<DT>(*at);
                 }
+            }
+            lds_barrier();   /* no wait for the block that is on its way */
         }
-#pragma unroll
-        for (int x = 0; x < LD; x++) {
-            const int e = threadIdx.x + 256 * x, r = e / CH, ch = e % CH;
-            *reinterpret_cast<u4 *>(K + r * DH + EPC * (ch ^ (r & (CH - 1)))) = kr[x];
-            *reinterpret_cast<u4 *>(V + r * VP + EPC * ch) = vr[x];
-        }
-        /* a buffer is filled again two blocks on, and every wave has passed the barrier between only once it is done
-         * with the buffer */
-        __syncthreads();
-        if (b + 1 < w.blocks.total) fetch(w.blocks.at(b + 1) * KB);
-
         /* no query of this wave sees any of the block, or it has no query */
         if (pw1 < pw0 || k0 - pw1 > a.ahead || (pw0 - (k0 + KB - 1) >= a.window && k0 >= a.sinks)) continue;
         f16v s[NK];
@@ -639,28 +655,55 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
         for (int n = 0; n < NK; n++)
 #pragma unroll
             for (int i = 0; i < 16; i++) s[n][i] = 0.0f;
-#pragma unroll
-        for (int x = 0; x < QR; x++)
+        u4 kf[3][NK];   /* K's operands, two steps ahead */
+        auto read_k = [&](int x) __attribute__((always_inline)) {
 #pragma unroll
             for (int n = 0; n < NK; n++) {
                 const int r = 32 * n + col;
-                const u4 kk = *reinterpret_cast<const u4 *>(K + r * DH + EPC * ((2 * x + h) ^ (r & (CH - 1))));
+                kf[x % 3][n] = *reinterpret_cast<const u4 *>(K + r * DH + EPC * ((2 * x + h) ^ (r & (CH - 1))));
+            }
+        };
+        read_k(0);
+        read_k(1);
+#pragma unroll
+        for (int x = 0; x < QR; x++) {
+            if (x + 2 < QR) read_k(x + 2);
+#pragma unroll
+            for (int n = 0; n < NK; n++) {
                 if constexpr (F32) {
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kk[e]), __uint_as_float(q[x][e]), s[n],
-                                                                    0, 0, 0);
+                        s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[x % 3][n][e]),
+                                                                    __uint_as_float(q[x][e]), s[n], 0, 0, 0);
                 } else {
-                    s[n] = mfma32<DT>(kk, q[x], s[n]);
+                    s[n] = mfma32<DT>(kf[x % 3][n], q[x], s[n]);
                 }
             }
+        }
+        u4 vf[2][DH / 32];   /* 16-bit V's operands for 16 keys: of each eight, this half of the lanes has four */
+        auto read_v = [&](int k2) __attribute__((always_inline)) {
+            if constexpr (!F32) {
+                const int r = 16 * k2 + 4 * h + ((lane & 15) >> 2);
+                const uint16_t *row = reinterpret_cast<const uint16_t *>(V) + r * DH;
+#pragma unroll
+                for (int d = 0; d < DH / 32; d++) {
+                    const int at = 8 * place(r, 4 * d) + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                    const u2 va = lds_tr(row + at), vb = lds_tr(row + 8 * DH + at);
+                    vf[k2 & 1][d] = u4{va[0], va[1], vb[0], vb[1]};
+                }
+            }
+        };
+        read_v(0);
         if (!w.all_seen(a, k0, KB, pw0, pw1)) {
+            /* key e of the block (from this lane's first) is seen up to `last`, from `first` on or below `sink` */
+            const int base = k0 + 4 * h, last = imin(p + a.ahead, w.Lk - 1) - base, first = p - a.window + 1 - base,
+                      sink = a.sinks - base;
 #pragma unroll
             for (int n = 0; n < NK; n++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int key = k0 + 32 * n + 8 * (i / 4) + 4 * h + i % 4;
-                    if (!(key < w.Lk && key_visible(key, p, a.window, a.ahead, a.sinks))) s[n][i] = -INFINITY;
+                    const int e = 32 * n + 8 * (i / 4) + i % 4;
+                    if ((e > last) | ((e < first) & (e >= sink))) s[n][i] = -INFINITY;
                 }
         }
         float top = s[0][0];
@@ -668,9 +711,15 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
         for (int n = 0; n < NK; n++)
 #pragma unroll
             for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
-        const float mn = fmaxf(m, max_halves(top) * a.c), mu = mn == -INFINITY ? 0.0f : mn;
-        const float fade = exp2_fast(m - mu);
-        m = mn;
+        top = max_halves(top) * a.c;
+        if (__any(top > m + kSlack)) {   /* also the first block's: m is −inf there */
+            const float mn = fmaxf(m, top), fade = exp2_fast(m - (mn == -INFINITY ? 0.0f : mn));
+            m = mn;
+            l *= fade;
+#pragma unroll
+            for (int d = 0; d < DH / 32; d++) o[d] *= fade;
+        }
+        const float mu = m == -INFINITY ? 0.0f : m;
         float sum = 0.0f;
 #pragma unroll
         for (int n = 0; n < NK; n++)
@@ -679,39 +728,28 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
                 s[n][i] = exp2_fast(__builtin_fmaf(s[n][i], a.c, -mu));
                 sum += s[n][i];
             }
-        l = __builtin_fmaf(l, fade, sum);
-        if (__any(fade != 1.0f)) {
-#pragma unroll
-            for (int d = 0; d < DH / 32; d++) o[d] *= fade;
-        }
+        l += sum;
         if constexpr (F32) {
 #pragma unroll
             for (int n = 0; n < NK; n++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const E *row = V + (32 * n + 8 * (i / 4) + 4 * h + i % 4) * VP + col;
+                    const E *row = V + (32 * n + 8 * (i / 4) + 4 * h + i % 4) * DH + col;
 #pragma unroll
                     for (int d = 0; d < DH / 32; d++)
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(row[32 * d], s[n][i], o[d], 0, 0, 0);
                 }
         } else {
 #pragma unroll
-            for (int n = 0; n < NK; n++)
+            for (int k2 = 0; k2 < 2 * NK; k2++) {
+                if (k2 + 1 < 2 * NK) read_v(k2 + 1);
+                float pv[8];
 #pragma unroll
-                for (int k2 = 0; k2 < 2; k2++) {   /* 16 keys: of each eight, this half of the lanes has four */
-                    float pv[8];
+                for (int j = 0; j < 8; j++) pv[j] = s[k2 / 2][8 * (k2 & 1) + j];
+                const u4 pw = pack<DT>(pv);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) pv[j] = s[n][8 * k2 + j];
-                    const u4 pw = pack<DT>(pv);
-                    const uint16_t *row = reinterpret_cast<const uint16_t *>(V) +
-                                          (32 * n + 16 * k2 + 4 * h + ((lane & 15) >> 2)) * VP + 16 * ((lane >> 4) & 1) +
-                                          4 * (lane & 3);
-#pragma unroll
-                    for (int d = 0; d < DH / 32; d++) {
-                        const u2 va = lds_tr(row + 32 * d), vb = lds_tr(row + 8 * VP + 32 * d);
-                        o[d] = mfma32<DT>(u4{va[0], va[1], vb[0], vb[1]}, pw, o[d]);
-                    }
-                }
+                for (int d = 0; d < DH / 32; d++) o[d] = mfma32<DT>(vf[k2 & 1][d], pw, o[d]);
+            }
         }
     }
     l = sum_halves(l);

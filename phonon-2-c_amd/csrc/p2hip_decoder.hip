@@ -82,6 +82,8 @@ int check_rows(const char *name, const char *what, int dtype, const void *p, int
     if (!p || !aligned(p, 16)) return fail(P2H_E_ARG, "%s: %s is NULL or not 16-byte aligned", name, what);
     if (ld < width || (size_t)ld * elem_size(dtype) % 16 != 0)
         return fail(P2H_E_ARG, "%s: pitch %d of %s must be >= %d and a multiple of 16 bytes", name, ld, what, width);
+    /* a block's rows are addressed by 32-bit offsets from its first */
+    if (ld >= 1 << 23) return fail(P2H_E_ARG, "%s: pitch %d of %s must be below 2^23", name, ld, what);
     return P2H_OK;
 }
 

@@ -19,6 +19,8 @@
 
 #include <type_traits>
 
+#include "p2hip_async.h"
+
 namespace p2k {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
@@ -774,24 +776,6 @@ __global__ __launch_bounds__(256) void combine_softmax_wave(int rows, int T, flo
     }
 }
 
-/* Direct global → LDS loads (16 bytes per lane into 16-byte lane slots at lds + 16·lane). Issued from inline
- * assembly so that the compiler adds no waits of its own for them: the GEMM waits for them explicitly (wait_vm),
- * and the compiler's waits for its own loads stay correct since the vector-memory counter retires in order. */
-__device__ __forceinline__ void dma_16(const void *src, const void *lds)
-{
-    const uint32_t a = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(a) : "memory", "m0");
-}
-
-/* s_waitcnt vmcnt(N) alone (expcnt and lgkmcnt left open); a compiler barrier for memory operations */
-template <int N>
-__device__ __forceinline__ void wait_vm()
-{
-    static_assert(N >= 0 && N < 64, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((N & 0xF) | (0x7 << 4) | (0xF << 8) | ((N >> 4) << 14));
-    asm volatile("" ::: "memory");
-}
-
 /* A 16-byte load into registers, issued from inline assembly as dma_16 is: the caller waits for it explicitly
  * (wait_vm) and then passes the registers through pin16, after which the compiler may read them. */
 __device__ __forceinline__ v4u load16_async(const void *src)
@@ -801,12 +785,6 @@ __device__ __forceinline__ v4u load16_async(const void *src)
     return r;
 }
 __device__ __forceinline__ void pin16(v4u &r) { asm volatile("" : "+v"(r)); }
-
-/* this wave's LDS reads complete, then the workgroup barrier; no wait on vector memory */
-__device__ __forceinline__ void lds_barrier()
-{
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
 
 /* Relative-position self-attention of one head for 16 query rows (encoder.c:495-523 between the projections): the
  * scores S[i][j] = (Q_u[i]·K[j] + Q_v[i]·P[j + T − 1 − i])·scale, their softmax over j as combine_softmax_rows
