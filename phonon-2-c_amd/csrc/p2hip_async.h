@@ -31,12 +31,12 @@ __device__ __forceinline__ void lds_barrier()
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-/* dma_16 with a base that is the same for the whole wave and a byte offset per lane (below 2^31): no 64-bit addresses in
- * the lanes' registers. */
-__device__ __forceinline__ void dma_16(const void *base, uint32_t offset, const void *lds)
+/* dma_16 through a buffer descriptor: a byte offset per lane from its base; lanes whose bytes end past its size read
+ * nothing. */
+__device__ __forceinline__ void dma_16(__amdgpu_buffer_rsrc_t from, uint32_t offset, const void *lds)
 {
     const uint32_t a = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(a)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(a)
                  : "memory", "m0");
 }
 

@@ -25,6 +25,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
@@ -107,10 +108,14 @@ template <int DT> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c)
 
 /* Transposing LDS read of 16-bit values: of the 4 × 16 values that the 16 lanes of a group address (lane i: 4 values,
  * row i / 4, columns 4·(i % 4) ..), lane i gets column i's four. */
-__device__ __forceinline__ u2 lds_tr(const uint16_t *p)
+__device__ __forceinline__ u2 lds_tr(uint32_t at)   /* an LDS byte address */
 {
     typedef __attribute__((address_space(3))) s4 *lds4;
-    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p)));
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at)));
+}
+__device__ __forceinline__ u2 lds_tr(const uint16_t *p)
+{
+    return lds_tr((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint16_t *)(p));
 }
 
 /* max and sum over lanes l, l ^ 16, l ^ 32, l ^ 48, and over l, l ^ 32 */
@@ -416,7 +421,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope(RopeArgs a)
 /* ── attention over a window ───────────────────────────────────────────────────────────────────────────────── */
 
 struct WinArgs {
-    int q_rows, k_rows, n_seqs, heads, kv, ldq, ldk, ldv, ldo, window, ahead, sinks, tiles;
+    int q_rows, k_rows, n_seqs, heads, kv, ldq, ldk, ldv, ldo, window, ahead, sinks, tiles, hpw;
     float c;   /* scale · log2 e */
     const int *qs, *ks;
     const void *q, *k, *v;
@@ -459,18 +464,21 @@ __device__ __forceinline__ bool find_tile(const int *qs, int n_seqs, int q_rows,
     return false;
 }
 
-/* whether 16 bytes of elements hold an infinity or a NaN */
-template <int DT> __device__ __forceinline__ bool odd_values(u4 v)
+/* A sum to which 16 bytes of elements add 0, or a NaN if one of them is an infinity or a NaN: their products with zeros */
+template <int DT> __device__ __forceinline__ float odd_sum(u4 v, float sum)
 {
-    constexpr uint32_t E = DT == T_F32 ? 0x7f800000u : DT == T_F16 ? 0x7c007c00u : 0x7f807f80u;
-    constexpr uint32_t H = E & 0xffff0000u, L = E & 0xffffu;
-    bool odd = false;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        odd |= (v[i] & H) == H;
-        if (DT != T_F32) odd |= (v[i] & L) == L;
+        if constexpr (DT == T_F32) sum = __builtin_fmaf(__uint_as_float(v[i]), 0.0f, sum);
+        else if constexpr (DT == T_F16) sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, v[i]), h2{0, 0}, sum, false);
+        else sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, v[i]), b2{0, 0}, sum, false);
     }
-    return odd;
+    return sum;
+}
+template <int DT> __device__ __forceinline__ bool odd_values(u4 v)
+{
+    const float z = odd_sum<DT>(v, 0.0f);
+    return z != z;
 }
 
 /* the infinities and NaN among 16 bytes of elements replaced by zeros */
@@ -518,13 +526,14 @@ struct WinTile {
  * is added to the stored outputs here: any positive weight of an infinity or a NaN is that. Rare, so simple: one thread
  * per output, over every key of the blocks concerned. */
 template <int DT, int DH>
-__device__ __forceinline__ void add_odd_values(const WinArgs &a, const WinTile &w, int kvh, int head, int qb, int kb)
+__device__ __forceinline__ void add_odd_values(const WinArgs &a, const WinTile &w, int kvh, int head0, int n_heads, int qb,
+                                               int kb)
 {
     typedef typename Elem<DT>::type E;
     const E *vh = static_cast<const E *>(a.v) + (size_t)w.ka * a.ldv + (size_t)kvh * DH;
     const int n = imin(qb, w.Lq - w.i0);
-    for (int e = threadIdx.x; e < n * DH; e += blockDim.x) {
-        const int i = w.i0 + e / DH, d = e % DH, p = i + w.off;
+    for (int e = threadIdx.x; e < n * DH * n_heads; e += blockDim.x) {
+        const int head = head0 + e % (n_heads * DH) / DH, d = e % DH, i = w.i0 + e / (n_heads * DH), p = i + w.off;
         float more = 0.0f;
         for (int b = 0; b < w.blocks.total; b++) {
             const int k0 = w.blocks.at(b) * kb;
@@ -541,55 +550,309 @@ __device__ __forceinline__ void add_odd_values(const WinArgs &a, const WinTile &
     }
 }
 
-/* The window kernels' workgroups: a head and a tile. Query heads of one key head are apart by kv_heads, so that with 8 key
- * heads (or a multiple) each XCD, which takes every eighth workgroup, reads the keys of its own. Later tiles, which see
- * more keys where the window is long, come first. */
-__device__ __forceinline__ bool win_tile_of(const WinArgs &a, int qb, int *head, int *kvh, int *seq, int *tile)
+/* The window kernels' workgroups: a tile of queries of `hpw` query heads that read one key head, the first of them
+ * returned. Those of different key heads are next to each other, so that with 8 key heads (or a multiple) each XCD, which
+ * takes every eighth workgroup, reads the keys of its own. Later tiles, which see more keys where the window is long,
+ * come first. */
+__device__ __forceinline__ bool win_tile_of(const WinArgs &a, int hpw, int qb, int *head, int *kvh, int *seq, int *tile)
 {
-    const int id = blockIdx.x % a.heads;
+    const int sets = a.heads / hpw, id = blockIdx.x % sets;
     *kvh = id % a.kv;
-    *head = *kvh * (a.heads / a.kv) + id / a.kv;
-    return find_tile(a.qs, a.n_seqs, a.q_rows, qb, a.tiles - 1 - (int)(blockIdx.x / a.heads), seq, tile);
+    *head = *kvh * (a.heads / a.kv) + id / a.kv * hpw;
+    return find_tile(a.qs, a.n_seqs, a.q_rows, qb, a.tiles - 1 - (int)(blockIdx.x / sets), seq, tile);
 }
 
-/* O for 128 queries of one head, 32 for each of the four waves, in blocks of KB = 32·NK keys that pass through LDS by
- * direct loads, two buffers in turn: while one is multiplied the next block is on its way. Blocks without a visible key
- * are not touched.
+/* Where a 16-byte piece cc of row r lies in V's part of the LDS, 16-bit rows of CH pieces: its 64-byte group is moved
+ * so that a transposing read (8 rows, one group) falls into different banks. */
+template <int CH> __device__ __forceinline__ constexpr int v_place(int r, int cc)
+{
+    return cc ^ (CH == 16 ? 4 * (r & 3) : 4 * ((r >> 1) & 1));
+}
+
+/* The loads of a block of KB rows of one matrix by the NW waves of a workgroup, straight into LDS: per lane and load
+ * an offset from the block's first row, the 16-byte piece chosen so that it lands where `place` wants it. Rows past the
+ * last are not read: what lies in their place is kept from the result by the masks. */
+template <class E, int DH, int KB, int NW> struct BlockLoads {
+    static constexpr int EPC = 16 / sizeof(E), CH = DH / EPC, LD = KB * CH / (64 * NW), RPL = 64 / CH;
+    uint32_t off[LD];
+    int ld;
+    const E *base;
+    template <class P> __device__ __forceinline__ BlockLoads(const E *b, int pitch, int lane, int wave, P place)
+        : ld(pitch), base(b)
+    {
+#pragma unroll
+        for (int x = 0; x < LD; x++) {
+            const int r = RPL * (LD * wave + x) + lane / CH;
+            off[x] = (uint32_t)(r * ld + EPC * place(r, lane % CH)) * sizeof(E);
+        }
+    }
+    /* the block of rows k0 .. of `rows` */
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t from(int k0, int rows) const
+    {
+        const int last = imin(rows - k0, KB) - 1;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<E *>(base + (size_t)k0 * ld), 0,
+                                                 (int)((uint32_t)(last * ld + DH) * sizeof(E)), 0x00020000);
+    }
+    __device__ __forceinline__ void fetch(int x, __amdgpu_buffer_rsrc_t r, E *to, int wave) const
+    {
+        dma_16(r, off[x], to + 64 * EPC * (LD * wave + x));
+    }
+    __device__ __forceinline__ void fetch(int k0, int rows, E *to, int wave) const
+    {
+        const __amdgpu_buffer_rsrc_t r = from(k0, rows);
+#pragma unroll
+        for (int x = 0; x < LD; x++) fetch(x, r, to, wave);
+    }
+    /* what this lane's loads brought, once they have come: infinities and NaN become zeros; whether there were some */
+    template <int DT> static __device__ __forceinline__ bool clean(E *to, int lane, int wave)
+    {
+        u4 *at = reinterpret_cast<u4 *>(to) + 64 * LD * wave + lane;
+        float z = 0.0f;
+#pragma unroll
+        for (int x = 0; x < LD; x++) z = odd_sum<DT>(at[64 * x], z);
+        if (z == z) return false;
+#pragma unroll
+        for (int x = 0; x < LD; x++) at[64 * x] = only_finite<DT>(at[64 * x]);
+        return true;
+    }
+};
+
+/* Where the exponentials of a block have a sum above 2^kSlack in some lane, the reference they are taken from is raised to
+ * the largest score so far and they are taken again. It is not raised otherwise, so that most blocks need no maximum and
+ * leave O as it is: a weight stays below 2^kSlack, which every type holds, and relative to their sum nothing changes. */
+constexpr float kSlack = 1024.0f;
+
+/* 32 queries of one head in a wave: lane % 32 is the query, 16-bit rows. */
+template <int DH> struct WinSub {
+    f16v o[DH / 32], s[2];   /* O^T so far; the scores of a block */
+    u4 q[DH / 16], pw[4];    /* the query, elements 8(2x + lane / 32) .. of every 16; a block's weights, 16 keys each */
+    float m, l;              /* the reference, in powers of two, and this lane's sum of weights */
+    int p, full0, full1;     /* this lane's query's place; blocks from full0 to full1 on are seen whole by all queries */
+};
+
+/* O for 128 rows, 32 for each of four waves; 16-bit rows. The rows are 128 / hpw queries of each of hpw (1, 2 or 4) query
+ * heads that read the same key head: the fewer queries, the fewer keys that some of them must not see. The keys come in
+ * blocks of 64 through LDS, K and V in two buffers each; blocks without a visible key are not touched.
  *
- * Per block and wave S^T = K·Q^T by 32 × 32 products (keys in rows, queries in columns), so that a lane holds 16 keys of
- * one query: the running maximum and sum of its softmax need one exchange with the lane 32 away, and the weights are
+ * Per block and 32 queries S^T = K·Q^T by 32 × 32 products (keys in rows, queries in columns), so that a lane holds 32
+ * keys of one query: the sum of its weights needs one exchange with the lane 32 away, at the end, and the weights are
  * already laid out as the operand of O^T += V^T·P^T, whatever order that product takes the keys in, as V's operand reads
- * the same order out of LDS. 16-bit weights: the exponentials are rounded to the rows' type for that product and summed
- * unrounded in 32 bits; fp32 rows multiply in fp32 throughout.
+ * the same order out of LDS. The exponentials are rounded to the rows' type for that product and summed unrounded in 32
+ * bits.
  *
- * The exponentials are taken relative to a reference that is raised only when some query's maximum has come 2^kSlack
- * above it, since most blocks raise some maximum a little and each time all of O would be scaled: weights stay below
- * 2^kSlack, which every type holds, and relative to their sum nothing changes. */
-constexpr float kSlack = 8.0f;
-template <int DT, int DH, int NK>
+ * A block's exponentials take the vector unit about as long as its products take the matrix unit: two workgroups a CU put
+ * two waves on each SIMD, of which one can multiply while the other takes exponentials. For that a wave's products are
+ * one stretch without waits: the scores of block b together with the output product of block b − 1, in QR equal stages,
+ * each stage's operands read from LDS two stages ahead, and one of the loads of K of block b + 1 and V of block b issued
+ * in each (all at once they would wait for each other: a CU takes 64 bytes a cycle). One barrier a block: there the loads
+ * of the block before have come, and everyone is done with what the next ones overwrite. */
+template <int DT, int DH>
 __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
 {
     typedef typename Elem<DT>::type E;
-    constexpr bool F32 = DT == T_F32;
-    constexpr int KB = 32 * NK;
-    constexpr int EPC = kPer16<DT>, CH = DH / EPC;   /* elements per 16 bytes, those per row */
-    constexpr int LD = KB * CH / 256, RPL = 64 / CH; /* direct loads per wave and block, of K and of V; rows of each */
-    __shared__ __align__(16) E lds[2][2 * KB * DH];
+    constexpr int KB = 64, CH = DH / 8, QR = DH / 16, NT = DH / 32;
+    typedef BlockLoads<E, DH, KB, 4> Loads;
+    static_assert(2 * Loads::LD == QR, "one load a stage");
+    __shared__ __align__(16) E lds[4][KB * DH];   /* K of even and odd blocks, V of even and odd blocks */
+
+    int head0, kvh, seq, tile;
+    if (!win_tile_of(a, a.hpw, 128 / a.hpw, &head0, &kvh, &seq, &tile)) return;
+    const WinTile w(a, seq, tile, 128 / a.hpw, KB);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5,
+              col = lane & 31;
+    const int head = head0 + wave % a.hpw, sub = 32 * (wave / a.hpw);   /* this wave's head and its first query */
+
+    /* K's row r has its piece cc at place cc ^ (r mod CH): the operand reads (32 rows, one piece) fall into different
+     * banks */
+    const Loads kl(static_cast<const E *>(a.k) + (size_t)w.ka * a.ldk + (size_t)kvh * DH, a.ldk, lane, wave,
+                   [](int r, int cc) { return cc ^ (r & (CH - 1)); });
+    const Loads vl(static_cast<const E *>(a.v) + (size_t)w.ka * a.ldv + (size_t)kvh * DH, a.ldv, lane, wave,
+                   [](int r, int cc) { return v_place<CH>(r, cc); });
+    const int n_blocks = w.blocks.total;
+    if (n_blocks > 0) kl.fetch(w.blocks.at(0) * KB, w.Lk, lds[0], wave);
+
+    WinSub<DH> u;
+    const int iq = w.i0 + sub + col;
+    {
+        const E *row = static_cast<const E *>(a.q) + (size_t)(w.qa + imin(iq, w.Lq - 1)) * a.ldq + (size_t)head * DH;
+#pragma unroll
+        for (int x = 0; x < QR; x++) u.q[x] = *reinterpret_cast<const u4 *>(row + 8 * (2 * x + h));
+    }
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) u.o[d][i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) u.pw[k] = u4{0, 0, 0, 0};
+    u.m = -INFINITY;
+    u.l = 0.0f;
+    u.p = iq + w.off;
+    u.full0 = imin(w.p0 + sub + 31, w.Lq - 1 + w.off) - a.window + 1;
+    u.full1 = imin(w.Lk - 1, w.p0 + sub + a.ahead) - (KB - 1);
+    bool odd = false;
+
+    /* LDS byte addresses. K's operand x of 32 keys: row col, piece 2x + h, so that the pieces of a row are an exclusive or
+     * apart; V's operand for dimensions 32d .. and 16 keys, of each eight of which this half of the lanes has four: the
+     * 64-byte groups of a row are. */
+    constexpr uint32_t BUF = KB * DH * 2;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
+    const int vr = 4 * h + ((lane & 15) >> 2);
+    const uint32_t k_at = lds0 + col * DH * 2 + 16 * (h ^ (col & (CH - 1)));
+    const uint32_t v_at = lds0 + 2 * BUF + vr * DH * 2 + 16 * v_place<CH>(vr, 0) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    auto read_k = [&](uint32_t at, int n, int x) __attribute__((always_inline)) {
+        typedef __attribute__((address_space(3))) const u4 *lds16;
+        return *(lds16)(uintptr_t)((at ^ (32 * x)) + 32 * n * DH * 2);
+    };
+    auto read_v = [&](uint32_t at, int k2, int d) __attribute__((always_inline)) {
+        const uint32_t x = (at ^ (64 * d)) + 16 * k2 * DH * 2;
+        const u2 va = lds_tr(x), vb = lds_tr(x + 8 * DH * 2);
+        return u4{va[0], va[1], vb[0], vb[1]};
+    };
+    /* this wave's loads have come; of V of block b, where some query must not see a key, what is not finite is put aside */
+    auto come = [&](int b) __attribute__((always_inline)) {
+        wait_vm<0>();
+        if (b >= 0 && !w.all_seen(a, w.blocks.at(b) * KB, KB, w.p0, w.p1))
+            odd |= Loads::template clean<DT>(lds[2 + (b & 1)], lane, wave);
+        lds_barrier();
+    };
+    /* What a query must not see of the block at k0, where its 32 queries do not all see all of it. Key e of the block is
+     * seen up to `last`, from `first` on or below `sink`: bit e of 64; this lane has keys 8j + 4h .. + 3 of every eight. */
+    auto mask = [&](int k0) __attribute__((always_inline)) {
+        if (k0 <= u.full1 && (k0 >= u.full0 || k0 < a.sinks - (KB - 1))) return;
+        const int last = imin(u.p + a.ahead, w.Lk - 1) - k0, first = u.p - a.window + 1 - k0, sink = a.sinks - k0;
+        auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
+        const unsigned long long bits = (below(last + 1) & (~below(first) | below(sink))) >> (4 * h);
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const uint32_t seen = (uint32_t)__builtin_amdgcn_sbfe((int)(bits >> (32 * n)), 8 * (i / 4) + i % 4, 1);
+                u.s[n][i] = __uint_as_float((__float_as_uint(u.s[n][i]) & seen) | (0xff800000u & ~seen));
+            }
+    };
+    /* weights 8·k .. 8·k + 7 of u's scores from the reference mu on, added to sum */
+    auto weights = [&](int k, float mu, float &sum) __attribute__((always_inline)) {
+        float pv[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            pv[i] = exp2_fast(__builtin_fmaf(u.s[k / 2][8 * (k & 1) + i], a.c, -mu));
+            sum += pv[i];
+        }
+        u.pw[k] = pack<DT>(pv);
+    };
+    /* the weights' sum goes into l; before, where it is too large or there is no reference yet, they are taken again from
+     * the largest score */
+    auto settle = [&](float sum) __attribute__((always_inline)) {
+        if (__any(sum > kSlack || u.m == -INFINITY)) {
+            float top = u.s[0][0];
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) top = fmaxf(top, u.s[n][i]);
+            const float mn = fmaxf(u.m, max_halves(top) * a.c), mu = mn == -INFINITY ? 0.0f : mn;
+            const float fade = exp2_fast(u.m - mu);
+            u.m = mn;
+            u.l *= fade;
+#pragma unroll
+            for (int d = 0; d < NT; d++) u.o[d] *= fade;
+            sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) weights(k, mu, sum);
+        }
+        u.l += sum;
+    };
+    if (n_blocks > 0) {
+        /* the first block has no weights before it: zeros, with zeros for V */
+        for (int x = threadIdx.x; x < KB * CH; x += 256) reinterpret_cast<u4 *>(lds[3])[x] = u4{0, 0, 0, 0};
+        for (int b = 0; b < n_blocks; b++) {
+            const int k0 = w.blocks.at(b) * KB;
+            /* past the last block that one's K again, which nothing reads */
+            const __amdgpu_buffer_rsrc_t next_k = kl.from(w.blocks.at(imin(b + 1, n_blocks - 1)) * KB, w.Lk),
+                                         this_v = vl.from(k0, w.Lk);
+            const uint32_t ka = k_at + (b & 1) * BUF, va = v_at + ((b & 1) ^ 1) * BUF;
+            u4 kf[3][2], vf[3][2];
+            auto read = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    kf[t % 3][j] = read_k(ka, j, t);
+                    vf[t % 3][j] = read_v(va, (2 * t + j) / NT, (2 * t + j) % NT);
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < 16; i++) u.s[0][i] = u.s[1][i] = 0.0f;
+            come(b - 1);
+            read(0);
+            read(1);
+#pragma unroll
+            for (int t = 0; t < QR; t++) {   /* the barriers to the scheduler keep this order */
+                if (t + 2 < QR) read(t + 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int z = 2 * t + j;
+                    u.s[j] = mfma32<DT>(kf[t % 3][j], u.q[t], u.s[j]);
+                    u.o[z % NT] = mfma32<DT>(vf[t % 3][j], u.pw[z / NT], u.o[z % NT]);
+                }
+                if (t < Loads::LD) kl.fetch(t, next_k, lds[(b & 1) ^ 1], wave);
+                else vl.fetch(t - Loads::LD, this_v, lds[2 + (b & 1)], wave);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            mask(k0);
+            const float mu = u.m == -INFINITY ? 0.0f : u.m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) weights(k, mu, sum);
+            settle(sum);
+        }
+        come(n_blocks - 1);
+        const uint32_t va = v_at + ((n_blocks - 1) & 1) * BUF;
+#pragma unroll
+        for (int k2 = 0; k2 < 4; k2++)
+#pragma unroll
+            for (int d = 0; d < NT; d++) u.o[d] = mfma32<DT>(read_v(va, k2, d), u.pw[k2], u.o[d]);
+    }
+    const float l = sum_halves(u.l), inv = l == 0.0f ? 0.0f : 1.0f / l;
+    E *row = static_cast<E *>(a.o) + (size_t)(w.qa + imin(iq, w.Lq - 1)) * a.ldo + (size_t)head * DH + 8 * h;
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+            /* of 16 elements this lane has 4 of the first eight and 4 of the second; the lane 32 away the others */
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = u.o[d][4 * k + j] * inv;
+            const u4 x = pack<DT>(v);
+            const auto e0 = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+            const auto e1 = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+            if (iq < w.Lq) *reinterpret_cast<u4 *>(row + 32 * d + 8 * k) = u4{e0[0], e1[0], e0[1], e1[1]};
+        }
+    /* the barrier in it also puts the stores above before the reads behind it */
+    if (__syncthreads_or(odd)) add_odd_values<DT, DH>(a, w, kvh, head0, a.hpw, 128 / a.hpw, KB);
+}
+
+/* attention_win for fp32 rows, multiplied in fp32 throughout: its products take the matrix unit several times as long as
+ * everything else takes, so nothing is gained by running them together with the exponentials. Blocks of 32 keys, two
+ * buffers in turn: while one is multiplied the next is on its way. */
+template <int DH>
+__global__ __launch_bounds__(256, 2) void attention_win_f32(WinArgs a)
+{
+    constexpr int DT = T_F32, KB = 32, CH = DH / 4, QR = DH / 8;
+    __shared__ __align__(16) float lds[2][2 * KB * DH];
 
     int head, kvh, seq, tile;
-    if (!win_tile_of(a, 128, &head, &kvh, &seq, &tile)) return;
+    if (!win_tile_of(a, 1, 128, &head, &kvh, &seq, &tile)) return;
     const WinTile w(a, seq, tile, 128, KB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5,
               col = lane & 31;
     const int iq = w.i0 + 32 * wave + col, p = iq + w.off;
     const int pw0 = w.p0 + 32 * wave, pw1 = imin(pw0 + 31, w.Lq - 1 + w.off);   /* this wave's places */
 
-    constexpr int QR = DH / (2 * EPC);   /* this lane's query: elements EPC·(2s + h) .. of every 2·EPC */
-    u4 q[QR];
+    u4 q[QR];   /* this lane's query: elements 4(2x + h) .. of every 8 */
     {
-        const E *row = static_cast<const E *>(a.q) + (size_t)(w.qa + imin(iq, w.Lq - 1)) * a.ldq + (size_t)head * DH;
+        const float *row = static_cast<const float *>(a.q) + (size_t)(w.qa + imin(iq, w.Lq - 1)) * a.ldq +
+                           (size_t)head * DH;
 #pragma unroll
-        for (int s = 0; s < QR; s++) q[s] = *reinterpret_cast<const u4 *>(row + EPC * (2 * s + h));
+        for (int x = 0; x < QR; x++) q[x] = *reinterpret_cast<const u4 *>(row + 4 * (2 * x + h));
     }
     f16v o[DH / 32];
 #pragma unroll
@@ -599,120 +862,52 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
     float m = -INFINITY, l = 0.0f;   /* the reference, in powers of two, and this lane's sum of weights */
     bool odd = false;
 
-    /* Row r's 16-byte piece cc lies at place cc ^ (r mod CH) of K's row, so that the operand reads (32 rows, one piece)
-     * fall into different banks. 16-bit V: its 64-byte piece s lies at place s ^ (r mod pieces), and a transposing read
-     * (8 rows, one 64-byte piece) falls into different banks; fp32 V is read along its rows. */
-    auto place = [](int r, int cc) { return F32 ? cc : cc ^ (CH == 16 ? 4 * (r & 3) : 4 * ((r >> 1) & 1)); };
-    const E *kh = static_cast<const E *>(a.k) + (size_t)w.ka * a.ldk + (size_t)kvh * DH;
-    const E *vh = static_cast<const E *>(a.v) + (size_t)w.ka * a.ldv + (size_t)kvh * DH;
-    uint32_t koff[LD], voff[LD];
-#pragma unroll
-    for (int x = 0; x < LD; x++) {
-        const int r = RPL * (wave * LD + x) + lane / CH, cc = lane % CH;
-        koff[x] = (uint32_t)(r * a.ldk + EPC * (cc ^ (r & (CH - 1)))) * sizeof(E);
-        voff[x] = (uint32_t)(r * a.ldv + EPC * place(r, cc)) * sizeof(E);
-    }
-    auto fetch = [&](int k0, E *to) __attribute__((always_inline)) {
-        const E *kb = kh + (size_t)k0 * a.ldk, *vb = vh + (size_t)k0 * a.ldv;
-        const int left = w.Lk - k0;
-#pragma unroll
-        for (int x = 0; x < LD; x++) {
-            const int u = wave * LD + x;
-            uint32_t ko = koff[x], vo = voff[x];
-            if (left < KB) {   /* past the sequence its last row, which the masks leave out */
-                const int r = RPL * u + lane / CH, back = r < left ? 0 : r - (left - 1);
-                ko -= (uint32_t)(back * a.ldk) * sizeof(E);
-                vo -= (uint32_t)(back * a.ldv) * sizeof(E);
-            }
-            dma_16(kb, ko, to + 64 * EPC * u);
-            dma_16(vb, vo, to + KB * DH + 64 * EPC * u);
-        }
+    const BlockLoads<float, DH, KB, 4> kl(static_cast<const float *>(a.k) + (size_t)w.ka * a.ldk + (size_t)kvh * DH, a.ldk,
+                                       lane, wave, [](int r, int cc) { return cc ^ (r & (CH - 1)); });
+    const BlockLoads<float, DH, KB, 4> vl(static_cast<const float *>(a.v) + (size_t)w.ka * a.ldv + (size_t)kvh * DH, a.ldv,
+                                       lane, wave, [](int, int cc) { return cc; });
+    auto fetch = [&](int k0, float *to) __attribute__((always_inline)) {
+        kl.fetch(k0, w.Lk, to, wave);
+        vl.fetch(k0, w.Lk, to + KB * DH, wave);
     };
 
     if (w.blocks.total > 0) fetch(w.blocks.at(0) * KB, lds[0]);
     for (int b = 0; b < w.blocks.total; b++) {
         const int k0 = w.blocks.at(b) * KB;
-        E *K = lds[b & 1], *V = K + KB * DH;
-        /* this wave's loads have come, then everyone's; and every wave is done with the other buffer */
+        float *K = lds[b & 1], *V = K + KB * DH;
+        /* this wave's loads have come, and of V, where some query must not see a key, what is not finite is put aside; then
+         * everyone's, and every wave is done with the other buffer */
         wait_vm<0>();
+        if (!w.all_seen(a, k0, KB, w.p0, w.p1)) odd |= BlockLoads<float, DH, KB, 4>::template clean<DT>(V, lane, wave);
         __syncthreads();
         if (b + 1 < w.blocks.total) fetch(w.blocks.at(b + 1) * KB, lds[(b + 1) & 1]);
-        if (!w.all_seen(a, k0, KB, w.p0, w.p1)) {
-#pragma unroll
-            for (int x = 0; x < LD; x++) {
-                u4 *at = reinterpret_cast<u4 *>(V) + 256 * x + threadIdx.x;
-                if (odd_values<DT>(*at)) {
-                    odd = true;
-                    *at = only_finite<DT>(*at);
-                }
-            }
-            lds_barrier();   /* no wait for the block that is on its way */
-        }
         /* no query of this wave sees any of the block, or it has no query */
         if (pw1 < pw0 || k0 - pw1 > a.ahead || (pw0 - (k0 + KB - 1) >= a.window && k0 >= a.sinks)) continue;
-        f16v s[NK];
+        f16v s;
 #pragma unroll
-        for (int n = 0; n < NK; n++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[n][i] = 0.0f;
-        u4 kf[3][NK];   /* K's operands, two steps ahead */
-        auto read_k = [&](int x) __attribute__((always_inline)) {
-#pragma unroll
-            for (int n = 0; n < NK; n++) {
-                const int r = 32 * n + col;
-                kf[x % 3][n] = *reinterpret_cast<const u4 *>(K + r * DH + EPC * ((2 * x + h) ^ (r & (CH - 1))));
-            }
-        };
-        read_k(0);
-        read_k(1);
+        for (int i = 0; i < 16; i++) s[i] = 0.0f;
 #pragma unroll
         for (int x = 0; x < QR; x++) {
-            if (x + 2 < QR) read_k(x + 2);
+            const u4 k = *reinterpret_cast<const u4 *>(K + col * DH + 4 * ((2 * x + h) ^ (col & (CH - 1))));
 #pragma unroll
-            for (int n = 0; n < NK; n++) {
-                if constexpr (F32) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[x % 3][n][e]),
-                                                                    __uint_as_float(q[x][e]), s[n], 0, 0, 0);
-                } else {
-                    s[n] = mfma32<DT>(kf[x % 3][n], q[x], s[n]);
-                }
-            }
+            for (int e = 0; e < 4; e++)
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(q[x][e]), s, 0, 0, 0);
         }
-        u4 vf[2][DH / 32];   /* 16-bit V's operands for 16 keys: of each eight, this half of the lanes has four */
-        auto read_v = [&](int k2) __attribute__((always_inline)) {
-            if constexpr (!F32) {
-                const int r = 16 * k2 + 4 * h + ((lane & 15) >> 2);
-                const uint16_t *row = reinterpret_cast<const uint16_t *>(V) + r * DH;
-#pragma unroll
-                for (int d = 0; d < DH / 32; d++) {
-                    const int at = 8 * place(r, 4 * d) + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                    const u2 va = lds_tr(row + at), vb = lds_tr(row + 8 * DH + at);
-                    vf[k2 & 1][d] = u4{va[0], va[1], vb[0], vb[1]};
-                }
-            }
-        };
-        read_v(0);
         if (!w.all_seen(a, k0, KB, pw0, pw1)) {
             /* key e of the block (from this lane's first) is seen up to `last`, from `first` on or below `sink` */
             const int base = k0 + 4 * h, last = imin(p + a.ahead, w.Lk - 1) - base, first = p - a.window + 1 - base,
                       sink = a.sinks - base;
 #pragma unroll
-            for (int n = 0; n < NK; n++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int e = 32 * n + 8 * (i / 4) + i % 4;
-                    if ((e > last) | ((e < first) & (e >= sink))) s[n][i] = -INFINITY;
-                }
+            for (int i = 0; i < 16; i++) {
+                const int e = 8 * (i / 4) + i % 4;
+                if ((e > last) | ((e < first) & (e >= sink))) s[i] = -INFINITY;
+            }
         }
-        float top = s[0][0];
+        float top = s[0];
 #pragma unroll
-        for (int n = 0; n < NK; n++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
+        for (int i = 0; i < 16; i++) top = fmaxf(top, s[i]);
         top = max_halves(top) * a.c;
-        if (__any(top > m + kSlack)) {   /* also the first block's: m is −inf there */
+        if (__any(top > m + 8.0f)) {   /* the reference is raised where a maximum is 2^8 above it, and in the first block */
             const float mn = fmaxf(m, top), fade = exp2_fast(m - (mn == -INFINITY ? 0.0f : mn));
             m = mn;
             l *= fade;
@@ -722,47 +917,30 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
         const float mu = m == -INFINITY ? 0.0f : m;
         float sum = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NK; n++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                s[n][i] = exp2_fast(__builtin_fmaf(s[n][i], a.c, -mu));
-                sum += s[n][i];
-            }
+        for (int i = 0; i < 16; i++) {
+            s[i] = exp2_fast(__builtin_fmaf(s[i], a.c, -mu));
+            sum += s[i];
+        }
         l += sum;
-        if constexpr (F32) {
 #pragma unroll
-            for (int n = 0; n < NK; n++)
+        for (int i = 0; i < 16; i++) {
+            const float *row = V + (8 * (i / 4) + 4 * h + i % 4) * DH + col;
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const E *row = V + (32 * n + 8 * (i / 4) + 4 * h + i % 4) * DH + col;
-#pragma unroll
-                    for (int d = 0; d < DH / 32; d++)
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(row[32 * d], s[n][i], o[d], 0, 0, 0);
-                }
-        } else {
-#pragma unroll
-            for (int k2 = 0; k2 < 2 * NK; k2++) {
-                if (k2 + 1 < 2 * NK) read_v(k2 + 1);
-                float pv[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) pv[j] = s[k2 / 2][8 * (k2 & 1) + j];
-                const u4 pw = pack<DT>(pv);
-#pragma unroll
-                for (int d = 0; d < DH / 32; d++) o[d] = mfma32<DT>(vf[k2 & 1][d], pw, o[d]);
-            }
+            for (int d = 0; d < DH / 32; d++)
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(row[32 * d], s[i], o[d], 0, 0, 0);
         }
     }
     l = sum_halves(l);
     if (iq < w.Lq) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        E *row = static_cast<E *>(a.o) + (size_t)(w.qa + iq) * a.ldo + (size_t)head * DH + 4 * h;
+        float *row = static_cast<float *>(a.o) + (size_t)(w.qa + iq) * a.ldo + (size_t)head * DH + 4 * h;
 #pragma unroll
         for (int d = 0; d < DH / 32; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) row[32 * d + 8 * (i / 4) + i % 4] = Elem<DT>::put(o[d][i] * inv);
+            for (int i = 0; i < 16; i++) row[32 * d + 8 * (i / 4) + i % 4] = o[d][i] * inv;
     }
     /* the barrier in it also puts the stores above before the reads behind it */
-    if (__syncthreads_or(odd)) add_odd_values<DT, DH>(a, w, kvh, head, 128, KB);
+    if (__syncthreads_or(odd)) add_odd_values<DT, DH>(a, w, kvh, head, 1, 128, KB);
 }
 
 /* ── attention of few queries ──────────────────────────────────────────────────────────────────────────────── */
@@ -986,7 +1164,7 @@ __global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_win_few(W
     constexpr int NB = DT == T_F32 ? 1 : 2, KB = 16 * NB, EPC = kPer16<DT>;
     __shared__ __align__(16) unsigned char lds[few_lds_bytes<DT, DH, NW>()];
     int head, kvh, seq, tile;
-    if (!win_tile_of(a, 16, &head, &kvh, &seq, &tile)) return;
+    if (!win_tile_of(a, 1, 16, &head, &kvh, &seq, &tile)) return;
     const WinTile w(a, seq, tile, 16, KB);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int i = imin(w.i0 + (lane & 15), w.Lq - 1), p = i + w.off;
@@ -1026,7 +1204,7 @@ __global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_win_few(W
         static_cast<E *>(a.o)[(size_t)(w.qa + w.i0 + e / DH) * a.ldo + (size_t)head * DH + e % DH] =
             Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
     }
-    if (__syncthreads_or(odd)) add_odd_values<DT, DH>(a, w, kvh, head, 16, KB);
+    if (__syncthreads_or(odd)) add_odd_values<DT, DH>(a, w, kvh, head, 1, 16, KB);
 }
 
 /* One workgroup: one sequence, one key head, up to 16 of the query heads that read it, one part of its key blocks, which

@@ -349,23 +349,26 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
             return fail(P2H_E_ARG, "%s: dO overlaps dK or dV", name);
     }
     if (overlap(o, Rows{(const char *)dQ, ldq * es, q_w, q_rows})) return fail(P2H_E_ARG, "%s: dO overlaps dQ", name);
-    /* tiles of 16 or 128 queries: at most one more per sequence than the rows fill */
+    /* The queries of a tile and the query heads a workgroup takes (its kernel says why); at most one tile more per
+     * sequence than the rows fill. */
+    const int G = heads / kv_heads, hpw = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
     const bool few = (long long)((q_rows + 127) / 128) * heads < 256;
-    const int qb = few ? 16 : 128;
+    const int qb = few ? 16 : dtype == P2H_F32 ? 128 : 128 / hpw, per = few || dtype == P2H_F32 ? 1 : hpw;
     const long long tiles = (long long)(dQStart ? q_rows / qb + p2k::imin(n_seqs, q_rows) : (q_rows + qb - 1) / qb);
     if (tiles * heads > INT_MAX) return fail(P2H_E_ARG, "%s: %lld tiles of %d heads", name, tiles, heads);
     if (int rc = ensure_init()) return rc;
     p2k::WinArgs a{};
     a.q_rows = q_rows; a.k_rows = k_rows; a.n_seqs = n_seqs; a.heads = heads; a.kv = kv_heads;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo; a.window = window; a.ahead = ahead; a.sinks = sinks;
-    a.tiles = (int)tiles; a.c = scale * p2k::kLog2e;
+    a.tiles = (int)tiles; a.hpw = per; a.c = scale * p2k::kLog2e;
     a.qs = dQStart; a.ks = dKStart; a.q = dQ; a.k = dK; a.v = dV; a.o = dO;
     hipStream_t s = stream_of(stream);
-    const dim3 grid((unsigned)(tiles * heads));
+    const dim3 grid((unsigned)(tiles * (heads / per)));
     by_type_dim(dtype, head_dim, [&](auto t, auto d) {
         constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
         if (few) hipLaunchKernelGGL((p2k::attention_win_few<DT, DH, 8>), grid, dim3(512), 0, s, a);
-        else hipLaunchKernelGGL((p2k::attention_win<DT, DH, DT == p2k::T_F32 ? 1 : 2>), grid, dim3(256), 0, s, a);
+        else if constexpr (DT == p2k::T_F32) hipLaunchKernelGGL((p2k::attention_win_f32<DH>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((p2k::attention_win<DT, DH>), grid, dim3(256), 0, s, a);
     });
     HIPCHK(hipGetLastError());
     return P2H_OK;
