@@ -736,8 +736,8 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             pv[i] = exp2_fast(__builtin_fmaf(u.s[k / 2][8 * (k & 1) + i], a.c, -mu));
-            sum += pv[i];
         }
+        sum += ((pv[0] + pv[1]) + (pv[2] + pv[3])) + ((pv[4] + pv[5]) + (pv[6] + pv[7]));
         u.pw[k] = pack<DT>(pv);
     };
     /* the weights' sum goes into l; before, where it is too large or there is no reference yet, they are taken again from
@@ -781,6 +781,7 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
 #pragma unroll
             for (int i = 0; i < 16; i++) u.s[0][i] = u.s[1][i] = 0.0f;
             come(b - 1);
+            __builtin_amdgcn_s_setprio(1);   /* products first: the other wave's exponentials fill what they leave */
             read(0);
             read(1);
 #pragma unroll
@@ -797,6 +798,7 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
                 else vl.fetch(t - Loads::LD, this_v, lds[2 + (b & 1)], wave);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_setprio(0);
             mask(k0);
             const float mu = u.m == -INFINITY ? 0.0f : u.m;
             float sum = 0.0f;
