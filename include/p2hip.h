@@ -388,7 +388,7 @@ size_t p2h_q4_weight_device_bytes(const P2hQ4Weight *w);
 /* Y [M][N] = alpha · X [M][K] · W + beta · Y for few rows (beta 0 does not read Y): a matrix-vector product per row,
  * the weight read once for every 16 rows. X and Y of type `dtype`, pitches ldx >= K and ldy >= N elements, no alignment
  * beyond the element's (16-byte aligned rows load faster). A row's outputs are the same bits whatever M is. X and Y
- * must not overlap. */
+ * must not overlap. A group's products are summed before its scale is applied: values of |x| from 2^118 up may overflow. */
 int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int ldx, const P2hQ4Weight *w, float beta,
                 void *dY, int ldy, void *stream);
 

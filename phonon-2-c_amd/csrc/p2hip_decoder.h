@@ -196,18 +196,45 @@ struct Q4Args {
     const void *sc;
 };
 
-/* Two codes of a record word, nibbles i and i + 4, as fp16 code − zero: 1024 + code has the code in its low bits, and
- * adding −(1024 + zero) is exact. */
-__device__ __forceinline__ h2 q4_pair(uint32_t w, int i, h2 bias)
+/* A record word's eight codes as matrix-core operand. fp16: code − zero; 1024 + code has the code in its low bits, 1024 + 16
+ * code where it lies four bits up, and adding −(1024 + zero), or a sixteenth and −(64 + zero), is exact: 9 instructions
+ * for 8 weights. bf16: the same by way of fp32, of which the upper halves are all there is: 25; or (CODES) the code, as
+ * fp8 (e4m3) has 0 .. 15 times 2^-9 in the bits 0 .. 15, which one conversion turns into two bf16 values: 8. */
+template <int DT, bool CODES = false>
+__device__ __forceinline__ u4 q4_operand(uint32_t w, _Float16 bias, uint32_t low, uint32_t magic)
 {
-    const uint32_t t = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-    return __builtin_bit_cast(h2, t) + bias;
+    u4 v;
+    if constexpr (CODES) {
+        typedef __bf16 bb __attribute__((ext_vector_type(2)));
+        w = __builtin_amdgcn_perm(w, w, 0x03010200u);   /* nibbles i and i + 4 into neighbouring bytes */
+        const uint32_t a = w & 0x0f0f0f0fu, b = (w >> 4) & 0x0f0f0f0fu;
+        v[0] = __builtin_bit_cast(uint32_t, (bb)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 512.0f, false));
+        v[1] = __builtin_bit_cast(uint32_t, (bb)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 512.0f, false));
+        v[2] = __builtin_bit_cast(uint32_t, (bb)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 512.0f, true));
+        v[3] = __builtin_bit_cast(uint32_t, (bb)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 512.0f, true));
+    } else {
+        const h2 one = {bias, bias}, up = {(_Float16)0.0625f, (_Float16)0.0625f};
+        const h2 six = one + h2{(_Float16)960.0f, (_Float16)960.0f};   /* −(64 + zero) */
+        const uint32_t w8 = w >> 8;
+        h2 d[4];
+        d[0] = __builtin_bit_cast(h2, (w & low) | magic) + one;
+        d[1] = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & (low << 4)) | magic), up, six);
+        d[2] = __builtin_bit_cast(h2, (w8 & low) | magic) + one;
+        d[3] = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w8 & (low << 4)) | magic), up, six);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (DT == T_F16) v[i] = __builtin_bit_cast(uint32_t, d[i]);
+            else v[i] = __builtin_amdgcn_perm(__float_as_uint((float)d[i][1]), __float_as_uint((float)d[i][0]), 0x07060302u);
+        }
+    }
+    return v;
 }
 
 /* Eight fp32 values as three bf16 pieces each, the upper 16 bits of what is left after the pieces before: exact, as 8 + 8
- * + 8 bits hold the 24 of a float. Nothing is left of an infinity. */
-__device__ __forceinline__ void cut3(uint32_t (&v)[8], u4 (&xp)[3])
+ * + 8 bits hold the 24 of a float. Nothing is left of an infinity where they are looked for (INF), a NaN otherwise. */
+template <bool INF> __device__ __forceinline__ void cut3(u4 lo, u4 hi, u4 (&xp)[3])
 {
+    uint32_t v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
     for (int p = 0; p < 3; p++) {
 #pragma unroll
@@ -216,107 +243,181 @@ __device__ __forceinline__ void cut3(uint32_t (&v)[8], u4 (&xp)[3])
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const float left = __uint_as_float(v[j]) - __uint_as_float(v[j] & 0xffff0000u);
-            v[j] = p == 0 && (v[j] & 0x7fffffffu) == 0x7f800000u ? 0u : __float_as_uint(left);
+            v[j] = INF && p == 0 && (v[j] & 0x7fffffffu) == 0x7f800000u ? 0u : __float_as_uint(left);
         }
     }
 }
 
-/* Y rows 16·blockIdx.y .. of 16 columns: each of the WV waves sums its 128-row units of K, unit after unit, and the waves'
- * sums are added in order in LDS. A group's products are summed as whole (code − zero) times x, exact factors in both
- * operands, and scaled once per group in 32 bits.
+/* Y rows 16·blockIdx.y .. of 16·NT columns: each of the WV waves sums its 128-row units of K, unit after unit, and the
+ * waves' sums are added in order in LDS. A group's products are summed as whole (code − zero) times x, exact factors in
+ * both operands, and scaled once per group in 32 bits.
  *
- * fp16 rows multiply as fp16. bf16 rows multiply as bf16 (whole numbers up to 15 are exact there too). fp32 rows are cut
- * into three bf16 pieces (8 + 8 + 8 bits, the pieces of a non-finite value are that value and zeros), which sum to the
- * row exactly: three products into the same sums. */
-template <int DT, int GROUP, bool ZP, int WV>
+ * fp16 rows multiply as fp16, with code − zero. bf16 rows multiply as bf16 (whole numbers up to 15 are exact there too),
+ * with the codes themselves; the zero point times the sum of the group's x, a product with ones, goes off the group's sum.
+ * fp32 rows are cut into three bf16 pieces, which sum to the row exactly: three products into the same sums. Sums of codes
+ * are a few times as large as sums of code − zero, which costs about a bit and a half of the 32-bit sums: fp32 rows
+ * come within 3e-7 of the exact result (relative, 2-norm), as fp32 multiplication does. Where a unit's sums of x are not
+ * finite the unit is multiplied again with code − zero, as an infinity would meet itself. Operand rows past M repeat the
+ * last row and are not stored.
+ *
+ * ONE: a single fp32 row, which each wave cuts through its part of the LDS, two values a lane; otherwise all 16 lanes of
+ * an operand column group would cut the same values.
+ *
+ * What a unit needs from memory (a record of 1 KB per 16 columns, its scales, 128 values of each row) is requested while
+ * the unit before is multiplied; rows that end inside a unit or are not 16-byte aligned are read by the element. */
+template <int DT, int GROUP, bool ZP, int WV, int NT, bool ONE>
 __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
 {
     typedef typename Elem<DT>::type E;
-    constexpr int GPU = 128 / GROUP, NP = DT == T_F32 ? 3 : 1;
-    __shared__ float part[WV][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int m0 = 16 * blockIdx.y, rows = imin(16, a.M - m0), tile = blockIdx.x;
+    constexpr int GPU = 128 / GROUP, NP = DT == T_F32 ? 3 : 1, XL = DT == T_F32 ? 2 : 1;
+    __shared__ float part[WV][256 * NT];
+    __shared__ __align__(16) uint16_t cut[ONE ? WV : 1][ONE ? 3 * 128 : 8];   /* ONE: a unit's pieces, by wave */
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int m0 = 16 * blockIdx.y, rows = imin(16, a.M - m0), tile0 = blockIdx.x * NT;
+    const int tiles = (a.N + 15) / 16;
     const E *x = static_cast<const E *>(a.x) + (size_t)(m0 + imin(c, rows - 1)) * a.ldx;
-    const bool have = c < rows;
-    f4 total = {0, 0, 0, 0};
-    for (int u = wave; u < a.units; u += WV) {
-        const size_t tu = (size_t)tile * a.units + u;
-        const u4 r = a.rec[tu * 64 + lane];
-        float scale[GPU];
-        h2 bias[GPU];
-        if constexpr (ZP) {
-            const uint32_t *p = static_cast<const uint32_t *>(a.sc) + (tu * 16 + c) * GPU;
+    uint32_t low = 0x000f000fu, magic = 0x64006400u;   /* kept in registers: an instruction takes one constant */
+    asm("" : "+v"(low), "+s"(magic));
+
+    struct Unit {
+        u4 rec[NT], x[ONE ? 1 : 4 * XL];   /* ONE: this lane's two of the row's 128 values, in x[0] */
+        uint32_t sc[NT][GPU];   /* ZP: scale and bias; else the scale's bits */
+    };
+    const int whole = a.vec ? a.K / 128 : 0;   /* units whose rows are read 16 bytes at a time */
+    auto load = [&](Unit &n, int u) __attribute__((always_inline)) {
 #pragma unroll
-            for (int q = 0; q < GPU; q++) {
-                const h2 v = __builtin_bit_cast(h2, p[q]);
-                scale[q] = (float)v[0];
-                bias[q] = h2{v[1], v[1]};
-            }
+        for (int t = 0; t < NT; t++) {
+            const size_t tu = (size_t)imin(tile0 + t, tiles - 1) * a.units + u;
+            n.rec[t] = a.rec[tu * 64 + lane];
+#pragma unroll
+            for (int q = 0; q < GPU; q++)
+                n.sc[t][q] = ZP ? static_cast<const uint32_t *>(a.sc)[(tu * 16 + c) * GPU + q]
+                                : (uint32_t) static_cast<const uint16_t *>(a.sc)[(tu * 16 + c) * GPU + q];
+        }
+        if constexpr (ONE) {
+            const long long k = 128ll * u + 2 * lane;
+            const float *xf = static_cast<const float *>(a.x);
+            n.x[0][0] = k < a.K ? __float_as_uint(xf[k]) : 0u;
+            n.x[0][1] = k + 1 < a.K ? __float_as_uint(xf[k + 1]) : 0u;
+        } else if (u < whole) {
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+#pragma unroll
+                for (int i = 0; i < XL; i++)
+                    n.x[XL * b + i] = *reinterpret_cast<const u4 *>(x + 128 * u + 32 * b + 8 * g + 4 * i);
         } else {
-            const _Float16 *p = static_cast<const _Float16 *>(a.sc) + (tu * 16 + c) * GPU;
 #pragma unroll
-            for (int q = 0; q < GPU; q++) {
-                scale[q] = (float)p[q];
-                bias[q] = h2{(_Float16)-1032.0f, (_Float16)-1032.0f};
+            for (int b = 0; b < 4; b++) {
+                E v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const long long k = 128ll * u + 32 * b + 8 * g + j;
+                    v[j] = k < a.K ? x[k] : Elem<DT>::put(0.0f);
+                }
+                __builtin_memcpy(&n.x[XL * b], v, sizeof v);
             }
         }
-        f4 acc = {0, 0, 0, 0};
+    };
+    f4 total[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) total[t] = f4{0, 0, 0, 0};
+    /* one unit into total; CODES: whether the sums of x that go with it are all finite */
+    auto add = [&](const Unit &n, auto codes) __attribute__((always_inline)) {
+        constexpr bool CODES = decltype(codes)::value;
+        const u4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        if constexpr (ONE) {
+            /* this lane's two values cut as cut3 does, into the wave's LDS: 128 of each piece */
+            uint32_t v[2] = {n.x[0][0], n.x[0][1]};
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+                reinterpret_cast<uint32_t *>(cut[wave])[64 * p + lane] = __builtin_amdgcn_perm(v[1], v[0], 0x07060302u);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float left = __uint_as_float(v[j]) - __uint_as_float(v[j] & 0xffff0000u);
+                    v[j] = !CODES && p == 0 && (v[j] & 0x7fffffffu) == 0x7f800000u ? 0u : __float_as_uint(left);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   /* a wave's LDS operations complete in order */
+            __builtin_amdgcn_wave_barrier();
+        }
+        f4 acc[NT], ones = {0, 0, 0, 0}, every = {0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < NT; t++) acc[t] = f4{0, 0, 0, 0};
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-            const int k = 128 * u + 32 * b + 8 * g;
-            /* this lane's eight values of its row */
+            const bool last = (b + 1) % (GROUP / 32) == 0;   /* of its group */
             u4 xp[NP];
-            if (a.vec && k + 8 <= a.K) {
-                if constexpr (DT == T_F32) {
-                    const u4 v0 = *reinterpret_cast<const u4 *>(x + k), v1 = *reinterpret_cast<const u4 *>(x + k + 4);
-                    uint32_t v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+            if constexpr (ONE)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = have ? v[j] : 0u;
-                    cut3(v, xp);
-                } else {
-                    const u4 v = *reinterpret_cast<const u4 *>(x + k);
-                    xp[0] = have ? v : u4{0, 0, 0, 0};
-                }
-            } else {
-                float v[8];
+                for (int p = 0; p < 3; p++) xp[p] = *reinterpret_cast<const u4 *>(cut[wave] + 128 * p + 32 * b + 8 * g);
+            else if constexpr (DT == T_F32) cut3<!CODES>(n.x[2 * b], n.x[2 * b + 1], xp);
+            else xp[0] = n.x[b];
+            if constexpr (CODES)
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = have && k + j < a.K ? Elem<DT>::get(x[k + j]) : 0.0f;
-                if constexpr (DT == T_F32) {
-                    uint32_t w[8];
+                for (int p = 0; p < NP; p++) ones = mfma16<T_BF16>(xp[p], one, ones);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) w[j] = __float_as_uint(v[j]);
-                    cut3(w, xp);
-                } else {
-                    xp[0] = pack<DT>(v);
+            for (int t = 0; t < NT; t++) {
+                const uint32_t s = n.sc[t][b * GPU / 4];
+                const h2 sb = __builtin_bit_cast(h2, s);
+                const _Float16 bias = ZP ? sb[1] : (_Float16)-1032.0f;
+                const u4 wv = q4_operand<DT, CODES>(n.rec[t][b], bias, low, magic);
+#pragma unroll
+                for (int p = 0; p < NP; p++) acc[t] = mfma16<DT == T_F16 ? T_F16 : T_BF16>(xp[p], wv, acc[t]);
+                if (last) {
+                    if constexpr (CODES) acc[t] += ((float)bias + 1024.0f) * ones;
+                    total[t] += (float)sb[0] * acc[t];
+                    acc[t] = f4{0, 0, 0, 0};
                 }
             }
-            u4 wv;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const h2 d = q4_pair(r[b], i, bias[b * GPU / 4]);
-                if constexpr (DT == T_F16) wv[i] = __builtin_bit_cast(uint32_t, d);
-                else   /* fp16 whole numbers → fp32 → their upper halves, which are all there is */
-                    wv[i] = __builtin_amdgcn_perm(__float_as_uint((float)d[1]), __float_as_uint((float)d[0]), 0x07060302u);
-            }
-#pragma unroll
-            for (int p = 0; p < NP; p++) acc = mfma16<DT == T_F16 ? T_F16 : T_BF16>(xp[p], wv, acc);
-            if ((b + 1) % (GROUP / 32) == 0) {
-                total += scale[b * GPU / 4] * acc;
-                acc = f4{0, 0, 0, 0};
+            if (CODES && last) {
+                every += ones;
+                ones = f4{0, 0, 0, 0};
             }
         }
+        const float all = (every[0] + every[1]) + (every[2] + every[3]);
+        return !__any(!(__builtin_fabsf(all) < INFINITY));
+    };
+    auto multiply = [&](const Unit &n) __attribute__((always_inline)) {
+        if constexpr (DT == T_F16) {
+            add(n, std::false_type{});
+        } else {
+            f4 before[NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++) before[t] = total[t];
+            if (!add(n, std::true_type{})) {
+                Unit again = n;   /* as if loaded anew, or the compiler keeps what both have in common in registers */
+#pragma unroll
+                for (int i = 0; i < (int)(sizeof n.x / sizeof n.x[0]); i++) asm volatile("" : "+v"(again.x[i]));
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    asm volatile("" : "+v"(again.rec[t]));
+                    total[t] = before[t];
+                }
+                add(again, std::false_type{});
+            }
+        }
+    };
+    Unit now, next;
+    int u = wave;
+    if (u < a.units) load(now, u);
+    for (; u < a.units; u += WV) {
+        if (u + WV < a.units) load(next, u + WV);
+        multiply(now);
+        now = next;
     }
     /* row 4g + i, column c of this wave's sums */
 #pragma unroll
-    for (int i = 0; i < 4; i++) part[wave][16 * (4 * g + i) + c] = total[i];
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) part[wave][(4 * g + i) * 16 * NT + 16 * t + c] = total[t][i];
     __syncthreads();
-    for (int t = threadIdx.x; t < 16 * rows; t += 64 * WV) {
-        const int n = 16 * tile + (t & 15);
+    for (int t = threadIdx.x; t < 16 * NT * rows; t += 64 * WV) {
+        const int n = 16 * tile0 + t % (16 * NT);
         float s = part[0][t];
 #pragma unroll
         for (int w = 1; w < WV; w++) s += part[w][t];
         if (n < a.N) {
-            E *y = static_cast<E *>(a.y) + (size_t)(m0 + (t >> 4)) * a.ldy + n;
+            E *y = static_cast<E *>(a.y) + (size_t)(m0 + t / (16 * NT)) * a.ldy + n;
             s *= a.alpha;
             if (a.beta != 0.0f) s = __builtin_fmaf(a.beta, Elem<DT>::get(*y), s);
             *y = Elem<DT>::put(s);

@@ -230,16 +230,41 @@ int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int
     a.alpha = alpha; a.beta = beta; a.x = dX; a.y = dY;
     a.rec = (const p2k::u4 *)w->base;
     a.sc = w->base + w->sc_off;
-    const dim3 grid((unsigned)w->tiles, (unsigned)((M + 15) / 16));
+    const unsigned row_blocks = (unsigned)((M + 15) / 16);
     hipStream_t s = stream_of(stream);
     by_type(dtype, [&](auto t) {
         auto launch = [&](auto group, auto zp) {
             constexpr int DT = decltype(t)::value, G = decltype(group)::value;
             constexpr bool Z = decltype(zp)::value != 0;
-            if (w->units > 4 && w->tiles < 2048)
-                hipLaunchKernelGGL((p2k::q4_gemv<DT, G, Z, 16>), grid, dim3(1024), 0, s, a);
-            else
-                hipLaunchKernelGGL((p2k::q4_gemv<DT, G, Z, 4>), grid, dim3(256), 0, s, a);
+            auto go = [&](auto wv, auto nt) {
+                constexpr int WV = decltype(wv)::value, NT = decltype(nt)::value;
+                const dim3 grid((unsigned)((w->tiles + NT - 1) / NT), row_blocks);
+                if constexpr (DT == p2k::T_F32) {
+                    if (M == 1) {
+                        hipLaunchKernelGGL((p2k::q4_gemv<DT, G, Z, WV, NT, true>), grid, dim3(64 * WV), 0, s, a);
+                        return;
+                    }
+                }
+                if constexpr (DT != p2k::T_F32 || WV < 16)
+                    hipLaunchKernelGGL((p2k::q4_gemv<DT, G, Z, WV, NT, false>), grid, dim3(64 * WV), 0, s, a);
+            };
+            /* Wide weights: a wave takes two column tiles with its rows' values (fp16 13 x 8192 x 8192: 12.9 us, one tile
+             * 18.3), four where such workgroups, one a CU, fill their last round (16384 columns: 19.3 against 23.4; 16389
+             * columns, one workgroup more than CUs: 29.6 against 27.8). Narrow ones: more waves on a long K (bf16 1 x 4096
+             * x 1024: 16 waves 4.0 us, 8 waves 4.3, 4 waves 6.3; 1 x 1024 x 1024: 2.5, 2.4, 2.6). fp32 rows from 2 on need
+             * their registers (8 x 4096 x 4096: 8 waves 10.6 us, 16 waves 16.7). */
+            const int fours = (w->tiles + 3) / 4, cus = cu_count();
+            const bool fill = w->tiles >= 3 * cus && 4ll * fours >= 3ll * cus * ((fours + cus - 1) / cus);
+            if constexpr (DT != p2k::T_F32) {
+                if (fill) {
+                    go(ic<8>{}, ic<4>{});
+                    return;
+                }
+            }
+            if (w->tiles >= 2 * cus) go(ic<8>{}, ic<2>{});
+            else if (w->units >= 32 && w->tiles <= cus && (DT != p2k::T_F32 || M == 1)) go(ic<16>{}, ic<1>{});
+            else if (w->units > 4) go(ic<8>{}, ic<1>{});
+            else go(ic<4>{}, ic<1>{});
         };
         auto by_zero = [&](auto group) {
             if (w->zeros) launch(group, ic<1>{});
