@@ -374,14 +374,21 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
             return fail(P2H_E_ARG, "%s: dO overlaps dK or dV", name);
     }
     if (overlap(o, Rows{(const char *)dQ, ldq * es, q_w, q_rows})) return fail(P2H_E_ARG, "%s: dO overlaps dQ", name);
+    if ((q_rows / 16 + (long long)p2k::imin(n_seqs, q_rows) + 1) * heads > INT_MAX)
+        return fail(P2H_E_ARG, "%s: %d rows of %d heads in %d sequences are too many for one call", name, q_rows, heads, n_seqs);
+    if (int rc = ensure_init()) return rc;
     /* The queries of a tile and the query heads a workgroup takes (its kernel says why); at most one tile more per
      * sequence than the rows fill. */
     const int G = heads / kv_heads, hpw = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
-    const bool few = (long long)((q_rows + 127) / 128) * heads < 256;
+    /* Few queries go 16 to a workgroup whose waves share the keys. 16-bit rows: below 64 workgroups of 128 rows (8 heads,
+     * all keys: 375 queries 11.0 us against 12.8, 750 18.1 against 19.2, 1500 39.6 against 31.8). fp32 rows, whose products
+     * take ten times as long: while those do not fill the device (1500 queries 87 us against 202, 4000 445 against 526, 32
+     * heads of 2000 483 against 366), but for short windows only below 128 (window 256, 3000 queries: 85 against 65). */
+    const long long full = (long long)((q_rows + 127) / 128) * heads;
+    const bool few = dtype != P2H_F32 ? full < 64
+                                      : full <= cu_count() && (full < 128 || (long long)window + ahead >= 512);
     const int qb = few ? 16 : dtype == P2H_F32 ? 128 : 128 / hpw, per = few || dtype == P2H_F32 ? 1 : hpw;
     const long long tiles = (long long)(dQStart ? q_rows / qb + p2k::imin(n_seqs, q_rows) : (q_rows + qb - 1) / qb);
-    if (tiles * heads > INT_MAX) return fail(P2H_E_ARG, "%s: %lld tiles of %d heads", name, tiles, heads);
-    if (int rc = ensure_init()) return rc;
     p2k::WinArgs a{};
     a.q_rows = q_rows; a.k_rows = k_rows; a.n_seqs = n_seqs; a.heads = heads; a.kv = kv_heads;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo; a.window = window; a.ahead = ahead; a.sinks = sinks;
@@ -399,16 +406,17 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
     return P2H_OK;
 }
 
-/* how many workgroups share the keys of one sequence and key head */
+/* How many workgroups share the keys of one sequence and key head: one for every 4 blocks (a block for each wave: one
+ * sequence of 2000 bf16 tokens over 8 key heads 9.3 us, 12.3 with 11 blocks each, 22.7 unsplit), as long as all together
+ * are at most two a CU (2 sequences of 131072: 100 us with 32 to 64 parts, 113 with 256; 32 of 8192, 256 groups: 188 us
+ * in 2 parts or unsplit, 199 in 16). */
 static int page_splits(const P2hKvCache *c, int n_seqs, int heads, int max_len, int window, int sinks)
 {
     const int G = heads / c->heads, kb = c->dtype == P2H_F32 ? 16 : 32;
     const long long groups = (long long)n_seqs * c->heads * ((G + 15) / 16);
     const long long keys = p2k::imin(max_len, window) + (long long)p2k::imin(sinks, p2k::imax(max_len - window, 0));
-    const long long most = keys / (8 * kb);   /* at least two blocks for each of a workgroup's four waves */
-    long long n = groups > 0 ? 4ll * 256 / groups : 1;
-    if (n > most) n = most;
-    return n < 1 ? 1 : n > 256 ? 256 : (int)n;
+    const long long n = groups > 0 ? p2k::imin((int)(512 / groups), (int)(keys / (4 * kb))) : 1;
+    return n < 1 ? 1 : (int)n;
 }
 
 static int check_paged(const char *name, const P2hKvCache *cache, int n_seqs, int heads, int max_len)
@@ -466,7 +474,9 @@ int p2h_attention_paged(const P2hKvCache *cache, int n_seqs, int heads, const vo
     hipStream_t s = stream_of(stream);
     by_type_dim(dtype, cache->head_dim, [&](auto t, auto d) {
         constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
-        if (grid >= cu_count()) hipLaunchKernelGGL((p2k::attention_page<DT, DH, 4>), dim3((unsigned)grid), dim3(256), 0, s, a);
+        /* unsplit long sequences in 8 waves (64 of 4096 tokens: 184 us against 187; 16 of 1000: 20.4 against 21.9) */
+        if (splits > 1 || max_len <= 128)
+            hipLaunchKernelGGL((p2k::attention_page<DT, DH, 4>), dim3((unsigned)grid), dim3(256), 0, s, a);
         else hipLaunchKernelGGL((p2k::attention_page<DT, DH, 8>), dim3((unsigned)grid), dim3(512), 0, s, a);
         if (splits > 1)
             hipLaunchKernelGGL((p2k::attention_join<DT, DH>), dim3((unsigned)(n_seqs * heads)),
