@@ -438,27 +438,19 @@ struct RopeArgs {
     const int *pos, *slots;
 };
 
-/* One workgroup per row: 16 bytes of a head per lane, a head's lanes side by side, so that the mean square is a
- * reduction inside a row of lanes. The row's angles are made once, in 64 bits, as turns reduced to an eighth of a circle
- * (float then holds them to 2^-27 of a radian) and their sines and cosines are shared by all heads through LDS. */
-template <int DT, int DH>
-__global__ __launch_bounds__(256) void qk_norm_rope(RopeArgs a)
+/* One workgroup of NTHR threads per row: 16 bytes of a head per lane, a head's lanes side by side, so that the mean square
+ * is a reduction inside a row of lanes. The row's angles are made once, in 64 bits, as turns reduced to an eighth of a
+ * circle (float then holds them to 2^-27 of a radian), and their sines and cosines are shared by all heads through LDS,
+ * while the row's first values are on their way. Bound by memory: 6000 rows of 32 + 8 + 8 bf16 heads, 147 MB, in 33.5 us
+ * (4.4 TB/s, a copy reaches 4.8); loading 4 heads a thread ahead took 35.9, making the angles before the first load 34.6.
+ * Few rows take 1024 threads, all of a row's heads at once (16 rows 3.9 us, 5.7 with 256 threads). */
+template <int DT, int DH, int NTHR>
+__global__ __launch_bounds__(NTHR) void qk_norm_rope(RopeArgs a)
 {
     typedef typename Elem<DT>::type E;
-    constexpr int VE = kPer16<DT>, LPH = DH / VE, HPP = 256 / LPH;   /* lanes per head, heads per pass */
+    constexpr int VE = kPer16<DT>, LPH = DH / VE, HPP = NTHR / LPH;
     __shared__ float2 turn[DH / 2];   /* (cos, sin) */
     const int t = blockIdx.x, hl = threadIdx.x / LPH, l = threadIdx.x % LPH, half = a.rot / 2;
-    if ((int)threadIdx.x < half) {
-        const double turns = (double)a.pos[t] * (double)a.freq[threadIdx.x] * 0.15915494309189533577;
-        const double f = turns - __builtin_rint(turns), qd = __builtin_rint(4.0 * f);
-        const float r = (float)(f - 0.25 * qd);   /* |r| <= 1/8 turn */
-        float s, c;
-        sincospif(2.0f * r, &s, &c);
-        const int q = (int)qd & 3;
-        const float cs = (q & 1) ? s : c, sn = (q & 1) ? c : s;
-        turn[threadIdx.x] = float2{(q == 1 || q == 2) ? -cs : cs, (q & 2) ? -sn : sn};
-    }
-    __syncthreads();
     const E *row = static_cast<const E *>(a.x) + (size_t)t * a.ldx;
     const int n_heads = a.heads + a.kv * (a.slots_in_cache ? 2 : 1);
     long long slot = -1;
@@ -466,8 +458,24 @@ __global__ __launch_bounds__(256) void qk_norm_rope(RopeArgs a)
         slot = a.slots[t];
         if (slot >= a.slots_in_cache) slot = -1;
     }
-    for (int h = hl; h < n_heads; h += HPP) {
-        const u4 raw = *reinterpret_cast<const u4 *>(row + (size_t)h * DH + VE * l);
+    for (int h0 = 0; h0 < n_heads; h0 += HPP) {
+        const int h = h0 + hl;
+        u4 raw = {0, 0, 0, 0};
+        if (h < n_heads) raw = *reinterpret_cast<const u4 *>(row + (size_t)h * DH + VE * l);
+        if (h0 == 0) {
+            if ((int)threadIdx.x < half) {
+                const double turns = (double)a.pos[t] * (double)a.freq[threadIdx.x] * 0.15915494309189533577;
+                const double f = turns - __builtin_rint(turns), qd = __builtin_rint(4.0 * f);
+                const float r = (float)(f - 0.25 * qd);   /* |r| <= 1/8 turn */
+                float s, c;
+                sincospif(2.0f * r, &s, &c);
+                const int q = (int)qd & 3;
+                const float cs = (q & 1) ? s : c, sn = (q & 1) ? c : s;
+                turn[threadIdx.x] = float2{(q == 1 || q == 2) ? -cs : cs, (q & 2) ? -sn : sn};
+            }
+            __syncthreads();
+        }
+        if (h >= n_heads) break;
         u4 res = raw;
         const bool is_q = h < a.heads, is_v = h >= a.heads + a.kv;
         if (!is_v) {   /* the same for all lanes of a head */

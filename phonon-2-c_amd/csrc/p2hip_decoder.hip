@@ -333,8 +333,9 @@ int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, co
     }
     hipStream_t s = stream_of(stream);
     by_type_dim(dtype, head_dim, [&](auto t, auto d) {
-        hipLaunchKernelGGL((p2k::qk_norm_rope<decltype(t)::value, decltype(d)::value>), dim3((unsigned)T), dim3(256), 0, s,
-                           a);
+        constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
+        if (T <= 256) hipLaunchKernelGGL((p2k::qk_norm_rope<DT, DH, 1024>), dim3((unsigned)T), dim3(1024), 0, s, a);
+        else hipLaunchKernelGGL((p2k::qk_norm_rope<DT, DH, 256>), dim3((unsigned)T), dim3(256), 0, s, a);
     });
     HIPCHK(hipGetLastError());
     return P2H_OK;
