@@ -388,7 +388,9 @@ size_t p2h_q4_weight_device_bytes(const P2hQ4Weight *w);
 /* Y [M][N] = alpha · X [M][K] · W + beta · Y for few rows (beta 0 does not read Y): a matrix-vector product per row,
  * the weight read once for every 16 rows. X and Y of type `dtype`, pitches ldx >= K and ldy >= N elements, no alignment
  * beyond the element's (16-byte aligned rows load faster). A row's outputs are the same bits whatever M is. X and Y
- * must not overlap. A group's products are summed before its scale is applied: values of |x| from 2^118 up may overflow. */
+ * must not overlap. A group's products are summed before its scale is applied: values of |x| from 2^118 up may overflow.
+ * fp16 rows sum x · (code − zero); the others sum x · code and x · zero apart, in 32 bits: near a weight of 0 their errors
+ * are those of the two sums. */
 int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int ldx, const P2hQ4Weight *w, float beta,
                 void *dY, int ldy, void *stream);
 
@@ -407,7 +409,7 @@ typedef struct P2hKvCache {
  * (n[2i], n[2i + 1]). Queries go to dQ (pitch ldq). Keys go to dK (pitch ldk) unless it is NULL, and, with a cache, keys
  * and the row's values (as they are) into the row's slot dSlots[row]; a row whose slot lies outside the cache (a padded
  * row: −1) is not put into it. Slots inside it are distinct. The value part of the rows is read only with a cache.
- * dQ and dK may be the very q and k columns of dQKV; no other overlap. */
+ * dQ and dK may be the very q and k columns of dQKV; no other overlap, with the cache neither. */
 int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, const void *dQKV, int ldqkv,
                      const float *dGammaQ, const float *dGammaK, float eps, int rot, int interleaved,
                      const float *dFreq, const int *dPos, void *dQ, int ldq, void *dK, int ldk,
@@ -419,7 +421,7 @@ int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, co
  * query i of Lq stands at p = i + Lk − Lq. Key j is visible to it iff j <= p + ahead and (p − j < window or j <
  * sinks): `window` >= 1 places back, itself included, `ahead` >= 0 places on, and the first `sinks` >= 0 places (1 << 30
  * reaches everything). A query that sees no key gets zeros; rows outside every sequence are left as they were.
- * scale > 0. At most 2^30 rows. O must not overlap the inputs. */
+ * scale > 0. Fewer than 2^30 rows. O must not overlap the inputs. */
 int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const int *dQStart, const int *dKStart,
                          int heads, int kv_heads, int head_dim, const void *dQ, int ldq, const void *dK, int ldk,
                          const void *dV, int ldv, float scale, int window, int ahead, int sinks, void *dO, int ldo,
@@ -431,7 +433,8 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
  * that. Tokens of a page number outside [0, pages) are not seen. The keys of one sequence are split over workgroups
  * where there are few sequences, planned for lengths up to max_len (other lengths are right as well), and a second
  * kernel joins the parts kept in the workspace, p2h_attention_paged_workspace_bytes(...) bytes, 16-byte aligned (0: the
- * call does not split). Without a workspace (NULL) it runs unsplit. Calls sharing a workspace are stream-ordered. */
+ * call does not split). Without a workspace (NULL) it runs unsplit. Calls sharing a workspace are stream-ordered. dO
+ * overlaps nothing the call reads, nor the workspace. */
 size_t p2h_attention_paged_workspace_bytes(const P2hKvCache *cache, int n_seqs, int heads, int max_len, int window,
                                            int sinks);
 int p2h_attention_paged(const P2hKvCache *cache, int n_seqs, int heads, const void *dQ, int ldq, const int *dTable,

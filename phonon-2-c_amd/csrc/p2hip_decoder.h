@@ -256,9 +256,9 @@ template <bool INF> __device__ __forceinline__ void cut3(u4 lo, u4 hi, u4 (&xp)[
  * with the codes themselves; the zero point times the sum of the group's x, a product with ones, goes off the group's sum.
  * fp32 rows are cut into three bf16 pieces, which sum to the row exactly: three products into the same sums. Sums of codes
  * are a few times as large as sums of code − zero, which costs about a bit and a half of the 32-bit sums: fp32 rows
- * come within 3e-7 of the exact result (relative, 2-norm), as fp32 multiplication does. Where a unit's sums of x are not
- * finite the unit is multiplied again with code − zero, as an infinity would meet itself. Operand rows past M repeat the
- * last row and are not stored.
+ * come within 3e-7 of the exact result (relative, 2-norm), as fp32 multiplication does. A row whose sum of x in a unit is
+ * not finite takes that unit's products with code − zero, as an infinity would meet itself; the rows beside it do not
+ * change. Operand rows past M repeat the last row and are not stored.
  *
  * ONE: a single fp32 row, which each wave cuts through its part of the LDS, two values a lane; otherwise all 16 lanes of
  * an operand column group would cut the same values.
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
     f4 total[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) total[t] = f4{0, 0, 0, 0};
-    /* one unit into total; CODES: whether the sums of x that go with it are all finite */
+    /* one unit into total; CODES: the sums of x that go with it, of this lane's rows 4g + i */
     auto add = [&](const Unit &n, auto codes) __attribute__((always_inline)) {
         constexpr bool CODES = decltype(codes)::value;
         const u4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
@@ -374,8 +374,7 @@ __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
                 ones = f4{0, 0, 0, 0};
             }
         }
-        const float all = (every[0] + every[1]) + (every[2] + every[3]);
-        return !__any(!(__builtin_fabsf(all) < INFINITY));
+        return every;
     };
     auto multiply = [&](const Unit &n) __attribute__((always_inline)) {
         if constexpr (DT == T_F16) {
@@ -384,16 +383,25 @@ __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
             f4 before[NT];
 #pragma unroll
             for (int t = 0; t < NT; t++) before[t] = total[t];
-            if (!add(n, std::true_type{})) {
+            const f4 every = add(n, std::true_type{});
+            const float all = (every[0] + every[1]) + (every[2] + every[3]);
+            if (__any(!(__builtin_fabsf(all) < INFINITY))) {
+                f4 by_codes[NT];
                 Unit again = n;   /* as if loaded anew, or the compiler keeps what both have in common in registers */
 #pragma unroll
                 for (int i = 0; i < (int)(sizeof n.x / sizeof n.x[0]); i++) asm volatile("" : "+v"(again.x[i]));
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     asm volatile("" : "+v"(again.rec[t]));
+                    by_codes[t] = total[t];
                     total[t] = before[t];
                 }
                 add(again, std::false_type{});
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (__builtin_fabsf(every[i]) < INFINITY) total[t][i] = by_codes[t][i];
             }
         }
     };
@@ -726,9 +734,9 @@ template <class E, int DH, int KB, int NW> struct BlockLoads {
     }
 };
 
-/* Where the exponentials of a block have a sum above 2^kSlack in some lane, the reference they are taken from is raised to
+/* Where the exponentials of a block have a sum above kSlack in some lane, the reference they are taken from is raised to
  * the largest score so far and they are taken again. It is not raised otherwise, so that most blocks need no maximum and
- * leave O as it is: a weight stays below 2^kSlack, which every type holds, and relative to their sum nothing changes. */
+ * leave O as it is: a weight stays below kSlack, which every type holds, and relative to their sum nothing changes. */
 constexpr float kSlack = 1024.0f;
 
 /* 32 queries of one head in a wave: lane % 32 is the query, 16-bit rows. */
@@ -795,7 +803,7 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
     for (int k = 0; k < 4; k++) u.pw[k] = u4{0, 0, 0, 0};
     u.m = -INFINITY;
     u.l = 0.0f;
-    u.p = iq + w.off;
+    u.p = imin(iq, w.Lq - 1) + w.off;
     u.full0 = imin(w.p0 + sub + 31, w.Lq - 1 + w.off) - a.window + 1;
     u.full1 = imin(w.Lk - 1, w.p0 + sub + a.ahead) - (KB - 1);
     bool odd = false;
@@ -955,7 +963,7 @@ __global__ __launch_bounds__(256, 2) void attention_win_f32(WinArgs a)
     const WinTile w(a, seq, tile, 128, KB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5,
               col = lane & 31;
-    const int iq = w.i0 + 32 * wave + col, p = iq + w.off;
+    const int iq = w.i0 + 32 * wave + col, p = imin(iq, w.Lq - 1) + w.off;
     const int pw0 = w.p0 + 32 * wave, pw1 = imin(pw0 + 31, w.Lq - 1 + w.off);   /* this wave's places */
 
     u4 q[QR];   /* this lane's query: elements 4(2x + h) .. of every 8 */

@@ -99,6 +99,17 @@ int check_cache(const char *name, const P2hKvCache *c)
     return P2H_OK;
 }
 
+/* a cache's keys or values as one row, and whether rows share a byte with either */
+Rows cache_row(const P2hKvCache *c, const void *p)
+{
+    const size_t bytes = (size_t)c->pages * c->heads * c->page * c->head_dim * elem_size(c->dtype);
+    return Rows{(const char *)p, bytes, bytes, bytes ? 1 : 0};
+}
+bool overlap(const Rows &a, const P2hKvCache *c)
+{
+    return overlap(a, cache_row(c, c->K)) || overlap(a, cache_row(c, c->V));
+}
+
 int log2_of(int page)
 {
     int s = 0;
@@ -245,14 +256,14 @@ int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int
                         return;
                     }
                 }
-                if constexpr (DT != p2k::T_F32 || WV < 16)
-                    hipLaunchKernelGGL((p2k::q4_gemv<DT, G, Z, WV, NT, false>), grid, dim3(64 * WV), 0, s, a);
+                hipLaunchKernelGGL((p2k::q4_gemv<DT, G, Z, WV, NT, false>), grid, dim3(64 * WV), 0, s, a);
             };
             /* Wide weights: a wave takes two column tiles with its rows' values (fp16 13 x 8192 x 8192: 12.9 us, one tile
              * 18.3), four where such workgroups, one a CU, fill their last round (16384 columns: 19.3 against 23.4; 16389
              * columns, one workgroup more than CUs: 29.6 against 27.8). Narrow ones: more waves on a long K (bf16 1 x 4096
-             * x 1024: 16 waves 4.0 us, 8 waves 4.3, 4 waves 6.3; 1 x 1024 x 1024: 2.5, 2.4, 2.6). fp32 rows from 2 on need
-             * their registers (8 x 4096 x 4096: 8 waves 10.6 us, 16 waves 16.7). */
+             * x 1024: 16 waves 4.0 us, 8 waves 4.3, 4 waves 6.3; 1 x 1024 x 1024: 2.5, 2.4, 2.6). fp32 rows need
+             * their registers (8 x 4096 x 4096: 8 waves 10.6 us, 16 waves 16.7). The number of rows does not enter: a row
+             * is summed in the same order whatever it is. */
             const int fours = (w->tiles + 3) / 4, cus = cu_count();
             const bool fill = w->tiles >= 3 * cus && 4ll * fours >= 3ll * cus * ((fours + cus - 1) / cus);
             if constexpr (DT != p2k::T_F32) {
@@ -262,7 +273,7 @@ int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int
                 }
             }
             if (w->tiles >= 2 * cus) go(ic<8>{}, ic<2>{});
-            else if (w->units >= 32 && w->tiles <= cus && (DT != p2k::T_F32 || M == 1)) go(ic<16>{}, ic<1>{});
+            else if (w->units >= 32 && w->tiles <= cus) go(ic<DT == p2k::T_F32 ? 8 : 16>{}, ic<1>{});
             else if (w->units > 4) go(ic<8>{}, ic<1>{});
             else go(ic<4>{}, ic<1>{});
         };
@@ -293,6 +304,8 @@ int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, co
     if (!(eps >= 0.0f)) return fail(P2H_E_ARG, "%s: eps = %g", name, (double)eps);
     if (cache) {
         if (int rc = check_cache(name, cache)) return rc;
+        if (overlap(cache_row(cache, cache->K), cache_row(cache, cache->V)))
+            return fail(P2H_E_ARG, "%s: the cache's keys and values overlap", name);
         if (cache->dtype != dtype || cache->heads != kv_heads || cache->head_dim != head_dim)
             return fail(P2H_E_ARG, "%s: the cache holds %d heads of %d, type %d", name, cache->heads, cache->head_dim,
                         cache->dtype);
@@ -320,7 +333,9 @@ int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, co
         if (k_in ? overlap(k, xq) || overlap(k, xv) : overlap(k, x))
             return fail(P2H_E_ARG, "%s: dK overlaps dQKV other than in place", name);
         if (overlap(q, k)) return fail(P2H_E_ARG, "%s: dQ and dK overlap", name);
+        if (cache && overlap(k, cache)) return fail(P2H_E_ARG, "%s: dK overlaps the cache", name);
     }
+    if (cache && (overlap(x, cache) || overlap(q, cache))) return fail(P2H_E_ARG, "%s: dQKV or dQ overlaps the cache", name);
     if (int rc = ensure_init()) return rc;
     p2k::RopeArgs a{};
     a.T = T; a.heads = heads; a.kv = kv_heads; a.rot = rot; a.interleaved = interleaved != 0;
@@ -455,13 +470,17 @@ int p2h_attention_paged(const P2hKvCache *cache, int n_seqs, int heads, const vo
     const size_t es = elem_size(dtype), w = (size_t)heads * cache->head_dim * es;
     if (overlap(Rows{(const char *)dO, ldo * es, w, n_seqs}, Rows{(const char *)dQ, ldq * es, w, n_seqs}))
         return fail(P2H_E_ARG, "%s: dO overlaps dQ", name);
+    const Rows o{(const char *)dO, ldo * es, w, n_seqs};
     int splits = workspace ? page_splits(cache, n_seqs, heads, max_len, window, sinks) : 1;
     if (splits > 1) {
         const size_t need = (size_t)n_seqs * heads * splits * (cache->head_dim + 2) * 4;
         if (workspace_bytes < need || !aligned(workspace, 16))
             return fail(P2H_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", name, workspace_bytes,
                         need);
+        if (overlap(o, Rows{(const char *)workspace, need, need, 1}))
+            return fail(P2H_E_ARG, "%s: dO overlaps the workspace", name);
     }
+    if (overlap(o, cache)) return fail(P2H_E_ARG, "%s: dO overlaps the cache", name);
     const int G = heads / cache->heads, q_groups = (G + 15) / 16;
     const long long grid = (long long)splits * cache->heads * q_groups * n_seqs;
     if (grid > INT_MAX || (long long)n_seqs * heads > INT_MAX)

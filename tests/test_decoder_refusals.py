@@ -128,3 +128,21 @@ def test_empty_calls():
     assert win(qr=0, q=None, o=None) == 0
     assert win(n=0, qs=A, ks=A) == 0
     assert paged(n=0, q=None, o=None) == 0
+
+
+@pytest.mark.parametrize("kw,part", [
+    (dict(x=A + (1 << 20), cache=cache(dK=8 * A, dV=2 * A + 1024), slots=A, q=20 * A), "dQKV or dQ overlaps the cache"),
+    (dict(cache=cache(dK=8 * A, dV=2 * A + 1024), slots=A), "dQKV or dQ overlaps the cache"),
+    (dict(cache=cache(dK=3 * A - 16, dV=8 * A), slots=A), "dK overlaps the cache"),
+    (dict(cache=cache(dK=8 * A, dV=8 * A + 4 * 2 * 16 * 64 * 2 - 16), slots=A), "keys and values overlap")])
+def test_rope_and_its_cache(kw, part):
+    refused(rope(**kw), part)
+
+
+def test_paged_output_apart_from_what_it_reads():
+    c = cache(dK=8 * A, dV=9 * A)
+    size = 4 * 2 * 16 * 64 * 2
+    refused(paged(c, o=8 * A + size - 16), "dO overlaps the cache")
+    refused(paged(c, o=9 * A - 256 * 2 - 16), "dO overlaps the cache")
+    need = P.attention_paged_workspace_bytes(c, 1, 4, 100000)
+    refused(paged(c, n=1, most=100000, window=1 << 30, ws=2 * A - need + 16, wsb=need), "dO overlaps the workspace")

@@ -95,6 +95,52 @@ def test_q4_wide_range_and_non_finite(t):
     D.check(got[3:4, fin], want[3:4, fin], D.q4_bound(t, x3, w, want[3:4], 1.0, K)[:, fin], t)
 
 
+# wide, wider, long and narrow: the forms with two and with four column tiles a wave and with 16 waves
+Q4_FORMS = [(1, 300, 8201, 32, True), (5, 300, 8201, 64, False), (1, 200, 16325, 128, True), (18, 200, 16325, 32, False),
+            (1, 4000, 40, 64, True), (3, 4097, 1030, 128, False), (16, 8200, 24, 32, True)]
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("M,K,N,group,zeros", Q4_FORMS)
+def test_q4_forms(t, M, K, N, group, zeros):
+    rng = rng_of(t, M, K, N, group, "forms")
+    x, wt = D.rows(rng, t, M, K), D.q4_weight(rng, K, N, group, zeros)
+    w, x64 = D.q4_values(*wt, K, N, group), D.to_f64(t, x)
+    for ldx in (K, K + 1):   # the second: rows of no alignment
+        got = D.to_f64(t, D.run_q4(t, x, wt, K, N, group, ldx=ldx))
+        D.check(got, x64 @ w, D.q4_bound(t, x64, w, x64 @ w, 1.0, K), f"{t} {M}x{K}x{N} pitch {ldx}")
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("K,N", ((4200, 48), (300, 8201), (200, 16325), (700, 31)))
+def test_q4_rows_do_not_depend_on_each_other(t, K, N):
+    """A row alone, among others and beside rows with infinities and NaN: the same bits."""
+    rng = rng_of(t, K, N, "apart")
+    x, wt = D.rows(rng, t, 18, K), D.q4_weight(rng, K, N, 64, True)
+    many = D.run_q4(t, x, wt, K, N, 64)
+    odd = x.copy()
+    odd[2, K // 2] = D.to_type(t, [np.inf])[0]
+    odd[9, K - 1] = D.to_type(t, [np.nan])[0]
+    beside = D.run_q4(t, odd, wt, K, N, 64)
+    for m in (0, 3, 15, 17):
+        assert np.array_equal(D.run_q4(t, x[m:m + 1], wt, K, N, 64)[0], many[m]), m
+    for m in set(range(18)) - {2, 9}:
+        assert np.array_equal(beside[m], many[m]), m
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_q4_codes_at_their_zero_point(t):
+    """Weights of 0: bf16 and fp32 rows sum code and zero point apart, each off by what q4_bound counts of its own size."""
+    K, N, group = 700, 32, 128
+    rng = rng_of(t, "zero point")
+    codes, scales, _ = D.q4_weight(rng, K, N, group, False)
+    x = D.rows(rng, t, 4, K)
+    zeros = np.full((6, N // 2), 0x33, np.uint8)
+    got = D.to_f64(t, D.run_q4(t, x, (np.full_like(codes, 0x33), scales, zeros), K, N, group))
+    both = 2 * 3 * np.repeat(scales.astype(np.float64), group, 0)[:K]
+    D.check(got, np.zeros((4, N)), D.q4_bound(t, D.to_f64(t, x), both, np.zeros((4, N)), 1.0, K) + D.HALF[t] * np.abs(got), t)
+
+
 def test_q4_bytes_and_wrap():
     K, N, group = 1024, 256, 128
     rng = rng_of("wrap")
@@ -185,6 +231,24 @@ def test_rope_into_the_cache(t, page):
     assert np.array_equal(plain[0], q) and np.array_equal(plain[1], k)
 
 
+@pytest.mark.parametrize("t", D.TYPES)
+def test_rope_many_rows_as_few(t):
+    """More rows than the form with 1024 threads takes, with a cache: the bits of the same rows in small calls."""
+    T, H, Hk, Dh, rot, page = 300, 6, 2, 64, 32, 32
+    rng, qkv, gq, gk, freq, pos = rope_inputs(t, T, H, Hk, Dh, rot, "many")
+    slots = rng.permutation(10 * page)[:T].astype(np.int32)
+    q, k, kc, vc = run_rope(t, qkv, H, Hk, Dh, gq, gk, 1e-5, rot, True, freq, pos, page, 10, slots)
+    for a in range(0, T, 100):
+        b = a + 100
+        r = run_rope(t, qkv[a:b], H, Hk, Dh, gq, gk, 1e-5, rot, True, freq, pos[a:b], page, 10, slots[a:b])
+        assert np.array_equal(q[a:b], r[0]) and np.array_equal(k[a:b], r[1])
+        at = (slots[a:b] // page, slice(None), slots[a:b] % page)
+        assert np.array_equal(kc[at], r[2][at]) and np.array_equal(vc[at], r[3][at])
+    x = D.to_f64(t, qkv).reshape(T, H + 2 * Hk, Dh)
+    want, size_of = D.norm_rope(x[:, :H], gq, 1e-5, rot, True, freq, pos)
+    D.check(D.to_f64(t, q).reshape(T, H, Dh), want, D.rope_bound(t, want, size_of, Dh), t)
+
+
 @pytest.mark.parametrize("pos", (0, 1, 131071, 2 ** 31 - 1, -5))
 def test_rope_far_positions(pos):
     """The angle is the product in 64 bits: 2^31 radians and more are reduced without loss."""
@@ -259,6 +323,48 @@ def test_window_many_rows(t):
     want, bound = window_want(t, q, k, v, qs, ks, H, Hk, Dh, 0.2, window, ahead, sinks)
     D.check(D.to_f64(t, got[:, :H * Dh]), want, bound, t)
     assert (got[:, H * Dh:].view(np.uint16) == 0xFFFF).all()
+
+
+BIG = [  # rows for the form with 128 of them a workgroup, of 1, 2 and 4 query heads
+    ((513,), 0, 32, 32, 300, 7, 0), ((450, 0, 70), 25, 32, 16, 200, 0, 40), ((600,), -37, 32, 8, 256, 64, 3),
+    ((520, 3), 130, 32, 4, EVERY, 0, 0), ((1100,), 0, 32, 8, EVERY, EVERY, 0), ((65, 513), 0, 36, 6, 1, 0, 1)]
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("Dh", (64, 128))
+@pytest.mark.parametrize("lens,past,H,Hk,window,ahead,sinks", BIG)
+def test_window_forms(t, Dh, lens, past, H, Hk, window, ahead, sinks):
+    q, k, v, qs, ks = window_case(t, lens, past, H, Hk, Dh, "big")
+    got = D.run_window(t, q, k, v, H, Hk, Dh, Dh ** -0.5, window, ahead, sinks, qs, ks)
+    want, bound = window_want(t, q, k, v, qs, ks, H, Hk, Dh, Dh ** -0.5, window, ahead, sinks)
+    D.check(D.to_f64(t, got), want, bound, f"{t} {Dh} {lens}")
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("Dh", (64, 128))
+def test_window_forms_large_scores(t, Dh):
+    """Scores in the hundreds over many blocks: the reference is raised again and again."""
+    H, Hk = 32, 8
+    q, k, v, qs, ks = window_case(t, (530,), 60, H, Hk, Dh, "raise", scale=6.0)
+    k[::50] = D.to_type(t, 0.25 * D.to_f64(t, k[::50]))
+    got = D.run_window(t, q, k, v, H, Hk, Dh, 1.0, 400, 0, 3, qs, ks)
+    want, bound = window_want(t, q, k, v, qs, ks, H, Hk, Dh, 1.0, 400, 0, 3)
+    D.check(D.to_f64(t, got), want, bound, t)
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_window_forms_ignore_what_they_mask(t):
+    H, Hk, Dh, n, window = 32, 16, 128, 600, 64
+    q, k, v, qs, ks = window_case(t, (n,), 0, H, Hk, Dh, "hide")
+    want, bound = window_want(t, q, k, v, qs, ks, H, Hk, Dh, 0.09, window, 0, 0)
+    for what in (np.inf, -np.inf, np.nan):
+        k2, v2 = k.copy(), v.copy()
+        k2[200] = v2[200] = D.to_type(t, np.full(Hk * Dh, what))
+        f = D.to_f64(t, D.run_window(t, q, k2, v2, H, Hk, Dh, 0.09, window, 0, 0, qs, ks))
+        sees = (np.arange(n) >= 200) & (np.arange(n) < 200 + window)
+        D.check(f[~sees], want[~sees], bound[~sees], f"{t} {what}")
+        if what != what:
+            assert np.isnan(f[sees]).all()
 
 
 @pytest.mark.parametrize("t", D.TYPES)
@@ -550,3 +656,34 @@ def test_two_streams_at_once():
             A.step()
             P.sync()
             assert np.array_equal(L.out(s.ptr), A.out())
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_two_graphs_share_a_workspace(t):
+    """Two captured steps with one workspace, replayed in turn on one stream: each as it is alone."""
+    rng = rng_of(t, "shared")
+    H, Hk, Dh, page = 4, 1, 64, 16
+    s, made = P.Stream(), []
+    ws = None
+    for lens in ((900, 40), (1, 1500)):
+        q, kc, vc, table = paged_case(t, lens, H, Hk, page, Dh, "shared")
+        bufs = [D.device(a) for a in (q, kc, vc, table, np.asarray(lens, np.int32))]
+        cache = P.KvCache(t, Hk, Dh, page, kc.shape[0], bufs[1].ptr, bufs[2].ptr)
+        if ws is None:
+            ws = P.Workspace(P.attention_paged_workspace_bytes(cache, 2, H, 1500))
+            assert ws.nbytes > 0
+        do = D.preset(t, (2, H * Dh))
+        with P.Graph(s) as g:
+            P.attention_paged_dev(cache, 2, H, bufs[0].ptr, H * Dh, bufs[3].ptr, table.shape[1], bufs[4].ptr, 1500, 0.1,
+                                  EVERY, 0, do.ptr, H * Dh, ws.ptr, ws.nbytes, s.ptr)
+        alone = D.run_paged(t, q, kc, vc, table, lens, H, 0.1, EVERY, 0, True, 1500)
+        made.append((g, do, alone, bufs))
+    for _ in range(3):
+        for g, do, _, _ in made:
+            do.upload(np.full(do.nbytes, 0xFF, np.uint8))
+        P.sync()
+        for g, _, _, _ in made:
+            g.launch()
+        s.sync()
+        for _, do, alone, _ in made:
+            assert np.array_equal(do.download((2, H * Dh), D.np_type(t)).view(np.uint16), alone.view(np.uint16))
