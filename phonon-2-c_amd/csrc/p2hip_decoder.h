@@ -1085,149 +1085,195 @@ template <int DH> struct FewState {
     }
 };
 
-/* One block of 32 (fp32: 16) keys from global memory into the state of 16 queries: S^T = K·Q^T by 16 × 16 products, K's
- * operand straight from its rows (a lane reads 16 bytes of one key), then O^T += V^T·P^T as in attention_win: 16-bit V
- * passes through the wave's own LDS for its transposing read, fp32 V is read as the operand takes it.
+/* A block of 32 (fp32: 16) keys from k0 on: each 16 of them, t, have their rows at k[t] and v[t], of which have[t] >= 1 can
+ * be read; the rows behind are read as the last of these. `whole`: every query sees every key of the block, and what is
+ * read is those. */
+template <int DT> struct FewPlace {
+    static constexpr int NB = DT == T_F32 ? 1 : 2, KB = 16 * NB;
+    const typename Elem<DT>::type *k[NB], *v[NB];
+    int have[NB], k0;
+    bool whole, there[NB];   /* there: in a page of the cache (in its place page 0 is read) */
+};
+
+/* Its rows in registers: K as the operand takes it (a lane has 16 bytes of one key), V as its rows lie (16-bit), or as the
+ * operand takes it (fp32). */
+template <int DT, int DH> struct FewRows {
+    static constexpr int NB = FewPlace<DT>::NB, EPC = kPer16<DT>, CH = DH / 8, RPL = 64 / CH;
+    u4 k[NB][DH / (4 * EPC)], v[DT == T_F32 ? 1 : 32 / RPL];
+    float vf[4][DT == T_F32 ? DH / 16 : 1];
+    __device__ __forceinline__ void keys(const FewPlace<DT> &p, int ld)
+    {
+        const int g = (threadIdx.x & 63) >> 4, x16 = threadIdx.x & 15;
+#pragma unroll
+        for (int t = 0; t < NB; t++)
+#pragma unroll
+            for (int x = 0; x < DH / (4 * EPC); x++)
+                k[t][x] = *reinterpret_cast<const u4 *>(p.k[t] + (size_t)imin(x16, p.have[t] - 1) * ld + EPC * (4 * x + g));
+    }
+    __device__ __forceinline__ void values(const FewPlace<DT> &p, int ld)
+    {
+        const int lane = threadIdx.x & 63, g = lane >> 4, x16 = lane & 15;
+        if constexpr (DT == T_F32) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int d = 0; d < DH / 16; d++)
+                    vf[i][d] = p.v[0][(size_t)imin(4 * g + i, p.have[0] - 1) * ld + 16 * d + x16];
+        } else {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int r = 0; r < 16 / RPL; r++)
+                    v[t * 16 / RPL + r] = *reinterpret_cast<const u4 *>(
+                        p.v[t] + (size_t)imin(RPL * r + lane / CH, p.have[t] - 1) * ld + 8 * (lane % CH));
+        }
+    }
+};
+
+/* Blocks b, b + step, … below `end` into the state of 16 queries: S^T = K·Q^T by 16 × 16 products, then O^T += V^T·P^T as in
+ * attention_win; 16-bit V passes through the wave's own LDS for its transposing read.
  *
- * Each 16 keys t have their rows at kb[t] and vb[t] with pitches ldk and ldv; rows from have[t] on are read as the last
- * one that is there (have[t] 0: none is read). seen(k) says whether this lane's query sees key k of the block, and kept(k)
- * whether V row k enters the product at all; neither is asked where `whole`. */
-template <int DT, int DH, class Seen, class Kept>
-__device__ __forceinline__ void few_block(FewState<DH> &st, const u4 (&q)[DH / (4 * kPer16<DT>)], float c,
-                                          const typename Elem<DT>::type *const (&kb)[DT == T_F32 ? 1 : 2],
-                                          const typename Elem<DT>::type *const (&vb)[DT == T_F32 ? 1 : 2],
-                                          const int (&have)[DT == T_F32 ? 1 : 2], int ldk, int ldv, bool whole, Seen seen,
-                                          Kept kept, bool clean, bool &odd, uint16_t *Vs)
+ * A wave has nothing else to do while it waits for memory, so what the next block of 16-bit rows needs is requested as soon
+ * as the registers are free: its keys behind the products with this block's, its values once these lie in LDS. fp32 rows
+ * take the matrix unit eight times as long and have no registers left for that. place_of(b, hint(b)) says
+ * where a block lies, from what hint read (a page table's entries) a block earlier. The last block has code of its own, as
+ * the wait for a load that may or may not have been followed by others is a wait for all of them. seen(p, k) says whether this lane's
+ * query sees key k of the block at p, and kept(p, k) whether V row k enters the product at all; neither is asked where
+ * p.whole. CLEAN: infinities and NaN in V are put aside there, which `odd` notes. */
+template <int DT, int DH, bool CLEAN, class Hint, class PlaceOf, class Seen, class Kept>
+__device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / (4 * kPer16<DT>)], float c, int b, int end,
+                                           int step, int ldk, int ldv, Hint hint, PlaceOf place_of, Seen seen, Kept kept,
+                                           bool &odd, uint16_t *Vs)
 {
     constexpr int NT = DH / 16, VP = DH + 16;
     const int lane = threadIdx.x & 63, g = lane >> 4, x16 = lane & 15;
+    if (b >= end) return;
     auto soften = [&](float top) __attribute__((always_inline)) {
         const float mn = fmaxf(st.m, max_quarters(top) * c), mu = mn == -INFINITY ? 0.0f : mn;
         const float fade = exp2_fast(st.m - mu);
         st.m = mn;
         return float2{mu, fade};
     };
-    if constexpr (DT == T_F32) {
-        float v[4][NT];
-        f4 s = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
-        if (have[0] > 0) {
-            u4 k[NT];
-#pragma unroll
-            for (int x = 0; x < NT; x++)
-                k[x] = *reinterpret_cast<const u4 *>(kb[0] + (size_t)imin(x16, have[0] - 1) * ldk + 4 * (4 * x + g));
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int d = 0; d < NT; d++) v[i][d] = vb[0][(size_t)imin(4 * g + i, have[0] - 1) * ldv + 16 * d + x16];
+    FewRows<DT, DH> rows;
+    FewPlace<DT> now, next;
+    auto ahead = hint(b);
+    auto block = [&](auto last) __attribute__((always_inline)) {
+        constexpr bool MORE = !decltype(last)::value;
+        if constexpr (MORE) {
+            next = place_of(b + step, ahead);
+            ahead = hint(imin(b + 2 * step, end - 1));
+        }
+        if constexpr (DT == T_F32) {
+            f4 s = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
 #pragma unroll
             for (int x = 0; x < NT; x++)
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
-                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[x][e]), __uint_as_float(q[x][e]), s, 0, 0, 0);
-                    s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[x][e + 1]), __uint_as_float(q[x][e + 1]), s1,
-                                                              0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(rows.k[0][x][e]), __uint_as_float(q[x][e]), s, 0,
+                                                             0, 0);
+                    s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(rows.k[0][x][e + 1]),
+                                                              __uint_as_float(q[x][e + 1]), s1, 0, 0, 0);
                 }
             s += s1;
-        } else {
+            if (!now.whole) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 4; i++) {
+                    if (!seen(now, 4 * g + i)) s[i] = -INFINITY;
+                    const bool keep = kept(now, 4 * g + i);
 #pragma unroll
-                for (int d = 0; d < NT; d++) v[i][d] = 0.0f;
-        }
-        if (!whole) {
+                    for (int d = 0; d < NT; d++) {
+                        const bool fin = !CLEAN || __builtin_fabsf(rows.vf[i][d]) < INFINITY;
+                        odd |= keep && !fin;
+                        if (!keep || !fin) rows.vf[i][d] = 0.0f;
+                    }
+                }
+            }
+            const float2 mf = soften(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+            float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (!seen(4 * g + i)) s[i] = -INFINITY;
-                const bool keep = kept(4 * g + i);
+                s[i] = exp2_fast(__builtin_fmaf(s[i], c, -mf.x));
+                sum += s[i];
+            }
+            st.l = __builtin_fmaf(st.l, mf.y, sum);
 #pragma unroll
-                for (int d = 0; d < NT; d++) {
-                    const bool fin = !clean || __builtin_fabsf(v[i][d]) < INFINITY;
-                    odd |= keep && !fin;
-                    if (!keep || !fin) v[i][d] = 0.0f;
+            for (int d = 0; d < NT; d++) st.o[d] *= mf.y;
+#pragma unroll
+            for (int i = 0; i < 4; i++)   /* neighbouring products do not wait for each other */
+#pragma unroll
+                for (int d = 0; d < NT; d++)
+                    st.o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.vf[i][d], s[i], st.o[d], 0, 0, 0);
+        } else {
+            constexpr int CH = FewRows<DT, DH>::CH, RPL = FewRows<DT, DH>::RPL;   /* pieces of a row, rows per load */
+            f4 s[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                s[t] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int x = 0; x < DH / 32; x++) s[t] = mfma16<DT>(rows.k[t][x], q[x], s[t]);
+            }
+            if constexpr (MORE) rows.keys(next, ldk);
+            if (!now.whole) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (!seen(now, 16 * t + 4 * g + i)) s[t][i] = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < 32 / RPL; r++) {
+                    if (!kept(now, RPL * r + lane / CH)) rows.v[r] = u4{0, 0, 0, 0};
+                    if (CLEAN && odd_values<DT>(rows.v[r])) {
+                        odd = true;
+                        rows.v[r] = only_finite<DT>(rows.v[r]);
+                    }
                 }
             }
+#pragma unroll
+            for (int r = 0; r < 32 / RPL; r++)
+                *reinterpret_cast<u4 *>(Vs + (RPL * r + lane / CH) * VP + 8 * (lane % CH)) = rows.v[r];
+            if constexpr (MORE) rows.values(next, ldv);
+            const float2 mf = soften(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
+            float sum = 0.0f, w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                w[i] = exp2_fast(__builtin_fmaf(s[i / 4][i % 4], c, -mf.x));
+                sum += w[i];
+            }
+            st.l = __builtin_fmaf(st.l, mf.y, sum);
+            const u4 pw = pack<DT>(w);
+            /* a wave's LDS operations complete in order, and no other wave touches its part; the fences keep the compiler
+             * from moving reads and writes across each other */
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const uint16_t *vp = Vs + (4 * g + (x16 >> 2)) * VP + 4 * (x16 & 3);
+#pragma unroll
+            for (int d = 0; d < NT; d++) {
+                const u2 va = lds_tr(vp + 16 * d), vb2 = lds_tr(vp + 16 * VP + 16 * d);
+                st.o[d] = mfma16<DT>(u4{va[0], va[1], vb2[0], vb2[1]}, pw, st.o[d] * mf.y);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
-        const float2 mf = soften(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            s[i] = exp2_fast(__builtin_fmaf(s[i], c, -mf.x));
-            sum += s[i];
-        }
-        st.l = __builtin_fmaf(st.l, mf.y, sum);
-#pragma unroll
-        for (int d = 0; d < NT; d++) {
-            st.o[d] *= mf.y;
-#pragma unroll
-            for (int i = 0; i < 4; i++) st.o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d], s[i], st.o[d], 0, 0, 0);
+    };
+    if constexpr (DT == T_F32) {
+        for (; b < end; b += step) {
+            now = place_of(b, ahead);
+            ahead = hint(imin(b + step, end - 1));
+            rows.keys(now, ldk);
+            rows.values(now, ldv);
+            block(std::true_type{});
         }
     } else {
-        constexpr int CH = DH / 8, RPL = 64 / CH;   /* 16-byte pieces of a row, rows per load */
-        u4 k[2][DH / 32], v[32 / RPL];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            if (have[t] > 0) {
-#pragma unroll
-                for (int x = 0; x < DH / 32; x++)
-                    k[t][x] = *reinterpret_cast<const u4 *>(kb[t] + (size_t)imin(x16, have[t] - 1) * ldk + 8 * (4 * x + g));
-#pragma unroll
-                for (int r = 0; r < 16 / RPL; r++)
-                    v[t * 16 / RPL + r] = *reinterpret_cast<const u4 *>(
-                        vb[t] + (size_t)imin(RPL * r + lane / CH, have[t] - 1) * ldv + 8 * (lane % CH));
-            } else {
-#pragma unroll
-                for (int x = 0; x < DH / 32; x++) k[t][x] = u4{0, 0, 0, 0};
-#pragma unroll
-                for (int r = 0; r < 16 / RPL; r++) v[t * 16 / RPL + r] = u4{0, 0, 0, 0};
-            }
+        now = place_of(b, ahead);
+        ahead = hint(imin(b + step, end - 1));
+        rows.keys(now, ldk);
+        rows.values(now, ldv);
+        for (; b + step < end; b += step) {
+            block(std::false_type{});
+            now = next;
         }
-        f4 s[2];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            s[t] = f4{0, 0, 0, 0};
-#pragma unroll
-            for (int x = 0; x < DH / 32; x++) s[t] = mfma16<DT>(k[t][x], q[x], s[t]);
-        }
-        if (!whole) {
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (!seen(16 * t + 4 * g + i)) s[t][i] = -INFINITY;
-#pragma unroll
-            for (int r = 0; r < 32 / RPL; r++) {
-                if (!kept(RPL * r + lane / CH)) v[r] = u4{0, 0, 0, 0};
-                if (clean && odd_values<DT>(v[r])) {
-                    odd = true;
-                    v[r] = only_finite<DT>(v[r]);
-                }
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 32 / RPL; r++)
-            *reinterpret_cast<u4 *>(Vs + (RPL * r + lane / CH) * VP + 8 * (lane % CH)) = v[r];
-        const float2 mf = soften(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
-        float sum = 0.0f, w[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            w[i] = exp2_fast(__builtin_fmaf(s[i / 4][i % 4], c, -mf.x));
-            sum += w[i];
-        }
-        st.l = __builtin_fmaf(st.l, mf.y, sum);
-        const u4 pw = pack<DT>(w);
-        /* a wave's LDS operations complete in order, and no other wave touches its part; the fences keep the compiler
-         * from moving reads and writes across each other */
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const uint16_t *vp = Vs + (4 * g + (x16 >> 2)) * VP + 4 * (x16 & 3);
-#pragma unroll
-        for (int d = 0; d < NT; d++) {
-            const u2 va = lds_tr(vp + 16 * d), vb2 = lds_tr(vp + 16 * VP + 16 * d);
-            st.o[d] = mfma16<DT>(u4{va[0], va[1], vb2[0], vb2[1]}, pw, st.o[d] * mf.y);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        block(std::true_type{});
     }
 }
 
@@ -1280,12 +1326,12 @@ template <int DT, int DH, int NW>
 __global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_win_few(WinArgs a)
 {
     typedef typename Elem<DT>::type E;
-    constexpr int NB = DT == T_F32 ? 1 : 2, KB = 16 * NB, EPC = kPer16<DT>;
+    constexpr int NB = FewPlace<DT>::NB, KB = FewPlace<DT>::KB, EPC = kPer16<DT>;
     __shared__ __align__(16) unsigned char lds[few_lds_bytes<DT, DH, NW>()];
     int head, kvh, seq, tile;
     if (!win_tile_of(a, 1, 16, &head, &kvh, &seq, &tile)) return;
     const WinTile w(a, seq, tile, 16, KB);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const int i = imin(w.i0 + (lane & 15), w.Lq - 1), p = i + w.off;
     u4 q[DH / (4 * EPC)];
     {
@@ -1297,24 +1343,26 @@ __global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_win_few(W
     const E *vh = static_cast<const E *>(a.v) + (size_t)w.ka * a.ldv + (size_t)kvh * DH;
     FewState<DH> st;
     bool odd = false;
-    for (int b = wave; b < w.blocks.total; b += NW) {
-        const int k0 = __builtin_amdgcn_readfirstlane(w.blocks.at(b) * KB);
-        const E *kb[NB], *vb[NB];
-        int have[NB];
+    few_blocks<DT, DH, true>(
+        st, q, a.c, wave, w.blocks.total, NW, a.ldk, a.ldv, [](int) { return 0; },
+        [&](int b, int) __attribute__((always_inline)) {
+            FewPlace<DT> p;
+            p.k0 = w.blocks.at(b) * KB;
 #pragma unroll
-        for (int t = 0; t < NB; t++) {
-            have[t] = imax(imin(16, w.Lk - k0 - 16 * t), 0);
-            kb[t] = kh + (size_t)(k0 + 16 * t) * a.ldk;
-            vb[t] = vh + (size_t)(k0 + 16 * t) * a.ldv;
-        }
-        few_block<DT, DH>(
-            st, q, a.c, kb, vb, have, a.ldk, a.ldv, w.all_seen(a, k0, KB, w.p0, w.p1),
-            [&](int k) __attribute__((always_inline)) {
-                return k0 + k < w.Lk && key_visible(k0 + k, p, a.window, a.ahead, a.sinks);
-            },
-            [&](int k) __attribute__((always_inline)) { return k0 + k < w.Lk; }, true, odd,
-            reinterpret_cast<uint16_t *>(lds) + wave * 32 * (DH + 16));
-    }
+            for (int t = 0; t < NB; t++) {
+                const int row = imin(p.k0 + 16 * t, w.Lk - 1);
+                p.have[t] = imin(16, w.Lk - row);
+                p.k[t] = kh + (size_t)row * a.ldk;
+                p.v[t] = vh + (size_t)row * a.ldv;
+            }
+            p.whole = w.all_seen(a, p.k0, KB, w.p0, w.p1);
+            return p;
+        },
+        [&](const FewPlace<DT> &b, int k) __attribute__((always_inline)) {
+            return b.k0 + k < w.Lk && key_visible(b.k0 + k, p, a.window, a.ahead, a.sinks);
+        },
+        [&](const FewPlace<DT> &b, int k) __attribute__((always_inline)) { return b.k0 + k < w.Lk; }, odd,
+        reinterpret_cast<uint16_t *>(lds) + wave * 32 * (DH + 16));
     float *J = reinterpret_cast<float *>(lds);
     few_store<DH, NW>(st, J);
     for (int e = threadIdx.x; e < imin(16, w.Lq - w.i0) * DH; e += 64 * NW) {
@@ -1333,15 +1381,15 @@ template <int DT, int DH, int NW>
 __global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_page(PageArgs a)
 {
     typedef typename Elem<DT>::type E;
-    constexpr int NB = DT == T_F32 ? 1 : 2, KB = 16 * NB, EPC = kPer16<DT>;
+    constexpr int NB = FewPlace<DT>::NB, KB = FewPlace<DT>::KB, EPC = kPer16<DT>;
     __shared__ __align__(16) unsigned char lds[few_lds_bytes<DT, DH, NW>()];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     const int split = blockIdx.x % a.splits, kvh = (blockIdx.x / a.splits) % a.kv;
     const int qg = (blockIdx.x / a.splits / a.kv) % a.q_groups, seq = blockIdx.x / a.splits / a.kv / a.q_groups;
     const int G = a.heads / a.kv, nq = imin(16, G - 16 * qg), head0 = kvh * G + 16 * qg;
 
     const int *row = a.table + (size_t)seq * a.table_ld;
-    const int len = kept_length(a.len[seq], a.table_ld, 1 << a.page_shift);
+    const int len = a.pages ? kept_length(a.len[seq], a.table_ld, 1 << a.page_shift) : 0;
     const int w0 = imax(len - a.window, 0);
     const KeyBlocks blocks = key_blocks(w0, len, a.sinks, KB);
     int b0, b1;
@@ -1358,27 +1406,41 @@ __global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_page(Page
     const int in_page = (1 << a.page_shift) - 1;
     FewState<DH> st;
     bool odd = false;
-    for (int b = b0 + wave; b < b1; b += NW) {
-        const int k0 = __builtin_amdgcn_readfirstlane(blocks.at(b) * KB);
-        const E *kb[NB], *vb[NB];
-        int have[NB];
-        bool whole = true;
+    struct Entries {
+        int e[NB];
+    };
+    auto seen = [&](const FewPlace<DT> &b, int k) __attribute__((always_inline)) {
+        const int key = b.k0 + k;
+        return b.there[NB == 2 ? k >> 4 : 0] && key < len && (key >= w0 || key < a.sinks);
+    };
+    few_blocks<DT, DH, false>(
+        st, q, a.c, b0 + wave, b1, NW, DH, DH,
+        [&](int b) __attribute__((always_inline)) {
+            Entries n;   /* pages hold a multiple of 16 tokens */
 #pragma unroll
-        for (int t = 0; t < NB; t++) {   /* pages hold a multiple of 16 tokens */
-            const int key = k0 + 16 * t;
-            const int page = key < len ? page_of(row, a.table_ld, key, a.page_shift, a.pages) : -1;
-            const size_t at = (size_t)imax(page, 0) * a.kv * page_elems + (size_t)(key & in_page) * DH;
-            have[t] = page >= 0 ? 16 : 0;
-            kb[t] = kc + at;
-            vb[t] = vc + at;
-            whole &= page >= 0 && key + 15 < len && (key >= w0 || key + 15 < a.sinks);
-        }
-        auto seen = [&](int k) __attribute__((always_inline)) {
-            return have[NB == 2 ? k >> 4 : 0] > 0 && k0 + k < len && (k0 + k >= w0 || k0 + k < a.sinks);
-        };
-        few_block<DT, DH>(st, q, a.c, kb, vb, have, DH, DH, whole, seen, seen, false, odd,
-                          reinterpret_cast<uint16_t *>(lds) + wave * 32 * (DH + 16));
-    }
+            for (int t = 0; t < NB; t++) {
+                const int key = blocks.at(b) * KB + 16 * t;
+                n.e[t] = key < len ? page_entry(row, a.table_ld, key, a.page_shift) : -1;
+            }
+            return n;
+        },
+        [&](int b, Entries n) __attribute__((always_inline)) {
+            FewPlace<DT> p;
+            p.k0 = blocks.at(b) * KB;
+            p.whole = true;
+#pragma unroll
+            for (int t = 0; t < NB; t++) {
+                const int key = p.k0 + 16 * t, page = page_in(n.e[t], a.pages);
+                const size_t at = (size_t)imax(page, 0) * a.kv * page_elems + (size_t)(key & in_page) * DH;
+                p.have[t] = 16;
+                p.there[t] = page >= 0;
+                p.k[t] = kc + at;
+                p.v[t] = vc + at;
+                p.whole &= page >= 0 && key + 15 < len && (key >= w0 || key + 15 < a.sinks);
+            }
+            return p;
+        },
+        seen, seen, odd, reinterpret_cast<uint16_t *>(lds) + wave * 32 * (DH + 16));
     float *J = reinterpret_cast<float *>(lds);
     few_store<DH, NW>(st, J);
     for (int e = threadIdx.x; e < nq * DH; e += 64 * NW) {

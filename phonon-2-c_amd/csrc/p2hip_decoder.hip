@@ -397,9 +397,9 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
      * sequence than the rows fill. */
     const int G = heads / kv_heads, hpw = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
     /* Few queries go 16 to a workgroup whose waves share the keys. 16-bit rows: below 64 workgroups of 128 rows (8 heads,
-     * all keys: 375 queries 11.0 us against 12.8, 750 18.1 against 19.2, 1500 39.6 against 31.8). fp32 rows, whose products
-     * take ten times as long: while those do not fill the device (1500 queries 87 us against 202, 4000 445 against 526, 32
-     * heads of 2000 483 against 366), but for short windows only below 128 (window 256, 3000 queries: 85 against 65). */
+     * all keys: 375 queries 12.5 us against 13.0, 750 17.0 against 19.2, 1500 38.7 against 31.7). fp32 rows, whose products
+     * take ten times as long: while those do not fill the device (1500 queries 81 us against 201, 4000 408 against 527, 32
+     * heads of 2000 446 against 365), but for short windows only below 128 (window 256, 3000 queries: 81 against 64). */
     const long long full = (long long)((q_rows + 127) / 128) * heads;
     const bool few = dtype != P2H_F32 ? full < 64
                                       : full <= cu_count() && (full < 128 || (long long)window + ahead >= 512);
@@ -422,17 +422,20 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
     return P2H_OK;
 }
 
-/* How many workgroups share the keys of one sequence and key head: one for every 4 blocks (a block for each wave: one
- * sequence of 2000 bf16 tokens over 8 key heads 9.3 us, 12.3 with 11 blocks each, 22.7 unsplit), as long as all together
- * are at most two a CU (2 sequences of 131072: 100 us with 32 to 64 parts, 113 with 256; 32 of 8192, 256 groups: 188 us
- * in 2 parts or unsplit, 199 in 16). */
+/* How many workgroups share the keys of one sequence and key head. Up to 192 KB of keys and values one: what a CU reads in
+ * the time that the second kernel costs (one bf16 sequence over 8 key heads of 128: 375 tokens 7.3 us against 8.5 split, 500
+ * 8.8 against 8.0, 2000 21.7 against 8.3; 16 fp16 heads of 64: 750 tokens 7.1 against 6.8). Above that one for every 4
+ * blocks, a block for each wave (2000 tokens in parts of 11 blocks a wave: 12.3), as long as all together are at most
+ * two a CU (2 sequences of 131072: 100 us with 32 to 64 parts, 113 with 256; 32 of 8192, 256 groups: 188 us in 2 parts or
+ * unsplit, 199 in 16). */
 static int page_splits(const P2hKvCache *c, int n_seqs, int heads, int max_len, int window, int sinks)
 {
     const int G = heads / c->heads, kb = c->dtype == P2H_F32 ? 16 : 32;
     const long long groups = (long long)n_seqs * c->heads * ((G + 15) / 16);
     const long long keys = p2k::imin(max_len, window) + (long long)p2k::imin(sinks, p2k::imax(max_len - window, 0));
-    const long long n = groups > 0 ? p2k::imin((int)(512 / groups), (int)(keys / (4 * kb))) : 1;
-    return n < 1 ? 1 : (int)n;
+    if (groups == 0 || 2 * keys * c->head_dim * (long long)elem_size(c->dtype) <= 192 << 10) return 1;
+    const int n = p2k::imin((int)(512 / groups), (int)(keys / (4 * kb)));
+    return n < 1 ? 1 : n;
 }
 
 static int check_paged(const char *name, const P2hKvCache *cache, int n_seqs, int heads, int max_len)

@@ -51,15 +51,15 @@ P2_HD void split_range(int total, int splits, int s, int *begin, int *end)
     *end = imin(*begin + per, total);
 }
 
-/* The page of key t of a sequence whose table row has table_ld entries, or −1 where the table has none or a number
- * outside the cache. Reads the table only inside the row. */
-P2_HD int page_of(const int32_t *row, int table_ld, int t, int page_shift, int pages)
+/* The entry for key t in a sequence's table row of table_ld entries, −1 where it has none; reads only inside the row. */
+P2_HD int page_entry(const int32_t *row, int table_ld, int t, int page_shift)
 {
     const int i = t >> page_shift;
-    if (t < 0 || i >= table_ld) return -1;
-    const int e = row[i];
-    return (uint32_t)e < (uint32_t)pages ? e : -1;
+    return t < 0 || i >= table_ld ? -1 : row[i];
 }
+
+/* The page that an entry names, −1 where that lies outside the cache. */
+P2_HD int page_in(int entry, int pages) { return (uint32_t)entry < (uint32_t)pages ? entry : -1; }
 
 /* A sequence's length as the kernels take it. */
 P2_HD int kept_length(int len, int table_ld, int page)

@@ -58,10 +58,10 @@ int main()
     const int want[ld] = {0, 8, -1, -1, -1};
     for (int shift = 4; shift <= 10; shift++)
         for (long long t = -20; t < (8ll << shift); t++) {
-            const int p = page_of(row, ld, (int)t, shift, pages);
+            const int p = page_in(page_entry(row, ld, (int)t, shift), pages);
             CHECK(p == (t >= 0 && (t >> shift) < ld ? want[t >> shift] : -1));
         }
-    CHECK(page_of(row, 0, 0, 4, pages) == -1 && page_of(row, ld, INT_MAX, 4, pages) == -1 && page_of(row, ld, 0, 4, 0) == -1);
+    CHECK(page_entry(row, 0, 0, 4) == -1 && page_entry(row, ld, INT_MAX, 4) == -1 && page_in(0, 0) == -1 && page_in(-1, 0) == -1);
     CHECK(kept_length(-1, 5, 16) == 0 && kept_length(81, 5, 16) == 80 && kept_length(80, 5, 16) == 80);
     CHECK(kept_length(INT_MAX, 1 << 20, 1024) == 1 << 30 && kept_length(7, 0, 16) == 0);
 
