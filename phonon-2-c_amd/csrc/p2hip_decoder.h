@@ -264,27 +264,40 @@ template <bool INF> __device__ __forceinline__ void cut3(u4 lo, u4 hi, u4 (&xp)[
  * an operand column group would cut the same values.
  *
  * What a unit needs from memory (a record of 1 KB per 16 columns, its scales, 128 values of each row) is requested while
- * the unit before is multiplied; rows that end inside a unit or are not 16-byte aligned are read by the element. */
+ * the unit before is multiplied. The rows' values are read along the rows and turned into operands through the wave's LDS:
+ * read as operands, neighbouring lanes would be in different rows, and such a load takes a CU four times as long (fp16 13 x
+ * 8192 x 16389: 28 us, with the waits for the next unit's loads that conditional loads bring; now 21.6). Rows that end
+ * inside a unit or are not 16-byte aligned are read by the element.
+ *
+ * Bound by memory where the weight is large: those 73 MB at 3.4 TB/s (a copy reaches 4.8); 1 x 1024 x 1024 takes 2.5 us, a
+ * launch and a few waits. */
 template <int DT, int GROUP, bool ZP, int WV, int NT, bool ONE>
 __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
 {
     typedef typename Elem<DT>::type E;
-    constexpr int GPU = 128 / GROUP, NP = DT == T_F32 ? 3 : 1, XL = DT == T_F32 ? 2 : 1;
+    constexpr int GPU = 128 / GROUP, NP = DT == T_F32 ? 3 : 1;
+    constexpr int VE = kPer16<DT>, PR = 128 / VE, XL = ONE ? 1 : 16 * PR / 64;   /* 16-byte pieces of a row; a lane's loads */
     __shared__ float part[WV][256 * NT];
-    __shared__ __align__(16) uint16_t cut[ONE ? WV : 1][ONE ? 3 * 128 : 8];   /* ONE: a unit's pieces, by wave */
+    /* by wave, a unit's 128 values: of 16 rows, a row's pieces followed by an empty one, so that 16 rows' pieces lie in
+     * different banks; ONE: of each of the row's three bf16 parts */
+    __shared__ __align__(16) u4 stage[WV][ONE ? 3 * 16 : 16 * (PR + 1)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     const int m0 = 16 * blockIdx.y, rows = imin(16, a.M - m0), tile0 = blockIdx.x * NT;
     const int tiles = (a.N + 15) / 16;
-    const E *x = static_cast<const E *>(a.x) + (size_t)(m0 + imin(c, rows - 1)) * a.ldx;
+    const E *x = static_cast<const E *>(a.x) + (size_t)m0 * a.ldx;
+    uint32_t at[XL];   /* this lane's pieces: 64 lanes read 64 / PR rows' 256 (fp32: 512) bytes */
+#pragma unroll
+    for (int i = 0; i < XL; i++)
+        at[i] = (uint32_t)imin(64 / PR * i + lane / PR, rows - 1) * (uint32_t)a.ldx + VE * (lane % PR);
     uint32_t low = 0x000f000fu, magic = 0x64006400u;   /* kept in registers: an instruction takes one constant */
     asm("" : "+v"(low), "+s"(magic));
 
     struct Unit {
-        u4 rec[NT], x[ONE ? 1 : 4 * XL];   /* ONE: this lane's two of the row's 128 values, in x[0] */
+        u4 rec[NT], x[XL];   /* ONE: this lane's two of the row's 128 values, in x[0] */
         uint32_t sc[NT][GPU];   /* ZP: scale and bias; else the scale's bits */
     };
-    const int whole = a.vec ? a.K / 128 : 0;   /* units whose rows are read 16 bytes at a time */
-    auto load = [&](Unit &n, int u) __attribute__((always_inline)) {
+    const int whole = ONE || a.vec ? a.K / 128 : 0;   /* units whose rows are read 16 bytes (ONE: 8) at a time */
+    auto load = [&](Unit &n, int u, auto all) __attribute__((always_inline)) {   /* all: a whole unit */
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const size_t tu = (size_t)imin(tile0 + t, tiles - 1) * a.units + u;
@@ -297,25 +310,37 @@ __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
         if constexpr (ONE) {
             const long long k = 128ll * u + 2 * lane;
             const float *xf = static_cast<const float *>(a.x);
-            n.x[0][0] = k < a.K ? __float_as_uint(xf[k]) : 0u;
-            n.x[0][1] = k + 1 < a.K ? __float_as_uint(xf[k + 1]) : 0u;
-        } else if (u < whole) {
+            n.x[0][0] = decltype(all)::value || k < a.K ? __float_as_uint(xf[k]) : 0u;
+            n.x[0][1] = decltype(all)::value || k + 1 < a.K ? __float_as_uint(xf[k + 1]) : 0u;
+        } else if constexpr (decltype(all)::value) {
 #pragma unroll
-            for (int b = 0; b < 4; b++)
-#pragma unroll
-                for (int i = 0; i < XL; i++)
-                    n.x[XL * b + i] = *reinterpret_cast<const u4 *>(x + 128 * u + 32 * b + 8 * g + 4 * i);
+            for (int i = 0; i < XL; i++) n.x[i] = *reinterpret_cast<const u4 *>(x + 128 * u + at[i]);
         } else {
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-                E v[8];
+            for (int i = 0; i < XL; i++) {
+                const E *row = x + (size_t)imin(64 / PR * i + lane / PR, rows - 1) * a.ldx;
+                E v[VE];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const long long k = 128ll * u + 32 * b + 8 * g + j;
-                    v[j] = k < a.K ? x[k] : Elem<DT>::put(0.0f);
+                for (int j = 0; j < VE; j++) {
+                    const long long k = 128ll * u + VE * (lane % PR) + j;
+                    v[j] = k < a.K ? row[k] : Elem<DT>::put(0.0f);
                 }
-                __builtin_memcpy(&n.x[XL * b], v, sizeof v);
+                __builtin_memcpy(&n.x[i], v, sizeof v);
             }
+        }
+    };
+    /* a wave's LDS operations complete in order, and no other wave touches its part; the fences keep the compiler from
+     * moving reads and writes across each other */
+    auto settle = [] {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    auto put = [&](const Unit &n) __attribute__((always_inline)) {
+        if constexpr (!ONE) {
+            settle();
+#pragma unroll
+            for (int i = 0; i < XL; i++) stage[wave][(64 / PR * i + lane / PR) * (PR + 1) + lane % PR] = n.x[i];
+            settle();
         }
     };
     f4 total[NT];
@@ -330,15 +355,14 @@ __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
             uint32_t v[2] = {n.x[0][0], n.x[0][1]};
 #pragma unroll
             for (int p = 0; p < 3; p++) {
-                reinterpret_cast<uint32_t *>(cut[wave])[64 * p + lane] = __builtin_amdgcn_perm(v[1], v[0], 0x07060302u);
+                reinterpret_cast<uint32_t *>(stage[wave])[64 * p + lane] = __builtin_amdgcn_perm(v[1], v[0], 0x07060302u);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     const float left = __uint_as_float(v[j]) - __uint_as_float(v[j] & 0xffff0000u);
                     v[j] = !CODES && p == 0 && (v[j] & 0x7fffffffu) == 0x7f800000u ? 0u : __float_as_uint(left);
                 }
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   /* a wave's LDS operations complete in order */
-            __builtin_amdgcn_wave_barrier();
+            settle();
         }
         f4 acc[NT], ones = {0, 0, 0, 0}, every = {0, 0, 0, 0};
 #pragma unroll
@@ -347,11 +371,12 @@ __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
         for (int b = 0; b < 4; b++) {
             const bool last = (b + 1) % (GROUP / 32) == 0;   /* of its group */
             u4 xp[NP];
+            const u4 *mine = stage[wave] + c * (PR + 1) + PR / 4 * b + PR / 16 * g;
             if constexpr (ONE)
 #pragma unroll
-                for (int p = 0; p < 3; p++) xp[p] = *reinterpret_cast<const u4 *>(cut[wave] + 128 * p + 32 * b + 8 * g);
-            else if constexpr (DT == T_F32) cut3<!CODES>(n.x[2 * b], n.x[2 * b + 1], xp);
-            else xp[0] = n.x[b];
+                for (int p = 0; p < NP; p++) xp[p] = stage[wave][16 * p + 4 * b + g];
+            else if constexpr (DT == T_F32) cut3<!CODES>(mine[0], mine[1], xp);
+            else xp[0] = mine[0];
             if constexpr (CODES)
 #pragma unroll
                 for (int p = 0; p < NP; p++) ones = mfma16<T_BF16>(xp[p], one, ones);
@@ -388,8 +413,7 @@ __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
             if (__any(!(__builtin_fabsf(all) < INFINITY))) {
                 f4 by_codes[NT];
                 Unit again = n;   /* as if loaded anew, or the compiler keeps what both have in common in registers */
-#pragma unroll
-                for (int i = 0; i < (int)(sizeof n.x / sizeof n.x[0]); i++) asm volatile("" : "+v"(again.x[i]));
+                if constexpr (ONE) asm volatile("" : "+v"(again.x[0]));
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     asm volatile("" : "+v"(again.rec[t]));
@@ -405,13 +429,21 @@ __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
             }
         }
     };
-    Unit now, next;
+    Unit n, now;
     int u = wave;
-    if (u < a.units) load(now, u);
-    for (; u < a.units; u += WV) {
-        if (u + WV < a.units) load(next, u + WV);
+    if (u < whole) load(n, u, std::true_type{});
+    for (; u < whole; u += WV) {
+        put(n);
+        now = n;
+        __builtin_amdgcn_sched_barrier(0);   /* the next unit's loads leave before this one's products */
+        if (u + WV < whole) load(n, u + WV, std::true_type{});
+        __builtin_amdgcn_sched_barrier(0);
         multiply(now);
-        now = next;
+    }
+    for (; u < a.units; u += WV) {
+        load(n, u, std::false_type{});
+        put(n);
+        multiply(n);
     }
     /* row 4g + i, column c of this wave's sums */
 #pragma unroll

@@ -237,7 +237,7 @@ int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int
     if (int rc = ensure_init()) return rc;
     p2k::Q4Args a{};
     a.M = M; a.N = N; a.K = K; a.units = w->units; a.ldx = ldx; a.ldy = ldy;
-    a.vec = aligned(dX, 16) && ldx * es % 16 == 0;
+    a.vec = aligned(dX, 16) && ldx * es % 16 == 0 && ldx < (1 << 25);   /* 16 rows within 32-bit offsets */
     a.alpha = alpha; a.beta = beta; a.x = dX; a.y = dY;
     a.rec = (const p2k::u4 *)w->base;
     a.sc = w->base + w->sc_off;
@@ -258,24 +258,28 @@ int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int
                 }
                 hipLaunchKernelGGL((p2k::q4_gemv<DT, G, Z, WV, NT, false>), grid, dim3(64 * WV), 0, s, a);
             };
-            /* Wide weights: a wave takes two column tiles with its rows' values (fp16 13 x 8192 x 8192: 12.9 us, one tile
-             * 18.3), four where such workgroups, one a CU, fill their last round (16384 columns: 19.3 against 23.4; 16389
-             * columns, one workgroup more than CUs: 29.6 against 27.8). Narrow ones: more waves on a long K (bf16 1 x 4096
-             * x 1024: 16 waves 4.0 us, 8 waves 4.3, 4 waves 6.3; 1 x 1024 x 1024: 2.5, 2.4, 2.6). fp32 rows need
-             * their registers (8 x 4096 x 4096: 8 waves 10.6 us, 16 waves 16.7). The number of rows does not enter: a row
-             * is summed in the same order whatever it is. */
-            const int fours = (w->tiles + 3) / 4, cus = cu_count();
-            const bool fill = w->tiles >= 3 * cus && 4ll * fours >= 3ll * cus * ((fours + cus - 1) / cus);
-            if constexpr (DT != p2k::T_F32) {
-                if (fill) {
-                    go(ic<8>{}, ic<4>{});
-                    return;
-                }
+            /* How many column tiles a wave takes with its rows' values, NT, and the waves that share a tile's K, WV. NT so
+             * that one workgroup a CU takes them all (fp16 13 x 4096: 768 tiles 8.1 us by threes, 9.9 by twos, 10.6 one by
+             * one; 1024 tiles 9.8 by fours, 12.5 by threes), fp32 rows at most three, for their registers. Of more tiles
+             * two (1025: 12.1 us, 12.5 by threes, 14.8 by fours), several fp32 rows three (9 x 4096, 1025 tiles: 23.0
+             * against 25.7); from eight a CU on four, in workgroups of four waves, as with a short K eight have one unit
+             * each (bf16 16 x 1024, 8000 tiles: 18.3 us against 25.8; fp16 13 x 4096, 2048 tiles: 18.0, 18.4). Sixteen waves
+             * where a long K has few tiles (bf16 1 x 14336, 256 tiles: 10.2 us against 11.7; K of 4096: 4.7, 4.8), but not
+             * for fp32 rows, whose values would not fit. WV, which sets the order of a row's sums, goes by the weight and
+             * the type alone. */
+            const int tiles = w->tiles, cus = cu_count();
+            if constexpr (DT == p2k::T_F32) {
+                if (tiles <= cus) go(ic<8>{}, ic<1>{});
+                else if (tiles <= 2 * cus || (tiles > 3 * cus && M == 1)) go(ic<8>{}, ic<2>{});
+                else go(ic<8>{}, ic<3>{});
+            } else {
+                if (tiles <= cus && w->units >= 64) go(ic<16>{}, ic<1>{});
+                else if (tiles <= cus) go(ic<8>{}, ic<1>{});
+                else if (tiles >= 8 * cus) go(ic<4>{}, ic<4>{});
+                else if (tiles <= 2 * cus || tiles > 4 * cus) go(ic<8>{}, ic<2>{});
+                else if (tiles <= 3 * cus) go(ic<8>{}, ic<3>{});
+                else go(ic<8>{}, ic<4>{});
             }
-            if (w->tiles >= 2 * cus) go(ic<8>{}, ic<2>{});
-            else if (w->units >= 32 && w->tiles <= cus) go(ic<DT == p2k::T_F32 ? 8 : 16>{}, ic<1>{});
-            else if (w->units > 4) go(ic<8>{}, ic<1>{});
-            else go(ic<4>{}, ic<1>{});
         };
         auto by_zero = [&](auto group) {
             if (w->zeros) launch(group, ic<1>{});

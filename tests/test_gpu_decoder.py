@@ -95,9 +95,10 @@ def test_q4_wide_range_and_non_finite(t):
     D.check(got[3:4, fin], want[3:4, fin], D.q4_bound(t, x3, w, want[3:4], 1.0, K)[:, fin], t)
 
 
-# wide, wider, long and narrow: the forms with two and with four column tiles a wave and with 16 waves
+# wide, wider, long and narrow: the forms with one to four column tiles a wave and with 4, 8 and 16 waves
 Q4_FORMS = [(1, 300, 8201, 32, True), (5, 300, 8201, 64, False), (1, 200, 16325, 128, True), (18, 200, 16325, 32, False),
-            (1, 4000, 40, 64, True), (3, 4097, 1030, 128, False), (16, 8200, 24, 32, True)]
+            (1, 4000, 40, 64, True), (3, 4097, 1030, 128, False), (16, 8200, 24, 32, True),
+            (2, 400, 5000, 64, True), (1, 600, 16500, 32, False), (9, 1100, 16500, 128, True), (17, 200, 32773, 128, True)]
 
 
 @pytest.mark.parametrize("t", D.TYPES)
@@ -112,7 +113,7 @@ def test_q4_forms(t, M, K, N, group, zeros):
 
 
 @pytest.mark.parametrize("t", D.TYPES)
-@pytest.mark.parametrize("K,N", ((4200, 48), (300, 8201), (200, 16325), (700, 31)))
+@pytest.mark.parametrize("K,N", ((4200, 48), (300, 8201), (200, 16325), (700, 31), (8500, 20), (1300, 16500)))
 def test_q4_rows_do_not_depend_on_each_other(t, K, N):
     """A row alone, among others and beside rows with infinities and NaN: the same bits."""
     rng = rng_of(t, K, N, "apart")
@@ -126,6 +127,13 @@ def test_q4_rows_do_not_depend_on_each_other(t, K, N):
         assert np.array_equal(D.run_q4(t, x[m:m + 1], wt, K, N, 64)[0], many[m]), m
     for m in set(range(18)) - {2, 9}:
         assert np.array_equal(beside[m], many[m]), m
+
+
+def test_q4_rows_far_apart():
+    M, K, N, group = 2, 300, 40, 64
+    rng = rng_of("far apart")
+    x, wt = D.rows(rng, "f16", M, K), D.q4_weight(rng, K, N, group, True)
+    assert np.array_equal(D.run_q4("f16", x, wt, K, N, group, ldx=1 << 25), D.run_q4("f16", x, wt, K, N, group))
 
 
 @pytest.mark.parametrize("t", D.TYPES)
