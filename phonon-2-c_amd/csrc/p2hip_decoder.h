@@ -962,6 +962,7 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
 #pragma unroll
             for (int d = 0; d < NT; d++) u.o[d] = mfma32<DT>(read_v(va, k2, d), u.pw[k2], u.o[d]);
     }
+    odd = __syncthreads_or(odd);   /* before the stores, as a barrier behind them would wait for them */
     const float l = sum_halves(u.l), inv = l == 0.0f ? 0.0f : 1.0f / l;
     E *row = static_cast<E *>(a.o) + (size_t)(w.qa + imin(iq, w.Lq - 1)) * a.ldo + (size_t)head * DH + 8 * h;
 #pragma unroll
@@ -977,8 +978,10 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
             const auto e1 = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
             if (iq < w.Lq) *reinterpret_cast<u4 *>(row + 32 * d + 8 * k) = u4{e0[0], e1[0], e0[1], e1[1]};
         }
-    /* the barrier in it also puts the stores above before the reads behind it */
-    if (__syncthreads_or(odd)) add_odd_values<DT, DH>(a, w, kvh, head0, a.hpw, 128 / a.hpw, KB);
+    if (odd) {
+        __syncthreads();   /* the stores above are there */
+        add_odd_values<DT, DH>(a, w, kvh, head0, a.hpw, 128 / a.hpw, KB);
+    }
 }
 
 /* attention_win for fp32 rows, multiplied in fp32 throughout: its products take the matrix unit several times as long as
@@ -1081,6 +1084,7 @@ __global__ __launch_bounds__(256, 2) void attention_win_f32(WinArgs a)
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(row[32 * d], s[i], o[d], 0, 0, 0);
         }
     }
+    odd = __syncthreads_or(odd);   /* before the stores, as a barrier behind them would wait for them */
     l = sum_halves(l);
     if (iq < w.Lq) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1090,8 +1094,10 @@ __global__ __launch_bounds__(256, 2) void attention_win_f32(WinArgs a)
 #pragma unroll
             for (int i = 0; i < 16; i++) row[32 * d + 8 * (i / 4) + i % 4] = o[d][i] * inv;
     }
-    /* the barrier in it also puts the stores above before the reads behind it */
-    if (__syncthreads_or(odd)) add_odd_values<DT, DH>(a, w, kvh, head, 1, 128, KB);
+    if (odd) {
+        __syncthreads();   /* the stores above are there */
+        add_odd_values<DT, DH>(a, w, kvh, head, 1, 128, KB);
+    }
 }
 
 /* ── attention of few queries ──────────────────────────────────────────────────────────────────────────────── */
@@ -1127,43 +1133,50 @@ template <int DT> struct FewPlace {
     bool whole, there[NB];   /* there: in a page of the cache (in its place page 0 is read) */
 };
 
-/* Its rows in registers: K as the operand takes it (a lane has 16 bytes of one key), V as its rows lie (16-bit), or as the
- * operand takes it (fp32). */
+/* Its rows in registers, 16 bytes a lane along the rows; fp32 V as its operand takes it: a lane's four neighbouring
+ * dimensions of a key belong to four products. */
 template <int DT, int DH> struct FewRows {
-    static constexpr int NB = FewPlace<DT>::NB, EPC = kPer16<DT>, CH = DH / 8, RPL = 64 / CH;
-    u4 k[NB][DH / (4 * EPC)], v[DT == T_F32 ? 1 : 32 / RPL];
-    float vf[4][DT == T_F32 ? DH / 16 : 1];
+    typedef typename Elem<DT>::type E;
+    static constexpr int NB = FewPlace<DT>::NB, EPC = kPer16<DT>, CH = DH / EPC, RPL = 64 / CH, LD = 16 / RPL;
+    u4 k[NB * LD], v[DT == T_F32 ? 4 * DH / 64 : NB * LD];
+    static __device__ __forceinline__ u4 get(const E *p) { return *reinterpret_cast<const u4 *>(p); }
+    static __device__ __forceinline__ u4 row_piece(const E *base, int have, int ld, int r)
+    {
+        const int lane = threadIdx.x & 63;
+        return get(base + (size_t)imin(RPL * r + lane / CH, have - 1) * ld + EPC * (lane % CH));
+    }
     __device__ __forceinline__ void keys(const FewPlace<DT> &p, int ld)
     {
-        const int g = (threadIdx.x & 63) >> 4, x16 = threadIdx.x & 15;
 #pragma unroll
-        for (int t = 0; t < NB; t++)
-#pragma unroll
-            for (int x = 0; x < DH / (4 * EPC); x++)
-                k[t][x] = *reinterpret_cast<const u4 *>(p.k[t] + (size_t)imin(x16, p.have[t] - 1) * ld + EPC * (4 * x + g));
+        for (int x = 0; x < NB * LD; x++) k[x] = row_piece(p.k[x / LD], p.have[x / LD], ld, x % LD);
     }
     __device__ __forceinline__ void values(const FewPlace<DT> &p, int ld)
     {
-        const int lane = threadIdx.x & 63, g = lane >> 4, x16 = lane & 15;
         if constexpr (DT == T_F32) {
+            const int g = (threadIdx.x & 63) >> 4, x16 = threadIdx.x & 15;
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int d = 0; d < DH / 16; d++)
-                    vf[i][d] = p.v[0][(size_t)imin(4 * g + i, p.have[0] - 1) * ld + 16 * d + x16];
+                for (int d = 0; d < DH / 64; d++)
+                    v[i * (DH / 64) + d] = get(p.v[0] + (size_t)imin(4 * g + i, p.have[0] - 1) * ld + 64 * d + 4 * x16);
         } else {
 #pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int r = 0; r < 16 / RPL; r++)
-                    v[t * 16 / RPL + r] = *reinterpret_cast<const u4 *>(
-                        p.v[t] + (size_t)imin(RPL * r + lane / CH, p.have[t] - 1) * ld + 8 * (lane % CH));
+            for (int x = 0; x < NB * LD; x++) v[x] = row_piece(p.v[x / LD], p.have[x / LD], ld, x % LD);
         }
+    }
+    /* rows as they were read into LDS of that pitch */
+    static __device__ __forceinline__ void put(const u4 *from, E *to, int pitch)
+    {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int x = 0; x < NB * LD; x++)
+            *reinterpret_cast<u4 *>(to + (RPL * x + lane / CH) * pitch + EPC * (lane % CH)) = from[x];
     }
 };
 
 /* Blocks b, b + step, … below `end` into the state of 16 queries: S^T = K·Q^T by 16 × 16 products, then O^T += V^T·P^T as in
- * attention_win; 16-bit V passes through the wave's own LDS for its transposing read.
+ * attention_win; K passes through the wave's own LDS, as an operand's neighbouring lanes are in different rows, and a load
+ * of such a pattern takes a CU four times as long as one along the rows; 16-bit V for its transposing read.
  *
  * A wave has nothing else to do while it waits for memory, so what the next block of 16-bit rows needs is requested as soon
  * as the registers are free: its keys behind the products with this block's, its values once these lie in LDS. fp32 rows
@@ -1175,9 +1188,11 @@ template <int DT, int DH> struct FewRows {
 template <int DT, int DH, bool CLEAN, class Hint, class PlaceOf, class Seen, class Kept>
 __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / (4 * kPer16<DT>)], float c, int b, int end,
                                            int step, int ldk, int ldv, Hint hint, PlaceOf place_of, Seen seen, Kept kept,
-                                           bool &odd, uint16_t *Vs)
+                                           bool &odd, unsigned char *own)
 {
-    constexpr int NT = DH / 16, VP = DH + 16;
+    typedef typename Elem<DT>::type E;
+    typedef FewRows<DT, DH> Rows;
+    constexpr int NT = DH / 16, VP = DH + 16, KP = DH + kPer16<DT>;   /* pitches that keep a read's rows in different banks */
     const int lane = threadIdx.x & 63, g = lane >> 4, x16 = lane & 15;
     if (b >= end) return;
     auto soften = [&](float top) __attribute__((always_inline)) {
@@ -1186,7 +1201,18 @@ __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / 
         st.m = mn;
         return float2{mu, fade};
     };
-    FewRows<DT, DH> rows;
+    /* a wave's LDS operations complete in order, and no other wave touches its part; the fences keep the compiler from
+     * moving reads and writes across each other */
+    auto order = [] {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    E *Ks = reinterpret_cast<E *>(own);
+    uint16_t *Vs = reinterpret_cast<uint16_t *>(own);
+    auto key = [&](int t, int x) __attribute__((always_inline)) {   /* the operand of keys 16t .., pieces 4x .. */
+        return *reinterpret_cast<const u4 *>(Ks + (16 * t + x16) * KP + kPer16<DT> * (4 * x + g));
+    };
+    Rows rows;
     FewPlace<DT> now, next;
     auto ahead = hint(b);
     auto block = [&](auto last) __attribute__((always_inline)) {
@@ -1195,17 +1221,21 @@ __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / 
             next = place_of(b + step, ahead);
             ahead = hint(imin(b + 2 * step, end - 1));
         }
+        Rows::put(rows.k, Ks, KP);
+        order();
         if constexpr (DT == T_F32) {
             f4 s = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
 #pragma unroll
-            for (int x = 0; x < NT; x++)
+            for (int x = 0; x < NT; x++) {
+                const u4 k = key(0, x);
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
-                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(rows.k[0][x][e]), __uint_as_float(q[x][e]), s, 0,
-                                                             0, 0);
-                    s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(rows.k[0][x][e + 1]),
-                                                              __uint_as_float(q[x][e + 1]), s1, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[e]), __uint_as_float(q[x][e]), s, 0, 0, 0);
+                    s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[e + 1]), __uint_as_float(q[x][e + 1]), s1, 0,
+                                                              0, 0);
                 }
+            }
+            order();
             s += s1;
             if (!now.whole) {
 #pragma unroll
@@ -1214,9 +1244,10 @@ __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / 
                     const bool keep = kept(now, 4 * g + i);
 #pragma unroll
                     for (int d = 0; d < NT; d++) {
-                        const bool fin = !CLEAN || __builtin_fabsf(rows.vf[i][d]) < INFINITY;
+                        uint32_t &v = reinterpret_cast<uint32_t *>(&rows.v[i * (DH / 64) + d / 4])[d % 4];
+                        const bool fin = !CLEAN || __builtin_fabsf(__uint_as_float(v)) < INFINITY;
                         odd |= keep && !fin;
-                        if (!keep || !fin) rows.vf[i][d] = 0.0f;
+                        if (!keep || !fin) v = 0u;
                     }
                 }
             }
@@ -1234,16 +1265,18 @@ __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / 
             for (int i = 0; i < 4; i++)   /* neighbouring products do not wait for each other */
 #pragma unroll
                 for (int d = 0; d < NT; d++)
-                    st.o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.vf[i][d], s[i], st.o[d], 0, 0, 0);
+                    st.o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(rows.v[i * (DH / 64) + d / 4][d % 4]), s[i],
+                                                                   st.o[d], 0, 0, 0);
         } else {
-            constexpr int CH = FewRows<DT, DH>::CH, RPL = FewRows<DT, DH>::RPL;   /* pieces of a row, rows per load */
+            constexpr int CH = Rows::CH, RPL = Rows::RPL;   /* pieces of a row, rows per load */
             f4 s[2];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 s[t] = f4{0, 0, 0, 0};
 #pragma unroll
-                for (int x = 0; x < DH / 32; x++) s[t] = mfma16<DT>(rows.k[t][x], q[x], s[t]);
+                for (int x = 0; x < DH / 32; x++) s[t] = mfma16<DT>(key(t, x), q[x], s[t]);
             }
+            order();
             if constexpr (MORE) rows.keys(next, ldk);
             if (!now.whole) {
 #pragma unroll
@@ -1260,9 +1293,7 @@ __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / 
                     }
                 }
             }
-#pragma unroll
-            for (int r = 0; r < 32 / RPL; r++)
-                *reinterpret_cast<u4 *>(Vs + (RPL * r + lane / CH) * VP + 8 * (lane % CH)) = rows.v[r];
+            Rows::put(rows.v, Ks, VP);
             if constexpr (MORE) rows.values(next, ldv);
             const float2 mf = soften(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                                            fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
@@ -1274,18 +1305,14 @@ __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / 
             }
             st.l = __builtin_fmaf(st.l, mf.y, sum);
             const u4 pw = pack<DT>(w);
-            /* a wave's LDS operations complete in order, and no other wave touches its part; the fences keep the compiler
-             * from moving reads and writes across each other */
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            order();
             const uint16_t *vp = Vs + (4 * g + (x16 >> 2)) * VP + 4 * (x16 & 3);
 #pragma unroll
             for (int d = 0; d < NT; d++) {
                 const u2 va = lds_tr(vp + 16 * d), vb2 = lds_tr(vp + 16 * VP + 16 * d);
                 st.o[d] = mfma16<DT>(u4{va[0], va[1], vb2[0], vb2[1]}, pw, st.o[d] * mf.y);
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            order();
         }
     };
     if constexpr (DT == T_F32) {
@@ -1311,16 +1338,17 @@ __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / 
 
 /* the waves' states into LDS as [wave][16 queries][DH + 2], the last two the maximum and the sum, and one output of their
  * join: sums relative to the returned maximum */
-template <int DH, int NW> __device__ __forceinline__ void few_store(FewState<DH> &st, float *J)
+template <int DT, int DH> __device__ __forceinline__ void few_store(FewState<DH> &st, float *J)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const float l = sum_quarters(st.l);
-    __syncthreads();   /* V's part of the LDS is done with */
+    __syncthreads();   /* the waves' own parts are done with */
     float *mine = J + (wave * 16 + (lane & 15)) * (DH + 2);
 #pragma unroll
     for (int d = 0; d < DH / 16; d++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) mine[16 * d + 4 * g + i] = st.o[d][i];
+        for (int i = 0; i < 4; i++)   /* fp32: product d has every fourth of 64 dimensions */
+            mine[DT == T_F32 ? 64 * (d / 4) + 4 * (4 * g + i) + d % 4 : 16 * d + 4 * g + i] = st.o[d][i];
     if (g == 0) {
         mine[DH] = st.m;
         mine[DH + 1] = l;
@@ -1346,9 +1374,11 @@ template <int DH, int NW> __device__ __forceinline__ void few_join(const float *
     *den = e;
 }
 
+/* a wave's own part: 16-bit V, or fp32 K */
+template <int DT, int DH> constexpr int few_own_bytes() { return DT == T_F32 ? 16 * (DH + 4) * 4 : 32 * (DH + 16) * 2; }
 template <int DT, int DH, int NW> constexpr int few_lds_bytes()
 {
-    constexpr int V = DT == T_F32 ? 0 : NW * 32 * (DH + 16) * 2, J = NW * 16 * (DH + 2) * 4;
+    constexpr int V = NW * few_own_bytes<DT, DH>(), J = NW * 16 * (DH + 2) * 4;
     return V > J ? V : J;
 }
 
@@ -1394,16 +1424,20 @@ __global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_win_few(W
             return b.k0 + k < w.Lk && key_visible(b.k0 + k, p, a.window, a.ahead, a.sinks);
         },
         [&](const FewPlace<DT> &b, int k) __attribute__((always_inline)) { return b.k0 + k < w.Lk; }, odd,
-        reinterpret_cast<uint16_t *>(lds) + wave * 32 * (DH + 16));
+        lds + wave * few_own_bytes<DT, DH>());
+    odd = __syncthreads_or(odd);   /* before the stores, as a barrier behind them would wait for them */
     float *J = reinterpret_cast<float *>(lds);
-    few_store<DH, NW>(st, J);
+    few_store<DT, DH>(st, J);
     for (int e = threadIdx.x; e < imin(16, w.Lq - w.i0) * DH; e += 64 * NW) {
         float top, num, den;
         few_join<DH, NW>(J, e / DH, e % DH, &top, &num, &den);
         static_cast<E *>(a.o)[(size_t)(w.qa + w.i0 + e / DH) * a.ldo + (size_t)head * DH + e % DH] =
             Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
     }
-    if (__syncthreads_or(odd)) add_odd_values<DT, DH>(a, w, kvh, head, 1, 16, KB);
+    if (odd) {
+        __syncthreads();   /* the stores above are there */
+        add_odd_values<DT, DH>(a, w, kvh, head, 1, 16, KB);
+    }
 }
 
 /* One workgroup: one sequence, one key head, up to 16 of the query heads that read it, one part of its key blocks, which
@@ -1472,9 +1506,9 @@ __global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_page(Page
             }
             return p;
         },
-        seen, seen, odd, reinterpret_cast<uint16_t *>(lds) + wave * 32 * (DH + 16));
+        seen, seen, odd, lds + wave * few_own_bytes<DT, DH>());
     float *J = reinterpret_cast<float *>(lds);
-    few_store<DH, NW>(st, J);
+    few_store<DT, DH>(st, J);
     for (int e = threadIdx.x; e < nq * DH; e += 64 * NW) {
         const int r = e / DH, d = e % DH;
         float top, num, den;

@@ -401,9 +401,9 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
      * sequence than the rows fill. */
     const int G = heads / kv_heads, hpw = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
     /* Few queries go 16 to a workgroup whose waves share the keys. 16-bit rows: below 64 workgroups of 128 rows (8 heads,
-     * all keys: 375 queries 12.5 us against 13.0, 750 17.0 against 19.2, 1500 38.7 against 31.7). fp32 rows, whose products
-     * take ten times as long: while those do not fill the device (1500 queries 81 us against 201, 4000 408 against 527, 32
-     * heads of 2000 446 against 365), but for short windows only below 128 (window 256, 3000 queries: 81 against 64). */
+     * all keys: 375 queries 9.4 us against 13.0, 750 15.3 against 19.4, 1500 both 31.7). fp32 rows, whose products take ten
+     * times as long: while those do not fill the device (1500 queries 73 us against 203, 4000 362 against 525, 32 heads of
+     * 2000 396 against 366), but for short windows only below 128 (window 256, 3000 queries: 69 against 65). */
     const long long full = (long long)((q_rows + 127) / 128) * heads;
     const bool few = dtype != P2H_F32 ? full < 64
                                       : full <= cu_count() && (full < 128 || (long long)window + ahead >= 512);
@@ -427,8 +427,8 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
 }
 
 /* How many workgroups share the keys of one sequence and key head. Up to 192 KB of keys and values one: what a CU reads in
- * the time that the second kernel costs (one bf16 sequence over 8 key heads of 128: 375 tokens 7.3 us against 8.5 split, 500
- * 8.8 against 8.0, 2000 21.7 against 8.3; 16 fp16 heads of 64: 750 tokens 7.1 against 6.8). Above that one for every 4
+ * about the time that the second kernel costs (one bf16 sequence over 8 key heads of 128: 375 tokens 6.9 us against 8.5
+ * split, 750 9.5 against 8.3, 2000 17.2 against 8.7; 16 fp16 heads of 64: 750 tokens 6.7 us, 1000 7.7 against 7.0). Above that one for every 4
  * blocks, a block for each wave (2000 tokens in parts of 11 blocks a wave: 12.3), as long as all together are at most
  * two a CU (2 sequences of 131072: 100 us with 32 to 64 parts, 113 with 256; 32 of 8192, 256 groups: 188 us in 2 parts or
  * unsplit, 199 in 16). */
