@@ -373,7 +373,8 @@ enum { P2H_F32 = 0, P2H_F16 = 1, P2H_BF16 = 2 };
 /* A device-resident weight [K, N] of 4-bit codes with a scale, and if wanted a zero point, for every `group` (32, 64
  * or 128) of its rows: w[k][n] = (code[k][n] − zero[k / group][n]) · scale[k / group][n], zero 8 where there are no
  * zero points. codes [K][ceil(N / 2)]: column n in the low (n even) or high half of byte n / 2; scales fp16 bits
- * [ceil(K / group)][N]; zeros packed as the codes, [ceil(K / group)][ceil(N / 2)], or NULL. Any K and N >= 1. */
+ * [ceil(K / group)][N]; zeros packed as the codes, [ceil(K / group)][ceil(N / 2)], or NULL. Any K and N >= 1 of up to 2^35
+ * codes, N up to 2^27. */
 typedef struct P2hQ4Weight P2hQ4Weight;
 
 /* From host memory, or from device memory (read during the call only). Synchronous; NULL on failure. */
@@ -390,7 +391,8 @@ size_t p2h_q4_weight_device_bytes(const P2hQ4Weight *w);
  * beyond the element's (16-byte aligned rows load faster). A row's outputs are the same bits whatever M is. X and Y
  * must not overlap. A group's products are summed before its scale is applied: values of |x| from 2^118 up may overflow.
  * fp16 rows sum x · (code − zero); the others sum x · code and x · zero apart, in 32 bits: near a weight of 0 their errors
- * are those of the two sums. */
+ * are those of the two sums. Of an fp32 value two parts of 8 bits each lie 8 and 16 binary places below it; what of them
+ * is under 2^-126 counts as zero, so values below 2^-110 have fewer bits. */
 int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int ldx, const P2hQ4Weight *w, float beta,
                 void *dY, int ldy, void *stream);
 
@@ -409,7 +411,7 @@ typedef struct P2hKvCache {
  * (n[2i], n[2i + 1]). Queries go to dQ (pitch ldq). Keys go to dK (pitch ldk) unless it is NULL, and, with a cache, keys
  * and the row's values (as they are) into the row's slot dSlots[row]; a row whose slot lies outside the cache (a padded
  * row: −1) is not put into it. Slots inside it are distinct. The value part of the rows is read only with a cache.
- * dQ and dK may be the very q and k columns of dQKV; no other overlap, with the cache neither. */
+ * T is below 2^24. dQ and dK may be the very q and k columns of dQKV; no other overlap, with the cache neither. */
 int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, const void *dQKV, int ldqkv,
                      const float *dGammaQ, const float *dGammaK, float eps, int rot, int interleaved,
                      const float *dFreq, const int *dPos, void *dQ, int ldq, void *dK, int ldk,

@@ -29,6 +29,8 @@ struct P2hQ4Weight {
 
 namespace {
 
+constexpr size_t kGridThreads = (size_t)1 << 32;   /* a launch has fewer threads */
+
 inline size_t elem_size(int dtype) { return dtype == P2H_F32 ? 4 : 2; }
 inline bool is_type(int dtype) { return dtype == P2H_F32 || dtype == P2H_F16 || dtype == P2H_BF16; }
 
@@ -163,8 +165,8 @@ static int q4_check(const char *name, const void *codes, const void *scales, int
     if (!codes || !scales || !aligned(scales, 2)) return fail(P2H_E_ARG, "%s: NULL codes or scales, or scales not aligned", name);
     if (K < 1 || N < 1 || K > (1 << 28) || N > (1 << 28)) return fail(P2H_E_ARG, "%s: K = %d, N = %d", name, K, N);
     if (group != 32 && group != 64 && group != 128) return fail(P2H_E_ARG, "%s: group = %d (32, 64 or 128)", name, group);
-    /* one thread per record word, at most 2^31 workgroups of 256 */
-    if ((size_t)((N - 1) / 16 + 1) * ((K - 1) / 128 + 1) >= (size_t)INT_MAX)
+    /* one thread per record word, and at most 512 per two column tiles: a grid has fewer than 2^32 threads */
+    if (N > 1 << 27 || (size_t)((N - 1) / 16 + 1) * ((K - 1) / 128 + 1) * 256 >= kGridThreads)
         return fail(P2H_E_ARG, "%s: K = %d by N = %d is too large", name, K, N);
     return P2H_OK;
 }
@@ -302,7 +304,7 @@ int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, co
 {
     const char *name = "p2h_qk_norm_rope";
     if (int rc = check_heads(name, dtype, heads, kv_heads, head_dim)) return rc;
-    if (T < 0) return fail(P2H_E_ARG, "%s: T = %d", name, T);
+    if (T < 0 || (size_t)T * 256 >= kGridThreads) return fail(P2H_E_ARG, "%s: T = %d (below 2^24)", name, T);
     if (rot < 0 || rot > head_dim || rot % 16 != 0)
         return fail(P2H_E_ARG, "%s: rot = %d (a multiple of 16 up to head_dim = %d)", name, rot, head_dim);
     if (!(eps >= 0.0f)) return fail(P2H_E_ARG, "%s: eps = %g", name, (double)eps);
@@ -394,7 +396,9 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
             return fail(P2H_E_ARG, "%s: dO overlaps dK or dV", name);
     }
     if (overlap(o, Rows{(const char *)dQ, ldq * es, q_w, q_rows})) return fail(P2H_E_ARG, "%s: dO overlaps dQ", name);
-    if ((q_rows / 16 + (long long)p2k::imin(n_seqs, q_rows) + 1) * heads > INT_MAX)
+    /* workgroups of 256 threads for 128 rows of one head, and for at most one tile more of each sequence; few queries are
+     * far from the limit */
+    if ((size_t)(q_rows / 128 + p2k::imin(n_seqs, q_rows) + 1) * heads * 256 >= kGridThreads)
         return fail(P2H_E_ARG, "%s: %d rows of %d heads in %d sequences are too many for one call", name, q_rows, heads, n_seqs);
     if (int rc = ensure_init()) return rc;
     /* The queries of a tile and the query heads a workgroup takes (its kernel says why); at most one tile more per
@@ -490,7 +494,7 @@ int p2h_attention_paged(const P2hKvCache *cache, int n_seqs, int heads, const vo
     if (overlap(o, cache)) return fail(P2H_E_ARG, "%s: dO overlaps the cache", name);
     const int G = heads / cache->heads, q_groups = (G + 15) / 16;
     const long long grid = (long long)splits * cache->heads * q_groups * n_seqs;
-    if (grid > INT_MAX || (long long)n_seqs * heads > INT_MAX)
+    if ((size_t)grid * 512 >= kGridThreads || (size_t)n_seqs * heads * 512 >= kGridThreads)
         return fail(P2H_E_ARG, "%s: %d sequences of %d heads are too many for one call", name, n_seqs, heads);
     if (int rc = ensure_init()) return rc;
     p2k::PageArgs a{};

@@ -146,3 +146,10 @@ def test_paged_output_apart_from_what_it_reads():
     refused(paged(c, o=9 * A - 256 * 2 - 16), "dO overlaps the cache")
     need = P.attention_paged_workspace_bytes(c, 1, 4, 100000)
     refused(paged(c, n=1, most=100000, window=1 << 30, ws=2 * A - need + 16, wsb=need), "dO overlaps the workspace")
+
+
+def test_too_many_for_one_launch():
+    refused(rope(T=1 << 24), "below 2^24")
+    refused(win(qr=1 << 29, kr=1 << 29, heads=8, o=1 << 50, k=1 << 51, v=1 << 52, ldk=256, ldq=1024, ldo=1024), "too many")
+    refused(paged(cache(dK=1 << 50, dV=1 << 51), n=65536, heads=256, q=1 << 45, ldq=16384, o=1 << 47, ldo=16384), "too many")
+    assert not P.hip().p2h_q4_weight_wrap(A, A, None, 1 << 20, 1 << 16, 32) and "too large" in P.last_error()

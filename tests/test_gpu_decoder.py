@@ -129,6 +129,20 @@ def test_q4_rows_do_not_depend_on_each_other(t, K, N):
         assert np.array_equal(beside[m], many[m]), m
 
 
+@pytest.mark.parametrize("M", (1, 5))
+@pytest.mark.parametrize("scale", (2.0 ** -100, 2.0 ** -115, 2.0 ** -125))
+def test_q4_tiny_fp32_rows(M, scale):
+    """Of each value's pieces below the smallest normal number nothing counts: under two of 2^-126 a value, times its code
+    and its zero point."""
+    K, N, group = 300, 40, 64
+    rng = rng_of("tiny", M)
+    x, wt = D.rows(rng, "f32", M, K, scale=scale), D.q4_weight(rng, K, N, group, True)
+    w, x64 = D.q4_values(*wt, K, N, group), D.to_f64("f32", x)
+    lost = 2 * 2.0 ** -126 * 30 * np.repeat(wt[1].astype(np.float64), group, 0)[:K].sum(0)
+    got = D.run_q4("f32", x, wt, K, N, group).astype(np.float64)
+    D.check(got, x64 @ w, D.q4_bound("f32", x64, w, x64 @ w, 1.0, K) + lost, str(scale))
+
+
 def test_q4_rows_far_apart():
     M, K, N, group = 2, 300, 40, 64
     rng = rng_of("far apart")
@@ -509,6 +523,51 @@ def test_paged_equals_window():
     b = D.run_window(t, q, k, v, H, Hk, Dh, 0.1, 100, 0, 4)
     _, bound = paged_want(t, q, kc, vc, table, (n,), H, 0.1, 100, 4)
     assert (np.abs(a.astype(np.float64) - b) <= 2 * bound).all()
+
+
+# ── offsets beyond 32 bits ──────────────────────────────────────────────────────────────────────────────────────
+
+def test_cache_beyond_32_bits():
+    """A cache of more than 2^32 elements whose last pages are used: written by the rotation, read by the attention."""
+    t, H, Hk, Dh, page, pages, n = "bf16", 8, 8, 128, 1024, 4110, 1500
+    dk, dv = (P.DeviceBuffer(pages * Hk * page * Dh * 2) for _ in range(2))
+    assert pages * Hk * page * Dh > 1 << 32
+    small_k, small_v = (P.DeviceBuffer(2 * Hk * page * Dh * 2) for _ in range(2))
+    big, small = P.KvCache(t, Hk, Dh, page, pages, dk.ptr, dv.ptr), P.KvCache(t, Hk, Dh, page, 2, small_k.ptr, small_v.ptr)
+    _, qkv, gq, gk, freq, pos = rope_inputs(t, n, H, Hk, Dh, Dh, "far pages")
+    dx, dgq, dgk, df, dp = (D.device(a) for a in (qkv, gq, gk, freq, pos))
+    dq, outs = D.preset(t, (n, H * Dh)), []
+    for cache, order in ((big, (pages - 1, pages - 3)), (small, (1, 0))):
+        at = np.arange(n)
+        slots = (np.array(order)[at // page] * page + at % page).astype(np.int32)
+        ds, dt, dl = D.device(slots), D.device(np.array([order], np.int32)), D.device(np.array([n], np.int32))
+        do = D.preset(t, (1, H * Dh))
+        P.qk_norm_rope_dev(t, n, H, Hk, Dh, dx.ptr, 3 * H * Dh, dgq.ptr, dgk.ptr, 1e-6, Dh, False, df.ptr, dp.ptr, dq.ptr,
+                           H * Dh, None, 0, cache, ds.ptr)
+        P.attention_paged_dev(cache, 1, H, dq.ptr, H * Dh, dt.ptr, 2, dl.ptr, n, 0.1, EVERY, 0, do.ptr, H * Dh)
+        outs.append(do.download((1, H * Dh), np.uint16))
+    assert np.isfinite(D.to_f64(t, outs[1])).all() and np.array_equal(*outs)
+
+
+@pytest.mark.parametrize("t,H", (("f16", 1), ("f32", 1), ("f16", 64), ("f32", 64)))
+def test_window_rows_beyond_32_bits(t, H):
+    """Rows so far apart that the last ones lie past 2^31 elements (in both forms): the bits of rows side by side."""
+    n, Dh, ld = 150, 64, (1 << 23) - 64
+    ld = ld if H == 1 else 1 << 22
+    n = n if H == 1 else 530
+    q, k, v, _, _ = window_case(t, (n,), 0, H, H, Dh, "far rows")
+    want = D.run_window(t, q, k, v, H, H, Dh, 0.125, 100, 0, 3)
+    es, first = D.size(t), 400 if H == 1 else 0   # H 1: rows 400 .. of a larger buffer are the sequence
+    bufs = [P.DeviceBuffer(((n + first - 1) * ld + H * Dh) * es) for _ in range(4)]
+    assert (n + first - 1) * ld > 1 << 31
+    for b, a in zip(bufs, (q, k, v)):
+        for r in range(n):
+            b.upload(a[r], offset=(r + first) * ld * es)
+    starts = D.device(np.array([first, first + n], np.int32))
+    P.attention_window_dev(t, n + first, n + first, 1, starts.ptr, starts.ptr, H, H, Dh, bufs[0].ptr, ld, bufs[1].ptr, ld,
+                           bufs[2].ptr, ld, 0.125, 100, 0, 3, bufs[3].ptr, ld)
+    got = np.stack([bufs[3].download((H * Dh,), D.np_type(t), offset=(r + first) * ld * es) for r in range(n)])
+    assert np.array_equal(got, want)
 
 
 # ── together, streams and graphs ────────────────────────────────────────────────────────────────────────────────
