@@ -391,8 +391,8 @@ size_t p2h_q4_weight_device_bytes(const P2hQ4Weight *w);
  * beyond the element's (16-byte aligned rows load faster). A row's outputs are the same bits whatever M is. X and Y
  * must not overlap. A group's products are summed before its scale is applied: values of |x| from 2^118 up may overflow.
  * fp16 rows sum x · (code − zero); the others sum x · code and x · zero apart, in 32 bits: near a weight of 0 their errors
- * are those of the two sums. Of an fp32 value two parts of 8 bits each lie 8 and 16 binary places below it; what of them
- * is under 2^-126 counts as zero, so values below 2^-110 have fewer bits. */
+ * are those of the two sums. Of an fp32 value what lies under 2^-133 counts as zero: below 2^-110 it
+ * has fewer bits. */
 int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int ldx, const P2hQ4Weight *w, float beta,
                 void *dY, int ldy, void *stream);
 

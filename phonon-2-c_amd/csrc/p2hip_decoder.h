@@ -231,7 +231,7 @@ __device__ __forceinline__ u4 q4_operand(uint32_t w, _Float16 bias, uint32_t low
 }
 
 /* Eight fp32 values as three bf16 pieces each, the upper 16 bits of what is left after the pieces before: exact, as 8 + 8
- * + 8 bits hold the 24 of a float (down to 2^-110: the matrix unit takes pieces under 2^-126 as zero). Nothing is left of
+ * + 8 bits hold the 24 of a float (down to 2^-110: bf16 ends at 2^-133). Nothing is left of
  * an infinity where they are looked for (INF), a NaN otherwise. */
 template <bool INF> __device__ __forceinline__ void cut3(u4 lo, u4 hi, u4 (&xp)[3])
 {

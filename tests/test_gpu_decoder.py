@@ -132,13 +132,12 @@ def test_q4_rows_do_not_depend_on_each_other(t, K, N):
 @pytest.mark.parametrize("M", (1, 5))
 @pytest.mark.parametrize("scale", (2.0 ** -100, 2.0 ** -115, 2.0 ** -125))
 def test_q4_tiny_fp32_rows(M, scale):
-    """Of each value's pieces below the smallest normal number nothing counts: under two of 2^-126 a value, times its code
-    and its zero point."""
+    """Three bf16 pieces hold a value down to 2^-133: less than that is lost of each, times its code and its zero point."""
     K, N, group = 300, 40, 64
     rng = rng_of("tiny", M)
     x, wt = D.rows(rng, "f32", M, K, scale=scale), D.q4_weight(rng, K, N, group, True)
     w, x64 = D.q4_values(*wt, K, N, group), D.to_f64("f32", x)
-    lost = 2 * 2.0 ** -126 * 30 * np.repeat(wt[1].astype(np.float64), group, 0)[:K].sum(0)
+    lost = 2.0 ** -133 * 30 * np.repeat(wt[1].astype(np.float64), group, 0)[:K].sum(0)
     got = D.run_q4("f32", x, wt, K, N, group).astype(np.float64)
     D.check(got, x64 @ w, D.q4_bound("f32", x64, w, x64 @ w, 1.0, K) + lost, str(scale))
 
