@@ -578,40 +578,39 @@ struct WinArgs {
     void *o;
 };
 
-/* Which sequence and which of its tiles of `rows` queries tile number `id` is: the sequences' tile counts are summed 64 at
- * a time over the lanes of a wave. False past the last tile. */
-__device__ __forceinline__ bool find_tile(const int *qs, int n_seqs, int q_rows, int rows, int id, int *seq, int *tile)
+/* A sequence's query rows [qa, qb) and key rows [ka, kb), and one of its tiles. */
+struct WinSeq {
+    int qa, qb, ka, kb, tile;
+};
+
+/* The sequence that tile number `id` of `rows` queries falls to and which of its tiles it is: the last sequence whose first
+ * number (tile_start) is not above it, looked for by 64 lanes at once, so that up to 64 sequences take one wait for memory
+ * and 4096 two. False where the sequence has no such tile. */
+__device__ __forceinline__ bool find_tile(const WinArgs &a, int rows, int id, WinSeq *seq)
 {
-    if (!qs) {
-        *seq = 0;
-        *tile = id;
-        return (long long)id * rows < q_rows;
+    if (!a.qs) {
+        *seq = WinSeq{0, a.q_rows, 0, a.k_rows, id};
+        return (long long)id * rows < a.q_rows;
     }
     const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int s0 = 0; s0 < n_seqs; s0 += 64) {
-        int n = 0;
-        if (s0 + lane < n_seqs) {
-            int a, b;
-            seq_rows(qs, s0 + lane, q_rows, &a, &b);
-            n = (b - a + rows - 1) / rows;
-        }
-        int sum = n;   /* of this lane's sequence and those before it */
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const int v = __shfl_up(sum, o);
-            if (lane >= o) sum += v;
-        }
-        const unsigned long long in = __ballot(id < before + sum);
-        if (in) {
-            const int at = __ffsll(in) - 1;
-            *seq = s0 + at;   /* the same in every lane: kept in scalar registers */
-            *tile = id - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(n, at));
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(sum, 63);
+    int lo = 0, hi = a.n_seqs;   /* it is one of these */
+    while (hi - lo > 64) {
+        const int step = (hi - lo + 63) / 64, s = lo + lane * step;
+        const int k = __popcll(__ballot(s < hi && tile_start(a.qs, s, a.q_rows, rows) <= id));
+        lo += imax(k - 1, 0) * step;
+        hi = imin(lo + step, hi);
     }
-    return false;
+    int qa = 0, qb = 0, ka = 0, kb = 0, first = id + 1;
+    if (lo + lane < hi) {
+        seq_rows(a.qs, lo + lane, a.q_rows, &qa, &qb);
+        seq_rows(a.ks, lo + lane, a.k_rows, &ka, &kb);
+        first = tile_start(a.qs, lo + lane, a.q_rows, rows);
+    }
+    const int at = __popcll(__ballot(first <= id)) - 1;
+    if (at < 0) return false;
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };   /* the same in every lane: scalar registers */
+    *seq = WinSeq{of(qa), of(qb), of(ka), of(kb), id - of(first)};
+    return seq->tile >= 0 && seq->tile < (seq->qb - seq->qa + rows - 1) / rows;
 }
 
 /* A sum to which 16 bytes of elements add 0, or a NaN if one of them is an infinity or a NaN: their products with zeros */
@@ -650,14 +649,13 @@ template <int DT> __device__ __forceinline__ u4 only_finite(u4 v)
 struct WinTile {
     int i0, Lq, Lk, off, p0, p1, qa, ka;
     KeyBlocks blocks;
-    __device__ __forceinline__ WinTile(const WinArgs &a, int seq, int tile, int qb, int kb)
+    __device__ __forceinline__ WinTile(const WinArgs &a, const WinSeq &s, int qb, int kb)
     {
-        int q1, k1;
-        seq_rows(a.qs, seq, a.q_rows, &qa, &q1);
-        seq_rows(a.ks, seq, a.k_rows, &ka, &k1);
-        Lq = q1 - qa;
-        Lk = k1 - ka;
-        i0 = tile * qb;
+        qa = s.qa;
+        ka = s.ka;
+        Lq = s.qb - qa;
+        Lk = s.kb - ka;
+        i0 = s.tile * qb;
         off = Lk - Lq;
         p0 = i0 + off;
         p1 = imin(i0 + qb, Lq) - 1 + off;
@@ -704,12 +702,12 @@ __device__ __forceinline__ void add_odd_values(const WinArgs &a, const WinTile &
  * returned. Those of different key heads are next to each other, so that with 8 key heads (or a multiple) each XCD, which
  * takes every eighth workgroup, reads the keys of its own. Later tiles, which see more keys where the window is long,
  * come first. */
-__device__ __forceinline__ bool win_tile_of(const WinArgs &a, int hpw, int qb, int *head, int *kvh, int *seq, int *tile)
+__device__ __forceinline__ bool win_tile_of(const WinArgs &a, int hpw, int qb, int *head, int *kvh, WinSeq *seq)
 {
     const int sets = a.heads / hpw, id = blockIdx.x % sets;
     *kvh = id % a.kv;
     *head = *kvh * (a.heads / a.kv) + id / a.kv * hpw;
-    return find_tile(a.qs, a.n_seqs, a.q_rows, qb, a.tiles - 1 - (int)(blockIdx.x / sets), seq, tile);
+    return find_tile(a, qb, a.tiles - 1 - (int)(blockIdx.x / sets), seq);
 }
 
 /* Where a 16-byte piece cc of row r lies in V's part of the LDS, 16-bit rows of CH pieces: its 64-byte group is moved
@@ -808,9 +806,10 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
     static_assert(2 * Loads::LD == QR, "one load a stage");
     __shared__ __align__(16) E lds[4][KB * DH];   /* K of even and odd blocks, V of even and odd blocks */
 
-    int head0, kvh, seq, tile;
-    if (!win_tile_of(a, a.hpw, 128 / a.hpw, &head0, &kvh, &seq, &tile)) return;
-    const WinTile w(a, seq, tile, 128 / a.hpw, KB);
+    int head0, kvh;
+    WinSeq seq;
+    if (!win_tile_of(a, a.hpw, 128 / a.hpw, &head0, &kvh, &seq)) return;
+    const WinTile w(a, seq, 128 / a.hpw, KB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5,
               col = lane & 31;
     const int head = head0 + wave % a.hpw, sub = 32 * (wave / a.hpw);   /* this wave's head and its first query */
@@ -998,9 +997,10 @@ __global__ __launch_bounds__(256, 2) void attention_win_f32(WinArgs a)
     constexpr int DT = T_F32, KB = 32, CH = DH / 4, QR = DH / 8;
     __shared__ __align__(16) float lds[2][2 * KB * DH];
 
-    int head, kvh, seq, tile;
-    if (!win_tile_of(a, 1, 128, &head, &kvh, &seq, &tile)) return;
-    const WinTile w(a, seq, tile, 128, KB);
+    int head, kvh;
+    WinSeq seq;
+    if (!win_tile_of(a, 1, 128, &head, &kvh, &seq)) return;
+    const WinTile w(a, seq, 128, KB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5,
               col = lane & 31;
     const int iq = w.i0 + 32 * wave + col, p = imin(iq, w.Lq - 1) + w.off;
@@ -1396,9 +1396,10 @@ __global__ __launch_bounds__(64 * NW, DH == 64 ? 4 : 3) void attention_win_few(W
     typedef typename Elem<DT>::type E;
     constexpr int NB = FewPlace<DT>::NB, KB = FewPlace<DT>::KB, EPC = kPer16<DT>;
     __shared__ __align__(16) unsigned char lds[few_lds_bytes<DT, DH, NW>()];
-    int head, kvh, seq, tile;
-    if (!win_tile_of(a, 1, 16, &head, &kvh, &seq, &tile)) return;
-    const WinTile w(a, seq, tile, 16, KB);
+    int head, kvh;
+    WinSeq seq;
+    if (!win_tile_of(a, 1, 16, &head, &kvh, &seq)) return;
+    const WinTile w(a, seq, 16, KB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const int i = imin(w.i0 + (lane & 15), w.Lq - 1), p = i + w.off;
     u4 q[DH / (4 * EPC)];

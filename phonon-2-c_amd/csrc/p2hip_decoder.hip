@@ -396,13 +396,13 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
             return fail(P2H_E_ARG, "%s: dO overlaps dK or dV", name);
     }
     if (overlap(o, Rows{(const char *)dQ, ldq * es, q_w, q_rows})) return fail(P2H_E_ARG, "%s: dO overlaps dQ", name);
-    /* workgroups of 256 threads for 128 rows of one head, and for at most one tile more of each sequence; few queries are
-     * far from the limit */
-    if ((size_t)(q_rows / 128 + p2k::imin(n_seqs, q_rows) + 1) * heads * 256 >= kGridThreads)
+    /* at most 512 threads for 128 rows of one head and for one tile more of each sequence; 16 rows a workgroup, where they
+     * are few, make 2048 of them */
+    if (((size_t)(q_rows / 128 + 1) + n_seqs) * heads + 2048 >= kGridThreads / 512)
         return fail(P2H_E_ARG, "%s: %d rows of %d heads in %d sequences are too many for one call", name, q_rows, heads, n_seqs);
     if (int rc = ensure_init()) return rc;
-    /* The queries of a tile and the query heads a workgroup takes (its kernel says why); at most one tile more per
-     * sequence than the rows fill. */
+    /* The queries of a tile and the query heads a workgroup takes (its kernel says why); one tile more per sequence than
+     * the rows fill (tile_start). */
     const int G = heads / kv_heads, hpw = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
     /* Few queries go 16 to a workgroup whose waves share the keys. 16-bit rows: below 64 workgroups of 128 rows (8 heads,
      * all keys: 375 queries 9.4 us against 13.0, 750 15.3 against 19.4, 1500 both 31.7). fp32 rows, whose products take ten
@@ -412,7 +412,7 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
     const bool few = dtype != P2H_F32 ? full < 64
                                       : full <= cu_count() && (full < 128 || (long long)window + ahead >= 512);
     const int qb = few ? 16 : dtype == P2H_F32 ? 128 : 128 / hpw, per = few || dtype == P2H_F32 ? 1 : hpw;
-    const long long tiles = (long long)(dQStart ? q_rows / qb + p2k::imin(n_seqs, q_rows) : (q_rows + qb - 1) / qb);
+    const long long tiles = (long long)(dQStart ? q_rows / qb + n_seqs : (q_rows + qb - 1) / qb);
     p2k::WinArgs a{};
     a.q_rows = q_rows; a.k_rows = k_rows; a.n_seqs = n_seqs; a.heads = heads; a.kv = kv_heads;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo; a.window = window; a.ahead = ahead; a.sinks = sinks;

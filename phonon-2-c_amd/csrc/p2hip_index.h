@@ -80,4 +80,11 @@ P2_HD void seq_rows(const int32_t *start, int s, int rows, int *a, int *b)
     *b = imin(imax(start[s + 1], *a), rows);
 }
 
+/* The number of sequence s's first tile of `rows` queries, its others following: floors of the rows before it, and one for
+ * every sequence before it, which is never too few. Numbers from tile_start(n) on belong to no sequence. */
+P2_HD int tile_start(const int32_t *start, int s, int rows_in_all, int rows)
+{
+    return imin(imax(start[s], 0), rows_in_all) / rows + s;
+}
+
 }  // namespace p2k

@@ -73,6 +73,21 @@ int main()
             seq_rows(st, s, rows, &a, &b);
             CHECK(a >= 0 && a <= b && b <= rows);
         }
+    /* every tile of every sequence has one number below rows / bs + n, whatever sequences are empty */
+    srand(3);
+    for (int it = 0; it < 3000; it++) {
+        const int n = 1 + rand() % 9, bs = 16 << (rand() % 4);
+        std::vector<int32_t> st(n + 1);
+        st[0] = rand() % 40;
+        for (int s = 0; s < n; s++) st[s + 1] = st[s] + (rand() % 3 ? rand() % (3 * bs) : 0);
+        const int rows = st[n] + rand() % 40;
+        for (int s = 0; s < n; s++) {
+            const int first = tile_start(st.data(), s, rows, bs), next = tile_start(st.data(), s + 1, rows, bs);
+            CHECK(first >= 0 && first < next);
+            CHECK(first + (st[s + 1] - st[s] + bs - 1) / bs <= next);
+            CHECK(first + (st[s + 1] - st[s] + bs - 1) / bs <= rows / bs + n);
+        }
+    }
     int a, b;
     seq_rows(nullptr, 0, 12, &a, &b);
     CHECK(a == 0 && b == 12);

@@ -424,6 +424,20 @@ def test_window_large_scores(t):
     D.check(D.to_f64(t, got), want, bound, t)
 
 
+@pytest.mark.parametrize("t,H", (("f32", 1), ("f16", 1), ("bf16", 16)))
+@pytest.mark.parametrize("n", (64, 65, 200, 4200))
+def test_window_many_sequences(t, H, n):
+    """More sequences than are looked up at once, empty ones among them, in both forms."""
+    Dh = 64
+    rng = rng_of(t, n, "many sequences")
+    lens = rng.integers(0, 6 if n > 1000 else 30, n)
+    qs = np.concatenate(([0], np.cumsum(lens)))
+    q, k, v = (D.rows(rng, t, int(qs[-1]), H * Dh) for _ in range(3))
+    got = D.run_window(t, q, k, v, H, H, Dh, 0.125, EVERY, 0, 0, qs, qs)
+    want, bound = window_want(t, q, k, v, qs, qs, H, H, Dh, 0.125, EVERY, 0, 0)
+    D.check(D.to_f64(t, got), want, bound, f"{t} {n}")
+
+
 def test_window_leaves_rows_outside_the_sequences():
     H, Hk, Dh = 2, 2, 64
     q, k, v, _, _ = window_case("f32", (40,), 0, H, Hk, Dh, "rest")
