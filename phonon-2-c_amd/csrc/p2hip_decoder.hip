@@ -405,11 +405,14 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
      * the rows fill (tile_start). */
     const int G = heads / kv_heads, hpw = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
     /* Few queries go 16 to a workgroup whose waves share the keys. 16-bit rows: below 64 workgroups of 128 rows (8 heads,
-     * all keys: 375 queries 9.4 us against 13.0, 750 15.3 against 19.4, 1500 both 31.7). fp32 rows, whose products take ten
-     * times as long: while those do not fill the device (1500 queries 73 us against 203, 4000 362 against 525, 32 heads of
-     * 2000 396 against 366), but for short windows only below 128 (window 256, 3000 queries: 69 against 65). */
+     * all keys: 375 queries 9.4 us against 13.0, 750 15.3 against 19.4, 1500 both 31.7), and with heads of 64 and long keys,
+     * whose blocks a tile takes one after the other, up to 128 (2000 queries of 8 heads 21.6 us against 30.0, 8000 of 2 57
+     * against 99; 4000 of 8 58 against 54). fp32 rows, whose products take ten times as long: while those do not fill the
+     * device (1500 queries 73 us against 203, 4000 362 against 525, 32 heads of 2000 396 against 366), but for short
+     * windows only below 128 (window 256, 3000 queries: 69 against 65). */
     const long long full = (long long)((q_rows + 127) / 128) * heads;
-    const bool few = dtype != P2H_F32 ? full < 64
+    const bool long_keys = p2k::imin(k_rows / n_seqs, window + p2k::imin(ahead, k_rows)) >= 1000;
+    const bool few = dtype != P2H_F32 ? full < 64 || (head_dim == 64 && full <= 128 && long_keys)
                                       : full <= cu_count() && (full < 128 || (long long)window + ahead >= 512);
     const int qb = few ? 16 : dtype == P2H_F32 ? 128 : 128 / hpw, per = few || dtype == P2H_F32 ? 1 : hpw;
     const long long tiles = (long long)(dQStart ? q_rows / qb + n_seqs : (q_rows + qb - 1) / qb);
