@@ -231,8 +231,8 @@ __device__ __forceinline__ u4 q4_operand(uint32_t w, _Float16 bias, uint32_t low
 }
 
 /* Eight fp32 values as three bf16 pieces each, the upper 16 bits of what is left after the pieces before: exact, as 8 + 8
- * + 8 bits hold the 24 of a float (down to 2^-110: bf16 ends at 2^-133). Nothing is left of
- * an infinity where they are looked for (INF), a NaN otherwise. */
+ * + 8 bits hold the 24 of a float (down to 2^-110: bf16 ends at 2^-133). Nothing is left of an infinity
+ * where they are looked for (INF), a NaN otherwise. */
 template <bool INF> __device__ __forceinline__ void cut3(u4 lo, u4 hi, u4 (&xp)[3])
 {
     uint32_t v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -572,6 +572,7 @@ __global__ __launch_bounds__(NTHR) void qk_norm_rope(RopeArgs a)
 
 struct WinArgs {
     int q_rows, k_rows, n_seqs, heads, kv, ldq, ldk, ldv, ldo, window, ahead, sinks, tiles, hpw;
+    int turn;   /* workgroups from this one on take the tiles from the first on (win_tile_of) */
     float c;   /* scale · log2 e */
     const int *qs, *ks;
     const void *q, *k, *v;
@@ -701,13 +702,16 @@ __device__ __forceinline__ void add_odd_values(const WinArgs &a, const WinTile &
 /* The window kernels' workgroups: a tile of queries of `hpw` query heads that read one key head, the first of them
  * returned. Those of different key heads are next to each other, so that with 8 key heads (or a multiple) each XCD, which
  * takes every eighth workgroup, reads the keys of its own. Later tiles, which see more keys where the window is long,
- * come first. */
+ * come first; the second workgroups of the CUs, where there are no third ones, take the tiles from the other end, so that
+ * each CU has one with many keys and one with few (2000 causal queries of 32 heads of 128: fp32 292 us, 364 in one order;
+ * bf16 49.8, 52.6). */
 __device__ __forceinline__ bool win_tile_of(const WinArgs &a, int hpw, int qb, int *head, int *kvh, WinSeq *seq)
 {
     const int sets = a.heads / hpw, id = blockIdx.x % sets;
     *kvh = id % a.kv;
     *head = *kvh * (a.heads / a.kv) + id / a.kv * hpw;
-    return find_tile(a, qb, a.tiles - 1 - (int)(blockIdx.x / sets), seq);
+    const int b = blockIdx.x;
+    return find_tile(a, qb, b < a.turn ? a.tiles - 1 - b / sets : (b - a.turn) / sets, seq);
 }
 
 /* Where a 16-byte piece cc of row r lies in V's part of the LDS, 16-bit rows of CH pieces: its 64-byte group is moved
@@ -989,7 +993,7 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
 
 /* attention_win for fp32 rows, multiplied in fp32 throughout: its products take the matrix unit several times as long as
  * everything else takes, so nothing is gained by running them together with the exponentials. Blocks of 32 keys, two
- * buffers in turn: while one is multiplied the next is on its way. 2000 causal queries of 32 heads of 128: 366 us, 90
+ * buffers in turn: while one is multiplied the next is on its way. 2000 causal queries of 32 heads of 128: 292 us, 112
  * TFLOP/s (a large fp32 product reaches 153). */
 template <int DH>
 __global__ __launch_bounds__(256, 2) void attention_win_f32(WinArgs a)

@@ -408,7 +408,7 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
      * all keys: 375 queries 9.4 us against 13.0, 750 15.3 against 19.4, 1500 both 31.7), and with heads of 64 and long keys,
      * whose blocks a tile takes one after the other, up to 128 (2000 queries of 8 heads 21.6 us against 30.0, 8000 of 2 57
      * against 99; 4000 of 8 58 against 54). fp32 rows, whose products take ten times as long: while those do not fill the
-     * device (1500 queries 73 us against 203, 4000 362 against 525, 32 heads of 2000 396 against 366), but for short
+     * device (1500 queries 73 us against 203, 4000 362 against 525, 32 heads of 2000 396 against 292), but for short
      * windows only below 128 (window 256, 3000 queries: 69 against 65). */
     const long long full = (long long)((q_rows + 127) / 128) * heads;
     const bool long_keys = p2k::imin(k_rows / n_seqs, window + p2k::imin(ahead, k_rows)) >= 1000;
@@ -422,7 +422,9 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
     a.tiles = (int)tiles; a.hpw = per; a.c = scale * p2k::kLog2e;
     a.qs = dQStart; a.ks = dKStart; a.q = dQ; a.k = dK; a.v = dV; a.o = dO;
     hipStream_t s = stream_of(stream);
-    const dim3 grid((unsigned)(tiles * (heads / per)));
+    const int sets = heads / per, wgs = (int)tiles * sets, cus = cu_count();
+    a.turn = !few && wgs > cus && wgs <= 2 * cus && sets <= cus ? cus / sets * sets : wgs;
+    const dim3 grid((unsigned)wgs);
     by_type_dim(dtype, head_dim, [&](auto t, auto d) {
         constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
         if (few) hipLaunchKernelGGL((p2k::attention_win_few<DT, DH, 8>), grid, dim3(512), 0, s, a);
