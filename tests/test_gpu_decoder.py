@@ -348,7 +348,8 @@ def test_window_many_rows(t):
 
 BIG = [  # rows for the form with 128 of them a workgroup, of 1, 2 and 4 query heads
     ((513,), 0, 32, 32, 300, 7, 0), ((450, 0, 70), 25, 32, 16, 200, 0, 40), ((600,), -37, 32, 8, 256, 64, 3),
-    ((520, 3), 130, 32, 4, EVERY, 0, 0), ((1100,), 0, 32, 8, EVERY, EVERY, 0), ((65, 513), 0, 36, 6, 1, 0, 1)]
+    ((520, 3), 130, 32, 4, EVERY, 0, 0), ((1100,), 0, 32, 8, EVERY, EVERY, 0), ((65, 513), 0, 36, 6, 1, 0, 1),
+    ((700, 5, 400), 9, 32, 8, 300, 0, 2)]
 
 
 @pytest.mark.parametrize("t", D.TYPES)
