@@ -270,8 +270,8 @@ template <bool INF> __device__ __forceinline__ void cut3(u4 lo, u4 hi, u4 (&xp)[
  * 8192 x 16389: 28 us, with the waits for the next unit's loads that conditional loads bring; now 21.6). Rows that end
  * inside a unit or are not 16-byte aligned are read by the element.
  *
- * Bound by memory where the weight is large: those 73 MB at 3.4 TB/s (a copy reaches 4.8); 1 x 1024 x 1024 takes 2.5 us, a
- * launch and a few waits. */
+ * Bound by memory where the weight is large: those 73 MB at 3.4 TB/s from HBM (a copy reaches 4.8), 17.6 us where the
+ * memory-side cache holds part of it; 1 x 1024 x 1024 takes 2.5 us, a launch and a few waits. */
 template <int DT, int GROUP, bool ZP, int WV, int NT, bool ONE>
 __global__ __launch_bounds__(64 * WV) void q4_gemv(Q4Args a)
 {
