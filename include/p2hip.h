@@ -377,7 +377,8 @@ enum { P2H_F32 = 0, P2H_F16 = 1, P2H_BF16 = 2 };
  * codes, N up to 2^27. */
 typedef struct P2hQ4Weight P2hQ4Weight;
 
-/* From host memory, or from device memory (read during the call only). Synchronous; NULL on failure. */
+/* From host memory, or from device memory (read during the call only, on the calling thread's stream: what writes it on
+ * another has to be done). Synchronous; NULL on failure. */
 P2hQ4Weight *p2h_q4_weight_upload(const unsigned char *codes, const uint16_t *scales, const unsigned char *zeros,
                                   int K, int N, int group);
 P2hQ4Weight *p2h_q4_weight_wrap(const void *d_codes, const void *d_scales, const void *d_zeros, int K, int N,
