@@ -769,10 +769,20 @@ template <class E, int DH, int KB, int NW> struct BlockLoads {
     }
 };
 
-/* Where the exponentials of a block have a sum above kSlack in some lane, the reference they are taken from is raised to
- * the largest score so far and they are taken again. It is not raised otherwise, so that most blocks need no maximum and
- * leave O as it is: a weight stays below kSlack, which every type holds, and relative to their sum nothing changes. */
-constexpr float kSlack = 1024.0f;
+/* Weights enter their product with V in the rows' type. fp16 keeps nothing under 2^-25, which many keys together, or one
+ * with a large value beside values near 0, can make felt; so the reference that weights are taken from stands kLift powers
+ * of two under the largest score (weights up to 2^kLift, and what is under 2^-(25 + kLift) of the largest is lost: 2^-40).
+ * Sums carry the same factor, so that it leaves with the division. bf16 ends where fp32 does and needs none. */
+template <int DT> constexpr float kLift = DT == T_F16 ? 15.0f : 0.0f;
+
+/* attention_win raises its reference only where the exponentials of a block have a sum above kWinSlack in some lane: then
+ * to the largest score so far, and they are taken again. It is not raised otherwise, so that most blocks need no maximum
+ * and leave O as it is: a weight stays below the slack, which every type holds, and relative to their sum nothing changes.
+ * fp16 ends at 65504, so that lift and slack share what is there: a lift of 2^6 loses what is under 2^-31 of the largest
+ * and leaves the slack what it is in bf16. Higher lifts raise the reference more often (6000 rows of 32 heads of 128, scores
+ * of deviation 2: 2^5 110 us, 2^8 112, 2^10 115; rising scores 108, 112, 118). */
+template <int DT> constexpr float kWinLift = DT == T_F16 ? 6.0f : 0.0f;
+template <int DT> constexpr float kWinSlack = DT == T_F16 ? 65504.0f : 1024.0f;
 
 /* 32 queries of one head in a wave: lane % 32 is the query, 16-bit rows. */
 template <int DH> struct WinSub {
@@ -899,13 +909,13 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
     /* the weights' sum goes into l; before, where it is too large or there is no reference yet, they are taken again from
      * the largest score */
     auto settle = [&](float sum) __attribute__((always_inline)) {
-        if (__any(sum > kSlack || u.m == -INFINITY)) {
+        if (__any(sum > kWinSlack<DT> || u.m == -INFINITY)) {
             float top = u.s[0][0];
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) top = fmaxf(top, u.s[n][i]);
-            const float mn = fmaxf(u.m, max_halves(top) * a.c), mu = mn == -INFINITY ? 0.0f : mn;
+            const float mn = fmaxf(u.m, __builtin_fmaf(max_halves(top), a.c, -kWinLift<DT>)), mu = mn == -INFINITY ? 0.0f : mn;
             const float fade = exp2_fast(u.m - mu);
             u.m = mn;
             u.l *= fade;
@@ -1117,11 +1127,11 @@ struct PageArgs {
     const void *q, *kc, *vc;
     const int *table, *len;
     void *o;
-    float *part;   /* [sequence][head][split][DH + 2] where splits > 1: sums, maximum, sum of weights */
+    float *part;   /* [sequence][head][split][DH + 2] where splits > 1: sums, reference, sum of weights */
 };
 
-/* The softmax state of up to 16 queries (lane % 16) over the blocks that one wave has taken: O^T tiles, running maximum
- * and this lane's share of the sum of weights. */
+/* The softmax state of up to 16 queries (lane % 16) over the blocks that one wave has taken: O^T tiles, the reference (the
+ * running maximum less kLift) and this lane's share of the sum of weights. */
 template <int DH> struct FewState {
     f4 o[DH / 16];
     float m, l;
@@ -1205,7 +1215,7 @@ __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / 
     const int lane = threadIdx.x & 63, g = lane >> 4, x16 = lane & 15;
     if (b >= end) return;
     auto soften = [&](float top) __attribute__((always_inline)) {
-        const float mn = fmaxf(st.m, max_quarters(top) * c), mu = mn == -INFINITY ? 0.0f : mn;
+        const float mn = fmaxf(st.m, __builtin_fmaf(max_quarters(top), c, -kLift<DT>)), mu = mn == -INFINITY ? 0.0f : mn;
         const float fade = exp2_fast(st.m - mu);
         st.m = mn;
         return float2{mu, fade};
@@ -1345,8 +1355,8 @@ __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / 
     }
 }
 
-/* the waves' states into LDS as [wave][16 queries][DH + 2], the last two the maximum and the sum, and one output of their
- * join: sums relative to the returned maximum */
+/* the waves' states into LDS as [wave][16 queries][DH + 2], the last two the reference and the sum, and one output of their
+ * join: sums relative to the largest reference, which is returned */
 template <int DT, int DH> __device__ __forceinline__ void few_store(FewState<DH> &st, float *J)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;

@@ -768,3 +768,47 @@ def test_two_graphs_share_a_workspace(t):
         s.sync()
         for _, do, alone, _ in made:
             assert np.array_equal(do.download((2, H * Dh), D.np_type(t)).view(np.uint16), alone.view(np.uint16))
+
+
+# ── weights far below the largest ───────────────────────────────────────────────────────────────────────────────
+
+def dominated(n, nq, H, Hk, Dh, key):
+    """fp16 rows whose first key takes nearly all of the weight, with a value of 0; the others' weights are about 2^-26 of
+    its, so that all of the result is theirs."""
+    rng = rng_of(n, H, Dh, key, "dominated")
+    q, k = np.zeros((nq, H, Dh)), np.zeros((n, Hk, Dh))
+    q[..., 0], k[0, :, 0] = 1.0, 18.0
+    k[1:, :, 0] = rng.uniform(-0.5, 0.5, (n - 1, Hk))
+    v = rng.uniform(0.5, 1.5, (n, Hk, Dh)) * rng.choice((-30, 30), (1, Hk, Dh))
+    v[0] = 0.0
+    return D.to_type("f16", q), D.to_type("f16", k), D.to_type("f16", v)
+
+
+@pytest.mark.parametrize("nq,H,Hk,Dh", ((16, 128, 16, 128), (16, 136, 17, 64), (1, 2, 1, 64), (20, 1, 1, 128)))
+def test_window_small_fp16_weights(nq, H, Hk, Dh):
+    """Weights are rounded to fp16 for their product with V: to half a step, and down to 2^-31 of the largest one."""
+    n = 20000
+    q, k, v = dominated(n, nq, H, Hk, Dh, "window")
+    flat = [a.reshape(a.shape[0], -1) for a in (q, k, v)]
+    got = D.to_f64("f16", D.run_window("f16", *flat, H, Hk, Dh, 1.0, EVERY, EVERY, 0))
+    s = np.array([0, nq]), np.array([0, n])
+    want, bound = window_want("f16", *flat, *s, H, Hk, Dh, 1.0, EVERY, EVERY, 0)
+    lost = 2.0 ** -31 * np.abs(D.to_f64("f16", v)).sum(0)
+    D.check(got, want, bound + np.repeat(lost, H // Hk, 0).reshape(1, -1), f"{nq} {H} {Dh}")
+
+
+@pytest.mark.parametrize("n,split", ((20000, False), (20000, True), (700, True)))
+@pytest.mark.parametrize("Dh", (64, 128))
+def test_paged_small_fp16_weights(n, split, Dh):
+    """As above; here a weight is taken relative to the largest one of its wave's keys and held down to 2^-40 of it."""
+    H, Hk, page = 4, 2, 16
+    q, k, v = dominated(n, 1, H, Hk, Dh, "paged")
+    per = -(-n // page)
+    table = rng_of("dominated pages").permutation(per).astype(np.int32)[None]
+    kc, vc = (np.zeros((per, Hk, page, Dh), np.float16) for _ in range(2))
+    j = np.arange(n)
+    kc[table[0, j // page], :, j % page], vc[table[0, j // page], :, j % page] = k, v
+    got = D.to_f64("f16", D.run_paged("f16", q.reshape(1, -1), kc, vc, table, (n,), H, 1.0, EVERY, 0, split))
+    want, bound = paged_want("f16", q.reshape(1, -1), kc, vc, table, (n,), H, 1.0, EVERY, 0)
+    lost = 2.0 ** -40 * np.abs(D.to_f64("f16", v)).sum(0)
+    D.check(got, want, bound + np.repeat(lost, H // Hk, 0).reshape(1, -1), f"{n} {split} {Dh}")
