@@ -178,6 +178,9 @@ int p2host::fail(int rc, const char *fmt, ...)
     va_start(ap, fmt);
     vsnprintf(t_err, sizeof t_err, fmt, ap);
     va_end(ap);
+    /* The runtime keeps a failed call's error for the thread until it is asked for, and the next launch, which is judged by
+     * it, would seem to have failed: a refused allocation was reported by the upload or the kernel after it. */
+    if (rc == P2H_E_DEVICE || rc == P2H_E_NOMEM) (void)hipGetLastError();
     return rc;
 }
 
@@ -449,7 +452,10 @@ int p2h_stream_hold(void *stream, unsigned usec)
 float p2h_event_elapsed_ms(void *start, void *stop)
 {
     float ms = -1.0f;
-    if (hipEventElapsedTime(&ms, (hipEvent_t)start, (hipEvent_t)stop) != hipSuccess) return -1.0f;
+    if (hipEventElapsedTime(&ms, (hipEvent_t)start, (hipEvent_t)stop) != hipSuccess) {
+        (void)hipGetLastError();   /* answered here, as p2host::fail answers others */
+        return -1.0f;
+    }
     return ms;
 }
 

@@ -14,7 +14,7 @@
 
 namespace p2host {
 
-/* set this thread's error message and return rc */
+/* set this thread's error message and return rc; the runtime's own error, if rc reports one, is thereby taken */
 P2_HIDDEN int fail(int rc, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 P2_HIDDEN int ensure_init();
 P2_HIDDEN hipStream_t stream_of(void *s);   /* NULL: the calling thread's own stream */

@@ -812,3 +812,30 @@ def test_paged_small_fp16_weights(n, split, Dh):
     want, bound = paged_want("f16", q.reshape(1, -1), kc, vc, table, (n,), H, 1.0, EVERY, 0)
     lost = 2.0 ** -40 * np.abs(D.to_f64("f16", v)).sum(0)
     D.check(got, want, bound + np.repeat(lost, H // Hk, 0).reshape(1, -1), f"{n} {split} {Dh}")
+
+
+# ── errors ──────────────────────────────────────────────────────────────────────────────────────────────────────
+
+def test_a_refused_allocation_is_reported_once():
+    """What follows it on the thread works: an upload, a linear, a five-value weight."""
+    K, N, group = 128, 32, 32
+    rng = rng_of("refused")
+    x, wt = D.rows(rng, "f32", 2, K), D.q4_weight(rng, K, N, group, True)
+    want = D.run_q4("f32", x, wt, K, N, group)
+    planes = P.gen_fv_weight(1, 1, 128, 64)
+    w, dx, dy = P.Q4Weight(*wt, K, N, group), D.device(x), D.preset("f32", (2, N))
+
+    def refuse():
+        with pytest.raises(P.P2Error, match="hipMalloc"):
+            P.DeviceBuffer(1 << 50)
+
+    refuse()
+    P.Q4Weight(*wt, K, N, group)
+    refuse()
+    P.q4_gemv_dev("f32", 2, N, K, 1.0, dx.ptr, K, w, 0.0, dy.ptr, N)
+    assert np.array_equal(dy.download((2, N), np.float32), want)
+    refuse()
+    P.FvWeight(*planes, 128, 64)
+    with pytest.raises(P.P2Error):
+        P.Event().elapsed_ms(P.Event())   # never recorded
+    P.q4_gemv_dev("f32", 2, N, K, 1.0, dx.ptr, K, w, 0.0, dy.ptr, N)
