@@ -439,7 +439,7 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
  * where there are few sequences, planned for lengths up to max_len (other lengths are right as well), and a second
  * kernel joins the parts kept in the workspace, p2h_attention_paged_workspace_bytes(...) bytes, 16-byte aligned (0: the
  * call does not split). Without a workspace (NULL) it runs unsplit. Calls sharing a workspace are stream-ordered. dO
- * overlaps nothing the call reads, nor the workspace. */
+ * and the workspace overlap nothing the call reads, nor each other. */
 size_t p2h_attention_paged_workspace_bytes(const P2hKvCache *cache, int n_seqs, int heads, int max_len, int window,
                                            int sinks);
 int p2h_attention_paged(const P2hKvCache *cache, int n_seqs, int heads, const void *dQ, int ldq, const int *dTable,

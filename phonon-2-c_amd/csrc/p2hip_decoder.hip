@@ -493,8 +493,13 @@ int p2h_attention_paged(const P2hKvCache *cache, int n_seqs, int heads, const vo
         if (workspace_bytes < need || !aligned(workspace, 16))
             return fail(P2H_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", name, workspace_bytes,
                         need);
-        if (overlap(o, Rows{(const char *)workspace, need, need, 1}))
-            return fail(P2H_E_ARG, "%s: dO overlaps the workspace", name);
+        const Rows ws{(const char *)workspace, need, need, 1};
+        if (overlap(o, ws)) return fail(P2H_E_ARG, "%s: dO overlaps the workspace", name);
+        /* it is written while other workgroups still read */
+        if (overlap(ws, Rows{(const char *)dQ, ldq * es, w, n_seqs}) || overlap(ws, cache) ||
+            overlap(ws, Rows{(const char *)dLen, 4, 4, n_seqs}) ||
+            overlap(ws, Rows{(const char *)dTable, (size_t)table_ld * 4, (size_t)table_ld * 4, table_ld ? n_seqs : 0}))
+            return fail(P2H_E_ARG, "%s: the workspace overlaps dQ, the cache, the lengths or the page table", name);
     }
     if (overlap(o, cache)) return fail(P2H_E_ARG, "%s: dO overlaps the cache", name);
     const int G = heads / cache->heads, q_groups = (G + 15) / 16;

@@ -148,6 +148,20 @@ def test_paged_output_apart_from_what_it_reads():
     refused(paged(c, n=1, most=100000, window=1 << 30, ws=2 * A - need + 16, wsb=need), "dO overlaps the workspace")
 
 
+def test_paged_workspace_apart_from_what_it_reads():
+    """The parts are written while other workgroups still read queries, keys, lengths and pages."""
+    c = cache(dK=8 * A, dV=9 * A)
+    size = 4 * 2 * 16 * 64 * 2
+    need = P.attention_paged_workspace_bytes(c, 1, 4, 100000)
+    big = dict(n=1, most=100000, window=1 << 30, wsb=need, q=20 * A, lens=30 * A, table=40 * A, ld=7, o=50 * A)
+    for ws in (8 * A, 8 * A + size - 16, 9 * A - need + 16, 9 * A,   # the cache
+               20 * A, 20 * A - need + 16, 20 * A + 496,             # one row of 256 queries
+               30 * A, 30 * A - need + 16, 40 * A + 16, 40 * A - need + 16):
+        refused(paged(c, ws=ws, **big), "workspace overlaps")
+    for ws in (8 * A + size, 9 * A - need, 20 * A + 512, 30 * A + 16, 40 * A + 32):   # side by side: refused only for dO
+        refused(paged(c, ws=ws, **dict(big, o=8 * A + 16)), "dO overlaps the cache")
+
+
 def test_too_many_for_one_launch():
     refused(rope(T=1 << 24), "below 2^24")
     refused(win(qr=1 << 29, kr=1 << 29, heads=8, o=1 << 50, k=1 << 51, v=1 << 52, ldk=256, ldq=1024, ldo=1024), "too many")
