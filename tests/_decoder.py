@@ -210,3 +210,41 @@ def gather(t, cache, row, n, page, pages):
     held = (p >= 0) & (p < pages)
     vals = to_f64(t, cache)[np.where(held, p, 0), :, j % page]
     return np.where(held[:, None, None], vals, 0.0), held
+
+
+# ── how far 32-bit results may be off on the whole ──────────────────────────────────────────────────────────────
+
+# Relative 2-norms of the error of fp32 results, beside the elementwise bounds, which count every rounding at its worst and
+# would let a loss of half the bits pass.
+#
+# q4: a matrix product drops what lies below the last place of its sum, up to a step of 2^-23 (products of 2^-26 beside one
+# of 1 lose 7/8 of it together), rms 0.58 · 2 · 2^-24 of a sum that grows to its full size as a random walk does: n products
+# make 1.15 · sqrt(n / 2) · 2^-24 of the result. A group of 128 takes three pieces by four products, 12 (2.8), of x · code;
+# codes have an rms of 8.8, code − zero one of 6.5 (any zero point) or 4.6 (all 8), so that this is up to 1.9 times as much
+# of the result (5.4). x · zero the same by 1.7 (4.8), but it is one sum for all outputs of a row: twice that may come for a
+# single row (9.6). Then 33 groups' sums in a wave at most (2.4), the waves' 8 and the scales (1.5), to nearest:
+# sqrt(5.4² + 9.6² + 2.4² + 1.5²) = 11.4, against 16 allowed.
+Q4_NORM = 16 * FP32
+# Attention at scores of about 1: a score of 64 or 128 products, 5; its exponent less the reference and the exponential, 3;
+# a weighted sum of up to 1100 keys, two or four at a time, 0.58 · sqrt(550 / 2) = 9.6, or less where waves share them; the
+# sum of weights and the quotient 1: sqrt(5² + 3² + 9.6² + 1) = 11.3, against 16 allowed.
+ATTENTION_NORM = 16 * FP32
+
+
+def norm_off(got, want):
+    return float(np.sqrt(((got - want) ** 2).sum() / (want ** 2).sum()))
+
+
+def pieces(x, n):
+    """The first n of the bf16 pieces (upper 16 bits of what is left) that an fp32 value is cut into, summed."""
+    left, out = np.asarray(x, np.float32).copy(), np.zeros(np.shape(x))
+    for _ in range(n):
+        p = (left.view(np.uint32) & np.uint32(0xFFFF0000)).view(np.float32)
+        out += p
+        left -= p
+    return out
+
+
+def short(x, bits):
+    """fp32 values with `bits` significant bits, the rest cut off."""
+    return (np.asarray(x, np.float32).view(np.uint32) & np.uint32(0xFFFFFFFF << (24 - bits) & 0xFFFFFFFF)).view(np.float32)

@@ -839,3 +839,40 @@ def test_a_refused_allocation_is_reported_once():
     with pytest.raises(P.P2Error):
         P.Event().elapsed_ms(P.Event())   # never recorded
     P.q4_gemv_dev("f32", 2, N, K, 1.0, dx.ptr, K, w, 0.0, dy.ptr, N)
+
+
+# ── fp32 results on the whole ───────────────────────────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("M", (1, 5, 18))
+@pytest.mark.parametrize("group,zeros", ((32, False), (32, True), (64, True), (128, False), (128, True)))
+@pytest.mark.parametrize("K,N", ((1024, 48), (4096, 40), (8200, 24), (1000, 8201), (1024, 16400)))
+def test_q4_fp32_on_the_whole(M, K, N, group, zeros):
+    rng = rng_of(M, K, N, group, zeros, "whole")
+    x, wt = D.rows(rng, "f32", M, K), D.q4_weight(rng, K, N, group, zeros)
+    want = x.astype(np.float64) @ D.q4_values(*wt, K, N, group)
+    off = D.norm_off(D.run_q4("f32", x, wt, K, N, group).astype(np.float64), want)
+    assert off <= D.Q4_NORM, off / D.FP32
+
+
+@pytest.mark.parametrize("Dh", (64, 128))
+@pytest.mark.parametrize("lens,past,H,Hk,window,ahead,sinks", WIN + BIG)
+def test_window_fp32_on_the_whole(Dh, lens, past, H, Hk, window, ahead, sinks):
+    q, k, v, qs, ks = window_case("f32", lens, past, H, Hk, Dh, "whole")
+    got = D.run_window("f32", q, k, v, H, Hk, Dh, Dh ** -0.5, window, ahead, sinks, qs, ks)
+    want, _ = window_want("f32", q, k, v, qs, ks, H, Hk, Dh, Dh ** -0.5, window, ahead, sinks)
+    if want.any():
+        off = D.norm_off(got.astype(np.float64), want)
+        assert off <= D.ATTENTION_NORM, off / D.FP32
+    else:
+        assert not got.any()
+
+
+@pytest.mark.parametrize("split", (False, True))
+@pytest.mark.parametrize("Dh", (64, 128))
+@pytest.mark.parametrize("lens,H,Hk,page,window,sinks", PAGED)
+def test_paged_fp32_on_the_whole(split, Dh, lens, H, Hk, page, window, sinks):
+    q, kc, vc, table = paged_case("f32", lens, H, Hk, page, Dh, "whole")
+    want, _ = paged_want("f32", q, kc, vc, table, lens, H, Dh ** -0.5, window, sinks)
+    got = D.run_paged("f32", q, kc, vc, table, lens, H, Dh ** -0.5, window, sinks, split, 40000 if split else None)
+    off = D.norm_off(got.astype(np.float64), want)
+    assert off <= D.ATTENTION_NORM, off / D.FP32
