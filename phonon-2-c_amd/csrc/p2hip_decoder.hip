@@ -396,24 +396,17 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
             return fail(P2H_E_ARG, "%s: dO overlaps dK or dV", name);
     }
     if (overlap(o, Rows{(const char *)dQ, ldq * es, q_w, q_rows})) return fail(P2H_E_ARG, "%s: dO overlaps dQ", name);
-    /* at most 512 threads for 128 rows of one head and for one tile more of each sequence; 16 rows a workgroup, where they
-     * are few, make 2048 of them */
+    /* at most 256 threads for 128 rows of one head and for one tile more of each sequence; 512 where they go by 16 queries,
+     * which is looked at there */
     if (((size_t)(q_rows / 128 + 1) + n_seqs) * heads + 2048 >= kGridThreads / 512)
         return fail(P2H_E_ARG, "%s: %d rows of %d heads in %d sequences are too many for one call", name, q_rows, heads, n_seqs);
     if (int rc = ensure_init()) return rc;
     /* The queries of a tile and the query heads a workgroup takes (its kernel says why); one tile more per sequence than
      * the rows fill (tile_start). */
     const int G = heads / kv_heads, hpw = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
-    /* Few queries go 16 to a workgroup whose waves share the keys. 16-bit rows: below 64 workgroups of 128 rows (8 heads,
-     * all keys: 375 queries 9.4 us against 13.0, 750 15.3 against 19.4, 1500 both 31.7), and with heads of 64 and long keys,
-     * whose blocks a tile takes one after the other, up to 128 (2000 queries of 8 heads 21.6 us against 30.0, 8000 of 2 57
-     * against 99; 4000 of 8 58 against 54). fp32 rows, whose products take ten times as long: while those do not fill the
-     * device (1500 queries 73 us against 203, 4000 362 against 525, 32 heads of 2000 396 against 292), but for short
-     * windows only below 128 (window 256, 3000 queries: 69 against 65). */
-    const long long full = (long long)((q_rows + 127) / 128) * heads;
-    const bool long_keys = p2k::imin(k_rows / n_seqs, window + p2k::imin(ahead, k_rows)) >= 1000;
-    const bool few = dtype != P2H_F32 ? full < 64 || (head_dim == 64 && full <= 128 && long_keys)
-                                      : full <= cu_count() && (full < 128 || (long long)window + ahead >= 512);
+    const size_t few_wgs = ((size_t)q_rows / 16 + n_seqs) * heads;
+    const bool few = few_wgs < kGridThreads / 512 && p2k::few_queries(dtype == P2H_F32, head_dim, q_rows, k_rows, n_seqs, heads,
+                                                                      window, ahead, cu_count());
     const int qb = few ? 16 : dtype == P2H_F32 ? 128 : 128 / hpw, per = few || dtype == P2H_F32 ? 1 : hpw;
     const long long tiles = (long long)(dQStart ? q_rows / qb + n_seqs : (q_rows + qb - 1) / qb);
     p2k::WinArgs a{};
@@ -437,10 +430,11 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
 
 /* How many workgroups share the keys of one sequence and key head. Up to 192 KB of keys and values one: what a CU reads in
  * about the time that the second kernel costs (one bf16 sequence over 8 key heads of 128: 375 tokens 6.9 us against 8.5
- * split, 750 9.5 against 8.3, 2000 17.2 against 8.7; 16 fp16 heads of 64: 750 tokens 6.7 us, 1000 7.7 against 7.0). Above that one for every 4
- * blocks, a block for each wave (2000 tokens in parts of 11 blocks a wave: 12.3), as long as all together are at most
- * two a CU (2 sequences of 131072: 100 us with 32 to 64 parts, 113 with 256; 32 of 8192, 256 groups: 188 us in 2 parts or
- * unsplit, 199 in 16). */
+ * split, 750 9.5 against 8.3, 2000 17.2 against 8.7; 16 fp16 heads of 64: 750 tokens 6.7 us, 1000 7.7 against 7.0).
+ * Above that one for every 4 blocks, a block for each wave (2000 tokens in parts of 11 blocks a wave: 12.3), as long as all
+ * together are at most 512, two for each of 256 CUs (2 sequences of 131072: 100 us with 32 to 64 parts, 113 with 256; 32 of
+ * 8192, 256 groups: 188 us in 2 parts or unsplit, 199 in 16); a number, as the workspace's size is asked for where there may
+ * be no device. */
 static int page_splits(const P2hKvCache *c, int n_seqs, int heads, int max_len, int window, int sinks)
 {
     const int G = heads / c->heads, kb = c->dtype == P2H_F32 ? 16 : 32;

@@ -87,4 +87,30 @@ P2_HD int tile_start(const int32_t *start, int s, int rows_in_all, int rows)
     return imin(imax(start[s], 0), rows_in_all) / rows + s;
 }
 
+/* Whether a windowed call goes by 16 queries a workgroup, whose waves share the keys, or by tiles of 128 rows (16-bit rows:
+ * of up to four query heads that read one key head). What counts is workgroups: those of 16 queries, by the mean length of
+ * the sequences, which with their number is all that the host knows of them.
+ *
+ * 16-bit rows: 16 queries while they make fewer than 512 workgroups (8 heads of 128, all keys: 375 queries 9.4 us against
+ * 13.0, 750 15.3 against 19.4, 1500 both 31.7; 64 heads, 16 queries behind 8000 keys 56 against 135), with heads of 64 and
+ * long keys, whose blocks a tile takes one after the other, up to 1024 (2000 queries of 8 heads 21.6 us against 30.0, 8000
+ * of 2 57 against 99; 4000 of 8 58 against 54). Sequences of one query are that many workgroups in either form, fewer where
+ * tiles share key heads (64 sequences of 1000 keys, 32 heads over 8: 84 us, in tiles 44; 256 of 1000, heads of 64: 214, 117).
+ *
+ * fp32 rows, whose products take ten times as long: while 128-row tiles do not fill the device (1500 queries 73 us against
+ * 203, 4000 362 against 525, 32 heads of 2000 396 against 292), but for short windows only below 128 of them (window 256,
+ * 3000 queries: 69 against 65); and where sequences have at most 16 queries, since a tile multiplies 128 all the same (256
+ * sequences of 8 queries and 100 keys, 32 heads: 0.53 of the tiles' time; of 17 queries 1.02). */
+P2_HD bool few_queries(bool f32, int head_dim, int q_rows, int k_rows, int n_seqs, int heads, int window, int ahead, int cus)
+{
+    const int seqs = imin(n_seqs, q_rows), mean = (q_rows - 1) / seqs + 1;
+    const long long wgs = (long long)heads * seqs * ((mean - 1) / 16 + 1);
+    if (!f32) {
+        const bool long_keys = imin(k_rows / n_seqs, window + imin(ahead, k_rows)) >= 1000;
+        return wgs < 512 || (head_dim == 64 && wgs <= 1024 && long_keys);
+    }
+    const long long full = (long long)((q_rows - 1) / 128 + 1) * heads;
+    return mean <= 16 || (full <= cus && (full < 128 || (long long)window + ahead >= 512));
+}
+
 }  // namespace p2k

@@ -104,3 +104,43 @@ def test_index_arithmetic(tmp_path):
                     "-I", CSRC, "-o", str(exe), str(src)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
+
+
+RULE = r"""
+#include <cstdio>
+#include <climits>
+#include "p2hip_index.h"
+using namespace p2k;
+#define CHECK(c) do { if (!(c)) { printf("line %d: %s\n", __LINE__, #c); return 1; } } while (0)
+
+int main()
+{
+    const int all = 1 << 30;
+    auto f16 = [&](int dh, int q, int k, int n, int heads) { return few_queries(false, dh, q, k, n, heads, all, 0, 256); };
+    auto f32 = [&](int q, int k, int n, int heads, int w) { return few_queries(true, 128, q, k, n, heads, w, 0, 256); };
+    /* one sequence */
+    CHECK(f16(128, 375, 375, 1, 8) && f16(128, 750, 750, 1, 8) && !f16(128, 1500, 1500, 1, 8) && !f16(128, 6000, 6000, 1, 32));
+    CHECK(f16(64, 2000, 2000, 1, 8) && !f16(64, 4000, 4000, 1, 8) && !f16(64, 1100, 900, 1, 8));
+    CHECK(f16(128, 16, 8000, 1, 64) && f16(128, 1, 8000, 1, 256));
+    CHECK(f32(438, 438, 1, 8, 128) && f32(4000, 4000, 1, 8, all) && !f32(2000, 2000, 1, 32, all) && !f32(3000, 3000, 1, 8, 256));
+    /* many sequences of few queries are many workgroups whatever their rows come to */
+    CHECK(!f16(128, 64, 64000, 64, 32) && !f16(64, 256, 256000, 256, 32) && !f16(64, 64 * 8, 64 * 4000, 64, 32));
+    CHECK(f16(128, 16, 16000, 16, 8) && f16(64, 16 * 8, 16 * 1000, 16, 32) && !f16(64, 16 * 8, 16 * 100, 16, 32));
+    /* a tile of fp32 rows multiplies 128 of them whatever it holds */
+    CHECK(f32(256 * 8, 256 * 100, 256, 32, all) && f32(256 * 16, 256 * 100, 256, 32, all) && !f32(256 * 17, 256 * 100, 256, 32, all));
+    /* empty sequences, no keys and the largest numbers */
+    CHECK(f16(128, 1, 0, 100000, 8) && few_queries(true, 64, 1, 1, INT_MAX, 1, all, all, 256));
+    CHECK(!few_queries(false, 64, all - 1, all - 1, 1, 65536, all, all, 256) && !few_queries(true, 128, all - 1, all - 1, 7, 65536, 1, 0, 256));
+    puts("ok");
+    return 0;
+}
+"""
+
+
+def test_rule_for_few_queries(tmp_path):
+    src, exe = tmp_path / "rule.cpp", tmp_path / "rule"
+    src.write_text(RULE)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                    "-I", CSRC, "-o", str(exe), str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr

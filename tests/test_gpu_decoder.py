@@ -784,10 +784,11 @@ def dominated(n, nq, H, Hk, Dh, key):
     return D.to_type("f16", q), D.to_type("f16", k), D.to_type("f16", v)
 
 
-@pytest.mark.parametrize("nq,H,Hk,Dh", ((16, 128, 16, 128), (16, 136, 17, 64), (1, 2, 1, 64), (20, 1, 1, 128)))
-def test_window_small_fp16_weights(nq, H, Hk, Dh):
+@pytest.mark.parametrize("n,nq,H,Hk,Dh", (
+    (20000, 16, 128, 16, 128), (20000, 16, 136, 17, 64), (20000, 1, 2, 1, 64), (20000, 20, 1, 1, 128),
+    (3000, 80, 128, 16, 128), (900, 100, 136, 17, 64), (20000, 600, 16, 2, 128)))   # the last three in tiles of 128 rows
+def test_window_small_fp16_weights(n, nq, H, Hk, Dh):
     """Weights are rounded to fp16 for their product with V: to half a step, and down to 2^-31 of the largest one."""
-    n = 20000
     q, k, v = dominated(n, nq, H, Hk, Dh, "window")
     flat = [a.reshape(a.shape[0], -1) for a in (q, k, v)]
     got = D.to_f64("f16", D.run_window("f16", *flat, H, Hk, Dh, 1.0, EVERY, EVERY, 0))
@@ -839,6 +840,18 @@ def test_a_refused_allocation_is_reported_once():
     with pytest.raises(P.P2Error):
         P.Event().elapsed_ms(P.Event())   # never recorded
     P.q4_gemv_dev("f32", 2, N, K, 1.0, dx.ptr, K, w, 0.0, dy.ptr, N)
+
+
+# ── many sequences of few queries ───────────────────────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("lens,past,H,Hk,Dh", (((1,) * 64, 40, 32, 8, 128), ((3, 1, 0, 8) * 20, 70, 24, 4, 64),
+                                               ((17,) * 30, 0, 24, 4, 128), ((2,) * 5, 1100, 32, 8, 64)))
+def test_window_batches_of_few_queries(t, lens, past, H, Hk, Dh):
+    q, k, v, qs, ks = window_case(t, lens, past, H, Hk, Dh, "batch")
+    got = D.run_window(t, q, k, v, H, Hk, Dh, Dh ** -0.5, EVERY, 0, 0, qs, ks)
+    want, bound = window_want(t, q, k, v, qs, ks, H, Hk, Dh, Dh ** -0.5, EVERY, 0, 0)
+    D.check(D.to_f64(t, got), want, bound, f"{t} {Dh} {H}")
 
 
 # ── fp32 results on the whole ───────────────────────────────────────────────────────────────────────────────────
