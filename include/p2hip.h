@@ -391,7 +391,7 @@ size_t p2h_q4_weight_device_bytes(const P2hQ4Weight *w);
 
 /* Y [M][N] = alpha · X [M][K] · W + beta · Y for few rows (beta 0 does not read Y): a matrix-vector product per row,
  * the weight read once for every 16 rows. X and Y of type `dtype`, pitches ldx >= K and ldy >= N elements, no alignment
- * beyond the element's (16-byte aligned rows load faster). A row's outputs are the same bits whatever M is. X and Y
+ * beyond the element's (rows that are all 16-byte aligned load several times faster). A row's outputs are the same bits whatever M is. X and Y
  * must not overlap. A group's products are summed before its scale is applied: values of |x| from 2^118 up may overflow.
  * fp16 rows sum x · (code − zero); the others sum x · code and x · zero apart, in 32 bits: near a weight of 0 their errors
  * are those of the two sums. Of an fp32 value what lies under 2^-133 counts as zero: below 2^-110 it

@@ -239,7 +239,7 @@ int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int
     if (int rc = ensure_init()) return rc;
     p2k::Q4Args a{};
     a.M = M; a.N = N; a.K = K; a.units = w->units; a.ldx = ldx; a.ldy = ldy;
-    a.vec = aligned(dX, 16) && ldx * es % 16 == 0 && ldx < (1 << 25);   /* 16 rows within 32-bit offsets */
+    a.vec = p2k::rows_by_16((uintptr_t)dX, ldx, (int)es, M);
     a.alpha = alpha; a.beta = beta; a.x = dX; a.y = dY;
     a.rec = (const p2k::u4 *)w->base;
     a.sc = w->base + w->sc_off;

@@ -128,6 +128,9 @@ int main()
     CHECK(f16(128, 16, 16000, 16, 8) && f16(64, 16 * 8, 16 * 1000, 16, 32) && !f16(64, 16 * 8, 16 * 100, 16, 32));
     /* a tile of fp32 rows multiplies 128 of them whatever it holds */
     CHECK(f32(256 * 8, 256 * 100, 256, 32, all) && f32(256 * 16, 256 * 100, 256, 32, all) && !f32(256 * 17, 256 * 100, 256, 32, all));
+    /* rows of a linear: a single one has no pitch */
+    CHECK(rows_by_16(32, 1019, 2, 1) && rows_by_16(32, INT_MAX, 4, 1) && !rows_by_16(34, 1024, 2, 1) && !rows_by_16(40, 8, 2, 1));
+    CHECK(rows_by_16(32, 1024, 2, 2) && !rows_by_16(32, 1020, 2, 2) && rows_by_16(32, 1020, 4, 13) && !rows_by_16(32, 1 << 25, 2, 2));
     /* empty sequences, no keys and the largest numbers */
     CHECK(f16(128, 1, 0, 100000, 8) && few_queries(true, 64, 1, 1, INT_MAX, 1, all, all, 256));
     CHECK(!few_queries(false, 64, all - 1, all - 1, 1, 65536, all, all, 256) && !few_queries(true, 128, all - 1, all - 1, 7, 65536, 1, 0, 256));

@@ -142,6 +142,17 @@ def test_q4_tiny_fp32_rows(M, scale):
     D.check(got, x64 @ w, D.q4_bound("f32", x64, w, x64 @ w, 1.0, K) + lost, str(scale))
 
 
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("K", (1019, 4100, 130))
+def test_q4_one_row_has_no_pitch(t, K):
+    """Whatever pitch a single row is given with: the same bits."""
+    rng = rng_of(t, K, "one row")
+    x, wt = D.rows(rng, t, 1, K), D.q4_weight(rng, K, 70, 64, True)
+    want = D.run_q4(t, x, wt, K, 70, 64, ldx=-(-K // 8) * 8)
+    for ldx in (K, K + 1, 1 << 25):
+        assert np.array_equal(D.run_q4(t, x, wt, K, 70, 64, ldx=ldx), want), ldx
+
+
 def test_q4_rows_far_apart():
     M, K, N, group = 2, 300, 40, 64
     rng = rng_of("far apart")
