@@ -329,13 +329,13 @@ int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, co
     const size_t es = elem_size(dtype);
     const Rows x{(const char *)dQKV, ldqkv * es, in_w * es, T}, q{(const char *)dQ, ldq * es, q_w * es, T};
     const Rows xk{x.p + q_w * es, x.ld, in_w * es - q_w * es, T};   /* the rows from their keys on */
-    /* in place: exactly the q columns, apart from everything else */
-    const bool q_in = dQ == dQKV && ldq == ldqkv;
+    /* in place: exactly the q columns, apart from everything else (a single row has no pitch) */
+    const bool q_in = dQ == dQKV && (ldq == ldqkv || T == 1);
     if (q_in ? overlap(q, xk) : overlap(q, x)) return fail(P2H_E_ARG, "%s: dQ overlaps dQKV other than in place", name);
     if (dK) {
         const Rows k{(const char *)dK, ldk * es, k_w * es, T};
         const Rows xq{x.p, x.ld, q_w * es, T}, xv{xk.p + k_w * es, x.ld, xk.w - k_w * es, xk.w > k_w * es ? T : 0};
-        const bool k_in = k.p == xk.p && ldk == ldqkv;
+        const bool k_in = k.p == xk.p && (ldk == ldqkv || T == 1);
         if (k_in ? overlap(k, xq) || overlap(k, xv) : overlap(k, x))
             return fail(P2H_E_ARG, "%s: dK overlaps dQKV other than in place", name);
         if (overlap(q, k)) return fail(P2H_E_ARG, "%s: dQ and dK overlap", name);

@@ -139,6 +139,18 @@ def test_rope_and_its_cache(kw, part):
     refused(rope(**kw), part)
 
 
+def test_rope_of_one_row_in_place():
+    """A single row has no pitch: in place whatever pitches are given. That it passes is seen by what is refused next."""
+    last = dict(cache=cache(dK=8 * A, dV=A + 1024 - 16), slots=A)   # the cache's values on the row's end
+    for kw in (dict(q=A, ldq=256), dict(q=A, ldq=512), dict(q=A, ldq=256, k=A + 512, ldk=128),
+               dict(q=A, ldq=1024, k=A + 512, ldk=256)):
+        refused(rope(T=1, **dict(dict(k=3 * A), **kw), **last), "dQKV or dQ overlaps the cache")
+        if kw["ldq"] != 512:
+            refused(rope(T=2, **dict(dict(k=3 * A), **kw), **last), "dQ overlaps dQKV")
+    refused(rope(T=1, q=A + 16, ldq=256), "dQ overlaps dQKV")
+    refused(rope(T=1, q=A, ldq=256, k=A + 528, ldk=128), "dK overlaps dQKV")
+
+
 def test_paged_output_apart_from_what_it_reads():
     c = cache(dK=8 * A, dV=9 * A)
     size = 4 * 2 * 16 * 64 * 2

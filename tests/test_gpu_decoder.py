@@ -294,6 +294,19 @@ def test_rope_far_positions(pos):
     D.check(q.astype(np.float64).reshape(T, 1, Dh), want, D.rope_bound("f32", want, size_of, Dh) + extra, str(pos))
 
 
+@pytest.mark.parametrize("t", D.TYPES)
+def test_rope_one_row_in_place(t):
+    """A single row has no pitch: in place with the heads' width as pitch."""
+    H, Hk, Dh = 4, 2, 64
+    _, qkv, gq, gk, freq, pos = rope_inputs(t, 1, H, Hk, Dh, Dh, "one")
+    q, k = run_rope(t, qkv, H, Hk, Dh, gq, gk, 1e-6, Dh, False, freq, pos)
+    dx, dgq, dgk, df, dp = (D.device(a) for a in (qkv, gq, gk, freq, pos))
+    P.qk_norm_rope_dev(t, 1, H, Hk, Dh, dx.ptr, qkv.shape[1], dgq.ptr, dgk.ptr, 1e-6, Dh, False, df.ptr, dp.ptr, dx.ptr, H * Dh,
+                       dx.ptr + H * Dh * D.size(t), Hk * Dh)
+    got = dx.download(qkv.shape, D.np_type(t))
+    assert np.array_equal(got, np.concatenate((q, k, qkv[:, (H + Hk) * Dh:]), 1))
+
+
 def test_rope_zero_row_and_empty_call():
     T, H, Hk, Dh = 2, 2, 1, 64
     _, qkv, gq, gk, freq, pos = rope_inputs("bf16", T, H, Hk, Dh, 64, "zero")
