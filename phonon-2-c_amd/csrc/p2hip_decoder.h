@@ -485,7 +485,8 @@ struct RopeArgs {
  * circle (float then holds them to 2^-27 of a radian), and their sines and cosines are shared by all heads through LDS,
  * while the row's first values are on their way. Bound by memory: 6000 rows of 32 + 8 + 8 bf16 heads, 147 MB, in 33.5 us
  * (4.4 TB/s, a copy reaches 4.8); loading 4 heads a thread ahead took 35.9, making the angles before the first load 34.6.
- * Few rows take 1024 threads, all of a row's heads at once (16 rows 3.9 us, 5.7 with 256 threads). */
+ * Few rows take 1024 threads, all of a row's heads at once (16 rows 3.9 us, 5.7 with 256 threads). Heads whose squares
+ * leave the range of 32 bits (values from 2^60 up; without an eps to speak of, below 2^-48) are moved into it first. */
 template <int DT, int DH, int NTHR>
 __global__ __launch_bounds__(NTHR) void qk_norm_rope(RopeArgs a)
 {
@@ -521,15 +522,30 @@ __global__ __launch_bounds__(NTHR) void qk_norm_rope(RopeArgs a)
         u4 res = raw;
         const bool is_q = h < a.heads, is_v = h >= a.heads + a.kv;
         if (!is_v) {   /* the same for all lanes of a head */
-            float v[VE];
+            float v[VE], gm[VE];
+#pragma unroll
+            for (int i = 0; i < VE; i++) gm[i] = (is_q ? a.gq : a.gk)[VE * l + i];   /* on their way during the sum */
             unpack<DT>(raw, v);
             float ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < VE; i++) ss = __builtin_fmaf(v[i], v[i], ss);
 #pragma unroll
             for (int o = 1; o < LPH; o *= 2) ss += __shfl_xor(ss, o, LPH);
-            const float inv = 1.0f / sqrtf(ss * (1.0f / DH) + a.eps);
-            const float *gm = (is_q ? a.gq : a.gk) + VE * l;
+            float eps = a.eps;
+            if (DT != T_F16 && __builtin_expect(!(ss < INFINITY) || (ss < 0x1p-90f && eps < 0x1p-60f), false)) {
+                /* squares that leave the range of 32 bits, the same for all lanes of a head: of the head times a power of two */
+                const float by = ss < 1.0f ? 0x1p90f : 0x1p-68f;
+                eps = eps * by * by;
+                ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < VE; i++) {
+                    v[i] *= by;
+                    ss = __builtin_fmaf(v[i], v[i], ss);
+                }
+#pragma unroll
+                for (int o = 1; o < LPH; o *= 2) ss += __shfl_xor(ss, o, LPH);
+            }
+            const float inv = 1.0f / sqrtf(ss * (1.0f / DH) + eps);
 #pragma unroll
             for (int i = 0; i < VE; i++) v[i] = v[i] * inv * gm[i];
             if (a.interleaved) {

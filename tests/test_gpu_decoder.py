@@ -294,6 +294,23 @@ def test_rope_far_positions(pos):
     D.check(q.astype(np.float64).reshape(T, 1, Dh), want, D.rope_bound("f32", want, size_of, Dh) + extra, str(pos))
 
 
+@pytest.mark.parametrize("t", ("f32", "bf16"))
+@pytest.mark.parametrize("scale,eps", ((1e19, 1e-6), (3e20, 0.0), (1e37, 1e-6), (1e-16, 0.0), (1e-22, 0.0), (1e-37, 0.0),
+                                       (1e-22, 1e-30), (1e-14, 1e-28), (1e-20, 1e-6)))
+def test_rope_heads_of_any_size(t, scale, eps):
+    """Squares may leave the range of 32 bits, the norm does not."""
+    T, H, Hk, Dh, rot = 3, 4, 2, 128, 64
+    _, qkv, gq, gk, freq, pos = rope_inputs(t, T, H, Hk, Dh, rot, "size")
+    qkv = D.to_type(t, D.to_f64(t, qkv) / 3 * scale)
+    qkv[1, :Dh] = D.to_type(t, D.to_f64(t, qkv[1, :Dh]) / scale)   # an ordinary head beside them
+    q, k = run_rope(t, qkv, H, Hk, Dh, gq, gk, eps, rot, False, freq, pos)
+    x = D.to_f64(t, qkv).reshape(T, H + 2 * Hk, Dh)
+    eps = float(np.float32(eps))
+    for got, part, g, n in ((q, x[:, :H], gq, H), (k, x[:, H:H + Hk], gk, Hk)):
+        want, size_of = D.norm_rope(part, g, eps, rot, False, freq, pos)
+        D.check(D.to_f64(t, got).reshape(T, n, Dh), want, D.rope_bound(t, want, size_of, Dh), f"{t} {scale} {eps}")
+
+
 @pytest.mark.parametrize("t", D.TYPES)
 def test_rope_one_row_in_place(t):
     """A single row has no pitch: in place with the heads' width as pitch."""
