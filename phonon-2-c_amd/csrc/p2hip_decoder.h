@@ -871,7 +871,7 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
     u.l = 0.0f;
     u.p = imin(iq, w.Lq - 1) + w.off;
     u.full0 = imin(w.p0 + sub + 31, w.Lq - 1 + w.off) - a.window + 1;
-    u.full1 = imin(w.Lk - 1, w.p0 + sub + a.ahead) - (KB - 1);
+    u.full1 = last_seen_by_all(w.p0 + sub, w.Lk, a.ahead) - (KB - 1);
     bool odd = false;
 
     /* LDS byte addresses. K's operand x of 32 keys: row col, piece 2x + h, so that the pieces of a row are an exclusive or
@@ -899,12 +899,12 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
         lds_barrier();
     };
     /* What a query must not see of the block at k0, where its 32 queries do not all see all of it. Key e of the block is
-     * seen up to `last`, from `first` on or below `sink`: bit e of 64; this lane has keys 8j + 4h .. + 3 of every eight. */
+     * bit e of 64; this lane has keys 8j + 4h .. + 3 of every eight. */
     auto mask = [&](int k0) __attribute__((always_inline)) {
         if (k0 <= u.full1 && (k0 >= u.full0 || k0 < a.sinks - (KB - 1))) return;
-        const int last = imin(u.p + a.ahead, w.Lk - 1) - k0, first = u.p - a.window + 1 - k0, sink = a.sinks - k0;
+        const KeySpan span = key_span(k0, u.p, w.Lk, a.window, a.ahead, a.sinks);
         auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
-        const unsigned long long bits = (below(last + 1) & (~below(first) | below(sink))) >> (4 * h);
+        const unsigned long long bits = (below(span.last + 1) & (~below(span.first) | below(span.sink))) >> (4 * h);
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -1084,13 +1084,11 @@ __global__ __launch_bounds__(256, 2) void attention_win_f32(WinArgs a)
                 s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(q[x][e]), s, 0, 0, 0);
         }
         if (!w.all_seen(a, k0, KB, pw0, pw1)) {
-            /* key e of the block (from this lane's first) is seen up to `last`, from `first` on or below `sink` */
-            const int base = k0 + 4 * h, last = imin(p + a.ahead, w.Lk - 1) - base, first = p - a.window + 1 - base,
-                      sink = a.sinks - base;
+            const KeySpan span = key_span(k0 + 4 * h, p, w.Lk, a.window, a.ahead, a.sinks);   /* from this lane's first key */
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int e = 8 * (i / 4) + i % 4;
-                if ((e > last) | ((e < first) & (e >= sink))) s[i] = -INFINITY;
+                if ((e > span.last) | ((e < span.first) & (e >= span.sink))) s[i] = -INFINITY;
             }
         }
         float top = s[0];

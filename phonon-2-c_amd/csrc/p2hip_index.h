@@ -43,6 +43,22 @@ P2_HD bool key_visible(int j, int p, int window, int ahead, int sinks)
     return j - p <= ahead && (p - j < window || j < sinks);
 }
 
+/* The same for the keys from k0 on: k0 + e, below Lk, is visible iff e <= last and (e >= first or e < sink). No key stands
+ * before place 0, so that neither does the window's first: with blocks of a tile (k0 <= p + 127 + ahead) nothing here leaves
+ * 32 bits. */
+struct KeySpan {
+    int last, first, sink;
+};
+
+P2_HD KeySpan key_span(int k0, int p, int Lk, int window, int ahead, int sinks)
+{
+    return KeySpan{imin(p + ahead, Lk - 1) - k0, imax(p - window + 1, 0) - k0, sinks - k0};
+}
+
+/* The last key that the queries at places p and on all see (apart from where their windows begin); p may lie behind the
+ * last place. */
+P2_HD int last_seen_by_all(int p, int Lk, int ahead) { return imin(Lk - 1, imin(p, Lk - 1) + ahead); }
+
 /* Part s of `splits` of `total` blocks: [begin, end). */
 P2_HD void split_range(int total, int splits, int s, int *begin, int *end)
 {

@@ -147,3 +147,49 @@ def test_rule_for_few_queries(tmp_path):
                     "-I", CSRC, "-o", str(exe), str(src)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
+
+
+SPANS = r"""
+#include <cstdio>
+#include <initializer_list>
+#include "p2hip_index.h"
+using namespace p2k;
+#define CHECK(c) do { if (!(c)) { printf("line %d: %s\n", __LINE__, #c); return 1; } } while (0)
+
+int main()
+{
+    const int all = 1 << 30, big = all - 1;
+    /* places from the first query of 2^30 - 1 without a key to the last key of 2^30 - 1, at every end of the limits */
+    const int ps[] = {-big, -big + 1, -130, -1, 0, 1, 77, big - 130, big - 2, big - 1}, ks[] = {0, 28, 64, 4096, big - 130, big - 63, big + 3};
+    for (int Lk : {1, 200, big})
+        for (int window : {1, 64, big, all})
+            for (int ahead : {0, 5, big, all})
+                for (int sinks : {0, 7, all})
+                    for (int p : ps) {
+                        if (p >= Lk) continue;
+                        for (int k0 : ks) {
+                            if (k0 > (long long)p + 127 + ahead) continue;   /* no query of the tile sees the block */
+                            const KeySpan s = key_span(k0, p, Lk, window, ahead, sinks);
+                            for (int e = 0; e < 64 && k0 + e < Lk; e++)
+                                CHECK(key_visible(k0 + e, p, window, ahead, sinks) == (e <= s.last && (e >= s.first || e < s.sink)));
+                            CHECK(k0 < Lk || s.last < 0);
+                        }
+                        for (int more : {0, 32, 96}) {
+                            const int to = last_seen_by_all(p + more, Lk, ahead);
+                            CHECK(to < Lk);
+                            if (p + more < Lk && to >= 0) CHECK((long long)to - (p + more) <= ahead && (to == Lk - 1 || (long long)to + 1 - (p + more) > ahead));
+                        }
+                    }
+    puts("ok");
+    return 0;
+}
+"""
+
+
+def test_key_spans(tmp_path):
+    src, exe = tmp_path / "spans.cpp", tmp_path / "spans"
+    src.write_text(SPANS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                    "-I", CSRC, "-o", str(exe), str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
