@@ -375,8 +375,8 @@ enum { P2H_F32 = 0, P2H_F16 = 1, P2H_BF16 = 2 };
 /* A device-resident weight [K, N] of 4-bit codes with a scale, and if wanted a zero point, for every `group` (32, 64
  * or 128) of its rows: w[k][n] = (code[k][n] − zero[k / group][n]) · scale[k / group][n], zero 8 where there are no
  * zero points. codes [K][ceil(N / 2)]: column n in the low (n even) or high half of byte n / 2; scales fp16 bits
- * [ceil(K / group)][N]; zeros packed as the codes, [ceil(K / group)][ceil(N / 2)], or NULL. Any K and N >= 1 of up to 2^35
- * codes, N up to 2^27. */
+ * [ceil(K / group)][N]; zeros packed as the codes, [ceil(K / group)][ceil(N / 2)], or NULL. Any K from 1 to 2^28 and N from
+ * 1 to 2^27 with ceil(K / 128) · ceil(N / 16) below 2^24: up to 2^35 codes. */
 typedef struct P2hQ4Weight P2hQ4Weight;
 
 /* From host memory, or from device memory (read during the call only, on the calling thread's stream: what writes it on
@@ -390,7 +390,7 @@ int    p2h_q4_weight_shape(const P2hQ4Weight *w, int *K, int *N, int *group);
 size_t p2h_q4_weight_device_bytes(const P2hQ4Weight *w);
 
 /* Y [M][N] = alpha · X [M][K] · W + beta · Y for few rows (beta 0 does not read Y): a matrix-vector product per row,
- * the weight read once for every 16 rows. X and Y of type `dtype`, pitches ldx >= K and ldy >= N elements, no alignment
+ * the weight read and decoded once for every 16 rows (at most 2^20 − 16 of them). X and Y of type `dtype`, pitches ldx >= K and ldy >= N elements, no alignment
  * beyond the element's (rows that are all 16-byte aligned load several times faster). A row's outputs are the same bits whatever M is. X and Y
  * must not overlap. A group's products are summed before its scale is applied: values of |x| from 2^118 up may overflow.
  * fp16 rows sum x · (code − zero); the others sum x · code and x · zero apart, in 32 bits: near a weight of 0 their errors
@@ -426,7 +426,8 @@ int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, co
  * query i of Lq stands at p = i + Lk − Lq. Key j is visible to it iff j <= p + ahead and (p − j < window or j <
  * sinks): `window` >= 1 places back, itself included, `ahead` >= 0 places on, and the first `sinks` >= 0 places (1 << 30
  * reaches everything). A query that sees no key gets zeros; rows outside every sequence are left as they were.
- * scale > 0. Fewer than 2^30 rows. O must not overlap the inputs. */
+ * scale > 0. Fewer than 2^30 rows, and (q_rows / 128 + 1 + n_seqs) · heads below 2^23 − 2^11. O must not overlap the
+ * inputs. A value of V that is not finite makes what sees it infinite or NaN. */
 int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const int *dQStart, const int *dKStart,
                          int heads, int kv_heads, int head_dim, const void *dQ, int ldq, const void *dK, int ldk,
                          const void *dV, int ldv, float scale, int window, int ahead, int sinks, void *dO, int ldo,
@@ -435,7 +436,7 @@ int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const in
 /* The same for one new token per sequence over a cache: query row s of dQ stands at the last of the dLen[s] tokens whose
  * pages are dTable[s · table_ld ..] (token t in page dTable[s · table_ld + t / page]); the visible keys are those with
  * len − 1 − t < window or t < sinks. Length 0 gives zeros; a length beyond table_ld · page (at most 2^30) counts as
- * that. Tokens of a page number outside [0, pages) are not seen. The keys of one sequence are split over workgroups
+ * that. Tokens of a page number outside [0, pages) are not seen. At most 65536 sequences, n_seqs · heads below 2^23. The keys of one sequence are split over workgroups
  * where there are few sequences, planned for lengths up to max_len (other lengths are right as well), and a second
  * kernel joins the parts kept in the workspace, p2h_attention_paged_workspace_bytes(...) bytes, 16-byte aligned (0: the
  * call does not split). Without a workspace (NULL) it runs unsplit. Calls sharing a workspace are stream-ordered. dO

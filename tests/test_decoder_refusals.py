@@ -139,6 +139,21 @@ def test_rope_and_its_cache(kw, part):
     refused(rope(**kw), part)
 
 
+@pytest.mark.parametrize("kw,part", [(dict(K=(1 << 28) + 1), "K ="), (dict(N=(1 << 27) + 1, K=1), "too large"),
+                                     (dict(K=1 << 28, N=16 * 8), "too large"), (dict(K=128 << 12, N=16 << 12), "too large")])
+def test_q4_weight_limits(kw, part):
+    """K to 2^28, N to 2^27, ceil(K / 128) · ceil(N / 16) below 2^24."""
+    test_q4_weight("p2h_q4_weight_wrap", kw, part)
+
+
+def test_launch_limits():
+    """As the header states them: (q_rows / 128 + 1 + n_seqs) · heads below 2^23 − 2^11; n_seqs · heads below 2^23."""
+    far = dict(q=1 << 45, k=1 << 46, v=1 << 47, o=1 << 48)
+    refused(win(n=(1 << 21) - 512 - 1, qs=A, ks=A, **far), "too many")
+    refused(win(n=(1 << 21) - 512 - 2, qs=A, ks=A, **dict(far, o=(1 << 45) + 16)), "dO overlaps dQ")
+    refused(paged(cache(dK=1 << 50, dV=1 << 51), n=65536, heads=128, q=1 << 45, ldq=8192, o=1 << 47, ldo=8192), "too many")
+
+
 def test_rope_of_one_row_in_place():
     """A single row has no pitch: in place whatever pitches are given. That it passes is seen by what is refused next."""
     last = dict(cache=cache(dK=8 * A, dV=A + 1024 - 16), slots=A)   # the cache's values on the row's end
