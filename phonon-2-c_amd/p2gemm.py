@@ -880,12 +880,13 @@ def block_workspace_bytes(mode, T):
 # Device-pointer entry points, asynchronous on `stream`; dtype "f32", "f16" or "bf16" is the type of every row and cache.
 
 class Q4Weight:
-    """A device-resident weight [K, N] of 4-bit codes [K, ceil(N/2)] with fp16 scales [ceil(K/group), N] and, if given,
-    zero points packed as the codes, uploaded from host arrays."""
+    """A device-resident weight [K, N] of 4-bit codes [K, ceil(N/2)] with fp16 scales [ceil(K/group), N] (or their bits as
+    uint16) and, if given, zero points packed as the codes, uploaded from host arrays."""
 
     def __init__(self, codes, scales, zeros, K, N, group):
         c = np.ascontiguousarray(codes, np.uint8)
-        s = np.ascontiguousarray(scales, np.float16)
+        s = np.ascontiguousarray(scales)
+        s = s.view(np.float16) if s.dtype == np.uint16 else s.astype(np.float16)
         z = None if zeros is None else np.ascontiguousarray(zeros, np.uint8)
         groups, half = -(-K // group), (N + 1) // 2
         assert c.size == K * half and s.size == groups * N and (z is None or z.size == groups * half)

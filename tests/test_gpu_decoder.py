@@ -173,6 +173,16 @@ def test_q4_codes_at_their_zero_point(t):
     D.check(got, np.zeros((4, N)), D.q4_bound(t, D.to_f64(t, x), both, np.zeros((4, N)), 1.0, K) + D.HALF[t] * np.abs(got), t)
 
 
+def test_q4_scales_as_bits():
+    """fp16 scales given as uint16 are their bits, as in the C header, not numbers."""
+    K, N, group = 100, 24, 32
+    rng = rng_of("bits")
+    codes, scales, zeros = D.q4_weight(rng, K, N, group, True)
+    x = D.rows(rng, "f32", 2, K)
+    want = D.run_q4("f32", x, (codes, scales, zeros), K, N, group)
+    assert np.array_equal(D.run_q4("f32", x, (codes, scales.view(np.uint16), zeros), K, N, group), want)
+
+
 def test_q4_bytes_and_wrap():
     K, N, group = 1024, 256, 128
     rng = rng_of("wrap")
