@@ -792,6 +792,18 @@ template <class E, int DH, int KB, int NW> struct BlockLoads {
  * Sums carry the same factor, so that it leaves with the division. bf16 ends where fp32 does and needs none. */
 template <int DT> constexpr float kLift = DT == T_F16 ? 15.0f : 0.0f;
 
+/* A score's place less the lift. In two instructions: as one, the constant or c would take a register of its own, which
+ * attention_page of fp16 heads of 128 does not have (8 bytes a lane in scratch). */
+__device__ __forceinline__ float lifted(float score, float c, float lift)
+{
+    float x = score * c;
+    if (lift != 0.0f) {
+        asm("" : "+v"(x));
+        x -= lift;
+    }
+    return x;
+}
+
 /* attention_win raises its reference only where the exponentials of a block have a sum above kWinSlack in some lane: then
  * to the largest score so far, and they are taken again. It is not raised otherwise, so that most blocks need no maximum
  * and leave O as it is: a weight stays below the slack, which every type holds, and relative to their sum nothing changes.
@@ -932,7 +944,7 @@ __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
             for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) top = fmaxf(top, u.s[n][i]);
-            const float mn = fmaxf(u.m, __builtin_fmaf(max_halves(top), a.c, -kWinLift<DT>)), mu = mn == -INFINITY ? 0.0f : mn;
+            const float mn = fmaxf(u.m, lifted(max_halves(top), a.c, kWinLift<DT>)), mu = mn == -INFINITY ? 0.0f : mn;
             const float fade = exp2_fast(u.m - mu);
             u.m = mn;
             u.l *= fade;
@@ -1230,7 +1242,7 @@ __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / 
     const int lane = threadIdx.x & 63, g = lane >> 4, x16 = lane & 15;
     if (b >= end) return;
     auto soften = [&](float top) __attribute__((always_inline)) {
-        const float mn = fmaxf(st.m, __builtin_fmaf(max_quarters(top), c, -kLift<DT>)), mu = mn == -INFINITY ? 0.0f : mn;
+        const float mn = fmaxf(st.m, lifted(max_quarters(top), c, kLift<DT>)), mu = mn == -INFINITY ? 0.0f : mn;
         const float fade = exp2_fast(st.m - mu);
         st.m = mn;
         return float2{mu, fade};

@@ -131,3 +131,12 @@ def test_exact_kernels_do_not_spill():
     assert len(kernels) >= 6, sorted(kernels)
     spills = {n: k[".private_segment_fixed_size"] for n, k in kernels.items() if k[".private_segment_fixed_size"]}
     assert not spills, spills
+
+
+def test_decoder_kernels_do_not_spill():
+    """The decoder step's kernels stand close to their registers' bounds and keep everything in them."""
+    names = ("attention_win", "attention_page", "attention_join", "q4_gemv", "qk_norm_rope")
+    kernels = {n: k for n, k in _kernel_metadata(P.HIP_SO).items() if any(a in n for a in names)}
+    assert len(kernels) >= 40, sorted(kernels)
+    spills = {n: k[".private_segment_fixed_size"] for n, k in kernels.items() if k[".private_segment_fixed_size"]}
+    assert not spills, spills
