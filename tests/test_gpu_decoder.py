@@ -893,6 +893,19 @@ def test_a_refused_allocation_is_reported_once():
     P.q4_gemv_dev("f32", 2, N, K, 1.0, dx.ptr, K, w, 0.0, dy.ptr, N)
 
 
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("H,Dh,starts", ((2, 64, True), (32, 128, False), (48, 64, True)))
+def test_window_without_keys(t, H, Dh, starts):
+    """No key rows at all, and then no pointers to any: zeros in both forms."""
+    n = 700 if H > 2 else 40
+    q = D.rows(rng_of(t, H, "no keys"), t, n, H * Dh)
+    dq, do = D.device(q), D.preset(t, (n, H * Dh))
+    qs, ks = D.device(np.array([0, 0, n], np.int32)), D.device(np.zeros(3, np.int32))
+    P.attention_window_dev(t, n, 0, 2 if starts else 1, qs.ptr if starts else None, ks.ptr if starts else None, H, H, Dh, dq.ptr,
+                           H * Dh, None, 0, None, 0, 0.1, EVERY, EVERY, 5, do.ptr, H * Dh)
+    assert not D.to_f64(t, do.download((n, H * Dh), D.np_type(t))).any()
+
+
 # ── many sequences of few queries ───────────────────────────────────────────────────────────────────────────────
 
 @pytest.mark.parametrize("t", D.TYPES)
