@@ -829,17 +829,21 @@ template <int DH> struct WinSub {
  * keys of one query: the sum of its weights needs one exchange with the lane 32 away, at the end, and the weights are
  * already laid out as the operand of O^T += V^T·P^T, whatever order that product takes the keys in, as V's operand reads
  * the same order out of LDS. The exponentials are rounded to the rows' type for that product and summed unrounded in 32
- * bits.
+ * bits: against 64 bits the output is off by 0.0021 (bf16, relative 2-norm; fp16 2.6e-4), of which rounding it makes 0.0016
+ * (2.0e-4). A second product with what the rounding left brings it down to that, at 148 us instead of 116 (6000 rows as
+ * below) and 166 instead of 110 (ragged prompts, heads of 64), so one product it is.
  *
- * A block's exponentials take the vector unit about as long as its products take the matrix unit: two workgroups a CU put
- * two waves on each SIMD, of which one can multiply while the other takes exponentials. For that a wave's products are
+ * A block's exponentials take the vector unit about as long as its products take the matrix unit: two workgroups a CU (heads
+ * of 64, whose registers are fewer: three) put two waves on each SIMD, of which one can multiply while the other takes exponentials. For that a wave's products are
  * one stretch without waits: the scores of block b together with the output product of block b − 1, in QR equal stages,
  * each stage's operands read from LDS two stages ahead, and one of the loads of K of block b + 1 and V of block b issued
  * in each (all at once they would wait for each other: a CU takes 64 bytes a cycle). One barrier a block: there the loads
  * of the block before have come, and everyone is done with what the next ones overwrite.
  *
  * 6000 bf16 rows of 32 heads of 128 (8 key heads), window 1024: 113 us, 0.82 PFLOP/s of visible pairs (a large product
- * reaches 1.2); the matrix unit is busy 42 % of the time, the exponentials and what belongs to them about as long. */
+ * reaches 1.2). For 85 % of that the SIMDs have a wave; of this the matrix unit is busy 51 %, the vector unit 49 %, together
+ * the whole: the two waves hardly overlap. The LDS is busy 26 %. Heads of 64 (ragged prompts): 81 %, of which 48, 73 and 36 %
+ * (a third of that conflicts: their K rows of 128 bytes are placed as rows of 256). */
 template <int DT, int DH>
 __global__ __launch_bounds__(256, 2) void attention_win(WinArgs a)
 {
@@ -1226,11 +1230,15 @@ template <int DT, int DH> struct FewRows {
  *
  * A wave has nothing else to do while it waits for memory, so what the next block of 16-bit rows needs is requested as soon
  * as the registers are free: its keys behind the products with this block's, its values once these lie in LDS. fp32 rows
- * take the matrix unit eight times as long and have no registers left for that. place_of(b, hint(b)) says
- * where a block lies, from what hint read (a page table's entries) a block earlier. The last block has code of its own, as
- * the wait for a load that may or may not have been followed by others is a wait for all of them. seen(p, k) says whether this lane's
- * query sees key k of the block at p, and kept(p, k) whether V row k enters the product at all; neither is asked where
- * p.whole. CLEAN: infinities and NaN in V are put aside there, which `odd` notes. */
+ * take the matrix unit eight times as long and wait for each block instead: requests ahead did not fit the 168 registers
+ * that three waves a SIMD leave (a workgroup of eight waves is two a SIMD, so that heads of 128 could be given 256).
+ * place_of(b, hint(b)) says where a block lies, from what hint read (a page table's entries) a block earlier. The last block
+ * has code of its own, as the wait for a load that may or may not have been followed by others is a wait for all of them.
+ * seen(p, k) says whether this lane's query sees key k of the block at p, and kept(p, k) whether V row k enters the product
+ * at all; neither is asked where p.whole. CLEAN: infinities and NaN in V are put aside there, which `odd` notes.
+ *
+ * 16-bit weights are rounded for their product with V, as attention_win says; a second product with the rest would cost 2 to
+ * 9 % (32 sequences of 8192 bf16 tokens 187 -> 190 us, 16 of 1000 18.5 -> 20.2). */
 template <int DT, int DH, bool CLEAN, class Hint, class PlaceOf, class Seen, class Kept>
 __device__ __forceinline__ void few_blocks(FewState<DH> &st, const u4 (&q)[DH / (4 * kPer16<DT>)], float c, int b, int end,
                                            int step, int ldk, int ldv, Hint hint, PlaceOf place_of, Seen seen, Kept kept,
