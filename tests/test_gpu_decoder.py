@@ -953,3 +953,107 @@ def test_paged_fp32_on_the_whole(split, Dh, lens, H, Hk, page, window, sinks):
     got = D.run_paged("f32", q, kc, vc, table, lens, H, Dh ** -0.5, window, sinks, split, 40000 if split else None)
     off = D.norm_off(got.astype(np.float64), want)
     assert off <= D.ATTENTION_NORM, off / D.FP32
+
+
+# ── calls that the documentation allows ─────────────────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("H,Hk,Dh", ((2, 1, 64), (32, 8, 128)))
+def test_window_in_a_graph_sees_new_starts(t, H, Hk, Dh):
+    """A captured call reads its sequences' starts when it is replayed, in both forms; eager work lies between replays."""
+    n = 600
+    q, k, v, _, _ = window_case(t, (n,), 0, H, Hk, Dh, "graph")
+    dq, dk, dv = D.device(q), D.device(k), D.device(v)
+    dqs, dks = D.device(np.zeros(4, np.int32)), D.device(np.zeros(4, np.int32))
+    do, s = D.preset(t, (n, H * Dh)), P.Stream()
+    with P.Graph(s) as g:
+        P.attention_window_dev(t, n, n, 3, dqs.ptr, dks.ptr, H, Hk, Dh, dq.ptr, H * Dh, dk.ptr, Hk * Dh, dv.ptr, Hk * Dh, 0.1,
+                               90, 2, 3, do.ptr, H * Dh, s.ptr)
+    for qs, ks in (([0, 200, 200, 600], [0, 150, 300, 600]), ([5, 6, 300, 333], [0, 0, 600, 600]), ([0, 0, 0, 600], [1, 2, 3, 599])):
+        dqs.upload(np.array(qs, np.int32))
+        dks.upload(np.array(ks, np.int32))
+        do.upload(np.full(do.nbytes, 0xFF, np.uint8))
+        P.sync()
+        g.launch()
+        s.sync()
+        eager = D.run_window(t, q, k, v, H, Hk, Dh, 0.1, 90, 2, 3, qs, ks)
+        assert np.array_equal(do.download((n, H * Dh), D.np_type(t)).view(np.uint16), eager.view(np.uint16)), (qs, ks)
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_paged_sequences_share_pages(t):
+    """A page may stand in several sequences' rows, and more than once in one: the bits of pages of their own."""
+    H, Hk, Dh, page, lens = 8, 2, 64, 16, (150, 150, 70)
+    q, kc, vc, table = paged_case(t, lens, H, Hk, page, Dh, "share")
+    table[1, :6] = table[0, :6]
+    table[2, 1] = table[2, 2] = table[0, 3]
+    own, k2, v2 = table.copy(), [kc], [vc]
+    at = kc.shape[0]
+    for s in range(3):
+        for p in range(-(-lens[s] // page)):
+            k2.append(kc[table[s, p]:table[s, p] + 1])
+            v2.append(vc[table[s, p]:table[s, p] + 1])
+            own[s, p] = at
+            at += 1
+    k2, v2 = np.concatenate(k2), np.concatenate(v2)
+    for split in (False, True):
+        a = D.run_paged(t, q, kc, vc, table, lens, H, 0.1, EVERY, 0, split, 40000)
+        b = D.run_paged(t, q, k2, v2, own, lens, H, 0.1, EVERY, 0, split, 40000)
+        assert np.array_equal(a.view(np.uint16), b.view(np.uint16))
+
+
+def test_layers_on_two_threads():
+    """Two host threads, each with its stream and its buffers, at once: the results of one after the other."""
+    import threading
+    t, B, S = "bf16", 2, 10
+    xs = D.rows(rng_of("threads"), t, S, B, Layer.C)
+
+    def run(seed, out):
+        L, s = Layer(t, B, 2, seed), P.Stream()
+        got = []
+        for n in range(S):
+            L.place(xs[n], np.full(B, n))
+            P.sync()
+            L.step(s.ptr)
+            got.append(L.out(s.ptr))
+        out.append(np.stack(got))
+
+    alone, both = [[], []], [[], []]
+    for i, seed in enumerate(("one", "two")):
+        run(seed, alone[i])
+    threads = [threading.Thread(target=run, args=(seed, both[i])) for i, seed in enumerate(("one", "two"))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for a, b in zip(alone, both):
+        assert len(b) == 1 and np.array_equal(a[0], b[0])
+
+
+@pytest.mark.parametrize("t,M", (("bf16", 1), ("f32", 1), ("f16", 3)))
+def test_q4_weight_beyond_32_bits(t, M):
+    """A weight of nearly 2^35 codes, its records past 2^32 bytes: the rows and columns at its ends."""
+    K, N, group = 1 << 18, 131056, 128
+    half, groups = N // 2, K // group
+    dc, ds = P.DeviceBuffer(K * half), P.DeviceBuffer(groups * N * 2)
+    for b, byte in ((dc, 0x99), (ds, 0x3C)):   # code 9, less 8, by the fp16 of bits 0x3C3C
+        assert P.hip().p2h_memset(b.ptr, byte, b.nbytes, None) == 0
+    P.sync()
+    scale = float(np.array([0x3C3C], np.uint16).view(np.float16)[0])
+    rows, rng = (0, 1, K // 2 + 5, K - 1), rng_of("beyond")
+    w = np.full((len(rows), N), 1.0)
+    for i, r in enumerate(rows):   # these rows have codes of their own in the last and the first 64 columns
+        for c0 in (0, half - 32):
+            codes = rng.integers(0, 256, 32, dtype=np.uint8)
+            dc.upload(codes, offset=r * half + c0)
+            w[i, 2 * c0:2 * c0 + 64] = D.nibbles(codes[None], 64)[0] - 8.0
+    weight = P.Q4Weight.wrap(dc.ptr, ds.ptr, None, K, N, group)
+    del dc, ds
+    x = np.zeros((M, K))
+    x[:, rows] = rng.integers(1, 4, (M, len(rows)))
+    dx, dy = D.device(D.to_type(t, x)), D.preset(t, (M, N))
+    P.q4_gemv_dev(t, M, N, K, 1.0, dx.ptr, K, weight, 0.0, dy.ptr, N)
+    got = D.to_f64(t, dy.download((M, N), D.np_type(t)))
+    want = x[:, rows] @ w * scale
+    assert np.array_equal(got, D.to_f64(t, D.to_type(t, want)))   # sums of small whole numbers, one scale each group: exact
+    weight.free()
