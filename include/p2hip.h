@@ -357,12 +357,13 @@ int    p2h_conformer_stack(int mode, const P2hBlock *blocks, int n_blocks, int T
 
 /* ── a decoder layer's step: 4-bit linears, head norms with rotation, attention over many or cached keys ──────────
  *  No counterpart in the reference, whose decoder is an LSTM: for callers that put a text decoder with attention behind
- *  the encoder. (The encoder's own attention adds a relative-position product, which these do not have.) Rows are as everywhere here (row-major,
- *  heads side by side, head h at columns head_dim·h; fused q | k | v rows as the block's qkv linear makes them), but of
- *  any of three element types, one type for all the rows and caches of a call. Sums, softmax statistics, norms and
- *  states are held in 32 bits and outputs rounded once. 16-bit attention also rounds each softmax weight to the type, for
- *  its product with V (not for the sum that it is divided by): half a step of the weight; fp16 keeps weights down to 2^-31
- *  of the query's largest. Weighted sums are divided at the end: values of V from 2^90 up may overflow on the way.
+ *  the encoder. (The encoder's own attention adds a relative-position product, which these do not have.) Rows are as
+ *  everywhere here (row-major, heads side by side, head h at columns head_dim·h; fused q | k | v rows as the block's qkv
+ *  linear makes them), but of any of three element types, one type for all the rows and caches of a call. Sums, softmax
+ *  statistics, norms and states are held in 32 bits and outputs rounded once. 16-bit attention also rounds each softmax
+ *  weight to the type, for its product with V (not for the sum that it is divided by): half a step of the weight; fp16
+ *  keeps weights down to 2^-31 of the query's largest. Weighted sums are divided at the end: values of V from 2^90 up may
+ *  overflow on the way.
  *
  *  Query heads are shared evenly: query head h reads key head h / (heads / kv_heads). head_dim is 64 or 128. Pointers
  *  to rows and caches are 16-byte aligned and row pitches whole multiples of 16 bytes, below 2^23 elements, unless an
