@@ -636,9 +636,10 @@ template <int DT> __device__ __forceinline__ float odd_sum(u4 v, float sum)
 {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if constexpr (DT == T_F32) sum = __builtin_fmaf(__uint_as_float(v[i]), 0.0f, sum);
-        else if constexpr (DT == T_F16) sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, v[i]), h2{0, 0}, sum, false);
-        else sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, v[i]), b2{0, 0}, sum, false);
+        const uint32_t w = v[i];   /* a bit cast of v[i] itself takes element 0, whatever i */
+        if constexpr (DT == T_F32) sum = __builtin_fmaf(__uint_as_float(w), 0.0f, sum);
+        else if constexpr (DT == T_F16) sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{0, 0}, sum, false);
+        else sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{0, 0}, sum, false);
     }
     return sum;
 }

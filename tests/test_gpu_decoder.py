@@ -1057,3 +1057,21 @@ def test_q4_weight_beyond_32_bits(t, M):
     want = x[:, rows] @ w * scale
     assert np.array_equal(got, D.to_f64(t, D.to_type(t, want)))   # sums of small whole numbers, one scale each group: exact
     weight.free()
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("lens,H", (((90,), 2), ((1200,), 32)))
+def test_window_single_values_that_are_not_finite(t, lens, H):
+    """One infinity or NaN in a value, at any of the places of the 16 bytes that are looked at together: it reaches that
+    dimension of the queries that see it, and nothing else."""
+    Hk, Dh, window = 1, 64, 10
+    q, k, v, qs, ks = window_case(t, lens, 0, H, Hk, Dh, "single")
+    clean = D.to_f64(t, D.run_window(t, q, k, v, H, Hk, Dh, 0.125, window, 0, 0, qs, ks)).reshape(-1, H, Dh)
+    for d in range(16):
+        at, v2 = 30 + d, v.copy()
+        v2[at, 16 + d] = D.to_type(t, np.array([(np.inf, np.nan, -np.inf)[d % 3]]))[0]
+        got = D.to_f64(t, D.run_window(t, q, k, v2, H, Hk, Dh, 0.125, window, 0, 0, qs, ks)).reshape(-1, H, Dh)
+        odd = np.zeros(got.shape, bool)
+        odd[at:at + window, :, 16 + d] = True
+        assert np.array_equal(~np.isfinite(got), odd), (t, d)
+        assert np.array_equal(got[~odd], clean[~odd]), (t, d)
