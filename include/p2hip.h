@@ -448,6 +448,88 @@ int p2h_attention_paged(const P2hKvCache *cache, int n_seqs, int heads, const vo
                         int table_ld, const int *dLen, int max_len, float scale, int window, int sinks, void *dO,
                         int ldo, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ── a served batch's step: an 8-bit cache, shared prefixes, adapters ───────────────────────────────────────────────
+ *  No counterpart in the reference. What is said of the step above holds here too (types, rows, heads, alignment, device
+ *  arrays, streams); sums, softmax statistics and scales are 32-bit and outputs are rounded once. */
+
+/* Keys and values kept as 8-bit codes with one scale for every token's head: value = code · scale. K and V each
+ * [pages][heads][page][head_dim], two's complement, −127 .. 127; KScale and VScale each [pages][heads][page]. Pages and
+ * slots are those of P2hKvCache, and nothing in a page needs a value before it is written. Half the memory of 16-bit rows
+ * (head_dim + 4 bytes a head). */
+typedef struct P2hKvCacheQ8 {
+    int heads, head_dim, page, pages;
+    void *K, *V;                /* 16-byte aligned */
+    float *KScale, *VScale;
+} P2hKvCacheQ8;
+
+/* p2h_qk_norm_rope with the keys and values put into an 8-bit cache: scale = a / 127 and code = round-half-even(x · (127 /
+ * a)), a the largest |x| of the head; keys are taken as they are in 32 bits, before any rounding to the rows' type. A value is
+ * off by at most half a scale. A head whose a is below 2^-100 is kept as zeros, one with a value that is not finite as a NaN
+ * (its scale). `cache` is not NULL; everything else is as there. */
+int p2h_qk_norm_rope_q8(int dtype, int T, int heads, int kv_heads, int head_dim, const void *dQKV, int ldqkv,
+                        const float *dGammaQ, const float *dGammaK, float eps, int rot, int interleaved,
+                        const float *dFreq, const int *dPos, void *dQ, int ldq, void *dK, int ldk,
+                        const P2hKvCacheQ8 *cache, const int *dSlots, void *stream);
+
+/* Kept keys and values as rows, for p2h_attention_window over a prompt's next rows and all before them: sequence s's tokens 0,
+ * 1, … (through its pages dTable[s · table_ld ..], as in p2h_attention_paged) become the rows dStart[s] .. dStart[s + 1] − 1
+ * of dK (pitch ldk) and dV (pitch ldv), heads side by side, code · scale rounded to the type. dStart does not descend and
+ * lies inside [0, rows]. Tokens beyond the table, or of a page number outside [0, pages), become zeros; rows of no sequence
+ * are left as they were. Fewer than 2^30 rows, at most 65536 sequences. dK, dV and the cache do not overlap. */
+int p2h_kv_rows_q8(int dtype, const P2hKvCacheQ8 *cache, int rows, int n_seqs, const int *dStart, const int *dTable,
+                   int table_ld, void *dK, int ldk, void *dV, int ldv, void *stream);
+
+/* p2h_attention_paged over an 8-bit cache, queries and outputs of type `dtype`: o = Σ w · scale_v · code_v / Σ w, w the softmax
+ * weights of scale · scale_k · (q · code_k). Codes are exact in the products; a weight times its value's scale is rounded to
+ * 8 bits for bf16 rows, to 16 for fp16 rows, and not at all for fp32 rows, whose queries of less than 2^-110 have fewer bits. */
+size_t p2h_attention_paged_q8_workspace_bytes(const P2hKvCacheQ8 *cache, int n_seqs, int heads, int max_len, int window,
+                                              int sinks);
+int p2h_attention_paged_q8(int dtype, const P2hKvCacheQ8 *cache, int n_seqs, int heads, const void *dQ, int ldq,
+                           const int *dTable, int table_ld, const int *dLen, int max_len, float scale, int window,
+                           int sinks, void *dO, int ldo, void *workspace, size_t workspace_bytes, void *stream);
+
+/* p2h_attention_paged for sequences that come in groups which share a prefix, whose keys are read once for the group: group g
+ * is the sequences dGroup[g] .. dGroup[g + 1] − 1 (starts that do not descend, inside [0, n_seqs]) and shares its first
+ * dShared[g] tokens, which are found through the table row of the group's first sequence; behind them each sequence has its
+ * own row's. Lengths dLen count from the first token, prefix included; one that ends inside the prefix sees that much of it.
+ * dShared may be 0, end inside a page, and lie beyond a length. The outputs of sequences of no group are left as they were.
+ * max_shared and max_own plan the work: the longest prefix and the most tokens that a sequence has behind one; other
+ * numbers are right as well. The workspace is needed: p2h_attention_shared_workspace_bytes(...) bytes, 16-byte aligned;
+ * calls sharing it are stream-ordered. dO and the workspace overlap nothing the call reads, nor each other. */
+size_t p2h_attention_shared_workspace_bytes(const P2hKvCache *cache, int n_seqs, int n_groups, int heads, int max_shared,
+                                            int max_own, int window, int sinks);
+int p2h_attention_shared(const P2hKvCache *cache, int n_seqs, int n_groups, int heads, const void *dQ, int ldq,
+                         const int *dGroup, const int *dShared, const int *dTable, int table_ld, const int *dLen,
+                         int max_shared, int max_own, float scale, int window, int sinks, void *dO, int ldo,
+                         void *workspace, size_t workspace_bytes, void *stream);
+/* The same over an 8-bit cache. */
+size_t p2h_attention_shared_q8_workspace_bytes(const P2hKvCacheQ8 *cache, int n_seqs, int n_groups, int heads,
+                                               int max_shared, int max_own, int window, int sinks);
+int p2h_attention_shared_q8(int dtype, const P2hKvCacheQ8 *cache, int n_seqs, int n_groups, int heads, const void *dQ,
+                            int ldq, const int *dGroup, const int *dShared, const int *dTable, int table_ld,
+                            const int *dLen, int max_shared, int max_own, float scale, int window, int sinks, void *dO,
+                            int ldo, void *workspace, size_t workspace_bytes, void *stream);
+
+/* `count` low-rank adapters of a linear [K, N], of type `dtype` in device memory: A [count][rank][K], B [count][N][rank],
+ * scale [count]. rank is 8, 16, 32, 64 or 128 (a lower one is filled up with zeros); A and B are 16-byte aligned. The memory
+ * is the caller's; adapters may be exchanged in it between calls. */
+typedef struct P2hAdapters {
+    int dtype, count, rank, K, N;
+    const void *A, *B;
+    const float *scale;
+} P2hAdapters;
+
+/* Y[m] = Z[m] + scale[i] · (X[m] · A[i]ᵀ) · B[i]ᵀ for every row m, i = dIndex[m]: what a row's own adapter adds to the linear that
+ * all rows share, whichever entry made Z. Z may be Y itself (same pitch; a single row has none) or NULL for zeros. A row whose
+ * index lies outside [0, count) has no adapter: Y[m] = Z[m]. X [M][K], Z and Y [M][N] of the adapters' type, no alignment
+ * beyond the element's (rows of X and K that are multiples of 16 bytes load several times faster). Products with A are
+ * summed in 32 bits, that sum and its products with B are 32-bit too. Neighbouring rows of one adapter share what is read
+ * of it, 16 at a time. At most 2^20 − 16 rows. The workspace is needed: p2h_adapters_workspace_bytes(...) bytes, 16-byte
+ * aligned; calls sharing it are stream-ordered. Apart from Z and Y nothing overlaps. */
+size_t p2h_adapters_workspace_bytes(const P2hAdapters *adapters, int M);
+int p2h_adapters_add(const P2hAdapters *adapters, int M, const void *dX, int ldx, const int *dIndex, const void *dZ,
+                     int ldz, void *dY, int ldy, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

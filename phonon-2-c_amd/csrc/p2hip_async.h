@@ -31,6 +31,20 @@ __device__ __forceinline__ void lds_barrier()
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+/* dma_16 from a base that is the same for all lanes and an offset of each, and the same of 4 bytes per lane (at lds +
+ * 4·lane) from an address of each */
+__device__ __forceinline__ void dma_16(const void *base, uint32_t offset, const void *lds)
+{
+    const uint32_t a = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(a)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void dma_4(const void *src, const void *lds)
+{
+    const uint32_t a = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(a) : "memory", "m0");
+}
+
 /* dma_16 through a buffer descriptor: a byte offset per lane from its base; lanes whose bytes end past its size read
  * nothing. */
 __device__ __forceinline__ void dma_16(__amdgpu_buffer_rsrc_t from, uint32_t offset, const void *lds)

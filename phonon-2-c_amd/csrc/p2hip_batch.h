@@ -1,0 +1,828 @@
+/*  p2hip_batch.h – gfx950 kernels of a served batch's step (included once, by p2hip_batch.hip).
+ *
+ *  Kernels:
+ *    kv_rows_q8      kept 8-bit keys and values back as rows
+ *    attend          one query per sequence over pages of rows or of 8-bit codes, prefixes of groups of sequences read once
+ *    attend_join     adds the parts of each query
+ *    adapter_shrink  rows times the first matrix of their adapters
+ *    adapter_expand  that times the second, added to the rows of the projection beside it
+ */
+#pragma once
+
+#include "p2hip_async.h"
+#include "p2hip_elem.h"
+#include "p2hip_index.h"
+
+namespace p2k {
+
+/* a word that is the same for all lanes, read through the scalar cache: vector loads would be waited for together with the
+ * direct loads into LDS that are on their way */
+__device__ __forceinline__ int scalar_int(const int *p)
+{
+    typedef __attribute__((address_space(4))) const int *c4;
+    return *(c4)(uintptr_t)p;
+}
+
+/* The last s of [0, n) with le(s), which holds up to some s and not behind it; −1 where it holds for none. 64 lanes look at
+ * once, so that up to 64 take one wait for memory and 4096 two. */
+template <class F> __device__ __forceinline__ int wave_last(int n, F le)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = n;
+    while (hi - lo > 64) {
+        const int step = (hi - lo + 63) / 64, s = lo + lane * step;
+        const int k = __popcll(__ballot(s < hi && le(s)));
+        lo += imax(k - 1, 0) * step;
+        hi = imin(lo + step, hi);
+    }
+    return lo + __popcll(__ballot(lo + lane < hi && le(lo + lane))) - 1;
+}
+
+/* ── an 8-bit cache read back ──────────────────────────────────────────────────────────────────────────────── */
+
+struct KvRowsArgs {
+    int rows, n_seqs, kv, page_shift, pages, table_ld, ldk, ldv, per;   /* per: rows a workgroup */
+    const int *start, *table;
+    const int8_t *kc, *vc;
+    const float *ks, *vs;
+    void *k, *v;
+};
+
+constexpr int kRowsMost = 32;   /* rows a workgroup at most */
+
+/* Rows `per` · blockIdx.x ..: where each row's token lies is looked up first, one thread a row; then 16 bytes of output a
+ * lane along the rows, K's heads and V's. Bound by memory. */
+template <int DT, int DH>
+__global__ __launch_bounds__(256) void kv_rows_q8(KvRowsArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int VE = kPer16<DT>, LPH = DH / VE;
+    __shared__ long long at[kRowsMost];   /* (page · kv << page_shift) + place; −1: no such token; −2: no sequence's row */
+    const int r0 = blockIdx.x * a.per, n = imin(a.per, a.rows - r0);
+    if (threadIdx.x < 64) {
+        auto begins = [&](int s) { return imin(imax(a.start[s], 0), a.rows); };
+        const int first = wave_last(a.n_seqs, [&](int s) { return begins(s) <= r0; });
+        const int last = wave_last(a.n_seqs, [&](int s) { return begins(s) <= r0 + n - 1; });
+        const int r = r0 + (int)threadIdx.x;
+        if (r < r0 + n) {
+            int s = first, end = last + 1;   /* the last sequence that begins at or before r is one of these */
+            while (end - s > 1) {
+                const int mid = (s + end) / 2;
+                if (begins(mid) <= r) s = mid;
+                else end = mid;
+            }
+            int qa = 0, qb = 0;
+            if (s >= 0) seq_rows(a.start, s, a.rows, &qa, &qb);
+            long long to = -2;
+            if (r < qb) {
+                const int t = r - qa;
+                const int page = page_in(page_entry(a.table + (size_t)s * a.table_ld, a.table_ld, t, a.page_shift), a.pages);
+                to = page < 0 ? -1 : (((long long)page * a.kv) << a.page_shift) + (t & ((1 << a.page_shift) - 1));
+            }
+            at[threadIdx.x] = to;
+        }
+    }
+    __syncthreads();
+    const int per_row = 2 * a.kv * LPH;
+    for (int u = threadIdx.x; u < n * per_row; u += 256) {
+        const int i = u / per_row, p = u % per_row, is_v = p >= a.kv * LPH, h = (is_v ? p - a.kv * LPH : p) / LPH, l = p % LPH;
+        const long long token = at[i];
+        if (token < -1) continue;
+        float v[VE];
+        if (token < 0) {
+#pragma unroll
+            for (int j = 0; j < VE; j++) v[j] = 0.0f;
+        } else {
+            const size_t head = (size_t)token + ((size_t)h << a.page_shift);
+            const float s = (is_v ? a.vs : a.ks)[head];
+            const int8_t *c = (is_v ? a.vc : a.kc) + head * DH + VE * l;
+            uint32_t w[VE / 4];
+            __builtin_memcpy(w, c, VE);
+#pragma unroll
+            for (int j = 0; j < VE; j++) v[j] = (float)(int8_t)(w[j / 4] >> (8 * (j % 4))) * s;
+        }
+        E *row = static_cast<E *>(is_v ? a.v : a.k) + (size_t)(r0 + i) * (is_v ? a.ldv : a.ldk) + (size_t)h * DH + VE * l;
+        *reinterpret_cast<u4 *>(row) = pack<DT>(v);
+    }
+}
+
+/* ── one query per sequence over pages ─────────────────────────────────────────────────────────────────────── */
+
+enum { C_ROWS = 0, C_Q8 = 1 };
+
+struct BatchArgs {
+    int n_seqs, n_groups, heads, kv, page_shift, pages, table_ld, ldq, ldo, window, sinks;
+    int p_tiles, p_parts, p_wgs;   /* of prefixes: tiles of query rows, parts of the keys, workgroups, first in the grid */
+    int q_groups, o_parts;         /* of what each sequence has alone: tiles of a key head's queries, parts */
+    float c;                       /* scale · log2 e */
+    const void *q, *kc, *vc;
+    const float *ks, *vs;
+    const int *table, *len, *group, *shared;   /* group: NULL without prefixes */
+    void *o;
+    float *part;   /* [sequence][head][p_parts + o_parts][DH + 2]: sums, reference, sum of weights; NULL: one part, straight to o */
+};
+
+/* A block of keys as it lies in a wave's LDS: rows of CH pieces of 16 bytes, brought by LD direct loads of RPL rows each.
+ * Pieces are moved within a row so that operand reads fall into different banks: k_place for 16 keys' reads of one piece,
+ * v_place for V's (16 bits: 32 bytes of 8 rows; codes: 64 bytes of 4 rows; fp32: whole rows). */
+template <int CK, int DT, int DH> struct KeptBlock {
+    static constexpr bool Q8 = CK == C_Q8, F32 = !Q8 && DT == T_F32;
+    static constexpr int KB = F32 ? 16 : 32, NB = KB / 16, RB = Q8 ? DH : F32 ? 4 * DH : 2 * DH, CH = RB / 16, RPL = 64 / CH,
+                         LD = KB / RPL, BYTES = KB * RB, STAGE = 2 * BYTES + (Q8 ? 256 : 0), LOADS = 2 * LD + Q8;
+    static __device__ __forceinline__ constexpr int k_place(int r, int p)
+    {
+        return p ^ (CH >= 16 ? r & 15 : (r / (16 / (CH < 16 ? CH : 16))) & (CH - 1));
+    }
+    static __device__ __forceinline__ constexpr int v_place(int r, int p)
+    {
+        if (F32) return p;
+        if (Q8) return CH == 8 ? p ^ (4 * ((r >> 1) & 1)) : p;
+        return p ^ (CH == 16 ? 2 * (r & 7) : 2 * ((r >> 1) & 3));
+    }
+    /* the key of a block that product t has in row m: a lane's results are rows 4g + i, of codes so that its four groups of
+     * lanes have neighbouring keys */
+    static __device__ __forceinline__ constexpr int key_of(int t, int m) { return 16 * t + (Q8 ? 4 * (m & 3) + (m >> 2) : m); }
+};
+
+/* the upper halves of two floats, of a in the lower half */
+__device__ __forceinline__ uint32_t upper_halves(float a, float b)
+{
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+
+/* byte j of w, a code, as a float */
+template <int J> __device__ __forceinline__ float code_at(uint32_t w) { return (float)(int8_t)(w >> (8 * J)); }
+
+/* eight codes as an operand of the 16-bit type; whole numbers up to 127 are exact in both */
+template <int DT> __device__ __forceinline__ u4 code_operand(uint32_t w0, uint32_t w1)
+{
+    u4 v;
+    auto two = [](float a, float b) {
+        if constexpr (DT == T_F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+        else return upper_halves(a, b);
+    };
+    v[0] = two(code_at<0>(w0), code_at<1>(w0));
+    v[1] = two(code_at<2>(w0), code_at<3>(w0));
+    v[2] = two(code_at<0>(w1), code_at<1>(w1));
+    v[3] = two(code_at<2>(w1), code_at<3>(w1));
+    return v;
+}
+
+/* Eight floats as NP bf16 operands that sum to them: the upper 16 bits of what is left after the ones before; of one or two
+ * the last is rounded. */
+template <int NP> __device__ __forceinline__ void bf16_pieces(const float (&x)[8], u4 (&p)[NP])
+{
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = x[i];
+#pragma unroll
+    for (int n = 0; n < NP; n++) {
+        if (n == NP - 1 && NP < 3) {
+            p[n] = pack<T_BF16>(v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[n][i] = upper_halves(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] -= __uint_as_float(__float_as_uint(v[i]) & 0xffff0000u);
+        }
+    }
+}
+
+/* What one workgroup takes: `rows` query rows from number r0 on, of the sequences from seq0 on, row r being query head kvh · G
+ * + r % G of sequence seq0 + r / G; of the keys [t0, t1) that the table row `pages` names, part `split` of `splits`. Its
+ * result is part `slot` of `parts`. */
+struct BatchItem {
+    int seq0, r0, rows, kvh, t0, t1, split, splits, slot, parts;
+    const int *pages;
+};
+
+template <int CK, int DT, int DH, int NQ, int NW> constexpr int attend_lds()
+{
+    constexpr int V = NW * 2 * KeptBlock<CK, DT, DH>::STAGE, J = NW * 16 * NQ * (DH + 2) * 4;
+    return V > J ? V : J;
+}
+
+template <int CK, int DT, int DH, int NQ, int NW>
+__device__ __forceinline__ void attend_item(const BatchArgs &a, const BatchItem &w, unsigned char *lds)
+{
+    typedef typename Elem<DT>::type E;
+    typedef KeptBlock<CK, DT, DH> B;
+    constexpr bool Q8 = B::Q8, F32 = B::F32;
+    constexpr int NB = B::NB, KB = B::KB, CH = B::CH, RPL = B::RPL, LD = B::LD, NT = DH / 16;
+    /* operands of a query: fp32 rows 16-byte pieces; 16-bit rows and codes one of 8 values for every 32 dimensions, codes of
+     * fp32 rows three bf16 pieces each */
+    constexpr int NP = Q8 && DT == T_F32 ? 3 : 1, QS = F32 ? DH / 16 : DH / 32;
+    constexpr int WP = !Q8 ? 1 : DT == T_F32 ? 3 : DT == T_F16 ? 2 : 1;   /* pieces of a weight times V's scale */
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, x16 = lane & 15;
+    const int G = a.heads / a.kv;
+
+    int len[NQ];
+    u4 q[NQ][QS][NP];
+    int least = 1 << 30, most = 0;
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int r = w.r0 + imin(16 * n + x16, w.rows - 1), seq = w.seq0 + r / G;
+        len[n] = a.pages ? kept_length(a.len[seq], a.table_ld, 1 << a.page_shift) : 0;
+        least = imin(least, len[n]);
+        most = imax(most, len[n]);
+        const E *row = static_cast<const E *>(a.q) + (size_t)seq * a.ldq + (size_t)(w.kvh * G + r % G) * DH;
+#pragma unroll
+        for (int s = 0; s < QS; s++) {
+            if constexpr (!Q8) {
+                q[n][s][0] = *reinterpret_cast<const u4 *>(row + kPer16<DT> * (4 * s + g));
+            } else {
+                const E *p = row + 64 * (s / 2) + 16 * g + 8 * (s % 2);   /* in the order of the codes' pieces */
+                if constexpr (DT == T_F32) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = p[i];
+                    bf16_pieces<3>(v, q[n][s]);
+                } else {
+                    q[n][s][0] = *reinterpret_cast<const u4 *>(p);
+                }
+            }
+        }
+    }
+    if (w.r0 / G != (w.r0 + w.rows - 1) / G) {
+#pragma unroll
+        for (int o = 1; o < 16; o *= 2) {
+            least = imin(least, __shfl_xor(least, o));
+            most = imax(most, __shfl_xor(most, o));
+        }
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+
+    /* blocks are counted from the one that t0 lies in */
+    const int tb = w.t0 & ~(KB - 1), end_key = imin(most, w.t1);
+    const KeyBlocks blocks = key_blocks(imax(least - a.window, w.t0) - tb, end_key - tb, imax(a.sinks - tb, 0), KB);
+    int b0, b1;
+    split_range(blocks.total, w.splits, w.split, &b0, &b1);
+
+    struct Place {
+        int k0;
+        bool there[NB], whole;
+    };
+    struct Entries {
+        int e[NB];
+    };
+    auto hint = [&](int b) __attribute__((always_inline)) {
+        Entries n;   /* pages hold a multiple of 16 tokens */
+#pragma unroll
+        for (int t = 0; t < NB; t++) {
+            const int i = (tb + blocks.at(b) * KB + 16 * t) >> a.page_shift;
+            n.e[t] = i < a.table_ld ? scalar_int(w.pages + i) : -1;
+        }
+        return n;
+    };
+    auto seen_by = [&](int key, int ln) __attribute__((always_inline)) {   /* of those in pages that are there */
+        return key >= w.t0 && key < imin(ln, w.t1) && (key >= ln - a.window || key < a.sinks);
+    };
+
+    unsigned char *const own = lds + wave * 2 * B::STAGE;
+    uint32_t koff[LD], voff[LD];   /* of this lane's 16 bytes from the first row of 16 */
+#pragma unroll
+    for (int x = 0; x < LD; x++) {
+        const int r = RPL * x + lane / CH;
+        koff[x] = (r & 15) * B::RB + 16 * B::k_place(r, lane % CH);
+        voff[x] = (r & 15) * B::RB + 16 * B::v_place(r, lane % CH);
+    }
+    auto fetch = [&](int b, const Entries &n, unsigned char *to) __attribute__((always_inline)) {
+        Place p;
+        p.k0 = tb + blocks.at(b) * KB;
+        p.whole = p.k0 >= w.t0 && p.k0 + KB <= imin(least, w.t1) && (p.k0 >= most - a.window || p.k0 + KB <= a.sinks);
+        size_t token[NB];
+#pragma unroll
+        for (int t = 0; t < NB; t++) {
+            const int key = p.k0 + 16 * t, page = page_in(n.e[t], a.pages);
+            p.there[t] = page >= 0 && key < end_key;
+            p.whole &= page >= 0;
+            token[t] = (((size_t)imax(page, 0) * a.kv + w.kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+        }
+        const unsigned char *kc = static_cast<const unsigned char *>(a.kc), *vc = static_cast<const unsigned char *>(a.vc);
+#pragma unroll
+        for (int x = 0; x < LD; x++) dma_16(kc + token[RPL * x / 16] * B::RB, koff[x], to + 1024 * x);
+        if constexpr (Q8) {   /* K's 32 scales and V's, in the order of a lane's results */
+            const int key = B::key_of(0, lane & 15);
+            dma_4((lane < 32 ? a.ks : a.vs) + (lane & 16 ? token[1] : token[0]) + key, to + 2 * B::BYTES);
+        }
+#pragma unroll
+        for (int x = 0; x < LD; x++) dma_16(vc + token[RPL * x / 16] * B::RB, voff[x], to + B::BYTES + 1024 * x);
+        return p;
+    };
+
+    f4 o[NQ][NT];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < NT; d++) o[n][d] = f4{0, 0, 0, 0};
+    }
+    bool odd = false;
+
+    int b = b0 + wave;
+    if (b < b1) {
+        Place now = fetch(b, hint(b), own), next = now;
+        Entries ahead = hint(imin(b + NW, b1 - 1));
+        int stage = 0;
+        auto block = [&](auto last) __attribute__((always_inline)) {
+            constexpr bool MORE = !decltype(last)::value;
+            const unsigned char *Ks = own + stage * B::STAGE, *Vs = Ks + B::BYTES;
+            if constexpr (MORE) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   /* what reads of the other stage brought */
+                next = fetch(b + NW, ahead, own + (stage ^ 1) * B::STAGE);
+                ahead = hint(imin(b + 2 * NW, b1 - 1));
+            }
+            wait_vm<(MORE ? B::LOADS : 0) + LD>();
+            f4 s[NQ][NB];
+#pragma unroll
+            for (int n = 0; n < NQ; n++)
+#pragma unroll
+                for (int t = 0; t < NB; t++) s[n][t] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < NB; t++) {
+                const int row = B::key_of(t, x16);
+                const unsigned char *kr = Ks + row * B::RB;
+                if constexpr (Q8) {
+#pragma unroll
+                    for (int x = 0; x < QS / 2; x++) {
+                        const u4 k = *reinterpret_cast<const u4 *>(kr + 16 * B::k_place(row, 4 * x + g));
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const u4 kf = code_operand<DT == T_F16 ? T_F16 : T_BF16>(k[2 * e], k[2 * e + 1]);
+#pragma unroll
+                            for (int n = 0; n < NQ; n++)
+#pragma unroll
+                                for (int p = 0; p < NP; p++)
+                                    s[n][t] = mfma16<DT == T_F16 ? T_F16 : T_BF16>(kf, q[n][2 * x + e][p], s[n][t]);
+                        }
+                    }
+                } else if constexpr (F32) {
+#pragma unroll
+                    for (int x = 0; x < QS; x++) {
+                        const u4 k = *reinterpret_cast<const u4 *>(kr + 16 * B::k_place(row, 4 * x + g));
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+#pragma unroll
+                            for (int n = 0; n < NQ; n++)
+                                s[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[e]),
+                                                                               __uint_as_float(q[n][x][0][e]), s[n][t], 0, 0, 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < QS; x++) {
+                        const u4 k = *reinterpret_cast<const u4 *>(kr + 16 * B::k_place(row, 4 * x + g));
+#pragma unroll
+                        for (int n = 0; n < NQ; n++) s[n][t] = mfma16<DT>(k, q[n][x][0], s[n][t]);
+                    }
+                }
+            }
+            f4 vs[NB];
+            if constexpr (Q8) {
+                const f4 *sc = reinterpret_cast<const f4 *>(Ks + 2 * B::BYTES);
+#pragma unroll
+                for (int t = 0; t < NB; t++) {
+                    const f4 ks = sc[4 * t + g];
+                    vs[t] = sc[8 + 4 * t + g];
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) s[n][t] *= ks;
+                }
+            }
+            float wt[NQ][4 * NB];
+            u4 pw[NQ][WP];
+#pragma unroll
+            for (int n = 0; n < NQ; n++) {
+                bool in[4 * NB];
+                if (!now.whole) {
+#pragma unroll
+                    for (int t = 0; t < NB; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            in[4 * t + i] = now.there[t] && seen_by(now.k0 + B::key_of(t, 4 * g + i), len[n]);
+                            if (!in[4 * t + i]) s[n][t][i] = -INFINITY;
+                        }
+                }
+                float top = s[n][0][0];
+#pragma unroll
+                for (int t = 0; t < NB; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) top = fmaxf(top, s[n][t][i]);
+                const float mn = fmaxf(m[n], lifted(max_quarters(top), a.c, Q8 ? 0.0f : kLift<DT>));
+                const float mu = mn == -INFINITY ? 0.0f : mn, fade = exp2_fast(m[n] - mu);
+                m[n] = mn;
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < NB; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float x = exp2_fast(__builtin_fmaf(s[n][t][i], a.c, -mu));
+                        sum += x;
+                        wt[n][4 * t + i] = x;
+                    }
+                l[n] = __builtin_fmaf(l[n], fade, sum);
+#pragma unroll
+                for (int d = 0; d < NT; d++) o[n][d] *= fade;
+                if constexpr (Q8) {
+                    float wv[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        wv[i] = wt[n][i] * vs[i / 4][i % 4];
+                        if (!now.whole && !in[i]) wv[i] = 0.0f;   /* whatever the scale of what is not seen */
+                    }
+                    bf16_pieces<WP>(wv, pw[n]);
+                } else if constexpr (!F32) {
+                    pw[n][0] = pack<DT>(wt[n]);
+                }
+            }
+            wait_vm<MORE ? B::LOADS : 0>();
+            if constexpr (!Q8) {
+                if (!now.whole) {
+                    /* a weight of 0 times what is not finite would be a NaN: rows that no query sees become zeros, and of the
+                     * others what is not finite, which `odd` notes */
+                    u4 *v = reinterpret_cast<u4 *>(own + stage * B::STAGE + B::BYTES) + lane;
+#pragma unroll
+                    for (int x = 0; x < LD; x++) {
+                        const int key = now.k0 + RPL * x + lane / CH;
+                        const bool keep = now.there[RPL * x / 16] && key >= w.t0 && key < end_key &&
+                                          (key >= least - a.window || key < a.sinks);
+                        if (!keep) {
+                            v[64 * x] = u4{0, 0, 0, 0};
+                        } else if (odd_values<DT>(v[64 * x])) {
+                            odd = true;
+                            v[64 * x] = only_finite<DT>(v[64 * x]);
+                        }
+                    }
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                }
+            }
+            if constexpr (Q8) {
+#pragma unroll
+                for (int h = 0; h < DH / 64; h++) {
+                    uint32_t dw[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int row = B::key_of(j / 4, 4 * g + j % 4);
+                        dw[j] = *reinterpret_cast<const uint32_t *>(Vs + row * B::RB + 16 * B::v_place(row, 4 * h + x16 / 4) +
+                                                                    4 * (x16 % 4));
+                    }
+                    auto tile = [&](auto jj) __attribute__((always_inline)) {
+                        constexpr int J = decltype(jj)::value;
+                        u4 vf;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) vf[i] = upper_halves(code_at<J>(dw[2 * i]), code_at<J>(dw[2 * i + 1]));
+#pragma unroll
+                        for (int n = 0; n < NQ; n++)
+#pragma unroll
+                            for (int p = 0; p < WP; p++) o[n][4 * h + J] = mfma16<T_BF16>(vf, pw[n][p], o[n][4 * h + J]);
+                    };
+                    tile(std::integral_constant<int, 0>{});
+                    tile(std::integral_constant<int, 1>{});
+                    tile(std::integral_constant<int, 2>{});
+                    tile(std::integral_constant<int, 3>{});
+                }
+            } else if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int h = 0; h < DH / 64; h++) {
+                        const u4 v = *reinterpret_cast<const u4 *>(Vs + (4 * g + i) * B::RB + 16 * (16 * h + x16));
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+#pragma unroll
+                            for (int n = 0; n < NQ; n++)
+                                o[n][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[e]), wt[n][i],
+                                                                                       o[n][4 * h + e], 0, 0, 0);
+                    }
+            } else {
+                const int r = 4 * g + (x16 >> 2);
+#pragma unroll
+                for (int d = 0; d < NT; d++) {
+                    const unsigned char *at = Vs + r * B::RB + 16 * B::v_place(r, 2 * d + ((x16 & 3) >> 1)) + 8 * (x16 & 1);
+                    const u2 va = lds_tr(reinterpret_cast<const uint16_t *>(at)),
+                             vb = lds_tr(reinterpret_cast<const uint16_t *>(at + 16 * B::RB));
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) o[n][d] = mfma16<DT>(u4{va[0], va[1], vb[0], vb[1]}, pw[n][0], o[n][d]);
+                }
+            }
+            now = next;
+            stage ^= 1;
+        };
+        for (; b + NW < b1; b += NW) block(std::false_type{});
+        block(std::true_type{});
+    }
+
+    if constexpr (!Q8) odd = __syncthreads_or(odd);
+    else __syncthreads();   /* the waves' own parts are done with */
+    float *J = reinterpret_cast<float *>(lds);   /* [wave][16 · NQ rows][DH + 2] */
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const float sum = sum_quarters(l[n]);
+        float *mine = J + ((wave * NQ + n) * 16 + x16) * (DH + 2);
+#pragma unroll
+        for (int d = 0; d < NT; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                mine[Q8 || F32 ? 64 * (d / 4) + 4 * (4 * g + i) + d % 4 : 16 * d + 4 * g + i] = o[n][d][i];
+        if (g == 0) {
+            mine[DH] = m[n];
+            mine[DH + 1] = sum;
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < w.rows * DH; e += 64 * NW) {
+        const int r = e / DH, d = e % DH, seq = w.seq0 + (w.r0 + r) / G, head = w.kvh * G + (w.r0 + r) % G;
+        float top = -INFINITY, num = 0.0f, den = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NW; v++) top = fmaxf(top, J[(v * 16 * NQ + r) * (DH + 2) + DH]);
+        const float mu = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int v = 0; v < NW; v++) {
+            const float *j = J + (v * 16 * NQ + r) * (DH + 2);
+            const float f = exp2_fast(j[DH] - mu);
+            num = __builtin_fmaf(f, j[d], num);
+            den = __builtin_fmaf(f, j[DH + 1], den);
+        }
+        if constexpr (!Q8) {
+            if (odd) {   /* rare, so simple: any positive weight of an infinity or a NaN is that */
+                const int ln = kept_length(a.len[seq], a.table_ld, 1 << a.page_shift);
+                float more = 0.0f;
+                for (int bb = b0; bb < b1; bb++)
+                    for (int key = tb + blocks.at(bb) * KB; key < tb + blocks.at(bb) * KB + KB; key++) {
+                        const int page = page_in(page_entry(w.pages, a.table_ld, key, a.page_shift), a.pages);
+                        if (page < 0 || !seen_by(key, ln)) continue;
+                        const size_t token = (((size_t)page * a.kv + w.kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+                        const float x = Elem<DT>::get(static_cast<const E *>(a.vc)[token * DH + d]);
+                        if (!(__builtin_fabsf(x) < INFINITY)) more += x;
+                    }
+                if (!(__builtin_fabsf(more) < INFINITY)) num += more;
+            }
+        }
+        if (!a.part) {
+            static_cast<E *>(a.o)[(size_t)seq * a.ldo + (size_t)head * DH + d] = Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
+        } else {
+            float *to = a.part + (((size_t)seq * a.heads + head) * w.parts + w.slot) * (DH + 2);
+            to[d] = num;
+            if (d == 0) {
+                to[DH] = top;
+                to[DH + 1] = den;
+            }
+        }
+    }
+}
+
+/* group g's sequences [sa, sb) */
+__device__ __forceinline__ int group_start(const BatchArgs &a, int g) { return imin(imax(a.group[g], 0), a.n_seqs); }
+
+template <int CK, int DT, int DH, int NQ, int NW>
+__global__ __launch_bounds__(64 * NW) void attend(BatchArgs a)
+{
+    __shared__ __align__(16) unsigned char lds[attend_lds<CK, DT, DH, NQ, NW>()];
+    const int G = a.heads / a.kv;
+    BatchItem w;
+    if ((int)blockIdx.x < a.p_wgs) {
+        constexpr int TR = 16 * NQ;
+        const int id = blockIdx.x / a.kv;
+        w.kvh = blockIdx.x % a.kv;
+        w.split = id / a.p_tiles;
+        const int tile = id % a.p_tiles;
+        /* tiles are numbered as tile_start does, rows being G for each sequence */
+        const int gr = wave_last(a.n_groups, [&](int s) { return group_start(a, s) * G / TR + s <= tile; });
+        if (gr < 0) return;
+        const int sa = group_start(a, gr), sb = imax(group_start(a, gr + 1), sa);
+        w.r0 = (tile - (sa * G / TR + gr)) * TR;
+        if (w.r0 >= (sb - sa) * G) return;
+        w.seq0 = sa;
+        w.rows = imin(TR, (sb - sa) * G - w.r0);
+        w.t0 = 0;
+        w.t1 = imax(a.shared[gr], 0);
+        w.pages = a.table + (size_t)sa * a.table_ld;
+        w.splits = a.p_parts;
+        w.slot = w.split;
+        w.parts = a.p_parts + a.o_parts;
+        attend_item<CK, DT, DH, NQ, NW>(a, w, lds);
+        return;
+    }
+    int id = blockIdx.x - a.p_wgs;
+    w.kvh = id % a.kv;
+    id /= a.kv;
+    w.split = id % a.o_parts;
+    id /= a.o_parts;
+    w.r0 = 16 * (id % a.q_groups);
+    w.seq0 = id / a.q_groups;
+    w.rows = imin(16, G - w.r0);
+    w.t0 = 0;
+    w.t1 = 1 << 30;
+    w.pages = a.table + (size_t)w.seq0 * a.table_ld;
+    w.splits = a.o_parts;
+    w.slot = a.p_parts + w.split;
+    w.parts = a.p_parts + a.o_parts;
+    if (a.group) {
+        const int gr = wave_last(a.n_groups, [&](int s) { return group_start(a, s) <= w.seq0; });
+        if (gr < 0 || w.seq0 >= group_start(a, gr + 1)) {   /* in no group: attend_join leaves its rows as they are */
+            if (w.split == 0 && threadIdx.x < w.rows)
+                a.part[(((size_t)w.seq0 * a.heads + w.kvh * G + w.r0 + threadIdx.x) * w.parts + w.slot) * (DH + 2) + DH + 1] = -1.0f;
+            return;
+        }
+        w.t0 = imax(a.shared[gr], 0);
+    }
+    attend_item<CK, DT, DH, 1, NW>(a, w, lds);
+}
+
+/* The parts of one query added up by one wave, DH / 64 outputs a lane. */
+template <int DT, int DH>
+__global__ __launch_bounds__(256) void attend_join(BatchArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int PER = DH / 64;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, parts = a.p_parts + a.o_parts;
+    if (row >= a.n_seqs * a.heads) return;
+    const float *p = a.part + (size_t)row * parts * (DH + 2);
+    if (p[(size_t)a.p_parts * (DH + 2) + DH + 1] < 0.0f) return;   /* a sequence of no group */
+    float top = -INFINITY;
+    for (int s = lane; s < parts; s += 64) top = fmaxf(top, p[(size_t)s * (DH + 2) + DH]);
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+    const float mu = top == -INFINITY ? 0.0f : top;
+    float num[PER], den = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; i++) num[i] = 0.0f;
+#pragma unroll 8
+    for (int s = 0; s < parts; s++) {
+        const float *j = p + (size_t)s * (DH + 2);
+        const float f = exp2_fast(j[DH] - mu);
+#pragma unroll
+        for (int i = 0; i < PER; i++) num[i] = __builtin_fmaf(f, j[PER * lane + i], num[i]);
+        den = __builtin_fmaf(f, j[DH + 1], den);
+    }
+    E *o = static_cast<E *>(a.o) + (size_t)(row / a.heads) * a.ldo + (size_t)(row % a.heads) * DH + PER * lane;
+#pragma unroll
+    for (int i = 0; i < PER; i++) o[i] = Elem<DT>::put(den == 0.0f ? 0.0f : num[i] / den);
+}
+
+/* ── adapters ──────────────────────────────────────────────────────────────────────────────────────────────── */
+
+struct AdapterArgs {
+    int M, N, K, count, ldx, ldz, ldy, parts, chunk;   /* parts of `chunk` dimensions of K */
+    const void *x, *z, *a, *b;
+    const float *scale;
+    const int *index;
+    void *y;
+    float *h;   /* [parts][M][rank] */
+};
+
+/* The adapters of up to 16 rows, each once: f(adapter, rows), the rows as bits, in the order of their first rows. */
+template <class F> __device__ __forceinline__ void each_adapter(int mine, int rows, F f)
+{
+    uint32_t left = (uint32_t)__ballot((int)(threadIdx.x & 63) < rows && mine >= 0) & 0xffffu;
+    while (left) {
+        const int at = __builtin_ctz(left), ad = __builtin_amdgcn_readlane(mine, at);
+        const uint32_t those = (uint32_t)__ballot(mine == ad) & left;
+        f(ad, those);
+        left &= ~those;
+    }
+}
+
+/* Four steps of 4 dimensions of 16 × 16 fp32 products, or one of 32 16-bit ones */
+template <int DT> __device__ __forceinline__ f4 mfma_piece(u4 a, u4 b, f4 c)
+{
+    if constexpr (DT == T_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+        return c;
+    } else {
+        return mfma16<DT>(a, b, c);
+    }
+}
+
+/* 16 bytes of a row from element k on, zeros behind element `end`; VEC: all there and aligned */
+template <int DT, bool VEC> __device__ __forceinline__ u4 row_piece(const typename Elem<DT>::type *row, int k, int end)
+{
+    typedef typename Elem<DT>::type E;
+    if constexpr (VEC) {
+        return *reinterpret_cast<const u4 *>(row + k);
+    } else {
+        E v[kPer16<DT>];
+#pragma unroll
+        for (int j = 0; j < kPer16<DT>; j++) v[j] = k + j < end ? row[k + j] : Elem<DT>::put(0.0f);
+        u4 r;
+        __builtin_memcpy(&r, v, sizeof v);
+        return r;
+    }
+}
+
+/* H[part][m][r] = the sum over the part's dimensions k of X[m][k] · A[adapter of m][r][k], 16 rows a workgroup. */
+template <int DT, int RANK, bool VEC>
+__global__ __launch_bounds__(256) void adapter_shrink(AdapterArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int VE = kPer16<DT>, STEP = 4 * VE, RT = (RANK + 15) / 16, NW = 4;
+    __shared__ float sum[NW][16][16 * RT + 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int m0 = 16 * blockIdx.x, rows = imin(16, a.M - m0), k0 = blockIdx.y * a.chunk, k1 = imin(k0 + a.chunk, a.K);
+    const int id = a.index[m0 + imin(c, rows - 1)], mine = (unsigned)id < (unsigned)a.count ? id : -1;
+    const E *x = static_cast<const E *>(a.x) + (size_t)(m0 + imin(c, rows - 1)) * a.ldx;
+    f4 total[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) total[t] = f4{0, 0, 0, 0};
+    each_adapter(mine, rows, [&](int ad, uint32_t those) {
+        f4 acc[RT];
+#pragma unroll
+        for (int t = 0; t < RT; t++) acc[t] = f4{0, 0, 0, 0};
+        const E *am = static_cast<const E *>(a.a) + (size_t)ad * RANK * a.K;
+        for (int k = k0 + STEP * wave; k < k1; k += STEP * NW) {
+            const int kk = k + VE * g;
+            if (VEC && k + STEP <= k1) {
+                const u4 xv = row_piece<DT, true>(x, kk, k1);
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+                    acc[t] = mfma_piece<DT>(xv, row_piece<DT, true>(am + (size_t)imin(16 * t + c, RANK - 1) * a.K, kk, k1), acc[t]);
+            } else {
+                const u4 xv = row_piece<DT, false>(x, kk, k1);
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+                    acc[t] = mfma_piece<DT>(xv, row_piece<DT, false>(am + (size_t)imin(16 * t + c, RANK - 1) * a.K, kk, k1), acc[t]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if ((those >> (4 * g + i)) & 1) total[t][i] = acc[t][i];
+    });
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[wave][4 * g + i][16 * t + c] = total[t][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * RANK; e += 256) {
+        const int r = e / RANK, j = e % RANK;
+        a.h[((size_t)blockIdx.y * a.M + m0 + r) * RANK + j] =
+            (sum[0][r][j] + sum[1][r][j]) + (sum[2][r][j] + sum[3][r][j]);
+    }
+}
+
+/* Y[m][n] = Z[m][n] + scale · the sum over r of H[m][r] · B[adapter of m][n][r]: 16 rows and 256 columns a workgroup, in fp32
+ * products (B's values are exact in fp32), rounded once. */
+template <int DT, int RANK>
+__global__ __launch_bounds__(256) void adapter_expand(AdapterArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int RS = RANK / 4;   /* a lane's elements of a row of rank: RS · g .. */
+    __shared__ float hs[16][RANK + 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int m0 = 16 * blockIdx.y, rows = imin(16, a.M - m0), n0 = 256 * blockIdx.x + 64 * wave;
+    const int id = a.index[m0 + imin(c, rows - 1)], mine = (unsigned)id < (unsigned)a.count ? id : -1;
+    for (int e = threadIdx.x; e < 16 * RANK; e += 256) {
+        const int r = e / RANK;
+        float s = 0.0f;
+        if (r < rows) {
+            const int ad = a.index[m0 + r];
+            if ((unsigned)ad < (unsigned)a.count) {
+                for (int p = 0; p < a.parts; p++) s += a.h[((size_t)p * a.M + m0) * RANK + e];
+                s *= a.scale[ad];
+            }
+        }
+        hs[r][e % RANK] = s;
+    }
+    __syncthreads();
+    if (n0 >= a.N) return;
+    float h[RS];
+#pragma unroll
+    for (int s = 0; s < RS; s++) h[s] = hs[c][RS * g + s];
+    /* products' rows are columns of Y: row 4g + i of product t is column n0 + 16g + 4t + i, so that a lane has 16 neighbours */
+    f4 y[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) y[t] = f4{0, 0, 0, 0};
+    each_adapter(mine, rows, [&](int ad, uint32_t those) {
+        const bool in = (those >> c) & 1;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int n = imin(n0 + 16 * (c >> 2) + 4 * t + (c & 3), a.N - 1);
+            const E *b = static_cast<const E *>(a.b) + ((size_t)ad * a.N + n) * RANK + RS * g;
+            E v[RS];
+            __builtin_memcpy(v, b, sizeof v);
+            f4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < RS; s++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(Elem<DT>::get(v[s]), h[s], acc, 0, 0, 0);
+            if (in) y[t] = acc;
+        }
+    });
+    if (c >= rows) return;
+    const E *z = static_cast<const E *>(a.z) + (size_t)(m0 + c) * a.ldz;
+    E *out = static_cast<E *>(a.y) + (size_t)(m0 + c) * a.ldy;
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int n = n0 + 16 * g + 4 * t + i;
+            if (n >= a.N) continue;
+            const E before = a.z ? z[n] : Elem<DT>::put(0.0f);
+            out[n] = mine < 0 ? before : Elem<DT>::put(Elem<DT>::get(before) + y[t][i]);
+        }
+}
+
+}  // namespace p2k

@@ -1,0 +1,364 @@
+/*  p2hip_batch.hip – the device-pointer C ABI of a served batch's step (include/p2hip.h) over the kernels in
+ *  p2hip_batch.h: an 8-bit cache read back and attended, prefixes shared by groups of sequences, adapters.
+ *
+ *  As in p2hip.hip every shape, stride and alignment that a kernel assumes is checked before its launch, the arguments
+ *  before the device, so that a call is refused the same way with or without one.
+ */
+#include "p2hip_args.h"
+
+#include "p2hip_batch.h"
+
+using namespace p2host;
+
+namespace {
+
+constexpr int kWaves = 4;   /* of a workgroup of attend */
+
+/* How the queries and keys of a call go over workgroups. */
+struct Plan {
+    int p_tiles = 0, p_parts = 0, q_groups = 1, o_parts = 1;
+    int parts() const { return p_parts + o_parts; }
+    size_t bytes(int n_seqs, int heads, int head_dim) const
+    {
+        return (size_t)n_seqs * heads * parts() * (head_dim + 2) * 4;
+    }
+};
+
+/* Keys over workgroups: one for every 4 blocks a wave, as long as all together are at most 512, two for each of 256 CUs; a
+ * number, as the workspace's size is asked for where there may be no device. */
+int parts_of(long long groups, long long keys, int block)
+{
+    const long long most = groups ? 512 / groups : 1, n = keys / (4ll * block);
+    return (int)(n < 1 || most < 1 ? 1 : n < most ? n : most);
+}
+
+int block_of(bool q8, int dtype) { return !q8 && dtype == P2H_F32 ? 16 : 32; }
+
+/* the tokens of at most `n` that a window and first keys leave */
+long long left_of(int n, int window, int sinks)
+{
+    return p2k::imin(n, window) + (long long)p2k::imin(sinks, p2k::imax(n - window, 0));
+}
+
+Plan paged_plan(const CacheView &c, int n_seqs, int heads, int max_len, int window, int sinks)
+{
+    Plan p;
+    p.q_groups = (heads / c.heads + 15) / 16;
+    p.o_parts = parts_of((long long)n_seqs * c.heads * p.q_groups, left_of(max_len, window, sinks), 32);
+    return p;
+}
+
+Plan shared_plan(const CacheView &c, bool q8, int dtype, int n_seqs, int n_groups, int heads, int max_shared, int max_own,
+                 int window, int sinks)
+{
+    Plan p;
+    const int G = heads / c.heads, kb = block_of(q8, dtype);
+    p.q_groups = (G + 15) / 16;
+    p.p_tiles = n_seqs * G / 16 + n_groups;
+    const int rows = n_groups ? (n_seqs * G + n_groups - 1) / n_groups : 0;   /* of a group, as the host knows them */
+    p.p_parts = parts_of((long long)n_groups * ((rows + 15) / 16) * c.heads, left_of(max_shared, window, sinks), kb);
+    p.o_parts = parts_of((long long)n_seqs * c.heads * p.q_groups, left_of(max_own, window, sinks), kb);
+    return p;
+}
+
+int check_seqs(const char *name, int dtype, const CacheView &c, int n_seqs, int heads, int table_ld)
+{
+    if (int rc = check_heads(name, dtype, heads, c.heads, c.head_dim)) return rc;
+    if (n_seqs < 0 || n_seqs > 65536) return fail(P2H_E_ARG, "%s: %d sequences (at most 65536)", name, n_seqs);
+    if (table_ld < 0 || (long long)table_ld * c.page > (1 << 30))
+        return fail(P2H_E_ARG, "%s: table rows of %d pages of %d (at most 2^30 tokens)", name, table_ld, c.page);
+    return P2H_OK;
+}
+
+int check_tokens(const char *name, int n)
+{
+    return n < 0 || n > (1 << 30) ? fail(P2H_E_ARG, "%s: up to %d tokens (0 .. 2^30)", name, n) : P2H_OK;
+}
+
+Rows ints(const int *p, int ld, int n) { return Rows{(const char *)p, (size_t)ld * 4, (size_t)ld * 4, ld > 0 && p ? n : 0}; }
+
+/* Attention over a cache of either kind; `group` NULL without prefixes. */
+int attention(const char *name, int dtype, const CacheView &c, bool q8, const Plan &plan, int n_seqs, int n_groups, int heads,
+              const void *dQ, int ldq, const int *dGroup, const int *dShared, const int *dTable, int table_ld,
+              const int *dLen, float scale, int window, int sinks, void *dO, int ldo, void *workspace,
+              size_t workspace_bytes, void *stream)
+{
+    if (int rc = check_rows(name, "dQ", dtype, dQ, ldq, heads * c.head_dim)) return rc;
+    if (int rc = check_rows(name, "dO", dtype, dO, ldo, heads * c.head_dim)) return rc;
+    if (!dLen || (table_ld > 0 && !dTable)) return fail(P2H_E_ARG, "%s: NULL lengths or page table", name);
+    const size_t es = elem_size(dtype), width = (size_t)heads * c.head_dim * es;
+    const Rows q{(const char *)dQ, ldq * es, width, n_seqs}, o{(const char *)dO, ldo * es, width, n_seqs};
+    if (overlap(o, q)) return fail(P2H_E_ARG, "%s: dO overlaps dQ", name);
+    const bool parted = dGroup || plan.parts() > 1;
+    if (parted) {
+        const size_t need = plan.bytes(n_seqs, heads, c.head_dim);
+        if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+            return fail(P2H_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", name, workspace_bytes,
+                        need);
+        const Rows ws{(const char *)workspace, need, need, 1};
+        if (overlap(o, ws)) return fail(P2H_E_ARG, "%s: dO overlaps the workspace", name);
+        /* it is written while other workgroups still read */
+        if (overlap(ws, q) || overlap(ws, c) || overlap(ws, ints(dLen, 1, n_seqs)) ||
+            overlap(ws, ints(dTable, table_ld, n_seqs)) || overlap(ws, ints(dGroup, 1, n_groups + 1)) ||
+            overlap(ws, ints(dShared, 1, n_groups)))
+            return fail(P2H_E_ARG, "%s: the workspace overlaps what the call reads", name);
+    }
+    if (overlap(o, c)) return fail(P2H_E_ARG, "%s: dO overlaps the cache", name);
+    if (overlap(o, ints(dLen, 1, n_seqs)) || overlap(o, ints(dTable, table_ld, n_seqs)) ||
+        overlap(o, ints(dGroup, 1, n_groups + 1)) || overlap(o, ints(dShared, 1, n_groups)))
+        return fail(P2H_E_ARG, "%s: dO overlaps lengths, pages or groups", name);
+    const size_t p_wgs = (size_t)plan.p_tiles * plan.p_parts * c.heads;
+    const size_t wgs = p_wgs + (size_t)n_seqs * plan.q_groups * plan.o_parts * c.heads;
+    if (wgs * 64 * kWaves >= kGridThreads || (size_t)n_seqs * heads >= 1u << 23)
+        return fail(P2H_E_ARG, "%s: %d sequences of %d heads are too many for one call", name, n_seqs, heads);
+    if (int rc = ensure_init()) return rc;
+    p2k::BatchArgs a{};
+    a.n_seqs = n_seqs; a.n_groups = n_groups; a.heads = heads; a.kv = c.heads; a.page_shift = log2_of(c.page);
+    a.pages = c.pages; a.table_ld = table_ld; a.ldq = ldq; a.ldo = ldo; a.window = window; a.sinks = sinks;
+    a.p_tiles = plan.p_tiles; a.p_parts = plan.p_parts; a.p_wgs = (int)p_wgs;
+    a.q_groups = plan.q_groups; a.o_parts = plan.o_parts; a.c = scale * p2k::kLog2e;
+    a.q = dQ; a.kc = c.K; a.vc = c.V; a.ks = c.ks; a.vs = c.vs;
+    a.table = dTable; a.len = dLen; a.group = dGroup; a.shared = dShared; a.o = dO;
+    a.part = parted ? (float *)workspace : nullptr;
+    hipStream_t s = stream_of(stream);
+    by_type_dim(dtype, c.head_dim, [&](auto t, auto d) {
+        constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
+        if (q8) hipLaunchKernelGGL((p2k::attend<p2k::C_Q8, DT, DH, 1, kWaves>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, s, a);
+        else hipLaunchKernelGGL((p2k::attend<p2k::C_ROWS, DT, DH, 1, kWaves>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, s, a);
+        if (parted)
+            hipLaunchKernelGGL((p2k::attend_join<DT, DH>), dim3((unsigned)(((size_t)n_seqs * heads + 3) / 4)), dim3(256), 0, s, a);
+    });
+    HIPCHK(hipGetLastError());
+    return P2H_OK;
+}
+
+size_t shared_bytes(const char *name, const P2hKvCache *rows, const P2hKvCacheQ8 *q8, int n_seqs, int n_groups, int heads,
+                    int max_shared, int max_own, int window, int sinks)
+{
+    if (rows ? check_cache(name, rows) : check_cache(name, q8)) return 0;
+    const CacheView c(rows, q8);
+    const int dtype = rows ? rows->dtype : P2H_BF16;
+    if (check_seqs(name, dtype, c, n_seqs, heads, 0) || check_scale(name, 1.0f, window, 0, sinks) ||
+        check_tokens(name, max_shared) || check_tokens(name, max_own))
+        return 0;
+    if (n_groups < 0 || n_groups > 65536) {
+        fail(P2H_E_ARG, "%s: %d groups (at most 65536)", name, n_groups);
+        return 0;
+    }
+    return shared_plan(c, q8 != nullptr, dtype, n_seqs, n_groups, heads, max_shared, max_own, window, sinks)
+        .bytes(n_seqs, heads, c.head_dim);
+}
+
+int shared(const char *name, int dtype, const P2hKvCache *rows, const P2hKvCacheQ8 *q8, int n_seqs, int n_groups, int heads,
+           const void *dQ, int ldq, const int *dGroup, const int *dShared, const int *dTable, int table_ld, const int *dLen,
+           int max_shared, int max_own, float scale, int window, int sinks, void *dO, int ldo, void *workspace,
+           size_t workspace_bytes, void *stream)
+{
+    if (int rc = rows ? check_cache(name, rows) : check_cache(name, q8)) return rc;
+    const CacheView c(rows, q8);
+    if (int rc = check_seqs(name, dtype, c, n_seqs, heads, table_ld)) return rc;
+    if (int rc = check_scale(name, scale, window, 0, sinks)) return rc;
+    if (int rc = check_tokens(name, max_shared)) return rc;
+    if (int rc = check_tokens(name, max_own)) return rc;
+    if (n_groups < 0 || n_groups > 65536) return fail(P2H_E_ARG, "%s: %d groups (at most 65536)", name, n_groups);
+    if (n_seqs == 0 || n_groups == 0) return P2H_OK;
+    if (!dGroup || !dShared) return fail(P2H_E_ARG, "%s: NULL groups or prefixes", name);
+    const Plan plan = shared_plan(c, q8 != nullptr, dtype, n_seqs, n_groups, heads, max_shared, max_own, window, sinks);
+    return attention(name, dtype, c, q8 != nullptr, plan, n_seqs, n_groups, heads, dQ, ldq, dGroup, dShared, dTable, table_ld,
+                     dLen, scale, window, sinks, dO, ldo, workspace, workspace_bytes, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+/* ── the 8-bit cache ───────────────────────────────────────────────────────────────────────────────────────── */
+
+int p2h_kv_rows_q8(int dtype, const P2hKvCacheQ8 *cache, int rows, int n_seqs, const int *dStart, const int *dTable,
+                   int table_ld, void *dK, int ldk, void *dV, int ldv, void *stream)
+{
+    const char *name = "p2h_kv_rows_q8";
+    if (int rc = check_cache(name, cache)) return rc;
+    const CacheView c(nullptr, cache);
+    if (int rc = check_seqs(name, dtype, c, n_seqs, c.heads, table_ld)) return rc;
+    if (rows < 0 || rows >= 1 << 30) return fail(P2H_E_ARG, "%s: %d rows (below 2^30)", name, rows);
+    if (rows == 0 || n_seqs == 0) return P2H_OK;
+    const int width = c.heads * c.head_dim;
+    if (int rc = check_rows(name, "dK", dtype, dK, ldk, width)) return rc;
+    if (int rc = check_rows(name, "dV", dtype, dV, ldv, width)) return rc;
+    if (!dStart || (table_ld > 0 && !dTable)) return fail(P2H_E_ARG, "%s: NULL starts or page table", name);
+    const size_t es = elem_size(dtype);
+    const Rows k{(const char *)dK, ldk * es, width * es, rows}, v{(const char *)dV, ldv * es, width * es, rows};
+    if (overlap(k, v)) return fail(P2H_E_ARG, "%s: dK and dV overlap", name);
+    if (overlap(k, c) || overlap(v, c)) return fail(P2H_E_ARG, "%s: dK or dV overlaps the cache", name);
+    for (const Rows &r : {ints(dStart, 1, n_seqs + 1), ints(dTable, table_ld, n_seqs)})
+        if (overlap(k, r) || overlap(v, r)) return fail(P2H_E_ARG, "%s: dK or dV overlaps starts or pages", name);
+    if (int rc = ensure_init()) return rc;
+    p2k::KvRowsArgs a{};
+    a.rows = rows; a.n_seqs = n_seqs; a.kv = c.heads; a.page_shift = log2_of(c.page); a.pages = c.pages;
+    a.table_ld = table_ld; a.ldk = ldk; a.ldv = ldv;
+    a.start = dStart; a.table = dTable; a.kc = (const int8_t *)c.K; a.vc = (const int8_t *)c.V; a.ks = c.ks; a.vs = c.vs;
+    a.k = dK; a.v = dV;
+    a.per = p2k::imin(p2k::imax(rows / 2048, 1), p2k::kRowsMost);
+    const unsigned grid = (unsigned)((rows - 1) / a.per + 1);
+    if ((size_t)grid * 256 >= kGridThreads) return fail(P2H_E_ARG, "%s: %d rows are too many for one call", name, rows);
+    hipStream_t s = stream_of(stream);
+    by_type_dim(dtype, c.head_dim, [&](auto t, auto d) {
+        hipLaunchKernelGGL((p2k::kv_rows_q8<decltype(t)::value, decltype(d)::value>), dim3(grid), dim3(256), 0, s, a);
+    });
+    HIPCHK(hipGetLastError());
+    return P2H_OK;
+}
+
+size_t p2h_attention_paged_q8_workspace_bytes(const P2hKvCacheQ8 *cache, int n_seqs, int heads, int max_len, int window,
+                                              int sinks)
+{
+    const char *name = "p2h_attention_paged_q8_workspace_bytes";
+    if (check_cache(name, cache)) return 0;
+    const CacheView c(nullptr, cache);
+    if (check_seqs(name, P2H_BF16, c, n_seqs, heads, 0) || check_scale(name, 1.0f, window, 0, sinks) ||
+        check_tokens(name, max_len))
+        return 0;
+    const Plan p = paged_plan(c, n_seqs, heads, max_len, window, sinks);
+    return p.parts() > 1 ? p.bytes(n_seqs, heads, c.head_dim) : 0;
+}
+
+int p2h_attention_paged_q8(int dtype, const P2hKvCacheQ8 *cache, int n_seqs, int heads, const void *dQ, int ldq,
+                           const int *dTable, int table_ld, const int *dLen, int max_len, float scale, int window,
+                           int sinks, void *dO, int ldo, void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *name = "p2h_attention_paged_q8";
+    if (int rc = check_cache(name, cache)) return rc;
+    const CacheView c(nullptr, cache);
+    if (int rc = check_seqs(name, dtype, c, n_seqs, heads, table_ld)) return rc;
+    if (int rc = check_scale(name, scale, window, 0, sinks)) return rc;
+    if (int rc = check_tokens(name, max_len)) return rc;
+    if (n_seqs == 0) return P2H_OK;
+    Plan plan = paged_plan(c, n_seqs, heads, max_len, window, sinks);
+    if (!workspace) plan.o_parts = 1;
+    return attention(name, dtype, c, true, plan, n_seqs, 0, heads, dQ, ldq, nullptr, nullptr, dTable, table_ld, dLen, scale,
+                     window, sinks, dO, ldo, workspace, workspace_bytes, stream);
+}
+
+/* ── shared prefixes ───────────────────────────────────────────────────────────────────────────────────────── */
+
+size_t p2h_attention_shared_workspace_bytes(const P2hKvCache *cache, int n_seqs, int n_groups, int heads, int max_shared,
+                                            int max_own, int window, int sinks)
+{
+    const char *name = "p2h_attention_shared_workspace_bytes";
+    if (!cache) return fail(P2H_E_ARG, "%s: NULL cache", name), 0;
+    return shared_bytes(name, cache, nullptr, n_seqs, n_groups, heads, max_shared, max_own, window, sinks);
+}
+
+int p2h_attention_shared(const P2hKvCache *cache, int n_seqs, int n_groups, int heads, const void *dQ, int ldq,
+                         const int *dGroup, const int *dShared, const int *dTable, int table_ld, const int *dLen,
+                         int max_shared, int max_own, float scale, int window, int sinks, void *dO, int ldo,
+                         void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *name = "p2h_attention_shared";
+    if (!cache) return fail(P2H_E_ARG, "%s: NULL cache", name);
+    return shared(name, cache->dtype, cache, nullptr, n_seqs, n_groups, heads, dQ, ldq, dGroup, dShared, dTable, table_ld,
+                  dLen, max_shared, max_own, scale, window, sinks, dO, ldo, workspace, workspace_bytes, stream);
+}
+
+size_t p2h_attention_shared_q8_workspace_bytes(const P2hKvCacheQ8 *cache, int n_seqs, int n_groups, int heads,
+                                               int max_shared, int max_own, int window, int sinks)
+{
+    return shared_bytes("p2h_attention_shared_q8_workspace_bytes", nullptr, cache, n_seqs, n_groups, heads, max_shared,
+                        max_own, window, sinks);
+}
+
+int p2h_attention_shared_q8(int dtype, const P2hKvCacheQ8 *cache, int n_seqs, int n_groups, int heads, const void *dQ,
+                            int ldq, const int *dGroup, const int *dShared, const int *dTable, int table_ld,
+                            const int *dLen, int max_shared, int max_own, float scale, int window, int sinks, void *dO,
+                            int ldo, void *workspace, size_t workspace_bytes, void *stream)
+{
+    return shared("p2h_attention_shared_q8", dtype, nullptr, cache, n_seqs, n_groups, heads, dQ, ldq, dGroup, dShared, dTable,
+                  table_ld, dLen, max_shared, max_own, scale, window, sinks, dO, ldo, workspace, workspace_bytes, stream);
+}
+
+/* ── adapters ──────────────────────────────────────────────────────────────────────────────────────────────── */
+
+static int check_adapters(const char *name, const P2hAdapters *ad, int M)
+{
+    if (!ad) return fail(P2H_E_ARG, "%s: NULL adapters", name);
+    if (!is_type(ad->dtype)) return fail(P2H_E_ARG, "%s: element type %d", name, ad->dtype);
+    if (ad->rank != 8 && ad->rank != 16 && ad->rank != 32 && ad->rank != 64 && ad->rank != 128)
+        return fail(P2H_E_ARG, "%s: rank = %d (8, 16, 32, 64 or 128)", name, ad->rank);
+    if (ad->count < 0 || ad->K < 1 || ad->N < 1 || ad->K > (1 << 23) || ad->N > (1 << 23))
+        return fail(P2H_E_ARG, "%s: %d adapters of [%d, %d]", name, ad->count, ad->K, ad->N);
+    if (M < 0 || M > 16 * 65535) return fail(P2H_E_ARG, "%s: M = %d (at most %d rows)", name, M, 16 * 65535);
+    return P2H_OK;
+}
+
+/* K over workgroups: so that there are 256 of them, at least 128 elements each. A number, as the workspace's size is asked
+ * for where there may be no device. */
+static int adapter_parts(const P2hAdapters *ad, int M)
+{
+    const int tiles = (M + 15) / 16, most = (ad->K + 127) / 128, want = (256 + tiles - 1) / (tiles > 0 ? tiles : 1);
+    return p2k::imax(p2k::imin(want, most), 1);
+}
+
+size_t p2h_adapters_workspace_bytes(const P2hAdapters *ad, int M)
+{
+    if (check_adapters("p2h_adapters_workspace_bytes", ad, M)) return 0;
+    return (size_t)adapter_parts(ad, M) * M * ad->rank * 4;
+}
+
+int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, const int *dIndex, const void *dZ, int ldz,
+                     void *dY, int ldy, void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *name = "p2h_adapters_add";
+    if (int rc = check_adapters(name, ad, M)) return rc;
+    if (M == 0) return P2H_OK;
+    const int K = ad->K, N = ad->N;
+    const size_t es = elem_size(ad->dtype);
+    if (!dX || !dY || ldx < K || ldy < N || (dZ && ldz < N) || !aligned(dX, es) || !aligned(dY, es) || !aligned(dZ, es))
+        return fail(P2H_E_ARG, "%s: NULL or unaligned rows, or ldx = %d < K = %d, ldz = %d or ldy = %d < N = %d", name, ldx, K,
+                    ldz, ldy, N);
+    if (!dIndex) return fail(P2H_E_ARG, "%s: NULL index", name);
+    if (ad->count > 0 && (!ad->A || !ad->B || !ad->scale || !aligned(ad->A, 16) || !aligned(ad->B, 16)))
+        return fail(P2H_E_ARG, "%s: adapters are NULL or not 16-byte aligned", name);
+    const size_t need = p2h_adapters_workspace_bytes(ad, M);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return fail(P2H_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", name, workspace_bytes, need);
+    const Rows x{(const char *)dX, ldx * es, K * es, M}, y{(const char *)dY, ldy * es, N * es, M};
+    const Rows z{(const char *)dZ, ldz * es, N * es, dZ ? M : 0}, ws{(const char *)workspace, need, need, 1};
+    const size_t a_bytes = (size_t)ad->count * ad->rank * K * es, b_bytes = (size_t)ad->count * ad->rank * N * es;
+    const Rows am{(const char *)ad->A, a_bytes, a_bytes, a_bytes ? 1 : 0}, bm{(const char *)ad->B, b_bytes, b_bytes, b_bytes ? 1 : 0};
+    const Rows sc{(const char *)ad->scale, (size_t)ad->count * 4, (size_t)ad->count * 4, ad->count ? 1 : 0};
+    const bool in_place = dZ == dY && (ldz == ldy || M == 1);
+    if (!in_place && overlap(y, z)) return fail(P2H_E_ARG, "%s: dY overlaps dZ other than in place", name);
+    for (const Rows &r : {x, am, bm, sc, ints(dIndex, 1, M)})
+        if (overlap(y, r) || overlap(ws, r)) return fail(P2H_E_ARG, "%s: dY or the workspace overlaps what the call reads", name);
+    if (overlap(ws, y) || overlap(ws, z)) return fail(P2H_E_ARG, "%s: the workspace overlaps dY or dZ", name);
+    if (int rc = ensure_init()) return rc;
+    p2k::AdapterArgs a{};
+    a.M = M; a.N = N; a.K = K; a.count = ad->count; a.ldx = ldx; a.ldz = ldz; a.ldy = ldy;
+    a.parts = adapter_parts(ad, M);
+    a.chunk = ((K - 1) / a.parts / 128 + 1) * 128;
+    a.x = dX; a.z = dZ; a.a = ad->A; a.b = ad->B; a.scale = ad->scale; a.index = dIndex; a.y = dY; a.h = (float *)workspace;
+    const bool vec = aligned(dX, 16) && (M == 1 || ldx * es % 16 == 0) && K * es % 16 == 0;
+    const unsigned tiles = (unsigned)((M + 15) / 16);
+    hipStream_t s = stream_of(stream);
+    by_type(ad->dtype, [&](auto t) {
+        auto go = [&](auto rank) {
+            constexpr int DT = decltype(t)::value, R = decltype(rank)::value;
+            const dim3 g1(tiles, (unsigned)a.parts), g2((unsigned)((N + 255) / 256), tiles);
+            if (vec) hipLaunchKernelGGL((p2k::adapter_shrink<DT, R, true>), g1, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((p2k::adapter_shrink<DT, R, false>), g1, dim3(256), 0, s, a);
+            hipLaunchKernelGGL((p2k::adapter_expand<DT, R>), g2, dim3(256), 0, s, a);
+        };
+        switch (ad->rank) {
+        case 8: go(ic<8>{}); break;
+        case 16: go(ic<16>{}); break;
+        case 32: go(ic<32>{}); break;
+        case 64: go(ic<64>{}); break;
+        default: go(ic<128>{}); break;
+        }
+    });
+    HIPCHK(hipGetLastError());
+    return P2H_OK;
+}
+
+}  /* extern "C" */

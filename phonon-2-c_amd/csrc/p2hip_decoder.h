@@ -9,138 +9,11 @@
  */
 #pragma once
 
-#include <hip/hip_runtime.h>
-#include <stdint.h>
-
-#include <type_traits>
-
 #include "p2hip_async.h"
+#include "p2hip_elem.h"
 #include "p2hip_index.h"
 
 namespace p2k {
-
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f16v __attribute__((ext_vector_type(16)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef short s4 __attribute__((ext_vector_type(4)));
-
-enum { T_F32 = 0, T_F16 = 1, T_BF16 = 2 };
-constexpr float kLog2e = 1.44269504088896340736f;
-
-/* ── element types ─────────────────────────────────────────────────────────────────────────────────────────── */
-
-template <int DT> struct Elem;
-template <> struct Elem<T_F32> {
-    typedef float type;
-    static __device__ __forceinline__ float get(float v) { return v; }
-    static __device__ __forceinline__ float put(float v) { return v; }
-};
-template <> struct Elem<T_F16> {
-    typedef _Float16 type;
-    static __device__ __forceinline__ float get(_Float16 v) { return (float)v; }
-    static __device__ __forceinline__ _Float16 put(float v) { return (_Float16)v; }
-};
-template <> struct Elem<T_BF16> {
-    typedef __bf16 type;
-    static __device__ __forceinline__ float get(__bf16 v) { return (float)v; }
-    static __device__ __forceinline__ __bf16 put(float v) { return (__bf16)v; }
-};
-
-/* 16 bytes of elements as floats, and back (each rounded to nearest even) */
-template <int DT> constexpr int kPer16 = DT == T_F32 ? 4 : 8;
-
-template <int DT> __device__ __forceinline__ void unpack(u4 r, float (&v)[kPer16<DT>])
-{
-    if constexpr (DT == T_F32) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = __uint_as_float(r[i]);
-    } else if constexpr (DT == T_F16) {
-        const h8 x = __builtin_bit_cast(h8, r);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = (float)x[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[2 * i] = __uint_as_float(r[i] << 16);
-            v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
-        }
-    }
-}
-
-template <int DT> __device__ __forceinline__ u4 pack(const float (&v)[kPer16<DT>])
-{
-    if constexpr (DT == T_F32) {
-        return u4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-    } else if constexpr (DT == T_F16) {
-        h8 x;
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (_Float16)v[i];
-        return __builtin_bit_cast(u4, x);
-    } else {
-        b8 x;
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (__bf16)v[i];
-        return __builtin_bit_cast(u4, x);
-    }
-}
-
-/* the matrix products of 16-bit operands, bits as u4 */
-template <int DT> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c)
-{
-    if constexpr (DT == T_F16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-}
-
-template <int DT> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c)
-{
-    if constexpr (DT == T_F16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-}
-
-/* Transposing LDS read of 16-bit values: of the 4 × 16 values that the 16 lanes of a group address (lane i: 4 values,
- * row i / 4, columns 4·(i % 4) ..), lane i gets column i's four. */
-__device__ __forceinline__ u2 lds_tr(uint32_t at)   /* an LDS byte address */
-{
-    typedef __attribute__((address_space(3))) s4 *lds4;
-    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at)));
-}
-__device__ __forceinline__ u2 lds_tr(const uint16_t *p)
-{
-    return lds_tr((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint16_t *)(p));
-}
-
-/* max and sum over lanes l, l ^ 16, l ^ 32, l ^ 48, and over l, l ^ 32 */
-__device__ __forceinline__ float max_halves(float v)
-{
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_halves(float v)
-{
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float max_quarters(float v)
-{
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float sum_quarters(float v)
-{
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-}
-
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 /* ── 4-bit weights ─────────────────────────────────────────────────────────────────────────────────────────── */
 
@@ -478,7 +351,34 @@ struct RopeArgs {
     void *q, *k, *kc, *vc;
     const float *gq, *gk, *freq;
     const int *pos, *slots;
+    float *ks, *vs;   /* Q8: the scales of kc's and vc's codes */
 };
+
+/* A head's values v (LPH lanes of VE each, x = lane of the head) as 8-bit codes at `to` and their scale at `s`: scale = largest
+ * |value| / 127, code = round-half-even(value · (127 / largest)), so that a value is off by half a step of its head's
+ * largest / 127. Below 2^-100 a head is zeros; one with a value that is not finite has a NaN as its scale. */
+template <int VE, int LPH> __device__ __forceinline__ void put_codes(const float (&v)[VE], int x, int8_t *to, float *s)
+{
+    uint32_t top = 0;   /* bits of |value|: in the order of the values, infinities and NaN above all */
+#pragma unroll
+    for (int i = 0; i < VE; i++) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < LPH; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o, LPH));
+    const bool finite = top < 0x7f800000u, some = finite && top >= 0x0d800000u;   /* 2^-100 */
+    const float most = __uint_as_float(top), by = some ? 127.0f / most : 0.0f;
+    uint32_t w[VE / 4];
+#pragma unroll
+    for (int i = 0; i < VE / 4; i++) {
+        w[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int code = some ? (int)__builtin_rintf(v[4 * i + j] * by) : 0;
+            w[i] |= ((uint32_t)code & 0xffu) << (8 * j);
+        }
+    }
+    __builtin_memcpy(__builtin_assume_aligned(to + VE * x, VE), w, VE);
+    if (x == 0) *s = some ? most / 127.0f : finite ? 0.0f : __builtin_nanf("");
+}
 
 /* One workgroup of NTHR threads per row: 16 bytes of a head per lane, a head's lanes side by side, so that the mean square
  * is a reduction inside a row of lanes. The row's angles are made once, in 64 bits, as turns reduced to an eighth of a
@@ -487,7 +387,7 @@ struct RopeArgs {
  * (4.4 TB/s, a copy reaches 4.8); loading 4 heads a thread ahead took 35.9, making the angles before the first load 34.6.
  * Few rows take 1024 threads, all of a row's heads at once (16 rows 3.9 us, 5.7 with 256 threads). Heads whose squares
  * leave the range of 32 bits (values from 2^60 up; without an eps to speak of, below 2^-48) are moved into it first. */
-template <int DT, int DH, int NTHR>
+template <int DT, int DH, int NTHR, bool Q8>
 __global__ __launch_bounds__(NTHR) void qk_norm_rope(RopeArgs a)
 {
     typedef typename Elem<DT>::type E;
@@ -520,9 +420,10 @@ __global__ __launch_bounds__(NTHR) void qk_norm_rope(RopeArgs a)
         }
         if (h >= n_heads) break;
         u4 res = raw;
+        float v[VE];
         const bool is_q = h < a.heads, is_v = h >= a.heads + a.kv;
         if (!is_v) {   /* the same for all lanes of a head */
-            float v[VE], gm[VE];
+            float gm[VE];
 #pragma unroll
             for (int i = 0; i < VE; i++) gm[i] = (is_q ? a.gq : a.gk)[VE * l + i];   /* on their way during the sum */
             unpack<DT>(raw, v);
@@ -579,8 +480,14 @@ __global__ __launch_bounds__(NTHR) void qk_norm_rope(RopeArgs a)
             *reinterpret_cast<u4 *>(static_cast<E *>(a.k) + (size_t)t * a.ldk + (size_t)hk * DH + VE * l) = res;
         if (!is_q && slot >= 0) {
             const size_t page = (size_t)(slot >> a.page_shift), off = (size_t)slot & ((1u << a.page_shift) - 1);
-            E *to = static_cast<E *>(is_v ? a.vc : a.kc) + (((page * a.kv + hk) << a.page_shift) + off) * DH + VE * l;
-            *reinterpret_cast<u4 *>(to) = res;
+            const size_t head = ((page * a.kv + hk) << a.page_shift) + off;
+            if constexpr (Q8) {   /* keys from their 32-bit values; values have not been through the norm */
+                if (is_v) unpack<DT>(raw, v);
+                put_codes<VE, LPH>(v, l, static_cast<int8_t *>(is_v ? a.vc : a.kc) + head * DH, (is_v ? a.vs : a.ks) + head);
+            } else {
+                E *to = static_cast<E *>(is_v ? a.vc : a.kc) + head * DH + VE * l;
+                *reinterpret_cast<u4 *>(to) = res;
+            }
         }
     }
 }
@@ -629,39 +536,6 @@ __device__ __forceinline__ bool find_tile(const WinArgs &a, int rows, int id, Wi
     auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };   /* the same in every lane: scalar registers */
     *seq = WinSeq{of(qa), of(qb), of(ka), of(kb), id - of(first)};
     return seq->tile >= 0 && seq->tile < (seq->qb - seq->qa + rows - 1) / rows;
-}
-
-/* A sum to which 16 bytes of elements add 0, or a NaN if one of them is an infinity or a NaN: their products with zeros */
-template <int DT> __device__ __forceinline__ float odd_sum(u4 v, float sum)
-{
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t w = v[i];   /* a bit cast of v[i] itself takes element 0, whatever i */
-        if constexpr (DT == T_F32) sum = __builtin_fmaf(__uint_as_float(w), 0.0f, sum);
-        else if constexpr (DT == T_F16) sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{0, 0}, sum, false);
-        else sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{0, 0}, sum, false);
-    }
-    return sum;
-}
-template <int DT> __device__ __forceinline__ bool odd_values(u4 v)
-{
-    const float z = odd_sum<DT>(v, 0.0f);
-    return z != z;
-}
-
-/* the infinities and NaN among 16 bytes of elements replaced by zeros */
-template <int DT> __device__ __forceinline__ u4 only_finite(u4 v)
-{
-    constexpr uint32_t E = DT == T_F32 ? 0x7f800000u : DT == T_F16 ? 0x7c007c00u : 0x7f807f80u;
-    constexpr uint32_t H = E & 0xffff0000u, L = E & 0xffffu;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        uint32_t keep = 0xffffffffu;
-        if ((v[i] & H) == H) keep = DT == T_F32 ? 0u : keep & 0xffffu;
-        if (DT != T_F32 && (v[i] & L) == L) keep &= 0xffff0000u;
-        v[i] &= keep;
-    }
-    return v;
 }
 
 /* One sequence's tile of queries: its rows, places and the key blocks that any of its queries sees. */
@@ -786,24 +660,6 @@ template <class E, int DH, int KB, int NW> struct BlockLoads {
         return true;
     }
 };
-
-/* Weights enter their product with V in the rows' type. fp16 keeps nothing under 2^-25, which many keys together, or one
- * with a large value beside values near 0, can make felt; so the reference that weights are taken from stands kLift powers
- * of two under the largest score (weights up to 2^kLift, and what is under 2^-(25 + kLift) of the largest is lost: 2^-40).
- * Sums carry the same factor, so that it leaves with the division. bf16 ends where fp32 does and needs none. */
-template <int DT> constexpr float kLift = DT == T_F16 ? 15.0f : 0.0f;
-
-/* A score's place less the lift. In two instructions: as one, the constant or c would take a register of its own, which
- * attention_page of fp16 heads of 128 does not have (8 bytes a lane in scratch). */
-__device__ __forceinline__ float lifted(float score, float c, float lift)
-{
-    float x = score * c;
-    if (lift != 0.0f) {
-        asm("" : "+v"(x));
-        x -= lift;
-    }
-    return x;
-}
 
 /* attention_win raises its reference only where the exponentials of a block have a sum above kWinSlack in some lane: then
  * to the largest score so far, and they are taken again. It is not raised otherwise, so that most blocks need no maximum

@@ -4,21 +4,15 @@
  *  As in p2hip.hip every shape, stride and alignment that a kernel assumes is checked before its launch, the arguments
  *  before the device, so that a call is refused the same way with or without one.
  */
-#include "p2hip_host.h"
+#include "p2hip_args.h"
 
 #include <climits>
-#include <cmath>
 #include <cstring>
 #include <new>
 
 #include "p2hip_decoder.h"
 
-using p2host::align_up;
-using p2host::aligned;
-using p2host::cu_count;
-using p2host::ensure_init;
-using p2host::fail;
-using p2host::stream_of;
+using namespace p2host;
 
 struct P2hQ4Weight {
     int K, N, group, tiles, units;
@@ -26,100 +20,6 @@ struct P2hQ4Weight {
     uint8_t *base;   /* the one device allocation: records, then scales */
     size_t sc_off, bytes;
 };
-
-namespace {
-
-constexpr size_t kGridThreads = (size_t)1 << 32;   /* a launch has fewer threads */
-
-inline size_t elem_size(int dtype) { return dtype == P2H_F32 ? 4 : 2; }
-inline bool is_type(int dtype) { return dtype == P2H_F32 || dtype == P2H_F16 || dtype == P2H_BF16; }
-
-template <int V> using ic = std::integral_constant<int, V>;
-
-/* f(type, …) with the element type as a constant */
-template <class F> void by_type(int dtype, F f)
-{
-    if (dtype == P2H_F32) f(ic<p2k::T_F32>{});
-    else if (dtype == P2H_F16) f(ic<p2k::T_F16>{});
-    else f(ic<p2k::T_BF16>{});
-}
-
-/* f(type, head_dim) */
-template <class F> void by_type_dim(int dtype, int head_dim, F f)
-{
-    by_type(dtype, [&](auto t) {
-        if (head_dim == 64) f(t, ic<64>{});
-        else f(t, ic<128>{});
-    });
-}
-
-/* M rows of `w` bytes at pitch `ld` bytes, as a range */
-struct Rows {
-    const char *p;
-    size_t ld, w;
-    int M;
-    const char *end() const { return p + (M ? (size_t)(M - 1) * ld + w : 0); }
-};
-
-/* whether two sets of rows share a byte: apart as ranges, or of one pitch with their columns apart */
-bool overlap(const Rows &a, const Rows &b)
-{
-    if (a.M <= 0 || b.M <= 0 || a.end() <= b.p || b.end() <= a.p) return false;
-    if (a.ld != b.ld) return true;
-    const size_t d = a.p <= b.p ? (size_t)(b.p - a.p) % a.ld : (a.ld - (size_t)(a.p - b.p) % a.ld) % a.ld;
-    return !(d >= a.w && d + b.w <= a.ld);
-}
-
-int check_heads(const char *name, int dtype, int heads, int kv_heads, int head_dim)
-{
-    if (!is_type(dtype)) return fail(P2H_E_ARG, "%s: element type %d", name, dtype);
-    if (head_dim != 64 && head_dim != 128) return fail(P2H_E_ARG, "%s: head_dim = %d (64 or 128)", name, head_dim);
-    if (kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || heads > 65536)
-        return fail(P2H_E_ARG, "%s: %d heads over %d key heads", name, heads, kv_heads);
-    return P2H_OK;
-}
-
-int check_rows(const char *name, const char *what, int dtype, const void *p, int ld, int width)
-{
-    if (!p || !aligned(p, 16)) return fail(P2H_E_ARG, "%s: %s is NULL or not 16-byte aligned", name, what);
-    if (ld < width || (size_t)ld * elem_size(dtype) % 16 != 0)
-        return fail(P2H_E_ARG, "%s: pitch %d of %s must be >= %d and a multiple of 16 bytes", name, ld, what, width);
-    /* a block's rows are addressed by 32-bit offsets from its first */
-    if (ld >= 1 << 23) return fail(P2H_E_ARG, "%s: pitch %d of %s must be below 2^23", name, ld, what);
-    return P2H_OK;
-}
-
-int check_cache(const char *name, const P2hKvCache *c)
-{
-    if (!c) return fail(P2H_E_ARG, "%s: NULL cache", name);
-    if (!is_type(c->dtype) || c->heads < 1 || c->heads > 65536 || (c->head_dim != 64 && c->head_dim != 128))
-        return fail(P2H_E_ARG, "%s: cache of type %d with %d heads of %d", name, c->dtype, c->heads, c->head_dim);
-    if (c->page < 16 || c->page > 1024 || (c->page & (c->page - 1)) != 0 || c->pages < 0)
-        return fail(P2H_E_ARG, "%s: %d pages of %d tokens (a power of two, 16 .. 1024)", name, c->pages, c->page);
-    if (c->pages > 0 && (!c->K || !c->V || !aligned(c->K, 16) || !aligned(c->V, 16)))
-        return fail(P2H_E_ARG, "%s: cache memory is NULL or not 16-byte aligned", name);
-    return P2H_OK;
-}
-
-/* a cache's keys or values as one row, and whether rows share a byte with either */
-Rows cache_row(const P2hKvCache *c, const void *p)
-{
-    const size_t bytes = (size_t)c->pages * c->heads * c->page * c->head_dim * elem_size(c->dtype);
-    return Rows{(const char *)p, bytes, bytes, bytes ? 1 : 0};
-}
-bool overlap(const Rows &a, const P2hKvCache *c)
-{
-    return overlap(a, cache_row(c, c->K)) || overlap(a, cache_row(c, c->V));
-}
-
-int log2_of(int page)
-{
-    int s = 0;
-    while ((1 << s) < page) s++;
-    return s;
-}
-
-}  // namespace
 
 extern "C" {
 
@@ -297,24 +197,24 @@ int p2h_q4_gemv(int dtype, int M, int N, int K, float alpha, const void *dX, int
 
 /* ── head norms, rotation and the cache ────────────────────────────────────────────────────────────────────── */
 
-int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, const void *dQKV, int ldqkv,
+/* both entries: into a cache of rows, of 8-bit codes (q8), or into none */
+static int norm_rope(const char *name, int dtype, int T, int heads, int kv_heads, int head_dim, const void *dQKV, int ldqkv,
                      const float *dGammaQ, const float *dGammaK, float eps, int rot, int interleaved, const float *dFreq,
-                     const int *dPos, void *dQ, int ldq, void *dK, int ldk, const P2hKvCache *cache, const int *dSlots,
-                     void *stream)
+                     const int *dPos, void *dQ, int ldq, void *dK, int ldk, const P2hKvCache *rows, const P2hKvCacheQ8 *q8,
+                     const int *dSlots, void *stream)
 {
-    const char *name = "p2h_qk_norm_rope";
+    const CacheView view(rows, q8), *cache = rows || q8 ? &view : nullptr;
     if (int rc = check_heads(name, dtype, heads, kv_heads, head_dim)) return rc;
     if (T < 0 || (size_t)T * 256 >= kGridThreads) return fail(P2H_E_ARG, "%s: T = %d (below 2^24)", name, T);
     if (rot < 0 || rot > head_dim || rot % 16 != 0)
         return fail(P2H_E_ARG, "%s: rot = %d (a multiple of 16 up to head_dim = %d)", name, rot, head_dim);
     if (!(eps >= 0.0f)) return fail(P2H_E_ARG, "%s: eps = %g", name, (double)eps);
     if (cache) {
-        if (int rc = check_cache(name, cache)) return rc;
-        if (overlap(cache_row(cache, cache->K), cache_row(cache, cache->V)))
-            return fail(P2H_E_ARG, "%s: the cache's keys and values overlap", name);
-        if (cache->dtype != dtype || cache->heads != kv_heads || cache->head_dim != head_dim)
+        if (int rc = rows ? check_cache(name, rows) : check_cache(name, q8)) return rc;
+        if (overlap(*cache)) return fail(P2H_E_ARG, "%s: the cache's keys and values overlap", name);
+        if ((rows && rows->dtype != dtype) || cache->heads != kv_heads || cache->head_dim != head_dim)
             return fail(P2H_E_ARG, "%s: the cache holds %d heads of %d, type %d", name, cache->heads, cache->head_dim,
-                        cache->dtype);
+                        rows ? rows->dtype : dtype);
     }
     if (!cache && !dK) return fail(P2H_E_ARG, "%s: neither dK nor a cache takes the keys", name);
     if (T == 0) return P2H_OK;
@@ -339,38 +239,56 @@ int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, co
         if (k_in ? overlap(k, xq) || overlap(k, xv) : overlap(k, x))
             return fail(P2H_E_ARG, "%s: dK overlaps dQKV other than in place", name);
         if (overlap(q, k)) return fail(P2H_E_ARG, "%s: dQ and dK overlap", name);
-        if (cache && overlap(k, cache)) return fail(P2H_E_ARG, "%s: dK overlaps the cache", name);
+        if (cache && overlap(k, *cache)) return fail(P2H_E_ARG, "%s: dK overlaps the cache", name);
     }
-    if (cache && (overlap(x, cache) || overlap(q, cache))) return fail(P2H_E_ARG, "%s: dQKV or dQ overlaps the cache", name);
+    if (cache && (overlap(x, *cache) || overlap(q, *cache))) return fail(P2H_E_ARG, "%s: dQKV or dQ overlaps the cache", name);
     if (int rc = ensure_init()) return rc;
     p2k::RopeArgs a{};
     a.T = T; a.heads = heads; a.kv = kv_heads; a.rot = rot; a.interleaved = interleaved != 0;
     a.ldx = ldqkv; a.ldq = ldq; a.ldk = ldk; a.eps = eps;
     a.x = dQKV; a.q = dQ; a.k = dK; a.gq = dGammaQ; a.gk = dGammaK; a.freq = dFreq; a.pos = dPos;
     if (cache) {
-        a.kc = cache->K; a.vc = cache->V; a.slots = dSlots;
+        a.kc = cache->K; a.vc = cache->V; a.ks = cache->ks; a.vs = cache->vs; a.slots = dSlots;
         a.page_shift = log2_of(cache->page);
         a.slots_in_cache = (long long)cache->pages * cache->page;
     }
     hipStream_t s = stream_of(stream);
     by_type_dim(dtype, head_dim, [&](auto t, auto d) {
         constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
-        if (T <= 256) hipLaunchKernelGGL((p2k::qk_norm_rope<DT, DH, 1024>), dim3((unsigned)T), dim3(1024), 0, s, a);
-        else hipLaunchKernelGGL((p2k::qk_norm_rope<DT, DH, 256>), dim3((unsigned)T), dim3(256), 0, s, a);
+        auto go = [&](auto codes) {
+            constexpr bool Q8 = decltype(codes)::value != 0;
+            if (T <= 256) hipLaunchKernelGGL((p2k::qk_norm_rope<DT, DH, 1024, Q8>), dim3((unsigned)T), dim3(1024), 0, s, a);
+            else hipLaunchKernelGGL((p2k::qk_norm_rope<DT, DH, 256, Q8>), dim3((unsigned)T), dim3(256), 0, s, a);
+        };
+        if (q8) go(ic<1>{});
+        else go(ic<0>{});
     });
     HIPCHK(hipGetLastError());
     return P2H_OK;
 }
 
-/* ── attention ─────────────────────────────────────────────────────────────────────────────────────────────── */
-
-static int check_scale(const char *name, float scale, int window, int ahead, int sinks)
+int p2h_qk_norm_rope(int dtype, int T, int heads, int kv_heads, int head_dim, const void *dQKV, int ldqkv,
+                     const float *dGammaQ, const float *dGammaK, float eps, int rot, int interleaved, const float *dFreq,
+                     const int *dPos, void *dQ, int ldq, void *dK, int ldk, const P2hKvCache *cache, const int *dSlots,
+                     void *stream)
 {
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(P2H_E_ARG, "%s: scale = %g must be positive", name, (double)scale);
-    if (window < 1 || window > (1 << 30) || ahead < 0 || ahead > (1 << 30) || sinks < 0 || sinks > (1 << 30))
-        return fail(P2H_E_ARG, "%s: window = %d (1 .. 2^30), ahead = %d, sinks = %d (0 .. 2^30)", name, window, ahead, sinks);
-    return P2H_OK;
+    return norm_rope("p2h_qk_norm_rope", dtype, T, heads, kv_heads, head_dim, dQKV, ldqkv, dGammaQ, dGammaK, eps, rot,
+                     interleaved, dFreq, dPos, dQ, ldq, dK, ldk, cache, nullptr, dSlots, stream);
 }
+
+int p2h_qk_norm_rope_q8(int dtype, int T, int heads, int kv_heads, int head_dim, const void *dQKV, int ldqkv,
+                        const float *dGammaQ, const float *dGammaK, float eps, int rot, int interleaved, const float *dFreq,
+                        const int *dPos, void *dQ, int ldq, void *dK, int ldk, const P2hKvCacheQ8 *cache, const int *dSlots,
+                        void *stream)
+{
+    const char *name = "p2h_qk_norm_rope_q8";
+    if (!cache) return fail(P2H_E_ARG, "%s: NULL cache", name);
+    return norm_rope(name, dtype, T, heads, kv_heads, head_dim, dQKV, ldqkv, dGammaQ, dGammaK, eps, rot, interleaved, dFreq,
+                     dPos, dQ, ldq, dK, ldk, nullptr, cache, dSlots, stream);
+}
+
+
+/* ── attention ─────────────────────────────────────────────────────────────────────────────────────────────── */
 
 int p2h_attention_window(int dtype, int q_rows, int k_rows, int n_seqs, const int *dQStart, const int *dKStart, int heads,
                          int kv_heads, int head_dim, const void *dQ, int ldq, const void *dK, int ldk, const void *dV,

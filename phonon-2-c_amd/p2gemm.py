@@ -123,6 +123,19 @@ _HIP_SIG = {
                                   _i, _vp]),
     "p2h_attention_paged_workspace_bytes": (_sz, [_vp, _i, _i, _i, _i, _i]),
     "p2h_attention_paged": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _f, _i, _i, _vp, _i, _vp, _sz, _vp]),
+    "p2h_qk_norm_rope_q8": (_i, [_i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _f, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp,
+                                 _vp]),
+    "p2h_kv_rows_q8": (_i, [_i, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _vp, _i, _vp]),
+    "p2h_attention_paged_q8_workspace_bytes": (_sz, [_vp, _i, _i, _i, _i, _i]),
+    "p2h_attention_paged_q8": (_i, [_i, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _f, _i, _i, _vp, _i, _vp, _sz, _vp]),
+    "p2h_attention_shared_workspace_bytes": (_sz, [_vp, _i, _i, _i, _i, _i, _i, _i]),
+    "p2h_attention_shared": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _i, _i, _vp, _i, _vp, _sz,
+                                  _vp]),
+    "p2h_attention_shared_q8_workspace_bytes": (_sz, [_vp, _i, _i, _i, _i, _i, _i, _i]),
+    "p2h_attention_shared_q8": (_i, [_i, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _i, _i, _vp, _i,
+                                     _vp, _sz, _vp]),
+    "p2h_adapters_workspace_bytes": (_sz, [_vp, _i]),
+    "p2h_adapters_add": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _sz, _vp]),
 }
 
 _hip = None
@@ -961,6 +974,91 @@ def attention_paged_dev(cache, n_seqs, heads, dQ, ldq, dTable, table_ld, dLen, m
     """One new token per sequence over a KvCache."""
     _ok(hip().p2h_attention_paged(C.byref(cache), n_seqs, heads, dQ, ldq, dTable, table_ld, dLen, max_len, scale, window,
                                   sinks, dO, ldo, ws, ws_bytes, stream), "p2h_attention_paged")
+
+
+# ── a served batch's step: an 8-bit cache, shared prefixes, adapters ──────────────────────────────────────────────
+# As above: device-pointer entry points, asynchronous on `stream`.
+
+class KvCacheQ8(C.Structure):
+    """P2hKvCacheQ8: `pages` pages of `page` tokens of `heads` key heads as 8-bit codes at device addresses dK and dV, each
+    [pages][heads][page][head_dim], with one fp32 scale for every token's head at dKScale and dVScale, each
+    [pages][heads][page]. The memory stays the caller's."""
+    _fields_ = [("heads", _i), ("head_dim", _i), ("page", _i), ("pages", _i), ("K", _vp), ("V", _vp), ("KScale", _vp),
+                ("VScale", _vp)]
+
+    def __init__(self, heads, head_dim, page, pages, dK, dV, dKScale, dVScale):
+        super().__init__(heads, head_dim, page, pages, dK, dV, dKScale, dVScale)
+
+
+class Adapters(C.Structure):
+    """P2hAdapters: `count` low-rank adapters of a linear [K, N] at device addresses dA [count][rank][K], dB [count][N][rank]
+    and dScale [count] (fp32). The memory stays the caller's."""
+    _fields_ = [("dtype", _i), ("count", _i), ("rank", _i), ("K", _i), ("N", _i), ("A", _vp), ("B", _vp), ("scale", _vp)]
+
+    def __init__(self, dtype, count, rank, K, N, dA, dB, dScale):
+        super().__init__(TYPES.get(dtype, dtype), count, rank, K, N, dA, dB, dScale)
+
+
+def qk_norm_rope_q8_dev(dtype, T, heads, kv_heads, head_dim, dQKV, ldqkv, dGammaQ, dGammaK, eps, rot, interleaved, dFreq,
+                        dPos, dQ, ldq, dK, ldk, cache, dSlots, stream=None):
+    """qk_norm_rope_dev with the keys and values into a KvCacheQ8."""
+    _ok(hip().p2h_qk_norm_rope_q8(TYPES.get(dtype, dtype), T, heads, kv_heads, head_dim, dQKV, ldqkv, dGammaQ, dGammaK, eps,
+                                  rot, int(interleaved), dFreq, dPos, dQ, ldq, dK, ldk, C.byref(cache), dSlots, stream),
+        "p2h_qk_norm_rope_q8")
+
+
+def kv_rows_q8_dev(dtype, cache, rows, n_seqs, dStart, dTable, table_ld, dK, ldk, dV, ldv, stream=None):
+    """The first tokens that sequences keep in a KvCacheQ8 as rows dStart[s] .. dStart[s + 1] − 1 of dK and dV."""
+    _ok(hip().p2h_kv_rows_q8(TYPES.get(dtype, dtype), C.byref(cache), rows, n_seqs, dStart, dTable, table_ld, dK, ldk, dV,
+                             ldv, stream), "p2h_kv_rows_q8")
+
+
+def attention_paged_q8_workspace_bytes(cache, n_seqs, heads, max_len, window=EVERY_KEY, sinks=0):
+    return hip().p2h_attention_paged_q8_workspace_bytes(C.byref(cache), n_seqs, heads, max_len, window, sinks)
+
+
+def attention_paged_q8_dev(dtype, cache, n_seqs, heads, dQ, ldq, dTable, table_ld, dLen, max_len, scale, window, sinks, dO,
+                           ldo, ws=None, ws_bytes=0, stream=None):
+    """One new token per sequence over a KvCacheQ8."""
+    _ok(hip().p2h_attention_paged_q8(TYPES.get(dtype, dtype), C.byref(cache), n_seqs, heads, dQ, ldq, dTable, table_ld, dLen,
+                                     max_len, scale, window, sinks, dO, ldo, ws, ws_bytes, stream),
+        "p2h_attention_paged_q8")
+
+
+def attention_shared_workspace_bytes(cache, n_seqs, n_groups, heads, max_shared, max_own, window=EVERY_KEY, sinks=0):
+    return hip().p2h_attention_shared_workspace_bytes(C.byref(cache), n_seqs, n_groups, heads, max_shared, max_own, window,
+                                                      sinks)
+
+
+def attention_shared_dev(cache, n_seqs, n_groups, heads, dQ, ldq, dGroup, dShared, dTable, table_ld, dLen, max_shared,
+                         max_own, scale, window, sinks, dO, ldo, ws, ws_bytes, stream=None):
+    """One new token per sequence over a KvCache, the prefix that a group of sequences shares read once."""
+    _ok(hip().p2h_attention_shared(C.byref(cache), n_seqs, n_groups, heads, dQ, ldq, dGroup, dShared, dTable, table_ld, dLen,
+                                   max_shared, max_own, scale, window, sinks, dO, ldo, ws, ws_bytes, stream),
+        "p2h_attention_shared")
+
+
+def attention_shared_q8_workspace_bytes(cache, n_seqs, n_groups, heads, max_shared, max_own, window=EVERY_KEY, sinks=0):
+    return hip().p2h_attention_shared_q8_workspace_bytes(C.byref(cache), n_seqs, n_groups, heads, max_shared, max_own, window,
+                                                         sinks)
+
+
+def attention_shared_q8_dev(dtype, cache, n_seqs, n_groups, heads, dQ, ldq, dGroup, dShared, dTable, table_ld, dLen,
+                            max_shared, max_own, scale, window, sinks, dO, ldo, ws, ws_bytes, stream=None):
+    """attention_shared_dev over a KvCacheQ8."""
+    _ok(hip().p2h_attention_shared_q8(TYPES.get(dtype, dtype), C.byref(cache), n_seqs, n_groups, heads, dQ, ldq, dGroup,
+                                      dShared, dTable, table_ld, dLen, max_shared, max_own, scale, window, sinks, dO, ldo,
+                                      ws, ws_bytes, stream), "p2h_attention_shared_q8")
+
+
+def adapters_workspace_bytes(adapters, M):
+    return hip().p2h_adapters_workspace_bytes(C.byref(adapters), M)
+
+
+def adapters_add_dev(adapters, M, dX, ldx, dIndex, dZ, ldz, dY, ldy, ws, ws_bytes, stream=None):
+    """Y [M, N] = Z + what each row's own one of the Adapters (none outside [0, count)) makes of X [M, K]."""
+    _ok(hip().p2h_adapters_add(C.byref(adapters), M, dX, ldx, dIndex, dZ, ldz, dY, ldy, ws, ws_bytes, stream),
+        "p2h_adapters_add")
 
 
 # ── the generator ───────────────────────────────────────────────────────────────────────────────────────────────

@@ -140,3 +140,12 @@ def test_decoder_kernels_do_not_spill():
     assert len(kernels) >= 40, sorted(kernels)
     spills = {n: k[".private_segment_fixed_size"] for n, k in kernels.items() if k[".private_segment_fixed_size"]}
     assert not spills, spills
+
+
+def test_batch_kernels_do_not_spill():
+    """So do the kernels of a served batch's step."""
+    names = ("kv_rows_q8", "6attend", "attend_join", "adapter_shrink", "adapter_expand")
+    kernels = {n: k for n, k in _kernel_metadata(P.HIP_SO).items() if any(a in n for a in names)}
+    assert len(kernels) >= 40, sorted(kernels)
+    spills = {n: k[".private_segment_fixed_size"] for n, k in kernels.items() if k[".private_segment_fixed_size"]}
+    assert not spills, spills
