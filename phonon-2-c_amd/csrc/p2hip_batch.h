@@ -665,7 +665,7 @@ __global__ __launch_bounds__(256) void attend_join(BatchArgs a)
 /* ── adapters ──────────────────────────────────────────────────────────────────────────────────────────────── */
 
 struct AdapterArgs {
-    int M, N, K, count, ldx, ldz, ldy, parts, chunk;   /* parts of `chunk` dimensions of K */
+    int M, N, K, count, ldx, ldz, ldy, parts, chunk, vec;   /* parts of `chunk` dimensions of K; vec: rows of Z and Y by 16 bytes */
     const void *x, *z, *a, *b;
     const float *scale;
     const int *index;
@@ -673,16 +673,33 @@ struct AdapterArgs {
     float *h;   /* [parts][M][rank] */
 };
 
-/* The adapters of up to 16 rows, each once: f(adapter, rows), the rows as bits, in the order of their first rows. */
-template <class F> __device__ __forceinline__ void each_adapter(int mine, int rows, F f)
+/* The adapters of a workgroup's rows (up to 64), each once, with its rows as bits, in the order of their first rows; rows
+ * without one come as adapter −1. */
+struct AdapterList {
+    int n, of[64];
+    unsigned long long rows[64];
+};
+
+__device__ __forceinline__ void list_adapters(const AdapterArgs &a, int m0, int rows, AdapterList *list)
 {
-    uint32_t left = (uint32_t)__ballot((int)(threadIdx.x & 63) < rows && mine >= 0) & 0xffffu;
-    while (left) {
-        const int at = __builtin_ctz(left), ad = __builtin_amdgcn_readlane(mine, at);
-        const uint32_t those = (uint32_t)__ballot(mine == ad) & left;
-        f(ad, those);
-        left &= ~those;
+    if (threadIdx.x < 64) {
+        const int lane = threadIdx.x;
+        const int id = lane < rows ? a.index[m0 + lane] : -1, mine = (unsigned)id < (unsigned)a.count ? id : -1;
+        unsigned long long left = __ballot(lane < rows);
+        int n = 0;
+        while (left) {
+            const int ad = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+            const unsigned long long those = __ballot(mine == ad) & left;
+            if (lane == 0) {
+                list->of[n] = ad;
+                list->rows[n] = those;
+            }
+            n++;
+            left &= ~those;
+        }
+        if (lane == 0) list->n = n;
     }
+    __syncthreads();
 }
 
 /* Four steps of 4 dimensions of 16 × 16 fp32 products, or one of 32 16-bit ones */
@@ -714,115 +731,188 @@ template <int DT, bool VEC> __device__ __forceinline__ u4 row_piece(const typena
     }
 }
 
-/* H[part][m][r] = the sum over the part's dimensions k of X[m][k] · A[adapter of m][r][k], 16 rows a workgroup. */
-template <int DT, int RANK, bool VEC>
-__global__ __launch_bounds__(256) void adapter_shrink(AdapterArgs a)
+/* The sums over dimensions [k0, k1) of 16 rows of X from m0 on times their adapters' A, each adapter by a wave or, where there
+ * are fewer adapters than waves, by several that share the dimensions: sum[part][row][r], as many parts as returned. */
+template <int DT, int RANK, int NW, bool VEC>
+__device__ __forceinline__ int shrink_rows(const AdapterArgs &a, const AdapterList &list, int m0, int rows, int k0, int k1,
+                                           float (*sum)[16][RANK + 1])
 {
     typedef typename Elem<DT>::type E;
-    constexpr int VE = kPer16<DT>, STEP = 4 * VE, RT = (RANK + 15) / 16, NW = 4;
-    __shared__ float sum[NW][16][16 * RT + 1];
+    constexpr int VE = kPer16<DT>, STEP = 4 * VE, RT = (RANK + 15) / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
-    const int m0 = 16 * blockIdx.x, rows = imin(16, a.M - m0), k0 = blockIdx.y * a.chunk, k1 = imin(k0 + a.chunk, a.K);
-    const int id = a.index[m0 + imin(c, rows - 1)], mine = (unsigned)id < (unsigned)a.count ? id : -1;
+    const int n = __builtin_amdgcn_readfirstlane(list.n);
+    int sets = 1;   /* adapters at a time */
+    while (sets < n && sets < NW) sets *= 2;
+    const int parts = NW / sets, part = wave / sets;
     const E *x = static_cast<const E *>(a.x) + (size_t)(m0 + imin(c, rows - 1)) * a.ldx;
-    f4 total[RT];
-#pragma unroll
-    for (int t = 0; t < RT; t++) total[t] = f4{0, 0, 0, 0};
-    each_adapter(mine, rows, [&](int ad, uint32_t those) {
+    for (int j = wave % sets; j < n; j += sets) {
+        const int ad = __builtin_amdgcn_readfirstlane(list.of[j]);
+        if (ad < 0) continue;
+        const uint32_t those = (uint32_t)list.rows[j];
         f4 acc[RT];
 #pragma unroll
         for (int t = 0; t < RT; t++) acc[t] = f4{0, 0, 0, 0};
         const E *am = static_cast<const E *>(a.a) + (size_t)ad * RANK * a.K;
-        for (int k = k0 + STEP * wave; k < k1; k += STEP * NW) {
-            const int kk = k + VE * g;
-            if (VEC && k + STEP <= k1) {
-                const u4 xv = row_piece<DT, true>(x, kk, k1);
+        int k = k0 + STEP * part;
+        if constexpr (VEC) {
+#pragma unroll 4
+            for (; k + STEP <= k1; k += STEP * parts) {
+                const u4 xv = row_piece<DT, true>(x, k + VE * g, k1);
 #pragma unroll
                 for (int t = 0; t < RT; t++)
-                    acc[t] = mfma_piece<DT>(xv, row_piece<DT, true>(am + (size_t)imin(16 * t + c, RANK - 1) * a.K, kk, k1), acc[t]);
-            } else {
-                const u4 xv = row_piece<DT, false>(x, kk, k1);
-#pragma unroll
-                for (int t = 0; t < RT; t++)
-                    acc[t] = mfma_piece<DT>(xv, row_piece<DT, false>(am + (size_t)imin(16 * t + c, RANK - 1) * a.K, kk, k1), acc[t]);
+                    acc[t] = mfma_piece<DT>(xv, row_piece<DT, true>(am + (size_t)imin(16 * t + c, RANK - 1) * a.K, k + VE * g, k1),
+                                            acc[t]);
             }
+        }
+        for (; k < k1; k += STEP * parts) {
+            const u4 xv = row_piece<DT, false>(x, k + VE * g, k1);
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+                acc[t] = mfma_piece<DT>(xv, row_piece<DT, false>(am + (size_t)imin(16 * t + c, RANK - 1) * a.K, k + VE * g, k1),
+                                        acc[t]);
         }
 #pragma unroll
         for (int t = 0; t < RT; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if ((those >> (4 * g + i)) & 1) total[t][i] = acc[t][i];
-    });
-#pragma unroll
-    for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) sum[wave][4 * g + i][16 * t + c] = total[t][i];
+                if (((those >> (4 * g + i)) & 1) && 16 * t + c < RANK) sum[part][4 * g + i][16 * t + c] = acc[t][i];
+    }
     __syncthreads();
-    for (int e = threadIdx.x; e < rows * RANK; e += 256) {
-        const int r = e / RANK, j = e % RANK;
-        a.h[((size_t)blockIdx.y * a.M + m0 + r) * RANK + j] =
-            (sum[0][r][j] + sum[1][r][j]) + (sum[2][r][j] + sum[3][r][j]);
+    return parts;
+}
+
+/* H[part][m][r] = the sum over the part's dimensions k of X[m][k] · A[adapter of m][r][k], 16 rows a workgroup. */
+template <int DT, int RANK, int NW, bool VEC>
+__global__ __launch_bounds__(64 * NW) void adapter_shrink(AdapterArgs a)
+{
+    __shared__ float sum[NW][16][RANK + 1];
+    __shared__ AdapterList list;
+    const int m0 = 16 * blockIdx.x, rows = imin(16, a.M - m0), k0 = blockIdx.y * a.chunk;
+    list_adapters(a, m0, rows, &list);
+    const int parts = shrink_rows<DT, RANK, NW, VEC>(a, list, m0, rows, k0, imin(k0 + a.chunk, a.K), sum);
+    for (int e = threadIdx.x; e < rows * RANK; e += 64 * NW) {   /* rows without an adapter hold anything */
+        float s = 0.0f;
+        for (int p = 0; p < parts; p++) s += sum[p][e / RANK][e % RANK];
+        a.h[((size_t)blockIdx.y * a.M + m0) * RANK + e] = s;
     }
 }
 
-/* Y[m][n] = Z[m][n] + scale · the sum over r of H[m][r] · B[adapter of m][n][r]: 16 rows and 256 columns a workgroup, in fp32
- * products (B's values are exact in fp32), rounded once. */
+/* Row 4g + i of product t is this column of 64, so that a lane's results are 16 bytes of neighbours (16-bit rows: of two
+ * products) and four lanes' 64. */
+template <int DT> __device__ __forceinline__ constexpr int expand_column(int t, int r)
+{
+    return DT == T_F32 ? 16 * t + r : 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3);
+}
+
+/* 64 columns from n0 on of those of 16 rows from m0 on: Y = Z + Σ h · B, h this lane's RANK / 4 of row m0 + lane % 16 (times the
+ * adapter's scale), b its elements of B's rows, in fp32 products (B's values are exact in fp32), rounded once. */
 template <int DT, int RANK>
-__global__ __launch_bounds__(256) void adapter_expand(AdapterArgs a)
+__device__ __forceinline__ void expand_rows(const AdapterArgs &a, uint32_t those, int m0, int n0, const float (&h)[RANK / 4],
+                                            const typename Elem<DT>::type (&b)[4][RANK / 4], float (*tile)[65])
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int RS = RANK / 4, VE = kPer16<DT>, NV = 16 / VE;   /* 16-byte pieces of a lane */
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const bool whole = a.vec && n0 + 64 <= a.N, in = (those >> c) & 1;
+    const E *z = static_cast<const E *>(a.z);
+    E *y = static_cast<E *>(a.y);
+    u4 zv[NV];
+    if (whole) {
+#pragma unroll
+        for (int p = 0; p < NV; p++) {
+            zv[p] = u4{0, 0, 0, 0};
+            if (z && in) zv[p] = *reinterpret_cast<const u4 *>(z + (size_t)(m0 + c) * a.ldz + n0 + 4 * VE * p + VE * g);
+        }
+    }
+    f4 acc[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) acc[t] = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < RS; s++)
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(Elem<DT>::get(b[t][s]), h[s], acc[t], 0, 0, 0);
+    if (whole) {
+#pragma unroll
+        for (int p = 0; p < NV; p++) {
+            float v[VE];
+            unpack<DT>(zv[p], v);
+#pragma unroll
+            for (int j = 0; j < VE; j++) v[j] += acc[VE / 4 * p + j / 4][j % 4];
+            if (in) *reinterpret_cast<u4 *>(y + (size_t)(m0 + c) * a.ldy + n0 + 4 * VE * p + VE * g) = pack<DT>(v);
+        }
+    } else {
+        /* through the wave's LDS, so that lanes have neighbouring columns of one row */
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) tile[c][expand_column<DT>(t, 4 * g + i)] = acc[t][i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (n0 + lane < a.N)
+            for (uint32_t left = those; left; left &= left - 1) {
+                const int r = __builtin_ctz(left);
+                const E before = z ? z[(size_t)(m0 + r) * a.ldz + n0 + lane] : Elem<DT>::put(0.0f);
+                y[(size_t)(m0 + r) * a.ldy + n0 + lane] = Elem<DT>::put(Elem<DT>::get(before) + tile[r][lane]);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+/* Y[m][n] = Z[m][n] + scale · the sum over r of H[m][r] · B[adapter of m][n][r]: 16 · RT rows and 64 · U columns a workgroup, its
+ * waves taking an adapter's 64 columns each. FUSED: H is made here, from all of K. */
+template <int DT, int RANK, int NW, int RT, int U, bool FUSED, bool VEC>
+__global__ __launch_bounds__(64 * NW) void adapter_expand(AdapterArgs a)
 {
     typedef typename Elem<DT>::type E;
     constexpr int RS = RANK / 4;   /* a lane's elements of a row of rank: RS · g .. */
-    __shared__ float hs[16][RANK + 1];
+    __shared__ float tile[NW][16][65];
+    __shared__ AdapterList list;
+    __shared__ float sum[FUSED ? NW : 1][16][RANK + 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
-    const int m0 = 16 * blockIdx.y, rows = imin(16, a.M - m0), n0 = 256 * blockIdx.x + 64 * wave;
-    const int id = a.index[m0 + imin(c, rows - 1)], mine = (unsigned)id < (unsigned)a.count ? id : -1;
-    for (int e = threadIdx.x; e < 16 * RANK; e += 256) {
-        const int r = e / RANK;
-        float s = 0.0f;
-        if (r < rows) {
-            const int ad = a.index[m0 + r];
-            if ((unsigned)ad < (unsigned)a.count) {
-                for (int p = 0; p < a.parts; p++) s += a.h[((size_t)p * a.M + m0) * RANK + e];
-                s *= a.scale[ad];
-            }
+    const int m0 = 16 * RT * blockIdx.y, rows = imin(16 * RT, a.M - m0);
+    list_adapters(a, m0, rows, &list);
+    int parts = a.parts;
+    if constexpr (FUSED) parts = shrink_rows<DT, RANK, NW, VEC>(a, list, m0, rows, 0, a.K, sum);
+    const int n = __builtin_amdgcn_readfirstlane(list.n);
+    for (int task = wave; task < n * U; task += NW) {
+        const int j = task / U, n0 = 64 * (blockIdx.x * U + task % U), ad = __builtin_amdgcn_readfirstlane(list.of[j]);
+        if (n0 >= a.N) continue;
+        const unsigned long long all = (unsigned long long)__builtin_amdgcn_readfirstlane((int)(list.rows[j] >> 32)) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readfirstlane((int)list.rows[j]);
+        if (ad < 0) {   /* no adapter: Z as it is */
+            if (a.z == a.y && a.ldz == a.ldy) continue;
+            for (int r = 0; r < rows; r++)
+                if (((all >> r) & 1) && n0 + lane < a.N)
+                    static_cast<E *>(a.y)[(size_t)(m0 + r) * a.ldy + n0 + lane] =
+                        a.z ? static_cast<const E *>(a.z)[(size_t)(m0 + r) * a.ldz + n0 + lane] : Elem<DT>::put(0.0f);
+            continue;
         }
-        hs[r][e % RANK] = s;
+        E b[4][RS];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            __builtin_memcpy(b[t], static_cast<const E *>(a.b) +
+                                       ((size_t)ad * a.N + imin(n0 + expand_column<DT>(t, c), a.N - 1)) * RANK + RS * g, sizeof b[t]);
+        const float scale = a.scale[ad];
+        for (int q = 0; q < RT; q++) {
+            const uint32_t those = (uint32_t)(all >> (16 * q)) & 0xffffu;
+            if (RT > 1 && !those) continue;
+            float h[RS];
+#pragma unroll
+            for (int s = 0; s < RS; s++) h[s] = 0.0f;
+            if ((those >> c) & 1)
+                for (int p = 0; p < parts; p++) {
+                    const float *from = FUSED ? &sum[FUSED ? p : 0][c][RS * g]
+                                              : a.h + ((size_t)p * a.M + m0 + 16 * q + c) * RANK + RS * g;
+#pragma unroll
+                    for (int s = 0; s < RS; s++) h[s] += from[s];
+                }
+#pragma unroll
+            for (int s = 0; s < RS; s++) h[s] *= scale;
+            expand_rows<DT, RANK>(a, those, m0 + 16 * q, n0, h, b, tile[wave]);
+        }
     }
-    __syncthreads();
-    if (n0 >= a.N) return;
-    float h[RS];
-#pragma unroll
-    for (int s = 0; s < RS; s++) h[s] = hs[c][RS * g + s];
-    /* products' rows are columns of Y: row 4g + i of product t is column n0 + 16g + 4t + i, so that a lane has 16 neighbours */
-    f4 y[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) y[t] = f4{0, 0, 0, 0};
-    each_adapter(mine, rows, [&](int ad, uint32_t those) {
-        const bool in = (those >> c) & 1;
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int n = imin(n0 + 16 * (c >> 2) + 4 * t + (c & 3), a.N - 1);
-            const E *b = static_cast<const E *>(a.b) + ((size_t)ad * a.N + n) * RANK + RS * g;
-            E v[RS];
-            __builtin_memcpy(v, b, sizeof v);
-            f4 acc = {0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < RS; s++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(Elem<DT>::get(v[s]), h[s], acc, 0, 0, 0);
-            if (in) y[t] = acc;
-        }
-    });
-    if (c >= rows) return;
-    const E *z = static_cast<const E *>(a.z) + (size_t)(m0 + c) * a.ldz;
-    E *out = static_cast<E *>(a.y) + (size_t)(m0 + c) * a.ldy;
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int n = n0 + 16 * g + 4 * t + i;
-            if (n >= a.N) continue;
-            const E before = a.z ? z[n] : Elem<DT>::put(0.0f);
-            out[n] = mine < 0 ? before : Elem<DT>::put(Elem<DT>::get(before) + y[t][i]);
-        }
 }
 
 }  // namespace p2k

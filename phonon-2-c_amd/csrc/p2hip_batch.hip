@@ -291,11 +291,16 @@ static int check_adapters(const char *name, const P2hAdapters *ad, int M)
     return P2H_OK;
 }
 
-/* K over workgroups: so that there are 256 of them, at least 128 elements each. A number, as the workspace's size is asked
- * for where there may be no device. */
+/* Adapters that 16 rows may have between them, as the host knows it */
+static int adapters_of_16(const P2hAdapters *ad, int M) { return p2k::imin(p2k::imin(M, 16), p2k::imax(ad->count, 1)); }
+
+/* K over workgroups, 0: everything in one launch, each workgroup making H for itself, while that is little to read. A number,
+ * as the workspace's size is asked for where there may be no device. */
 static int adapter_parts(const P2hAdapters *ad, int M)
 {
-    const int tiles = (M + 15) / 16, most = (ad->K + 127) / 128, want = (256 + tiles - 1) / (tiles > 0 ? tiles : 1);
+    const int tiles = (M + 15) / 16, n = adapters_of_16(ad, M);
+    if (tiles <= 1 && (size_t)n * ad->rank * ad->K * elem_size(ad->dtype) <= 128 << 10) return 0;
+    const int least = n <= 2 ? 512 : 128, most = (ad->K + least - 1) / least, want = (256 + tiles - 1) / (tiles > 0 ? tiles : 1);
     return p2k::imax(p2k::imin(want, most), 1);
 }
 
@@ -320,10 +325,10 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
     if (ad->count > 0 && (!ad->A || !ad->B || !ad->scale || !aligned(ad->A, 16) || !aligned(ad->B, 16)))
         return fail(P2H_E_ARG, "%s: adapters are NULL or not 16-byte aligned", name);
     const size_t need = p2h_adapters_workspace_bytes(ad, M);
-    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return fail(P2H_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", name, workspace_bytes, need);
     const Rows x{(const char *)dX, ldx * es, K * es, M}, y{(const char *)dY, ldy * es, N * es, M};
-    const Rows z{(const char *)dZ, ldz * es, N * es, dZ ? M : 0}, ws{(const char *)workspace, need, need, 1};
+    const Rows z{(const char *)dZ, ldz * es, N * es, dZ ? M : 0}, ws{(const char *)workspace, need, need, need ? 1 : 0};
     const size_t a_bytes = (size_t)ad->count * ad->rank * K * es, b_bytes = (size_t)ad->count * ad->rank * N * es;
     const Rows am{(const char *)ad->A, a_bytes, a_bytes, a_bytes ? 1 : 0}, bm{(const char *)ad->B, b_bytes, b_bytes, b_bytes ? 1 : 0};
     const Rows sc{(const char *)ad->scale, (size_t)ad->count * 4, (size_t)ad->count * 4, ad->count ? 1 : 0};
@@ -336,18 +341,33 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
     p2k::AdapterArgs a{};
     a.M = M; a.N = N; a.K = K; a.count = ad->count; a.ldx = ldx; a.ldz = ldz; a.ldy = ldy;
     a.parts = adapter_parts(ad, M);
-    a.chunk = ((K - 1) / a.parts / 128 + 1) * 128;
+    if (a.parts) a.chunk = ((K - 1) / a.parts / 128 + 1) * 128;
     a.x = dX; a.z = dZ; a.a = ad->A; a.b = ad->B; a.scale = ad->scale; a.index = dIndex; a.y = dY; a.h = (float *)workspace;
     const bool vec = aligned(dX, 16) && (M == 1 || ldx * es % 16 == 0) && K * es % 16 == 0;
-    const unsigned tiles = (unsigned)((M + 15) / 16);
+    a.vec = aligned(dY, 16) && (M == 1 || ldy * es % 16 == 0) && (!dZ || (aligned(dZ, 16) && (M == 1 || ldz * es % 16 == 0)));
+    const unsigned tiles = (unsigned)((M + 15) / 16), columns = (unsigned)((N - 1) / 64 + 1);
+    const int n = adapters_of_16(ad, M);
     hipStream_t s = stream_of(stream);
     by_type(ad->dtype, [&](auto t) {
         auto go = [&](auto rank) {
-            constexpr int DT = decltype(t)::value, R = decltype(rank)::value;
-            const dim3 g1(tiles, (unsigned)a.parts), g2((unsigned)((N + 255) / 256), tiles);
-            if (vec) hipLaunchKernelGGL((p2k::adapter_shrink<DT, R, true>), g1, dim3(256), 0, s, a);
-            else hipLaunchKernelGGL((p2k::adapter_shrink<DT, R, false>), g1, dim3(256), 0, s, a);
-            hipLaunchKernelGGL((p2k::adapter_expand<DT, R>), g2, dim3(256), 0, s, a);
+            constexpr int DT = decltype(t)::value, R = decltype(rank)::value, NS = R <= 32 ? 16 : 8;   /* waves that registers allow */
+            auto aligned_x = [&](auto v) {
+                constexpr bool V = decltype(v)::value != 0;
+                if (!a.parts)
+                    hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 8, 1, 1, true, V>), dim3(columns, tiles), dim3(512), 0, s, a);
+                else
+                    hipLaunchKernelGGL((p2k::adapter_shrink<DT, R, NS, V>), dim3(tiles, (unsigned)a.parts), dim3(64 * NS), 0, s, a);
+            };
+            if (vec) aligned_x(ic<1>{});
+            else aligned_x(ic<0>{});
+            if (!a.parts) return;
+            if (M > 512)
+                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 4, 4, 4, false, true>), dim3((columns + 3) / 4, (tiles + 3) / 4),
+                                   dim3(256), 0, s, a);
+            else if (n > 4)
+                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, NS, 1, 1, false, true>), dim3(columns, tiles), dim3(64 * NS), 0, s, a);
+            else
+                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 4, 1, 1, false, true>), dim3(columns, tiles), dim3(256), 0, s, a);
         };
         switch (ad->rank) {
         case 8: go(ic<8>{}); break;

@@ -176,7 +176,7 @@ def adapters(**kw):
 
 
 def add(ad=None, **kw):
-    a = dict(M=5, x=A, ldx=64, index=43 * A, z=2 * A, ldz=40, y=3 * A, ldy=40, ws=50 * A, wsb=1 << 19)
+    a = dict(M=40, x=A, ldx=64, index=43 * A, z=2 * A, ldz=40, y=3 * A, ldy=40, ws=50 * A, wsb=1 << 19)
     a.update(kw)
     ad = adapters() if ad is None else ad
     return P.hip().p2h_adapters_add(C.byref(ad), *(a[n] for n in ("M", "x", "ldx", "index", "z", "ldz", "y", "ldy", "ws", "wsb")),
@@ -200,8 +200,8 @@ def test_adapters(kw, part):
 
 
 def test_adapters_workspace():
-    need = P.adapters_workspace_bytes(adapters(), 5)
-    assert need >= 5 * 16 * 4
+    need = P.adapters_workspace_bytes(adapters(), 40)
+    assert need >= 40 * 16 * 4 and P.adapters_workspace_bytes(adapters(), 5) == 0
     for kw in (dict(ws=None), dict(wsb=need - 1), dict(ws=50 * A + 8)):
         assert add(**kw) == E_WORKSPACE and "workspace" in P.last_error()
     assert P.adapters_workspace_bytes(adapters(rank=3), 5) == 0 and "rank" in P.last_error()
