@@ -119,7 +119,10 @@ struct BatchArgs {
     const float *ks, *vs;
     const int *table, *len, *group, *shared;   /* group: NULL without prefixes */
     void *o;
-    float *part;   /* [sequence][head][p_parts + o_parts][DH + 2]: sums, reference, sum of weights; NULL: one part, straight to o */
+    /* of each part the weighted sums, [sequence][head][p_parts + o_parts][DH], and their reference and the sum of weights; NULL:
+     * one part, straight to o */
+    float *part;
+    float2 *stat;
 };
 
 /* A block of keys as it lies in a wave's LDS: rows of CH pieces of 16 bytes, brought by LD direct loads of RPL rows each.
@@ -563,18 +566,320 @@ __device__ __forceinline__ void attend_item(const BatchArgs &a, const BatchItem 
         if (!a.part) {
             static_cast<E *>(a.o)[(size_t)seq * a.ldo + (size_t)head * DH + d] = Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
         } else {
-            float *to = a.part + (((size_t)seq * a.heads + head) * w.parts + w.slot) * (DH + 2);
-            to[d] = num;
-            if (d == 0) {
-                to[DH] = top;
-                to[DH + 1] = den;
-            }
+            const size_t to = ((size_t)seq * a.heads + head) * w.parts + w.slot;
+            a.part[to * DH + d] = num;
+            if (d == 0) a.stat[to] = float2{top, den};
         }
     }
 }
 
 /* group g's sequences [sa, sb) */
 __device__ __forceinline__ int group_start(const BatchArgs &a, int g) { return imin(imax(a.group[g], 0), a.n_seqs); }
+
+/* The prefix that a group shares for 128 of its query rows, 32 for each of four waves; 16-bit rows. Keys come in blocks of 64
+ * through LDS, K and V in two buffers each, each wave bringing 16 keys of both, which lie in one page.
+ *
+ * As in windowed attention, S^T = K · Q^T by 32 × 32 products, so that a lane holds 32 keys of one row and its weights are laid
+ * out as the operand of O^T += V^T · P^T; the scores of block b run together with the output product of block b − 1, in
+ * stages of equal length, each stage's operands read from LDS two stages ahead and one of the next loads issued in each; the
+ * reference of the exponentials is raised only where a block's sum of weights leaves the type's range. One barrier a block. */
+constexpr int kTileRows = 128;
+template <int DT> constexpr float kTileLift = DT == T_F16 ? 6.0f : 0.0f;          /* fp16 weights up to 2^6 below … */
+template <int DT> constexpr float kTileSlack = DT == T_F16 ? 65504.0f : 1024.0f;  /* … a sum that every type holds */
+
+template <int DT, int DH> constexpr int tile_lds() { return 4 * 64 * DH * 2; }
+
+template <int DT, int DH>
+__device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem &w, unsigned char *lds)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int KB = 64, CH = DH / 8, RPL = 64 / CH, LD = 16 / RPL, QR = DH / 16, NT = DH / 32, RB = 2 * DH;
+    constexpr uint32_t BUF = KB * RB;
+    static_assert(2 * LD == QR, "one load a stage");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+    const int G = a.heads / a.kv;
+    auto k_place = [](int r, int p) { return p ^ (CH == 16 ? r & 15 : (r >> 1) & 7); };
+    auto v_place = [](int r, int p) { return p ^ (CH == 16 ? 4 * (r & 3) : 4 * ((r >> 1) & 1)); };
+
+    const int r = imin(32 * wave + col, w.rows - 1), seq = w.seq0 + (w.r0 + r) / G, head = w.kvh * G + (w.r0 + r) % G;
+    const int len = a.pages ? kept_length(a.len[seq], a.table_ld, 1 << a.page_shift) : 0;
+    u4 q[QR];
+    {
+        const E *row = static_cast<const E *>(a.q) + (size_t)seq * a.ldq + (size_t)head * DH;
+#pragma unroll
+        for (int x = 0; x < QR; x++) q[x] = *reinterpret_cast<const u4 *>(row + 8 * (2 * x + h));
+    }
+    /* of the wave's rows, and of all rows (the first one's sequence to the last one's) */
+    int wave_least = len, wave_most = len, least = 1 << 30, most = 0;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        wave_least = imin(wave_least, __shfl_xor(wave_least, o));
+        wave_most = imax(wave_most, __shfl_xor(wave_most, o));
+    }
+    for (int s = w.seq0 + w.r0 / G + lane; s <= w.seq0 + (w.r0 + w.rows - 1) / G; s += 64) {
+        const int n = a.pages ? kept_length(a.len[s], a.table_ld, 1 << a.page_shift) : 0;
+        least = imin(least, n);
+        most = imax(most, n);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        least = imin(least, __shfl_xor(least, o));
+        most = imax(most, __shfl_xor(most, o));
+    }
+    wave_least = __builtin_amdgcn_readfirstlane(wave_least);
+    wave_most = __builtin_amdgcn_readfirstlane(wave_most);
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+    const int end_key = imin(most, w.t1);
+    const KeyBlocks blocks = key_blocks(least - a.window, end_key, a.sinks, KB);
+    int b0, b1;
+    split_range(blocks.total, w.splits, w.split, &b0, &b1);
+
+    /* where 16 keys lie: of block b those that this wave brings, and which of the block's four sixteens are in a page */
+    struct Entries {
+        int mine, e[4];
+    };
+    auto entry = [&](int key) __attribute__((always_inline)) {
+        const int i = key >> a.page_shift;
+        return i < a.table_ld ? scalar_int(w.pages + i) : -1;
+    };
+    auto hint = [&](int b) __attribute__((always_inline)) {
+        const int k0 = blocks.at(b) * KB;
+        return Entries{entry(k0 + 16 * wave), {entry(k0), entry(k0 + 16), entry(k0 + 32), entry(k0 + 48)}};
+    };
+    auto token_of = [&](int b, const Entries &n) __attribute__((always_inline)) {
+        const int key = blocks.at(b) * KB + 16 * wave, page = imax(page_in(n.mine, a.pages), 0);
+        return ((((size_t)page * a.kv + w.kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * RB;
+    };
+    auto there = [&](const Entries &n) __attribute__((always_inline)) {
+        unsigned long long bits = 0;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            if (page_in(n.e[t], a.pages) >= 0) bits |= 0xffffull << (16 * t);
+        return bits;
+    };
+    uint32_t koff[LD], voff[LD];
+#pragma unroll
+    for (int x = 0; x < LD; x++) {
+        const int rr = RPL * x + lane / CH;
+        koff[x] = rr * RB + 16 * k_place(rr, lane % CH);
+        voff[x] = rr * RB + 16 * v_place(rr, lane % CH);
+    }
+    auto fetch = [&](int x, const unsigned char *from, const uint32_t (&off)[LD], uint32_t buffer) __attribute__((always_inline)) {
+        dma_16(from, off[x], lds + buffer * BUF + 16 * wave * RB + 1024 * x);
+    };
+    const unsigned char *kc = static_cast<const unsigned char *>(a.kc), *vc = static_cast<const unsigned char *>(a.vc);
+
+    f16v o[NT], s[2];
+    u4 pw[4];
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) pw[k] = u4{0, 0, 0, 0};
+    bool odd = false;
+
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
+    const int vr = 4 * h + ((lane & 15) >> 2);
+    const uint32_t k_at = lds0 + col * RB + 16 * k_place(col, h);
+    const uint32_t v_at = lds0 + 2 * BUF + vr * RB + 16 * v_place(vr, 0) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    auto read_k = [&](uint32_t at, int n, int x) __attribute__((always_inline)) {
+        typedef __attribute__((address_space(3))) const u4 *lds16;
+        return *(lds16)(uintptr_t)((at ^ (32 * x)) + 32 * n * RB);
+    };
+    auto read_v = [&](uint32_t at, int k2, int d) __attribute__((always_inline)) {
+        const uint32_t x = (at ^ (64 * d)) + 16 * k2 * RB;
+        const u2 va = lds_tr(x), vb = lds_tr(x + 8 * RB);
+        return u4{va[0], va[1], vb[0], vb[1]};
+    };
+    /* whether rows of lengths from lo to hi see all of the block at k0 */
+    auto all_seen = [&](int k0, int lo, int hi) __attribute__((always_inline)) {
+        return k0 + KB <= imin(lo, w.t1) && (k0 >= hi - a.window || k0 + KB <= a.sinks);
+    };
+    /* this wave's loads have come; of V of block b, where some row must not see a key, what no row sees and what is not finite
+     * becomes zeros, which `odd` notes of the latter: a weight of 0 times them would be a NaN */
+    auto come = [&](int b, unsigned long long held) __attribute__((always_inline)) {
+        wait_vm<0>();
+        if (b >= b0) {
+            const int k0 = blocks.at(b) * KB;
+            if (held != ~0ull || !all_seen(k0, least, most)) {
+                u4 *v = reinterpret_cast<u4 *>(lds + (2 + ((b - b0) & 1)) * BUF + 16 * wave * RB) + lane;
+#pragma unroll
+                for (int x = 0; x < LD; x++) {
+                    const int e = 16 * wave + RPL * x + lane / CH, key = k0 + e;
+                    const bool keep = ((held >> e) & 1) && key < end_key && (key >= least - a.window || key < a.sinks);
+                    if (!keep) {
+                        v[64 * x] = u4{0, 0, 0, 0};
+                    } else if (odd_values<DT>(v[64 * x])) {
+                        odd = true;
+                        v[64 * x] = only_finite<DT>(v[64 * x]);
+                    }
+                }
+            }
+        }
+        lds_barrier();
+    };
+    /* what a row must not see: key e of the block is bit e of 64; this lane has keys 8j + 4h .. + 3 of every eight */
+    auto mask = [&](int k0, unsigned long long held) __attribute__((always_inline)) {
+        if (held == ~0ull && all_seen(k0, wave_least, wave_most)) return;
+        auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
+        const unsigned long long bits = (below(imin(len, w.t1) - k0) & (~below(len - a.window - k0) | below(a.sinks - k0)) & held) >> (4 * h);
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const uint32_t seen = (uint32_t)__builtin_amdgcn_sbfe((int)(bits >> (32 * n)), 8 * (i / 4) + i % 4, 1);
+                s[n][i] = __uint_as_float((__float_as_uint(s[n][i]) & seen) | (0xff800000u & ~seen));
+            }
+    };
+    auto weights = [&](int k, float mu, float &sum) __attribute__((always_inline)) {
+        float pv[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) pv[i] = exp2_fast(__builtin_fmaf(s[k / 2][8 * (k & 1) + i], a.c, -mu));
+        sum += ((pv[0] + pv[1]) + (pv[2] + pv[3])) + ((pv[4] + pv[5]) + (pv[6] + pv[7]));
+        pw[k] = pack<DT>(pv);
+    };
+    auto settle = [&](float sum) __attribute__((always_inline)) {
+        if (__any(sum > kTileSlack<DT> || m == -INFINITY)) {
+            float top = s[0][0];
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
+            const float mn = fmaxf(m, lifted(max_halves(top), a.c, kTileLift<DT>)), mu = mn == -INFINITY ? 0.0f : mn;
+            const float fade = exp2_fast(m - mu);
+            m = mn;
+            l *= fade;
+#pragma unroll
+            for (int d = 0; d < NT; d++) o[d] *= fade;
+            sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) weights(k, mu, sum);
+        }
+        l += sum;
+    };
+    if (b0 < b1) {
+        Entries now = hint(b0);
+        {
+            const unsigned char *from = kc + token_of(b0, now);
+#pragma unroll
+            for (int x = 0; x < LD; x++) fetch(x, from, koff, 0);
+        }
+        Entries next = hint(imin(b0 + 1, b1 - 1));
+        unsigned long long held = there(now), held_before = 0;
+        /* the first block has no weights before it: zeros, with zeros for V */
+        for (int x = threadIdx.x; x < KB * CH; x += 256) reinterpret_cast<u4 *>(lds + 3 * BUF)[x] = u4{0, 0, 0, 0};
+        for (int b = b0; b < b1; b++) {
+            const int k0 = blocks.at(b) * KB, odd_block = (b - b0) & 1;
+            /* past the last block that one's K again, which nothing reads */
+            const unsigned char *next_k = kc + token_of(imin(b + 1, b1 - 1), next), *this_v = vc + token_of(b, now);
+            const uint32_t ka = k_at + odd_block * BUF, va = v_at + (odd_block ^ 1) * BUF;
+            u4 kf[3][2], vf[3][2];
+            auto read = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    kf[t % 3][j] = read_k(ka, j, t);
+                    vf[t % 3][j] = read_v(va, (2 * t + j) / NT, (2 * t + j) % NT);
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[0][i] = s[1][i] = 0.0f;
+            come(b - 1, held_before);
+            const Entries after = hint(imin(b + 2, b1 - 1));
+            __builtin_amdgcn_s_setprio(1);   /* products first: the other wave's exponentials fill what they leave */
+            read(0);
+            read(1);
+#pragma unroll
+            for (int t = 0; t < QR; t++) {   /* the barriers to the scheduler keep this order */
+                if (t + 2 < QR) read(t + 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int z = 2 * t + j;
+                    s[j] = mfma32<DT>(kf[t % 3][j], q[t], s[j]);
+                    o[z % NT] = mfma32<DT>(vf[t % 3][j], pw[z / NT], o[z % NT]);
+                }
+                if (t < LD) fetch(t, next_k, koff, odd_block ^ 1);
+                else fetch(t - LD, this_v, voff, 2 + odd_block);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            mask(k0, held);
+            const float mu = m == -INFINITY ? 0.0f : m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) weights(k, mu, sum);
+            settle(sum);
+            held_before = held;
+            now = next;
+            next = after;
+            held = there(now);
+        }
+        come(b1 - 1, held_before);
+        const uint32_t va = v_at + ((b1 - 1 - b0) & 1) * BUF;
+#pragma unroll
+        for (int k2 = 0; k2 < 4; k2++)
+#pragma unroll
+            for (int d = 0; d < NT; d++) o[d] = mfma32<DT>(read_v(va, k2, d), pw[k2], o[d]);
+    }
+    odd = __syncthreads_or(odd);
+    const float sum = sum_halves(l);
+    if (32 * wave + col >= w.rows) return;
+    const size_t to = ((size_t)seq * a.heads + head) * w.parts + w.slot;
+    if (odd) {   /* rare, so simple: any positive weight of an infinity or a NaN is that */
+        for (int b = b0; b < b1; b++)
+            for (int key = blocks.at(b) * KB; key < blocks.at(b) * KB + KB; key++) {
+                const int page = page_in(page_entry(w.pages, a.table_ld, key, a.page_shift), a.pages);
+                if (page < 0 || key >= imin(len, w.t1) || !(key >= len - a.window || key < a.sinks)) continue;
+                const size_t token = (((size_t)page * a.kv + w.kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+#pragma unroll
+                for (int d = 0; d < NT; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float x = Elem<DT>::get(static_cast<const E *>(a.vc)[token * DH + 32 * d + 8 * (i / 4) + 4 * h + i % 4]);
+                        if (!(__builtin_fabsf(x) < INFINITY)) o[d][i] += x;
+                    }
+            }
+    }
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            *reinterpret_cast<f4 *>(a.part + to * DH + 32 * d + 8 * i + 4 * h) = f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+    if (h == 0) a.stat[to] = float2{m, sum};
+}
+
+/* this workgroup's tile of TR rows of a group's prefix; false where there is none */
+template <int TR> __device__ __forceinline__ bool prefix_item(const BatchArgs &a, BatchItem *w)
+{
+    const int G = a.heads / a.kv, id = blockIdx.x / a.kv, tile = id % a.p_tiles;
+    w->kvh = blockIdx.x % a.kv;
+    w->split = id / a.p_tiles;
+    /* tiles are numbered as tile_start does, rows being G for each sequence */
+    const int gr = wave_last(a.n_groups, [&](int s) { return group_start(a, s) * G / TR + s <= tile; });
+    if (gr < 0) return false;
+    const int sa = group_start(a, gr), sb = imax(group_start(a, gr + 1), sa);
+    w->r0 = (tile - (sa * G / TR + gr)) * TR;
+    if (w->r0 >= (sb - sa) * G) return false;
+    w->seq0 = sa;
+    w->rows = imin(TR, (sb - sa) * G - w->r0);
+    w->t0 = 0;
+    w->t1 = imax(a.shared[gr], 0);
+    w->pages = a.table + (size_t)sa * a.table_ld;
+    w->splits = a.p_parts;
+    w->slot = w->split;
+    w->parts = a.p_parts + a.o_parts;
+    return true;
+}
+
+template <int DT, int DH> __global__ __launch_bounds__(256, 2) void attend_prefix(BatchArgs a)
+{
+    __shared__ __align__(16) unsigned char lds[tile_lds<DT, DH>()];
+    BatchItem w;
+    if (prefix_item<kTileRows>(a, &w)) attend_tile<DT, DH>(a, w, lds);
+}
 
 template <int CK, int DT, int DH, int NQ, int NW>
 __global__ __launch_bounds__(64 * NW) void attend(BatchArgs a)
@@ -583,26 +888,7 @@ __global__ __launch_bounds__(64 * NW) void attend(BatchArgs a)
     const int G = a.heads / a.kv;
     BatchItem w;
     if ((int)blockIdx.x < a.p_wgs) {
-        constexpr int TR = 16 * NQ;
-        const int id = blockIdx.x / a.kv;
-        w.kvh = blockIdx.x % a.kv;
-        w.split = id / a.p_tiles;
-        const int tile = id % a.p_tiles;
-        /* tiles are numbered as tile_start does, rows being G for each sequence */
-        const int gr = wave_last(a.n_groups, [&](int s) { return group_start(a, s) * G / TR + s <= tile; });
-        if (gr < 0) return;
-        const int sa = group_start(a, gr), sb = imax(group_start(a, gr + 1), sa);
-        w.r0 = (tile - (sa * G / TR + gr)) * TR;
-        if (w.r0 >= (sb - sa) * G) return;
-        w.seq0 = sa;
-        w.rows = imin(TR, (sb - sa) * G - w.r0);
-        w.t0 = 0;
-        w.t1 = imax(a.shared[gr], 0);
-        w.pages = a.table + (size_t)sa * a.table_ld;
-        w.splits = a.p_parts;
-        w.slot = w.split;
-        w.parts = a.p_parts + a.o_parts;
-        attend_item<CK, DT, DH, NQ, NW>(a, w, lds);
+        if (prefix_item<16 * NQ>(a, &w)) attend_item<CK, DT, DH, NQ, NW>(a, w, lds);
         return;
     }
     int id = blockIdx.x - a.p_wgs;
@@ -623,7 +909,7 @@ __global__ __launch_bounds__(64 * NW) void attend(BatchArgs a)
         const int gr = wave_last(a.n_groups, [&](int s) { return group_start(a, s) <= w.seq0; });
         if (gr < 0 || w.seq0 >= group_start(a, gr + 1)) {   /* in no group: attend_join leaves its rows as they are */
             if (w.split == 0 && threadIdx.x < w.rows)
-                a.part[(((size_t)w.seq0 * a.heads + w.kvh * G + w.r0 + threadIdx.x) * w.parts + w.slot) * (DH + 2) + DH + 1] = -1.0f;
+                a.stat[((size_t)w.seq0 * a.heads + w.kvh * G + w.r0 + threadIdx.x) * w.parts + w.slot] = float2{0.0f, -1.0f};
             return;
         }
         w.t0 = imax(a.shared[gr], 0);
@@ -639,10 +925,11 @@ __global__ __launch_bounds__(256) void attend_join(BatchArgs a)
     constexpr int PER = DH / 64;
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, parts = a.p_parts + a.o_parts;
     if (row >= a.n_seqs * a.heads) return;
-    const float *p = a.part + (size_t)row * parts * (DH + 2);
-    if (p[(size_t)a.p_parts * (DH + 2) + DH + 1] < 0.0f) return;   /* a sequence of no group */
+    const float *p = a.part + (size_t)row * parts * DH + PER * lane;
+    const float2 *st = a.stat + (size_t)row * parts;
+    if (st[a.p_parts].y < 0.0f) return;   /* a sequence of no group */
     float top = -INFINITY;
-    for (int s = lane; s < parts; s += 64) top = fmaxf(top, p[(size_t)s * (DH + 2) + DH]);
+    for (int s = lane; s < parts; s += 64) top = fmaxf(top, st[s].x);
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
     const float mu = top == -INFINITY ? 0.0f : top;
@@ -651,11 +938,11 @@ __global__ __launch_bounds__(256) void attend_join(BatchArgs a)
     for (int i = 0; i < PER; i++) num[i] = 0.0f;
 #pragma unroll 8
     for (int s = 0; s < parts; s++) {
-        const float *j = p + (size_t)s * (DH + 2);
-        const float f = exp2_fast(j[DH] - mu);
+        const float2 of = st[s];
+        const float f = exp2_fast(of.x - mu);
 #pragma unroll
-        for (int i = 0; i < PER; i++) num[i] = __builtin_fmaf(f, j[PER * lane + i], num[i]);
-        den = __builtin_fmaf(f, j[DH + 1], den);
+        for (int i = 0; i < PER; i++) num[i] = __builtin_fmaf(f, p[(size_t)s * DH + i], num[i]);
+        den = __builtin_fmaf(f, of.y, den);
     }
     E *o = static_cast<E *>(a.o) + (size_t)(row / a.heads) * a.ldo + (size_t)(row % a.heads) * DH + PER * lane;
 #pragma unroll

@@ -17,10 +17,11 @@ constexpr int kWaves = 4;   /* of a workgroup of attend */
 /* How the queries and keys of a call go over workgroups. */
 struct Plan {
     int p_tiles = 0, p_parts = 0, q_groups = 1, o_parts = 1;
+    bool tiled = false;   /* prefixes by tiles of p2k::kTileRows rows */
     int parts() const { return p_parts + o_parts; }
     size_t bytes(int n_seqs, int heads, int head_dim) const
     {
-        return (size_t)n_seqs * heads * parts() * (head_dim + 2) * 4;
+        return (size_t)n_seqs * heads * parts() * (head_dim + 2) * 4;   /* sums, reference, sum of weights */
     }
 };
 
@@ -54,9 +55,11 @@ Plan shared_plan(const CacheView &c, bool q8, int dtype, int n_seqs, int n_group
     Plan p;
     const int G = heads / c.heads, kb = block_of(q8, dtype);
     p.q_groups = (G + 15) / 16;
-    p.p_tiles = n_seqs * G / 16 + n_groups;
     const int rows = n_groups ? (n_seqs * G + n_groups - 1) / n_groups : 0;   /* of a group, as the host knows them */
-    p.p_parts = parts_of((long long)n_groups * ((rows + 15) / 16) * c.heads, left_of(max_shared, window, sinks), kb);
+    p.tiled = !q8 && dtype != P2H_F32 && rows > 32;
+    const int tr = p.tiled ? p2k::kTileRows : 16;
+    p.p_tiles = n_seqs * G / tr + n_groups;
+    p.p_parts = parts_of((long long)n_groups * ((rows + tr - 1) / tr) * c.heads, left_of(max_shared, window, sinks), kb);
     p.o_parts = parts_of((long long)n_seqs * c.heads * p.q_groups, left_of(max_own, window, sinks), kb);
     return p;
 }
@@ -108,21 +111,26 @@ int attention(const char *name, int dtype, const CacheView &c, bool q8, const Pl
         overlap(o, ints(dGroup, 1, n_groups + 1)) || overlap(o, ints(dShared, 1, n_groups)))
         return fail(P2H_E_ARG, "%s: dO overlaps lengths, pages or groups", name);
     const size_t p_wgs = (size_t)plan.p_tiles * plan.p_parts * c.heads;
-    const size_t wgs = p_wgs + (size_t)n_seqs * plan.q_groups * plan.o_parts * c.heads;
-    if (wgs * 64 * kWaves >= kGridThreads || (size_t)n_seqs * heads >= 1u << 23)
+    const size_t o_wgs = (size_t)n_seqs * plan.q_groups * plan.o_parts * c.heads, wgs = (plan.tiled ? 0 : p_wgs) + o_wgs;
+    if ((p_wgs + o_wgs) * 64 * kWaves >= kGridThreads || (size_t)n_seqs * heads >= 1u << 23)
         return fail(P2H_E_ARG, "%s: %d sequences of %d heads are too many for one call", name, n_seqs, heads);
     if (int rc = ensure_init()) return rc;
     p2k::BatchArgs a{};
     a.n_seqs = n_seqs; a.n_groups = n_groups; a.heads = heads; a.kv = c.heads; a.page_shift = log2_of(c.page);
     a.pages = c.pages; a.table_ld = table_ld; a.ldq = ldq; a.ldo = ldo; a.window = window; a.sinks = sinks;
-    a.p_tiles = plan.p_tiles; a.p_parts = plan.p_parts; a.p_wgs = (int)p_wgs;
+    a.p_tiles = plan.p_tiles; a.p_parts = plan.p_parts; a.p_wgs = plan.tiled ? 0 : (int)p_wgs;
     a.q_groups = plan.q_groups; a.o_parts = plan.o_parts; a.c = scale * p2k::kLog2e;
     a.q = dQ; a.kc = c.K; a.vc = c.V; a.ks = c.ks; a.vs = c.vs;
     a.table = dTable; a.len = dLen; a.group = dGroup; a.shared = dShared; a.o = dO;
     a.part = parted ? (float *)workspace : nullptr;
+    a.stat = parted ? (float2 *)(a.part + (size_t)n_seqs * heads * plan.parts() * c.head_dim) : nullptr;
     hipStream_t s = stream_of(stream);
     by_type_dim(dtype, c.head_dim, [&](auto t, auto d) {
         constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
+        if constexpr (DT != p2k::T_F32) {
+            if (plan.tiled)
+                hipLaunchKernelGGL((p2k::attend_prefix<DT, DH>), dim3((unsigned)p_wgs), dim3(256), 0, s, a);
+        }
         if (q8) hipLaunchKernelGGL((p2k::attend<p2k::C_Q8, DT, DH, 1, kWaves>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, s, a);
         else hipLaunchKernelGGL((p2k::attend<p2k::C_ROWS, DT, DH, 1, kWaves>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, s, a);
         if (parted)

@@ -289,7 +289,10 @@ SHARED = [  # groups of (shared, lengths); heads, key heads, page, window, sinks
     ([(700, (701, 900, 1500)), (650, (2000,))], 8, 8, 16, 300, 0),
     ([(700, (701, 900, 1500, 640)), (10, (20, 300))], 4, 1, 16, 90, 25),
     ([(50, (300, 500)), (90, (95, 200))], 20, 1, 256, 64, 130),
-    ([(2100, (2101, 2200, 3000) * 12)], 4, 4, 1024, EVERY, 7)]
+    ([(2100, (2101, 2200, 3000) * 12)], 4, 4, 1024, EVERY, 7),
+    ([(700, (701, 900, 640, 0, 1100, 33) * 7)], 8, 2, 16, 250, 70),      # many rows: tiles
+    ([(333, (334,) * 33), (90, (95, 40) * 20), (1, (2,) * 50)], 16, 4, 32, EVERY, 0),
+    ([(1500, (1501, 1600) * 40)], 4, 1, 64, 1300, 0)]
 
 
 def shared_case(t, groups, H, Hk, page, Dh, key="s", before=0, behind=0):
@@ -301,7 +304,7 @@ def shared_case(t, groups, H, Hk, page, Dh, key="s", before=0, behind=0):
     for _, g in groups:
         at += len(g)
         starts.append(at)
-    needs, kind = [], []
+    needs = []
     for s in range(len(lens)):
         needs.append(-(-lens[s] // page))
     for g, (m, _) in enumerate(groups):   # the first one's row holds the whole prefix, whatever its own length
@@ -312,7 +315,6 @@ def shared_case(t, groups, H, Hk, page, Dh, key="s", before=0, behind=0):
         for s in range(starts[g] + 1, starts[g + 1]):
             n = min(m // page, needs[s])
             table[s, :n] = table[starts[g], :n]
-    del kind
     reach = list(lens)
     for g, (m, _) in enumerate(groups):
         if starts[g] < starts[g + 1]:
@@ -382,10 +384,11 @@ def test_shared_many_groups(kind, n):
 
 
 @pytest.mark.parametrize("t", D.TYPES)
-def test_shared_values_that_are_not_finite(t):
+@pytest.mark.parametrize("H,Dh", ((2, 64), (20, 64), (40, 128)))
+def test_shared_values_that_are_not_finite(t, H, Dh):
     """Infinities and NaN among the kept values reach the sequences that see them, and no others, in a prefix of which a
-    window leaves each sequence another part, and in what is each one's own."""
-    H, Hk, page, Dh, window = 2, 1, 16, 64, 60
+    window leaves each sequence another part, and in what is each one's own; few rows and many."""
+    Hk, page, window = 1, 16, 60
     groups = [(100, (101, 120, 150, 190))]
     rng, lens, starts, shared, table, pages, reach = shared_case(t, groups, H, Hk, page, Dh, "odd")
     kc, vc = (D.rows(rng, t, pages, Hk, page, Dh) for _ in range(2))
@@ -403,11 +406,12 @@ def test_shared_values_that_are_not_finite(t):
 
 
 @pytest.mark.parametrize("kind", ("rows", "q8"))
-def test_shared_device_arrays_outside_their_ranges(kind):
+@pytest.mark.parametrize("H", (4, 64))
+def test_shared_device_arrays_outside_their_ranges(kind, H):
     """Lengths, prefixes, pages and groups that no program means reach nothing outside the buffers."""
-    t, H, Hk, page, Dh = "bf16", 4, 2, 16, 64
+    t, Hk, page, Dh = "bf16", 2, 16, 64
     rng, lens, starts, shared, table, pages, reach = shared_case(t, [(40, (41, 50, 77))], H, Hk, page, Dh)
-    cache, K, V = shared_cache(rng, t, kind, pages, Hk, page, Dh, table, [table.shape[1] * page] * 0 or reach)
+    cache, K, V = shared_cache(rng, t, kind, pages, Hk, page, Dh, table, reach)
     q = D.rows(rng, t, 3, H * Dh)
     big = 2 ** 31 - 1
     for st, sh, ln in (([0, 3], [big], [big, -big, 50]), ([0, 3], [-big], lens), ([-big, big], [40], lens),
@@ -421,6 +425,20 @@ def test_shared_device_arrays_outside_their_ranges(kind):
     a = B.run_shared(t, q, cache, starts, [10 ** 6], full, [10 ** 6, 20, 0], H, 0.1, EVERY, 0, 40, 60)
     b = B.run_shared(t, q, cache, starts, [32], full, [32, 20, 0], H, 0.1, EVERY, 0, 40, 60)
     assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("kind", ("rows", "q8"))
+@pytest.mark.parametrize("H", (4, 48))
+def test_shared_pages_that_are_not_there(t, kind, H):
+    """Tokens of a page number outside the cache are not seen, in the prefix by nobody, behind it by their own sequence."""
+    Hk, page, Dh = 2, 16, 64
+    rng, lens, starts, shared, table, pages, reach = shared_case(t, [(200, (201, 230, 260, 150))], H, Hk, page, Dh, "holes")
+    table[0, 3], table[0, 9], table[1, 13], table[2, 14] = -1, pages, 2 ** 31 - 1, -9
+    cache, K, V = shared_cache(rng, t, kind, pages, Hk, page, Dh, np.where((table < 0) | (table >= pages), 0, table), reach)
+    q = D.rows(rng, t, 4, H * Dh)
+    want, bound = B.paged_want(t, q, K, V, table, lens, H, 0.1, EVERY, 0, kind == "q8", starts, shared)
+    D.check(D.to_f64(t, B.run_shared(t, q, cache, starts, shared, table, lens, H, 0.1, EVERY, 0, 200, 60)), want, bound, t)
 
 
 @pytest.mark.parametrize("Dh", (64, 128))
