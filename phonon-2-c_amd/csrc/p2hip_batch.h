@@ -11,6 +11,7 @@
 
 #include "p2hip_async.h"
 #include "p2hip_elem.h"
+#include "p2hip_few.h"
 #include "p2hip_index.h"
 
 namespace p2k {
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(256) void kv_rows_q8(KvRowsArgs a)
 
 /* ── one query per sequence over pages ─────────────────────────────────────────────────────────────────────── */
 
-enum { C_ROWS = 0, C_Q8 = 1 };
+enum { C_ROWS = 0, C_Q8 = 1 };   /* a cache of rows, of codes */
 
 struct BatchArgs {
     int n_seqs, n_groups, heads, kv, page_shift, pages, table_ld, ldq, ldo, window, sinks;
@@ -125,26 +126,17 @@ struct BatchArgs {
     float2 *stat;
 };
 
-/* A block of keys as it lies in a wave's LDS: rows of CH pieces of 16 bytes, brought by LD direct loads of RPL rows each.
- * Pieces are moved within a row so that operand reads fall into different banks: k_place for 16 keys' reads of one piece,
- * v_place for V's (16 bits: 32 bytes of 8 rows; codes: 64 bytes of 4 rows; fp32: whole rows). */
-template <int CK, int DT, int DH> struct KeptBlock {
-    static constexpr bool Q8 = CK == C_Q8, F32 = !Q8 && DT == T_F32;
-    static constexpr int KB = F32 ? 16 : 32, NB = KB / 16, RB = Q8 ? DH : F32 ? 4 * DH : 2 * DH, CH = RB / 16, RPL = 64 / CH,
-                         LD = KB / RPL, BYTES = KB * RB, STAGE = 2 * BYTES + (Q8 ? 256 : 0), LOADS = 2 * LD + Q8;
-    static __device__ __forceinline__ constexpr int k_place(int r, int p)
-    {
-        return p ^ (CH >= 16 ? r & 15 : (r / (16 / (CH < 16 ? CH : 16))) & (CH - 1));
-    }
-    static __device__ __forceinline__ constexpr int v_place(int r, int p)
-    {
-        if (F32) return p;
-        if (Q8) return CH == 8 ? p ^ (4 * ((r >> 1) & 1)) : p;
-        return p ^ (CH == 16 ? 2 * (r & 7) : 2 * ((r >> 1) & 3));
-    }
-    /* the key of a block that product t has in row m: a lane's results are rows 4g + i, of codes so that its four groups of
-     * lanes have neighbouring keys */
-    static __device__ __forceinline__ constexpr int key_of(int t, int m) { return 16 * t + (Q8 ? 4 * (m & 3) + (m >> 2) : m); }
+/* A block of 32 keys' codes as it lies in a wave's LDS: rows of CH pieces of 16 bytes, brought by LD direct loads of RPL rows
+ * each, and their scales. Pieces are moved within a row so that operand reads fall into different banks: k_place for one piece
+ * of 16 keys, v_place for 64 bytes of 4 keys. */
+template <int DH> struct CodeBlock {
+    static constexpr int KB = 32, CH = DH / 16, RPL = 64 / CH, LD = KB / RPL, BYTES = KB * DH, STAGE = 2 * BYTES + 256,
+                         LOADS = 2 * LD + 1;
+    static __device__ __forceinline__ constexpr int k_place(int r, int p) { return p ^ ((r / (16 / CH)) & (CH - 1)); }
+    static __device__ __forceinline__ constexpr int v_place(int r, int p) { return CH == 8 ? p ^ (4 * ((r >> 1) & 1)) : p; }
+    /* the key of a block that product t has in row m: a lane's results are rows 4g + i, its four groups of lanes having
+     * neighbouring keys */
+    static __device__ __forceinline__ constexpr int key_of(int t, int m) { return 16 * t + 4 * (m & 3) + (m >> 2); }
 };
 
 /* the upper halves of two floats, of a in the lower half */
@@ -199,87 +191,231 @@ struct BatchItem {
     const int *pages;
 };
 
-template <int CK, int DT, int DH, int NQ, int NW> constexpr int attend_lds()
+/* its rows' lengths: this lane's (row lane % 16 of every 16), and of all of them the least and the largest */
+template <int NQ> struct RowLengths {
+    int of[NQ], least, most;
+    __device__ __forceinline__ RowLengths(const BatchArgs &a, const BatchItem &w)
+    {
+        const int G = a.heads / a.kv;
+        least = 1 << 30;
+        most = 0;
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const int r = w.r0 + imin(16 * n + (int)(threadIdx.x & 15), w.rows - 1);
+            of[n] = a.pages ? kept_length(a.len[w.seq0 + r / G], a.table_ld, 1 << a.page_shift) : 0;
+            least = imin(least, of[n]);
+            most = imax(most, of[n]);
+        }
+        if (w.r0 / G != (w.r0 + w.rows - 1) / G) {   /* more than one sequence */
+#pragma unroll
+            for (int o = 1; o < 16; o *= 2) {
+                least = imin(least, __shfl_xor(least, o));
+                most = imax(most, __shfl_xor(most, o));
+            }
+        }
+        least = __builtin_amdgcn_readfirstlane(least);
+        most = __builtin_amdgcn_readfirstlane(most);
+    }
+};
+
+/* The item's blocks of KB keys: those that a row of lengths least .. most sees something of, counted from the block that t0
+ * lies in, and the part [b0, b1) of them. */
+struct ItemBlocks {
+    int tb, end_key, b0, b1;
+    KeyBlocks blocks;
+    __device__ __forceinline__ ItemBlocks(const BatchArgs &a, const BatchItem &w, int least, int most, int kb)
+    {
+        tb = w.t0 & ~(kb - 1);
+        end_key = imin(most, w.t1);
+        blocks = key_blocks(imax(least - a.window, w.t0) - tb, end_key - tb, imax(a.sinks - tb, 0), kb);
+        split_range(blocks.total, w.splits, w.split, &b0, &b1);
+    }
+    __device__ __forceinline__ int key(int b, int kb) const { return tb + blocks.at(b) * kb; }
+};
+
+/* whether a row of that length sees a key, if a page holds it */
+__device__ __forceinline__ bool item_sees(const BatchArgs &a, const BatchItem &w, int key, int len)
 {
-    constexpr int V = NW * 2 * KeptBlock<CK, DT, DH>::STAGE, J = NW * 16 * NQ * (DH + 2) * 4;
+    return key >= w.t0 && key < imin(len, w.t1) && (key >= len - a.window || key < a.sinks);
+}
+/* whether rows of lengths least .. most see all n keys from k0 on */
+__device__ __forceinline__ bool item_sees_all(const BatchArgs &a, const BatchItem &w, int k0, int n, int least, int most)
+{
+    return k0 >= w.t0 && k0 + n <= imin(least, w.t1) && (k0 >= most - a.window || k0 + n <= a.sinks);
+}
+
+/* the place of a token of this item's key head among all heads' tokens, in a page that is there */
+__device__ __forceinline__ size_t token_at(const BatchArgs &a, const BatchItem &w, int page, int key)
+{
+    return (((size_t)page * a.kv + w.kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+}
+
+/* The sum of the values of dimension d that are not finite, among the keys of the blocks that a row of that length sees. Such
+ * values enter products as zeros where some row must not see them; what they do to those that do is added afterwards: any
+ * positive weight of an infinity or a NaN is that. Rare, so simple. */
+template <int DT, int DH>
+__device__ __forceinline__ float odd_values_of(const BatchArgs &a, const BatchItem &w, const ItemBlocks &in, int kb, int len, int d)
+{
+    typedef typename Elem<DT>::type E;
+    float more = 0.0f;
+    for (int b = in.b0; b < in.b1; b++)
+        for (int key = in.key(b, kb); key < in.key(b, kb) + kb; key++) {
+            const int page = page_in(page_entry(w.pages, a.table_ld, key, a.page_shift), a.pages);
+            if (page < 0 || !item_sees(a, w, key, len)) continue;
+            const float x = Elem<DT>::get(static_cast<const E *>(a.vc)[token_at(a, w, page, key) * DH + d]);
+            if (!(__builtin_fabsf(x) < INFINITY)) more += x;
+        }
+    return __builtin_fabsf(more) < INFINITY ? 0.0f : more;
+}
+
+/* one output of the item: straight to o, or as part of it */
+template <int DT, int DH>
+__device__ __forceinline__ void put_part(const BatchArgs &a, const BatchItem &w, int r, int d, float top, float num, float den)
+{
+    typedef typename Elem<DT>::type E;
+    const int G = a.heads / a.kv, seq = w.seq0 + (w.r0 + r) / G, head = w.kvh * G + (w.r0 + r) % G;
+    if (!a.part) {
+        static_cast<E *>(a.o)[(size_t)seq * a.ldo + (size_t)head * DH + d] = Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
+    } else {
+        const size_t to = ((size_t)seq * a.heads + head) * w.parts + w.slot;
+        a.part[to * DH + d] = num;
+        if (d == 0) a.stat[to] = float2{top, den};
+    }
+}
+
+/* An item of up to 16 rows over a cache of rows. */
+template <int DT, int DH, int NW>
+__device__ __forceinline__ void attend_rows(const BatchArgs &a, const BatchItem &w, unsigned char *lds)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int NB = FewPlace<DT>::NB, KB = FewPlace<DT>::KB, EPC = kPer16<DT>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+    const int G = a.heads / a.kv;
+    const RowLengths<1> len(a, w);
+    const ItemBlocks in(a, w, len.least, len.most, KB);
+    u4 q[DH / (4 * EPC)];
+    {
+        const int r = w.r0 + imin(lane & 15, w.rows - 1);
+        const E *p = static_cast<const E *>(a.q) + (size_t)(w.seq0 + r / G) * a.ldq + (size_t)(w.kvh * G + r % G) * DH;
+#pragma unroll
+        for (int s = 0; s < DH / (4 * EPC); s++) q[s] = *reinterpret_cast<const u4 *>(p + EPC * (4 * s + g));
+    }
+    FewState<DH> st;
+    bool odd = false;
+    struct Entries {
+        int e[NB];
+    };
+    auto there = [](const FewPlace<DT> &b, int k) __attribute__((always_inline)) { return b.there[NB == 2 ? k >> 4 : 0]; };
+    few_blocks<DT, DH, true>(
+        st, q, a.c, in.b0 + wave, in.b1, NW, DH, DH,
+        [&](int b) __attribute__((always_inline)) {
+            Entries n;   /* pages hold a multiple of 16 tokens */
+#pragma unroll
+            for (int t = 0; t < NB; t++) {
+                const int key = in.key(b, KB) + 16 * t;
+                n.e[t] = key < in.end_key ? page_entry(w.pages, a.table_ld, key, a.page_shift) : -1;
+            }
+            return n;
+        },
+        [&](int b, Entries n) __attribute__((always_inline)) {
+            FewPlace<DT> p;
+            p.k0 = in.key(b, KB);
+            p.whole = item_sees_all(a, w, p.k0, KB, len.least, len.most);
+#pragma unroll
+            for (int t = 0; t < NB; t++) {
+                const int page = page_in(n.e[t], a.pages);
+                const size_t at = token_at(a, w, imax(page, 0), p.k0 + 16 * t) * DH;
+                p.have[t] = 16;
+                p.there[t] = page >= 0;
+                p.k[t] = static_cast<const E *>(a.kc) + at;
+                p.v[t] = static_cast<const E *>(a.vc) + at;
+                p.whole &= page >= 0;
+            }
+            return p;
+        },
+        [&](const FewPlace<DT> &b, int k) __attribute__((always_inline)) {
+            return there(b, k) && item_sees(a, w, b.k0 + k, len.of[0]);
+        },
+        [&](const FewPlace<DT> &b, int k) __attribute__((always_inline)) {   /* seen by some row */
+            const int key = b.k0 + k;
+            return there(b, k) && key >= w.t0 && key < in.end_key && (key >= len.least - a.window || key < a.sinks);
+        },
+        odd, lds + wave * few_own_bytes<DT, DH>());
+    odd = __syncthreads_or(odd);
+    float *J = reinterpret_cast<float *>(lds);
+    few_store<DT, DH>(st, J);
+    for (int e = threadIdx.x; e < w.rows * DH; e += 64 * NW) {
+        const int r = e / DH, d = e % DH;
+        float top, num, den;
+        few_join<DH, NW>(J, r, d, &top, &num, &den);
+        if (odd) {
+            const int n = kept_length(a.len[w.seq0 + (w.r0 + r) / G], a.table_ld, 1 << a.page_shift);
+            num += odd_values_of<DT, DH>(a, w, in, KB, n, d);
+        }
+        put_part<DT, DH>(a, w, r, d, top, num, den);
+    }
+}
+
+template <int DH, int NQ, int NW> constexpr int codes_lds()
+{
+    constexpr int V = NW * 2 * CodeBlock<DH>::STAGE, J = NW * 16 * NQ * (DH + 2) * 4;
     return V > J ? V : J;
 }
 
-template <int CK, int DT, int DH, int NQ, int NW>
-__device__ __forceinline__ void attend_item(const BatchArgs &a, const BatchItem &w, unsigned char *lds)
+/* An item of up to 16 · NQ rows over a cache of codes. Each wave takes blocks of 32 keys in turn, its next block on its way into
+ * its own LDS while it multiplies one: S^T = K · Q^T and O^T += V^T · P^T by 16 × 16 × 32 products, codes as 16-bit operands (whole
+ * numbers up to 127 are exact), which one conversion and half a permutation make of each. The scales of K multiply the
+ * scores, those of V the weights.
+ *
+ * Nothing is lost but what is said here: fp32 queries and weights go in as three bf16 pieces that sum to them (queries down
+ * to 2^-110), fp16 queries as they are and their weights as two pieces, 16 bits (as one of fp16, a weight times its scale would
+ * leave the type's range), bf16 weights rounded to bf16. */
+template <int DT, int DH, int NQ, int NW>
+__device__ __forceinline__ void attend_codes(const BatchArgs &a, const BatchItem &w, unsigned char *lds)
 {
     typedef typename Elem<DT>::type E;
-    typedef KeptBlock<CK, DT, DH> B;
-    constexpr bool Q8 = B::Q8, F32 = B::F32;
-    constexpr int NB = B::NB, KB = B::KB, CH = B::CH, RPL = B::RPL, LD = B::LD, NT = DH / 16;
-    /* operands of a query: fp32 rows 16-byte pieces; 16-bit rows and codes one of 8 values for every 32 dimensions, codes of
-     * fp32 rows three bf16 pieces each */
-    constexpr int NP = Q8 && DT == T_F32 ? 3 : 1, QS = F32 ? DH / 16 : DH / 32;
-    constexpr int WP = !Q8 ? 1 : DT == T_F32 ? 3 : DT == T_F16 ? 2 : 1;   /* pieces of a weight times V's scale */
+    typedef CodeBlock<DH> B;
+    constexpr int KB = B::KB, CH = B::CH, RPL = B::RPL, LD = B::LD, NT = DH / 16, KT = DT == T_F16 ? T_F16 : T_BF16;
+    constexpr int NP = DT == T_F32 ? 3 : 1, WP = DT == T_F32 ? 3 : DT == T_F16 ? 2 : 1;   /* pieces of a query, of a weight */
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, x16 = lane & 15;
     const int G = a.heads / a.kv;
 
-    int len[NQ];
-    u4 q[NQ][QS][NP];
-    int least = 1 << 30, most = 0;
+    const RowLengths<NQ> len(a, w);
+    const ItemBlocks in(a, w, len.least, len.most, KB);
+    u4 q[NQ][DH / 32][NP];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
-        const int r = w.r0 + imin(16 * n + x16, w.rows - 1), seq = w.seq0 + r / G;
-        len[n] = a.pages ? kept_length(a.len[seq], a.table_ld, 1 << a.page_shift) : 0;
-        least = imin(least, len[n]);
-        most = imax(most, len[n]);
-        const E *row = static_cast<const E *>(a.q) + (size_t)seq * a.ldq + (size_t)(w.kvh * G + r % G) * DH;
+        const int r = w.r0 + imin(16 * n + x16, w.rows - 1);
+        const E *row = static_cast<const E *>(a.q) + (size_t)(w.seq0 + r / G) * a.ldq + (size_t)(w.kvh * G + r % G) * DH;
 #pragma unroll
-        for (int s = 0; s < QS; s++) {
-            if constexpr (!Q8) {
-                q[n][s][0] = *reinterpret_cast<const u4 *>(row + kPer16<DT> * (4 * s + g));
+        for (int s = 0; s < DH / 32; s++) {
+            const E *p = row + 64 * (s / 2) + 16 * g + 8 * (s % 2);   /* in the order of the codes' pieces */
+            if constexpr (DT == T_F32) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = p[i];
+                bf16_pieces<3>(v, q[n][s]);
             } else {
-                const E *p = row + 64 * (s / 2) + 16 * g + 8 * (s % 2);   /* in the order of the codes' pieces */
-                if constexpr (DT == T_F32) {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = p[i];
-                    bf16_pieces<3>(v, q[n][s]);
-                } else {
-                    q[n][s][0] = *reinterpret_cast<const u4 *>(p);
-                }
+                q[n][s][0] = *reinterpret_cast<const u4 *>(p);
             }
         }
     }
-    if (w.r0 / G != (w.r0 + w.rows - 1) / G) {
-#pragma unroll
-        for (int o = 1; o < 16; o *= 2) {
-            least = imin(least, __shfl_xor(least, o));
-            most = imax(most, __shfl_xor(most, o));
-        }
-    }
-    least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
-
-    /* blocks are counted from the one that t0 lies in */
-    const int tb = w.t0 & ~(KB - 1), end_key = imin(most, w.t1);
-    const KeyBlocks blocks = key_blocks(imax(least - a.window, w.t0) - tb, end_key - tb, imax(a.sinks - tb, 0), KB);
-    int b0, b1;
-    split_range(blocks.total, w.splits, w.split, &b0, &b1);
 
     struct Place {
         int k0;
-        bool there[NB], whole;
+        bool there[2], whole;
     };
     struct Entries {
-        int e[NB];
+        int e[2];
     };
     auto hint = [&](int b) __attribute__((always_inline)) {
         Entries n;   /* pages hold a multiple of 16 tokens */
 #pragma unroll
-        for (int t = 0; t < NB; t++) {
-            const int i = (tb + blocks.at(b) * KB + 16 * t) >> a.page_shift;
+        for (int t = 0; t < 2; t++) {
+            const int i = (in.key(b, KB) + 16 * t) >> a.page_shift;
             n.e[t] = i < a.table_ld ? scalar_int(w.pages + i) : -1;
         }
         return n;
-    };
-    auto seen_by = [&](int key, int ln) __attribute__((always_inline)) {   /* of those in pages that are there */
-        return key >= w.t0 && key < imin(ln, w.t1) && (key >= ln - a.window || key < a.sinks);
     };
 
     unsigned char *const own = lds + wave * 2 * B::STAGE;
@@ -287,30 +423,28 @@ __device__ __forceinline__ void attend_item(const BatchArgs &a, const BatchItem 
 #pragma unroll
     for (int x = 0; x < LD; x++) {
         const int r = RPL * x + lane / CH;
-        koff[x] = (r & 15) * B::RB + 16 * B::k_place(r, lane % CH);
-        voff[x] = (r & 15) * B::RB + 16 * B::v_place(r, lane % CH);
+        koff[x] = (r & 15) * DH + 16 * B::k_place(r, lane % CH);
+        voff[x] = (r & 15) * DH + 16 * B::v_place(r, lane % CH);
     }
     auto fetch = [&](int b, const Entries &n, unsigned char *to) __attribute__((always_inline)) {
         Place p;
-        p.k0 = tb + blocks.at(b) * KB;
-        p.whole = p.k0 >= w.t0 && p.k0 + KB <= imin(least, w.t1) && (p.k0 >= most - a.window || p.k0 + KB <= a.sinks);
-        size_t token[NB];
+        p.k0 = in.key(b, KB);
+        p.whole = item_sees_all(a, w, p.k0, KB, len.least, len.most);
+        size_t token[2];
 #pragma unroll
-        for (int t = 0; t < NB; t++) {
-            const int key = p.k0 + 16 * t, page = page_in(n.e[t], a.pages);
-            p.there[t] = page >= 0 && key < end_key;
+        for (int t = 0; t < 2; t++) {
+            const int page = page_in(n.e[t], a.pages);
+            p.there[t] = page >= 0;
             p.whole &= page >= 0;
-            token[t] = (((size_t)imax(page, 0) * a.kv + w.kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+            token[t] = token_at(a, w, imax(page, 0), p.k0 + 16 * t);
         }
         const unsigned char *kc = static_cast<const unsigned char *>(a.kc), *vc = static_cast<const unsigned char *>(a.vc);
 #pragma unroll
-        for (int x = 0; x < LD; x++) dma_16(kc + token[RPL * x / 16] * B::RB, koff[x], to + 1024 * x);
-        if constexpr (Q8) {   /* K's 32 scales and V's, in the order of a lane's results */
-            const int key = B::key_of(0, lane & 15);
-            dma_4((lane < 32 ? a.ks : a.vs) + (lane & 16 ? token[1] : token[0]) + key, to + 2 * B::BYTES);
-        }
+        for (int x = 0; x < LD; x++) dma_16(kc + token[RPL * x / 16] * DH, koff[x], to + 1024 * x);
+        /* K's 32 scales and V's, in the order of a lane's results */
+        dma_4((lane < 32 ? a.ks : a.vs) + (lane & 16 ? token[1] : token[0]) + B::key_of(0, lane & 15), to + 2 * B::BYTES);
 #pragma unroll
-        for (int x = 0; x < LD; x++) dma_16(vc + token[RPL * x / 16] * B::RB, voff[x], to + B::BYTES + 1024 * x);
+        for (int x = 0; x < LD; x++) dma_16(vc + token[RPL * x / 16] * DH, voff[x], to + B::BYTES + 1024 * x);
         return p;
     };
 
@@ -323,12 +457,11 @@ __device__ __forceinline__ void attend_item(const BatchArgs &a, const BatchItem 
 #pragma unroll
         for (int d = 0; d < NT; d++) o[n][d] = f4{0, 0, 0, 0};
     }
-    bool odd = false;
 
-    int b = b0 + wave;
-    if (b < b1) {
+    int b = in.b0 + wave;
+    if (b < in.b1) {
         Place now = fetch(b, hint(b), own), next = now;
-        Entries ahead = hint(imin(b + NW, b1 - 1));
+        Entries ahead = hint(imin(b + NW, in.b1 - 1));
         int stage = 0;
         auto block = [&](auto last) __attribute__((always_inline)) {
             constexpr bool MORE = !decltype(last)::value;
@@ -336,189 +469,99 @@ __device__ __forceinline__ void attend_item(const BatchArgs &a, const BatchItem 
             if constexpr (MORE) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   /* what reads of the other stage brought */
                 next = fetch(b + NW, ahead, own + (stage ^ 1) * B::STAGE);
-                ahead = hint(imin(b + 2 * NW, b1 - 1));
+                ahead = hint(imin(b + 2 * NW, in.b1 - 1));
             }
-            wait_vm<(MORE ? B::LOADS : 0) + LD>();
-            f4 s[NQ][NB];
+            wait_vm<(MORE ? B::LOADS : 0) + LD>();   /* all but V's, and the next block's */
+            f4 s[NQ][2];
 #pragma unroll
-            for (int n = 0; n < NQ; n++)
+            for (int n = 0; n < NQ; n++) s[n][0] = s[n][1] = f4{0, 0, 0, 0};
 #pragma unroll
-                for (int t = 0; t < NB; t++) s[n][t] = f4{0, 0, 0, 0};
-#pragma unroll
-            for (int t = 0; t < NB; t++) {
+            for (int t = 0; t < 2; t++) {
                 const int row = B::key_of(t, x16);
-                const unsigned char *kr = Ks + row * B::RB;
-                if constexpr (Q8) {
 #pragma unroll
-                    for (int x = 0; x < QS / 2; x++) {
-                        const u4 k = *reinterpret_cast<const u4 *>(kr + 16 * B::k_place(row, 4 * x + g));
+                for (int x = 0; x < DH / 64; x++) {
+                    const u4 k = *reinterpret_cast<const u4 *>(Ks + row * DH + 16 * B::k_place(row, 4 * x + g));
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const u4 kf = code_operand<DT == T_F16 ? T_F16 : T_BF16>(k[2 * e], k[2 * e + 1]);
-#pragma unroll
-                            for (int n = 0; n < NQ; n++)
-#pragma unroll
-                                for (int p = 0; p < NP; p++)
-                                    s[n][t] = mfma16<DT == T_F16 ? T_F16 : T_BF16>(kf, q[n][2 * x + e][p], s[n][t]);
-                        }
-                    }
-                } else if constexpr (F32) {
-#pragma unroll
-                    for (int x = 0; x < QS; x++) {
-                        const u4 k = *reinterpret_cast<const u4 *>(kr + 16 * B::k_place(row, 4 * x + g));
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-#pragma unroll
-                            for (int n = 0; n < NQ; n++)
-                                s[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[e]),
-                                                                               __uint_as_float(q[n][x][0][e]), s[n][t], 0, 0, 0);
-                    }
-                } else {
-#pragma unroll
-                    for (int x = 0; x < QS; x++) {
-                        const u4 k = *reinterpret_cast<const u4 *>(kr + 16 * B::k_place(row, 4 * x + g));
-#pragma unroll
-                        for (int n = 0; n < NQ; n++) s[n][t] = mfma16<DT>(k, q[n][x][0], s[n][t]);
-                    }
-                }
-            }
-            f4 vs[NB];
-            if constexpr (Q8) {
-                const f4 *sc = reinterpret_cast<const f4 *>(Ks + 2 * B::BYTES);
-#pragma unroll
-                for (int t = 0; t < NB; t++) {
-                    const f4 ks = sc[4 * t + g];
-                    vs[t] = sc[8 + 4 * t + g];
-#pragma unroll
-                    for (int n = 0; n < NQ; n++) s[n][t] *= ks;
-                }
-            }
-            float wt[NQ][4 * NB];
-            u4 pw[NQ][WP];
-#pragma unroll
-            for (int n = 0; n < NQ; n++) {
-                bool in[4 * NB];
-                if (!now.whole) {
-#pragma unroll
-                    for (int t = 0; t < NB; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            in[4 * t + i] = now.there[t] && seen_by(now.k0 + B::key_of(t, 4 * g + i), len[n]);
-                            if (!in[4 * t + i]) s[n][t][i] = -INFINITY;
-                        }
-                }
-                float top = s[n][0][0];
-#pragma unroll
-                for (int t = 0; t < NB; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) top = fmaxf(top, s[n][t][i]);
-                const float mn = fmaxf(m[n], lifted(max_quarters(top), a.c, Q8 ? 0.0f : kLift<DT>));
-                const float mu = mn == -INFINITY ? 0.0f : mn, fade = exp2_fast(m[n] - mu);
-                m[n] = mn;
-                float sum = 0.0f;
-#pragma unroll
-                for (int t = 0; t < NB; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float x = exp2_fast(__builtin_fmaf(s[n][t][i], a.c, -mu));
-                        sum += x;
-                        wt[n][4 * t + i] = x;
-                    }
-                l[n] = __builtin_fmaf(l[n], fade, sum);
-#pragma unroll
-                for (int d = 0; d < NT; d++) o[n][d] *= fade;
-                if constexpr (Q8) {
-                    float wv[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        wv[i] = wt[n][i] * vs[i / 4][i % 4];
-                        if (!now.whole && !in[i]) wv[i] = 0.0f;   /* whatever the scale of what is not seen */
-                    }
-                    bf16_pieces<WP>(wv, pw[n]);
-                } else if constexpr (!F32) {
-                    pw[n][0] = pack<DT>(wt[n]);
-                }
-            }
-            wait_vm<MORE ? B::LOADS : 0>();
-            if constexpr (!Q8) {
-                if (!now.whole) {
-                    /* a weight of 0 times what is not finite would be a NaN: rows that no query sees become zeros, and of the
-                     * others what is not finite, which `odd` notes */
-                    u4 *v = reinterpret_cast<u4 *>(own + stage * B::STAGE + B::BYTES) + lane;
-#pragma unroll
-                    for (int x = 0; x < LD; x++) {
-                        const int key = now.k0 + RPL * x + lane / CH;
-                        const bool keep = now.there[RPL * x / 16] && key >= w.t0 && key < end_key &&
-                                          (key >= least - a.window || key < a.sinks);
-                        if (!keep) {
-                            v[64 * x] = u4{0, 0, 0, 0};
-                        } else if (odd_values<DT>(v[64 * x])) {
-                            odd = true;
-                            v[64 * x] = only_finite<DT>(v[64 * x]);
-                        }
-                    }
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    __builtin_amdgcn_wave_barrier();
-                }
-            }
-            if constexpr (Q8) {
-#pragma unroll
-                for (int h = 0; h < DH / 64; h++) {
-                    uint32_t dw[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int row = B::key_of(j / 4, 4 * g + j % 4);
-                        dw[j] = *reinterpret_cast<const uint32_t *>(Vs + row * B::RB + 16 * B::v_place(row, 4 * h + x16 / 4) +
-                                                                    4 * (x16 % 4));
-                    }
-                    auto tile = [&](auto jj) __attribute__((always_inline)) {
-                        constexpr int J = decltype(jj)::value;
-                        u4 vf;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) vf[i] = upper_halves(code_at<J>(dw[2 * i]), code_at<J>(dw[2 * i + 1]));
+                    for (int e = 0; e < 2; e++) {
+                        const u4 kf = code_operand<KT>(k[2 * e], k[2 * e + 1]);
 #pragma unroll
                         for (int n = 0; n < NQ; n++)
 #pragma unroll
-                            for (int p = 0; p < WP; p++) o[n][4 * h + J] = mfma16<T_BF16>(vf, pw[n][p], o[n][4 * h + J]);
-                    };
-                    tile(std::integral_constant<int, 0>{});
-                    tile(std::integral_constant<int, 1>{});
-                    tile(std::integral_constant<int, 2>{});
-                    tile(std::integral_constant<int, 3>{});
-                }
-            } else if constexpr (F32) {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int h = 0; h < DH / 64; h++) {
-                        const u4 v = *reinterpret_cast<const u4 *>(Vs + (4 * g + i) * B::RB + 16 * (16 * h + x16));
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-#pragma unroll
-                            for (int n = 0; n < NQ; n++)
-                                o[n][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[e]), wt[n][i],
-                                                                                       o[n][4 * h + e], 0, 0, 0);
+                            for (int p = 0; p < NP; p++) s[n][t] = mfma16<KT>(kf, q[n][2 * x + e][p], s[n][t]);
                     }
-            } else {
-                const int r = 4 * g + (x16 >> 2);
-#pragma unroll
-                for (int d = 0; d < NT; d++) {
-                    const unsigned char *at = Vs + r * B::RB + 16 * B::v_place(r, 2 * d + ((x16 & 3) >> 1)) + 8 * (x16 & 1);
-                    const u2 va = lds_tr(reinterpret_cast<const uint16_t *>(at)),
-                             vb = lds_tr(reinterpret_cast<const uint16_t *>(at + 16 * B::RB));
-#pragma unroll
-                    for (int n = 0; n < NQ; n++) o[n][d] = mfma16<DT>(u4{va[0], va[1], vb[0], vb[1]}, pw[n][0], o[n][d]);
                 }
+            }
+            const f4 *sc = reinterpret_cast<const f4 *>(Ks + 2 * B::BYTES);
+            f4 vs[2];
+            u4 pw[NQ][WP];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const f4 ks = sc[4 * t + g];
+                vs[t] = sc[8 + 4 * t + g];
+#pragma unroll
+                for (int n = 0; n < NQ; n++) s[n][t] *= ks;
+            }
+#pragma unroll
+            for (int n = 0; n < NQ; n++) {
+                bool seen[8];
+                if (!now.whole) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        seen[i] = now.there[i / 4] && item_sees(a, w, now.k0 + B::key_of(i / 4, 4 * g + i % 4), len.of[n]);
+                        if (!seen[i]) s[n][i / 4][i % 4] = -INFINITY;
+                    }
+                }
+                float top = s[n][0][0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) top = fmaxf(top, s[n][i / 4][i % 4]);
+                const float mn = fmaxf(m[n], max_quarters(top) * a.c);
+                const float mu = mn == -INFINITY ? 0.0f : mn, fade = exp2_fast(m[n] - mu);
+                m[n] = mn;
+                float wv[8], sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float x = exp2_fast(__builtin_fmaf(s[n][i / 4][i % 4], a.c, -mu));
+                    sum += x;
+                    wv[i] = x * vs[i / 4][i % 4];
+                    if (!now.whole && !seen[i]) wv[i] = 0.0f;   /* whatever the scale of what is not seen */
+                }
+                l[n] = __builtin_fmaf(l[n], fade, sum);
+#pragma unroll
+                for (int d = 0; d < NT; d++) o[n][d] *= fade;
+                bf16_pieces<WP>(wv, pw[n]);
+            }
+            wait_vm<MORE ? B::LOADS : 0>();
+#pragma unroll
+            for (int h = 0; h < DH / 64; h++) {
+                uint32_t dw[8];   /* four neighbouring dimensions of each of the lane's keys, one for each of four products */
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int row = B::key_of(j / 4, 4 * g + j % 4);
+                    dw[j] = *reinterpret_cast<const uint32_t *>(Vs + row * DH + 16 * B::v_place(row, 4 * h + x16 / 4) + 4 * (x16 % 4));
+                }
+                auto product = [&](auto jj) __attribute__((always_inline)) {
+                    constexpr int J = decltype(jj)::value;
+                    u4 vf;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) vf[i] = upper_halves(code_at<J>(dw[2 * i]), code_at<J>(dw[2 * i + 1]));
+#pragma unroll
+                    for (int n = 0; n < NQ; n++)
+#pragma unroll
+                        for (int p = 0; p < WP; p++) o[n][4 * h + J] = mfma16<T_BF16>(vf, pw[n][p], o[n][4 * h + J]);
+                };
+                product(std::integral_constant<int, 0>{});
+                product(std::integral_constant<int, 1>{});
+                product(std::integral_constant<int, 2>{});
+                product(std::integral_constant<int, 3>{});
             }
             now = next;
             stage ^= 1;
         };
-        for (; b + NW < b1; b += NW) block(std::false_type{});
+        for (; b + NW < in.b1; b += NW) block(std::false_type{});
         block(std::true_type{});
     }
 
-    if constexpr (!Q8) odd = __syncthreads_or(odd);
-    else __syncthreads();   /* the waves' own parts are done with */
+    __syncthreads();   /* the waves' own parts are done with */
     float *J = reinterpret_cast<float *>(lds);   /* [wave][16 · NQ rows][DH + 2] */
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
@@ -527,8 +570,7 @@ __device__ __forceinline__ void attend_item(const BatchArgs &a, const BatchItem 
 #pragma unroll
         for (int d = 0; d < NT; d++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                mine[Q8 || F32 ? 64 * (d / 4) + 4 * (4 * g + i) + d % 4 : 16 * d + 4 * g + i] = o[n][d][i];
+            for (int i = 0; i < 4; i++) mine[64 * (d / 4) + 4 * (4 * g + i) + d % 4] = o[n][d][i];
         if (g == 0) {
             mine[DH] = m[n];
             mine[DH + 1] = sum;
@@ -536,41 +578,23 @@ __device__ __forceinline__ void attend_item(const BatchArgs &a, const BatchItem 
     }
     __syncthreads();
     for (int e = threadIdx.x; e < w.rows * DH; e += 64 * NW) {
-        const int r = e / DH, d = e % DH, seq = w.seq0 + (w.r0 + r) / G, head = w.kvh * G + (w.r0 + r) % G;
-        float top = -INFINITY, num = 0.0f, den = 0.0f;
-#pragma unroll
-        for (int v = 0; v < NW; v++) top = fmaxf(top, J[(v * 16 * NQ + r) * (DH + 2) + DH]);
-        const float mu = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int v = 0; v < NW; v++) {
-            const float *j = J + (v * 16 * NQ + r) * (DH + 2);
-            const float f = exp2_fast(j[DH] - mu);
-            num = __builtin_fmaf(f, j[d], num);
-            den = __builtin_fmaf(f, j[DH + 1], den);
-        }
-        if constexpr (!Q8) {
-            if (odd) {   /* rare, so simple: any positive weight of an infinity or a NaN is that */
-                const int ln = kept_length(a.len[seq], a.table_ld, 1 << a.page_shift);
-                float more = 0.0f;
-                for (int bb = b0; bb < b1; bb++)
-                    for (int key = tb + blocks.at(bb) * KB; key < tb + blocks.at(bb) * KB + KB; key++) {
-                        const int page = page_in(page_entry(w.pages, a.table_ld, key, a.page_shift), a.pages);
-                        if (page < 0 || !seen_by(key, ln)) continue;
-                        const size_t token = (((size_t)page * a.kv + w.kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
-                        const float x = Elem<DT>::get(static_cast<const E *>(a.vc)[token * DH + d]);
-                        if (!(__builtin_fabsf(x) < INFINITY)) more += x;
-                    }
-                if (!(__builtin_fabsf(more) < INFINITY)) num += more;
-            }
-        }
-        if (!a.part) {
-            static_cast<E *>(a.o)[(size_t)seq * a.ldo + (size_t)head * DH + d] = Elem<DT>::put(den == 0.0f ? 0.0f : num / den);
-        } else {
-            const size_t to = ((size_t)seq * a.heads + head) * w.parts + w.slot;
-            a.part[to * DH + d] = num;
-            if (d == 0) a.stat[to] = float2{top, den};
-        }
+        const int r = e / DH, d = e % DH;
+        float top, num, den;
+        few_join<DH, NW, 16 * NQ>(J, r, d, &top, &num, &den);
+        put_part<DT, DH>(a, w, r, d, top, num, den);
     }
+}
+
+/* An item over a cache of either kind: 16 · NQ rows of codes, 16 of rows. */
+template <int CK, int DT, int DH, int NQ, int NW> constexpr int attend_lds()
+{
+    return CK == C_Q8 ? codes_lds<DH, NQ, NW>() : few_lds_bytes<DT, DH, NW>();
+}
+template <int CK, int DT, int DH, int NQ, int NW>
+__device__ __forceinline__ void attend_item(const BatchArgs &a, const BatchItem &w, unsigned char *lds)
+{
+    if constexpr (CK == C_Q8) attend_codes<DT, DH, NQ, NW>(a, w, lds);
+    else attend_rows<DT, DH, NW>(a, w, lds);
 }
 
 /* group g's sequences [sa, sb) */
@@ -630,10 +654,8 @@ __device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem 
     wave_most = __builtin_amdgcn_readfirstlane(wave_most);
     least = __builtin_amdgcn_readfirstlane(least);
     most = __builtin_amdgcn_readfirstlane(most);
-    const int end_key = imin(most, w.t1);
-    const KeyBlocks blocks = key_blocks(least - a.window, end_key, a.sinks, KB);
-    int b0, b1;
-    split_range(blocks.total, w.splits, w.split, &b0, &b1);
+    const ItemBlocks in(a, w, least, most, KB);
+    const int b0 = in.b0, b1 = in.b1;
 
     /* where 16 keys lie: of block b those that this wave brings, and which of the block's four sixteens are in a page */
     struct Entries {
@@ -644,12 +666,12 @@ __device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem 
         return i < a.table_ld ? scalar_int(w.pages + i) : -1;
     };
     auto hint = [&](int b) __attribute__((always_inline)) {
-        const int k0 = blocks.at(b) * KB;
+        const int k0 = in.key(b, KB);
         return Entries{entry(k0 + 16 * wave), {entry(k0), entry(k0 + 16), entry(k0 + 32), entry(k0 + 48)}};
     };
     auto token_of = [&](int b, const Entries &n) __attribute__((always_inline)) {
-        const int key = blocks.at(b) * KB + 16 * wave, page = imax(page_in(n.mine, a.pages), 0);
-        return ((((size_t)page * a.kv + w.kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * RB;
+        const int key = in.key(b, KB) + 16 * wave, page = imax(page_in(n.mine, a.pages), 0);
+        return token_at(a, w, page, key) * RB;
     };
     auto there = [&](const Entries &n) __attribute__((always_inline)) {
         unsigned long long bits = 0;
@@ -694,22 +716,18 @@ __device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem 
         const u2 va = lds_tr(x), vb = lds_tr(x + 8 * RB);
         return u4{va[0], va[1], vb[0], vb[1]};
     };
-    /* whether rows of lengths from lo to hi see all of the block at k0 */
-    auto all_seen = [&](int k0, int lo, int hi) __attribute__((always_inline)) {
-        return k0 + KB <= imin(lo, w.t1) && (k0 >= hi - a.window || k0 + KB <= a.sinks);
-    };
     /* this wave's loads have come; of V of block b, where some row must not see a key, what no row sees and what is not finite
      * becomes zeros, which `odd` notes of the latter: a weight of 0 times them would be a NaN */
     auto come = [&](int b, unsigned long long held) __attribute__((always_inline)) {
         wait_vm<0>();
         if (b >= b0) {
-            const int k0 = blocks.at(b) * KB;
-            if (held != ~0ull || !all_seen(k0, least, most)) {
+            const int k0 = in.key(b, KB);
+            if (held != ~0ull || !item_sees_all(a, w, k0, KB, least, most)) {
                 u4 *v = reinterpret_cast<u4 *>(lds + (2 + ((b - b0) & 1)) * BUF + 16 * wave * RB) + lane;
 #pragma unroll
                 for (int x = 0; x < LD; x++) {
                     const int e = 16 * wave + RPL * x + lane / CH, key = k0 + e;
-                    const bool keep = ((held >> e) & 1) && key < end_key && (key >= least - a.window || key < a.sinks);
+                    const bool keep = ((held >> e) & 1) && key < in.end_key && (key >= least - a.window || key < a.sinks);
                     if (!keep) {
                         v[64 * x] = u4{0, 0, 0, 0};
                     } else if (odd_values<DT>(v[64 * x])) {
@@ -723,7 +741,7 @@ __device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem 
     };
     /* what a row must not see: key e of the block is bit e of 64; this lane has keys 8j + 4h .. + 3 of every eight */
     auto mask = [&](int k0, unsigned long long held) __attribute__((always_inline)) {
-        if (held == ~0ull && all_seen(k0, wave_least, wave_most)) return;
+        if (held == ~0ull && item_sees_all(a, w, k0, KB, wave_least, wave_most)) return;
         auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
         const unsigned long long bits = (below(imin(len, w.t1) - k0) & (~below(len - a.window - k0) | below(a.sinks - k0)) & held) >> (4 * h);
 #pragma unroll
@@ -772,7 +790,7 @@ __device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem 
         /* the first block has no weights before it: zeros, with zeros for V */
         for (int x = threadIdx.x; x < KB * CH; x += 256) reinterpret_cast<u4 *>(lds + 3 * BUF)[x] = u4{0, 0, 0, 0};
         for (int b = b0; b < b1; b++) {
-            const int k0 = blocks.at(b) * KB, odd_block = (b - b0) & 1;
+            const int k0 = in.key(b, KB), odd_block = (b - b0) & 1;
             /* past the last block that one's K again, which nothing reads */
             const unsigned char *next_k = kc + token_of(imin(b + 1, b1 - 1), next), *this_v = vc + token_of(b, now);
             const uint32_t ka = k_at + odd_block * BUF, va = v_at + (odd_block ^ 1) * BUF;
@@ -828,27 +846,17 @@ __device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem 
     const float sum = sum_halves(l);
     if (32 * wave + col >= w.rows) return;
     const size_t to = ((size_t)seq * a.heads + head) * w.parts + w.slot;
-    if (odd) {   /* rare, so simple: any positive weight of an infinity or a NaN is that */
-        for (int b = b0; b < b1; b++)
-            for (int key = blocks.at(b) * KB; key < blocks.at(b) * KB + KB; key++) {
-                const int page = page_in(page_entry(w.pages, a.table_ld, key, a.page_shift), a.pages);
-                if (page < 0 || key >= imin(len, w.t1) || !(key >= len - a.window || key < a.sinks)) continue;
-                const size_t token = (((size_t)page * a.kv + w.kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
-#pragma unroll
-                for (int d = 0; d < NT; d++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float x = Elem<DT>::get(static_cast<const E *>(a.vc)[token * DH + 32 * d + 8 * (i / 4) + 4 * h + i % 4]);
-                        if (!(__builtin_fabsf(x) < INFINITY)) o[d][i] += x;
-                    }
-            }
-    }
 #pragma unroll
     for (int d = 0; d < NT; d++)
 #pragma unroll
         for (int i = 0; i < 4; i++)
             *reinterpret_cast<f4 *>(a.part + to * DH + 32 * d + 8 * i + 4 * h) = f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
     if (h == 0) a.stat[to] = float2{m, sum};
+    if (odd)
+        for (int i = 0; i < DH / 2; i++) {   /* those that this lane has just stored */
+            const int d = 8 * (i / 4) + 4 * h + i % 4;
+            a.part[to * DH + d] += odd_values_of<DT, DH>(a, w, in, KB, len, d);
+        }
 }
 
 /* this workgroup's tile of TR rows of a group's prefix; false where there is none */
@@ -881,38 +889,49 @@ template <int DT, int DH> __global__ __launch_bounds__(256, 2) void attend_prefi
     if (prefix_item<kTileRows>(a, &w)) attend_tile<DT, DH>(a, w, lds);
 }
 
-template <int CK, int DT, int DH, int NQ, int NW>
-__global__ __launch_bounds__(64 * NW) void attend(BatchArgs a)
+/* this workgroup's part of what a sequence has alone, 16 of a key head's queries; false where it has none */
+__device__ __forceinline__ bool own_item(const BatchArgs &a, BatchItem *w)
 {
-    __shared__ __align__(16) unsigned char lds[attend_lds<CK, DT, DH, NQ, NW>()];
     const int G = a.heads / a.kv;
-    BatchItem w;
-    if ((int)blockIdx.x < a.p_wgs) {
-        if (prefix_item<16 * NQ>(a, &w)) attend_item<CK, DT, DH, NQ, NW>(a, w, lds);
-        return;
-    }
     int id = blockIdx.x - a.p_wgs;
-    w.kvh = id % a.kv;
+    w->kvh = id % a.kv;
     id /= a.kv;
-    w.split = id % a.o_parts;
+    w->split = id % a.o_parts;
     id /= a.o_parts;
-    w.r0 = 16 * (id % a.q_groups);
-    w.seq0 = id / a.q_groups;
-    w.rows = imin(16, G - w.r0);
-    w.t0 = 0;
-    w.t1 = 1 << 30;
-    w.pages = a.table + (size_t)w.seq0 * a.table_ld;
-    w.splits = a.o_parts;
-    w.slot = a.p_parts + w.split;
-    w.parts = a.p_parts + a.o_parts;
-    if (a.group) {
-        const int gr = wave_last(a.n_groups, [&](int s) { return group_start(a, s) <= w.seq0; });
-        if (gr < 0 || w.seq0 >= group_start(a, gr + 1)) {   /* in no group: attend_join leaves its rows as they are */
-            if (w.split == 0 && threadIdx.x < w.rows)
-                a.stat[((size_t)w.seq0 * a.heads + w.kvh * G + w.r0 + threadIdx.x) * w.parts + w.slot] = float2{0.0f, -1.0f};
+    w->r0 = 16 * (id % a.q_groups);
+    w->seq0 = id / a.q_groups;
+    w->rows = imin(16, G - w->r0);
+    w->t0 = 0;
+    w->t1 = 1 << 30;
+    w->pages = a.table + (size_t)w->seq0 * a.table_ld;
+    w->splits = a.o_parts;
+    w->slot = a.p_parts + w->split;
+    w->parts = a.p_parts + a.o_parts;
+    if (!a.group) return true;
+    const int gr = wave_last(a.n_groups, [&](int s) { return group_start(a, s) <= w->seq0; });
+    if (gr < 0 || w->seq0 >= group_start(a, gr + 1)) {   /* in no group: attend_join leaves its rows as they are */
+        if (w->split == 0 && (int)threadIdx.x < w->rows)
+            a.stat[((size_t)w->seq0 * a.heads + w->kvh * G + w->r0 + threadIdx.x) * w->parts + w->slot] = float2{0.0f, -1.0f};
+        return false;
+    }
+    w->t0 = imax(a.shared[gr], 0);
+    return true;
+}
+
+/* Prefixes by 16 · NQ rows of a group, then what each sequence has alone. */
+template <int CK, int DT, int DH, int NQ, int NW>
+__global__ __launch_bounds__(64 * NW, CK == C_ROWS ? (DH == 64 ? 4 : 3) : 2) void attend(BatchArgs a)
+{
+    constexpr int L = attend_lds<CK, DT, DH, NQ, NW>(), L1 = attend_lds<CK, DT, DH, 1, NW>();
+    __shared__ __align__(16) unsigned char lds[L > L1 ? L : L1];
+    BatchItem w;
+    const bool prefix = (int)blockIdx.x < a.p_wgs;
+    if (!(prefix ? prefix_item<16 * NQ>(a, &w) : own_item(a, &w))) return;
+    if constexpr (NQ > 1) {
+        if (prefix) {
+            attend_item<CK, DT, DH, NQ, NW>(a, w, lds);
             return;
         }
-        w.t0 = imax(a.shared[gr], 0);
     }
     attend_item<CK, DT, DH, 1, NW>(a, w, lds);
 }
