@@ -805,7 +805,6 @@ __device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem 
 #pragma unroll
             for (int i = 0; i < 16; i++) s[0][i] = s[1][i] = 0.0f;
             come(b - 1, held_before);
-            const Entries after = hint(imin(b + 2, b1 - 1));
             __builtin_amdgcn_s_setprio(1);   /* products first: the other wave's exponentials fill what they leave */
             read(0);
             read(1);
@@ -824,6 +823,7 @@ __device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem 
                 __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_s_setprio(0);
+            const Entries after = hint(imin(b + 2, b1 - 1));   /* not among the LDS reads, which it would be waited for with */
             mask(k0, held);
             const float mu = m == -INFINITY ? 0.0f : m;
             float sum = 0.0f;
@@ -860,10 +860,10 @@ __device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem 
 }
 
 /* this workgroup's tile of TR rows of a group's prefix; false where there is none */
-template <int TR> __device__ __forceinline__ bool prefix_item(const BatchArgs &a, BatchItem *w)
+template <int TR> __device__ __forceinline__ bool prefix_item(const BatchArgs &a, int at, BatchItem *w)
 {
-    const int G = a.heads / a.kv, id = blockIdx.x / a.kv, tile = id % a.p_tiles;
-    w->kvh = blockIdx.x % a.kv;
+    const int G = a.heads / a.kv, id = at / a.kv, tile = id % a.p_tiles;
+    w->kvh = at % a.kv;
     w->split = id / a.p_tiles;
     /* tiles are numbered as tile_start does, rows being G for each sequence */
     const int gr = wave_last(a.n_groups, [&](int s) { return group_start(a, s) * G / TR + s <= tile; });
@@ -882,18 +882,10 @@ template <int TR> __device__ __forceinline__ bool prefix_item(const BatchArgs &a
     return true;
 }
 
-template <int DT, int DH> __global__ __launch_bounds__(256, 2) void attend_prefix(BatchArgs a)
-{
-    __shared__ __align__(16) unsigned char lds[tile_lds<DT, DH>()];
-    BatchItem w;
-    if (prefix_item<kTileRows>(a, &w)) attend_tile<DT, DH>(a, w, lds);
-}
-
 /* this workgroup's part of what a sequence has alone, 16 of a key head's queries; false where it has none */
-__device__ __forceinline__ bool own_item(const BatchArgs &a, BatchItem *w)
+__device__ __forceinline__ bool own_item(const BatchArgs &a, int id, BatchItem *w)
 {
     const int G = a.heads / a.kv;
-    int id = blockIdx.x - a.p_wgs;
     w->kvh = id % a.kv;
     id /= a.kv;
     w->split = id % a.o_parts;
@@ -926,7 +918,7 @@ __global__ __launch_bounds__(64 * NW, CK == C_ROWS ? (DH == 64 ? 4 : 3) : 2) voi
     __shared__ __align__(16) unsigned char lds[L > L1 ? L : L1];
     BatchItem w;
     const bool prefix = (int)blockIdx.x < a.p_wgs;
-    if (!(prefix ? prefix_item<16 * NQ>(a, &w) : own_item(a, &w))) return;
+    if (!(prefix ? prefix_item<16 * NQ>(a, blockIdx.x, &w) : own_item(a, blockIdx.x - a.p_wgs, &w))) return;
     if constexpr (NQ > 1) {
         if (prefix) {
             attend_item<CK, DT, DH, NQ, NW>(a, w, lds);
@@ -934,6 +926,25 @@ __global__ __launch_bounds__(64 * NW, CK == C_ROWS ? (DH == 64 ? 4 : 3) : 2) voi
         }
     }
     attend_item<CK, DT, DH, 1, NW>(a, w, lds);
+}
+
+/* Prefixes by tiles of 128 rows, and what each sequence has alone, a workgroup of either in turn while both last: the one waits
+ * for the matrix unit, the other for memory. */
+template <int DT, int DH>
+__global__ __launch_bounds__(256, 2) void attend_tiles(BatchArgs a)
+{
+    __shared__ __align__(16) unsigned char lds[tile_lds<DT, DH>()];
+    static_assert(tile_lds<DT, DH>() >= few_lds_bytes<DT, DH, 4>(), "what both need");
+    /* eight of the one and eight of the other in turn, one for each XCD; then the rest of the one, the rest of the other */
+    const int each = imin(a.p_wgs, (int)gridDim.x - a.p_wgs) / 8 * 8, id = blockIdx.x, rest = id - 2 * each;
+    const bool prefix = rest < 0 ? id / 8 % 2 == 0 : rest < a.p_wgs - each;
+    const int at = rest < 0 ? id / 16 * 8 + id % 8 : prefix ? each + rest : rest - (a.p_wgs - 2 * each);
+    BatchItem w;
+    if (prefix) {
+        if (prefix_item<kTileRows>(a, at, &w)) attend_tile<DT, DH>(a, w, lds);
+    } else {
+        if (own_item(a, at, &w)) attend_rows<DT, DH, 4>(a, w, lds);
+    }
 }
 
 /* The parts of one query added up by one wave, DH / 64 outputs a lane. */

@@ -111,14 +111,14 @@ int attention(const char *name, int dtype, const CacheView &c, bool q8, const Pl
         overlap(o, ints(dGroup, 1, n_groups + 1)) || overlap(o, ints(dShared, 1, n_groups)))
         return fail(P2H_E_ARG, "%s: dO overlaps lengths, pages or groups", name);
     const size_t p_wgs = (size_t)plan.p_tiles * plan.p_parts * c.heads;
-    const size_t o_wgs = (size_t)n_seqs * plan.q_groups * plan.o_parts * c.heads, wgs = (plan.tiled ? 0 : p_wgs) + o_wgs;
-    if ((p_wgs + o_wgs) * 64 * kWaves >= kGridThreads || (size_t)n_seqs * heads >= 1u << 23)
+    const size_t o_wgs = (size_t)n_seqs * plan.q_groups * plan.o_parts * c.heads, wgs = p_wgs + o_wgs;
+    if (wgs * 64 * kWaves >= kGridThreads || (size_t)n_seqs * heads >= 1u << 23)
         return fail(P2H_E_ARG, "%s: %d sequences of %d heads are too many for one call", name, n_seqs, heads);
     if (int rc = ensure_init()) return rc;
     p2k::BatchArgs a{};
     a.n_seqs = n_seqs; a.n_groups = n_groups; a.heads = heads; a.kv = c.heads; a.page_shift = log2_of(c.page);
     a.pages = c.pages; a.table_ld = table_ld; a.ldq = ldq; a.ldo = ldo; a.window = window; a.sinks = sinks;
-    a.p_tiles = plan.p_tiles; a.p_parts = plan.p_parts; a.p_wgs = plan.tiled ? 0 : (int)p_wgs;
+    a.p_tiles = plan.p_tiles; a.p_parts = plan.p_parts; a.p_wgs = (int)p_wgs;
     a.q_groups = plan.q_groups; a.o_parts = plan.o_parts; a.c = scale * p2k::kLog2e;
     a.q = dQ; a.kc = c.K; a.vc = c.V; a.ks = c.ks; a.vs = c.vs;
     a.table = dTable; a.len = dLen; a.group = dGroup; a.shared = dShared; a.o = dO;
@@ -127,12 +127,14 @@ int attention(const char *name, int dtype, const CacheView &c, bool q8, const Pl
     hipStream_t s = stream_of(stream);
     by_type_dim(dtype, c.head_dim, [&](auto t, auto d) {
         constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
-        if constexpr (DT != p2k::T_F32) {
-            if (plan.tiled)
-                hipLaunchKernelGGL((p2k::attend_prefix<DT, DH>), dim3((unsigned)p_wgs), dim3(256), 0, s, a);
+        const dim3 grid((unsigned)wgs), threads(64 * kWaves);
+        if (q8) {
+            hipLaunchKernelGGL((p2k::attend<p2k::C_Q8, DT, DH, 1, kWaves>), grid, threads, 0, s, a);
+        } else if (!plan.tiled) {
+            hipLaunchKernelGGL((p2k::attend<p2k::C_ROWS, DT, DH, 1, kWaves>), grid, threads, 0, s, a);
+        } else {
+            if constexpr (DT != p2k::T_F32) hipLaunchKernelGGL((p2k::attend_tiles<DT, DH>), grid, threads, 0, s, a);
         }
-        if (q8) hipLaunchKernelGGL((p2k::attend<p2k::C_Q8, DT, DH, 1, kWaves>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, s, a);
-        else hipLaunchKernelGGL((p2k::attend<p2k::C_ROWS, DT, DH, 1, kWaves>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, s, a);
         if (parted)
             hipLaunchKernelGGL((p2k::attend_join<DT, DH>), dim3((unsigned)(((size_t)n_seqs * heads + 3) / 4)), dim3(256), 0, s, a);
     });
