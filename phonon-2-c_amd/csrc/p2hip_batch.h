@@ -862,9 +862,11 @@ __device__ __forceinline__ void attend_tile(const BatchArgs &a, const BatchItem 
 /* this workgroup's tile of TR rows of a group's prefix; false where there is none */
 template <int TR> __device__ __forceinline__ bool prefix_item(const BatchArgs &a, int at, BatchItem *w)
 {
-    const int G = a.heads / a.kv, id = at / a.kv, tile = id % a.p_tiles;
+    /* All parts of a tile next to each other: numbers without a tile would otherwise fall on the same shader engines, to which
+     * workgroups go in turn, and leave the work to the others (a tile, none, a tile, …: 86 us in place of 55). */
+    const int G = a.heads / a.kv, id = at / a.kv, tile = id / a.p_parts;
     w->kvh = at % a.kv;
-    w->split = id / a.p_tiles;
+    w->split = id % a.p_parts;
     /* tiles are numbered as tile_start does, rows being G for each sequence */
     const int gr = wave_last(a.n_groups, [&](int s) { return group_start(a, s) * G / TR + s <= tile; });
     if (gr < 0) return false;
@@ -928,22 +930,17 @@ __global__ __launch_bounds__(64 * NW, CK == C_ROWS ? (DH == 64 ? 4 : 3) : 2) voi
     attend_item<CK, DT, DH, 1, NW>(a, w, lds);
 }
 
-/* Prefixes by tiles of 128 rows, and what each sequence has alone, a workgroup of either in turn while both last: the one waits
- * for the matrix unit, the other for memory. */
+/* Prefixes by tiles of 128 rows, then what each sequence has alone. */
 template <int DT, int DH>
 __global__ __launch_bounds__(256, 2) void attend_tiles(BatchArgs a)
 {
     __shared__ __align__(16) unsigned char lds[tile_lds<DT, DH>()];
     static_assert(tile_lds<DT, DH>() >= few_lds_bytes<DT, DH, 4>(), "what both need");
-    /* eight of the one and eight of the other in turn, one for each XCD; then the rest of the one, the rest of the other */
-    const int each = imin(a.p_wgs, (int)gridDim.x - a.p_wgs) / 8 * 8, id = blockIdx.x, rest = id - 2 * each;
-    const bool prefix = rest < 0 ? id / 8 % 2 == 0 : rest < a.p_wgs - each;
-    const int at = rest < 0 ? id / 16 * 8 + id % 8 : prefix ? each + rest : rest - (a.p_wgs - 2 * each);
     BatchItem w;
-    if (prefix) {
-        if (prefix_item<kTileRows>(a, at, &w)) attend_tile<DT, DH>(a, w, lds);
+    if ((int)blockIdx.x < a.p_wgs) {
+        if (prefix_item<kTileRows>(a, blockIdx.x, &w)) attend_tile<DT, DH>(a, w, lds);
     } else {
-        if (own_item(a, at, &w)) attend_rows<DT, DH, 4>(a, w, lds);
+        if (own_item(a, blockIdx.x - a.p_wgs, &w)) attend_rows<DT, DH, 4>(a, w, lds);
     }
 }
 

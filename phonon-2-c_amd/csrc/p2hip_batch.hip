@@ -18,6 +18,7 @@ constexpr int kWaves = 4;   /* of a workgroup of attend */
 struct Plan {
     int p_tiles = 0, p_parts = 0, q_groups = 1, o_parts = 1;
     bool tiled = false;   /* prefixes by tiles of p2k::kTileRows rows */
+    int nq = 1;           /* else by 16 · nq */
     int parts() const { return p_parts + o_parts; }
     size_t bytes(int n_seqs, int heads, int head_dim) const
     {
@@ -57,7 +58,8 @@ Plan shared_plan(const CacheView &c, bool q8, int dtype, int n_seqs, int n_group
     p.q_groups = (G + 15) / 16;
     const int rows = n_groups ? (n_seqs * G + n_groups - 1) / n_groups : 0;   /* of a group, as the host knows them */
     p.tiled = !q8 && dtype != P2H_F32 && rows > 32;
-    const int tr = p.tiled ? p2k::kTileRows : 16;
+    p.nq = q8 && rows > 16 ? 2 : 1;
+    const int tr = p.tiled ? p2k::kTileRows : 16 * p.nq;
     p.p_tiles = n_seqs * G / tr + n_groups;
     p.p_parts = parts_of((long long)n_groups * ((rows + tr - 1) / tr) * c.heads, left_of(max_shared, window, sinks), kb);
     p.o_parts = parts_of((long long)n_seqs * c.heads * p.q_groups, left_of(max_own, window, sinks), kb);
@@ -129,7 +131,8 @@ int attention(const char *name, int dtype, const CacheView &c, bool q8, const Pl
         constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
         const dim3 grid((unsigned)wgs), threads(64 * kWaves);
         if (q8) {
-            hipLaunchKernelGGL((p2k::attend<p2k::C_Q8, DT, DH, 1, kWaves>), grid, threads, 0, s, a);
+            if (plan.nq == 2) hipLaunchKernelGGL((p2k::attend<p2k::C_Q8, DT, DH, 2, kWaves>), grid, threads, 0, s, a);
+            else hipLaunchKernelGGL((p2k::attend<p2k::C_Q8, DT, DH, 1, kWaves>), grid, threads, 0, s, a);
         } else if (!plan.tiled) {
             hipLaunchKernelGGL((p2k::attend<p2k::C_ROWS, DT, DH, 1, kWaves>), grid, threads, 0, s, a);
         } else {
