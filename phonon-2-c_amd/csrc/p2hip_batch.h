@@ -236,7 +236,7 @@ struct ItemBlocks {
 /* whether a row of that length sees a key, if a page holds it */
 __device__ __forceinline__ bool item_sees(const BatchArgs &a, const BatchItem &w, int key, int len)
 {
-    return key >= w.t0 && key < imin(len, w.t1) && (key >= len - a.window || key < a.sinks);
+    return (key >= w.t0) & (key < imin(len, w.t1)) & ((key >= len - a.window) | (key < a.sinks));
 }
 /* whether rows of lengths least .. most see all n keys from k0 on */
 __device__ __forceinline__ bool item_sees_all(const BatchArgs &a, const BatchItem &w, int k0, int n, int least, int most)
@@ -355,6 +355,8 @@ __device__ __forceinline__ void attend_rows(const BatchArgs &a, const BatchItem 
         put_part<DT, DH>(a, w, r, d, top, num, den);
     }
 }
+
+constexpr float kCodeSlack = 1024.0f;   /* the largest sum of a lane's eight weights */
 
 template <int DH, int NQ, int NW> constexpr int codes_lds()
 {
@@ -503,31 +505,41 @@ __device__ __forceinline__ void attend_codes(const BatchArgs &a, const BatchItem
             }
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
-                bool seen[8];
+                f4 v[2] = {vs[0], vs[1]};
                 if (!now.whole) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        seen[i] = now.there[i / 4] && item_sees(a, w, now.k0 + B::key_of(i / 4, 4 * g + i % 4), len.of[n]);
-                        if (!seen[i]) s[n][i / 4][i % 4] = -INFINITY;
+                    for (int i = 0; i < 8; i++) {   /* whatever the scales of what is not seen */
+                        const bool seen = now.there[i / 4] & item_sees(a, w, now.k0 + B::key_of(i / 4, 4 * g + i % 4), len.of[n]);
+                        s[n][i / 4][i % 4] = seen ? s[n][i / 4][i % 4] : -INFINITY;
+                        v[i / 4][i % 4] = seen ? v[i / 4][i % 4] : 0.0f;
                     }
                 }
-                float top = s[n][0][0];
+                float x[8];
+                auto weights = [&]() __attribute__((always_inline)) {   /* from the reference on; their sum */
+                    const float mu = m[n] == -INFINITY ? 0.0f : m[n];
 #pragma unroll
-                for (int i = 1; i < 8; i++) top = fmaxf(top, s[n][i / 4][i % 4]);
-                const float mn = fmaxf(m[n], max_quarters(top) * a.c);
-                const float mu = mn == -INFINITY ? 0.0f : mn, fade = exp2_fast(m[n] - mu);
-                m[n] = mn;
-                float wv[8], sum = 0.0f;
+                    for (int i = 0; i < 8; i++) x[i] = exp2_fast(__builtin_fmaf(s[n][i / 4][i % 4], a.c, -mu));
+                    return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+                };
+                float sum = weights();
+                /* the reference is raised, to the largest score so far, only where weights have become large or there is none
+                 * yet: most blocks need no maximum and leave O as it is */
+                if (__any(!(sum <= kCodeSlack) || m[n] == -INFINITY)) {
+                    float top = s[n][0][0];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float x = exp2_fast(__builtin_fmaf(s[n][i / 4][i % 4], a.c, -mu));
-                    sum += x;
-                    wv[i] = x * vs[i / 4][i % 4];
-                    if (!now.whole && !seen[i]) wv[i] = 0.0f;   /* whatever the scale of what is not seen */
+                    for (int i = 1; i < 8; i++) top = fmaxf(top, s[n][i / 4][i % 4]);
+                    const float mn = fmaxf(m[n], max_quarters(top) * a.c);
+                    const float fade = exp2_fast(m[n] - (mn == -INFINITY ? 0.0f : mn));
+                    m[n] = mn;
+                    l[n] *= fade;
+#pragma unroll
+                    for (int d = 0; d < NT; d++) o[n][d] *= fade;
+                    sum = weights();
                 }
-                l[n] = __builtin_fmaf(l[n], fade, sum);
+                l[n] += sum;
+                float wv[8];
 #pragma unroll
-                for (int d = 0; d < NT; d++) o[n][d] *= fade;
+                for (int i = 0; i < 8; i++) wv[i] = x[i] * v[i / 4][i % 4];
                 bf16_pieces<WP>(wv, pw[n]);
             }
             wait_vm<MORE ? B::LOADS : 0>();
