@@ -131,7 +131,8 @@ struct BatchArgs {
  * of 16 keys, v_place for 64 bytes of 4 keys. */
 template <int DH> struct CodeBlock {
     static constexpr int KB = 32, CH = DH / 16, RPL = 64 / CH, LD = KB / RPL, BYTES = KB * DH, STAGE = 2 * BYTES + 256,
-                         LOADS = 2 * LD + 1;
+                         LOADS = 2 * LD + 1,
+                         STAGES = 2;   /* in a wave's LDS; three bring nothing (heads of 128: one workgroup a CU, 77 -> 105 us) */
     static __device__ __forceinline__ constexpr int k_place(int r, int p) { return p ^ ((r / (16 / CH)) & (CH - 1)); }
     static __device__ __forceinline__ constexpr int v_place(int r, int p) { return CH == 8 ? p ^ (4 * ((r >> 1) & 1)) : p; }
     /* the key of a block that product t has in row m: a lane's results are rows 4g + i, its four groups of lanes having
@@ -360,7 +361,7 @@ constexpr float kCodeSlack = 1024.0f;   /* the largest sum of a lane's eight wei
 
 template <int DH, int NQ, int NW> constexpr int codes_lds()
 {
-    constexpr int V = NW * 2 * CodeBlock<DH>::STAGE, J = NW * 16 * NQ * (DH + 2) * 4;
+    constexpr int V = NW * CodeBlock<DH>::STAGES * CodeBlock<DH>::STAGE, J = NW * 16 * NQ * (DH + 2) * 4;
     return V > J ? V : J;
 }
 
@@ -420,7 +421,8 @@ __device__ __forceinline__ void attend_codes(const BatchArgs &a, const BatchItem
         return n;
     };
 
-    unsigned char *const own = lds + wave * 2 * B::STAGE;
+    constexpr int NS = B::STAGES;
+    unsigned char *const own = lds + wave * NS * B::STAGE;
     uint32_t koff[LD], voff[LD];   /* of this lane's 16 bytes from the first row of 16 */
 #pragma unroll
     for (int x = 0; x < LD; x++) {
@@ -460,20 +462,26 @@ __device__ __forceinline__ void attend_codes(const BatchArgs &a, const BatchItem
         for (int d = 0; d < NT; d++) o[n][d] = f4{0, 0, 0, 0};
     }
 
-    int b = in.b0 + wave;
-    if (b < in.b1) {
-        Place now = fetch(b, hint(b), own), next = now;
-        Entries ahead = hint(imin(b + NW, in.b1 - 1));
+    const int first = in.b0 + wave;
+    if (first < in.b1) {
+        /* Blocks on their way: NS − 1 while one is multiplied. Those past the wave's last are that one again, so that there are
+         * always as many loads to wait for. */
+        const int final = first + (in.b1 - 1 - first) / NW * NW;
+        Place place[NS];
+#pragma unroll
+        for (int n = 0; n < NS - 1; n++) {
+            const int b = imin(first + n * NW, final);
+            place[n] = fetch(b, hint(b), own + n * B::STAGE);
+        }
+        Entries ahead = hint(imin(first + (NS - 1) * NW, final));
         int stage = 0;
-        auto block = [&](auto last) __attribute__((always_inline)) {
-            constexpr bool MORE = !decltype(last)::value;
+        for (int b = first; b < in.b1; b += NW) {
             const unsigned char *Ks = own + stage * B::STAGE, *Vs = Ks + B::BYTES;
-            if constexpr (MORE) {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   /* what reads of the other stage brought */
-                next = fetch(b + NW, ahead, own + (stage ^ 1) * B::STAGE);
-                ahead = hint(imin(b + 2 * NW, in.b1 - 1));
-            }
-            wait_vm<(MORE ? B::LOADS : 0) + LD>();   /* all but V's, and the next block's */
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   /* what reads of the stage before brought */
+            place[NS - 1] = fetch(imin(b + (NS - 1) * NW, final), ahead, own + (stage == 0 ? NS - 1 : stage - 1) * B::STAGE);
+            ahead = hint(imin(b + NS * NW, final));
+            const Place now = place[0];
+            wait_vm<(NS - 1) * B::LOADS + LD>();   /* all but V's, and the blocks behind */
             f4 s[NQ][2];
 #pragma unroll
             for (int n = 0; n < NQ; n++) s[n][0] = s[n][1] = f4{0, 0, 0, 0};
@@ -542,7 +550,7 @@ __device__ __forceinline__ void attend_codes(const BatchArgs &a, const BatchItem
                 for (int i = 0; i < 8; i++) wv[i] = x[i] * v[i / 4][i % 4];
                 bf16_pieces<WP>(wv, pw[n]);
             }
-            wait_vm<MORE ? B::LOADS : 0>();
+            wait_vm<(NS - 1) * B::LOADS>();
 #pragma unroll
             for (int h = 0; h < DH / 64; h++) {
                 uint32_t dw[8];   /* four neighbouring dimensions of each of the lane's keys, one for each of four products */
@@ -566,11 +574,11 @@ __device__ __forceinline__ void attend_codes(const BatchArgs &a, const BatchItem
                 product(std::integral_constant<int, 2>{});
                 product(std::integral_constant<int, 3>{});
             }
-            now = next;
-            stage ^= 1;
-        };
-        for (; b + NW < in.b1; b += NW) block(std::false_type{});
-        block(std::true_type{});
+#pragma unroll
+            for (int n = 0; n < NS - 1; n++) place[n] = place[n + 1];
+            stage = stage == NS - 1 ? 0 : stage + 1;
+        }
+        wait_vm<0>();   /* nothing comes into the LDS any more */
     }
 
     __syncthreads();   /* the waves' own parts are done with */
@@ -926,7 +934,7 @@ __device__ __forceinline__ bool own_item(const BatchArgs &a, int id, BatchItem *
 
 /* Prefixes by 16 · NQ rows of a group, then what each sequence has alone. */
 template <int CK, int DT, int DH, int NQ, int NW>
-__global__ __launch_bounds__(64 * NW, CK == C_ROWS ? (DH == 64 ? 4 : 3) : 2) void attend(BatchArgs a)
+__global__ __launch_bounds__(64 * NW, CK == C_ROWS ? (DH == 64 ? 4 : DT == T_F32 ? 3 : 2) : 2) void attend(BatchArgs a)
 {
     constexpr int L = attend_lds<CK, DT, DH, NQ, NW>(), L1 = attend_lds<CK, DT, DH, 1, NW>();
     __shared__ __align__(16) unsigned char lds[L > L1 ? L : L1];
@@ -991,7 +999,7 @@ __global__ __launch_bounds__(256) void attend_join(BatchArgs a)
 /* ── adapters ──────────────────────────────────────────────────────────────────────────────────────────────── */
 
 struct AdapterArgs {
-    int M, N, K, count, ldx, ldz, ldy, parts, chunk, vec;   /* parts of `chunk` dimensions of K; vec: rows of Z and Y by 16 bytes */
+    int M, N, K, count, ldx, ldz, ldy, parts, chunk, vec, units;   /* parts of `chunk` dimensions of K; vec: rows of Z and Y by 16 bytes; 64 columns a unit */
     const void *x, *z, *a, *b;
     const float *scale;
     const int *index;
@@ -1123,6 +1131,80 @@ __global__ __launch_bounds__(64 * NW) void adapter_shrink(AdapterArgs a)
     }
 }
 
+/* The same for many rows, 64 a workgroup, 16 a wave, whose X and A come through LDS 256 bytes of a row at a time, read along the
+ * rows: read as operands, neighbouring lanes would be in different rows. Two stages in turn. Rows of X and A are 16-byte
+ * aligned. */
+template <int RANK> constexpr int shrink_stage() { return (64 + RANK) * 256; }
+
+template <int DT, int RANK>
+__global__ __launch_bounds__(256) void adapter_shrink_rows(AdapterArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    constexpr int VE = kPer16<DT>, KC = 16 * VE, RT = (RANK + 15) / 16, ALD = RANK < 16 ? 1 : RANK / 16;   /* loads of A a wave */
+    __shared__ __align__(16) unsigned char lds[2 * shrink_stage<RANK>()];
+    __shared__ AdapterList list;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int m0 = 64 * blockIdx.x, rows = imin(64, a.M - m0), k0 = blockIdx.y * a.chunk, k1 = imin(k0 + a.chunk, a.K);
+    list_adapters(a, m0, rows, &list);
+    const int stages = k1 > k0 ? (k1 - k0 + KC - 1) / KC : 0, n = __builtin_amdgcn_readfirstlane(list.n);
+    const E *const x = static_cast<const E *>(a.x);
+    /* row r has its piece p at place p ^ (r mod 16); a load brings 4 rows */
+    auto place = [](int r, int p) { return p ^ (r & 15); };
+    auto fetch = [&](int ad, int st, unsigned char *to) __attribute__((always_inline)) {
+        const int k = k0 + KC * st;
+        auto piece = [&](int r) { return imin(k + VE * place(r, lane & 15), k1 - VE); };   /* past the end: the last one again */
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = 16 * wave + 4 * i + (lane >> 4);
+            dma_16(x + (size_t)(m0 + imin(r, rows - 1)) * a.ldx + piece(r), to + 1024 * (4 * wave + i));
+        }
+#pragma unroll
+        for (int i = 0; i < ALD; i++) {
+            const int load = RANK < 16 ? wave % (RANK / 4) : ALD * wave + i, r = 4 * load + (lane >> 4);
+            dma_16(static_cast<const E *>(a.a) + ((size_t)ad * RANK + r) * a.K + piece(r), to + 64 * 256 + 1024 * load);
+        }
+    };
+    for (int j = 0; j < n; j++) {
+        const int ad = __builtin_amdgcn_readfirstlane(list.of[j]);
+        if (ad < 0) continue;
+        const uint32_t those = (uint32_t)__builtin_amdgcn_readfirstlane((int)(list.rows[j] >> (16 * wave))) & 0xffffu;
+        f4 acc[RT];
+#pragma unroll
+        for (int t = 0; t < RT; t++) acc[t] = f4{0, 0, 0, 0};
+        if (stages > 0) fetch(ad, 0, lds);
+        for (int st = 0; st < stages; st++) {
+            unsigned char *const now = lds + (st & 1) * shrink_stage<RANK>();
+            /* the last stage's loads again, which nothing reads, so that there are always as many to wait for */
+            fetch(ad, imin(st + 1, stages - 1), lds + ((st & 1) ^ 1) * shrink_stage<RANK>());
+            wait_vm<4 + ALD>();
+            lds_barrier();
+            if (those) {
+                const int have = (k1 - k0 - KC * st) / VE;   /* pieces of this stage */
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const int p = 4 * s + g;
+                    auto read = [&](const unsigned char *base, int r) __attribute__((always_inline)) {
+                        u4 v = *reinterpret_cast<const u4 *>(base + 256 * r + 16 * place(r, p));
+                        return p < have ? v : u4{0, 0, 0, 0};
+                    };
+                    const u4 xv = read(now, 16 * wave + c);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) acc[t] = mfma_piece<DT>(xv, read(now + 64 * 256, imin(16 * t + c, RANK - 1)), acc[t]);
+                }
+            }
+            lds_barrier();   /* everyone is done with what the next loads overwrite */
+        }
+        wait_vm<0>();
+        lds_barrier();
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (((those >> (4 * g + i)) & 1) && 16 * t + c < RANK)
+                    a.h[((size_t)blockIdx.y * a.M + m0 + 16 * wave + 4 * g + i) * RANK + 16 * t + c] = acc[t][i];
+    }
+}
+
 /* Row 4g + i of product t is this column of 64, so that a lane's results are 16 bytes of neighbours (16-bit rows: of two
  * products) and four lanes' 64. */
 template <int DT> __device__ __forceinline__ constexpr int expand_column(int t, int r)
@@ -1130,26 +1212,34 @@ template <int DT> __device__ __forceinline__ constexpr int expand_column(int t, 
     return DT == T_F32 ? 16 * t + r : 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3);
 }
 
-/* 64 columns from n0 on of those of 16 rows from m0 on: Y = Z + Σ h · B, h this lane's RANK / 4 of row m0 + lane % 16 (times the
- * adapter's scale), b its elements of B's rows, in fp32 products (B's values are exact in fp32), rounded once. */
+/* What 64 columns from n0 on of those of 16 rows from m0 on need from memory, where whole rows are read 16 bytes at a time */
+template <int DT> struct ExpandRows {
+    static constexpr int VE = kPer16<DT>, NV = 16 / VE;
+    u4 z[NV];
+    __device__ __forceinline__ void load(const AdapterArgs &a, bool in, int m, int n0, int g)
+    {
+        typedef typename Elem<DT>::type E;
+#pragma unroll
+        for (int p = 0; p < NV; p++) {
+            z[p] = u4{0, 0, 0, 0};
+            if (a.z && in) z[p] = *reinterpret_cast<const u4 *>(static_cast<const E *>(a.z) + (size_t)m * a.ldz + n0 + 4 * VE * p + VE * g);
+        }
+    }
+};
+
+/* … and Y = Z + Σ h · B of them, h this lane's RANK / 4 of row m0 + lane % 16 (times the adapter's scale), b its elements of B's
+ * rows, in fp32 products (B's values are exact in fp32), rounded once. Rows that are not read 16 bytes at a time go through
+ * the wave's LDS, so that lanes have neighbouring columns of one row. */
 template <int DT, int RANK>
-__device__ __forceinline__ void expand_rows(const AdapterArgs &a, uint32_t those, int m0, int n0, const float (&h)[RANK / 4],
+__device__ __forceinline__ void expand_rows(const AdapterArgs &a, uint32_t those, int m0, int n0, bool whole,
+                                            const ExpandRows<DT> &rows, const float (&h)[RANK / 4],
                                             const typename Elem<DT>::type (&b)[4][RANK / 4], float (*tile)[65])
 {
     typedef typename Elem<DT>::type E;
-    constexpr int RS = RANK / 4, VE = kPer16<DT>, NV = 16 / VE;   /* 16-byte pieces of a lane */
+    constexpr int RS = RANK / 4, VE = kPer16<DT>, NV = 16 / VE;
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const bool whole = a.vec && n0 + 64 <= a.N, in = (those >> c) & 1;
     const E *z = static_cast<const E *>(a.z);
     E *y = static_cast<E *>(a.y);
-    u4 zv[NV];
-    if (whole) {
-#pragma unroll
-        for (int p = 0; p < NV; p++) {
-            zv[p] = u4{0, 0, 0, 0};
-            if (z && in) zv[p] = *reinterpret_cast<const u4 *>(z + (size_t)(m0 + c) * a.ldz + n0 + 4 * VE * p + VE * g);
-        }
-    }
     f4 acc[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) acc[t] = f4{0, 0, 0, 0};
@@ -1162,13 +1252,12 @@ __device__ __forceinline__ void expand_rows(const AdapterArgs &a, uint32_t those
 #pragma unroll
         for (int p = 0; p < NV; p++) {
             float v[VE];
-            unpack<DT>(zv[p], v);
+            unpack<DT>(rows.z[p], v);
 #pragma unroll
             for (int j = 0; j < VE; j++) v[j] += acc[VE / 4 * p + j / 4][j % 4];
-            if (in) *reinterpret_cast<u4 *>(y + (size_t)(m0 + c) * a.ldy + n0 + 4 * VE * p + VE * g) = pack<DT>(v);
+            if ((those >> c) & 1) *reinterpret_cast<u4 *>(y + (size_t)(m0 + c) * a.ldy + n0 + 4 * VE * p + VE * g) = pack<DT>(v);
         }
     } else {
-        /* through the wave's LDS, so that lanes have neighbouring columns of one row */
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -1221,23 +1310,192 @@ __global__ __launch_bounds__(64 * NW) void adapter_expand(AdapterArgs a)
             __builtin_memcpy(b[t], static_cast<const E *>(a.b) +
                                        ((size_t)ad * a.N + imin(n0 + expand_column<DT>(t, c), a.N - 1)) * RANK + RS * g, sizeof b[t]);
         const float scale = a.scale[ad];
-        for (int q = 0; q < RT; q++) {
-            const uint32_t those = (uint32_t)(all >> (16 * q)) & 0xffffu;
-            if (RT > 1 && !those) continue;
-            float h[RS];
+        const bool whole = a.vec && n0 + 64 <= a.N;
+        /* everything that 16 · RT rows need is requested before the first product */
+        ExpandRows<DT> zr[RT];
+        float h[RT][RS];
 #pragma unroll
-            for (int s = 0; s < RS; s++) h[s] = 0.0f;
-            if ((those >> c) & 1)
+        for (int q = 0; q < RT; q++) {
+            const bool in = (all >> (16 * q + c)) & 1;
+            if (whole) zr[q].load(a, in, m0 + 16 * q + c, n0, g);
+#pragma unroll
+            for (int s = 0; s < RS; s++) h[q][s] = 0.0f;
+            if (in) {
+#pragma unroll(RT > 1 ? 1 : RS <= 4 ? 8 : RS <= 8 ? 4 : 1)
                 for (int p = 0; p < parts; p++) {
                     const float *from = FUSED ? &sum[FUSED ? p : 0][c][RS * g]
                                               : a.h + ((size_t)p * a.M + m0 + 16 * q + c) * RANK + RS * g;
 #pragma unroll
-                    for (int s = 0; s < RS; s++) h[s] += from[s];
+                    for (int s = 0; s < RS; s++) h[q][s] += from[s];
                 }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < RT; q++) {
+            const uint32_t those = (uint32_t)(all >> (16 * q)) & 0xffffu;
+            if (RT > 1 && !those) continue;
+#pragma unroll
+            for (int s = 0; s < RS; s++) h[q][s] *= scale;
+            expand_rows<DT, RANK>(a, those, m0 + 16 * q, n0, whole, zr[q], h[q], b, tile[wave]);
+        }
+    }
+}
+
+/* The same for many rows whose Z and Y are read and written 16 bytes at a time: 64 rows a workgroup, 16 a wave, its columns 64
+ * at a time. An adapter's 64 rows of B come through LDS, shared by the waves, the next ones on their way meanwhile, and a
+ * wave's results leave through its LDS, so that loads and stores go along rows: with lanes in different rows, as the products
+ * have them, a CU takes four times as long for each, and that was the kernel's time (fp32 6000 x 4096, rank 32: 68 us). */
+template <int DT, int RANK> struct ExpandLds {
+    typedef typename Elem<DT>::type E;
+    static constexpr int RB = RANK * sizeof(E), CH = RB / 16;   /* a row of B, in pieces of 16 bytes */
+    static constexpr int LOADS = 64 * CH < 256 ? 1 : 64 * CH / 256;   /* a thread's pieces of 64 rows */
+    E b[2][64 * RANK];
+    float tile[4][16][68];
+    /* 16 rows' pieces fall into different banks */
+    static __device__ __forceinline__ int place(int r, int p) { return p ^ (CH >= 16 ? r & 15 : (r / (16 / CH)) & (CH - 1)); }
+};
+
+template <int DT, int RANK>
+__global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
+{
+    typedef typename Elem<DT>::type E;
+    typedef ExpandLds<DT, RANK> L;
+    constexpr int RS = RANK / 4, VE = kPer16<DT>, LPR = 64 / VE, RPL = 64 / LPR, NZ = 16 / RPL;   /* lanes a row, rows a load */
+    __shared__ __align__(16) L lds;
+    __shared__ AdapterList list;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int m0 = 64 * blockIdx.y, rows = imin(64, a.M - m0), mw = m0 + 16 * wave;
+    const int u0 = blockIdx.x * a.units, u1 = imin(u0 + a.units, (a.N + 63) / 64);
+    list_adapters(a, m0, rows, &list);
+    const int n = __builtin_amdgcn_readfirstlane(list.n);
+    /* rows of this wave with an adapter; this lane's row times its adapter's scale */
+    uint32_t some = 0;
+    float h[RS];
+#pragma unroll
+    for (int s = 0; s < RS; s++) h[s] = 0.0f;
+    for (int j = 0; j < n; j++) {
+        const int ad = __builtin_amdgcn_readfirstlane(list.of[j]);
+        const uint32_t those = (uint32_t)__builtin_amdgcn_readfirstlane((int)(list.rows[j] >> (16 * wave))) & 0xffffu;
+        if (ad < 0) continue;
+        some |= those;
+        if ((those >> c) & 1) {
+            const float scale = a.scale[ad];
+            for (int p = 0; p < a.parts; p++) {
+                const float *from = a.h + ((size_t)p * a.M + mw + c) * RANK + RS * g;
+#pragma unroll
+                for (int s = 0; s < RS; s++) h[s] += from[s];
+            }
 #pragma unroll
             for (int s = 0; s < RS; s++) h[s] *= scale;
-            expand_rows<DT, RANK>(a, those, m0 + 16 * q, n0, h, b, tile[wave]);
         }
+    }
+    /* rows RPL · i + lane / LPR, VE columns from VE · (lane % LPR) on */
+    const int zr = lane / LPR, zc = VE * (lane % LPR);
+    auto load_z = [&](int u, u4 (&z)[NZ]) __attribute__((always_inline)) {
+        const int col = 64 * u + zc;
+#pragma unroll
+        for (int i = 0; i < NZ; i++) {
+            const int r = RPL * i + zr;
+            z[i] = u4{0, 0, 0, 0};
+            if (!a.z || 16 * wave + r >= rows) continue;
+            const E *p = static_cast<const E *>(a.z) + (size_t)(mw + r) * a.ldz + col;
+            if (col + VE <= a.N) z[i] = *reinterpret_cast<const u4 *>(p);
+            else z[i] = row_piece<DT, false>(p, 0, a.N - col);
+        }
+    };
+    auto load_b = [&](int u, int ad, u4 (&b)[L::LOADS]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < L::LOADS; i++) {
+            const int at = 256 * i + (int)threadIdx.x, r = imin(64 * u + at / L::CH, a.N - 1);
+            b[i] = u4{0, 0, 0, 0};
+            if (at < 64 * L::CH && a.count)
+                b[i] = *reinterpret_cast<const u4 *>(static_cast<const E *>(a.b) + ((size_t)ad * a.N + r) * RANK + VE * (at % L::CH));
+        }
+    };
+    auto put_b = [&](const u4 (&b)[L::LOADS], E *to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < L::LOADS; i++) {
+            const int at = 256 * i + (int)threadIdx.x, r = at / L::CH;
+            if (at < 64 * L::CH) *reinterpret_cast<u4 *>(to + r * RANK + VE * L::place(r, at % L::CH)) = b[i];
+        }
+    };
+    auto adapter_of = [&](int j) { return imax(__builtin_amdgcn_readfirstlane(list.of[j]), 0); };   /* of none: any */
+    u4 z[NZ], zn[NZ], b[L::LOADS];
+    if (u0 >= u1) return;
+    load_b(u0, adapter_of(0), b);
+    load_z(u0, z);
+    int buffer = 0;
+    for (int u = u0; u < u1; u++) {
+        if (u + 1 < u1) load_z(u + 1, zn);
+        f4 y[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) y[t] = f4{0, 0, 0, 0};
+        for (int j = 0; j < n; j++) {
+            put_b(b, lds.b[buffer]);
+            lds_barrier();
+            const bool last = j + 1 == n;
+            if (!last || u + 1 < u1) load_b(last ? u + 1 : u, adapter_of(last ? 0 : j + 1), b);
+            const uint32_t those = (uint32_t)__builtin_amdgcn_readfirstlane((int)(list.rows[j] >> (16 * wave))) & 0xffffu;
+            if (those && __builtin_amdgcn_readfirstlane(list.of[j]) >= 0) {
+                const bool in = (those >> c) & 1;
+                const E *from = lds.b[buffer];
+                f4 acc[4];
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const int r = 16 * t + c;
+                    E v[RS];
+                    if constexpr (RS >= VE) {
+#pragma unroll
+                        for (int x = 0; x < RS / VE; x++)
+                            __builtin_memcpy(v + VE * x, __builtin_assume_aligned(from + r * RANK + VE * L::place(r, RS / VE * g + x), 16), 16);
+                    } else {
+                        __builtin_memcpy(v, __builtin_assume_aligned(from + r * RANK + VE * L::place(r, RS * g / VE) + RS * g % VE, sizeof v),
+                                         sizeof v);
+                    }
+                    acc[t] = f4{0, 0, 0, 0};
+#pragma unroll
+                    for (int s = 0; s < RS; s++)
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(Elem<DT>::get(v[s]), h[s], acc[t], 0, 0, 0);
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y[t][i] = in ? acc[t][i] : y[t][i];
+            }
+            buffer ^= 1;
+        }
+        /* this lane's four columns 16t + 4g .. of row c; back as VE columns of a row */
+#pragma unroll
+        for (int t = 0; t < 4; t++) *reinterpret_cast<f4 *>(&lds.tile[wave][c][16 * t + 4 * g]) = y[t];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int col = 64 * u + zc;
+#pragma unroll
+        for (int i = 0; i < NZ; i++) {
+            const int r = RPL * i + zr;
+            float v[VE];
+            unpack<DT>(z[i], v);
+#pragma unroll
+            for (int x = 0; x < VE; x += 4) {
+                const f4 add = *reinterpret_cast<const f4 *>(&lds.tile[wave][r][zc + x]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[x + e] += add[e];
+            }
+            const u4 out = (some >> r) & 1 ? pack<DT>(v) : z[i];   /* a row without an adapter as it is */
+            if (16 * wave + r >= rows || col >= a.N) continue;
+            E *p = static_cast<E *>(a.y) + (size_t)(mw + r) * a.ldy + col;
+            if (col + VE <= a.N) {
+                *reinterpret_cast<u4 *>(p) = out;
+            } else {
+                E e[VE];
+                __builtin_memcpy(e, &out, sizeof e);
+                for (int x = 0; x < a.N - col; x++) p[x] = e[x];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < NZ; i++) z[i] = zn[i];
     }
 }
 

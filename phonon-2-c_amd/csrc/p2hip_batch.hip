@@ -26,11 +26,11 @@ struct Plan {
     }
 };
 
-/* Keys over workgroups: one for every 4 blocks a wave, as long as all together are at most 512, two for each of 256 CUs; a
- * number, as the workspace's size is asked for where there may be no device. */
-int parts_of(long long groups, long long keys, int block)
+/* Keys over workgroups: one for every 4 blocks a wave, as long as all together are at most `workgroups`, two for each of 256
+ * CUs; a number, as the workspace's size is asked for where there may be no device. */
+int parts_of(long long groups, long long keys, int block, int workgroups = 512)
 {
-    const long long most = groups ? 512 / groups : 1, n = keys / (4ll * block);
+    const long long most = groups ? workgroups / groups : 1, n = keys / (4ll * block);
     return (int)(n < 1 || most < 1 ? 1 : n < most ? n : most);
 }
 
@@ -46,7 +46,9 @@ Plan paged_plan(const CacheView &c, int n_seqs, int heads, int max_len, int wind
 {
     Plan p;
     p.q_groups = (heads / c.heads + 15) / 16;
-    p.o_parts = parts_of((long long)n_seqs * c.heads * p.q_groups, left_of(max_len, window, sinks), 32);
+    /* a block of heads of 64 is little to wait for: four workgroups a CU (8 sequences of 32768: 41 us against 45) */
+    p.o_parts = parts_of((long long)n_seqs * c.heads * p.q_groups, left_of(max_len, window, sinks), 32,
+                         c.head_dim == 64 ? 1024 : 512);
     return p;
 }
 
@@ -307,19 +309,21 @@ static int check_adapters(const char *name, const P2hAdapters *ad, int M)
 /* Adapters that 16 rows may have between them, as the host knows it */
 static int adapters_of_16(const P2hAdapters *ad, int M) { return p2k::imin(p2k::imin(M, 16), p2k::imax(ad->count, 1)); }
 
+constexpr int kManyRows = 512;   /* above: 64 rows a workgroup */
+
 /* K over workgroups, 0: everything in one launch, each workgroup making H for itself, while that is little to read. A number,
  * as the workspace's size is asked for where there may be no device. */
 static int adapter_parts(const P2hAdapters *ad, int M)
 {
-    const int tiles = (M + 15) / 16, n = adapters_of_16(ad, M);
-    if (tiles <= 1 && (size_t)n * ad->rank * ad->K * elem_size(ad->dtype) <= 128 << 10) return 0;
-    const int least = n <= 2 ? 512 : 128, most = (ad->K + least - 1) / least, want = (256 + tiles - 1) / (tiles > 0 ? tiles : 1);
-    return p2k::imax(p2k::imin(want, most), 1);
+    const int n = adapters_of_16(ad, M), tiles = (M - 1) / (M > kManyRows ? 64 : 16) + 1;
+    if (M <= 16 && (size_t)n * ad->rank * ad->K * elem_size(ad->dtype) <= 128 << 10) return 0;
+    const int least = n <= 2 || M > kManyRows ? 256 : 128, want = ((M > kManyRows ? 384 : 256) + tiles - 1) / tiles;
+    return p2k::imax(p2k::imin(p2k::imin(want, 16), ad->K / least), 1);
 }
 
 size_t p2h_adapters_workspace_bytes(const P2hAdapters *ad, int M)
 {
-    if (check_adapters("p2h_adapters_workspace_bytes", ad, M)) return 0;
+    if (check_adapters("p2h_adapters_workspace_bytes", ad, M) || M == 0) return 0;
     return (size_t)adapter_parts(ad, M) * M * ad->rank * 4;
 }
 
@@ -360,6 +364,8 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
     a.vec = aligned(dY, 16) && (M == 1 || ldy * es % 16 == 0) && (!dZ || (aligned(dZ, 16) && (M == 1 || ldz * es % 16 == 0)));
     const unsigned tiles = (unsigned)((M + 15) / 16), columns = (unsigned)((N - 1) / 64 + 1);
     const int n = adapters_of_16(ad, M);
+    /* of many rows, columns a workgroup: three workgroups a CU */
+    a.units = p2k::imax(p2k::imin((int)((size_t)columns * ((tiles + 3) / 4) / 768), 16), 1);
     hipStream_t s = stream_of(stream);
     by_type(ad->dtype, [&](auto t) {
         auto go = [&](auto rank) {
@@ -368,15 +374,17 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
                 constexpr bool V = decltype(v)::value != 0;
                 if (!a.parts)
                     hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 8, 1, 1, true, V>), dim3(columns, tiles), dim3(512), 0, s, a);
+                else if (V && M > kManyRows)
+                    hipLaunchKernelGGL((p2k::adapter_shrink_rows<DT, R>), dim3((tiles + 3) / 4, (unsigned)a.parts), dim3(256), 0, s, a);
                 else
                     hipLaunchKernelGGL((p2k::adapter_shrink<DT, R, NS, V>), dim3(tiles, (unsigned)a.parts), dim3(64 * NS), 0, s, a);
             };
             if (vec) aligned_x(ic<1>{});
             else aligned_x(ic<0>{});
             if (!a.parts) return;
-            if (M > 512)
-                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 4, 4, 4, false, true>), dim3((columns + 3) / 4, (tiles + 3) / 4),
-                                   dim3(256), 0, s, a);
+            if (M > kManyRows && a.vec)
+                hipLaunchKernelGGL((p2k::adapter_expand_rows<DT, R>), dim3((columns + a.units - 1) / a.units, (tiles + 3) / 4), dim3(256),
+                                   0, s, a);
             else if (n > 4)
                 hipLaunchKernelGGL((p2k::adapter_expand<DT, R, NS, 1, 1, false, true>), dim3(columns, tiles), dim3(64 * NS), 0, s, a);
             else

@@ -459,7 +459,9 @@ def test_shared_fp32_on_the_whole(Dh, kind):
 
 ADAPTERS = [  # M, K, N, rank, adapters
     (1, 64, 16, 8, 1), (1, 1024, 1024, 8, 4), (5, 77, 143, 16, 3), (16, 129, 65, 32, 2), (17, 256, 300, 64, 20),
-    (33, 1000, 515, 128, 5), (100, 136, 7, 16, 4), (13, 4096, 257, 16, 13), (70, 1, 1, 8, 2), (3, 8192, 40, 32, 2)]
+    (33, 1000, 515, 128, 5), (100, 136, 7, 16, 4), (13, 4096, 257, 16, 13), (70, 1, 1, 8, 2), (3, 8192, 40, 32, 2),
+    (600, 72, 200, 8, 3), (515, 520, 136, 16, 5), (700, 264, 72, 32, 40), (530, 1160, 64, 64, 2), (577, 128, 328, 128, 3),
+    (513, 100, 131, 64, 4), (520, 136, 133, 32, 2), (514, 67, 64, 16, 2)]
 
 
 @pytest.mark.parametrize("t", D.TYPES)
@@ -468,7 +470,9 @@ def test_adapters(t, M, K, N, rank, count):
     rng = rng_of(t, M, K, N, rank)
     x, z = D.rows(rng, t, M, K), D.rows(rng, t, M, N)
     a, b, scale = B.adapter_set(rng, t, count, rank, K, N)
-    for index in (rng.integers(-1, count + 1, M), np.sort(rng.integers(0, count, M)), np.full(M, count - 1)):
+    runs = np.sort(rng.integers(0, count, M))
+    runs[M // 3:M // 2] = -1
+    for index in (rng.integers(-1, count + 1, M), runs, np.full(M, count - 1)):
         want, bound = B.adapters_want(t, x, index, a, b, scale, z)
         got = B.run_adapters(t, x, index, a, b, scale, z)
         D.check(D.to_f64(t, got), want, bound, f"{t} {M} {K} {N} {rank}")
@@ -479,14 +483,15 @@ def test_adapters(t, M, K, N, rank, count):
 
 
 @pytest.mark.parametrize("t", D.TYPES)
-def test_adapters_pitches_and_no_rows_before(t):
-    M, K, N, rank, count = 37, 200, 133, 16, 6
+@pytest.mark.parametrize("M", (7, 37, 600))
+def test_adapters_pitches_and_no_rows_before(t, M):
+    K, N, rank, count = 200, 133, 16, 6
     rng = rng_of(t, "pitch")
     x, z = D.rows(rng, t, M, K), D.rows(rng, t, M, N)
     a, b, scale = B.adapter_set(rng, t, count, rank, K, N)
     index = rng.integers(-1, count, M)
     want = B.run_adapters(t, x, index, a, b, scale, z)
-    for pads in ((8, 3, 5), (1, 0, 16), (3, 7, 0)):
+    for pads in ((8, 3, 5), (1, 0, 16), (3, 7, 0), (8, 11, 27)):   # of the last, rows are 16 bytes apart
         got = B.run_adapters(t, x, index, a, b, scale, z, pads=pads)
         exp, bound = B.adapters_want(t, x, index, a, b, scale, z)
         D.check(D.to_f64(t, got[:, :N]), exp, bound, str(pads))
@@ -501,7 +506,7 @@ def test_adapters_pitches_and_no_rows_before(t):
 
 
 @pytest.mark.parametrize("t", D.TYPES)
-@pytest.mark.parametrize("M", (20, 300))
+@pytest.mark.parametrize("M", (7, 20, 300, 600))
 def test_adapters_do_not_reach_other_rows(t, M):
     """Adapters and rows that are not finite change no row of another adapter; zeros of both signs and NaN of rows without
     an adapter stay as they are."""
@@ -522,7 +527,22 @@ def test_adapters_do_not_reach_other_rows(t, M):
     assert not np.isfinite(D.to_f64(t, got[~keep])).any()
 
 
-@pytest.mark.parametrize("M,K,N,rank", ((40, 1024, 300, 64), (300, 1000, 64, 16), (5, 512, 700, 128)))
+@pytest.mark.parametrize("t", D.TYPES)
+@pytest.mark.parametrize("M", (0, 9, 50, 600))
+def test_no_adapters_at_all(t, M):
+    """A set of none, and one that no row has: Z as it is."""
+    rng = rng_of(t, "none")
+    x, z = D.rows(rng, t, M, 64), D.rows(rng, t, M, 40)
+    a, b, scale = B.adapter_set(rng, t, 2, 16, 64, 40)
+    assert np.array_equal(B.run_adapters(t, x, np.full(M, 2), a, b, scale, z).view(np.uint16), z.view(np.uint16))
+    dx, dz, di, dy = D.device(x), D.device(z), D.device(np.zeros(M, np.int32)), D.preset(t, (max(M, 1), 40))
+    ad = P.Adapters(t, 0, 16, 64, 40, None, None, None)
+    ws = P.Workspace(P.adapters_workspace_bytes(ad, M))
+    P.adapters_add_dev(ad, M, dx.ptr, 64, di.ptr, dz.ptr, 40, dy.ptr, 40, ws.ptr, ws.nbytes)
+    assert np.array_equal(dy.download((M, 40), D.np_type(t)).view(np.uint16), z.view(np.uint16))
+
+
+@pytest.mark.parametrize("M,K,N,rank", ((40, 1024, 300, 64), (300, 1000, 64, 16), (5, 512, 700, 128), (600, 1024, 64, 64)))
 def test_adapters_fp32_on_the_whole(M, K, N, rank):
     """Relative 2-norm of what the adapter adds: each product of the fp32 matrix unit may drop up to a step, rms 0.58 · 2 ·
     2^-24 of a sum that grows as a random walk: n products 1.15 · sqrt(n / 2) · 2^-24. A wave's quarter of K 256, 13; the
