@@ -1342,17 +1342,23 @@ __global__ __launch_bounds__(64 * NW) void adapter_expand(AdapterArgs a)
 }
 
 /* The same for many rows whose Z and Y are read and written 16 bytes at a time: 64 rows a workgroup, 16 a wave, its columns 64
- * at a time. An adapter's 64 rows of B come through LDS, shared by the waves, the next ones on their way meanwhile, and a
- * wave's results leave through its LDS, so that loads and stores go along rows: with lanes in different rows, as the products
- * have them, a CU takes four times as long for each, and that was the kernel's time (fp32 6000 x 4096, rank 32: 68 us). */
+ * at a time. Loads and stores go along rows: with lanes in different rows, as the products have them, a CU takes four times as
+ * long for each. An adapter's 64 rows of B come through LDS, shared by the waves, and each wave's 16 rows of Z too, where the
+ * sums are put in their place before they leave.
+ *
+ * Everything comes by direct loads, a step (64 columns of one adapter) or a unit (64 columns) ahead, and is waited for by
+ * number: the compiler's own waits, which do not know how many stores a path has issued, would wait for all of them. Such a
+ * number is that of loads and stores that are sure to have been issued since; `z_since` and `b_since` count them. */
 template <int DT, int RANK> struct ExpandLds {
     typedef typename Elem<DT>::type E;
-    static constexpr int RB = RANK * sizeof(E), CH = RB / 16;   /* a row of B, in pieces of 16 bytes */
-    static constexpr int LOADS = 64 * CH < 256 ? 1 : 64 * CH / 256;   /* a thread's pieces of 64 rows */
-    E b[2][64 * RANK];
-    float tile[4][16][68];
-    /* 16 rows' pieces fall into different banks */
-    static __device__ __forceinline__ int place(int r, int p) { return p ^ (CH >= 16 ? r & 15 : (r / (16 / CH)) & (CH - 1)); }
+    static constexpr int VE = kPer16<DT>, BCH = RANK / VE, ZCH = 64 / VE;   /* 16-byte pieces of a row of B, of 64 columns */
+    static constexpr int NB = BCH < 4 ? 1 : BCH / 4, NZ = ZCH / 4;          /* a wave's loads of 64 rows of B, of 16 of Z */
+    E b[2][64 * RANK], z[2][4][16 * 64];
+    /* where a row's piece lies, so that 16 rows' pieces fall into different banks */
+    template <int CH> static __device__ __forceinline__ int place(int r, int p)
+    {
+        return p ^ (CH >= 16 ? r & 15 : (r / (16 / CH)) & (CH - 1));
+    }
 };
 
 template <int DT, int RANK>
@@ -1360,23 +1366,26 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
 {
     typedef typename Elem<DT>::type E;
     typedef ExpandLds<DT, RANK> L;
-    constexpr int RS = RANK / 4, VE = kPer16<DT>, LPR = 64 / VE, RPL = 64 / LPR, NZ = 16 / RPL;   /* lanes a row, rows a load */
+    constexpr int RS = RANK / 4, VE = L::VE, BCH = L::BCH, ZCH = L::ZCH, NB = L::NB, NZ = L::NZ, RPL = 64 / ZCH;
     __shared__ __align__(16) L lds;
     __shared__ AdapterList list;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
-    const int m0 = 64 * blockIdx.y, rows = imin(64, a.M - m0), mw = m0 + 16 * wave;
-    const int u0 = blockIdx.x * a.units, u1 = imin(u0 + a.units, (a.N + 63) / 64);
+    const int m0 = 64 * blockIdx.y, rows = imin(64, a.M - m0), mw = m0 + 16 * wave, have = rows - 16 * wave;   /* this wave's rows */
+    const int u0 = blockIdx.x * a.units, units = imin(a.units, (a.N + 63) / 64 - u0);
+    if (units <= 0) return;
     list_adapters(a, m0, rows, &list);
     const int n = __builtin_amdgcn_readfirstlane(list.n);
+    auto adapter_of = [&](int j) { return __builtin_amdgcn_readfirstlane(list.of[j]); };
+    auto rows_of = [&](int j) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(list.rows[j] >> (16 * wave))) & 0xffffu; };
     /* rows of this wave with an adapter; this lane's row times its adapter's scale */
     uint32_t some = 0;
     float h[RS];
 #pragma unroll
     for (int s = 0; s < RS; s++) h[s] = 0.0f;
     for (int j = 0; j < n; j++) {
-        const int ad = __builtin_amdgcn_readfirstlane(list.of[j]);
-        const uint32_t those = (uint32_t)__builtin_amdgcn_readfirstlane((int)(list.rows[j] >> (16 * wave))) & 0xffffu;
+        const int ad = adapter_of(j);
         if (ad < 0) continue;
+        const uint32_t those = rows_of(j);
         some |= those;
         if ((those >> c) & 1) {
             const float scale = a.scale[ad];
@@ -1389,114 +1398,128 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
             for (int s = 0; s < RS; s++) h[s] *= scale;
         }
     }
-    /* rows RPL · i + lane / LPR, VE columns from VE · (lane % LPR) on */
-    const int zr = lane / LPR, zc = VE * (lane % LPR);
-    auto load_z = [&](int u, u4 (&z)[NZ]) __attribute__((always_inline)) {
-        const int col = 64 * u + zc;
+    const E *const zp = static_cast<const E *>(a.z ? a.z : a.y);   /* without Z what is read is not used */
+    const int ldz = a.z ? a.ldz : a.ldy, last_piece = a.N / VE - 1;   /* of a row's whole pieces */
+    const int zr = lane / ZCH, zc = lane % ZCH;
+    auto fetch_z = [&](int u, int buffer) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NZ; i++) {
-            const int r = RPL * i + zr;
-            z[i] = u4{0, 0, 0, 0};
-            if (!a.z || 16 * wave + r >= rows) continue;
-            const E *p = static_cast<const E *>(a.z) + (size_t)(mw + r) * a.ldz + col;
-            if (col + VE <= a.N) z[i] = *reinterpret_cast<const u4 *>(p);
-            else z[i] = row_piece<DT, false>(p, 0, a.N - col);
+            const int r = RPL * i + zr, row = m0 + imin(16 * wave + r, rows - 1);
+            dma_16(zp + (size_t)row * ldz + VE * imin(64 / VE * u + L::template place<ZCH>(r, zc), last_piece), lds.z[buffer][wave] + 512 / (8 / VE) * i);
         }
     };
-    auto load_b = [&](int u, int ad, u4 (&b)[L::LOADS]) __attribute__((always_inline)) {
+    auto fetch_b = [&](int u, int ad, int buffer) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < L::LOADS; i++) {
-            const int at = 256 * i + (int)threadIdx.x, r = imin(64 * u + at / L::CH, a.N - 1);
-            b[i] = u4{0, 0, 0, 0};
-            if (at < 64 * L::CH && a.count)
-                b[i] = *reinterpret_cast<const u4 *>(static_cast<const E *>(a.b) + ((size_t)ad * a.N + r) * RANK + VE * (at % L::CH));
+        for (int i = 0; i < NB; i++) {
+            const int load = BCH < 4 ? wave % BCH : NB * wave + i, at = 64 * load + lane, r = at / BCH;
+            dma_16(static_cast<const E *>(a.b) + ((size_t)imax(ad, 0) * a.N + imin(64 * u + r, a.N - 1)) * RANK +
+                       VE * L::template place<BCH>(r, at % BCH),
+                   lds.b[buffer] + 64 * VE * load);
         }
     };
-    auto put_b = [&](const u4 (&b)[L::LOADS], E *to) __attribute__((always_inline)) {
+    E *const y = static_cast<E *>(a.y) + (size_t)mw * a.ldy;
+    const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
+        y, 0, have > 0 ? (int)((uint32_t)((imin(have, 16) - 1) * a.ldy + a.N) * sizeof(E)) : 0, 0x00020000);
+
+    fetch_b(u0, adapter_of(0), 0);
+    fetch_z(u0, 0);
+    int buffer = 0, b_since = NZ, z_since = 0;   /* how many are sure to have been issued since the next step's B, the unit's Z */
+    for (int k = 0; k < units; k++) {
+        const int u = u0 + k;
+        f4 sum[4];
 #pragma unroll
-        for (int i = 0; i < L::LOADS; i++) {
-            const int at = 256 * i + (int)threadIdx.x, r = at / L::CH;
-            if (at < 64 * L::CH) *reinterpret_cast<u4 *>(to + r * RANK + VE * L::place(r, at % L::CH)) = b[i];
-        }
-    };
-    auto adapter_of = [&](int j) { return imax(__builtin_amdgcn_readfirstlane(list.of[j]), 0); };   /* of none: any */
-    u4 z[NZ], zn[NZ], b[L::LOADS];
-    if (u0 >= u1) return;
-    load_b(u0, adapter_of(0), b);
-    load_z(u0, z);
-    int buffer = 0;
-    for (int u = u0; u < u1; u++) {
-        if (u + 1 < u1) load_z(u + 1, zn);
-        f4 y[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) y[t] = f4{0, 0, 0, 0};
+        for (int t = 0; t < 4; t++) sum[t] = f4{0, 0, 0, 0};
         for (int j = 0; j < n; j++) {
-            put_b(b, lds.b[buffer]);
-            lds_barrier();
-            const bool last = j + 1 == n;
-            if (!last || u + 1 < u1) load_b(last ? u + 1 : u, adapter_of(last ? 0 : j + 1), b);
-            const uint32_t those = (uint32_t)__builtin_amdgcn_readfirstlane((int)(list.rows[j] >> (16 * wave))) & 0xffffu;
-            if (those && __builtin_amdgcn_readfirstlane(list.of[j]) >= 0) {
+            const bool end = j + 1 == n;
+            const uint32_t those = rows_of(j);
+            /* the next step's B and, in a unit's first step, the next unit's Z; past the last the same again, which nothing reads */
+            fetch_b(u0 + imin(k + end, units - 1), adapter_of(end ? 0 : j + 1), buffer ^ 1);
+            if (j == 0) fetch_z(u0 + imin(k + 1, units - 1), (k + 1) & 1);
+            b_since += NB + (j == 0 ? NZ : 0);
+            z_since += NB + (j == 0 ? NZ : 0);
+            if (b_since >= NB + 3 * NZ) wait_vm<NB + 3 * NZ>();
+            else if (b_since >= NB + 2 * NZ) wait_vm<NB + 2 * NZ>();
+            else if (b_since >= NB + NZ) wait_vm<NB + NZ>();
+            else wait_vm<NB>();
+            lds_barrier();   /* everyone's part of B */
+            b_since = j == 0 ? NZ : 0;
+            if (those && adapter_of(j) >= 0) {
                 const bool in = (those >> c) & 1;
                 const E *from = lds.b[buffer];
                 f4 acc[4];
+                E v[4][RS];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    const int r = 16 * t + c;
-                    E v[RS];
+                    const int r = expand_column<DT>(t, c);
                     if constexpr (RS >= VE) {
 #pragma unroll
                         for (int x = 0; x < RS / VE; x++)
-                            __builtin_memcpy(v + VE * x, __builtin_assume_aligned(from + r * RANK + VE * L::place(r, RS / VE * g + x), 16), 16);
+                            __builtin_memcpy(v[t] + VE * x, __builtin_assume_aligned(from + r * RANK + VE * L::template place<BCH>(r, RS / VE * g + x), 16), 16);
                     } else {
-                        __builtin_memcpy(v, __builtin_assume_aligned(from + r * RANK + VE * L::place(r, RS * g / VE) + RS * g % VE, sizeof v),
-                                         sizeof v);
+                        __builtin_memcpy(v[t], __builtin_assume_aligned(from + r * RANK + VE * L::template place<BCH>(r, RS * g / VE) + RS * g % VE, sizeof v[t]),
+                                         sizeof v[t]);
                     }
                     acc[t] = f4{0, 0, 0, 0};
-#pragma unroll
-                    for (int s = 0; s < RS; s++)
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(Elem<DT>::get(v[s]), h[s], acc[t], 0, 0, 0);
                 }
+#pragma unroll
+                for (int s = 0; s < RS; s++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(Elem<DT>::get(v[t][s]), h[s], acc[t], 0, 0, 0);
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) y[t][i] = in ? acc[t][i] : y[t][i];
+                    for (int i = 0; i < 4; i++) sum[t][i] = in ? acc[t][i] : sum[t][i];
             }
+            lds_barrier();   /* everyone is done with this step's B */
             buffer ^= 1;
         }
-        /* this lane's four columns 16t + 4g .. of row c; back as VE columns of a row */
+        if (z_since >= NB + 2 * NZ) wait_vm<NB + 2 * NZ>();
+        else wait_vm<NB + NZ>();
+        /* a lane's results are whole pieces of row c: into their places in LDS, and from there along rows */
+        E *const zl = lds.z[k & 1][wave];
 #pragma unroll
-        for (int t = 0; t < 4; t++) *reinterpret_cast<f4 *>(&lds.tile[wave][c][16 * t + 4 * g]) = y[t];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const int col = 64 * u + zc;
-#pragma unroll
-        for (int i = 0; i < NZ; i++) {
-            const int r = RPL * i + zr;
+        for (int p = 0; p < 16 / VE; p++) {
+            u4 *at = reinterpret_cast<u4 *>(zl + 64 * c + VE * L::template place<ZCH>(c, 4 * p + g));
+            const u4 before = a.z ? *at : u4{0, 0, 0, 0};
             float v[VE];
-            unpack<DT>(z[i], v);
+            unpack<DT>(before, v);
 #pragma unroll
-            for (int x = 0; x < VE; x += 4) {
-                const f4 add = *reinterpret_cast<const f4 *>(&lds.tile[wave][r][zc + x]);
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[x + e] += add[e];
-            }
-            const u4 out = (some >> r) & 1 ? pack<DT>(v) : z[i];   /* a row without an adapter as it is */
-            if (16 * wave + r >= rows || col >= a.N) continue;
-            E *p = static_cast<E *>(a.y) + (size_t)(mw + r) * a.ldy + col;
-            if (col + VE <= a.N) {
-                *reinterpret_cast<u4 *>(p) = out;
-            } else {
-                E e[VE];
-                __builtin_memcpy(e, &out, sizeof e);
-                for (int x = 0; x < a.N - col; x++) p[x] = e[x];
-            }
+            for (int x = 0; x < VE; x++) v[x] += sum[VE / 4 * p + x / 4][x % 4];
+            *at = (some >> c) & 1 ? pack<DT>(v) : before;   /* a row without an adapter as it is */
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int i = 0; i < NZ; i++) z[i] = zn[i];
+        for (int i = 0; i < NZ; i++) {
+            const int r = RPL * i + zr, col = 64 * u + VE * zc;
+            const u4 v = *reinterpret_cast<const u4 *>(zl + 64 * r + VE * L::template place<ZCH>(r, zc));
+            const bool whole = r < have && col + VE <= a.N;   /* others leave past the end, which writes nothing */
+            __builtin_amdgcn_raw_buffer_store_b128(v, out, whole ? (int)((uint32_t)(r * a.ldy + col) * sizeof(E)) : -16, 0, 0);
+        }
+        if (u == (a.N - 1) / 64 && a.N % VE != 0) {   /* the last columns, fewer than a piece: their Z was not loaded whole either */
+            const int col = a.N / VE * VE, t = (col - 64 * u) / VE;
+            if (g == t % 4 && c < have) {
+                float v[VE];
+#pragma unroll
+                for (int x = 0; x < VE; x++) v[x] = 0.0f;
+#pragma unroll
+                for (int p = 0; p < 16 / VE; p++)
+                    if (p == t / 4)
+#pragma unroll
+                        for (int x = 0; x < VE; x++) v[x] = sum[VE / 4 * p + x / 4][x % 4];
+#pragma unroll
+                for (int x = 0; x < VE; x++)
+                    if (col + x < a.N) {
+                        const E before = a.z ? static_cast<const E *>(a.z)[(size_t)(mw + c) * a.ldz + col + x] : Elem<DT>::put(0.0f);
+                        y[(size_t)c * a.ldy + col + x] = (some >> c) & 1 ? Elem<DT>::put(Elem<DT>::get(before) + v[x]) : before;
+                    }
+            }
+        }
+        b_since += NZ;
+        z_since = n > 1 ? 0 : NZ;
     }
+    wait_vm<0>();   /* nothing comes into the LDS any more */
 }
 
 }  // namespace p2k

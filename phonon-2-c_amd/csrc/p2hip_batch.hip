@@ -317,7 +317,7 @@ static int adapter_parts(const P2hAdapters *ad, int M)
 {
     const int n = adapters_of_16(ad, M), tiles = (M - 1) / (M > kManyRows ? 64 : 16) + 1;
     if (M <= 16 && (size_t)n * ad->rank * ad->K * elem_size(ad->dtype) <= 128 << 10) return 0;
-    const int least = n <= 2 || M > kManyRows ? 256 : 128, want = ((M > kManyRows ? 384 : 256) + tiles - 1) / tiles;
+    const int least = n <= 2 && M <= kManyRows ? 256 : 128, want = M > kManyRows ? 768 / tiles : (256 + tiles - 1) / tiles;
     return p2k::imax(p2k::imin(p2k::imin(want, 16), ad->K / least), 1);
 }
 
@@ -364,8 +364,9 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
     a.vec = aligned(dY, 16) && (M == 1 || ldy * es % 16 == 0) && (!dZ || (aligned(dZ, 16) && (M == 1 || ldz * es % 16 == 0)));
     const unsigned tiles = (unsigned)((M + 15) / 16), columns = (unsigned)((N - 1) / 64 + 1);
     const int n = adapters_of_16(ad, M);
-    /* of many rows, columns a workgroup: three workgroups a CU */
-    a.units = p2k::imax(p2k::imin((int)((size_t)columns * ((tiles + 3) / 4) / 768), 16), 1);
+    /* of many rows, columns a workgroup: as many workgroups as three a CU, so that they begin and end together */
+    const unsigned groups = (tiles + 3) / 4 < 768 ? 768 / ((tiles + 3) / 4) : 1;
+    a.units = (int)((columns + groups - 1) / groups);
     hipStream_t s = stream_of(stream);
     by_type(ad->dtype, [&](auto t) {
         auto go = [&](auto rank) {
@@ -382,7 +383,7 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
             if (vec) aligned_x(ic<1>{});
             else aligned_x(ic<0>{});
             if (!a.parts) return;
-            if (M > kManyRows && a.vec)
+            if (M > kManyRows && a.vec && N >= 64 && ad->count > 0)
                 hipLaunchKernelGGL((p2k::adapter_expand_rows<DT, R>), dim3((columns + a.units - 1) / a.units, (tiles + 3) / 4), dim3(256),
                                    0, s, a);
             else if (n > 4)

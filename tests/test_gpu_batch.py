@@ -532,14 +532,15 @@ def test_adapters_do_not_reach_other_rows(t, M):
 def test_no_adapters_at_all(t, M):
     """A set of none, and one that no row has: Z as it is."""
     rng = rng_of(t, "none")
-    x, z = D.rows(rng, t, M, 64), D.rows(rng, t, M, 40)
-    a, b, scale = B.adapter_set(rng, t, 2, 16, 64, 40)
+    N = 128
+    x, z = D.rows(rng, t, M, 64), D.rows(rng, t, M, N)
+    a, b, scale = B.adapter_set(rng, t, 2, 16, 64, N)
     assert np.array_equal(B.run_adapters(t, x, np.full(M, 2), a, b, scale, z).view(np.uint16), z.view(np.uint16))
-    dx, dz, di, dy = D.device(x), D.device(z), D.device(np.zeros(M, np.int32)), D.preset(t, (max(M, 1), 40))
-    ad = P.Adapters(t, 0, 16, 64, 40, None, None, None)
+    dx, dz, di, dy = D.device(x), D.device(z), D.device(np.zeros(M, np.int32)), D.preset(t, (max(M, 1), N))
+    ad = P.Adapters(t, 0, 16, 64, N, None, None, None)
     ws = P.Workspace(P.adapters_workspace_bytes(ad, M))
-    P.adapters_add_dev(ad, M, dx.ptr, 64, di.ptr, dz.ptr, 40, dy.ptr, 40, ws.ptr, ws.nbytes)
-    assert np.array_equal(dy.download((M, 40), D.np_type(t)).view(np.uint16), z.view(np.uint16))
+    P.adapters_add_dev(ad, M, dx.ptr, 64, di.ptr, dz.ptr, N, dy.ptr, N, ws.ptr, ws.nbytes)
+    assert np.array_equal(dy.download((M, N), D.np_type(t)).view(np.uint16), z.view(np.uint16))
 
 
 @pytest.mark.parametrize("M,K,N,rank", ((40, 1024, 300, 64), (300, 1000, 64, 16), (5, 512, 700, 128), (600, 1024, 64, 64)))
