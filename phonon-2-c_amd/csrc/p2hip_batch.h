@@ -1145,25 +1145,29 @@ __global__ __launch_bounds__(256) void adapter_shrink_rows(AdapterArgs a)
     __shared__ AdapterList list;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     const int m0 = 64 * blockIdx.x, rows = imin(64, a.M - m0), k0 = blockIdx.y * a.chunk, k1 = imin(k0 + a.chunk, a.K);
-    list_adapters(a, m0, rows, &list);
-    const int stages = k1 > k0 ? (k1 - k0 + KC - 1) / KC : 0, n = __builtin_amdgcn_readfirstlane(list.n);
+    const int stages = k1 > k0 ? (k1 - k0 + KC - 1) / KC : 0;
     const E *const x = static_cast<const E *>(a.x);
     /* row r has its piece p at place p ^ (r mod 16); a load brings 4 rows */
     auto place = [](int r, int p) { return p ^ (r & 15); };
-    auto fetch = [&](int ad, int st, unsigned char *to) __attribute__((always_inline)) {
-        const int k = k0 + KC * st;
-        auto piece = [&](int r) { return imin(k + VE * place(r, lane & 15), k1 - VE); };   /* past the end: the last one again */
+    auto piece = [&](int st, int r) { return imin(k0 + KC * st + VE * place(r, lane & 15), k1 - VE); };   /* past the end: the last one */
+    auto fetch_x = [&](int st, unsigned char *to) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = 16 * wave + 4 * i + (lane >> 4);
-            dma_16(x + (size_t)(m0 + imin(r, rows - 1)) * a.ldx + piece(r), to + 1024 * (4 * wave + i));
+            dma_16(x + (size_t)(m0 + imin(r, rows - 1)) * a.ldx + piece(st, r), to + 1024 * (4 * wave + i));
         }
+    };
+    auto fetch_a = [&](int ad, int st, unsigned char *to) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < ALD; i++) {
             const int load = RANK < 16 ? wave % (RANK / 4) : ALD * wave + i, r = 4 * load + (lane >> 4);
-            dma_16(static_cast<const E *>(a.a) + ((size_t)ad * RANK + r) * a.K + piece(r), to + 64 * 256 + 1024 * load);
+            dma_16(static_cast<const E *>(a.a) + ((size_t)ad * RANK + r) * a.K + piece(st, r), to + 64 * 256 + 1024 * load);
         }
     };
+    if (stages > 0) fetch_x(0, lds);   /* on its way while the adapters are looked up */
+    list_adapters(a, m0, rows, &list);
+    const int n = __builtin_amdgcn_readfirstlane(list.n);
+    bool fetched = true;
     for (int j = 0; j < n; j++) {
         const int ad = __builtin_amdgcn_readfirstlane(list.of[j]);
         if (ad < 0) continue;
@@ -1171,11 +1175,17 @@ __global__ __launch_bounds__(256) void adapter_shrink_rows(AdapterArgs a)
         f4 acc[RT];
 #pragma unroll
         for (int t = 0; t < RT; t++) acc[t] = f4{0, 0, 0, 0};
-        if (stages > 0) fetch(ad, 0, lds);
+        if (stages > 0) {
+            if (!fetched) fetch_x(0, lds);
+            fetch_a(ad, 0, lds);
+        }
+        fetched = false;
         for (int st = 0; st < stages; st++) {
             unsigned char *const now = lds + (st & 1) * shrink_stage<RANK>();
             /* the last stage's loads again, which nothing reads, so that there are always as many to wait for */
-            fetch(ad, imin(st + 1, stages - 1), lds + ((st & 1) ^ 1) * shrink_stage<RANK>());
+            unsigned char *const then = lds + ((st & 1) ^ 1) * shrink_stage<RANK>();
+            fetch_x(imin(st + 1, stages - 1), then);
+            fetch_a(ad, imin(st + 1, stages - 1), then);
             wait_vm<4 + ALD>();
             lds_barrier();
             if (those) {
@@ -1203,6 +1213,7 @@ __global__ __launch_bounds__(256) void adapter_shrink_rows(AdapterArgs a)
                 if (((those >> (4 * g + i)) & 1) && 16 * t + c < RANK)
                     a.h[((size_t)blockIdx.y * a.M + m0 + 16 * wave + 4 * g + i) * RANK + 16 * t + c] = acc[t][i];
     }
+    wait_vm<0>();   /* nothing comes into the LDS any more, whatever adapters there were */
 }
 
 /* Row 4g + i of product t is this column of 64, so that a lane's results are 16 bytes of neighbours (16-bit rows: of two
@@ -1373,6 +1384,17 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
     const int m0 = 64 * blockIdx.y, rows = imin(64, a.M - m0), mw = m0 + 16 * wave, have = rows - 16 * wave;   /* this wave's rows */
     const int u0 = blockIdx.x * a.units, units = imin(a.units, (a.N + 63) / 64 - u0);
     if (units <= 0) return;
+    const E *const zp = static_cast<const E *>(a.z ? a.z : a.y);   /* without Z what is read is not used */
+    const int ldz = a.z ? a.ldz : a.ldy, last_piece = a.N / VE - 1;   /* of a row's whole pieces */
+    const int zr = lane / ZCH, zc = lane % ZCH;
+    auto fetch_z = [&](int u, int buffer) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NZ; i++) {
+            const int r = RPL * i + zr, row = m0 + imin(16 * wave + r, rows - 1);
+            dma_16(zp + (size_t)row * ldz + VE * imin(64 / VE * u + L::template place<ZCH>(r, zc), last_piece), lds.z[buffer][wave] + 512 / (8 / VE) * i);
+        }
+    };
+    fetch_z(u0, 0);   /* on its way while the adapters are looked up */
     list_adapters(a, m0, rows, &list);
     const int n = __builtin_amdgcn_readfirstlane(list.n);
     auto adapter_of = [&](int j) { return __builtin_amdgcn_readfirstlane(list.of[j]); };
@@ -1389,6 +1411,7 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
         some |= those;
         if ((those >> c) & 1) {
             const float scale = a.scale[ad];
+#pragma unroll(RS <= 8 ? 8 : RS <= 16 ? 4 : 2)
             for (int p = 0; p < a.parts; p++) {
                 const float *from = a.h + ((size_t)p * a.M + mw + c) * RANK + RS * g;
 #pragma unroll
@@ -1398,16 +1421,6 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
             for (int s = 0; s < RS; s++) h[s] *= scale;
         }
     }
-    const E *const zp = static_cast<const E *>(a.z ? a.z : a.y);   /* without Z what is read is not used */
-    const int ldz = a.z ? a.ldz : a.ldy, last_piece = a.N / VE - 1;   /* of a row's whole pieces */
-    const int zr = lane / ZCH, zc = lane % ZCH;
-    auto fetch_z = [&](int u, int buffer) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NZ; i++) {
-            const int r = RPL * i + zr, row = m0 + imin(16 * wave + r, rows - 1);
-            dma_16(zp + (size_t)row * ldz + VE * imin(64 / VE * u + L::template place<ZCH>(r, zc), last_piece), lds.z[buffer][wave] + 512 / (8 / VE) * i);
-        }
-    };
     auto fetch_b = [&](int u, int ad, int buffer) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NB; i++) {
@@ -1422,8 +1435,7 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
         y, 0, have > 0 ? (int)((uint32_t)((imin(have, 16) - 1) * a.ldy + a.N) * sizeof(E)) : 0, 0x00020000);
 
     fetch_b(u0, adapter_of(0), 0);
-    fetch_z(u0, 0);
-    int buffer = 0, b_since = NZ, z_since = 0;   /* how many are sure to have been issued since the next step's B, the unit's Z */
+    int buffer = 0, b_since = 0, z_since = 0;   /* how many are sure to have been issued since the next step's B, the unit's Z */
     for (int k = 0; k < units; k++) {
         const int u = u0 + k;
         f4 sum[4];

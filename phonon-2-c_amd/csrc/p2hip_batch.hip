@@ -364,8 +364,9 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
     a.vec = aligned(dY, 16) && (M == 1 || ldy * es % 16 == 0) && (!dZ || (aligned(dZ, 16) && (M == 1 || ldz * es % 16 == 0)));
     const unsigned tiles = (unsigned)((M + 15) / 16), columns = (unsigned)((N - 1) / 64 + 1);
     const int n = adapters_of_16(ad, M);
-    /* of many rows, columns a workgroup: as many workgroups as three a CU, so that they begin and end together */
-    const unsigned groups = (tiles + 3) / 4 < 768 ? 768 / ((tiles + 3) / 4) : 1;
+    /* of many rows, columns a workgroup: as many workgroups as three a CU (16-bit rows: four), so that they begin and end
+     * together */
+    const unsigned slots = es == 4 ? 768 : 1024, groups = (tiles + 3) / 4 < slots ? slots / ((tiles + 3) / 4) : 1;
     a.units = (int)((columns + groups - 1) / groups);
     hipStream_t s = stream_of(stream);
     by_type(ad->dtype, [&](auto t) {
