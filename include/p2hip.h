@@ -524,8 +524,9 @@ typedef struct P2hAdapters {
  * index lies outside [0, count) has no adapter: Y[m] = Z[m]. X [M][K], Z and Y [M][N] of the adapters' type, no alignment
  * beyond the element's (rows of X and K that are multiples of 16 bytes load several times faster). Products with A are
  * summed in 32 bits, that sum and its products with B are 32-bit too. Neighbouring rows of one adapter share what is read
- * of it, 16 at a time. At most 2^20 − 16 rows. The workspace is needed: p2h_adapters_workspace_bytes(...) bytes, 16-byte
- * aligned; calls sharing it are stream-ordered. Apart from Z and Y nothing overlaps. */
+ * of it, 16 or 64 at a time. At most 2^20 − 16 rows, K and N at most 2^23. The workspace is p2h_adapters_workspace_bytes(...) bytes,
+ * 16-byte aligned, NULL where that is 0 (few rows of small adapters); calls sharing it are stream-ordered. Apart from Z and Y
+ * nothing overlaps. */
 size_t p2h_adapters_workspace_bytes(const P2hAdapters *adapters, int M);
 int p2h_adapters_add(const P2hAdapters *adapters, int M, const void *dX, int ldx, const int *dIndex, const void *dZ,
                      int ldz, void *dY, int ldy, void *workspace, size_t workspace_bytes, void *stream);

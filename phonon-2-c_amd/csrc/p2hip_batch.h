@@ -1089,7 +1089,7 @@ __device__ __forceinline__ int shrink_rows(const AdapterArgs &a, const AdapterLi
         const E *am = static_cast<const E *>(a.a) + (size_t)ad * RANK * a.K;
         int k = k0 + STEP * part;
         if constexpr (VEC) {
-#pragma unroll 4
+#pragma unroll(RT <= 2 ? 8 : 4)
             for (; k + STEP <= k1; k += STEP * parts) {
                 const u4 xv = row_piece<DT, true>(x, k + VE * g, k1);
 #pragma unroll
@@ -1238,19 +1238,31 @@ template <int DT> struct ExpandRows {
     }
 };
 
+constexpr int kTileRowsLds = 8;
+
 /* … and Y = Z + Σ h · B of them, h this lane's RANK / 4 of row m0 + lane % 16 (times the adapter's scale), b its elements of B's
  * rows, in fp32 products (B's values are exact in fp32), rounded once. Rows that are not read 16 bytes at a time go through
  * the wave's LDS, so that lanes have neighbouring columns of one row. */
 template <int DT, int RANK>
 __device__ __forceinline__ void expand_rows(const AdapterArgs &a, uint32_t those, int m0, int n0, bool whole,
                                             const ExpandRows<DT> &rows, const float (&h)[RANK / 4],
-                                            const typename Elem<DT>::type (&b)[4][RANK / 4], float (*tile)[65])
+                                            const typename Elem<DT>::type (&b)[4][RANK / 4], float (*tile)[68])
 {
     typedef typename Elem<DT>::type E;
     constexpr int RS = RANK / 4, VE = kPer16<DT>, NV = 16 / VE;
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const E *z = static_cast<const E *>(a.z);
     E *y = static_cast<E *>(a.y);
+    E zs[kTileRowsLds];
+    auto load_z = [&](uint32_t left) __attribute__((always_inline)) {   /* of the next kTileRowsLds rows */
+#pragma unroll
+        for (int k = 0; k < kTileRowsLds; k++) {
+            zs[k] = Elem<DT>::put(0.0f);
+            if (left && z && n0 + lane < a.N) zs[k] = z[(size_t)(m0 + __builtin_ctz(left)) * a.ldz + n0 + lane];
+            left &= left - 1;
+        }
+    };
+    if (!whole) load_z(those);
     f4 acc[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) acc[t] = f4{0, 0, 0, 0};
@@ -1269,93 +1281,90 @@ __device__ __forceinline__ void expand_rows(const AdapterArgs &a, uint32_t those
             if ((those >> c) & 1) *reinterpret_cast<u4 *>(y + (size_t)(m0 + c) * a.ldy + n0 + 4 * VE * p + VE * g) = pack<DT>(v);
         }
     } else {
+        /* kTileRowsLds of these rows at a time */
+        const int place = __popc(those & ((1u << c) - 1)), count = __popc(those);
+        uint32_t left = those;
+        for (int done = 0; done < count; done += kTileRowsLds) {
+            if (((those >> c) & 1) && place >= done && place < done + kTileRowsLds)
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+                for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) tile[c][expand_column<DT>(t, 4 * g + i)] = acc[t][i];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (n0 + lane < a.N)
-            for (uint32_t left = those; left; left &= left - 1) {
-                const int r = __builtin_ctz(left);
-                const E before = z ? z[(size_t)(m0 + r) * a.ldz + n0 + lane] : Elem<DT>::put(0.0f);
-                y[(size_t)(m0 + r) * a.ldy + n0 + lane] = Elem<DT>::put(Elem<DT>::get(before) + tile[r][lane]);
-            }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+                    for (int i = 0; i < 4; i++) tile[place - done][expand_column<DT>(t, 4 * g + i)] = acc[t][i];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int k = 0; k < kTileRowsLds; k++)
+                if (done + k < count) {
+                    const int r = __builtin_ctz(left);
+                    left &= left - 1;
+                    if (n0 + lane < a.N)
+                        y[(size_t)(m0 + r) * a.ldy + n0 + lane] = Elem<DT>::put(Elem<DT>::get(zs[k]) + tile[k][lane]);
+                }
+            load_z(left);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 }
 
-/* Y[m][n] = Z[m][n] + scale · the sum over r of H[m][r] · B[adapter of m][n][r]: 16 · RT rows and 64 · U columns a workgroup, its
- * waves taking an adapter's 64 columns each. FUSED: H is made here, from all of K. */
-template <int DT, int RANK, int NW, int RT, int U, bool FUSED, bool VEC>
+/* Y[m][n] = Z[m][n] + scale · the sum over r of H[m][r] · B[adapter of m][n][r]: 16 rows and 64 columns a workgroup, a wave taking
+ * one of its adapters at a time. FUSED: H is made here, from all of K. */
+template <int DT, int RANK, int NW, bool FUSED, bool VEC>
 __global__ __launch_bounds__(64 * NW) void adapter_expand(AdapterArgs a)
 {
     typedef typename Elem<DT>::type E;
     constexpr int RS = RANK / 4;   /* a lane's elements of a row of rank: RS · g .. */
-    __shared__ float tile[NW][16][65];
+    __shared__ float tile[NW][kTileRowsLds][68];
     __shared__ AdapterList list;
     __shared__ float sum[FUSED ? NW : 1][16][RANK + 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
-    const int m0 = 16 * RT * blockIdx.y, rows = imin(16 * RT, a.M - m0);
+    const int m0 = 16 * blockIdx.y, rows = imin(16, a.M - m0), n0 = 64 * blockIdx.x;
     list_adapters(a, m0, rows, &list);
     int parts = a.parts;
     if constexpr (FUSED) parts = shrink_rows<DT, RANK, NW, VEC>(a, list, m0, rows, 0, a.K, sum);
     const int n = __builtin_amdgcn_readfirstlane(list.n);
-    for (int task = wave; task < n * U; task += NW) {
-        const int j = task / U, n0 = 64 * (blockIdx.x * U + task % U), ad = __builtin_amdgcn_readfirstlane(list.of[j]);
-        if (n0 >= a.N) continue;
-        const unsigned long long all = (unsigned long long)__builtin_amdgcn_readfirstlane((int)(list.rows[j] >> 32)) << 32 |
-                                       (uint32_t)__builtin_amdgcn_readfirstlane((int)list.rows[j]);
+    for (int j = wave; j < n; j += NW) {
+        const int ad = __builtin_amdgcn_readfirstlane(list.of[j]);
+        const uint32_t those = (uint32_t)__builtin_amdgcn_readfirstlane((int)list.rows[j]);
         if (ad < 0) {   /* no adapter: Z as it is */
             if (a.z == a.y && a.ldz == a.ldy) continue;
             for (int r = 0; r < rows; r++)
-                if (((all >> r) & 1) && n0 + lane < a.N)
+                if (((those >> r) & 1) && n0 + lane < a.N)
                     static_cast<E *>(a.y)[(size_t)(m0 + r) * a.ldy + n0 + lane] =
                         a.z ? static_cast<const E *>(a.z)[(size_t)(m0 + r) * a.ldz + n0 + lane] : Elem<DT>::put(0.0f);
             continue;
         }
+        /* everything that the rows need is requested before the first product */
         E b[4][RS];
 #pragma unroll
         for (int t = 0; t < 4; t++)
             __builtin_memcpy(b[t], static_cast<const E *>(a.b) +
                                        ((size_t)ad * a.N + imin(n0 + expand_column<DT>(t, c), a.N - 1)) * RANK + RS * g, sizeof b[t]);
         const float scale = a.scale[ad];
-        const bool whole = a.vec && n0 + 64 <= a.N;
-        /* everything that 16 · RT rows need is requested before the first product */
-        ExpandRows<DT> zr[RT];
-        float h[RT][RS];
+        const bool whole = a.vec && n0 + 64 <= a.N, in = (those >> c) & 1;
+        ExpandRows<DT> z;
+        if (whole) z.load(a, in, m0 + c, n0, g);
+        float h[RS];
 #pragma unroll
-        for (int q = 0; q < RT; q++) {
-            const bool in = (all >> (16 * q + c)) & 1;
-            if (whole) zr[q].load(a, in, m0 + 16 * q + c, n0, g);
+        for (int s = 0; s < RS; s++) h[s] = 0.0f;
+        if (in) {
+#pragma unroll(RS <= 4 ? 8 : RS <= 8 ? 4 : 1)
+            for (int p = 0; p < parts; p++) {
+                const float *from = FUSED ? &sum[FUSED ? p : 0][c][RS * g] : a.h + ((size_t)p * a.M + m0 + c) * RANK + RS * g;
 #pragma unroll
-            for (int s = 0; s < RS; s++) h[q][s] = 0.0f;
-            if (in) {
-#pragma unroll(RT > 1 ? 1 : RS <= 4 ? 8 : RS <= 8 ? 4 : 1)
-                for (int p = 0; p < parts; p++) {
-                    const float *from = FUSED ? &sum[FUSED ? p : 0][c][RS * g]
-                                              : a.h + ((size_t)p * a.M + m0 + 16 * q + c) * RANK + RS * g;
-#pragma unroll
-                    for (int s = 0; s < RS; s++) h[q][s] += from[s];
-                }
+                for (int s = 0; s < RS; s++) h[s] += from[s];
             }
         }
 #pragma unroll
-        for (int q = 0; q < RT; q++) {
-            const uint32_t those = (uint32_t)(all >> (16 * q)) & 0xffffu;
-            if (RT > 1 && !those) continue;
-#pragma unroll
-            for (int s = 0; s < RS; s++) h[q][s] *= scale;
-            expand_rows<DT, RANK>(a, those, m0 + 16 * q, n0, whole, zr[q], h[q], b, tile[wave]);
-        }
+        for (int s = 0; s < RS; s++) h[s] *= scale;
+        expand_rows<DT, RANK>(a, those, m0, n0, whole, z, h, b, tile[wave]);
     }
 }
 
-/* The same for many rows whose Z and Y are read and written 16 bytes at a time: 64 rows a workgroup, 16 a wave, its columns 64
- * at a time. Loads and stores go along rows: with lanes in different rows, as the products have them, a CU takes four times as
- * long for each. An adapter's 64 rows of B come through LDS, shared by the waves, and each wave's 16 rows of Z too, where the
- * sums are put in their place before they leave.
+/* The same for many rows: 64 rows a workgroup, 16 a wave, its columns 64 at a time. Loads and stores go along rows: with lanes in
+ * different rows, as the products have them, a CU takes four times as long for each. An adapter's 64 rows of B come through LDS,
+ * shared by the waves, and each wave's sums leave through it. VEC: Z and Y are read and written 16 bytes at a time, Z through
+ * LDS too; otherwise by the element.
  *
  * Everything comes by direct loads, a step (64 columns of one adapter) or a unit (64 columns) ahead, and is waited for by
  * number: the compiler's own waits, which do not know how many stores a path has issued, would wait for all of them. Such a
@@ -1364,7 +1373,11 @@ template <int DT, int RANK> struct ExpandLds {
     typedef typename Elem<DT>::type E;
     static constexpr int VE = kPer16<DT>, BCH = RANK / VE, ZCH = 64 / VE;   /* 16-byte pieces of a row of B, of 64 columns */
     static constexpr int NB = BCH < 4 ? 1 : BCH / 4, NZ = ZCH / 4;          /* a wave's loads of 64 rows of B, of 16 of Z */
-    E b[2][64 * RANK], z[2][4][16 * 64];
+    E b[2][64 * RANK];
+    union {
+        E z[2][4][16 * 64];
+        float sum[4][16 * 64];   /* VEC false: the sums alone */
+    };
     /* where a row's piece lies, so that 16 rows' pieces fall into different banks */
     template <int CH> static __device__ __forceinline__ int place(int r, int p)
     {
@@ -1372,12 +1385,13 @@ template <int DT, int RANK> struct ExpandLds {
     }
 };
 
-template <int DT, int RANK>
+template <int DT, int RANK, bool VEC>
 __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
 {
     typedef typename Elem<DT>::type E;
     typedef ExpandLds<DT, RANK> L;
-    constexpr int RS = RANK / 4, VE = L::VE, BCH = L::BCH, ZCH = L::ZCH, NB = L::NB, NZ = L::NZ, RPL = 64 / ZCH;
+    constexpr int RS = RANK / 4, VE = L::VE, BCH = L::BCH, ZCH = L::ZCH, NB = L::NB, RPL = 64 / ZCH,
+                  NZ = VEC ? L::NZ : 0;   /* loads of 16 rows of Z, and stores, that are counted */
     __shared__ __align__(16) L lds;
     __shared__ AdapterList list;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
@@ -1394,7 +1408,7 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
             dma_16(zp + (size_t)row * ldz + VE * imin(64 / VE * u + L::template place<ZCH>(r, zc), last_piece), lds.z[buffer][wave] + 512 / (8 / VE) * i);
         }
     };
-    fetch_z(u0, 0);   /* on its way while the adapters are looked up */
+    if (VEC) fetch_z(u0, 0);   /* on its way while the adapters are looked up */
     list_adapters(a, m0, rows, &list);
     const int n = __builtin_amdgcn_readfirstlane(list.n);
     auto adapter_of = [&](int j) { return __builtin_amdgcn_readfirstlane(list.of[j]); };
@@ -1431,6 +1445,16 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
         }
     };
     E *const y = static_cast<E *>(a.y) + (size_t)mw * a.ldy;
+    /* VEC false: a lane's column of 16 rows */
+    const E *const zrow = static_cast<const E *>(a.z) + (size_t)mw * a.ldz;
+    auto load_column = [&](int u, E (&z)[16]) __attribute__((always_inline)) {
+        const int col = 64 * u + lane;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            z[r] = Elem<DT>::put(0.0f);
+            if (a.z && r < have && col < a.N) z[r] = zrow[(size_t)r * a.ldz + col];
+        }
+    };
     const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
         y, 0, have > 0 ? (int)((uint32_t)((imin(have, 16) - 1) * a.ldy + a.N) * sizeof(E)) : 0, 0x00020000);
 
@@ -1438,6 +1462,8 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
     int buffer = 0, b_since = 0, z_since = 0;   /* how many are sure to have been issued since the next step's B, the unit's Z */
     for (int k = 0; k < units; k++) {
         const int u = u0 + k;
+        E zs[VEC ? 1 : 16];
+        if constexpr (!VEC) load_column(u, zs);
         f4 sum[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) sum[t] = f4{0, 0, 0, 0};
@@ -1446,7 +1472,7 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
             const uint32_t those = rows_of(j);
             /* the next step's B and, in a unit's first step, the next unit's Z; past the last the same again, which nothing reads */
             fetch_b(u0 + imin(k + end, units - 1), adapter_of(end ? 0 : j + 1), buffer ^ 1);
-            if (j == 0) fetch_z(u0 + imin(k + 1, units - 1), (k + 1) & 1);
+            if (VEC && j == 0) fetch_z(u0 + imin(k + 1, units - 1), (k + 1) & 1);
             b_since += NB + (j == 0 ? NZ : 0);
             z_since += NB + (j == 0 ? NZ : 0);
             if (b_since >= NB + 3 * NZ) wait_vm<NB + 3 * NZ>();
@@ -1485,6 +1511,24 @@ __global__ __launch_bounds__(256) void adapter_expand_rows(AdapterArgs a)
             }
             lds_barrier();   /* everyone is done with this step's B */
             buffer ^= 1;
+        }
+        if constexpr (!VEC) {
+            float *const own = lds.sum[wave];
+#pragma unroll
+            for (int t = 0; t < 4; t++)   /* columns expand_column(t, 4g) .. + 3: four neighbours */
+                *reinterpret_cast<f4 *>(own + 64 * c + 4 * L::template place<16>(c, expand_column<DT>(t, 4 * g) / 4)) = sum[t];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int col = 64 * u + lane;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float add = own[64 * r + 4 * L::template place<16>(r, lane / 4) + lane % 4];
+                if (r < have && col < a.N)
+                    y[(size_t)r * a.ldy + col] = (some >> r) & 1 ? Elem<DT>::put(Elem<DT>::get(zs[r]) + add) : zs[r];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            continue;
         }
         if (z_since >= NB + 2 * NZ) wait_vm<NB + 2 * NZ>();
         else wait_vm<NB + NZ>();

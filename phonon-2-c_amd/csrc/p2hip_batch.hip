@@ -309,15 +309,18 @@ static int check_adapters(const char *name, const P2hAdapters *ad, int M)
 /* Adapters that 16 rows may have between them, as the host knows it */
 static int adapters_of_16(const P2hAdapters *ad, int M) { return p2k::imin(p2k::imin(M, 16), p2k::imax(ad->count, 1)); }
 
-constexpr int kManyRows = 512;   /* above: 64 rows a workgroup */
+/* Above this many rows a workgroup of the second product takes 64 rows, not 16 (bf16, K = 4096, rank 16, shrink and expand:
+ * 300 rows with N = 16384 25 -> 16 us, N = 16389 37 -> 27; 128 rows of as many adapters 35 -> 42), above kManyShrink one of the
+ * first too (300 rows 4.9 -> 7.6 us). */
+constexpr int kManyRows = 256, kManyShrink = 512;
 
 /* K over workgroups, 0: everything in one launch, each workgroup making H for itself, while that is little to read. A number,
  * as the workspace's size is asked for where there may be no device. */
 static int adapter_parts(const P2hAdapters *ad, int M)
 {
-    const int n = adapters_of_16(ad, M), tiles = (M - 1) / (M > kManyRows ? 64 : 16) + 1;
+    const int n = adapters_of_16(ad, M), tiles = (M - 1) / (M > kManyShrink ? 64 : 16) + 1;
     if (M <= 16 && (size_t)n * ad->rank * ad->K * elem_size(ad->dtype) <= 128 << 10) return 0;
-    const int least = n <= 2 && M <= kManyRows ? 256 : 128, want = M > kManyRows ? 768 / tiles : (256 + tiles - 1) / tiles;
+    const int least = n <= 2 && M <= kManyShrink ? 256 : 128, want = M > kManyShrink ? 768 / tiles : (256 + tiles - 1) / tiles;
     return p2k::imax(p2k::imin(p2k::imin(want, 16), ad->K / least), 1);
 }
 
@@ -371,12 +374,13 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
     hipStream_t s = stream_of(stream);
     by_type(ad->dtype, [&](auto t) {
         auto go = [&](auto rank) {
-            constexpr int DT = decltype(t)::value, R = decltype(rank)::value, NS = R <= 32 ? 16 : 8;   /* waves that registers allow */
+            constexpr int DT = decltype(t)::value, R = decltype(rank)::value, NS = R <= 32 ? 16 : 8,   /* waves that registers allow */
+                          NF = R == 128 && DT == P2H_F32 ? 4 : 8;
             auto aligned_x = [&](auto v) {
                 constexpr bool V = decltype(v)::value != 0;
                 if (!a.parts)
-                    hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 8, 1, 1, true, V>), dim3(columns, tiles), dim3(512), 0, s, a);
-                else if (V && M > kManyRows)
+                    hipLaunchKernelGGL((p2k::adapter_expand<DT, R, NF, true, V>), dim3(columns, tiles), dim3(64 * NF), 0, s, a);
+                else if (V && M > kManyShrink)
                     hipLaunchKernelGGL((p2k::adapter_shrink_rows<DT, R>), dim3((tiles + 3) / 4, (unsigned)a.parts), dim3(256), 0, s, a);
                 else
                     hipLaunchKernelGGL((p2k::adapter_shrink<DT, R, NS, V>), dim3(tiles, (unsigned)a.parts), dim3(64 * NS), 0, s, a);
@@ -384,13 +388,15 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
             if (vec) aligned_x(ic<1>{});
             else aligned_x(ic<0>{});
             if (!a.parts) return;
-            if (M > kManyRows && a.vec && N >= 64 && ad->count > 0)
-                hipLaunchKernelGGL((p2k::adapter_expand_rows<DT, R>), dim3((columns + a.units - 1) / a.units, (tiles + 3) / 4), dim3(256),
-                                   0, s, a);
+            const dim3 many((columns + a.units - 1) / a.units, (tiles + 3) / 4);
+            if (M > kManyRows && ad->count > 0 && a.vec && N >= 64)
+                hipLaunchKernelGGL((p2k::adapter_expand_rows<DT, R, true>), many, dim3(256), 0, s, a);
+            else if (M > kManyRows && ad->count > 0)
+                hipLaunchKernelGGL((p2k::adapter_expand_rows<DT, R, false>), many, dim3(256), 0, s, a);
             else if (n > 4)
-                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, NS, 1, 1, false, true>), dim3(columns, tiles), dim3(64 * NS), 0, s, a);
+                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 8, false, true>), dim3(columns, tiles), dim3(512), 0, s, a);
             else
-                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 4, 1, 1, false, true>), dim3(columns, tiles), dim3(256), 0, s, a);
+                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 4, false, true>), dim3(columns, tiles), dim3(256), 0, s, a);
         };
         switch (ad->rank) {
         case 8: go(ic<8>{}); break;
