@@ -214,7 +214,10 @@ int p2h_kv_rows_q8(int dtype, const P2hKvCacheQ8 *cache, int rows, int n_seqs, c
     a.table_ld = table_ld; a.ldk = ldk; a.ldv = ldv;
     a.start = dStart; a.table = dTable; a.kc = (const int8_t *)c.K; a.vc = (const int8_t *)c.V; a.ks = c.ks; a.vs = c.vs;
     a.k = dK; a.v = dV;
-    a.per = p2k::imin(p2k::imax(rows / 2048, 1), p2k::kRowsMost);
+    /* Rows a workgroup: what a lane writes in one go (13 ragged sequences of up to 8191 tokens, 8 heads of 128, bf16: 84 us;
+     * twice that 90, four times 93), fewer for fewer rows, so that each CU has some. */
+    const int units = width * 2 / (int)(16 / es);
+    a.per = p2k::imax(p2k::imin(p2k::imin(256 * p2k::kRowUnits / units, rows / 1024), p2k::kRowsMost), 1);
     const unsigned grid = (unsigned)((rows - 1) / a.per + 1);
     if ((size_t)grid * 256 >= kGridThreads) return fail(P2H_E_ARG, "%s: %d rows are too many for one call", name, rows);
     hipStream_t s = stream_of(stream);
