@@ -46,9 +46,12 @@ Plan paged_plan(const CacheView &c, int n_seqs, int heads, int max_len, int wind
 {
     Plan p;
     p.q_groups = (heads / c.heads + 15) / 16;
-    /* a block of heads of 64 is little to wait for: four workgroups a CU (8 sequences of 32768: 41 us against 45) */
-    p.o_parts = parts_of((long long)n_seqs * c.heads * p.q_groups, left_of(max_len, window, sinks), 32,
-                         c.head_dim == 64 ? 1024 : 512);
+    const long long keys = left_of(max_len, window, sinks);
+    /* below 5 · 128 tokens a wave's few blocks cost no more than joining parts (one sequence, 8 heads of 128, fp32: 375 tokens
+     * 7.9 us against 9.8 and the second launch, 700 11.7 against 10.5); a block of heads of 64 is little to wait for: four workgroups a CU (8 sequences of 32768: 41 us
+     * against 45) */
+    if (keys >= 5 * 4 * 32)
+        p.o_parts = parts_of((long long)n_seqs * c.heads * p.q_groups, keys, 32, c.head_dim == 64 ? 1024 : 512);
     return p;
 }
 
