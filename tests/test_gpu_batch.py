@@ -461,7 +461,8 @@ ADAPTERS = [  # M, K, N, rank, adapters
     (1, 64, 16, 8, 1), (1, 1024, 1024, 8, 4), (5, 77, 143, 16, 3), (16, 129, 65, 32, 2), (17, 256, 300, 64, 20),
     (33, 1000, 515, 128, 5), (100, 136, 7, 16, 4), (13, 4096, 257, 16, 13), (70, 1, 1, 8, 2), (3, 8192, 40, 32, 2),
     (600, 72, 200, 8, 3), (515, 520, 136, 16, 5), (700, 264, 72, 32, 40), (530, 1160, 64, 64, 2), (577, 128, 328, 128, 3),
-    (513, 100, 131, 64, 4), (520, 136, 133, 32, 2), (514, 67, 64, 16, 2)]
+    (513, 100, 131, 64, 4), (520, 136, 133, 32, 2), (514, 67, 64, 16, 2), (300, 264, 515, 16, 3), (257, 1024, 3, 8, 2),
+    (290, 72, 200, 128, 5), (400, 130, 257, 64, 40), (256, 96, 64, 32, 3)]
 
 
 @pytest.mark.parametrize("t", D.TYPES)
@@ -605,6 +606,27 @@ def test_adapters_beyond_32_bits():
     ws = P.Workspace(P.adapters_workspace_bytes(ad, M))
     P.adapters_add_dev(ad, M, dx.ptr, K, di.ptr, dz.ptr, N, dy.ptr, N, ws.ptr, ws.nbytes)
     D.check(D.to_f64(t, dy.download((M, N), np.uint16)), want, bound)
+
+
+def test_adapters_rows_far_apart():
+    """Sixteen rows of Y that reach over 2^32 bytes, in place and from another Z."""
+    t, M, K, N, rank, ldy = "f32", 257, 64, 64, 8, 72_000_000
+    assert 15 * ldy * 4 > 1 << 32
+    rng = rng_of("far rows")
+    a, b, scale = B.adapter_set(rng, t, 3, rank, K, N)
+    x, z, index = D.rows(rng, t, M, K), D.rows(rng, t, M, N), rng.integers(-1, 3, M)
+    want, bound = B.adapters_want(t, x, index, a, b, scale, z)
+    dx, dz, da, db, ds = (D.device(v) for v in (x, z, a, b, scale))
+    di, dy = D.device(index.astype(np.int32)), P.DeviceBuffer(((M - 1) * ldy + N) * 4)
+    ad = P.Adapters(t, 3, rank, K, N, da.ptr, db.ptr, ds.ptr)
+    ws = P.Workspace(P.adapters_workspace_bytes(ad, M))
+    for in_place in (False, True):
+        for m in range(M):
+            dy.upload(z[m] if in_place else np.zeros(N, np.float32), offset=m * ldy * 4)
+        P.adapters_add_dev(ad, M, dx.ptr, K, di.ptr, dy.ptr if in_place else dz.ptr, ldy if in_place else N, dy.ptr, ldy, ws.ptr,
+                           ws.nbytes)
+        got = np.stack([dy.download(N, np.float32, offset=m * ldy * 4) for m in range(M)])
+        D.check(D.to_f64(t, got), want, bound, str(in_place))
 
 
 # ── together, streams and graphs ────────────────────────────────────────────────────────────────────────────────
