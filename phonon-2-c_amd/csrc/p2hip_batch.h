@@ -298,7 +298,10 @@ __device__ __forceinline__ void put_part(const BatchArgs &a, const BatchItem &w,
     }
 }
 
-/* An item of up to 16 rows over a cache of rows. */
+/* An item of up to 16 rows over a cache of rows: each wave takes blocks of 32 keys (fp32 16) in turn and has its own running
+ * reference, sum and outputs, joined at the end. Bound by waits in turn where there are few keys (4 sequences behind 375, 8 fp32
+ * heads of 128: 8.5 us), by memory where each sequence has many (64 with 1500 keys each, 32 heads on 8 of 128, bf16, 403 MB:
+ * about 75 us, 5.3 TB/s). */
 template <int DT, int DH, int NW>
 __device__ __forceinline__ void attend_rows(const BatchArgs &a, const BatchItem &w, unsigned char *lds)
 {
@@ -386,7 +389,12 @@ template <int DH, int NQ, int NW> constexpr int codes_lds()
  *
  * Nothing is lost but what is said here: fp32 queries and weights go in as three bf16 pieces that sum to them (queries down
  * to 2^-110), fp16 queries as they are and their weights as two pieces, 16 bits (as one of fp16, a weight times its scale would
- * leave the type's range), bf16 weights rounded to bf16. */
+ * leave the type's range), bf16 weights rounded to bf16.
+ *
+ * 32 sequences of up to 8192 tokens, 32 heads on 8 of 128, bf16, 375 MB: 79 us with the join, 4.8 TB/s, bound by memory (with the
+ * maximum of every block taken and masks as branches 87). Three sequences of 8 behind 30001 tokens each, heads of 64, fp16:
+ * 34 us, of which the floor of 104 MB is 20.6: a workgroup's 2 · 16 rows take products of 16 rows twice, the rest is the start
+ * and end of 512 workgroups. One sequence of 375, fp32: 7.9 us, waits in turn (length, page, codes, join). */
 template <int DT, int DH, int NQ, int NW>
 __device__ __forceinline__ void attend_codes(const BatchArgs &a, const BatchItem &w, unsigned char *lds)
 {
@@ -640,7 +648,11 @@ __device__ __forceinline__ int group_start(const BatchArgs &a, int g) { return i
  * As in windowed attention, S^T = K · Q^T by 32 × 32 products, so that a lane holds 32 keys of one row and its weights are laid
  * out as the operand of O^T += V^T · P^T; the scores of block b run together with the output product of block b − 1, in
  * stages of equal length, each stage's operands read from LDS two stages ahead and one of the next loads issued in each; the
- * reference of the exponentials is raised only where a block's sum of weights leaves the type's range. One barrier a block. */
+ * reference of the exponentials is raised only where a block's sum of weights leaves the type's range. One barrier a block.
+ *
+ * 64 sequences behind 32768 tokens, 32 heads on 8 of 128, bf16: 55 us without their own keys, 0.62 PFLOP/s; 72 with 512 of their
+ * own each, which start when tiles end. Eight waves a workgroup with four buffers, one a CU, took 83; tiles and own parts in
+ * turn 74, as a SIMD's two waves of tiles fill each other's gaps. */
 constexpr int kTileRows = 128;
 template <int DT> constexpr float kTileLift = DT == T_F16 ? 6.0f : 0.0f;          /* fp16 weights up to 2^6 below … */
 template <int DT> constexpr float kTileSlack = DT == T_F16 ? 65504.0f : 1024.0f;  /* … a sum that every type holds */
@@ -978,7 +990,9 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(BatchArgs a)
     }
 }
 
-/* The parts of one query added up by one wave, DH / 64 outputs a lane. */
+/* The parts of one query added up by one wave, DH / 64 outputs a lane: o = Σ 2^(top_i − top) num_i / Σ 2^(top_i − top) den_i. Bound by
+ * waits (2.6 us for 8 queries, 2 parts) or reading the parts, which the memory-side cache holds (64 · 32 queries of 33 parts, 35
+ * MB: 8 us). */
 template <int DT, int DH>
 __global__ __launch_bounds__(256) void attend_join(BatchArgs a)
 {
@@ -1020,6 +1034,11 @@ struct AdapterArgs {
     void *y;
     float *h;   /* [parts][M][rank] */
 };
+
+/* Y = Z + scale · (X · Aᵀ) · Bᵀ in two kernels, the sums of the first, H, in fp32 between them, or in one where all of A that a
+ * tile of rows needs is little. fp32 throughout where the type is; 16-bit rows multiply A in 16-bit products with fp32 sums,
+ * and H in fp32 products with B's values, which are exact in fp32, so that nothing is rounded before Y. Rows of one adapter among
+ * 16 (64) share what is read of it. */
 
 /* The adapters of a workgroup's rows (up to 64), each once, with its rows as bits, in the order of their first rows; rows
  * without one come as adapter −1. */
@@ -1129,7 +1148,8 @@ __device__ __forceinline__ int shrink_rows(const AdapterArgs &a, const AdapterLi
     return parts;
 }
 
-/* H[part][m][r] = the sum over the part's dimensions k of X[m][k] · A[adapter of m][r][k], 16 rows a workgroup. */
+/* H[part][m][r] = the sum over the part's dimensions k of X[m][k] · A[adapter of m][r][k], 16 rows a workgroup. Bound by the
+ * waits for A, which each adapter's wave has alone: 32 rows of 16 adapters, K = 4096, rank 16, bf16: 7.4 us. */
 template <int DT, int RANK, int NW, bool VEC>
 __global__ __launch_bounds__(64 * NW) void adapter_shrink(AdapterArgs a)
 {
@@ -1147,7 +1167,8 @@ __global__ __launch_bounds__(64 * NW) void adapter_shrink(AdapterArgs a)
 
 /* The same for many rows, 64 a workgroup, 16 a wave, whose X and A come through LDS 256 bytes of a row at a time, read along the
  * rows: read as operands, neighbouring lanes would be in different rows. Two stages in turn. Rows of X and A are 16-byte
- * aligned. */
+ * aligned. fp32, 6000 rows of 375 an adapter, K = 1024, rank 32: 15 us, X at 1.6 TB/s: a workgroup's rows take the two
+ * stages' waits in turn. */
 template <int RANK> constexpr int shrink_stage() { return (64 + RANK) * 256; }
 
 template <int DT, int RANK>
@@ -1322,7 +1343,9 @@ __device__ __forceinline__ void expand_rows(const AdapterArgs &a, uint32_t those
 }
 
 /* Y[m][n] = Z[m][n] + scale · the sum over r of H[m][r] · B[adapter of m][n][r]: 16 rows and 64 columns a workgroup, a wave taking
- * one of its adapters at a time. FUSED: H is made here, from all of K. */
+ * one of its adapters at a time. FUSED: H is made here, from all of K. Bound by waits in turn: one row, 1024 × 1024, rank 8,
+ * fused 4.2 us; 32 rows of 16 adapters, N = 16384, rank 16, bf16 7.6, N = 16389 12.4, as the 514 workgroups are two more than the
+ * CUs hold at once (with 80 registers three would fit a CU, which spills: 15). */
 template <int DT, int RANK, int NW, bool FUSED, bool VEC>
 __global__ __launch_bounds__(64 * NW) void adapter_expand(AdapterArgs a)
 {
@@ -1378,7 +1401,8 @@ __global__ __launch_bounds__(64 * NW) void adapter_expand(AdapterArgs a)
 /* The same for many rows: 64 rows a workgroup, 16 a wave, its columns 64 at a time. Loads and stores go along rows: with lanes in
  * different rows, as the products have them, a CU takes four times as long for each. An adapter's 64 rows of B come through LDS,
  * shared by the waves, and each wave's sums leave through it. VEC: Z and Y are read and written 16 bytes at a time, Z through
- * LDS too; otherwise by the element.
+ * LDS too; otherwise by the element. fp32, 6000 rows of 375 an adapter, N = 4096, rank 32: 48 us, 4.1 TB/s, bound by memory
+ * (67 with the compiler's waits and lanes in different rows; both products by 16 rows 246, by 64 66); bf16, 300 rows of 20 an adapter, N = 16384, rank 16: 16 us, N = 16389 27.
  *
  * Everything comes by direct loads, a step (64 columns of one adapter) or a unit (64 columns) ahead, and is waited for by
  * number: the compiler's own waits, which do not know how many stores a path has issued, would wait for all of them. Such a
