@@ -300,8 +300,8 @@ __device__ __forceinline__ void put_part(const BatchArgs &a, const BatchItem &w,
 
 /* An item of up to 16 rows over a cache of rows: each wave takes blocks of 32 keys (fp32 16) in turn and has its own running
  * reference, sum and outputs, joined at the end. Bound by waits in turn where there are few keys (4 sequences behind 375, 8 fp32
- * heads of 128: 8.5 us), by memory where each sequence has many (64 with 1500 keys each, 32 heads on 8 of 128, bf16, 403 MB:
- * about 75 us, 5.3 TB/s). */
+ * heads of 128: 8.5 us), by memory where each sequence has many (64 sequences of up to 2000 tokens, 32 heads on 8 of 128, bf16, 357 MB:
+ * 80 us, 4.5 TB/s). */
 template <int DT, int DH, int NW>
 __device__ __forceinline__ void attend_rows(const BatchArgs &a, const BatchItem &w, unsigned char *lds)
 {
