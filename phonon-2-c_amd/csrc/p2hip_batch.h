@@ -918,7 +918,7 @@ template <int TR> __device__ __forceinline__ bool prefix_item(const BatchArgs &a
     if (gr < 0) return false;
     const int sa = group_start(a, gr), sb = imax(group_start(a, gr + 1), sa);
     w->r0 = (tile - (sa * G / TR + gr)) * TR;
-    if (w->r0 >= (sb - sa) * G) return false;
+    if (w->r0 < 0 || w->r0 >= (sb - sa) * G) return false;   /* below 0 where starts descend */
     w->seq0 = sa;
     w->rows = imin(TR, (sb - sa) * G - w->r0);
     w->t0 = 0;

@@ -427,6 +427,21 @@ def test_shared_device_arrays_outside_their_ranges(kind, H):
     assert np.array_equal(a, b)
 
 
+@pytest.mark.parametrize("kind", ("rows", "q8"))
+@pytest.mark.parametrize("H", (4, 64))
+def test_shared_starts_that_descend(kind, H):
+    """Groups whose starts go up and down, several of them and more than a wave looks at at once, reach nothing outside the
+    buffers (what they mean is not defined), and a call behind one is right."""
+    t, Hk, page, Dh = "bf16", 2, 16, 64
+    rng, lens, starts, shared, table, pages, reach = shared_case(t, [(40, (41, 50, 77, 60, 43))], H, Hk, page, Dh, "down")
+    cache, K, V = shared_cache(rng, t, kind, pages, Hk, page, Dh, table, reach)
+    q = D.rows(rng, t, 5, H * Dh)
+    for st in ([5, 0, 5], [0, 5, 0, 5], [5, 5, 0, 1, 0, 5], [4, 0, 3, 1, 2], list(rng.integers(0, 6, 200))):
+        B.run_shared(t, q, cache, st, [40] * (len(st) - 1), table, lens, H, 0.1, EVERY, 0, 40, 60)
+    want, bound = B.paged_want(t, q, K, V, table, lens, H, 0.1, EVERY, 0, kind == "q8", starts, shared)
+    D.check(D.to_f64(t, B.run_shared(t, q, cache, starts, shared, table, lens, H, 0.1, EVERY, 0, 40, 60)), want, bound, kind)
+
+
 @pytest.mark.parametrize("t", D.TYPES)
 @pytest.mark.parametrize("kind", ("rows", "q8"))
 @pytest.mark.parametrize("H", (4, 48))
