@@ -1385,7 +1385,7 @@ __global__ __launch_bounds__(64 * NW) void adapter_expand(AdapterArgs a)
 #pragma unroll
         for (int s = 0; s < RS; s++) h[s] = 0.0f;
         if (in) {
-#pragma unroll(RS <= 4 ? 8 : RS <= 8 ? 4 : 1)
+#pragma unroll(RS <= 4 ? 8 : RS <= 8 ? 4 : DT != T_F32 ? 2 : 1)   /* what registers allow */
             for (int p = 0; p < parts; p++) {
                 const float *from = FUSED ? &sum[FUSED ? p : 0][c][RS * g] : a.h + ((size_t)p * a.M + m0 + c) * RANK + RS * g;
 #pragma unroll
