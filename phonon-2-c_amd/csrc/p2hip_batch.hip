@@ -63,6 +63,8 @@ Plan shared_plan(const CacheView &c, bool q8, int dtype, int n_seqs, int n_group
     const int G = heads / c.heads, kb = block_of(q8, dtype);
     p.q_groups = (G + 15) / 16;
     const int rows = n_groups ? (n_seqs * G + n_groups - 1) / n_groups : 0;   /* of a group, as the host knows them */
+    /* bf16 behind 32768 tokens, with the join: 40 rows 51 us by tiles, 53 by 16 rows, 64 rows 55 and 63, 32 rows 50 and 49. 8 bits,
+     * three groups behind 30001: 20 rows 35 us by 32, 36 by 16, 32 rows 36 and 42, 16 rows 35 and 26. */
     p.tiled = !q8 && dtype != P2H_F32 && rows > 32;
     p.nq = q8 && rows > 16 ? 2 : 1;
     const int tr = p.tiled ? p2k::kTileRows : 16 * p.nq;
@@ -321,12 +323,14 @@ static int adapters_of_16(const P2hAdapters *ad, int M) { return p2k::imin(p2k::
  * first too (300 rows 4.9 -> 7.6 us). */
 constexpr int kManyRows = 256, kManyShrink = 512;
 
-/* K over workgroups, 0: everything in one launch, each workgroup making H for itself, while that is little to read. A number,
- * as the workspace's size is asked for where there may be no device. */
+/* K over workgroups, 0: everything in one launch, each workgroup making H for itself, while that is little to read (one row,
+ * 16-bit, rank 8, K = 1024, 16 KB: 4.2 us against 2.6 + 3.4; 128 KB: 7.8 against 3.0 + 3.7, N = 16389 12.4 against 8). A part has
+ * at least 128 dimensions, 256 where a wave has few rows' adapters: the second product adds the parts (one row, rank 64, K =
+ * 2048: 3.2 + 9.1 us with 128, 4.0 + 6.9 with 256). A number, as the workspace's size is asked for where there may be no device. */
 static int adapter_parts(const P2hAdapters *ad, int M)
 {
     const int n = adapters_of_16(ad, M), tiles = (M - 1) / (M > kManyShrink ? 64 : 16) + 1;
-    if (M <= 16 && (size_t)n * ad->rank * ad->K * elem_size(ad->dtype) <= 128 << 10) return 0;
+    if (M <= 16 && (size_t)n * ad->rank * ad->K * elem_size(ad->dtype) <= 64 << 10) return 0;
     const int least = n <= 2 && M <= kManyShrink ? 256 : 128, want = M > kManyShrink ? 768 / tiles : (256 + tiles - 1) / tiles;
     return p2k::imax(p2k::imin(p2k::imin(want, 16), ad->K / least), 1);
 }
@@ -373,7 +377,6 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
     const bool vec = aligned(dX, 16) && (M == 1 || ldx * es % 16 == 0) && K * es % 16 == 0;
     a.vec = aligned(dY, 16) && (M == 1 || ldy * es % 16 == 0) && (!dZ || (aligned(dZ, 16) && (M == 1 || ldz * es % 16 == 0)));
     const unsigned tiles = (unsigned)((M + 15) / 16), columns = (unsigned)((N - 1) / 64 + 1);
-    const int n = adapters_of_16(ad, M);
     /* of many rows, columns a workgroup: as many workgroups as three a CU (16-bit rows: four), so that they begin and end
      * together */
     const unsigned slots = es == 4 ? 768 : 1024, groups = (tiles + 3) / 4 < slots ? slots / ((tiles + 3) / 4) : 1;
@@ -400,10 +403,8 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
                 hipLaunchKernelGGL((p2k::adapter_expand_rows<DT, R, true>), many, dim3(256), 0, s, a);
             else if (M > kManyRows && ad->count > 0)
                 hipLaunchKernelGGL((p2k::adapter_expand_rows<DT, R, false>), many, dim3(256), 0, s, a);
-            else if (n > 4)
-                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 8, false, true>), dim3(columns, tiles), dim3(512), 0, s, a);
             else
-                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 4, false, true>), dim3(columns, tiles), dim3(256), 0, s, a);
+                hipLaunchKernelGGL((p2k::adapter_expand<DT, R, 8, false, true>), dim3(columns, tiles), dim3(512), 0, s, a);
         };
         switch (ad->rank) {
         case 8: go(ic<8>{}); break;

@@ -477,7 +477,8 @@ ADAPTERS = [  # M, K, N, rank, adapters
     (33, 1000, 515, 128, 5), (100, 136, 7, 16, 4), (13, 4096, 257, 16, 13), (70, 1, 1, 8, 2), (3, 8192, 40, 32, 2),
     (600, 72, 200, 8, 3), (515, 520, 136, 16, 5), (700, 264, 72, 32, 40), (530, 1160, 64, 64, 2), (577, 128, 328, 128, 3),
     (513, 100, 131, 64, 4), (520, 136, 133, 32, 2), (514, 67, 64, 16, 2), (300, 264, 515, 16, 3), (257, 1024, 3, 8, 2),
-    (290, 72, 200, 128, 5), (400, 130, 257, 64, 40), (256, 96, 64, 32, 3)]
+    (290, 72, 200, 128, 5), (400, 130, 257, 64, 40), (256, 96, 64, 32, 3),
+    (4, 64, 130, 128, 1), (2, 100, 70, 64, 2), (1, 32, 9, 32, 1), (16, 40, 100, 16, 16)]
 
 
 @pytest.mark.parametrize("t", D.TYPES)
