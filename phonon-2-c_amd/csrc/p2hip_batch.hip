@@ -399,7 +399,7 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
             else aligned_x(ic<0>{});
             if (!a.parts) return;
             const dim3 many((columns + a.units - 1) / a.units, (tiles + 3) / 4);
-            if (M > kManyRows && ad->count > 0 && a.vec && N >= 64 && 16 * ldy * es < 1ull << 32)   /* its stores' offsets */
+            if (M > kManyRows && ad->count > 0 && a.vec && N >= 64 && p2k::sixteen_rows_in_32_bits(ldy, (int)es))   /* its stores' offsets */
                 hipLaunchKernelGGL((p2k::adapter_expand_rows<DT, R, true>), many, dim3(256), 0, s, a);
             else if (M > kManyRows && ad->count > 0)
                 hipLaunchKernelGGL((p2k::adapter_expand_rows<DT, R, false>), many, dim3(256), 0, s, a);

@@ -111,6 +111,10 @@ P2_HD bool rows_by_16(uintptr_t p, int pitch, int elem_size, int rows)
     return p % 16 == 0 && (rows == 1 || ((long long)pitch * elem_size % 16 == 0 && pitch < 1 << 25));
 }
 
+/* Whether 16 rows of that pitch (of elements) lie within 32-bit offsets from the first, the last 16 bytes of that range left over
+ * for an offset past every row's end. */
+P2_HD bool sixteen_rows_in_32_bits(int pitch, int elem_size) { return 16ll * pitch * elem_size <= (1ll << 32) - 16; }
+
 /* Whether a windowed call goes by 16 queries a workgroup, whose waves share the keys, or by tiles of 128 rows (16-bit rows:
  * of up to four query heads that read one key head). What counts is workgroups: those of 16 queries, by the mean length of
  * the sequences, which with their number is all that the host knows of them.

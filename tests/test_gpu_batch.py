@@ -848,3 +848,22 @@ def test_two_graphs_share_a_workspace(t):
             s.sync()
             assert np.array_equal(do.download((len(lens), H * Dh), D.np_type(t)).view(np.uint16),
                                   alone(ln).view(np.uint16)), turn
+
+
+def test_adapters_rows_very_far_apart():
+    """Rows of Y so far apart that the size of sixteen, taken in 32 bits, is 0."""
+    t, M, K, N, rank, ldy = "bf16", 257, 64, 64, 8, 1 << 28
+    assert (16 * ldy) % (1 << 32) == 0
+    rng = rng_of("very far rows")
+    a, b, scale = B.adapter_set(rng, t, 3, rank, K, N)
+    x, z, index = D.rows(rng, t, M, K), D.rows(rng, t, M, N), rng.integers(-1, 3, M)
+    want, bound = B.adapters_want(t, x, index, a, b, scale, z)
+    dx, dz, da, db, ds = (D.device(v) for v in (x, z, a, b, scale))
+    di, dy = D.device(index.astype(np.int32)), P.DeviceBuffer(((M - 1) * ldy + N) * 2)
+    ad = P.Adapters(t, 3, rank, K, N, da.ptr, db.ptr, ds.ptr)
+    ws = P.Workspace(P.adapters_workspace_bytes(ad, M))
+    for m in range(M):
+        dy.upload(np.full(N, 0xFFFF, np.uint16), offset=m * ldy * 2)
+    P.adapters_add_dev(ad, M, dx.ptr, K, di.ptr, dz.ptr, N, dy.ptr, ldy, ws.ptr, ws.nbytes)
+    got = np.stack([dy.download(N, np.uint16, offset=m * ldy * 2) for m in range(M)])
+    D.check(D.to_f64(t, got), want, bound)
