@@ -493,6 +493,7 @@ int p2h_attention_paged_q8(int dtype, const P2hKvCacheQ8 *cache, int n_seqs, int
  * dShared[g] tokens, which are found through the table row of the group's first sequence; behind them each sequence has its
  * own row's. Lengths dLen count from the first token, prefix included; one that ends inside the prefix sees that much of it.
  * dShared may be 0, end inside a page, and lie beyond a length. The outputs of sequences of no group are left as they were.
+ * At most 65536 groups; n_seqs · heads below 2^23 and n_groups times the cache's heads below 2^23 − 2^19 are never too many.
  * max_shared and max_own plan the work: the longest prefix and the most tokens that a sequence has behind one; other
  * numbers are right as well. The workspace is needed: p2h_attention_shared_workspace_bytes(...) bytes, 16-byte aligned;
  * calls sharing it are stream-ordered. dO and the workspace overlap nothing the call reads, nor each other. */

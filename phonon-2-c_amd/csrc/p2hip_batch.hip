@@ -20,6 +20,8 @@ struct Plan {
     bool tiled = false;   /* prefixes by tiles of p2k::kTileRows rows */
     int nq = 1;           /* else by 16 · nq */
     int parts() const { return p_parts + o_parts; }
+    size_t prefix_workgroups(int kv) const { return (size_t)p_tiles * p_parts * kv; }
+    size_t workgroups(int n_seqs, int kv) const { return prefix_workgroups(kv) + (size_t)n_seqs * q_groups * o_parts * kv; }
     size_t bytes(int n_seqs, int heads, int head_dim) const
     {
         return (size_t)n_seqs * heads * parts() * (head_dim + 2) * 4;   /* sums, reference, sum of weights */
@@ -83,6 +85,21 @@ int check_seqs(const char *name, int dtype, const CacheView &c, int n_seqs, int 
     return P2H_OK;
 }
 
+/* before a plan is made: what its numbers of rows and workgroups stay within 32 bits for */
+int check_batch(const char *name, int n_seqs, int heads)
+{
+    return (size_t)n_seqs * heads >= 1u << 23
+               ? fail(P2H_E_ARG, "%s: %d sequences of %d heads are too many for one call", name, n_seqs, heads)
+               : P2H_OK;
+}
+
+int check_plan(const char *name, const Plan &plan, const CacheView &c, int n_seqs, int n_groups, int heads)
+{
+    return plan.workgroups(n_seqs, c.heads) * 64 * kWaves >= kGridThreads
+               ? fail(P2H_E_ARG, "%s: %d sequences of %d heads in %d groups are too many for one call", name, n_seqs, heads, n_groups)
+               : P2H_OK;
+}
+
 int check_tokens(const char *name, int n)
 {
     return n < 0 || n > (1 << 30) ? fail(P2H_E_ARG, "%s: up to %d tokens (0 .. 2^30)", name, n) : P2H_OK;
@@ -90,7 +107,7 @@ int check_tokens(const char *name, int n)
 
 Rows ints(const int *p, int ld, int n) { return Rows{(const char *)p, (size_t)ld * 4, (size_t)ld * 4, ld > 0 && p ? n : 0}; }
 
-/* Attention over a cache of either kind; `group` NULL without prefixes. */
+/* Attention over a cache of either kind, its plan checked; `group` NULL without prefixes. */
 int attention(const char *name, int dtype, const CacheView &c, bool q8, const Plan &plan, int n_seqs, int n_groups, int heads,
               const void *dQ, int ldq, const int *dGroup, const int *dShared, const int *dTable, int table_ld,
               const int *dLen, float scale, int window, int sinks, void *dO, int ldo, void *workspace,
@@ -120,15 +137,11 @@ int attention(const char *name, int dtype, const CacheView &c, bool q8, const Pl
     if (overlap(o, ints(dLen, 1, n_seqs)) || overlap(o, ints(dTable, table_ld, n_seqs)) ||
         overlap(o, ints(dGroup, 1, n_groups + 1)) || overlap(o, ints(dShared, 1, n_groups)))
         return fail(P2H_E_ARG, "%s: dO overlaps lengths, pages or groups", name);
-    const size_t p_wgs = (size_t)plan.p_tiles * plan.p_parts * c.heads;
-    const size_t o_wgs = (size_t)n_seqs * plan.q_groups * plan.o_parts * c.heads, wgs = p_wgs + o_wgs;
-    if (wgs * 64 * kWaves >= kGridThreads || (size_t)n_seqs * heads >= 1u << 23)
-        return fail(P2H_E_ARG, "%s: %d sequences of %d heads are too many for one call", name, n_seqs, heads);
     if (int rc = ensure_init()) return rc;
     p2k::BatchArgs a{};
     a.n_seqs = n_seqs; a.n_groups = n_groups; a.heads = heads; a.kv = c.heads; a.page_shift = log2_of(c.page);
     a.pages = c.pages; a.table_ld = table_ld; a.ldq = ldq; a.ldo = ldo; a.window = window; a.sinks = sinks;
-    a.p_tiles = plan.p_tiles; a.p_parts = plan.p_parts; a.p_wgs = (int)p_wgs;
+    a.p_tiles = plan.p_tiles; a.p_parts = plan.p_parts; a.p_wgs = (int)plan.prefix_workgroups(c.heads);
     a.q_groups = plan.q_groups; a.o_parts = plan.o_parts; a.c = scale * p2k::kLog2e;
     a.q = dQ; a.kc = c.K; a.vc = c.V; a.ks = c.ks; a.vs = c.vs;
     a.table = dTable; a.len = dLen; a.group = dGroup; a.shared = dShared; a.o = dO;
@@ -137,7 +150,7 @@ int attention(const char *name, int dtype, const CacheView &c, bool q8, const Pl
     hipStream_t s = stream_of(stream);
     by_type_dim(dtype, c.head_dim, [&](auto t, auto d) {
         constexpr int DT = decltype(t)::value, DH = decltype(d)::value;
-        const dim3 grid((unsigned)wgs), threads(64 * kWaves);
+        const dim3 grid((unsigned)plan.workgroups(n_seqs, c.heads)), threads(64 * kWaves);
         if (q8) {
             if (plan.nq == 2) hipLaunchKernelGGL((p2k::attend<p2k::C_Q8, DT, DH, 2, kWaves>), grid, threads, 0, s, a);
             else hipLaunchKernelGGL((p2k::attend<p2k::C_Q8, DT, DH, 1, kWaves>), grid, threads, 0, s, a);
@@ -159,15 +172,15 @@ size_t shared_bytes(const char *name, const P2hKvCache *rows, const P2hKvCacheQ8
     if (rows ? check_cache(name, rows) : check_cache(name, q8)) return 0;
     const CacheView c(rows, q8);
     const int dtype = rows ? rows->dtype : P2H_BF16;
-    if (check_seqs(name, dtype, c, n_seqs, heads, 0) || check_scale(name, 1.0f, window, 0, sinks) ||
-        check_tokens(name, max_shared) || check_tokens(name, max_own))
+    if (check_seqs(name, dtype, c, n_seqs, heads, 0) || check_batch(name, n_seqs, heads) ||
+        check_scale(name, 1.0f, window, 0, sinks) || check_tokens(name, max_shared) || check_tokens(name, max_own))
         return 0;
     if (n_groups < 0 || n_groups > 65536) {
         fail(P2H_E_ARG, "%s: %d groups (at most 65536)", name, n_groups);
         return 0;
     }
-    return shared_plan(c, q8 != nullptr, dtype, n_seqs, n_groups, heads, max_shared, max_own, window, sinks)
-        .bytes(n_seqs, heads, c.head_dim);
+    const Plan plan = shared_plan(c, q8 != nullptr, dtype, n_seqs, n_groups, heads, max_shared, max_own, window, sinks);
+    return check_plan(name, plan, c, n_seqs, n_groups, heads) ? 0 : plan.bytes(n_seqs, heads, c.head_dim);
 }
 
 int shared(const char *name, int dtype, const P2hKvCache *rows, const P2hKvCacheQ8 *q8, int n_seqs, int n_groups, int heads,
@@ -178,6 +191,7 @@ int shared(const char *name, int dtype, const P2hKvCache *rows, const P2hKvCache
     if (int rc = rows ? check_cache(name, rows) : check_cache(name, q8)) return rc;
     const CacheView c(rows, q8);
     if (int rc = check_seqs(name, dtype, c, n_seqs, heads, table_ld)) return rc;
+    if (int rc = check_batch(name, n_seqs, heads)) return rc;
     if (int rc = check_scale(name, scale, window, 0, sinks)) return rc;
     if (int rc = check_tokens(name, max_shared)) return rc;
     if (int rc = check_tokens(name, max_own)) return rc;
@@ -185,6 +199,7 @@ int shared(const char *name, int dtype, const P2hKvCache *rows, const P2hKvCache
     if (n_seqs == 0 || n_groups == 0) return P2H_OK;
     if (!dGroup || !dShared) return fail(P2H_E_ARG, "%s: NULL groups or prefixes", name);
     const Plan plan = shared_plan(c, q8 != nullptr, dtype, n_seqs, n_groups, heads, max_shared, max_own, window, sinks);
+    if (int rc = check_plan(name, plan, c, n_seqs, n_groups, heads)) return rc;
     return attention(name, dtype, c, q8 != nullptr, plan, n_seqs, n_groups, heads, dQ, ldq, dGroup, dShared, dTable, table_ld,
                      dLen, scale, window, sinks, dO, ldo, workspace, workspace_bytes, stream);
 }
@@ -240,11 +255,11 @@ size_t p2h_attention_paged_q8_workspace_bytes(const P2hKvCacheQ8 *cache, int n_s
     const char *name = "p2h_attention_paged_q8_workspace_bytes";
     if (check_cache(name, cache)) return 0;
     const CacheView c(nullptr, cache);
-    if (check_seqs(name, P2H_BF16, c, n_seqs, heads, 0) || check_scale(name, 1.0f, window, 0, sinks) ||
-        check_tokens(name, max_len))
+    if (check_seqs(name, P2H_BF16, c, n_seqs, heads, 0) || check_batch(name, n_seqs, heads) ||
+        check_scale(name, 1.0f, window, 0, sinks) || check_tokens(name, max_len))
         return 0;
     const Plan p = paged_plan(c, n_seqs, heads, max_len, window, sinks);
-    return p.parts() > 1 ? p.bytes(n_seqs, heads, c.head_dim) : 0;
+    return p.parts() > 1 && !check_plan(name, p, c, n_seqs, 0, heads) ? p.bytes(n_seqs, heads, c.head_dim) : 0;
 }
 
 int p2h_attention_paged_q8(int dtype, const P2hKvCacheQ8 *cache, int n_seqs, int heads, const void *dQ, int ldq,
@@ -255,11 +270,13 @@ int p2h_attention_paged_q8(int dtype, const P2hKvCacheQ8 *cache, int n_seqs, int
     if (int rc = check_cache(name, cache)) return rc;
     const CacheView c(nullptr, cache);
     if (int rc = check_seqs(name, dtype, c, n_seqs, heads, table_ld)) return rc;
+    if (int rc = check_batch(name, n_seqs, heads)) return rc;
     if (int rc = check_scale(name, scale, window, 0, sinks)) return rc;
     if (int rc = check_tokens(name, max_len)) return rc;
     if (n_seqs == 0) return P2H_OK;
     Plan plan = paged_plan(c, n_seqs, heads, max_len, window, sinks);
     if (!workspace) plan.o_parts = 1;
+    if (int rc = check_plan(name, plan, c, n_seqs, 0, heads)) return rc;
     return attention(name, dtype, c, true, plan, n_seqs, 0, heads, dQ, ldq, nullptr, nullptr, dTable, table_ld, dLen, scale,
                      window, sinks, dO, ldo, workspace, workspace_bytes, stream);
 }

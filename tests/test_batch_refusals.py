@@ -223,3 +223,29 @@ def test_too_many_for_one_launch():
     far = q8(dK=1 << 50, dV=1 << 51, dKScale=1 << 52, dVScale=1 << 53)
     refused(paged(far, n=65536, heads=256, q=1 << 45, ldq=16384, o=1 << 47, ldo=16384), "too many")
     refused(shared("q8", far, n=65536, heads=128, q=1 << 45, ldq=8192, o=1 << 47, ldo=8192, ws=1 << 48, wsb=1 << 47), "too many")
+
+
+@pytest.mark.parametrize("n,heads,kv,groups", ((65536, 65536, 1, 1), (65536, 65536, 65536, 1), (32768, 65536, 1, 7), (65536, 128, 2, 1),
+                                               (1, 256, 256, 65536)))
+def test_too_many_for_a_workspace_too(n, heads, kv, groups):
+    """What a call refuses has no workspace, also where the products of its numbers pass 32 bits."""
+    far = q8(heads=kv, dK=1 << 50, dV=1 << 51, dKScale=1 << 52, dVScale=1 << 53)
+    apart = row_cache(heads=kv, dK=1 << 50, dV=1 << 51)
+    assert P.attention_shared_q8_workspace_bytes(far, n, groups, heads, 100, 100) == 0 and "too many" in P.last_error()
+    assert P.attention_shared_workspace_bytes(apart, n, groups, heads, 100, 100) == 0 and "too many" in P.last_error()
+    ld = heads * 64
+    for kind, c in (("q8", far), ("rows", apart)):
+        refused(shared(kind, c, n=n, g=groups, heads=heads, q=1 << 45, ldq=ld, o=1 << 47, ldo=ld, ws=1 << 48, wsb=1 << 47), "too many")
+    if groups == 1:
+        assert P.attention_paged_q8_workspace_bytes(far, n, heads, 100000) == 0 and "too many" in P.last_error()
+
+
+def test_as_many_as_there_may_be():
+    """The most that is never too many: 2^23 - 1 rows of queries, and groups times key heads below 2^23 - 2^19."""
+    one = q8(heads=1, dK=1 << 50, dV=1 << 51, dKScale=1 << 52, dVScale=1 << 53)
+    many = q8(heads=120, dK=1 << 50, dV=1 << 51, dKScale=1 << 52, dVScale=1 << 53)
+    assert 65535 * 120 < (1 << 23) - (1 << 19) < 65535 * 121
+    assert P.attention_shared_q8_workspace_bytes(many, 65535, 65535, 120, 100, 100) > 0
+    assert P.attention_shared_q8_workspace_bytes(one, 65535, 65535, 128, 100, 100) > 0
+    assert P.attention_shared_q8_workspace_bytes(one, 65535, 1, 128, FAR, FAR) > 0
+    assert P.attention_shared_workspace_bytes(row_cache(heads=120, dK=1 << 50, dV=1 << 51), 65535, 65535, 120, 100, 100) > 0
