@@ -52,7 +52,7 @@ struct KvRowsArgs {
 constexpr int kRowsMost = 32;   /* rows a workgroup at most */
 constexpr int kRowUnits = 4;    /* units of 16 output bytes of a lane, all read before the first is written */
 
-/* k = code · scale, rounded once. Rows `per` · blockIdx.x ..: where each row's token lies is looked up first, one thread a row;
+/* k = code · scale, rounded once. Rows `per` times the workgroup's number ..: where each row's token lies is looked up first, one thread a row;
  * then 16 bytes of output a lane along the rows, K's heads and V's. A unit's row and its place there are carried on: a division
  * for each cost as much as the rest. Bound by memory: 13 ragged sequences of up to 8191 tokens, 8 heads of 128, to bf16, 458 MB:
  * 84 us, 5.4 TB/s (ordinary stores 93; a grid of 2048 with its rows in loops 113). */
@@ -62,7 +62,8 @@ __global__ __launch_bounds__(256) void kv_rows_q8(KvRowsArgs a)
     typedef typename Elem<DT>::type E;
     constexpr int VE = kPer16<DT>, LPH = DH / VE;
     __shared__ long long at[kRowsMost];   /* (page · kv << page_shift) + place; −1: no such token; −2: no sequence's row */
-    const int r0 = blockIdx.x * a.per, n = imin(a.per, a.rows - r0);
+    const int r0 = (int)(blockIdx.y * gridDim.x + blockIdx.x) * a.per, n = imin(a.per, a.rows - r0);
+    if (n <= 0) return;   /* of the last of several rows of workgroups */
     if (threadIdx.x < 64) {
         auto begins = [&](int s) { return imin(imax(a.start[s], 0), a.rows); };
         const int first = wave_last(a.n_seqs, [&](int s) { return begins(s) <= r0; });

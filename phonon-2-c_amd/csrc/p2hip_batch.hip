@@ -239,11 +239,11 @@ int p2h_kv_rows_q8(int dtype, const P2hKvCacheQ8 *cache, int rows, int n_seqs, c
      * twice that 90, four times 93), fewer for fewer rows, so that each CU has some. */
     const int units = width * 2 / (int)(16 / es);
     a.per = p2k::imax(p2k::imin(p2k::imin(256 * p2k::kRowUnits / units, rows / 1024), p2k::kRowsMost), 1);
-    const unsigned grid = (unsigned)((rows - 1) / a.per + 1);
-    if ((size_t)grid * 256 >= kGridThreads) return fail(P2H_E_ARG, "%s: %d rows are too many for one call", name, rows);
+    const unsigned wgs = (unsigned)((rows - 1) / a.per + 1), across = wgs < 1u << 23 ? wgs : 1u << 23;
+    const dim3 grid(across, (wgs - 1) / across + 1);
     hipStream_t s = stream_of(stream);
     by_type_dim(dtype, c.head_dim, [&](auto t, auto d) {
-        hipLaunchKernelGGL((p2k::kv_rows_q8<decltype(t)::value, decltype(d)::value>), dim3(grid), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((p2k::kv_rows_q8<decltype(t)::value, decltype(d)::value>), grid, dim3(256), 0, s, a);
     });
     HIPCHK(hipGetLastError());
     return P2H_OK;

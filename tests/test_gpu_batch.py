@@ -867,3 +867,34 @@ def test_adapters_rows_very_far_apart():
     P.adapters_add_dev(ad, M, dx.ptr, K, di.ptr, dz.ptr, N, dy.ptr, ldy, ws.ptr, ws.nbytes)
     got = np.stack([dy.download(N, np.uint16, offset=m * ldy * 2) for m in range(M)])
     D.check(D.to_f64(t, got), want, bound)
+
+
+def test_rows_q8_more_workgroups_than_a_grid_is_wide():
+    """2^29 rows and some, 137 GB of keys and values: tokens of three pages, again and again."""
+    t, Hk, Dh, page, rows = "bf16", 1, 64, 1024, (1 << 29) + 5000
+    rng = rng_of("many rows")
+    kept = B.Kept.random(rng, 3, Hk, page, Dh)
+    starts = np.array([0, 5, rows - 2000, rows - 7], np.int32)
+    table = rng.integers(0, 3, (3, (1 << 19) + 8)).astype(np.int32)
+    table[1, 700] = -1
+    dk, dv = (P.DeviceBuffer(rows * Dh * 2) for _ in range(2))
+    ds, dt = D.device(starts), D.device(table)
+    some = np.unique(np.concatenate((np.arange(5, 3000), 700 * page + 5 + np.arange(-3, page + 3), rng.integers(5, rows, 300),
+                                     (1 << 28) + np.arange(-40, 40), (1 << 29) + np.arange(-40, 40), rows - np.arange(2100, 1, -1))))
+    behind = np.full((7, Dh), 0xFFFF, np.uint16)
+    for d in (dk, dv):
+        d.upload(behind, offset=(rows - 7) * Dh * 2)
+    P.kv_rows_q8_dev(t, kept.c, rows, 3, ds.ptr, dt.ptr, table.shape[1], dk.ptr, Dh, dv.ptr, Dh)
+    runs = np.split(some, np.nonzero(np.diff(some) > 1)[0] + 1)
+    for d, c, sc in ((dk, kept.kc, kept.ks), (dv, kept.vc, kept.vs)):
+        values = D.to_type(t, c[:, 0].astype(np.float32) * sc[:, 0, :, None])   # [page][place][Dh]
+        assert np.array_equal(d.download((7, Dh), np.uint16, offset=(rows - 7) * Dh * 2), behind)
+        for run in runs:
+            run = run[run < rows - 7]
+            if run.size == 0:
+                continue
+            s = np.searchsorted(starts, run, side="right") - 1
+            at = run - starts[s]
+            p = table[s, at // page]
+            want = np.where((p >= 0)[:, None], values[np.maximum(p, 0), at % page], 0)
+            assert np.array_equal(d.download((run.size, Dh), np.uint16, offset=int(run[0]) * Dh * 2), want), run[0]
