@@ -105,6 +105,9 @@ int check_tokens(const char *name, int n)
     return n < 0 || n > (1 << 30) ? fail(P2H_E_ARG, "%s: up to %d tokens (0 .. 2^30)", name, n) : P2H_OK;
 }
 
+/* whether arrays of words are aligned: the scalar cache reads the aligned word that an address lies in */
+template <class... P> bool words(const P *...p) { return (aligned(p, 4) && ...); }
+
 Rows ints(const int *p, int ld, int n) { return Rows{(const char *)p, (size_t)ld * 4, (size_t)ld * 4, ld > 0 && p ? n : 0}; }
 
 /* Attention over a cache of either kind, its plan checked; `group` NULL without prefixes. */
@@ -116,6 +119,8 @@ int attention(const char *name, int dtype, const CacheView &c, bool q8, const Pl
     if (int rc = check_rows(name, "dQ", dtype, dQ, ldq, heads * c.head_dim)) return rc;
     if (int rc = check_rows(name, "dO", dtype, dO, ldo, heads * c.head_dim)) return rc;
     if (!dLen || (table_ld > 0 && !dTable)) return fail(P2H_E_ARG, "%s: NULL lengths or page table", name);
+    if (!words(dLen, dTable, dGroup, dShared))
+        return fail(P2H_E_ARG, "%s: lengths, pages or groups are not 4-byte aligned", name);
     const size_t es = elem_size(dtype), width = (size_t)heads * c.head_dim * es;
     const Rows q{(const char *)dQ, ldq * es, width, n_seqs}, o{(const char *)dO, ldo * es, width, n_seqs};
     if (overlap(o, q)) return fail(P2H_E_ARG, "%s: dO overlaps dQ", name);
@@ -223,6 +228,7 @@ int p2h_kv_rows_q8(int dtype, const P2hKvCacheQ8 *cache, int rows, int n_seqs, c
     if (int rc = check_rows(name, "dK", dtype, dK, ldk, width)) return rc;
     if (int rc = check_rows(name, "dV", dtype, dV, ldv, width)) return rc;
     if (!dStart || (table_ld > 0 && !dTable)) return fail(P2H_E_ARG, "%s: NULL starts or page table", name);
+    if (!words(dStart, dTable)) return fail(P2H_E_ARG, "%s: starts or pages are not 4-byte aligned", name);
     const size_t es = elem_size(dtype);
     const Rows k{(const char *)dK, ldk * es, width * es, rows}, v{(const char *)dV, ldv * es, width * es, rows};
     if (overlap(k, v)) return fail(P2H_E_ARG, "%s: dK and dV overlap", name);
@@ -369,9 +375,9 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
     if (!dX || !dY || ldx < K || ldy < N || (dZ && ldz < N) || !aligned(dX, es) || !aligned(dY, es) || !aligned(dZ, es))
         return fail(P2H_E_ARG, "%s: NULL or unaligned rows, or ldx = %d < K = %d, ldz = %d or ldy = %d < N = %d", name, ldx, K,
                     ldz, ldy, N);
-    if (!dIndex) return fail(P2H_E_ARG, "%s: NULL index", name);
-    if (ad->count > 0 && (!ad->A || !ad->B || !ad->scale || !aligned(ad->A, 16) || !aligned(ad->B, 16)))
-        return fail(P2H_E_ARG, "%s: adapters are NULL or not 16-byte aligned", name);
+    if (!dIndex || !words(dIndex)) return fail(P2H_E_ARG, "%s: NULL index, or not 4-byte aligned", name);
+    if (ad->count > 0 && (!ad->A || !ad->B || !ad->scale || !aligned(ad->A, 16) || !aligned(ad->B, 16) || !words(ad->scale)))
+        return fail(P2H_E_ARG, "%s: adapters are NULL or not 16-byte aligned (scales 4-byte)", name);
     const size_t need = p2h_adapters_workspace_bytes(ad, M);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return fail(P2H_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", name, workspace_bytes, need);

@@ -249,3 +249,16 @@ def test_as_many_as_there_may_be():
     assert P.attention_shared_q8_workspace_bytes(one, 65535, 65535, 128, 100, 100) > 0
     assert P.attention_shared_q8_workspace_bytes(one, 65535, 1, 128, FAR, FAR) > 0
     assert P.attention_shared_workspace_bytes(row_cache(heads=120, dK=1 << 50, dV=1 << 51), 65535, 65535, 120, 100, 100) > 0
+
+
+@pytest.mark.parametrize("off", (1, 2, 3))
+def test_arrays_of_words_that_are_not_aligned(off):
+    for name in ("start", "table"):
+        refused(rows(**{name: 5 * A + off}), "4-byte")
+    for name in ("lens", "table"):
+        refused(paged(**{name: 30 * A + off}), "4-byte")
+    for kind in ("rows", "q8"):
+        for name in ("lens", "table", "group", "shared"):
+            refused(shared(kind, **{name: 34 * A + off}), "4-byte")
+    refused(add(index=43 * A + off), "4-byte")
+    refused(add(adapters(dScale=42 * A + off)), "4-byte")
