@@ -481,7 +481,7 @@ int p2h_kv_rows_q8(int dtype, const P2hKvCacheQ8 *cache, int rows, int n_seqs, c
 
 /* p2h_attention_paged over an 8-bit cache, queries and outputs of type `dtype`: o = Σ w · scale_v · code_v / Σ w, w the softmax
  * weights of scale · scale_k · (q · code_k). Codes are exact in the products; a weight times its value's scale is rounded to
- * 8 bits for bf16 rows, to 16 for fp16 rows, and not at all for fp32 rows, whose queries of less than 2^-110 have fewer bits. */
+ * 16 bits for 16-bit rows and not at all for fp32 rows, whose queries of less than 2^-110 have fewer bits. */
 size_t p2h_attention_paged_q8_workspace_bytes(const P2hKvCacheQ8 *cache, int n_seqs, int heads, int max_len, int window,
                                               int sinks);
 int p2h_attention_paged_q8(int dtype, const P2hKvCacheQ8 *cache, int n_seqs, int heads, const void *dQ, int ldq,

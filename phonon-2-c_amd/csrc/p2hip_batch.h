@@ -389,8 +389,9 @@ template <int DH, int NQ, int NW> constexpr int codes_lds()
  * scores, those of V the weights.
  *
  * Nothing is lost but what is said here: fp32 queries and weights go in as three bf16 pieces that sum to them (queries down
- * to 2^-110), fp16 queries as they are and their weights as two pieces, 16 bits (as one of fp16, a weight times its scale would
- * leave the type's range), bf16 weights rounded to bf16.
+ * to 2^-110), 16-bit queries as they are and their weights as two pieces, 16 bits (as one of fp16, a weight times its scale would
+ * leave the type's range; as one of bf16, weights cost as much as the rounding of the output: off by 0.00235 of a bf16 output's
+ * norm, as two by 0.00166, that rounding alone, for 1 to 8 % of the time).
  *
  * 32 sequences of up to 8192 tokens, 32 heads on 8 of 128, bf16, 375 MB: 79 us with the join, 4.8 TB/s, bound by memory (with the
  * maximum of every block taken and masks as branches 87). Three sequences of 8 behind 30001 tokens each, heads of 64, fp16:
@@ -402,7 +403,7 @@ __device__ __forceinline__ void attend_codes(const BatchArgs &a, const BatchItem
     typedef typename Elem<DT>::type E;
     typedef CodeBlock<DH> B;
     constexpr int KB = B::KB, CH = B::CH, RPL = B::RPL, LD = B::LD, NT = DH / 16, KT = DT == T_F16 ? T_F16 : T_BF16;
-    constexpr int NP = DT == T_F32 ? 3 : 1, WP = DT == T_F32 ? 3 : DT == T_F16 ? 2 : 1;   /* pieces of a query, of a weight */
+    constexpr int NP = DT == T_F32 ? 3 : 1, WP = DT == T_F32 ? 3 : 2;   /* pieces of a query, of a weight */
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, x16 = lane & 15;
     const int G = a.heads / a.kv;
 

@@ -898,3 +898,26 @@ def test_rows_q8_more_workgroups_than_a_grid_is_wide():
             p = table[s, at // page]
             want = np.where((p >= 0)[:, None], values[np.maximum(p, 0), at % page], 0)
             assert np.array_equal(d.download((run.size, Dh), np.uint16, offset=int(run[0]) * Dh * 2), want), run[0]
+
+
+@pytest.mark.parametrize("t", ("f16", "bf16"))
+@pytest.mark.parametrize("Dh", (64, 128))
+def test_q8_loses_no_more_than_the_outputs_rounding(t, Dh):
+    """Relative 2-norm over many outputs. Rounding a value of mantissa m in [1, 2) to the type is off by an rms of eps / 2 / sqrt(3)
+    of its power of two, that over m of the value: over all at most as if every m were 1. What comes before it is 2^-16 a weight
+    and 32 bits. (Weights rounded to 8 bits would be as much again: over the limit, as m is spread.)"""
+    H, Hk, page = 32, 8, 16
+    lens = tuple(range(100, 900, 50))
+    q, kept, table = paged_case(t, lens, H, Hk, page, Dh, "rounding")
+    want, _ = B.paged_want(t, q, *kept.values(), table, lens, H, 0.05, EVERY, 0, True)
+    most = D.HALF[t] / 3 ** 0.5
+    for split in (False, True):
+        assert D.norm_off(D.to_f64(t, B.run_paged(t, q, kept, table, lens, H, 0.05, EVERY, 0, split)), want) <= most
+    for per in (1, 16):   # 16 rows at a time, and 32
+        groups = [(60, (61, 90, 300, 777) * per)]
+        rng, lens, starts, shared, table, pages, reach = shared_case(t, groups, H, Hk, page, Dh, "rounding")
+        cache, K, V = shared_cache(rng, t, "q8", pages, Hk, page, Dh, table, reach)
+        q = D.rows(rng, t, len(lens), H * Dh)
+        want, _ = B.paged_want(t, q, K, V, table, lens, H, 0.05, EVERY, 0, True, starts, shared)
+        off = D.norm_off(D.to_f64(t, B.run_shared(t, q, cache, starts, shared, table, lens, H, 0.05, EVERY, 0, 60, 717)), want)
+        assert off <= most, (per, off)
