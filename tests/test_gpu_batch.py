@@ -921,3 +921,106 @@ def test_q8_loses_no_more_than_the_outputs_rounding(t, Dh):
         want, _ = B.paged_want(t, q, K, V, table, lens, H, 0.05, EVERY, 0, True, starts, shared)
         off = D.norm_off(D.to_f64(t, B.run_shared(t, q, cache, starts, shared, table, lens, H, 0.05, EVERY, 0, 60, 717)), want)
         assert off <= most, (per, off)
+
+
+# ── together, each stage from what the one before it left ───────────────────────────────────────────────────────
+
+def codes_within(c, s, want, off):
+    """Codes [.., Dh] and scales of heads that are `want` in 64 bits, of which what was put in may be off by `off`."""
+    top = np.abs(want).max(-1)
+    assert (np.abs(s - top / 127) <= (off.max(-1) + 2 * D.FP32 * top) / 127).all()
+    s = s.astype(np.float64)[..., None]
+    assert (np.abs(c * s - want) <= 0.5 * s * (1 + 512 * D.FP32) + off).all()
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_layer_stage_by_stage(t):
+    """Six tokens of the batch: each entry's outputs from what the entries before it really left, within that entry's own
+    bounds. An adapter's part is many times those, so that none can be missing or another's."""
+    L = Layer(t, GROUPS, SHARES, 16, "stages")
+    n, H, Hk, DH = L.n, L.H, L.Hk, L.DH
+    rng = rng_of(t, "stages")
+    wq, wo = D.q4_values(*L.wq, L.C, L.W, 64), D.q4_values(*L.wo, H * DH, L.C, 32)
+    shares = np.repeat(L.shared, np.diff(L.groups))
+    for step in range(6):
+        x = D.rows(rng, t, n, L.C)
+        L.place(x, step)
+        L.step()
+        x64 = D.to_f64(t, x)
+        z = x64 @ wq * 0.05
+        of_z = D.q4_bound(t, x64, wq, z, 0.05, L.C)
+        y, of_y = B.adapters_want(t, x, L.index, *L.ad, D.to_type(t, z))
+        qkv = L.dqkv.download((n, L.W), D.np_type(t))
+        got, bound = D.to_f64(t, qkv), of_y + (of_z + D.HALF[t] * np.abs(z)) * (1 + 2 * D.HALF[t])
+        D.check(got, y, bound, f"{t} {step} qkv")
+        has = L.index >= 0
+        assert np.median((np.abs(y - z) / bound)[has]) > 20 and has.any()
+        pos = shares + step
+        heads = got.reshape(n, H + 2 * Hk, DH)
+        wantq, size_of = D.norm_rope(heads[:, :H], L.gq, 1e-6, DH, False, L.freq, pos)
+        q = L.dq.download((n, H * DH), D.np_type(t))
+        D.check(D.to_f64(t, q).reshape(wantq.shape), wantq, D.rope_bound(t, wantq, size_of, DH), f"{t} {step} q")
+        wantk, size_of = D.norm_rope(heads[:, H:H + Hk], L.gk, 1e-6, DH, False, L.freq, pos)
+        L.kept.kc, L.kept.vc, L.kept.ks, L.kept.vs = L.kept.download()
+        at, off = L.table[np.arange(n), pos // L.PAGE], pos % L.PAGE
+        codes_within(L.kept.kc[at, :, off], L.kept.ks[at, :, off], wantk, D.rope_bound("f32", wantk, size_of, DH))
+        vcode, vscale = B.codes_of(heads[:, H + Hk:].astype(np.float32))
+        assert np.array_equal(L.kept.vc[at, :, off], vcode) and np.array_equal(L.kept.vs[at, :, off], vscale)
+        want, bound = B.paged_want(t, q, *L.kept.values(), L.table, pos + 1, H, DH ** -0.5, L.WINDOW, L.SINKS, True, L.groups, L.shared)
+        o = L.do.download((n, H * DH), D.np_type(t))
+        D.check(D.to_f64(t, o), want, bound, f"{t} {step} o")
+        o64 = D.to_f64(t, o)
+        out = x64 + o64 @ wo * 0.05
+        bound = D.q4_bound(t, o64, wo, out, 0.05, H * DH) + 2 * D.FP32 * (np.abs(x64) + np.abs(out))
+        D.check(D.to_f64(t, L.out()), out, bound, f"{t} {step} out")
+
+
+@pytest.mark.parametrize("t", D.TYPES)
+def test_prompt_chunk_stage_by_stage(t):
+    """As test_prompt_chunk_over_kept_rows, every row of the windowed attention, from the rows that were really read back."""
+    H, Hk, Dh, page, rot = 4, 2, 64, 16, 64
+    past, chunk = (50, 0, 131), (20, 33, 7)
+    lens = [p + c for p, c in zip(past, chunk)]
+    T = sum(chunk)
+    rng, qkv, gq, gk, freq, _ = rope_inputs(t, T, H, Hk, Dh, rot, "chunk stages")
+    table, pages = B.tables(rng, [-(-n // page) for n in lens])
+    kept = B.fill_unwritten(B.Kept.random(rng, pages, Hk, page, Dh), table, past)
+    pos = np.concatenate([p + np.arange(c) for p, c in zip(past, chunk)]).astype(np.int32)
+    slots = table[np.repeat(np.arange(3), chunk), pos // page] * page + pos % page
+    q, _, kept.kc, kept.vc, kept.ks, kept.vs = run_rope(t, qkv, H, kept, gq, gk, 1e-6, rot, False, freq, pos, slots)
+    ks, qs = (np.concatenate(([0], np.cumsum(n))) for n in (lens, chunk))
+    k, v = B.run_rows(t, kept, ks, table, int(ks[-1]))
+    for got, want in zip((k, v), rows_want(t, kept, ks, table, int(ks[-1]))):
+        assert np.array_equal(got, want)
+    o = D.to_f64(t, D.run_window(t, q, k, v, H, Hk, Dh, 0.125, 60, 0, 2, qs, ks))
+    for s in range(3):
+        a, b = slice(qs[s], qs[s + 1]), slice(ks[s], ks[s + 1])
+        want, bound = D.attention(t, *(D.to_f64(t, x).reshape(len(x), -1, Dh) for x in (q[a], k[b], v[b])),
+                                  D.visible(chunk[s], lens[s], 60, 0, 2), 0.125)
+        D.check(o[a].reshape(want.shape), want, bound, f"{t} {s}")
+
+
+@pytest.mark.parametrize("H", (8, 96))
+def test_shared_cache_of_rows_beyond_32_bits(H):
+    """A prefix and own tokens in the last pages of a cache of more than 2^32 values, by 16 rows and by tiles: the results of a
+    small one."""
+    t, Hk, Dh, page, pages = "bf16", 8, 128, 1024, 4110
+    assert pages * Hk * page * Dh > 1 << 32
+    rng = rng_of("far rows of a cache")
+    used = 3
+    vals = [D.rows(rng, t, used, Hk, page, Dh) for _ in range(2)]
+    lens, B_ = (1500, 1101, 2100), 3
+    q = D.rows(rng, t, B_, H * Dh)
+    outs = []
+    for count, order in ((pages, (pages - 1, pages - 3, pages - 2)), (used, (0, 1, 2))):
+        one = Hk * page * Dh * 2
+        mem = [P.DeviceBuffer(count * one) for _ in range(2)]
+        for m, v in zip(mem, vals):
+            for i, p in enumerate(order):
+                m.upload(v[i], offset=p * one)
+        cache = P.KvCache(t, Hk, Dh, page, count, mem[0].ptr, mem[1].ptr)
+        table = np.array([order] * B_, np.int32)
+        outs.append(B.run_shared(t, q, cache, [0, B_], [1100], table, lens, H, 0.1, EVERY, 0, 1100, 1000))
+    want, bound = B.paged_want(t, q, *(D.to_f64(t, v) for v in vals), table, lens, H, 0.1, EVERY, 0, False)
+    D.check(D.to_f64(t, outs[1]), want, bound, str(H))
+    assert np.array_equal(*outs)
