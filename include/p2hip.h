@@ -523,9 +523,9 @@ typedef struct P2hAdapters {
 /* Y[m] = Z[m] + scale[i] · (X[m] · A[i]ᵀ) · B[i]ᵀ for every row m, i = dIndex[m]: what a row's own adapter adds to the linear that
  * all rows share, whichever entry made Z. Z may be Y itself (same pitch; a single row has none) or NULL for zeros. A row whose
  * index lies outside [0, count) has no adapter: Y[m] = Z[m]. X [M][K], Z and Y [M][N] of the adapters' type, no alignment
- * beyond the element's (rows of X and K that are multiples of 16 bytes load several times faster). Products with A are
- * summed in 32 bits, that sum and its products with B are 32-bit too. Neighbouring rows of one adapter share what is read
- * of it, 16 or 64 at a time. At most 2^20 − 16 rows, K and N at most 2^23. The workspace is p2h_adapters_workspace_bytes(...) bytes,
+ * beyond the element's (where rows of X and K are not multiples of 16 bytes the first product takes 1.4 to 3 times as
+ * long). Products with A are summed in 32 bits, that sum and its products with B are 32-bit too. Neighbouring rows of one
+ * adapter share what is read of it, 16 or 64 at a time. At most 2^20 − 16 rows, K and N at most 2^23. The workspace is p2h_adapters_workspace_bytes(...) bytes,
  * 16-byte aligned, NULL where that is 0 (few rows of small adapters); calls sharing it are stream-ordered. Apart from Z and Y
  * nothing overlaps. */
 size_t p2h_adapters_workspace_bytes(const P2hAdapters *adapters, int M);

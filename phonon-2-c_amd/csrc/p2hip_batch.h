@@ -1,11 +1,16 @@
 /*  p2hip_batch.h – gfx950 kernels of a served batch's step (included once, by p2hip_batch.hip).
  *
  *  Kernels:
- *    kv_rows_q8      kept 8-bit keys and values back as rows
- *    attend          one query per sequence over pages of rows or of 8-bit codes, prefixes of groups of sequences read once
- *    attend_join     adds the parts of each query
- *    adapter_shrink  rows times the first matrix of their adapters
- *    adapter_expand  that times the second, added to the rows of the projection beside it
+ *    kv_rows_q8           kept 8-bit keys and values back as rows
+ *    attend               one query per sequence over pages: prefixes of groups of sequences, read once for 16 query rows (8-bit
+ *                         codes: 16 or 32), and what each sequence has alone
+ *    attend_tiles         the same of 16-bit rows, prefixes read once for 128 query rows
+ *    attend_join          adds the parts of each query
+ *    adapter_shrink       rows times the first matrix of their adapters, 16 rows a workgroup
+ *    adapter_shrink_rows  the same of many aligned rows, 64 a workgroup
+ *    adapter_expand       that times the second, added to the rows of the projection beside it, 16 rows a workgroup; of few rows of
+ *                         small adapters with the first product too
+ *    adapter_expand_rows  the same of many rows, 64 a workgroup
  */
 #pragma once
 
@@ -393,10 +398,12 @@ template <int DH, int NQ, int NW> constexpr int codes_lds()
  * leave the type's range; as one of bf16, weights cost as much as the rounding of the output: off by 0.00235 of a bf16 output's
  * norm, as two by 0.00166, that rounding alone, for 1 to 8 % of the time).
  *
- * 32 sequences of up to 8192 tokens, 32 heads on 8 of 128, bf16, 375 MB: 79 us with the join, 4.8 TB/s, bound by memory (with the
- * maximum of every block taken and masks as branches 87). Three sequences of 8 behind 30001 tokens each, heads of 64, fp16:
- * 34 us, of which the floor of 104 MB is 20.6: a workgroup's 2 · 16 rows take products of 16 rows twice, the rest is the start
- * and end of 512 workgroups. One sequence of 375, fp32: 7.9 us, waits in turn (length, page, codes, join). */
+ * 32 sequences of up to 8192 tokens, 32 heads on 8 of 128, bf16 and fp16, 375 MB: 81 us with the join, 4.6 TB/s, bound by memory
+ * (fp32 85; the maximum of every block taken and masks as branches cost 8 more). Three groups of 8 sequences behind 30001 tokens
+ * each, heads of 64, fp16 and bf16: 36 us, of which the floor of 104 MB is 20.6: a workgroup's 2 · 16 rows take products of 16 rows
+ * twice, the rest is the start and end of 512 workgroups. 64 sequences behind 32768 tokens, 32 heads on 8 of 128: 95 us (fp32 120),
+ * vector unit 59 %: codes become operands anew for every 32 rows. One sequence of 375, fp32: 7.9 us, waits in turn (length, page,
+ * codes, join). */
 template <int DT, int DH, int NQ, int NW>
 __device__ __forceinline__ void attend_codes(const BatchArgs &a, const BatchItem &w, unsigned char *lds)
 {
@@ -654,7 +661,14 @@ __device__ __forceinline__ int group_start(const BatchArgs &a, int g) { return i
  *
  * 64 sequences behind 32768 tokens, 32 heads on 8 of 128, bf16: 55 us without their own keys, 0.62 PFLOP/s; 72 with 512 of their
  * own each, which start when tiles end. Eight waves a workgroup with four buffers, one a CU, took 83; tiles and own parts in
- * turn 74, as a SIMD's two waves of tiles fill each other's gaps. */
+ * turn 74, as a SIMD's two waves of tiles fill each other's gaps.
+ *
+ * Weights are rounded to the type for their product with V, not for their sum, as everywhere where rows are kept in 16 bits: of the
+ * same case 0.0023 of the outputs' norm off against 64 bits, where the rounding of the outputs is 0.0017. A second product with
+ * what the first lost leaves that alone and costs 12 to 20 % (with the join 78.5 -> 88.3 us, with 20 keys of their own 60.6 -> 72.2; fp16
+ * 78 -> 90). An fp16 weight under 2^-31 of the largest that its part of the prefix has had so far is lost (one of 2^-25 under a
+ * reference that stands 2^6 below): it takes 2^20 keys of one part, all just under that, to lose half a step of the sum. kLift would lose
+ * less, but its sums of 32 weights would leave the type. */
 constexpr int kTileRows = 128;
 template <int DT> constexpr float kTileLift = DT == T_F16 ? 6.0f : 0.0f;          /* fp16 weights up to 2^6 below … */
 template <int DT> constexpr float kTileSlack = DT == T_F16 ? 65504.0f : 1024.0f;  /* … a sum that every type holds */
@@ -993,8 +1007,8 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(BatchArgs a)
 }
 
 /* The parts of one query added up by one wave, DH / 64 outputs a lane: o = Σ 2^(top_i − top) num_i / Σ 2^(top_i − top) den_i. Bound by
- * waits (2.6 us for 8 queries, 2 parts) or reading the parts, which the memory-side cache holds (64 · 32 queries of 33 parts, 35
- * MB: 8 us). */
+ * waits (2.6 us for 8 queries, 2 parts; one query of 1024 parts, which a wave reads eight at a time, 44, where what made them took 10)
+ * or reading the parts, which the memory-side cache holds (64 · 32 queries of 33 parts, 35 MB: 8 us). */
 template <int DT, int DH>
 __global__ __launch_bounds__(256) void attend_join(BatchArgs a)
 {
@@ -1084,7 +1098,9 @@ template <int DT> __device__ __forceinline__ f4 mfma_piece(u4 a, u4 b, f4 c)
     }
 }
 
-/* 16 bytes of a row from element k on, zeros behind element `end`; VEC: all there and aligned */
+/* 16 bytes of a row from element k on, zeros behind element `end`; VEC: all there and aligned. Otherwise by the element, inside
+ * a row too: the first product of bf16, rank 16, K = 4095 against 4096: one row 4.4 us (3.1), 32 rows of as many requests 21 (7.6), 300 rows
+ * 9.3 (4.5); 6000 rows, K = 1023 against 1024, 20 (7.8, by 64 rows), fp32 of rank 32 26 (15). */
 template <int DT, bool VEC> __device__ __forceinline__ u4 row_piece(const typename Elem<DT>::type *row, int k, int end)
 {
     typedef typename Elem<DT>::type E;
@@ -1404,7 +1420,8 @@ __global__ __launch_bounds__(64 * NW) void adapter_expand(AdapterArgs a)
  * different rows, as the products have them, a CU takes four times as long for each. An adapter's 64 rows of B come through LDS,
  * shared by the waves, and each wave's sums leave through it. VEC: Z and Y are read and written 16 bytes at a time, Z through
  * LDS too; otherwise by the element. fp32, 6000 rows of 375 an adapter, N = 4096, rank 32: 48 us, 4.1 TB/s, bound by memory
- * (67 with the compiler's waits and lanes in different rows; both products by 16 rows 246, by 64 66); bf16, 300 rows of 20 an adapter, N = 16384, rank 16: 16 us, N = 16389 27.
+ * (201 MB of H, Z, B and Y once, of which the counters see 241; 67 with the compiler's waits and lanes in different rows; both
+ * products by 16 rows 246, by 64 66); bf16, 300 rows of 20 an adapter, N = 16384, rank 16: 16 us, N = 16389 27.
  *
  * Everything comes by direct loads, a step (64 columns of one adapter) or a unit (64 columns) ahead, and is waited for by
  * number: the compiler's own waits, which do not know how many stores a path has issued, would wait for all of them. Such a

@@ -72,6 +72,9 @@ Plan shared_plan(const CacheView &c, bool q8, int dtype, int n_seqs, int n_group
     const int tr = p.tiled ? p2k::kTileRows : 16 * p.nq;
     p.p_tiles = n_seqs * G / tr + n_groups;
     p.p_parts = parts_of((long long)n_groups * ((rows + tr - 1) / tr) * c.heads, left_of(max_shared, window, sinks), kb);
+    /* 512 workgroups for own keys of heads of 64 too, beside those of prefixes, where paged_plan takes 1024: three groups of 8 behind
+     * 30001 tokens with up to 1000 of their own each 42.1 us, 1024 41.2; behind 3000 with up to 20000 123.6, 1024 98.7. The workspace grows
+     * with the parts. */
     p.o_parts = parts_of((long long)n_seqs * c.heads * p.q_groups, left_of(max_own, window, sinks), kb);
     return p;
 }
@@ -341,15 +344,20 @@ static int check_adapters(const char *name, const P2hAdapters *ad, int M)
 /* Adapters that 16 rows may have between them, as the host knows it */
 static int adapters_of_16(const P2hAdapters *ad, int M) { return p2k::imin(p2k::imin(M, 16), p2k::imax(ad->count, 1)); }
 
-/* Above this many rows a workgroup of the second product takes 64 rows, not 16 (bf16, K = 4096, rank 16, shrink and expand:
- * 300 rows with N = 16384 25 -> 16 us, N = 16389 37 -> 27; 128 rows of as many adapters 35 -> 42), above kManyShrink one of the
- * first too (300 rows 4.9 -> 7.6 us). */
+/* Above kManyRows rows a workgroup of the second product takes 64 rows, not 16 (bf16, K = 4096, rank 16, shrink and expand:
+ * 300 rows of 20 an adapter with N = 16384 30 -> 22 us, N = 16389 37 -> 27, 400 rows of one 96 -> 78; but 200 of 20 21 -> 17 too; 128
+ * rows of as many adapters 35 -> 42), above kManyShrink one of the first too (both, N = 4096: 6000 fp32 rows, K = 1024, rank 32 65 ->
+ * 63 us, 3000 of 375 an adapter, bf16, K = 4096, 30 -> 27.5, 1200 of 20 26.9 either way; but 600 18.8 -> 20.3, fp32 600 17.8 -> 19.1, 1200
+ * 22 -> 24.6; 400 15.7 -> 17.8). */
 constexpr int kManyRows = 256, kManyShrink = 512;
 
 /* K over workgroups, 0: everything in one launch, each workgroup making H for itself, while that is little to read (one row,
  * 16-bit, rank 8, K = 1024, 16 KB: 4.2 us against 2.6 + 3.4; 128 KB: 7.8 against 3.0 + 3.7, N = 16389 12.4 against 8). A part has
  * at least 128 dimensions, 256 where a wave has few rows' adapters: the second product adds the parts (one row, rank 64, K =
- * 2048: 3.2 + 9.1 us with 128, 4.0 + 6.9 with 256). A number, as the workspace's size is asked for where there may be no device. */
+ * 2048: 3.2 + 9.1 us with 128, 4.0 + 6.9 with 256), and there are at most 16 (bf16, rank 16, N = 16389, both products: 32 rows, K =
+ * 4096 20.5 us, with 8 23.3, with 32 21.0; 64 rows 29.2, 31.8, 31.8; 17 rows, K = 8192 20.1, 27.2, 17.9; one row of rank 64, K = 8192 13.4, 12.8,
+ * 17.5). Above kManyShrink all together are at most 768, three a CU (6000 bf16 rows, K = 4096 48.7 us, 384 49.6, 1536 52.7; 600 and
+ * 1200 rows and K = 1024 the same with each). A number, as the workspace's size is asked for where there may be no device. */
 static int adapter_parts(const P2hAdapters *ad, int M)
 {
     const int n = adapters_of_16(ad, M), tiles = (M - 1) / (M > kManyShrink ? 64 : 16) + 1;
@@ -401,7 +409,8 @@ int p2h_adapters_add(const P2hAdapters *ad, int M, const void *dX, int ldx, cons
     a.vec = aligned(dY, 16) && (M == 1 || ldy * es % 16 == 0) && (!dZ || (aligned(dZ, 16) && (M == 1 || ldz * es % 16 == 0)));
     const unsigned tiles = (unsigned)((M + 15) / 16), columns = (unsigned)((N - 1) / 64 + 1);
     /* of many rows, columns a workgroup: as many workgroups as three a CU (16-bit rows: four), so that they begin and end
-     * together */
+     * together (both products, half as many, as many, twice as many: 6000 fp32 rows, K = 1024, N = 4096 77, 63, 64.5 us, 600 18.4, 19.2,
+     * 19.3; bf16, K = 4096, 300 rows, N = 16384 24.7, 21.7, 20.9, 1200 57.6, 48.3, 48.9, 6000, N = 4096 53.3, 48.7, 45.8) */
     const unsigned slots = es == 4 ? 768 : 1024, groups = (tiles + 3) / 4 < slots ? slots / ((tiles + 3) / 4) : 1;
     a.units = (int)((columns + groups - 1) / groups);
     hipStream_t s = stream_of(stream);

@@ -168,8 +168,8 @@ template <int DT> __device__ __forceinline__ u4 only_finite(u4 v)
 
 /* Weights enter their product with V in the rows' type. fp16 keeps nothing under 2^-25, which many keys together, or one
  * with a large value beside values near 0, can make felt; so the reference that weights are taken from stands kLift powers
- * of two under the largest score (weights up to 2^kLift, and what is under 2^-(25 + kLift) of the largest is lost: 2^-40).
- * Sums carry the same factor, so that it leaves with the division. bf16 ends where fp32 does and needs none. */
+ * of two under the largest score (weights up to 2^kLift, and what is under 2^-(25 + kLift) of the largest is lost: 2^-40; kernels whose
+ * sums of weights have to stay within the type lift by less and say so). Sums carry the same factor, so that it leaves with the division. bf16 ends where fp32 does and needs none. */
 template <int DT> constexpr float kLift = DT == T_F16 ? 15.0f : 0.0f;
 
 /* A score's place less the lift. In two instructions: as one, the constant or c would take a register of its own, which
