@@ -36,6 +36,9 @@ template <class F> void by_type_dim(int dtype, int head_dim, F f)
     });
 }
 
+/* whether arrays of words are aligned: the scalar cache reads the aligned word that an address lies in */
+template <class... P> bool words(const P *...p) { return (aligned(p, 4) && ...); }
+
 /* M rows of `w` bytes at pitch `ld` bytes, as a range */
 struct Rows {
     const char *p;

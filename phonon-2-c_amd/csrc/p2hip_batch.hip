@@ -108,9 +108,6 @@ int check_tokens(const char *name, int n)
     return n < 0 || n > (1 << 30) ? fail(P2H_E_ARG, "%s: up to %d tokens (0 .. 2^30)", name, n) : P2H_OK;
 }
 
-/* whether arrays of words are aligned: the scalar cache reads the aligned word that an address lies in */
-template <class... P> bool words(const P *...p) { return (aligned(p, 4) && ...); }
-
 Rows ints(const int *p, int ld, int n) { return Rows{(const char *)p, (size_t)ld * 4, (size_t)ld * 4, ld > 0 && p ? n : 0}; }
 
 /* Attention over a cache of either kind, its plan checked; `group` NULL without prefixes. */

@@ -226,6 +226,8 @@ static int norm_rope(const char *name, int dtype, int T, int heads, int kv_heads
     if (!dGammaQ || !dGammaK || !aligned(dGammaQ, 4) || !aligned(dGammaK, 4) || (rot > 0 && (!dFreq || !dPos)) ||
         (cache && !dSlots))
         return fail(P2H_E_ARG, "%s: NULL or unaligned norm weights, or NULL frequencies, positions or slots", name);
+    if (q8 && (!words(dSlots) || (rot > 0 && !words(dFreq, dPos))))
+        return fail(P2H_E_ARG, "%s: frequencies, positions or slots are not 4-byte aligned", name);
     const size_t es = elem_size(dtype);
     const Rows x{(const char *)dQKV, ldqkv * es, in_w * es, T}, q{(const char *)dQ, ldq * es, q_w * es, T};
     const Rows xk{x.p + q_w * es, x.ld, in_w * es - q_w * es, T};   /* the rows from their keys on */

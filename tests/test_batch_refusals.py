@@ -262,3 +262,9 @@ def test_arrays_of_words_that_are_not_aligned(off):
             refused(shared(kind, **{name: 34 * A + off}), "4-byte")
     refused(add(index=43 * A + off), "4-byte")
     refused(add(adapters(dScale=42 * A + off)), "4-byte")
+
+
+@pytest.mark.parametrize("off", (1, 2, 3))
+def test_rope_arrays_of_words_that_are_not_aligned(off):
+    for name in ("freq", "pos", "slots"):
+        refused(rope(**{name: A + off}), "4-byte")
